@@ -1,0 +1,210 @@
+"""Weights and the paged cache in 8 bits (E4M3 with a scale per block): the checking wrappers of their kernels.
+
+A scale is a power of two, 2^e with the smallest e >= -100 for which ``448 * 2^e`` is at least the block's largest magnitude,
+so that dividing by it is exact and a value is rounded once. Blocks are 128 x 128 of a weight, 128 channels of a token, and a
+page of one key/value head of the cache. The kernels take scales that are not powers of two as well (a checkpoint's), but
+for those of cache pages that they write themselves.
+"""
+from __future__ import annotations
+
+import ctypes
+from ctypes import c_void_p, c_int, c_float, c_longlong
+from typing import NamedTuple, Optional
+
+import torch
+
+from ..csrc.build import load_kernel_lib
+
+BLOCK = 128
+E4M3 = torch.float8_e4m3fn
+
+
+class Float8Weight(NamedTuple):
+    """A matrix in 8 bits: ``values [N, K]`` (E4M3, rows of unit stride that start on 16 bytes) and ``scales
+    [ceil(N / 128), ceil(K / 128)]`` (float32): ``w[n, k] = values[n, k] * scales[n // 128, k // 128]``."""
+    values: torch.Tensor
+    scales: torch.Tensor
+
+    @property
+    def shape(self):
+        return self.values.shape
+
+    @property
+    def dtype(self):
+        return self.values.dtype
+
+
+_FLOAT8_SIGNATURES = {
+    "gb_f8_quantize_rows": [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p],
+    "gb_f8_quantize_weight": [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_longlong, c_void_p, c_void_p],
+    "gb_f8_append": [c_void_p, c_int, c_longlong, c_void_p, c_int] + [c_void_p] * 7 + [c_int] * 6 + [c_void_p, c_int, c_int, c_void_p],
+    "gb_f8_attention_simple": [c_void_p, c_int] + [c_void_p] * 5 + [c_int] + [c_void_p] * 3 + [c_int] * 5 + [c_float, c_int, c_int, c_void_p],
+    "gb_f8_gemm": [c_void_p, c_int, c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p,
+                   c_void_p, c_void_p],
+    "gb_f8_gemm_error_check": [],
+    "gb_f8_gemm_set_error_sink": [c_void_p],
+}
+
+
+class Float8Ops:
+    """What ``CudaOps`` has of 8 bits. Everything is launched on torch's current stream; scratch memory belongs to the
+    stream (or to ``ws``, a step's workspace), and results do not depend on the order in which blocks finish."""
+
+    @property
+    def float8_lib(self):
+        """The library of the 8-bit kernels, compiled and loaded when a caller first needs it."""
+        if self._float8 is None:
+            L = load_kernel_lib("garuda_float8")
+            L.gb_last_error.restype = ctypes.c_char_p
+            for name, argtypes in _FLOAT8_SIGNATURES.items():
+                fn = getattr(L, name)
+                fn.argtypes, fn.restype = argtypes, c_int
+            L.gb_f8_gemm_scratch_bytes.argtypes = [c_int, c_int, c_int, ctypes.POINTER(c_longlong)]
+            L.gb_f8_gemm_scratch_bytes.restype = c_longlong
+            if L.gb_f8_gemm_set_error_sink(self.error_word.data_ptr()):
+                _need(False, "the 8-bit library could not be given the host's error word")
+            self._float8 = L
+        return self._float8
+
+    def _scratch8(self, name, shape, dtype, ws, zero=False):
+        """Scratch of this name: the step's, or one per stream."""
+        if ws is not None:
+            return ws.get(name, shape, dtype, zero=zero)
+        return self.private_ws.get(f"{name}@{self._stream()}", shape, dtype, zero=zero)
+
+    def check_float8_errors(self) -> None:
+        """Synchronises, and raises if an 8-bit kernel gave up on a wait since the last check."""
+        seen, self.error_word[0] = int(self.error_word[0]), 0
+        code = self.float8_lib.gb_f8_gemm_error_check() or seen
+        _need(not code, f"an 8-bit kernel gave up waiting: code {code}")
+
+    # ------------------------------------------------------------------ matrix products
+    def float8_weight(self, w: torch.Tensor) -> Float8Weight:
+        """``w [N, K]`` (bfloat16 or float32) in 8 bits with a scale per block of 128 x 128."""
+        self._on_device(w)
+        _need(w.dim() == 2 and w.stride(1) == 1 and w.numel() > 0, "float8_weight: a matrix with rows of unit stride")
+        N, K = w.shape
+        pitch, blocks = (K + 15) // 16 * 16, ((N + BLOCK - 1) // BLOCK, (K + BLOCK - 1) // BLOCK)
+        codes = torch.empty(N, pitch, dtype=E4M3, device=w.device)
+        scales = torch.empty(blocks, dtype=torch.float32, device=w.device)
+        self._check(self.float8_lib, self.float8_lib.gb_f8_quantize_weight(
+            w.data_ptr(), _tag(w, "float8_weight"), w.stride(0), N, K, codes.data_ptr(), pitch, scales.data_ptr(), self._stream()),
+            "float8_weight")
+        return Float8Weight(codes[:, :K], scales)
+
+    def linear_float8(self, a, w, out, accumulate: bool = False, alpha: float = 1.0, ws=None):
+        """``out[M, N] (+)= q(a) @ w^T``: ``w`` a ``Float8Weight`` (or a pair of its two tensors), ``a [M, K]`` bfloat16 or float32, its
+        rows rounded to 8 bits with a scale per token and 128 channels (``q``). Sums are 32-bit; ``out`` is bfloat16 or float32,
+        and float32 where ``accumulate`` adds ``alpha * product`` to what is there."""
+        values, scales = w
+        self._on_device(a, values, scales, out)
+        _need(a.dim() == 2 and values.dim() == 2 and out.dim() == 2, "linear_float8: operands must be matrices")
+        M, K = a.shape
+        N = values.shape[0]
+        if not (values.shape[1] == K and out.shape == (M, N)):
+            _need(False, f"linear_float8: shapes {tuple(a.shape)} x {tuple(values.shape)} -> {tuple(out.shape)}")
+        _need(K > 0, "linear_float8: no channels")
+        _need(values.dtype == E4M3, "linear_float8: weights must be float8_e4m3fn")
+        _need(scales.dtype == torch.float32 and scales.is_contiguous()
+              and tuple(scales.shape) == ((N + BLOCK - 1) // BLOCK, (K + BLOCK - 1) // BLOCK),
+              "linear_float8: one float32 scale per block of 128 x 128")
+        _need((values.stride(1) == 1 or K == 1) and (values.stride(0) % 16 == 0 or N <= 1) and values.data_ptr() % 16 == 0,
+              "linear_float8: rows of codes must start on 16 bytes (float8_weight makes such)")
+        _need(a.stride(1) == 1 or K == 1, "linear_float8: rows of a must have unit stride")
+        _need(out.is_contiguous() and out.dtype in (torch.float32, torch.bfloat16), "linear_float8: out must be contiguous, bfloat16 or float32")
+        _need(not accumulate or out.dtype == torch.float32, "linear_float8: accumulates into float32 only")
+        _need(accumulate or alpha == 1.0, "linear_float8: a multiplier goes with accumulation only")
+        if M == 0 or N == 0:
+            return
+        L = self.float8_lib
+        pitch = (K + 15) // 16 * 16
+        codes = self._scratch8("float8_codes", (M, pitch), torch.uint8, ws)
+        rows = self._scratch8("float8_scales", ((K + BLOCK - 1) // BLOCK, M), torch.float32, ws)
+        stream = self._stream()
+        self._check(L, L.gb_f8_quantize_rows(a.data_ptr(), _tag(a, "linear_float8 input"), a.stride(0), M, K, codes.data_ptr(), pitch,
+                                             rows.data_ptr(), stream), "quantize_rows")
+        counter_bytes = c_longlong(0)
+        part_bytes = int(L.gb_f8_gemm_scratch_bytes(M, N, K, ctypes.byref(counter_bytes)))
+        counters = self._scratch8("float8_counters", (int(counter_bytes.value),), torch.uint8, ws, zero=True)
+        parts = self._scratch8("float8_parts", (part_bytes,), torch.uint8, ws)
+        w_pitch = values.stride(0) if N > 1 else pitch
+        self._check(L, L.gb_f8_gemm(codes.data_ptr(), pitch, rows.data_ptr(), values.data_ptr(), w_pitch, scales.data_ptr(), out.data_ptr(),
+                                    _tag(out, "linear_float8 output"), M, N, K, int(accumulate), float(alpha), counters.data_ptr(),
+                                    parts.data_ptr(), stream), "linear_float8")
+
+    # ------------------------------------------------------------------ the cache
+    def _check_pools(self, what, k_pool, v_pool, k_scale, v_scale, kv_heads, page_size, head_dim):
+        for pool, scale in ((k_pool, k_scale), (v_pool, v_scale)):
+            _need(pool.dtype == E4M3 and pool.is_contiguous() and pool.dim() == 4
+                  and tuple(pool.shape[1:]) == (kv_heads, page_size, head_dim) and pool.data_ptr() % 16 == 0,
+                  f"{what}: pools must be float8_e4m3fn [pages, {kv_heads}, {page_size}, {head_dim}]")
+            _need(scale.dtype == torch.float32 and scale.is_contiguous() and tuple(scale.shape) == tuple(pool.shape[:2]),
+                  f"{what}: one float32 scale per page and head")
+        _need(k_pool.shape[0] == v_pool.shape[0], f"{what}: as many pages of keys as of values")
+
+    def _check_batch(self, what, cu_q, kv_lens, block_table):
+        R = kv_lens.shape[0]
+        for t in (cu_q, kv_lens, block_table):
+            _need(t.dtype == torch.int32 and t.is_contiguous(), f"{what}: cu_q, kv_lens and the block table must be contiguous int32")
+        _need(R > 0 and cu_q.numel() == R + 1 and block_table.dim() == 2 and block_table.shape[0] >= R,
+              f"{what}: cu_q, kv_lens and the block table disagree on the number of requests")
+        return R
+
+    def kv_append_float8(self, qkv, q_out, k_pool, v_pool, k_scale, v_scale, cu_q, kv_lens, block_table, heads, kv_heads, head_dim,
+                         cos_sin, interleaved, page_size):
+        """Split ``qkv [T, (heads + 2 kv_heads) head_dim]`` into heads, rotate queries and keys by ``cos_sin [T, head_dim / 2, 2]``
+        (``CudaOps.rope_table``; None: leave them; ``interleaved``: pairs (2i, 2i + 1) in place of (i, i + head_dim / 2)), write the
+        queries to ``q_out [T, heads, head_dim]``, and keys and values in 8 bits into their pages ``[pages, kv_heads, page_size,
+        head_dim]`` with one scale per page and head ``[pages, kv_heads]``. Request r's tokens ``cu_q[r]`` to ``cu_q[r + 1]`` are its last
+        positions of ``kv_lens[r]``; a page that held positions before them keeps these, in its new scale where that has grown."""
+        what = "kv_append_float8"
+        self._on_device(qkv, q_out, k_pool, v_pool, k_scale, v_scale, cu_q, kv_lens, block_table, cos_sin)
+        T = qkv.shape[0]
+        R = self._check_batch(what, cu_q, kv_lens, block_table)
+        self._check_pools(what, k_pool, v_pool, k_scale, v_scale, kv_heads, page_size, head_dim)
+        _need(heads % kv_heads == 0 and head_dim % 16 == 0, f"{what}: heads in whole groups, of a multiple of 16 channels")
+        _need(qkv.dim() == 2 and qkv.shape[1] == (heads + 2 * kv_heads) * head_dim and qkv.stride(1) == 1 and qkv.stride(0) % 2 == 0
+              and qkv.data_ptr() % 8 == 0, f"{what}: qkv must be [T, (heads + 2 kv_heads) head_dim] with rows of unit stride, on 8 bytes")
+        _need(q_out.is_contiguous() and tuple(q_out.shape) == (T, heads, head_dim) and q_out.data_ptr() % 8 == 0, f"{what}: q_out shape")
+        _need(cos_sin is None or (cos_sin.dtype == torch.float32 and cos_sin.is_contiguous() and tuple(cos_sin.shape) == (T, head_dim // 2, 2)
+                                  and cos_sin.data_ptr() % 16 == 0), f"{what}: cos_sin must be float32 [T, head_dim / 2, 2]")
+        L = self.float8_lib
+        self._check(L, L.gb_f8_append(
+            qkv.data_ptr(), _tag(qkv, "qkv"), qkv.stride(0), q_out.data_ptr(), _tag(q_out, "q_out"), k_pool.data_ptr(), v_pool.data_ptr(),
+            k_scale.data_ptr(), v_scale.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(), block_table.shape[1], T, R,
+            heads, kv_heads, head_dim, None if cos_sin is None else cos_sin.data_ptr(), int(bool(interleaved)), int(page_size), self._stream()),
+            what, 1 if T else 0)
+
+    def paged_attention_float8(self, q, k_pool, v_pool, k_scale, v_scale, block_table, cu_q, kv_lens, out, scale, window, page_size,
+                               num_requests, max_q_len, max_kv_len, ws=None, min_q_len: int = 1):
+        """Causal grouped-query attention over pages of codes (``kv_append_float8``): ``q [T, Hq, hd]`` and ``out [T, Hq * hd]``
+        bfloat16 (or float32, on the plain kernel). ``window`` w > 0: a query reads the last w positions, itself included."""
+        what = "paged_attention_float8"
+        self._on_device(q, k_pool, v_pool, k_scale, v_scale, block_table, cu_q, kv_lens, out)
+        T, Hq, hd = q.shape
+        Hkv = k_pool.shape[1]
+        R = self._check_batch(what, cu_q, kv_lens, block_table)
+        _need(R == num_requests, f"{what}: as many lengths as requests")
+        self._check_pools(what, k_pool, v_pool, k_scale, v_scale, Hkv, page_size, hd)
+        _need(Hq % Hkv == 0 and hd % 16 == 0 and hd <= 256, f"{what}: heads in whole groups, of a multiple of 16 channels up to 256")
+        _need(q.is_contiguous() and out.is_contiguous() and tuple(out.shape) == (T, Hq * hd) and q.dtype == out.dtype, f"{what}: q/out shape")
+        _need(q.data_ptr() % 8 == 0 and out.data_ptr() % 8 == 0, f"{what}: q and out on 8 bytes")
+        _need(scale > 0, f"{what}: a positive scale")
+        _need(block_table.shape[1] * page_size >= max_kv_len, f"{what}: the block table is too narrow for {max_kv_len} positions")
+        if T == 0:
+            return
+        L = self.float8_lib
+        self._check(L, L.gb_f8_attention_simple(
+            q.data_ptr(), _tag(q, "attention q"), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            block_table.data_ptr(), block_table.shape[1], cu_q.data_ptr(), kv_lens.data_ptr(), out.data_ptr(), T, R, Hq, Hkv, hd,
+            float(scale), int(window), int(page_size), self._stream()), what)
+
+
+def _need(cond, msg):
+    from . import ops
+    ops._need(cond, msg)
+
+
+def _tag(t, what):
+    from . import ops
+    return ops._tag(t, what)

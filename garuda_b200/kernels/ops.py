@@ -17,6 +17,7 @@ import numpy as np
 import torch
 
 from ..csrc.build import load_kernel_lib
+from .float8 import Float8Ops
 
 GB_F32, GB_BF16 = 0, 1
 _TAG = {torch.float32: GB_F32, torch.bfloat16: GB_BF16}
@@ -83,7 +84,7 @@ class ExpertRows:
         self.rows, self.pair_row, self.weights, self.identity, self.base = rows, pair_row, weights, identity, base
 
 
-class CudaOps:
+class CudaOps(Float8Ops):
     """Hand-written sm_100a kernels. ``tensor_cores=False`` keeps every matrix
     product and the attention on the plain 32-bit-arithmetic kernels (the true
     32-bit path uses them in any case)."""
@@ -100,6 +101,7 @@ class CudaOps:
         self._seq = None
         self._ssd = None
         self._memory = None
+        self._float8 = None
         self._declare_core()
         # A word of pinned host memory that a kernel whose bounded wait ran out writes its code to (the
         # device reaches pinned host memory directly); ``failed_wait`` reads it without a copy.
