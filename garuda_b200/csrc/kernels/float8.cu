@@ -12,7 +12,8 @@ namespace {
 using namespace f8;
 
 // ------------------------------------------------------------------ tokens into codes
-// a [M, K] -> codes [M, pitch] and scales [K / 128 rounded up][M]: per token and 128 channels. Sixteen lanes take a block, eight
+// a [M, K] -> codes [M, pitch] and, per token and 128 channels, the exponent byte of the scale (e + 127), those of four blocks in a
+// word: [blocks / 4 rounded up][M][4]. Sixteen lanes take a block, eight
 // channels each, so that a warp reads two blocks of a row (512 bytes of bfloat16) in one instruction; a block's largest
 // magnitude takes four shuffles. Bound by memory; what is read is kept in registers, so nothing is read twice.
 template <typename T, bool WIDE>
@@ -36,7 +37,7 @@ __device__ __forceinline__ void load8(const T* src, int have, float (&x)[8]) {
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256)
 quantize_rows_kernel(const T* __restrict__ a, long long lda, int M, int K, uint8_t* __restrict__ codes, int pitch,
-                     float* __restrict__ scales) {
+                     uint8_t* __restrict__ scales) {
   gb::pdl_launch_dependents();
   const int kb = (K + BLOCK - 1) / BLOCK;
   const long long block = ((long long)blockIdx.x * 256 + threadIdx.x) >> 4;       // of all rows'
@@ -61,7 +62,7 @@ quantize_rows_kernel(const T* __restrict__ a, long long lda, int M, int K, uint8
     c.y = encode4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
     *reinterpret_cast<uint2*>(codes + (size_t)row * pitch + k) = c;
   }
-  if ((threadIdx.x & 15) == 0) scales[(size_t)b * M + row] = power_of_two(e);
+  if ((threadIdx.x & 15) == 0) scales[((size_t)(b >> 2) * M + row) * 4 + (b & 3)] = (uint8_t)(e + 127);
 }
 
 // ------------------------------------------------------------------ weights into codes
@@ -334,7 +335,7 @@ __global__ void __launch_bounds__(128) attention_f8_simple_kernel(const Attentio
 GB_DEFINE_LAST_ERROR()
 
 // a [M, K] (rows lda apart) -> codes [M, pitch] (pitch a multiple of 16, at least K; the rest zeros) and scales
-// [ceil(K / 128)][M].
+// [ceil(K / 512)][M][4] as exponent bytes.
 GB_EXPORT int gb_f8_quantize_rows(const void* a, int tag, long long lda, int M, int K, void* codes, int pitch, void* scales, void* stream) {
   if (M < 0 || K <= 0 || pitch < K || pitch % 16 || (uintptr_t)codes % 16) return gb::fail(GB_BAD_ARGUMENT, "quantize_rows: %d x %d, pitch %d", M, K, pitch);
   if (M == 0) return GB_OK;
@@ -345,7 +346,7 @@ GB_EXPORT int gb_f8_quantize_rows(const void* a, int tag, long long lda, int M, 
     const bool wide = (uintptr_t)a % 16 == 0 && lda * (long long)sizeof(T) % 16 == 0;
     auto* kernel = wide ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>;
     return gb::check_pdl_launch(gb::launch_pdl(kernel, dim3((unsigned)grid), dim3(256), 0, (cudaStream_t)stream, dim3(1), (const T*)a, lda, M, K,
-                                               (uint8_t*)codes, pitch, (float*)scales), "quantize_rows");
+                                               (uint8_t*)codes, pitch, (uint8_t*)scales), "quantize_rows");
   });
 }
 

@@ -1,25 +1,29 @@
 // Matrix product in 8 bits: out[m, n] = sum over blocks b of 128 channels of
 //     sa[m, b] * sw[n / 128, b] * sum_{k in b} a8[m, k] w8[n, k],
-// codes in E4M3, scales in 32 bits: one per token and block for the tokens, one per 128 x 128 block for the weights.
+// codes in E4M3, scales powers of two: one per token and block for the tokens, one per 128 x 128 block for the weights.
 //
-// The weights' rows are the rows of the products (128 a CTA), the tokens their columns: up to 256, so that a weight is fetched once for
-// up to 256 tokens, and a step of a few tokens multiplies no padding but to 16. tcgen05.mma (kind::f8f6f4, 32 channels each, sums in 32
-// bits) leaves a block's sums in tensor memory; as every block has scales of its own, sums of several blocks cannot stay there:
-// eight warps read a block's 128 x tokens sums back and add them, scaled, to accumulators in registers, while the tensor cores
-// fill the other of two buffers. A lane holds a weight row, so the scales of a step are the same for all lanes: they are
-// multiplied (token's by weight's), put into shared memory by the warp that uses them, and read four at a time.
+// The scales are the tensor cores' own: tcgen05.mma of kind mxf8f6f4 multiplies every 32 channels of a row by a power of two that lies in
+// tensor memory (a byte, the exponent), so that one accumulator in tensor memory takes all of K. (With scales applied outside, every
+// block's 128 x 256 sums have to come back through registers: that form of this kernel took 1.6 us a block and pair of CTAs, five times
+// what the products take.) Four products of 32 channels share a block's byte; a 32-bit word holds a row's bytes of four
+// blocks, which the instruction chooses from, so scales are brought in once in four blocks.
+//
+// The weights' rows are the rows of the products (128 a CTA), the tokens their columns, up to 240 a tile: a weight is fetched once for
+// all of a tile's tokens, and a step of a few tokens multiplies no padding but to 16.
 //
 // Work is dealt in units of (tile, block), tile by tile, an equal stretch to every CTA (or pair of CTAs): few tokens on a wide
 // weight are bound by how evenly the weights' bytes are shared out, and many tokens leave no ragged last round. A tile that falls to
-// several CTAs is summed by the one that finishes last: each writes its part to scratch memory and counts itself; the last adds the
+// several workers is summed by the one that finishes last: each writes its part to scratch memory and counts itself; the last adds the
 // parts in the order of the channels, whoever it is, so that results do not depend on the order of arrival.
 //
-// PAIR: two CTAs of a cluster multiply 256 weight rows by up to 256 tokens (cta_group::2), each fetching half of the tokens' codes.
+// PAIR: two CTAs of a cluster multiply 256 weight rows by up to 240 tokens (cta_group::2), each fetching half of the tokens' codes.
 //   warp 0     TMA: a box of 128 bytes (128 channels) by 128 weight rows and one by the tokens, a ring of stages. Weights are asked for
 //              before the wait for the kernel in front, which makes the codes.
-//   warp 1     one elected lane: four products a unit, one commit (the stage's "empty" barrier is passed on by the epilogue: a commit
-//              costs the issuing lane as much as two products)
-//   warps 2-9  scale and add; at a tile's end write out, or write the part and perhaps add the parts up
+//   warp 1     one elected lane: scales into tensor memory, four products a unit
+//   warp 2     the scales of four blocks into shared memory: row r's word at 16 (r % 32) + 4 (r / 32) of 512 bytes for 128 rows, as
+//              the copy to tensor memory wants it (128 equal words for the weights, whose scale belongs to the block)
+//   warps 4-11 at a tile's end: write out, or write the part and perhaps add the parts up; the products go on in the
+//              other of two accumulators
 // Every wait is bounded.
 #include "float8.cuh"
 #include "error_word.cuh"
@@ -32,53 +36,61 @@ using namespace tc;
 
 constexpr int BK = f8::BLOCK;                   // channels per unit: 128 bytes, one swizzled row
 constexpr int BM = 128;                         // weight rows per CTA
-constexpr int THREADS = 64 + 256;
+constexpr int MAX_NT = 240;                     // tokens per tile: two accumulators leave room for the scales
+constexpr int THREADS = 128 + 256;
 constexpr int MAX_STAGES = 12;
-constexpr int SMEM_LIMIT = 232448;
+constexpr int SF_STAGES = 3, SF_BYTES = 3 * 512;        // the weights' words, the tokens' (up to 256)
+constexpr int SMEM_LIMIT = 232448, STATIC_BYTES = 1024;
+// tensor memory: accumulators at columns 0 and 256, scales in the gap behind the first
+constexpr uint32_t ACC_STRIDE = 256, SFA_COL = 240, SFB_COL = 244;
 
 struct Args {
-  const float* xs;          // [blocks][M]: the tokens' scales
+  const uint32_t* xs;       // [ceil(blocks / 4)][M]: the tokens' scales, four blocks' exponents a word
   const float* ws;          // [ceil(N / 128)][blocks]: the weights'
   void* out;                // [M, N]
   float* parts;             // scratch: [workers][2][CTAs of a worker][nt][128]
   int* counters;            // [tiles * CTAs of a worker], zero between launches
   int M, N, blocks;
-  int nt, tiles_m;          // tokens per tile (a multiple of 16; PAIR: of 32), tiles of tokens
+  int nt, tiles_m;          // tokens per tile (a multiple of 16), tiles of tokens
   int stages, workers;
   long long units;
   float alpha;
 };
 
-__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-      : "memory");
+// kind mxf8f6f4, both operands E4M3 and K-major, scales UE8M0 (bit 23), one per row and 32 channels; sums in 32 bits. `id`: which byte of
+// the scales' words (the same for both operands).
+__device__ __forceinline__ uint32_t instr_desc_mxf8(int m, int n, uint32_t id) {
+  return (id << 4) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24) | (id << 29);
 }
-__device__ __forceinline__ void mma_f8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-      : "memory");
+template <bool PAIR>
+__device__ __forceinline__ void mma_mxf8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, bool accumulate) {
+  if (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"((uint32_t)accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"((uint32_t)accumulate)
+        : "memory");
 }
-// Sums in 32 bits, both operands E4M3 and K-major.
-__device__ __forceinline__ uint32_t instr_desc_e4m3(int m, int n) {
-  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+// 512 bytes of shared memory (32 rows of 16 bytes) to four columns of tensor memory, the 32 rows to the lanes of every warp.
+template <bool PAIR>
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
+  if (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
-template <int N>
-__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[N]);
-template <>
-__device__ __forceinline__ void tmem_load<32>(uint32_t addr, uint32_t (&r)[32]) { tmem_ld_32(addr, r); }
-template <>
-__device__ __forceinline__ void tmem_load<16>(uint32_t addr, uint32_t (&r)[16]) { tmem_ld_16(addr, r); }
-template <>
-__device__ __forceinline__ void tmem_load<8>(uint32_t addr, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(addr)
-               : "memory");
+// Rows of 16 bytes one behind the other, eight to a group of 128 bytes, not swizzled.
+__device__ __forceinline__ uint64_t smem_desc_rows16(uint32_t addr) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+// The exponent byte of a scale; 255 (not a number) for one that is no positive power of two.
+__device__ __forceinline__ uint32_t scale_byte(float s) {
+  const uint32_t bits = __float_as_uint(s);
+  return (bits & 0x807FFFFFu) == 0 && bits != 0 ? bits >> 23 : 255u;
 }
 
 // Where a worker's stretch of units begins.
@@ -91,17 +103,21 @@ __device__ __forceinline__ int worker_of(long long units, int workers, long long
   return w;
 }
 
-// CH: tokens per epilogue thread (each of the two groups of four warps takes CH of the tile's columns, the second what is left)
-template <bool PAIR, int CH, typename OT, bool ADD>
+struct Place {
+  int tile, b;
+  __device__ __forceinline__ void next(int blocks) {
+    if (++b == blocks) b = 0, ++tile;
+  }
+};
+
+template <bool PAIR, typename OT, bool ADD>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const Args p) {
   constexpr int CTAS = PAIR ? 2 : 1;
-  constexpr int CHUNK = CH % 32 == 0 ? 32 : CH % 16 == 0 ? 16 : 8;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], acc_full[2], acc_empty[2];
+  __shared__ __align__(8) uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], sf_full[SF_STAGES], sf_empty[SF_STAGES], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_s, last_s;
-  __shared__ __align__(16) float scale_s[8][2][CH];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0;
@@ -109,14 +125,20 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
   const int x_rows = p.nt / CTAS;                                  // rows of the tokens' box
   const uint32_t stage_bytes = (uint32_t)(BM + x_rows) * BK;
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const int stages = p.stages;
+  const uint32_t sf_at = ring + stages * stage_bytes;              // behind the ring: the scales on their way
   const long long u_begin = first_unit(p.units, p.workers, worker), u_end = first_unit(p.units, p.workers, worker + 1);
   const int n_units = (int)(u_end - u_begin);
-  const int stages = p.stages;
+  const Place start = {(int)(u_begin / p.blocks), (int)(u_begin % p.blocks)};
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(smem_u32(&full_bar[s]), 1);
       mbar_init(smem_u32(&empty_bar[s]), 1);
+    }
+    for (int s = 0; s < SF_STAGES; ++s) {
+      mbar_init(smem_u32(&sf_full[s]), CTAS);
+      mbar_init(smem_u32(&sf_empty[s]), 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(smem_u32(&acc_full[a]), 1);
@@ -149,10 +171,6 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
     // ---------------------------------------------------------------- producer
     const bool leader = elect_one();
     bool go = true, ran_out;
-    struct Place { int tile, b; } at = {(int)(u_begin / p.blocks), (int)(u_begin % p.blocks)};
-    auto next = [&](Place& q) {
-      if (++q.b == p.blocks) q.b = 0, ++q.tile;
-    };
     auto load_w = [&](int s, const Place& q) {
       const uint32_t full = smem_u32(&full_bar[s]), bar = PAIR ? map_to_rank(full, 0) : full;
       const int row = (q.tile / p.tiles_m * CTAS + (int)rank) * BM;
@@ -168,17 +186,17 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
     };
     // the first stages' weights before the wait for the kernel that makes the codes
     const int early = min(stages, n_units);
-    Place q = at;
-    for (int i = 0; i < early; ++i, next(q))
+    Place q = start;
+    for (int i = 0; i < early; ++i, q.next(p.blocks))
       if (leader) load_w(i, q);
     __syncwarp();
     gb::pdl_wait();
-    q = at;
-    for (int i = 0; i < early; ++i, next(q))
+    q = start;
+    for (int i = 0; i < early; ++i, q.next(p.blocks))
       if (leader) load_x(i, q);
     __syncwarp();
     int s = 0, par = 0;
-    for (int i = early; i < n_units && go; ++i, next(q)) {
+    for (int i = early; i < n_units && go; ++i, q.next(p.blocks)) {
       if (!(go = mbar_wait_warp(smem_u32(&empty_bar[s]), par, aborted, ran_out))) {
         if (ran_out) gb_err::report(ERR_WAIT_EMPTY), *aborted = 1;
         break;
@@ -195,159 +213,203 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
   } else if (warp == 1) {
     if (rank == 0) {
       // -------------------------------------------------------------- the products' issuer
-      const uint32_t idesc = instr_desc_e4m3(CTAS * BM, p.nt);
-      const uint64_t da0 = smem_desc_sw128(ring), db0 = smem_desc_sw128(ring + BM * BK);
+      const uint32_t idesc0 = instr_desc_mxf8(CTAS * BM, p.nt, 0);
+      const uint64_t da0 = smem_desc_sw128(ring), db0 = smem_desc_sw128(ring + BM * BK), ds0 = smem_desc_rows16(sf_at);
       const bool leader = elect_one();
       bool go = true, ran_out;
-      int s = 0, par = 0;
-      for (int i = 0; i < n_units && go; ++i) {
-        const int as = i & 1;
-        if (!(go = mbar_wait_warp(smem_u32(&acc_empty[as]), ((i >> 1) & 1) ^ 1, aborted, ran_out))) {
-          if (ran_out) gb_err::report(ERR_WAIT_ACCUM), *aborted = 1;
-          break;
+      int s = 0, par = 0, sf = 0, sf_par = 0, t = 0;         // t: tiles (or parts) begun
+      Place q = start;
+      for (int i = 0; i < n_units; ++i, q.next(p.blocks)) {
+        const int as = t & 1;
+        if (i == 0 || q.b == 0) {          // a tile begins: both epilogue groups have read this accumulator
+          if (!(go = mbar_wait_warp(smem_u32(&acc_empty[as]), ((t >> 1) & 1) ^ 1, aborted, ran_out))) {
+            if (ran_out) gb_err::report(ERR_WAIT_ACCUM), *aborted = 1;
+            break;
+          }
+        }
+        if (i == 0 || (q.b & 3) == 0) {    // the scales of up to four blocks
+          if (!(go = mbar_wait_warp(smem_u32(&sf_full[sf]), sf_par, aborted, ran_out))) {
+            if (ran_out) gb_err::report(ERR_WAIT_FULL), *aborted = 1;
+            break;
+          }
+          tc_fence_after_sync();
+          if (leader) {
+            const uint64_t ds = ds0 + (uint64_t)(sf * (SF_BYTES >> 4));
+            copy_scales<PAIR>(tmem + SFA_COL, ds);
+            copy_scales<PAIR>(tmem + SFB_COL, ds + (512 >> 4));
+            if (p.nt > 128) copy_scales<PAIR>(tmem + SFB_COL + 4, ds + (1024 >> 4));
+            if (PAIR) mma_commit_pair(smem_u32(&sf_empty[sf]), 3);
+            else mma_commit(smem_u32(&sf_empty[sf]));
+          }
+          __syncwarp();
+          if (++sf == SF_STAGES) sf = 0, sf_par ^= 1;
         }
         if (!(go = mbar_wait_warp(smem_u32(&full_bar[s]), par, aborted, ran_out))) {
           if (ran_out) gb_err::report(ERR_WAIT_FULL), *aborted = 1;
           break;
         }
         tc_fence_after_sync();
-        const uint64_t da = da0 + (uint64_t)(s * (stage_bytes >> 4)), db = db0 + (uint64_t)(s * (stage_bytes >> 4));
+        const bool tile_ends = q.b + 1 == p.blocks || i + 1 == n_units;
         if (leader) {
+          const uint64_t da = da0 + (uint64_t)(s * (stage_bytes >> 4)), db = db0 + (uint64_t)(s * (stage_bytes >> 4));
+          const uint32_t id = (uint32_t)(q.b & 3), idesc = idesc0 | (id << 4) | (id << 29);
+          const bool more = i > 0 && q.b > 0;
 #pragma unroll
-          for (int k = 0; k < BK / 32; ++k) {
-            if (PAIR) mma_f8_pair(tmem + as * 256, da + 2 * k, db + 2 * k, idesc, k > 0);
-            else mma_f8(tmem + as * 256, da + 2 * k, db + 2 * k, idesc, k > 0);
+          for (int k = 0; k < BK / 32; ++k)
+            mma_mxf8<PAIR>(tmem + as * ACC_STRIDE, da + 2 * k, db + 2 * k, idesc, tmem + SFA_COL, tmem + SFB_COL, more || k > 0);
+          if (PAIR) mma_commit_pair(smem_u32(&empty_bar[s]), 3);
+          else mma_commit(smem_u32(&empty_bar[s]));
+          if (tile_ends) {
+            if (PAIR) mma_commit_pair(smem_u32(&acc_full[as]), 3);
+            else mma_commit(smem_u32(&acc_full[as]));
           }
-          if (PAIR) mma_commit_pair(smem_u32(&acc_full[as]), 3);
-          else mma_commit(smem_u32(&acc_full[as]));
         }
         __syncwarp();
+        if (tile_ends) ++t;
         if (++s == stages) s = 0, par ^= 1;
       }
     }
-  } else {
-    // ---------------------------------------------------------------- scale, add, write
-    const int ew = warp - 2, quarter = warp & 3, group = ew >> 2;
-    const int col0 = group * CH, cols = max(0, min(CH, p.nt - col0));        // this group's columns of the tile
-    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16) + col0;
-    const bool passes_on = threadIdx.x == 64;
-    float acc[CH];
-    gb::pdl_wait();          // the scales and, for ADD, the output
-    int tile = (int)(u_begin / p.blocks), b = (int)(u_begin % p.blocks), from = b;
-    int i = 0, s = 0;
-    // the scales of a unit: this lane's tokens' and the weight block's
-    constexpr int PER = (CH + 31) / 32;
-    float mine[PER];
-    auto fetch = [&](int t, int blk) {
-      const int m0 = t % p.tiles_m * p.nt + col0, nb = t / p.tiles_m * CTAS + (int)rank;
-      const float w = (nb * BM < p.N) ? p.ws[(size_t)nb * p.blocks + blk] : 0.f;
+  } else if (warp == 2) {
+    // ---------------------------------------------------------------- scales
+    bool go = true, ran_out;
+    int sf = 0, sf_par = 1;
+    gb::pdl_wait();          // the tokens' scales
+    const long long last = u_end;
+    long long u = u_begin;
+    Place q = start;
+    while (u < last) {
+      const int g = q.b >> 2, m0 = q.tile % p.tiles_m * p.nt, nb = q.tile / p.tiles_m * CTAS + (int)rank;
+      // this lane's tokens lane, 32 + lane, ...; lanes 0 to 3: the weights' blocks
+      uint32_t x[8];
 #pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const int c = j * 32 + lane;
-        mine[j] = (c < cols && m0 + c < p.M) ? p.xs[(size_t)blk * p.M + m0 + c] * w : 0.f;
+      for (int j = 0; j < 8; ++j) {
+        const int n = j * 32 + lane;
+        x[j] = n < p.nt && m0 + n < p.M ? p.xs[(size_t)g * p.M + m0 + n] : 0u;
       }
-    };
-    if (n_units > 0) fetch(tile, b);
-    bool ok = true;
-    for (; i < n_units; ++i) {
-      const int as = i & 1;
-      if (b == from) {
-#pragma unroll
-        for (int c = 0; c < CH; ++c) acc[c] = 0.f;
+      const int wb = 4 * g + lane;
+      uint32_t w = lane < 4 && wb < p.blocks && nb * BM < p.N ? scale_byte(p.ws[(size_t)nb * p.blocks + wb]) << (8 * lane) : 0u;
+      w |= __shfl_xor_sync(0xffffffffu, w, 1);
+      w |= __shfl_xor_sync(0xffffffffu, w, 2);
+      w = __shfl_sync(0xffffffffu, w, 0);
+      if (!(go = mbar_wait_warp(smem_u32(&sf_empty[sf]), sf_par, aborted, ran_out))) {
+        if (ran_out) gb_err::report(ERR_WAIT_EMPTY), *aborted = 1;
+        break;
       }
-      float* sc = scale_s[ew][as];
-#pragma unroll
-      for (int j = 0; j < PER; ++j)
-        if (j * 32 + lane < CH) sc[j * 32 + lane] = mine[j];
+      uint4* to = reinterpret_cast<uint4*>(smem_raw + (sf_at - smem_u32(smem_raw)) + sf * SF_BYTES) + lane;
+      to[0] = make_uint4(w, w, w, w);
+      to[32] = make_uint4(x[0], x[1], x[2], x[3]);
+      to[64] = make_uint4(x[4], x[5], x[6], x[7]);
+      fence_proxy_async();            // the tensor core reads them through the async proxy
       __syncwarp();
-      const bool tile_ends = b + 1 == p.blocks;
-      if (i + 1 < n_units) fetch(tile_ends ? tile + 1 : tile, tile_ends ? 0 : b + 1);
+      if (lane == 0) {
+        if (rank == 0) mbar_arrive(smem_u32(&sf_full[sf]));
+        else mbar_arrive_cluster(map_to_rank(smem_u32(&sf_full[sf]), 0));
+      }
+      if (++sf == SF_STAGES) sf = 0, sf_par ^= 1;
+      const int to_next = min(4 - (q.b & 3), p.blocks - q.b);
+      u += to_next;
+      q.b += to_next;
+      if (q.b == p.blocks) q.b = 0, ++q.tile;
+    }
+  } else if (warp >= 4) {
+    // ---------------------------------------------------------------- results
+    const int quarter = warp & 3, group = (warp - 4) >> 2;
+    // this group's columns of a tile: half of them, in whole sixteens
+    const int half = (p.nt / 16 + 1) / 2 * 16, col0 = group * half, cols = group ? p.nt - half : half;
+    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16) + col0;
+    gb::pdl_wait();          // for ADD the output; and the scratch that the launch in front may still read
+    bool ok = true;
+    long long u = u_begin;
+    Place q = start;
+#pragma unroll 1
+    for (int t = 0; u < u_end; ++t) {
+      const int as = t & 1;
+      const int n = (int)min((long long)(p.blocks - q.b), u_end - u);          // units of this part
+      const bool whole = n == p.blocks;
       if (ok) {
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_full[as]), (i >> 1) & 1) && !*aborted);
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_full[as]), (t >> 1) & 1) && !*aborted);
         if (!ok) {                // from here on this warp only keeps the others company at the barriers
           if (lane == 0 && !*aborted) gb_err::report(ERR_WAIT_ACCUM);
           *aborted = 1;
         }
       }
       tc_fence_after_sync();
-      if (passes_on && ok) mbar_arrive(smem_u32(&empty_bar[s]));       // the products have read the stage
-      if (++s == stages) s = 0;
+      const int row = (q.tile / p.tiles_m * CTAS + (int)rank) * BM + quarter * 32 + lane;
+      const int m0 = q.tile % p.tiles_m * p.nt + col0;
+      const int have = min(cols, p.M - m0);
+      OT* out = reinterpret_cast<OT*>(p.out) + (size_t)m0 * p.N + row;
+      auto put = [&](int c, float x) {
+        OT* to = out + (size_t)c * p.N;
+        *to = gb::from_float<OT>(ADD ? fmaf(p.alpha, x, gb::to_float(*to)) : x);
+      };
+      const size_t part_floats = (size_t)p.nt * BM;
+      auto part_of = [&](int w, int which) {
+        return p.parts + ((size_t)(w * 2 + which) * CTAS + rank) * part_floats + (size_t)col0 * BM + quarter * 32 + lane;
+      };
+      float* my = part_of(worker, t == 0 ? 0 : 1);
+      if (ok) {
+#pragma unroll 1
+        for (int c0 = 0; c0 < cols; c0 += 16) {
+          uint32_t v[16];
+          tmem_ld_16(lane_addr + as * ACC_STRIDE + c0, v);
+          tmem_ld_wait();
+          if (whole) {
+            if (row < p.N) {
 #pragma unroll
-      for (int c0 = 0; c0 < CH; c0 += CHUNK) {
-        if (c0 >= cols || !ok) break;
-        uint32_t v[CHUNK];
-        tmem_load<CHUNK>(lane_addr + as * 256 + c0, v);
-        tmem_ld_wait();
+              for (int e = 0; e < 16; ++e)
+                if (c0 + e < have) put(c0 + e, __uint_as_float(v[e]));
+            }
+          } else {
 #pragma unroll
-        for (int e = 0; e < CHUNK; e += 4) {
-          const float4 f = *reinterpret_cast<const float4*>(sc + c0 + e);
-          acc[c0 + e] = fmaf(__uint_as_float(v[e]), f.x, acc[c0 + e]);
-          acc[c0 + e + 1] = fmaf(__uint_as_float(v[e + 1]), f.y, acc[c0 + e + 1]);
-          acc[c0 + e + 2] = fmaf(__uint_as_float(v[e + 2]), f.z, acc[c0 + e + 2]);
-          acc[c0 + e + 3] = fmaf(__uint_as_float(v[e + 3]), f.w, acc[c0 + e + 3]);
+            for (int e = 0; e < 16; ++e)
+              if (c0 + e < have) my[(size_t)(c0 + e) * BM] = __uint_as_float(v[e]);
+          }
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          if (rank == 0) mbar_arrive(smem_u32(&acc_empty[as]));
+          else mbar_arrive_cluster(map_to_rank(smem_u32(&acc_empty[as]), 0));
         }
       }
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0 && ok) {
-        if (rank == 0) mbar_arrive(smem_u32(&acc_empty[as]));
-        else mbar_arrive_cluster(map_to_rank(smem_u32(&acc_empty[as]), 0));
-      }
-      if (tile_ends || i + 1 == n_units) {
-        // ---- the end of a tile, or of this worker's part of it
-        const int row = (tile / p.tiles_m * CTAS + (int)rank) * BM + quarter * 32 + lane;
-        const int m0 = tile % p.tiles_m * p.nt + col0;
-        const int have = min(cols, p.M - m0);
-        const bool whole = tile_ends && from == 0;
-        bool write = whole;
-        if (!whole) {
-          const size_t part_floats = (size_t)p.nt * BM;
-          auto part_of = [&](int w, int which) {
-            return p.parts + ((size_t)(w * 2 + which) * CTAS + rank) * part_floats + (size_t)col0 * BM + quarter * 32 + lane;
-          };
-          const long long t0 = (long long)tile * p.blocks;
-          float* my = part_of(worker, tile == (int)(u_begin / p.blocks) ? 0 : 1);
-#pragma unroll
-          for (int c = 0; c < CH; ++c)
-            if (c < have) my[(size_t)c * BM] = acc[c];
+      if (!whole) {
+        __threadfence();
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const long long t0 = (long long)q.tile * p.blocks;
+        const int first = worker_of(p.units, p.workers, t0), last = worker_of(p.units, p.workers, t0 + p.blocks - 1);
+        if (threadIdx.x == 128) {
+          int* counter = p.counters + (size_t)q.tile * CTAS + rank;
+          const int before = atomicAdd(counter, 1);
+          last_s = before == last - first;
+          if (last_s) *counter = 0;          // as the next launch expects it
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (last_s && ok && row < p.N) {
           __threadfence();
-          asm volatile("bar.sync 1, 256;" ::: "memory");
-          const int first = worker_of(p.units, p.workers, t0), last = worker_of(p.units, p.workers, t0 + p.blocks - 1);
-          if (threadIdx.x == 64) {
-            int* counter = p.counters + (size_t)tile * CTAS + rank;
-            const int before = atomicAdd(counter, 1);
-            last_s = before == last - first;
-            if (last_s) *counter = 0;          // as the next launch expects it
-          }
-          asm volatile("bar.sync 1, 256;" ::: "memory");
-          write = last_s != 0;
-          if (write) {
-            __threadfence();
+          // of the workers that share the tile only the first may have begun in front of it. Sixteen columns at a time, all of a
+          // part's loads under way at once.
+          const int which = (int)(first_unit(p.units, p.workers, first) / p.blocks) == q.tile ? 0 : 1;
+#pragma unroll 1
+          for (int c0 = 0; c0 < have; c0 += 16) {
+            float sum[16];
 #pragma unroll
-            for (int c = 0; c < CH; ++c) acc[c] = 0.f;
-            for (int w = first; w <= last; ++w) {
-              const float* part = part_of(w, (int)(first_unit(p.units, p.workers, w) / p.blocks) == tile ? 0 : 1);
+            for (int e = 0; e < 16; ++e) sum[e] = c0 + e < have ? __ldcg(part_of(first, which) + (size_t)(c0 + e) * BM) : 0.f;
+#pragma unroll 2
+            for (int w = first + 1; w <= last; ++w) {
+              const float* part = part_of(w, 0) + (size_t)c0 * BM;
 #pragma unroll
-              for (int c = 0; c < CH; ++c)
-                if (c < have) acc[c] += __ldcg(part + (size_t)c * BM);
+              for (int e = 0; e < 16; ++e) sum[e] += c0 + e < have ? __ldcg(part + (size_t)e * BM) : 0.f;
             }
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (c0 + e < have) put(c0 + e, sum[e]);
           }
         }
-        if (write && ok && row < p.N) {
-          OT* out = reinterpret_cast<OT*>(p.out) + (size_t)m0 * p.N + row;
-#pragma unroll
-          for (int c = 0; c < CH; ++c) {
-            if (c < have) {
-              OT* to = out + (size_t)c * p.N;
-              if (ADD) *to = gb::from_float<OT>(fmaf(p.alpha, acc[c], gb::to_float(*to)));
-              else *to = gb::from_float<OT>(acc[c]);
-            }
-          }
-        }
-        from = 0;
+        // (the flag is read before a next part's first barrier, and written behind it)
       }
-      if (tile_ends) b = 0, ++tile;
-      else ++b;
+      u += n;
+      q.b += n;
+      if (q.b == p.blocks) q.b = 0, ++q.tile;
     }
   }
   tc_fence_before_sync();
@@ -363,20 +425,20 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
 struct MapKey {
   const void* ptr;
   long long rows, cols, pitch;
-  int box_rows;
+  int box;
   bool operator==(const MapKey& o) const {
-    return ptr == o.ptr && rows == o.rows && cols == o.cols && pitch == o.pitch && box_rows == o.box_rows;
+    return ptr == o.ptr && rows == o.rows && cols == o.cols && pitch == o.pitch && box == o.box;
   }
 };
 struct MapKeyHash {
   size_t operator()(const MapKey& k) const {
     return std::hash<const void*>()(k.ptr) ^ (std::hash<long long>()(k.rows) * 31) ^ (std::hash<long long>()(k.cols) * 131) ^
-           (std::hash<long long>()(k.pitch) * 521) ^ (size_t)k.box_rows * 7919;
+           (std::hash<long long>()(k.pitch) * 521) ^ (size_t)k.box * 7919;
   }
 };
 
-// [rows, cols] bytes, rows `pitch` apart, through boxes of box_rows x 128 bytes with the 128-byte swizzle; outside it is zeros. (A map
-// says where a matrix lies and how long it is, not what it holds.)
+// [rows, cols] bytes, rows `pitch` apart, through boxes of `box` rows x 128 bytes with the 128-byte swizzle; outside it
+// is zeros. (A map says where a matrix lies and how long it is, not what it holds.)
 int tensor_map(const void* ptr, long long rows, long long cols, long long pitch, int box_rows, CUtensorMap* out) {
   static std::mutex mu;
   static std::unordered_map<MapKey, CUtensorMap, MapKeyHash> cache;
@@ -394,9 +456,8 @@ int tensor_map(const void* ptr, long long rows, long long cols, long long pitch,
   cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
   CUtensorMap m;
-  const CUresult r = fn(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = fn(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box,
+                        estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return gb::fail(GB_CUDA_ERROR, "cuTensorMapEncodeTiled failed with code %d for a %lld x %lld matrix of codes", (int)r, rows, cols);
   if (cache.size() > 4096) cache.clear();
@@ -407,7 +468,7 @@ int tensor_map(const void* ptr, long long rows, long long cols, long long pitch,
 
 struct Plan {
   bool pair;
-  int nt, ch, stages, workers;
+  int nt, stages, workers;
   int tiles_m, tiles_n;
   long long units;
 };
@@ -415,16 +476,14 @@ struct Plan {
 Plan make_plan(int M, int N, int K) {
   Plan q;
   q.pair = M > 512;
-  const int tiles = (M + 255) / 256, step = q.pair ? 32 : 16;
-  q.nt = ((M + tiles - 1) / tiles + step - 1) / step * step;
+  const int tiles = (M + MAX_NT - 1) / MAX_NT;
+  q.nt = ((M + tiles - 1) / tiles + 15) / 16 * 16;
   q.tiles_m = (M + q.nt - 1) / q.nt;
   const int ctas = q.pair ? 2 : 1, blocks = (K + BK - 1) / BK;
   q.tiles_n = (N + BM * ctas - 1) / (BM * ctas);
   q.units = (long long)q.tiles_m * q.tiles_n * blocks;
-  const int half = (q.nt + 1) / 2;
-  q.ch = half <= 8 ? 8 : half <= 16 ? 16 : half <= 32 ? 32 : half <= 64 ? 64 : half <= 96 ? 96 : 128;
   const int stage = (BM + q.nt / ctas) * BK;
-  const int most = (SMEM_LIMIT - 1024 - 2048 - 8 * 2 * q.ch * 4) / stage;
+  const int most = (SMEM_LIMIT - 1024 - STATIC_BYTES - SF_STAGES * SF_BYTES) / stage;
   q.stages = most < MAX_STAGES ? most : MAX_STAGES;
   const int room = tc_host::sm_count() / ctas;
   q.workers = (int)(q.units < room ? q.units : room);
@@ -434,26 +493,26 @@ Plan make_plan(int M, int N, int K) {
 long long part_bytes(const Plan& q) { return (long long)q.workers * 2 * (q.pair ? 2 : 1) * q.nt * BM * 4; }
 long long counter_bytes(const Plan& q) { return ((long long)q.tiles_m * q.tiles_n * (q.pair ? 2 : 1) * 4 + 255) / 256 * 256; }
 
-template <bool PAIR, int CH, typename OT, bool ADD>
+template <bool PAIR, typename OT, bool ADD>
 int launch(const Plan& q, const CUtensorMap& wm, const CUtensorMap& xm, const Args& a, cudaStream_t stream) {
-  auto kernel = gemm_f8_kernel<PAIR, CH, OT, ADD>;
+  auto kernel = gemm_f8_kernel<PAIR, OT, ADD>;
   static gb::OncePerDevice configured;
   if (configured.needed()) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT - 2048 - 8 * 2 * CH * 4);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT - STATIC_BYTES);
     if (e != cudaSuccess) return gb::fail(GB_CUDA_ERROR, "gemm_f8: %s", cudaGetErrorString(e));
     configured.done();
   }
   const int ctas = PAIR ? 2 : 1;
-  const size_t smem = (size_t)q.stages * (BM + q.nt / ctas) * BK + 1024;
+  const size_t smem = (size_t)q.stages * (BM + q.nt / ctas) * BK + SF_STAGES * SF_BYTES + 1024;
   return gb::check_pdl_launch(gb::launch_pdl(kernel, dim3((unsigned)(q.workers * ctas)), dim3(THREADS), smem, stream, dim3(ctas), wm, xm, a),
                               "gemm_f8");
 }
 
-template <bool PAIR, int CH>
+template <bool PAIR>
 int launch_out(const Plan& q, const CUtensorMap& wm, const CUtensorMap& xm, const Args& a, int out_tag, bool add, cudaStream_t stream) {
-  if (add) return launch<PAIR, CH, float, true>(q, wm, xm, a, stream);
-  if (out_tag == GB_F32) return launch<PAIR, CH, float, false>(q, wm, xm, a, stream);
-  return launch<PAIR, CH, __nv_bfloat16, false>(q, wm, xm, a, stream);
+  if (add) return launch<PAIR, float, true>(q, wm, xm, a, stream);
+  if (out_tag == GB_F32) return launch<PAIR, float, false>(q, wm, xm, a, stream);
+  return launch<PAIR, __nv_bfloat16, false>(q, wm, xm, a, stream);
 }
 
 }  // namespace
@@ -480,19 +539,11 @@ GB_EXPORT int gb_f8_gemm(const void* codes, int pitch, const void* xs, const voi
   if (rc) return rc;
   rc = tensor_map(codes, M, pitch, pitch, q.nt / ctas, &xm);
   if (rc) return rc;
-  Args a{(const float*)xs, (const float*)ws, out, (float*)parts, (int*)counters, M, N, (K + BK - 1) / BK, q.nt, q.tiles_m, q.stages,
+  Args a{(const uint32_t*)xs, (const float*)ws, out, (float*)parts, (int*)counters, M, N, (K + BK - 1) / BK, q.nt, q.tiles_m, q.stages,
          q.workers, q.units, accumulate ? alpha : 1.0f};
   const cudaStream_t st = (cudaStream_t)stream;
   const bool add = accumulate != 0;
-  if (q.pair) return launch_out<true, 128>(q, wm, xm, a, out_tag, add, st);
-  switch (q.ch) {
-    case 8: return launch_out<false, 8>(q, wm, xm, a, out_tag, add, st);
-    case 16: return launch_out<false, 16>(q, wm, xm, a, out_tag, add, st);
-    case 32: return launch_out<false, 32>(q, wm, xm, a, out_tag, add, st);
-    case 64: return launch_out<false, 64>(q, wm, xm, a, out_tag, add, st);
-    case 96: return launch_out<false, 96>(q, wm, xm, a, out_tag, add, st);
-    default: return launch_out<false, 128>(q, wm, xm, a, out_tag, add, st);
-  }
+  return q.pair ? launch_out<true>(q, wm, xm, a, out_tag, add, st) : launch_out<false>(q, wm, xm, a, out_tag, add, st);
 }
 
 GB_EXPORT int gb_f8_gemm_error_check() { return gb_err::fetch_and_clear(); }

@@ -2,8 +2,7 @@
 
 A scale is a power of two, 2^e with the smallest e >= -100 for which ``448 * 2^e`` is at least the block's largest magnitude,
 so that dividing by it is exact and a value is rounded once. Blocks are 128 x 128 of a weight, 128 channels of a token, and a
-page of one key/value head of the cache. The kernels take scales that are not powers of two as well (a checkpoint's), but
-for those of cache pages that they write themselves.
+page of one key/value head of the cache.
 """
 from __future__ import annotations
 
@@ -21,7 +20,7 @@ E4M3 = torch.float8_e4m3fn
 
 class Float8Weight(NamedTuple):
     """A matrix in 8 bits: ``values [N, K]`` (E4M3, rows of unit stride that start on 16 bytes) and ``scales
-    [ceil(N / 128), ceil(K / 128)]`` (float32): ``w[n, k] = values[n, k] * scales[n // 128, k // 128]``."""
+    [ceil(N / 128), ceil(K / 128)]`` (float32, powers of two): ``w[n, k] = values[n, k] * scales[n // 128, k // 128]``."""
     values: torch.Tensor
     scales: torch.Tensor
 
@@ -95,7 +94,8 @@ class Float8Ops:
     def linear_float8(self, a, w, out, accumulate: bool = False, alpha: float = 1.0, ws=None):
         """``out[M, N] (+)= q(a) @ w^T``: ``w`` a ``Float8Weight`` (or a pair of its two tensors), ``a [M, K]`` bfloat16 or float32, its
         rows rounded to 8 bits with a scale per token and 128 channels (``q``). Sums are 32-bit; ``out`` is bfloat16 or float32,
-        and float32 where ``accumulate`` adds ``alpha * product`` to what is there."""
+        and float32 where ``accumulate`` adds ``alpha * product`` to what is there. A scale of the weights that is no positive power of two
+        (``float8_weight`` makes none) turns the results of its 128 rows into NaN."""
         values, scales = w
         self._on_device(a, values, scales, out)
         _need(a.dim() == 2 and values.dim() == 2 and out.dim() == 2, "linear_float8: operands must be matrices")
@@ -119,7 +119,7 @@ class Float8Ops:
         L = self.float8_lib
         pitch = (K + 15) // 16 * 16
         codes = self._scratch8("float8_codes", (M, pitch), torch.uint8, ws)
-        rows = self._scratch8("float8_scales", ((K + BLOCK - 1) // BLOCK, M), torch.float32, ws)
+        rows = self._scratch8("float8_scales", ((K + 4 * BLOCK - 1) // (4 * BLOCK), M, 4), torch.uint8, ws)
         stream = self._stream()
         self._check(L, L.gb_f8_quantize_rows(a.data_ptr(), _tag(a, "linear_float8 input"), a.stride(0), M, K, codes.data_ptr(), pitch,
                                              rows.data_ptr(), stream), "quantize_rows")

@@ -78,16 +78,22 @@ def test_products_accumulate(ops, M, N, K, dtype):
 
 
 def test_products_of_strided_rows_and_scales_of_any_size(ops):
-    """Tokens as a slice of wider rows that start on two bytes; weights with scales that are no powers of two, as a checkpoint has."""
+    """Tokens as a slice of wider rows that start on two bytes; scales far apart; one that is no power of two spoils its rows, loudly."""
     M, N, K = 37, 200, 333
     a, w = operands(M, N, K, torch.bfloat16, seed=2)
     wide = torch.zeros(M, K + 10, dtype=torch.bfloat16)
     wide[:, 3:3 + K] = a
     w8 = ops.float8_weight(w.cuda())
-    w8 = type(w8)(w8.values, w8.scales * torch.rand(w8.scales.shape, generator=gen(4)).cuda().add(0.5))
+    w8 = type(w8)(w8.values, w8.scales * torch.pow(2.0, torch.randint(-30, 30, w8.scales.shape, generator=gen(4)).float()).cuda())
     out = torch.empty(M, N, dtype=torch.float32, device="cuda")
     ops.linear_float8(wide.cuda()[:, 3:3 + K], w8, out)
     check_product(out, a, w8)
+    for wrong in (w8.scales[1, 2].item() * 1.5, -1.0, 0.0, math.nan):
+        spoilt = w8.scales.clone()
+        spoilt[1, 2] = wrong
+        ops.linear_float8(wide.cuda()[:, 3:3 + K], (w8.values, spoilt), out)
+        assert torch.isnan(out[:, 128:]).all()
+        check_product(out[:, :128], a, type(w8)(w8.values[:128], w8.scales[:1]))
 
 
 def test_codes_at_the_ends_of_their_range(ops):
