@@ -11,10 +11,11 @@
 // The weights' rows are the rows of the products (128 a CTA), the tokens their columns, up to 240 a tile: a weight is fetched once for
 // all of a tile's tokens, and a step of a few tokens multiplies no padding but to 16.
 //
-// Work is dealt in units of (tile, block), tile by tile, an equal stretch to every CTA (or pair of CTAs): few tokens on a wide
-// weight are bound by how evenly the weights' bytes are shared out, and many tokens leave no ragged last round. A tile that falls to
-// several workers is summed by the one that finishes last: each writes its part to scratch memory and counts itself; the last adds the
-// parts in the order of the channels, whoever it is, so that results do not depend on the order of arrival.
+// Tiles are dealt in turn to the workers (a CTA, or a pair of CTAs) while there is a whole round of them, neighbours (the same weights, other
+// tokens) at the same time, so that L2 holds what is in use. What is left is dealt in units of (tile, block), an equal stretch
+// to every worker: few tokens on a wide weight are bound by how evenly the weights' bytes are shared out, and many tokens leave no ragged
+// last round. A tile that falls to several workers is summed by the one that finishes last: each writes its part to scratch memory and
+// counts itself; the last adds the parts in the order of the channels, whoever it is, so that results do not depend on the order of arrival.
 //
 // PAIR: two CTAs of a cluster multiply 256 weight rows by up to 240 tokens (cta_group::2), each fetching half of the tokens' codes.
 //   warp 0     TMA: a box of 128 bytes (128 channels) by 128 weight rows and one by the tokens, a ring of stages. Weights are asked for
@@ -29,6 +30,8 @@
 #include "error_word.cuh"
 #include "tc_common.cuh"
 #include "tc_host.cuh"
+
+#include <cmath>
 
 namespace {
 
@@ -52,8 +55,9 @@ struct Args {
   int* counters;            // [tiles * CTAs of a worker], zero between launches
   int M, N, blocks;
   int nt, tiles_m;          // tokens per tile (a multiple of 16), tiles of tokens
-  int stages, workers;
-  long long units;
+  int stages, workers, rounds;      // rounds: whole tiles for every worker
+  long long units;          // those of the tiles behind the rounds,
+  int share;                // and the workers that share these
   float alpha;
 };
 
@@ -103,10 +107,26 @@ __device__ __forceinline__ int worker_of(long long units, int workers, long long
   return w;
 }
 
-struct Place {
-  int tile, b;
-  __device__ __forceinline__ void next(int blocks) {
-    if (++b == blocks) b = 0, ++tile;
+// A worker's walk: tiles worker, worker + workers, ... of the rounds, then its stretch of the rest.
+struct Walk {
+  int tile, b, i, n;          // where it is; units done, units in all
+  int rest_tile, rest_b, tile0, in_rounds, blocks, step;
+  __device__ __forceinline__ void start(const Args& p, int worker) {
+    blocks = p.blocks, step = p.workers, tile0 = p.rounds * p.workers, in_rounds = p.rounds * p.blocks;
+    const long long from = worker < p.share ? first_unit(p.units, p.share, worker) : 0, to = worker < p.share ? first_unit(p.units, p.share, worker + 1) : 0;
+    rest_tile = tile0 + (int)(from / blocks), rest_b = (int)(from % blocks);
+    i = 0, n = in_rounds + (int)(to - from);
+    tile = p.rounds > 0 ? worker : rest_tile, b = p.rounds > 0 ? 0 : rest_b;
+  }
+  __device__ __forceinline__ bool more() const { return i < n; }
+  __device__ __forceinline__ bool begins() const { return b == 0 || i == in_rounds; }          // a tile, or this worker's part of one
+  __device__ __forceinline__ int left() const { return min(blocks - b, n - i); }               // units of it from here on
+  __device__ __forceinline__ void advance(int k) {       // by up to left()
+    i += k, b += k;
+    if (b < blocks) return;
+    b = 0;
+    if (tile >= tile0) ++tile;
+    else if ((tile += step) >= tile0) tile = rest_tile, b = rest_b;
   }
 };
 
@@ -127,9 +147,8 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const int stages = p.stages;
   const uint32_t sf_at = ring + stages * stage_bytes;              // behind the ring: the scales on their way
-  const long long u_begin = first_unit(p.units, p.workers, worker), u_end = first_unit(p.units, p.workers, worker + 1);
-  const int n_units = (int)(u_end - u_begin);
-  const Place start = {(int)(u_begin / p.blocks), (int)(u_begin % p.blocks)};
+  Walk q;
+  q.start(p, worker);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
@@ -171,32 +190,31 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
     // ---------------------------------------------------------------- producer
     const bool leader = elect_one();
     bool go = true, ran_out;
-    auto load_w = [&](int s, const Place& q) {
+    auto load_w = [&](int s, const Walk& q) {
       const uint32_t full = smem_u32(&full_bar[s]), bar = PAIR ? map_to_rank(full, 0) : full;
       const int row = (q.tile / p.tiles_m * CTAS + (int)rank) * BM;
       if (rank == 0) mbar_arrive_expect_tx(full, CTAS * stage_bytes);
       if (PAIR) tma_load_2d_pair(ring + s * stage_bytes, &w_map, bar, q.b * BK, row);
       else tma_load_2d(ring + s * stage_bytes, &w_map, bar, q.b * BK, row);
     };
-    auto load_x = [&](int s, const Place& q) {
+    auto load_x = [&](int s, const Walk& q) {
       const uint32_t full = smem_u32(&full_bar[s]), bar = PAIR ? map_to_rank(full, 0) : full;
       const int row = q.tile % p.tiles_m * p.nt + (int)rank * x_rows;
       if (PAIR) tma_load_2d_pair(ring + s * stage_bytes + BM * BK, &x_map, bar, q.b * BK, row);
       else tma_load_2d(ring + s * stage_bytes + BM * BK, &x_map, bar, q.b * BK, row);
     };
     // the first stages' weights before the wait for the kernel that makes the codes
-    const int early = min(stages, n_units);
-    Place q = start;
-    for (int i = 0; i < early; ++i, q.next(p.blocks))
-      if (leader) load_w(i, q);
+    const int early = min(stages, q.n);
+    Walk ahead = q;
+    for (; ahead.i < early; ahead.advance(1))
+      if (leader) load_w(ahead.i, ahead);
     __syncwarp();
     gb::pdl_wait();
-    q = start;
-    for (int i = 0; i < early; ++i, q.next(p.blocks))
-      if (leader) load_x(i, q);
+    for (; q.i < early; q.advance(1))
+      if (leader) load_x(q.i, q);
     __syncwarp();
     int s = 0, par = 0;
-    for (int i = early; i < n_units && go; ++i, q.next(p.blocks)) {
+    for (; q.more() && go; q.advance(1)) {
       if (!(go = mbar_wait_warp(smem_u32(&empty_bar[s]), par, aborted, ran_out))) {
         if (ran_out) gb_err::report(ERR_WAIT_EMPTY), *aborted = 1;
         break;
@@ -205,7 +223,7 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
       __syncwarp();
       if (++s == stages) s = 0, par ^= 1;
     }
-    if (leader && *aborted && n_units > 0) {
+    if (leader && *aborted && q.n > 0) {
       // wind down: the copies in flight need microseconds to land; two milliseconds before the shared memory is given up
       const unsigned long long t0 = globaltimer_ns();
       while (globaltimer_ns() - t0 < 2000000ull) {}
@@ -218,16 +236,16 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
       const bool leader = elect_one();
       bool go = true, ran_out;
       int s = 0, par = 0, sf = 0, sf_par = 0, t = 0;         // t: tiles (or parts) begun
-      Place q = start;
-      for (int i = 0; i < n_units; ++i, q.next(p.blocks)) {
+      for (; q.more(); q.advance(1)) {
         const int as = t & 1;
-        if (i == 0 || q.b == 0) {          // a tile begins: both epilogue groups have read this accumulator
+        const bool begins = q.begins(), tile_ends = q.left() == 1;
+        if (begins) {                      // a tile begins: both epilogue groups have read this accumulator
           if (!(go = mbar_wait_warp(smem_u32(&acc_empty[as]), ((t >> 1) & 1) ^ 1, aborted, ran_out))) {
             if (ran_out) gb_err::report(ERR_WAIT_ACCUM), *aborted = 1;
             break;
           }
         }
-        if (i == 0 || (q.b & 3) == 0) {    // the scales of up to four blocks
+        if (begins || (q.b & 3) == 0) {    // the scales of up to four blocks
           if (!(go = mbar_wait_warp(smem_u32(&sf_full[sf]), sf_par, aborted, ran_out))) {
             if (ran_out) gb_err::report(ERR_WAIT_FULL), *aborted = 1;
             break;
@@ -249,14 +267,12 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
           break;
         }
         tc_fence_after_sync();
-        const bool tile_ends = q.b + 1 == p.blocks || i + 1 == n_units;
         if (leader) {
           const uint64_t da = da0 + (uint64_t)(s * (stage_bytes >> 4)), db = db0 + (uint64_t)(s * (stage_bytes >> 4));
           const uint32_t id = (uint32_t)(q.b & 3), idesc = idesc0 | (id << 4) | (id << 29);
-          const bool more = i > 0 && q.b > 0;
 #pragma unroll
           for (int k = 0; k < BK / 32; ++k)
-            mma_mxf8<PAIR>(tmem + as * ACC_STRIDE, da + 2 * k, db + 2 * k, idesc, tmem + SFA_COL, tmem + SFB_COL, more || k > 0);
+            mma_mxf8<PAIR>(tmem + as * ACC_STRIDE, da + 2 * k, db + 2 * k, idesc, tmem + SFA_COL, tmem + SFB_COL, !begins || k > 0);
           if (PAIR) mma_commit_pair(smem_u32(&empty_bar[s]), 3);
           else mma_commit(smem_u32(&empty_bar[s]));
           if (tile_ends) {
@@ -274,10 +290,7 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
     bool go = true, ran_out;
     int sf = 0, sf_par = 1;
     gb::pdl_wait();          // the tokens' scales
-    const long long last = u_end;
-    long long u = u_begin;
-    Place q = start;
-    while (u < last) {
+    while (q.more()) {
       const int g = q.b >> 2, m0 = q.tile % p.tiles_m * p.nt, nb = q.tile / p.tiles_m * CTAS + (int)rank;
       // this lane's tokens lane, 32 + lane, ...; lanes 0 to 3: the weights' blocks
       uint32_t x[8];
@@ -306,10 +319,7 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
         else mbar_arrive_cluster(map_to_rank(smem_u32(&sf_full[sf]), 0));
       }
       if (++sf == SF_STAGES) sf = 0, sf_par ^= 1;
-      const int to_next = min(4 - (q.b & 3), p.blocks - q.b);
-      u += to_next;
-      q.b += to_next;
-      if (q.b == p.blocks) q.b = 0, ++q.tile;
+      q.advance(min(4 - (q.b & 3), q.left()));
     }
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- results
@@ -319,12 +329,10 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
     const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16) + col0;
     gb::pdl_wait();          // for ADD the output; and the scratch that the launch in front may still read
     bool ok = true;
-    long long u = u_begin;
-    Place q = start;
 #pragma unroll 1
-    for (int t = 0; u < u_end; ++t) {
+    for (int t = 0; q.more(); ++t) {
       const int as = t & 1;
-      const int n = (int)min((long long)(p.blocks - q.b), u_end - u);          // units of this part
+      const int n = q.left();          // units of this part
       const bool whole = n == p.blocks;
       if (ok) {
         ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_full[as]), (t >> 1) & 1) && !*aborted);
@@ -346,7 +354,7 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
       auto part_of = [&](int w, int which) {
         return p.parts + ((size_t)(w * 2 + which) * CTAS + rank) * part_floats + (size_t)col0 * BM + quarter * 32 + lane;
       };
-      float* my = part_of(worker, t == 0 ? 0 : 1);
+      float* my = part_of(worker, q.i == q.in_rounds ? 0 : 1);
       if (ok) {
 #pragma unroll 1
         for (int c0 = 0; c0 < cols; c0 += 16) {
@@ -375,10 +383,11 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
       if (!whole) {
         __threadfence();
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        const long long t0 = (long long)q.tile * p.blocks;
-        const int first = worker_of(p.units, p.workers, t0), last = worker_of(p.units, p.workers, t0 + p.blocks - 1);
+        const int rest = q.tile - q.tile0;
+        const long long t0 = (long long)rest * p.blocks;
+        const int first = worker_of(p.units, p.share, t0), last = worker_of(p.units, p.share, t0 + p.blocks - 1);
         if (threadIdx.x == 128) {
-          int* counter = p.counters + (size_t)q.tile * CTAS + rank;
+          int* counter = p.counters + (size_t)rest * CTAS + rank;
           const int before = atomicAdd(counter, 1);
           last_s = before == last - first;
           if (last_s) *counter = 0;          // as the next launch expects it
@@ -388,7 +397,7 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
           __threadfence();
           // of the workers that share the tile only the first may have begun in front of it. Sixteen columns at a time, all of a
           // part's loads under way at once.
-          const int which = (int)(first_unit(p.units, p.workers, first) / p.blocks) == q.tile ? 0 : 1;
+          const int which = (int)(first_unit(p.units, p.share, first) / p.blocks) == rest ? 0 : 1;
 #pragma unroll 1
           for (int c0 = 0; c0 < have; c0 += 16) {
             float sum[16];
@@ -407,9 +416,7 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
         }
         // (the flag is read before a next part's first barrier, and written behind it)
       }
-      u += n;
-      q.b += n;
-      if (q.b == p.blocks) q.b = 0, ++q.tile;
+      q.advance(n);
     }
   }
   tc_fence_before_sync();
@@ -468,9 +475,9 @@ int tensor_map(const void* ptr, long long rows, long long cols, long long pitch,
 
 struct Plan {
   bool pair;
-  int nt, stages, workers;
+  int nt, stages, workers, rounds, share;
   int tiles_m, tiles_n;
-  long long units;
+  long long units;          // of the tiles behind the rounds
 };
 
 Plan make_plan(int M, int N, int K) {
@@ -481,16 +488,32 @@ Plan make_plan(int M, int N, int K) {
   q.tiles_m = (M + q.nt - 1) / q.nt;
   const int ctas = q.pair ? 2 : 1, blocks = (K + BK - 1) / BK;
   q.tiles_n = (N + BM * ctas - 1) / (BM * ctas);
-  q.units = (long long)q.tiles_m * q.tiles_n * blocks;
+  const long long tiles_all = (long long)q.tiles_m * q.tiles_n, units = tiles_all * blocks;
   const int stage = (BM + q.nt / ctas) * BK;
   const int most = (SMEM_LIMIT - 1024 - STATIC_BYTES - SF_STAGES * SF_BYTES) / stage;
   q.stages = most < MAX_STAGES ? most : MAX_STAGES;
   const int room = tc_host::sm_count() / ctas;
-  q.workers = (int)(q.units < room ? q.units : room);
+  q.workers = (int)(units < room ? units : room);
+  q.rounds = (int)(tiles_all / q.workers);
+  // The tiles that are left, each among c workers: c from a model of what they take. A worker takes in about 67 KB a microsecond from L2, all
+  // together 6.4 GB a millisecond from memory; a part of a tile costs its bytes once out and once in, and about 0.7 us each way.
+  const long long rest = tiles_all - (long long)q.rounds * q.workers;
+  q.units = rest * blocks;
+  q.share = 0;
+  double best = 1e30;
+  for (int c = 1; rest > 0 && c <= 16; ++c) {
+    const long long most = rest * c < q.workers ? rest * c : q.workers, share = most < q.units ? most : q.units;
+    const double units_each = (double)((q.units + share - 1) / share);
+    const double unit = fmax(stage / 67e3, (double)share * ctas * BM * BK / 6.4e6);
+    const double parts = share > rest ? (rest * c <= q.workers ? c : (double)share / rest + 1) + 1 : 0;
+    const double us = units_each * unit + parts * (0.7 + (double)(M < q.nt ? M : q.nt) * BM * 4 / 67e3);
+    if (us < best) best = us, q.share = (int)share;
+    if (most == q.workers) break;
+  }
   return q;
 }
 
-long long part_bytes(const Plan& q) { return (long long)q.workers * 2 * (q.pair ? 2 : 1) * q.nt * BM * 4; }
+long long part_bytes(const Plan& q) { return (long long)(q.share > 0 ? q.share : 1) * 2 * (q.pair ? 2 : 1) * q.nt * BM * 4; }
 long long counter_bytes(const Plan& q) { return ((long long)q.tiles_m * q.tiles_n * (q.pair ? 2 : 1) * 4 + 255) / 256 * 256; }
 
 template <bool PAIR, typename OT, bool ADD>
@@ -540,7 +563,7 @@ GB_EXPORT int gb_f8_gemm(const void* codes, int pitch, const void* xs, const voi
   rc = tensor_map(codes, M, pitch, pitch, q.nt / ctas, &xm);
   if (rc) return rc;
   Args a{(const uint32_t*)xs, (const float*)ws, out, (float*)parts, (int*)counters, M, N, (K + BK - 1) / BK, q.nt, q.tiles_m, q.stages,
-         q.workers, q.units, accumulate ? alpha : 1.0f};
+         q.workers, q.rounds, q.units, q.share, accumulate ? alpha : 1.0f};
   const cudaStream_t st = (cudaStream_t)stream;
   const bool add = accumulate != 0;
   return q.pair ? launch_out<true>(q, wm, xm, a, out_tag, add, st) : launch_out<false>(q, wm, xm, a, out_tag, add, st);
