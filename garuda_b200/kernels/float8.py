@@ -37,7 +37,12 @@ _FLOAT8_SIGNATURES = {
     "gb_f8_quantize_rows": [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p],
     "gb_f8_quantize_weight": [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_longlong, c_void_p, c_void_p],
     "gb_f8_append": [c_void_p, c_int, c_longlong, c_void_p, c_int] + [c_void_p] * 7 + [c_int] * 6 + [c_void_p, c_int, c_int, c_void_p],
-    "gb_f8_attention_simple": [c_void_p, c_int] + [c_void_p] * 5 + [c_int] + [c_void_p] * 3 + [c_int] * 5 + [c_float, c_int, c_int, c_void_p],
+    "gb_f8_attention_simple": [c_void_p, c_int] + [c_void_p] * 5 + [c_int] + [c_void_p] * 3 + [c_int] * 5 + [c_float, c_int, c_int, c_int, c_void_p],
+    "gb_f8_attention_decode_takes": [c_int] * 4,
+    "gb_f8_attention_decode_rows": [c_int],
+    "gb_f8_attention_decode": [c_void_p] * 6 + [c_int] + [c_void_p] * 3 + [c_int, c_longlong] + [c_int] * 3 + [c_float] + [c_int] * 3 + [c_void_p] * 3,
+    "gb_f8_attention_decode_error_check": [],
+    "gb_f8_attention_decode_set_error_sink": [c_void_p],
     "gb_f8_gemm": [c_void_p, c_int, c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p,
                    c_void_p, c_void_p],
     "gb_f8_gemm_error_check": [],
@@ -60,7 +65,9 @@ class Float8Ops:
                 fn.argtypes, fn.restype = argtypes, c_int
             L.gb_f8_gemm_scratch_bytes.argtypes = [c_int, c_int, c_int, ctypes.POINTER(c_longlong)]
             L.gb_f8_gemm_scratch_bytes.restype = c_longlong
-            if L.gb_f8_gemm_set_error_sink(self.error_word.data_ptr()):
+            L.gb_f8_attention_decode_scratch.argtypes = [c_int, c_int, c_int, ctypes.POINTER(c_longlong)]
+            L.gb_f8_attention_decode_scratch.restype = c_longlong
+            if L.gb_f8_gemm_set_error_sink(self.error_word.data_ptr()) or L.gb_f8_attention_decode_set_error_sink(self.error_word.data_ptr()):
                 _need(False, "the 8-bit library could not be given the host's error word")
             self._float8 = L
         return self._float8
@@ -74,7 +81,8 @@ class Float8Ops:
     def check_float8_errors(self) -> None:
         """Synchronises, and raises if an 8-bit kernel gave up on a wait since the last check."""
         seen, self.error_word[0] = int(self.error_word[0]), 0
-        code = self.float8_lib.gb_f8_gemm_error_check() or seen
+        L = self.float8_lib
+        code = L.gb_f8_gemm_error_check() or L.gb_f8_attention_decode_error_check() or seen
         _need(not code, f"an 8-bit kernel gave up waiting: code {code}")
 
     # ------------------------------------------------------------------ matrix products
@@ -193,11 +201,25 @@ class Float8Ops:
         _need(block_table.shape[1] * page_size >= max_kv_len, f"{what}: the block table is too narrow for {max_kv_len} positions")
         if T == 0:
             return
-        L = self.float8_lib
-        self._check(L, L.gb_f8_attention_simple(
-            q.data_ptr(), _tag(q, "attention q"), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-            block_table.data_ptr(), block_table.shape[1], cu_q.data_ptr(), kv_lens.data_ptr(), out.data_ptr(), T, R, Hq, Hkv, hd,
-            float(scale), int(window), int(page_size), self._stream()), what)
+        L, g, stream = self.float8_lib, Hq // Hkv, self._stream()
+        above = -1             # requests of more rows (new tokens times heads of a group) than this are still to do
+        if q.dtype == torch.bfloat16 and L.gb_f8_attention_decode_takes(hd, int(page_size), g, R):
+            rows = L.gb_f8_attention_decode_rows(g)
+            if min_q_len * g <= rows:
+                counter_bytes = c_longlong(0)
+                parts = self._scratch8("float8_attention_parts", (int(L.gb_f8_attention_decode_scratch(R, Hkv, hd, ctypes.byref(counter_bytes))),),
+                                       torch.uint8, ws)
+                counters = self._scratch8("float8_attention_counters", (int(counter_bytes.value),), torch.uint8, ws, zero=True)
+                self._check(L, L.gb_f8_attention_decode(
+                    q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(),
+                    block_table.shape[1], cu_q.data_ptr(), kv_lens.data_ptr(), out.data_ptr(), R, k_pool.shape[0], Hq, Hkv, hd, float(scale),
+                    int(window), int(page_size), int(max_kv_len), parts.data_ptr(), counters.data_ptr(), stream), what)
+            above = rows
+        if above < 0 or max_q_len * g > above:
+            self._check(L, L.gb_f8_attention_simple(
+                q.data_ptr(), _tag(q, "attention q"), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                block_table.data_ptr(), block_table.shape[1], cu_q.data_ptr(), kv_lens.data_ptr(), out.data_ptr(), T, R, Hq, Hkv, hd,
+                float(scale), int(window), int(page_size), above, stream), what)
 
 
 def _need(cond, msg):
