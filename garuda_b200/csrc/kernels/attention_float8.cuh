@@ -5,6 +5,9 @@
 
 namespace attn8 {
 
+// A request with at most this many (token, head-of-group) rows is a decode request: each is two of a product's 16 (or 32) columns.
+inline int decode_rows(int g) { return g <= 8 ? 8 : 16; }
+
 struct Params {
   const __nv_bfloat16* q;        // [T, Hq, HD]
   const float *k_scale, *v_scale;        // [pages, Hkv]
@@ -13,11 +16,7 @@ struct Params {
   const int32_t* cu_q;           // [R + 1]
   const int32_t* kv_lens;        // [R]
   int table_width, R, Hq, Hkv, g, window, page;
-  int decode_rows;               // a request with at most this many (token, head-of-group) rows is a decode request
   float scale_log2;              // scale * log2(e)
 };
-
-// One query row of a decode request is two rows of a product (see attention_float8_decode.cu): eight a product, sixteen for wide groups.
-inline int decode_rows(int g) { return g <= 8 ? 8 : 16; }
 
 }  // namespace attn8

@@ -3,26 +3,34 @@
 //   s_j = (q . k8_j) * ks(page of j) * scale over keys [start, pos];  out = sum_j softmax(s)_j vs(page of j) v8_j
 // (garuda/src/llama/mod.rs:793-818; the window garuda/src/cache/mod.rs:333-338; query head h reads key/value head h / g).
 //
-// Bound by the stream of codes, 2 * HD bytes a key and head: so the codes go from shared memory into the matrix instructions as
-// they are (mma.sync m16n8k32 on E4M3; 1.4 of them a nanosecond and SM here, a tile of 32 keys takes 32), and what has more than four
-// bits is split instead: a query row, bfloat16 scaled by a power of two to a largest of at most 448, is the sum of two E4M3 rows
-// exactly (eight bits of mantissa are four and four; what is 2^-11 of the row's largest and below loses bits that the sum does not
-// see), and a weight exp(s - m) * 256 is a code and 1/32 of another, to 2^-9 of itself down to 2^-16 of the largest weight. The two
-// parts are rows i and i + 8 of one product, which has 16 rows anyway. Sums, maxima and denominators are 32-bit.
+// Bound by the stream of codes, 2 * HD bytes a key and head, so they go from shared memory into the matrix instructions as they are
+// (tcgen05.mma kind f8f6f4, 32-bit sums), and what has more than four bits is split instead: a query row, scaled by a power of two to a largest
+// of at most 448, is the sum of two E4M3 rows (a bfloat16's eight bits are four and four; what is 2^-11 of the row's largest and below
+// loses bits that the sum does not see), and a weight exp(s - m) is three codes, the second and third in units of 1/32 and 1/1024: twelve
+// bits, down to 2^-24 of the reference. (Groups of more than eight heads: two codes, nine bits, down to 2^-22, and a reference that
+// follows every larger score.) Products of one tile of 128 keys:
+//   S^T [128 keys, N] = K [128, HD] * Q [N, HD]^T         N = 16 (or 32): the rows' codes, then what these leave
+//   O [rows, HD]     += P [rows, 128] * V [128, HD]       P's rows: the weights' first codes, then the others; V as it lies, keys along its
+//                                                         rows. The products' other rows (128 in all) read whatever lies behind P, and
+//                                                         nobody reads their sums
+// A thread has a key: its N sums from tensor memory are its scores with all rows, so the 128 threads share out the exponentials evenly, and
+// what is per key (page, scales, mask) is per thread. (mma.sync on E4M3 takes 860 instructions for 32 keys, as this hardware has no
+// such product and converts; with the codes converted to halves by hand 700; both were bound by instructions at 5.0 TB/s and below. Here
+// 128 keys take some 500.) Maxima and denominators are 32-bit.
 //
-// Scales cost nothing per key: a page's ks goes into the factor that the exponent's multiply-add has anyway, its vs (a power of two)
-// into the constant of the same; the denominator takes it out again per sixteen keys. The accumulators hold sums in units of the
-// largest vs so far.
+// The maximum that weights refer to is common to the tile's 128 keys. It follows the running maximum only when some score exceeds it by more
+// than 2^3 (a vote a tile; following at once cost 0.8 us a time, some 14 times in 60 tiles), and then the sums in tensor
+// memory are brought to it. Scales cost nothing per key: ks goes into the score's factor, vs, as a power of two, into the
+// exponent, and the denominator takes it out again. The sums are in units of the largest vs so far.
 //
-// Work: the tiles (32 keys) of all requests and heads in a row, an equal stretch to every CTA, so that requests of unequal length do
-// not wait for the longest. Within a CTA a stretch's tiles go to the warps in turn; every warp has a ring of stages of its own that
-// TMA fills (a box per page, swizzled as ldmatrix undoes it), asked for as soon as a stage is free, across the borders of requests.
-// At a request's end the warps' sums are merged in shared memory; a request that falls to several CTAs is merged by the one that
-// finishes last, in their order, from scratch memory: results do not depend on who that is.
-//
-// The keys' order within a tile is free (sums run over it), and is chosen so that the scores lie in the lanes where the second product
-// wants its weights: slot s of sixteen holds key T(s) = s ^ ((s & 8) >> 2), which also keeps ldmatrix's eight rows on distinct
-// banks for keys and for values.
+// Work: the tiles of all requests and heads in a row, an equal stretch to every CTA, so that requests of unequal length do not wait for
+// the longest; a request that falls to several CTAs is merged by the one that finishes last, in their order, from scratch memory, so
+// that results do not depend on who that is. Within a CTA, the copies, the scores' products and the queries of the next request's head
+// run ahead across the border.
+//   warp 0     TMA: a box a page (swizzled) into a ring of stages; looks up pages and scales four tiles at a time, two steps ahead
+//   warp 1     one elected lane issues the products: S^T of a tile, then O += P V of the tile before
+//   warps 2-5  scores, maxima, weights; the next head's queries as codes; results
+// Two CTAs an SM (N = 16; one with N = 32). Every wait is bounded.
 #include "attention_float8.cuh"
 #include "error_word.cuh"
 #include "tc_common.cuh"
@@ -33,20 +41,26 @@ namespace {
 using namespace tc;
 using attn8::Params;
 
-constexpr int TK = 32;                  // keys per tile
-constexpr int WARPS = 4, THREADS = 32 * WARPS;
+constexpr int KT = 128;                 // keys per tile
+constexpr int THREADS = 192;
 constexpr int MAX_ROWS = 16;
-constexpr unsigned long long DRAIN_LIMIT_NS = 20000000ull;
+constexpr int SEGMENT = 2;              // what a request's head costs beside its tiles, in tiles
+constexpr uint32_t O_COL = 64, TMEM_COLS = 256;          // tensor memory: two buffers of S^T, then O
 
-template <int HD, int MT>
+template <int HD, int N>
 struct Shape {
-  static constexpr int ROWS = 8 * MT;
-  static constexpr int OPERAND = TK * HD, STAGE = 2 * OPERAND;          // bytes: keys, values
-  static constexpr int DEPTH = 24 * 1024 / STAGE;                       // stages of a warp's ring: 3 or 6
-  static constexpr int RING = WARPS * DEPTH * STAGE;                    // 96 KB: two CTAs an SM
+  static constexpr int ROWS = N / 2;                                    // query rows
+  static constexpr int OPERAND = KT * HD, STAGE = 2 * OPERAND;          // bytes: keys, values
+  static constexpr int CTAS = N == 16 ? 2 : 1;                          // per SM
+  static constexpr int STAGES = 192 * 1024 / CTAS / STAGE;              // 3 (6) of 32 KB, 6 (12) of 16 KB
+  static constexpr int PARTS = N == 16 ? 3 : 2;                         // codes of a weight
+  // weights go to 2^GROWTH of the reference and are multiplied by 2^UP: codes go to 448
+  static constexpr float GROWTH = PARTS == 3 ? 3.f : 0.f, UP = PARTS == 3 ? 5.f : 8.f;
+  static constexpr int P_BYTES = PARTS * ROWS * KT, Q_BYTES = N * 128;
+  static constexpr int RING_AT = 2 * P_BYTES + 2 * Q_BYTES;
+  static constexpr int BYTES = RING_AT + STAGES * STAGE;
   static constexpr int RS = HD + 2;                                     // a row's sums, maximum, denominator: a part in scratch memory
-  static constexpr int CW = 64 / MT, PASSES = HD / CW;                  // channels that the warps merge at a time
-  static constexpr int MERGE = WARPS * ROWS * CW * 4;                   // 8 KB
+  static_assert(RING_AT % 1024 == 0 && P_BYTES + KT * 128 <= BYTES, "swizzled tiles; P's 128 rows end inside");
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -54,478 +68,624 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
 }
-__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+// Sums in 32 bits, both operands E4M3.
+__device__ __forceinline__ constexpr uint32_t instr_desc_e4m3(int m, int n) {
+  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-// Two 16 x 16 blocks of bytes, transposed: lane l gives row l (of 32); r[0], r[1] hold rows 4 (l % 4) + 0..3 of columns l / 4 and
-// 8 + l / 4 of the first block, r[2], r[3] the same of the second.
-__device__ __forceinline__ void ldmatrix_trans_bytes(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+// Rows of 128 bytes (or of 64) as TMA swizzles them, eight to a group; for keys and queries the contraction lies along the row, for
+// values the rows are the contraction.
+template <int HD>
+__device__ __forceinline__ uint64_t smem_desc_rows(uint32_t addr) {
+  if (HD == 128) return smem_desc_sw128(addr);
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(512 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)4 << 61);
 }
-// Byte offset of 16-byte chunk `c` of row `row` in a tile as TMA swizzled it (rows of 128 bytes, or of 64).
+// Byte offset of 16-byte chunk `c` of row `row` in such a tile.
 template <int HD>
 __device__ __forceinline__ uint32_t swizzled(int row, int c) {
   return HD == 128 ? (uint32_t)(row * 128 + ((c ^ (row & 7)) << 4)) : (uint32_t)(row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
 }
-__device__ __forceinline__ int key_of_slot(int s) { return s ^ ((s & 8) >> 2); }          // within a tile: bit 4 stays
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[N]);
+template <>
+__device__ __forceinline__ void tmem_load<16>(uint32_t addr, uint32_t (&r)[16]) { tmem_ld_16(addr, r); }
+template <>
+__device__ __forceinline__ void tmem_load<32>(uint32_t addr, uint32_t (&r)[32]) { tmem_ld_32(addr, r); }
 
-// Two weights (times 256) as a code and 32 times what it leaves, as a code: hi, lo.
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  uint16_t h;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(h) : "f"(b), "f"(a));
-  const uint32_t back = f8::decode2_f16(h);
-  uint32_t both, left;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(both) : "f"(b), "f"(a));
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(left) : "r"(both), "r"(back));
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(left) : "r"(left), "r"(0x50005000u));          // 32
-  uint16_t l;
-  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(l) : "r"(left));
-  hi = h, lo = l;
+// Two weights as a code, 32 times what that leaves as a code, and (PARTS 3) 32 times what that leaves; in the low byte the first's.
+template <int PARTS>
+__device__ __forceinline__ void split(float a, float b, uint32_t (&code)[PARTS]) {
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) {
+    const uint16_t h = f8::encode2(a, b);
+    code[i] = h;
+    if (i + 1 < PARTS) {
+      const float2 back = f8::decode2(h);
+      a = (a - back.x) * 32.f, b = (b - back.y) * 32.f;
+    }
+  }
 }
+__device__ __forceinline__ void st_shared_u8(uint32_t addr, uint32_t v) { asm volatile("st.shared.u8 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+// Barrier of the four softmax warps; true for all if `mine` is for one.
+__device__ __forceinline__ bool any_of_four(bool mine) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r) : "r"((uint32_t)mine) : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void sync_four() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
 
-// MT: products of eight query rows each (1, or 2 for groups of more than eight heads)
-template <int HD, int MT>
-__global__ void __launch_bounds__(THREADS, 2)
+struct Bars {
+  uint64_t full[12], empty[12], s_ready[2], p_ready[2], pv_done[2], q_ready[2], o_free;
+  uint32_t tmem_base;
+  int abort, last[2];
+  int2 total, scan[6];
+  float2 scales[12][8];            // a stage's ks of each sixteen keys (negative: no page there) and log2 of vs
+  float factor[2][MAX_ROWS];       // per row of a head's queries: 2^e * scale * log2(e)
+  float top[4][MAX_ROWS], corr[MAX_ROWS], vtop[4], lsum[4][MAX_ROWS];
+};
+
+template <int HD, int N>
+__global__ void __launch_bounds__(THREADS, Shape<HD, N>::CTAS)
 attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const Params p,
-                           const int box_rows, const int min_tiles, float* __restrict__ partials, int* __restrict__ counters) {
-  using S = Shape<HD, MT>;
-  constexpr int RS = S::RS, ROWS = S::ROWS, CW = S::CW;
+                           const int min_tiles, float* __restrict__ partials, int* __restrict__ counters) {
+  using S = Shape<HD, N>;
+  constexpr int RS = S::RS, ROWS = S::ROWS, STAGES = S::STAGES;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t full_bar[WARPS * S::DEPTH];
-  __shared__ __align__(16) float4 scale_s[WARPS * S::DEPTH];           // a stage's ks of its sixteens (negative: no page), and log2 vs
-  __shared__ float2 ml_s[WARPS][ROWS];         // the warps' maxima and denominators
-  __shared__ int abort_s, last_s, scan_s[WARPS], total_s;
+  __shared__ Bars bars;
+  uint8_t* const base = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
+  const uint32_t p_at = smem_u32(base), q_at = p_at + 2 * S::P_BYTES, ring = p_at + S::RING_AT;
+  int* const cum = reinterpret_cast<int*>(base + S::BYTES);            // [R + 1]: tiles of a head of the requests in front
+  int* const cost = cum + p.R + 1;                                     // [R + 1]: the same with SEGMENT more for every request with tiles
+  int* const begin_s = cost + p.R + 1;                                 // [R + 1]: cu_q
+  int* const len_s = begin_s + p.R + 1;                                // [R]: kv_lens
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint8_t* ring = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
-  float* red = reinterpret_cast<float*>(ring + S::RING);               // [warps][rows][CW]
-  int* cum = reinterpret_cast<int*>(ring + S::RING + S::MERGE);        // [R + 1]: tiles of a head of the requests in front
-
   if (threadIdx.x == 0) {
-    for (int s = 0; s < WARPS * S::DEPTH; ++s) mbar_init(smem_u32(&full_bar[s]), 1);
-    abort_s = 0;
-    total_s = 0;
+    for (int s = 0; s < STAGES; ++s) mbar_init(smem_u32(&bars.full[s]), 2), mbar_init(smem_u32(&bars.empty[s]), 1);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&bars.s_ready[b]), 1);
+      mbar_init(smem_u32(&bars.p_ready[b]), 128);
+      mbar_init(smem_u32(&bars.pv_done[b]), 1);
+      mbar_init(smem_u32(&bars.q_ready[b]), 128);
+    }
+    mbar_init(smem_u32(&bars.o_free), 32);
+    bars.abort = 0, bars.total = make_int2(0, 0);
     fence_barrier_init();
     fence_proxy_async();
     prefetch_tensormap(&k_map);
     prefetch_tensormap(&v_map);
   }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&bars.tmem_base), TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
   __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = bars.tmem_base;
+  volatile int* aborted = &bars.abort;
   gb::pdl_launch_dependents();
 
   // ---- every request's tiles (the batch's lengths are there before the step's first kernel)
-  auto span = [&](int r, int& lo, int& hi, int& pos0, int& nrows) {          // first and last key that any row reads
-    const int q_len = p.cu_q[r + 1] - p.cu_q[r], kv_len = p.kv_lens[r];
-    nrows = q_len * p.g;
-    pos0 = kv_len - q_len;
-    lo = p.window > 0 ? max(0, pos0 + 1 - p.window) : 0;
-    hi = kv_len - 1;
+  struct Span {
+    int lo, hi, pos0, nrows, q_begin;      // first and last key that any row reads
+  };
+  auto span_of = [&](int q_begin, int q_end, int kv_len) {
+    Span s;
+    s.q_begin = q_begin, s.nrows = (q_end - q_begin) * p.g, s.pos0 = kv_len - (q_end - q_begin);
+    s.lo = p.window > 0 ? max(0, s.pos0 + 1 - p.window) : 0;
+    s.hi = kv_len - 1;
+    return s;
   };
   for (int r0 = 0; r0 < p.R; r0 += THREADS) {
     const int r = r0 + threadIdx.x;
-    int lo, hi, pos0, nrows, n = 0;
+    int n = 0;
     if (r < p.R) {
-      span(r, lo, hi, pos0, nrows);
-      if (nrows > 0 && nrows <= p.decode_rows && hi >= lo) n = hi / TK - lo / TK + 1;
+      const int q0 = p.cu_q[r], q1 = p.cu_q[r + 1], kv = p.kv_lens[r];
+      begin_s[r] = q0, len_s[r] = kv;
+      if (r + 1 == p.R) begin_s[r + 1] = q1;
+      const Span s = span_of(q0, q1, kv);
+      if (s.nrows > 0 && s.nrows <= ROWS && s.hi >= s.lo) n = s.hi / KT - s.lo / KT + 1;
     }
-    int inc = n;
+    int2 inc = make_int2(n, n > 0 ? 1 : 0);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += v;
+      const int u = __shfl_up_sync(0xffffffffu, inc.x, o), v = __shfl_up_sync(0xffffffffu, inc.y, o);
+      if (lane >= o) inc.x += u, inc.y += v;
     }
-    if (lane == 31) scan_s[warp] = inc;
+    if (lane == 31) bars.scan[warp] = inc;
     __syncthreads();
-    int before = total_s;
+    int2 before = bars.total;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w)
-      if (w < warp) before += scan_s[w];
-    if (r < p.R) cum[r] = before + inc - n;
+    for (int w = 0; w < THREADS / 32; ++w)
+      if (w < warp) before.x += bars.scan[w].x, before.y += bars.scan[w].y;
+    before.x += inc.x, before.y += inc.y;          // with this request
+    if (r < p.R) {
+      cum[r] = before.x - n, cost[r] = before.x - n + SEGMENT * (before.y - (n > 0 ? 1 : 0));
+      if (r + 1 == p.R) cum[r + 1] = before.x, cost[r + 1] = before.x + SEGMENT * before.y;
+    }
     __syncthreads();
-    if (threadIdx.x == THREADS - 1) total_s = before + inc;
+    if (threadIdx.x == THREADS - 1) bars.total = before;
     __syncthreads();
   }
-  if (threadIdx.x == 0) cum[p.R] = total_s;
-  __syncthreads();
-  const long long tiles = (long long)total_s * p.Hkv;
-  // as many CTAs as leave each min_tiles, and no more than share a request's head usefully
-  const int workers = (int)max(1ll, min((long long)gridDim.x, tiles / min_tiles));
+  // Stretches are equal in cost: a request's head is its tiles and SEGMENT behind them.
+  const long long tiles = (long long)cum[p.R] * p.Hkv, costs = (long long)cost[p.R] * p.Hkv;
+  const int workers = (int)max(1ll, min((long long)gridDim.x, tiles / min_tiles));          // each has min_tiles or so at least
   const int cta = blockIdx.x;
-  if (cta >= workers || tiles == 0) {
-    gb::pdl_wait();        // the next kernel counts on this one having waited for those in front
-    return;
-  }
-  auto begins_at = [&](int w) { return tiles * w / workers; };
-  const long long a_begin = begins_at(cta), a_end = begins_at(cta + 1);
-  volatile int* aborted = &abort_s;
-
-  // request, head and tile of a tile in the row of all
-  auto locate = [&](long long a, int& r, int& kvh, int& t, int& n) {
+  auto find = [&](const int* sums, long long at) {     // the last request whose heads begin at or before it
     int lo = 0, hi = p.R;
-    while (hi - lo > 1) {
+    while (hi - lo > 1) {              // (of requests without tiles at the same place the last one: it has some)
       const int mid = (lo + hi) >> 1;
-      if ((long long)cum[mid] * p.Hkv <= a) lo = mid;
+      if ((long long)sums[mid] * p.Hkv <= at) lo = mid;
       else hi = mid;
     }
-    r = lo;                        // (of requests without tiles at the same place the last one: it has some)
-    n = cum[r + 1] - cum[r];
-    const int rem = (int)(a - (long long)cum[r] * p.Hkv);
-    kvh = rem / n, t = rem % n;
+    return lo;
   };
+  auto begins_at = [&](int w) -> long long {           // the first tile of worker w's stretch, in the row of all tiles
+    if (w >= workers) return tiles;
+    const long long c = costs * w / workers;
+    const int r = find(cost, c), n = cum[r + 1] - cum[r], rem = (int)(c - (long long)cost[r] * p.Hkv);
+    return (long long)cum[r] * p.Hkv + (long long)(rem / (n + SEGMENT)) * n + min(rem % (n + SEGMENT), n);
+  };
+  const long long a_begin = cta < workers && tiles > 0 ? begins_at(cta) : 0, a_end = cta < workers && tiles > 0 ? begins_at(cta + 1) : 0;
+  const int my_tiles = (int)(a_end - a_begin);
 
-  // ---- this warp's tiles a_begin + warp, + WARPS, ... through its ring. Lane i looks tile `base + i` up and asks for its copies.
-  const int mine_n = (int)((a_end - a_begin - warp + WARPS - 1) / WARPS);
-  const int boxes = TK / box_rows;                 // 1 or 2
-  int looked_up = -32;
-  int pg[2] = {-1, -1}, line = 0, head = 0;
-  float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
-  int issued = 0;
-  auto issue = [&](int t) {
-    if (t >= mine_n) return;
-    issued = t + 1;
-    if (t >= looked_up + 32) {
-      looked_up = t;
-      if (t + lane < mine_n) {
-        int r, tile, n, lo, hi, pos0, nrows;
-        locate(a_begin + warp + (long long)WARPS * (t + lane), r, head, tile, n);
-        span(r, lo, hi, pos0, nrows);
-        const int key0 = (lo / TK + tile) * TK;
-        const int32_t* table = p.block_table + (size_t)r * p.table_width;
-        line = key0 % p.page;
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {              // the page of each sixteen
-          const int key = key0 + 16 * b, slot = key / p.page;
-          const int page = key <= hi && slot < p.table_width ? table[slot] : -1;
-          const size_t where = (size_t)max(page, 0) * p.Hkv + head;
-          // no page: nothing is read there
-          const float ks = page >= 0 ? p.k_scale[where] : -1.f, vs = page >= 0 ? p.v_scale[where] : 1.f;
-          pg[b] = page;
-          const float ev = log2f(vs);
-          if (b == 0) sc.x = ks, sc.z = ev;
-          else sc.y = ks, sc.w = ev;
-        }
-      }
-    }
-    const int s = warp * S::DEPTH + t % S::DEPTH;
-    if (lane == t - looked_up) {
-      const uint32_t bar = smem_u32(&full_bar[s]), kdst = smem_u32(ring + s * S::STAGE), vdst = kdst + S::OPERAND;
-      scale_s[s] = sc;
-      // what the warp read from or wrote to this stage is ordered before the copies that overwrite it
-      fence_proxy_async();
-      mbar_arrive_expect_tx(bar, S::STAGE);
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        if (b >= boxes) break;
-        // a page that is not there (-1) is outside the tensor and reads as zeros
-        tma_load_4d(kdst + b * box_rows * HD, &k_map, bar, 0, boxes == 1 ? line : 0, head, pg[b]);
-        tma_load_4d(vdst + b * box_rows * HD, &v_map, bar, 0, boxes == 1 ? line : 0, head, pg[b]);
-      }
-    }
-    __syncwarp();
+  // A segment: one request's head, or this CTA's part of it: tiles first .. first + count of its n
+  struct Segment {
+    int r, kvh, first, n, count;
   };
-  // Everything that is read comes from the kernels in front, the pages among it: a page that this step writes is encoded again.
+  auto segment_at = [&](long long a) {
+    Segment g;
+    const int lo = find(cum, a);
+    g.r = lo, g.n = cum[lo + 1] - cum[lo];
+    const int rem = (int)(a - (long long)cum[lo] * p.Hkv);
+    g.kvh = rem / g.n, g.first = rem % g.n;
+    g.count = (int)min((long long)(g.n - g.first), a_end - a);
+    return g;
+  };
+  auto span_at = [&](int r) { return span_of(begin_s[r], begin_s[r + 1], len_s[r]); };
+
+  // Everything else comes from the kernels in front, the pages among it: a page that this step writes is encoded again.
   gb::pdl_wait();
-  for (int t = 0; t < S::DEPTH; ++t) issue(t);
 
-  int t = 0;                       // of this warp's tiles
-  for (long long a = a_begin; a < a_end;) {
-    // ---- one request's head (or this CTA's part of it): tiles first .. first + count of its n
-    int r, kvh, first, n, lo, hi, pos0, nrows;
-    locate(a, r, kvh, first, n);
-    span(r, lo, hi, pos0, nrows);
-    const int count = (int)min((long long)(n - first), a_end - a);
-    const int q_begin = p.cu_q[r];
-
-    // the query rows as codes: row lane / 4 (of each eight), hi and lo
-    uint32_t qf[MT][HD / 32][4];
-    float factor[MT];              // of a row's raw products, times ks: 2^e * scale * log2(e)
-    int row_pos[MT], row_start[MT];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const int row = mt * 8 + lane / 4;
-      const bool there = row < nrows;
-      row_pos[mt] = there ? pos0 + row / p.g : -1;
-      row_start[mt] = there && p.window > 0 ? max(0, row_pos[mt] + 1 - p.window) : 0;
-      const __nv_bfloat16* src = p.q + ((size_t)(q_begin + (there ? row / p.g : 0)) * p.Hq + kvh * p.g + (there ? row % p.g : 0)) * HD + 4 * (lane % 4);
-      uint2 raw[HD / 16];
-      float largest = 0.f;
-#pragma unroll
-      for (int c = 0; c < HD / 16; ++c) {
-        raw[c] = there ? *reinterpret_cast<const uint2*>(src + c * 16) : make_uint2(0u, 0u);
-        const float x[4] = {__uint_as_float(raw[c].x << 16), __uint_as_float(raw[c].x & 0xFFFF0000u), __uint_as_float(raw[c].y << 16),
-                            __uint_as_float(raw[c].y & 0xFFFF0000u)};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) largest = fmaxf(largest, fabsf(x[e]));
+  if (my_tiles > 0 && warp == 0) {
+    // ---------------------------------------------------------------- copies
+    // Lane i looks up sixteen keys: block i % 8 of tile i / 8 of four.
+    struct Lookup {
+      int head, key, r, page;      // (r < 0: no tile)
+      float ks, vs;
+    } now, ahead;
+    const int sub = lane & 7, per_page = p.page >> 4;        // sixteens of a page: 1 to 8
+    auto look_pages = [&](Lookup& u, int t0) {
+      u.r = -1, u.page = -1;
+      const int t = t0 + (lane >> 3);
+      if (t >= my_tiles) return;
+      const Segment g = segment_at(a_begin + t);
+      const Span s = span_at(g.r);
+      u.r = g.r, u.head = g.kvh, u.key = (s.lo / KT + g.first) * KT + 16 * sub;
+      // a page of which no key is read is not fetched
+      const int slot = u.key / p.page, first = slot * p.page;
+      if (first <= s.hi && first + p.page > s.lo && slot < p.table_width) u.page = p.block_table[(size_t)g.r * p.table_width + slot];
+    };
+    auto look_scales = [&](Lookup& u) {
+      const size_t where = (size_t)max(u.page, 0) * p.Hkv + (u.r < 0 ? 0 : u.head);
+      u.ks = u.page >= 0 ? p.k_scale[where] : -1.f;
+      u.vs = u.page >= 0 ? p.v_scale[where] : 1.f;
+    };
+    // a stage's barrier takes two arrivals: the copies asked for, the scales written
+    const uint32_t page_bytes = (uint32_t)p.page * HD;
+    auto copy = [&](int t, int s) {
+      const bool there = (lane >> 3) == (t & 3) && now.page >= 0 && sub % per_page == 0;
+      const int pages = __popc(__ballot_sync(0xffffffffu, there));
+      const uint32_t full = smem_u32(&bars.full[s]);
+      if (lane == 0) {
+        if (pages > 0) mbar_arrive_expect_tx(full, 2 * pages * page_bytes);
+        else mbar_arrive(full);
       }
-      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-      const int e2 = f8::scale_exponent(largest);
-      const float inv = f8::power_of_two(-e2);
-      factor[mt] = f8::power_of_two(e2) * p.scale_log2;
-#pragma unroll
-      for (int c = 0; c < HD / 16; ++c) {
-        const float x[4] = {__uint_as_float(raw[c].x << 16) * inv, __uint_as_float(raw[c].x & 0xFFFF0000u) * inv,
-                            __uint_as_float(raw[c].y << 16) * inv, __uint_as_float(raw[c].y & 0xFFFF0000u) * inv};
-        const uint32_t h = f8::encode4(x[0], x[1], x[2], x[3]);
-        const float4 back = f8::decode4(h);
-        const int kk = c >> 1, odd = (c & 1) * 2;
-        qf[mt][kk][odd] = h;                                       // row i: the code
-        qf[mt][kk][odd + 1] = f8::encode4(x[0] - back.x, x[1] - back.y, x[2] - back.z, x[3] - back.w);       // row i + 8: what it leaves
+      __syncwarp();
+      if (there) {
+        const uint32_t kdst = ring + s * S::STAGE + sub * 16 * HD;
+        tma_load_4d(kdst, &k_map, full, 0, 0, now.head, now.page);
+        tma_load_4d(kdst + S::OPERAND, &v_map, full, 0, 0, now.head, now.page);
       }
+    };
+    auto write_scales = [&](int t, int s) {
+      if ((lane >> 3) == (t & 3)) bars.scales[s][sub] = make_float2(now.ks, log2f(now.vs));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bars.full[s]));          // (after what the other lanes wrote)
+    };
+    // the first tiles' copies do not wait for their scales
+    const int early = min(min(my_tiles, STAGES), 4);
+    look_pages(now, 0);
+    for (int i = 0; i < early; ++i) copy(i, i);
+    look_scales(now);
+    for (int i = 0; i < early; ++i) write_scales(i, i);
+    look_pages(ahead, 4);
+    int s = early % STAGES, par = early == STAGES ? 0 : 1, t = early;
+    if (early == 4) look_scales(ahead);
+    for (; t < my_tiles; ++t) {
+      if ((t & 3) == 0) now = ahead, look_pages(ahead, t + 4);
+      if ((t & 3) == 2 || (t == 3 && early == 3)) look_scales(ahead);
+      bool ran_out;
+      if (!mbar_wait_warp(smem_u32(&bars.empty[s]), par, aborted, ran_out)) {
+        if (ran_out) gb_err::report(ERR_WAIT_EMPTY), *aborted = 1;
+        break;
+      }
+      copy(t, s);
+      write_scales(t, s);
+      if (++s == STAGES) s = 0, par ^= 1;
     }
-
-    float o[MT][HD / 8][4], m[MT], l[MT];
-    float vref = -200.f;           // log2 of the vs in whose units the sums are
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      m[mt] = -INFINITY, l[mt] = 0.f;
-#pragma unroll
-      for (int i = 0; i < HD / 8; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[mt][i][e] = 0.f;
+    if (*aborted && lane == 0 && t > 0) {
+      // wind down: the copies in flight need microseconds to land; two milliseconds before the shared memory is given up
+      const unsigned long long t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 2000000ull) {}
     }
-
-    for (; t < mine_n; ++t) {
-      const long long at = a_begin + warp + (long long)WARPS * t - a;           // within this segment
-      if (at >= count) break;
-      const int s = warp * S::DEPTH + t % S::DEPTH;
-      const bool gave_up = __shfl_sync(0xffffffffu, (int)*aborted, 0) != 0;
-      if (t >= issued) continue;       // (only after a wait ran out)
-      const bool have = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full_bar[s]), (t / S::DEPTH) & 1, gave_up ? DRAIN_LIMIT_NS : WAIT_LIMIT_NS));
-      if (!have) {
-        if (lane == 0) gb_err::report(ERR_WAIT_FULL);
-        *aborted = 1;
-        continue;
-      }
-      if (gave_up) continue;       // what was asked for has landed; nothing more is asked for
-      const uint32_t ks_addr = smem_u32(ring + s * S::STAGE), vs_addr = ks_addr + S::OPERAND;
-      const float4 scales = scale_s[s];
-      const int key0 = (lo / TK + first + (int)at) * TK;
-      const bool edge = key0 < lo || key0 + TK - 1 > hi;
-      if (edge) {
-        // value rows that no query may read are cleared (a weight of zero times a code that is no number would spoil a sum)
-        for (int e = lane; e < TK * (HD / 16); e += 32) {
-          const int key = e / (HD / 16), c = e % (HD / 16);
-          if (key0 + key < lo || key0 + key > hi)
-            *reinterpret_cast<uint4*>(ring + s * S::STAGE + S::OPERAND + swizzled<HD>(key, c)) = make_uint4(0u, 0u, 0u, 0u);
+  } else if (my_tiles > 0 && warp == 1) {
+    // ---------------------------------------------------------------- products
+    constexpr uint32_t idesc_s = instr_desc_e4m3(KT, N), idesc_o = instr_desc_e4m3(KT, HD) | INSTR_B_MN_MAJOR;
+    const uint64_t dk0 = smem_desc_rows<HD>(ring), dq0 = smem_desc_rows<HD>(q_at), dv0 = smem_desc_rows<HD>(ring + S::OPERAND),
+                   dp0 = smem_desc_sw128(p_at);
+    const bool leader = elect_one();
+    bool ok = true, ran_out = false;
+    int s = 0, par = 0, sp = 0;            // the stage of S^T and its phase, the stage of P V
+    int seg_s = 0, left_s = 0, seg_o = 0, left_o = 0;      // segments begun (by S^T, by P V), tiles left of them
+    long long a_s = a_begin, a_o = a_begin;
+    for (int t = 0; t <= my_tiles && ok; ++t) {
+      if (t < my_tiles) {
+        if (left_s == 0) {
+          const Segment g = segment_at(a_s);
+          left_s = g.count, a_s += g.count;
+          ok = mbar_wait_warp(smem_u32(&bars.q_ready[seg_s & 1]), (seg_s >> 1) & 1, aborted, ran_out);
+          ++seg_s;
+        }
+        if (ok) ok = mbar_wait_warp(smem_u32(&bars.full[s]), par, aborted, ran_out);
+        if (!ok) break;
+        tc_fence_after_sync();
+        if (leader) {
+          const uint64_t dk = dk0 + (uint64_t)(s * (S::STAGE >> 4)), dq = dq0 + (uint64_t)(((seg_s - 1) & 1) * (S::Q_BYTES >> 4));
+#pragma unroll
+          for (int k = 0; k < HD / 32; ++k) mma_f8(tmem + (t & 1) * 32, dk + 2 * k, dq + 2 * k, idesc_s, k > 0);
+          mma_commit(smem_u32(&bars.s_ready[t & 1]));
         }
         __syncwarp();
+        --left_s;
+        if (++s == STAGES) s = 0, par ^= 1;
       }
-      // ---- scores: rows' hi and lo by 32 keys
-      float sr[MT][4][4];
+      if (t > 0) {
+        const int u = t - 1;
+        bool first = false;
+        if (left_o == 0) {
+          const Segment g = segment_at(a_o);
+          left_o = g.count, a_o += g.count, first = true;
+          // the results of the segment in front have been read
+          if (seg_o > 0) ok = mbar_wait_warp(smem_u32(&bars.o_free), (seg_o - 1) & 1, aborted, ran_out);
+          ++seg_o;
+        }
+        if (ok) ok = mbar_wait_warp(smem_u32(&bars.p_ready[u & 1]), (u >> 1) & 1, aborted, ran_out);
+        if (!ok) break;
+        tc_fence_after_sync();
+        if (leader) {
+          const uint64_t dp = dp0 + (uint64_t)((u & 1) * (S::P_BYTES >> 4)), dv = dv0 + (uint64_t)(sp * (S::STAGE >> 4));
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+          for (int k = 0; k < KT / 32; ++k) mma_f8(tmem + O_COL, dp + 2 * k, dv + (uint64_t)(k * (32 * HD >> 4)), idesc_o, !first || k > 0);
+          mma_commit(smem_u32(&bars.pv_done[u & 1]));
+          mma_commit(smem_u32(&bars.empty[sp]));
+        }
+        __syncwarp();
+        --left_o;
+        if (++sp == STAGES) sp = 0;
+      }
+    }
+    if (!ok) {
+      if (ran_out && lane == 0) gb_err::report(ERR_WAIT_ACCUM);
+      *aborted = 1;
+    }
+  } else if (my_tiles > 0) {
+    // ---------------------------------------------------------------- scores and weights
+    const int x = threadIdx.x - 64, quarter = warp & 3, sw = warp - 2;
+    const int key_i = quarter * 32 + lane;                         // this thread's key of a tile
+    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
+    bool ok = true;
+    auto wait = [&](uint64_t& bar, int phase) {
+      if (ok && (!mbar_wait(smem_u32(&bar), phase & 1) || *aborted)) {
+        if (!*aborted) gb_err::report(ERR_WAIT_ACCUM);
+        ok = false, *aborted = 1;
+      }
+    };
+    // the queries of a segment as codes: thread x has row x / (HD / 16), 16 channels
+    uint4 raw[2];
+    const int qrow = x / (HD / 16), qc = x % (HD / 16);
+    auto ask_queries = [&](const Segment& g) {
+      const Span s = span_at(g.r);
+      const bool there = qrow < s.nrows && qrow < ROWS;
+      const uint4* src = reinterpret_cast<const uint4*>(
+          p.q + ((size_t)(s.q_begin + (there ? qrow / p.g : 0)) * p.Hq + g.kvh * p.g + (there ? qrow % p.g : 0)) * HD + 16 * qc);
+      raw[0] = there ? src[0] : make_uint4(0u, 0u, 0u, 0u);
+      raw[1] = there ? src[1] : make_uint4(0u, 0u, 0u, 0u);
+    };
+    auto put_queries = [&](int seg) {
+      const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+      float largest = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+      for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xFFFF0000u))));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sr[mt][j][e] = 0.f;
+      for (int o = HD / 32; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+      const int e2 = f8::scale_exponent(largest);
+      const float inv = f8::power_of_two(-e2);
+      uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        // column n of product j is slot 4 (n / 2) + 2 (j & 1) + n % 2 of sixteen j / 2
-        const int nn = lane & 7, krow = (j >> 1) * 16 + key_of_slot(4 * (nn >> 1) + 2 * (j & 1) + (nn & 1));
+      for (int i = 0; i < 4; ++i) {
+        const float a = __uint_as_float(w[2 * i] << 16) * inv, b = __uint_as_float(w[2 * i] & 0xFFFF0000u) * inv;
+        const float c = __uint_as_float(w[2 * i + 1] << 16) * inv, d = __uint_as_float(w[2 * i + 1] & 0xFFFF0000u) * inv;
+        hi[i] = f8::encode4(a, b, c, d);
+        const float4 back = f8::decode4(hi[i]);
+        lo[i] = f8::encode4(a - back.x, b - back.y, c - back.z, d - back.w);
+      }
+      if (qrow < ROWS) {
+        uint8_t* to = base + 2 * S::P_BYTES + (seg & 1) * S::Q_BYTES;
+        *reinterpret_cast<uint4*>(to + swizzled<HD>(qrow, qc)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(to + swizzled<HD>(qrow + ROWS, qc)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if (qc == 0) bars.factor[seg & 1][qrow] = f8::power_of_two(e2) * p.scale_log2;
+      }
+      fence_proxy_async();            // the tensor core reads them through the async proxy
+      mbar_arrive(smem_u32(&bars.q_ready[seg & 1]));
+    };
+    // segments that other CTAs have a part of: the first and the last at most; merged at the end
+    struct Shared {
+      long long seg0;
+      Segment g;
+      int nrows, q_begin;
+    } shared[2];
+    int n_shared = 0, t = 0, s = 0, par = 0;
+    // the queries of a segment are put while the one in front is at work, and asked for one segment earlier still
+    Segment now = segment_at(a_begin), next, later;
+    long long a = a_begin;
+    ask_queries(now);
+    put_queries(0);
+    sync_four();                      // the factors
+    if (a + now.count < a_end) next = segment_at(a + now.count), ask_queries(next);
+    for (int seg = 0; a < a_end; ++seg) {
+      const Segment g = now;
+      const Span w = span_at(g.r);
+      bool asked = a + g.count < a_end;
+      float m[ROWS], l[ROWS], vref = -200.f;       // vref: log2 of the vs in whose units the sums are
 #pragma unroll
-        for (int h = 0; h < HD / 64; ++h) {
-          uint32_t b[4];
-          ldmatrix_x4(b, ks_addr + swizzled<HD>(krow, 4 * h + (lane >> 3)));
+      for (int r = 0; r < ROWS; ++r) m[r] = -INFINITY, l[r] = 0.f;
+
+      for (int j = 0; j < g.count; ++j, ++t) {
+        wait(bars.s_ready[t & 1], t >> 1);
+        wait(bars.full[s], par);                   // (over already)
+        tc_fence_after_sync();
+        const float2 sc = bars.scales[s][key_i >> 4];
+        const int key0 = (w.lo / KT + g.first + j) * KT, key = key0 + key_i;
+        const bool readable = key >= w.lo && key <= w.hi && sc.x >= 0.f;
+        // no mask for a tile that lies before the first row's position, inside the last row's window, on pages that are there
+        const bool full = key0 + KT - 1 <= w.pos0 && (p.window <= 0 || key0 >= w.hi + 1 - p.window) && sc.x >= 0.f;
+        float v[ROWS];
+        {
+          uint32_t raw_s[N];
+          tmem_load<N>(lane_addr + (t & 1) * 32, raw_s);
+          tmem_ld_wait();
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            mma_e4m3(sr[mt][j], qf[mt][2 * h], b[0], b[1]);
-            mma_e4m3(sr[mt][j], qf[mt][2 * h + 1], b[2], b[3]);
+          for (int r = 0; r < ROWS; ++r) v[r] = (__uint_as_float(raw_s[r]) + __uint_as_float(raw_s[r + ROWS])) * (bars.factor[seg & 1][r] * sc.x);
+        }
+        if (!full) {
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r) {
+            const int pos = w.pos0 + r / p.g;
+            if (!readable || key > pos || (p.window > 0 && key + p.window <= pos)) v[r] = -INFINITY;
+          }
+          // A value row that nobody reads is cleared: a weight of zero times a code that is no number would spoil a sum.
+          if (!readable) {
+            uint8_t* row = base + S::RING_AT + s * S::STAGE + S::OPERAND + key_i * HD;
+#pragma unroll
+            for (int c = 0; c < HD / 16; ++c) reinterpret_cast<uint4*>(row)[c] = make_uint4(0u, 0u, 0u, 0u);
           }
         }
-      }
-      // ---- mask, maximum
-      const bool full = !edge && scales.x >= 0.f && scales.y >= 0.f && key0 + TK - 1 <= pos0 &&
-                        (p.window <= 0 || key0 >= hi + 1 - p.window);
-      float sv[MT][8];             // slots (j, e) as 2 j + e, in powers of two
-      bool more = false;
+        const float ev = readable ? sc.y : -200.f;
+        bool more = ev > vref;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const float f0 = factor[mt] * scales.x, f1 = factor[mt] * scales.y;
-        float mx = m[mt];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int j = i >> 1, e = i & 1;
-          float x = (sr[mt][j][e] + sr[mt][j][e + 2]) * (j < 2 ? f0 : f1);
-          if (!full) {
-            const int key = key0 + (j >> 1) * 16 + key_of_slot(4 * (lane & 3) + 2 * (j & 1) + e);
-            if (key < row_start[mt] || key > row_pos[mt] || (j < 2 ? scales.x : scales.y) < 0.f) x = -INFINITY;
+        for (int r = 0; r < ROWS; ++r)
+          if (r < w.nrows) more = more || !(v[r] <= m[r] + S::GROWTH);          // (a score that is no number stays one)
+        // a score far above the reference (rare after a request's first tiles), or a larger vs: everything is brought to it
+        if (any_of_four(more)) {
+          if (j > 0) {
+            wait(bars.pv_done[(t - 1) & 1], (t - 1) >> 1);
+            tc_fence_after_sync();
           }
-          sv[mt][i] = x;
-          mx = fmaxf(mx, x);
-        }
-        more = more || mx > m[mt];
-      }
-      // a larger score than any so far (rare after the first tiles), or a larger vs: everything is brought to it
-      if (__any_sync(0xffffffffu, more)) {
+          const float vt = gb::warp_max(ev);
+          if (lane == 0) bars.vtop[sw] = vt;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          float mx = m[mt];
+          for (int r = 0; r < ROWS; ++r)
+            if (r < w.nrows) {
+              const float top = gb::warp_max(v[r]);
+              if (lane == 0) bars.top[sw][r] = top;
+            }
+          sync_four();
+          const float v_new = fmaxf(vref, fmaxf(fmaxf(bars.vtop[0], bars.vtop[1]), fmaxf(bars.vtop[2], bars.vtop[3])));
+          const float v_corr = exp2_fast(vref - v_new);
+          vref = v_new;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) mx = fmaxf(mx, sv[mt][i]);
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const float corr = m[mt] == -INFINITY ? 0.f : exp2_fast(m[mt] - mx);
-          m[mt] = mx;
-          l[mt] *= corr;
-#pragma unroll
-          for (int i = 0; i < HD / 8; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[mt][i][e] *= corr;
-        }
-      }
-      const float evm = fmaxf(scales.x >= 0.f ? scales.z : -200.f, scales.y >= 0.f ? scales.w : -200.f);
-      if (evm > vref) {
-        const float corr = exp2_fast(vref - evm);
-        vref = evm;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int i = 0; i < HD / 8; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[mt][i][e] *= corr;
-      }
-      // ---- weights * 256 * vs / 2^vref as two codes each, the denominator without vs
-      uint32_t pf[MT][4];
-      // (2^-100 of the largest vs is nothing; and without a page the weights are zeros)
-      const float up0 = 8.f + fminf(fmaxf(scales.z - vref, -100.f), 0.f), up1 = 8.f + fminf(fmaxf(scales.w - vref, -100.f), 0.f);
-      const float down0 = exp2_fast(-up0), down1 = exp2_fast(-up1);
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const float base = m[mt] == -INFINITY ? 0.f : -m[mt];
-        float w[8], l0 = 0.f, l1 = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          w[i] = exp2_fast(sv[mt][i] + (base + (i < 4 ? up0 : up1)));
-          if (i < 4) l0 += w[i];
-          else l1 += w[i];
-        }
-        l[mt] += l0 * down0 + l1 * down1;
-        uint32_t h[4], q[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) split2(w[2 * j], w[2 * j + 1], h[j], q[j]);
-        pf[mt][0] = h[0] | (h[1] << 16), pf[mt][1] = q[0] | (q[1] << 16);
-        pf[mt][2] = h[2] | (h[3] << 16), pf[mt][3] = q[2] | (q[3] << 16);
-      }
-      // ---- sums of the values
-      const int vrow = key_of_slot(lane);          // slot lane of 32 (bit 4 stays)
-#pragma unroll
-      for (int c = 0; c < HD / 16; ++c) {
-        uint32_t b[4];
-        ldmatrix_trans_bytes(b, vs_addr + swizzled<HD>(vrow, c));
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          mma_e4m3(o[mt][2 * c], pf[mt], b[0], b[2]);
-          mma_e4m3(o[mt][2 * c + 1], pf[mt], b[1], b[3]);
-        }
-      }
-      __syncwarp();                // every lane is done with the stage before it is filled again
-      issue(t + S::DEPTH);
-    }
-    // ---- the warps' sums are merged in shared memory, CW channels at a time
-    const float unit = exp2_fast(vref - 8.f);
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      l[mt] += __shfl_xor_sync(0xffffffffu, l[mt], 1);
-      l[mt] += __shfl_xor_sync(0xffffffffu, l[mt], 2);
-      if (lane % 4 == 0) ml_s[warp][mt * 8 + lane / 4] = make_float2(m[mt], l[mt]);
-    }
-    const bool whole = first == 0 && count == n;
-    const long long seg0 = a - first;              // the segment's first tile in the row of all
-    float* my_part = partials + ((size_t)cta * 2 + (a == a_begin ? 0 : 1)) * (MAX_ROWS * RS);
-    constexpr int LANES = THREADS / ROWS;          // threads of a row: 16 or 8
-    const int row = threadIdx.x / LANES, sub = threadIdx.x % LANES;
-    __nv_bfloat16* const dst = p.out + ((size_t)(q_begin + (row < nrows ? row / p.g : 0)) * p.Hq + kvh * p.g + (row < nrows ? row % p.g : 0)) * HD;
-#pragma unroll
-    for (int pass = 0; pass < S::PASSES; ++pass) {
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        float* to = red + (warp * ROWS + mt * 8 + lane / 4) * CW + (lane % 4) * 2;
-#pragma unroll
-        for (int i = 0; i < CW / 8; ++i) {
-          const float* x = o[mt][pass * (CW / 8) + i];
-          *reinterpret_cast<float2*>(to + i * 8) = make_float2((x[0] + x[2] * 0.03125f) * unit, (x[1] + x[3] * 0.03125f) * unit);
-        }
-      }
-      __syncthreads();
-      float f[WARPS], mm = -INFINITY, ll = 0.f;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, ml_s[w][row].x);
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float2 x = ml_s[w][row];
-        f[w] = x.x == -INFINITY ? 0.f : exp2_fast(x.x - mm);
-        ll += f[w] > 0.f ? f[w] * x.y : 0.f;
-      }
-      if (row < nrows) {
-        const float inv = ll > 0.f ? 1.0f / ll : 0.f;
-#pragma unroll
-        for (int c = 2 * sub; c < CW; c += 2 * LANES) {
-          float2 v = make_float2(0.f, 0.f);
-#pragma unroll
-          for (int w = 0; w < WARPS; ++w) {
-            const float2 x = *reinterpret_cast<const float2*>(red + (w * ROWS + row) * CW + c);
-            if (f[w] > 0.f) v.x += f[w] * x.x, v.y += f[w] * x.y;          // (a warp without a key has nothing)
+          for (int r = 0; r < ROWS; ++r) {
+            if (r >= w.nrows) continue;
+            const float m_new = fmaxf(m[r], fmaxf(fmaxf(bars.top[0][r], bars.top[1][r]), fmaxf(bars.top[2][r], bars.top[3][r])));
+            const float corr = m[r] == -INFINITY ? 0.f : exp2_fast(m[r] - m_new);
+            m[r] = m_new;
+            l[r] *= corr;
+            if (x == r) bars.corr[r] = corr * v_corr;
           }
-          if (whole) gb::store_pair(dst + pass * CW + c, v.x * inv, v.y * inv);
-          else __stcg(reinterpret_cast<float2*>(my_part + row * RS + pass * CW + c), v);
+          sync_four();
+          if (quarter == 0 && j > 0) {             // the sums' rows lie in its lanes: r, r + ROWS, r + 2 ROWS
+            const float corr = lane < S::PARTS * ROWS && lane % ROWS < w.nrows ? bars.corr[lane % ROWS] : 1.f;
+#pragma unroll
+            for (int h = 0; h < HD / 32; ++h) {
+              uint32_t o[32];
+              tmem_ld_32(lane_addr + O_COL + h * 32, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
+              tmem_st_32(lane_addr + O_COL + h * 32, o);
+            }
+            tmem_st_wait();
+          }
         }
-        if (!whole && pass == 0 && sub == 0) __stcg(reinterpret_cast<float2*>(my_part + row * RS + HD), make_float2(mm, ll));
-      }
-      __syncthreads();             // the buffer is free for the next pass, or the next segment
-    }
-    if (!whole) {
-      // ---- several CTAs: who counts the last arrival adds the parts up, in the CTAs' order
-      int w0 = (int)(seg0 * workers / tiles), w1 = (int)((seg0 + n - 1) * workers / tiles);
-      while (w0 + 1 < workers && begins_at(w0 + 1) <= seg0) ++w0;
-      while (w0 > 0 && begins_at(w0) > seg0) --w0;
-      while (w1 + 1 < workers && begins_at(w1 + 1) <= seg0 + n - 1) ++w1;
-      while (w1 > 0 && begins_at(w1) > seg0 + n - 1) --w1;
-      if (threadIdx.x == 0) {      // (behind the barrier in front: all have written their part)
-        __threadfence();
-        int* counter = counters + (size_t)r * p.Hkv + kvh;
-        last_s = atomicAdd(counter, 1) == w1 - w0;
-        if (last_s) *counter = 0;                  // as the next launch expects it
-        __threadfence();
-      }
-      __syncthreads();
-      if (last_s) {
-        auto part_of = [&](int w) {      // only the first of them may hold another segment's end in front of its part
-          return partials + ((size_t)w * 2 + (w == w0 && begins_at(w0) < seg0 ? 1 : 0)) * (MAX_ROWS * RS);
-        };
-        if (row < nrows) {
-          constexpr int PER = HD / LANES / 2;
-          float mm = -INFINITY, ll = 0.f;
-          float2 v[PER];
-          for (int w = w0; w <= w1; ++w) mm = fmaxf(mm, __ldcg(part_of(w) + row * RS + HD));
+        if (t >= 2) wait(bars.pv_done[t & 1], (t - 2) >> 1);       // P's buffer is free
+        // weights * 2^UP * vs / 2^vref as two codes each, the denominator without vs. (2^-100 of the largest vs is nothing; and where
+        // nothing is read the weights are zeros.)
+        const float up = S::UP + fminf(fmaxf(sc.y - vref, -100.f), 0.f), down = exp2_fast(-up);
+        const uint32_t p_base = p_at + (t & 1) * S::P_BYTES + (key_i & 15), chunk = (uint32_t)key_i >> 4;
 #pragma unroll
-          for (int i = 0; i < PER; ++i) v[i] = make_float2(0.f, 0.f);
-#pragma unroll 4
-          for (int w = w0; w <= w1; ++w) {
-            const float* part = part_of(w) + row * RS;
-            const float2 x = __ldcg(reinterpret_cast<const float2*>(part + HD));
-            const float f = x.x == -INFINITY ? 0.f : exp2_fast(x.x - mm);
-            ll += f > 0.f ? f * x.y : 0.f;
+        for (int r = 0; r < ROWS; r += 2) {
+          if (r >= w.nrows) break;
+          const float wa = exp2_fast(v[r] + (up - (m[r] == -INFINITY ? 0.f : m[r])));
+          const float wb = exp2_fast(v[r + 1] + (up - (m[r + 1] == -INFINITY ? 0.f : m[r + 1])));
+          l[r] = fmaf(wa, down, l[r]), l[r + 1] = fmaf(wb, down, l[r + 1]);
+          uint32_t code[S::PARTS];
+          split<S::PARTS>(wa, wb, code);
+          // row r of P: 128 bytes, its chunks of 16 swizzled
+          const uint32_t a0 = p_base + r * 128 + ((chunk ^ (r & 7)) << 4), a1 = p_base + (r + 1) * 128 + ((chunk ^ ((r + 1) & 7)) << 4);
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-              const float2 y = __ldcg(reinterpret_cast<const float2*>(part + 2 * (sub + LANES * i)));
-              if (f > 0.f) v[i].x += f * y.x, v[i].y += f * y.y;
+          for (int i = 0; i < S::PARTS; ++i) st_shared_u8(a0 + i * ROWS * 128, code[i]), st_shared_u8(a1 + i * ROWS * 128, code[i] >> 8);
+        }
+        fence_proxy_async();            // the tensor core reads weights and values through the async proxy
+        tc_fence_before_sync();
+        mbar_arrive(smem_u32(&bars.p_ready[t & 1]));
+        if (++s == STAGES) s = 0, par ^= 1;
+        if (asked && (j == 1 || j + 1 == g.count)) {
+          put_queries(seg + 1);
+          asked = false;
+          if (a + g.count + next.count < a_end) later = segment_at(a + g.count + next.count), ask_queries(later);
+        }
+      }
+      // ---- the segment's results
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+        if (r < w.nrows) {
+          const float sum = gb::warp_sum(l[r]);
+          if (lane == 0) bars.lsum[sw][r] = sum;
+        }
+      wait(bars.pv_done[(t - 1) & 1], (t - 1) >> 1);
+      tc_fence_after_sync();
+      sync_four();
+      const bool whole = g.first == 0 && g.count == g.n;
+      if (quarter == 0) {
+        const int r = lane % ROWS;
+        const bool mine = lane < w.nrows && ok;
+        float mr = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i)
+          if (i == r) mr = m[i];
+        const float ll = (bars.lsum[0][r] + bars.lsum[1][r]) + (bars.lsum[2][r] + bars.lsum[3][r]);
+        const float unit = exp2_fast(vref - S::UP), inv = ll > 0.f ? 1.0f / ll : ll == ll ? 0.f : ll;
+        const float f = whole ? unit * inv : unit;
+        __nv_bfloat16* const dst = p.out + ((size_t)(w.q_begin + r / p.g) * p.Hq + g.kvh * p.g + r % p.g) * HD;
+        float* const part = partials + ((size_t)cta * 2 + (a == a_begin ? 0 : 1)) * (MAX_ROWS * RS) + r * RS;
+#pragma unroll
+        for (int h = 0; h < HD / 16; ++h) {
+          uint32_t o[16];
+          tmem_ld_16(lane_addr + O_COL + h * 16, o);
+          tmem_ld_wait();
+          float y[16];
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            const float hi = __uint_as_float(o[c]);
+            float lo = __shfl_sync(0xffffffffu, hi, (lane + ROWS) & 31);
+            if (S::PARTS == 3) lo = fmaf(__shfl_sync(0xffffffffu, hi, (lane + 2 * ROWS) & 31), 0.03125f, lo);
+            // (nothing seen: the sums mean nothing)
+            y[c] = mr == -INFINITY && ll == ll ? 0.f : fmaf(lo, 0.03125f, hi) * f;
+          }
+          if (mine) {
+#pragma unroll
+            for (int c = 0; c < 16; c += 2) {
+              if (whole) gb::store_pair(dst + h * 16 + c, y[c], y[c + 1]);
+              else __stcg(reinterpret_cast<float2*>(part + h * 16 + c), make_float2(y[c], y[c + 1]));
             }
           }
-          const float inv = ll > 0.f ? 1.0f / ll : 0.f;
+        }
+        if (mine && !whole) __stcg(reinterpret_cast<float2*>(part + HD), make_float2(mr, ll));
+        tc_fence_before_sync();
+        mbar_arrive(smem_u32(&bars.o_free));
+      }
+      if (!whole) {
+        const Shared y = {a - g.first, g, w.nrows, w.q_begin};
+        if (n_shared == 0) shared[0] = y;
+        else shared[1] = y;
+        ++n_shared;
+      }
+      a += g.count;
+      now = next, next = later;
+    }
+    // ---- segments of several CTAs: who counts the last arrival adds the parts up, in the CTAs' order
+    sync_four();                       // the parts are written
+    auto worker_of = [&](const Segment& g, int tile) {             // whose stretch holds this tile
+      const long long c = (long long)cost[g.r] * p.Hkv + (long long)g.kvh * (g.n + SEGMENT) + tile;
+      int w = (int)(c * workers / costs);
+      while (w + 1 < workers && costs * (w + 1) / workers <= c) ++w;
+      while (w > 0 && costs * w / workers > c) --w;
+      return w;
+    };
+    int c0[2], c1[2];
+    bool behind[2];                    // whether the first of them has another segment's end in front of its part
 #pragma unroll
-          for (int i = 0; i < PER; ++i) gb::store_pair(dst + 2 * (sub + LANES * i), v[i].x * inv, v[i].y * inv);
+    for (int i = 0; i < 2; ++i) {
+      c0[i] = c1[i] = 0, behind[i] = false;
+      if (i < n_shared) {
+        c0[i] = worker_of(shared[i].g, 0), c1[i] = worker_of(shared[i].g, shared[i].g.n - 1);
+        behind[i] = begins_at(c0[i]) < shared[i].seg0;
+      }
+    }
+    if (x < n_shared) {
+      __threadfence();
+      const Segment& g = x == 0 ? shared[0].g : shared[1].g;
+      int* counter = counters + (size_t)g.r * p.Hkv + g.kvh;
+      const bool last = atomicAdd(counter, 1) == (x == 0 ? c1[0] - c0[0] : c1[1] - c0[1]);
+      if (last) *counter = 0;                        // as the next launch expects it
+      bars.last[x] = last;
+      __threadfence();
+    }
+    sync_four();
+    constexpr int LANES = 128 / ROWS, PER = HD / LANES / 2;          // threads of a row, pairs of channels of a thread
+    const int row = x / LANES, sub = x % LANES;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (i >= n_shared || !bars.last[i] || row >= shared[i].nrows || !ok) continue;
+      auto part_of = [&](int c) { return partials + ((size_t)c * 2 + (c == c0[i] && behind[i] ? 1 : 0)) * (MAX_ROWS * RS) + row * RS; };
+      float mm = -INFINITY, ll = 0.f;
+      float2 v[PER];
+#pragma unroll 4
+      for (int c = c0[i]; c <= c1[i]; ++c) mm = fmaxf(mm, __ldcg(part_of(c) + HD));
+#pragma unroll
+      for (int e = 0; e < PER; ++e) v[e] = make_float2(0.f, 0.f);
+#pragma unroll 4
+      for (int c = c0[i]; c <= c1[i]; ++c) {
+        const float* part = part_of(c);
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + HD));
+        const float f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - mm);
+        ll += f > 0.f ? f * ml.y : ml.y == ml.y ? 0.f : ml.y;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+          const float2 y = __ldcg(reinterpret_cast<const float2*>(part + 2 * (sub + LANES * e)));
+          if (f > 0.f) v[e].x += f * y.x, v[e].y += f * y.y;
         }
       }
-      __syncthreads();             // the flag is free for the next segment
+      const float inv = ll > 0.f ? 1.0f / ll : ll == ll ? 0.f : ll;
+      const Segment& g = shared[i].g;
+      __nv_bfloat16* const dst = p.out + ((size_t)(shared[i].q_begin + row / p.g) * p.Hq + g.kvh * p.g + row % p.g) * HD;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) gb::store_pair(dst + 2 * (sub + LANES * e), v[e].x * inv, v[e].y * inv);
     }
-    a += count;
   }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, TMEM_COLS);
 }
 
 // ------------------------------------------------------------------ host side
@@ -542,7 +702,7 @@ struct MapKeyHash {
   }
 };
 
-// Pools [pages][heads][page][hd] of bytes through boxes [1][1][min(page, 32)][hd], swizzled over the rows' width.
+// Pools [pages][heads][page][hd] of bytes through boxes [1][1][page][hd], swizzled over the rows' width.
 int pool_map(const void* ptr, int page, int heads, long long pages, int hd, CUtensorMap* out) {
   static std::mutex mu;
   static std::unordered_map<MapKey, CUtensorMap, MapKeyHash> cache;
@@ -557,7 +717,7 @@ int pool_map(const void* ptr, int page, int heads, long long pages, int hd, CUte
   if (!fn) return gb::fail(GB_CUDA_ERROR, "cuTensorMapEncodeTiled is not available from this driver");
   cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)page, (cuuint64_t)heads, (cuuint64_t)pages};
   cuuint64_t strides[3] = {(cuuint64_t)hd, (cuuint64_t)hd * page, (cuuint64_t)hd * page * heads};
-  cuuint32_t box[4] = {(cuuint32_t)hd, (cuuint32_t)(page < TK ? page : TK), 1, 1};
+  cuuint32_t box[4] = {(cuuint32_t)hd, (cuuint32_t)page, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUtensorMap m;
   const CUresult r = fn(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -570,30 +730,33 @@ int pool_map(const void* ptr, int page, int heads, long long pages, int hd, CUte
   return GB_OK;
 }
 
-constexpr int CTAS = 2;               // per SM
-constexpr int MAX_REQUESTS = 1024;    // their tiles' sums lie in shared memory
+constexpr int MAX_REQUESTS = 256;    // of one launch: their lengths lie in shared memory
 
-template <int HD, int MT>
-int launch(const Params& p, const CUtensorMap& km, const CUtensorMap& vm, int grid, int min_tiles, void* parts, void* counters, cudaStream_t stream) {
-  auto kernel = attention_f8_decode_kernel<HD, MT>;
-  using S = Shape<HD, MT>;
-  constexpr int MOST = 1024 + S::RING + S::MERGE + (MAX_REQUESTS + 1) * 4;
+template <int HD, int N>
+int launch(const Params& p, const CUtensorMap& km, const CUtensorMap& vm, long long tiles_most, int min_tiles, void* parts, void* counters,
+           cudaStream_t stream) {
+  using S = Shape<HD, N>;
+  auto kernel = attention_f8_decode_kernel<HD, N>;
+  constexpr int LENGTHS = (4 * MAX_REQUESTS + 3) * 4;
+  static_assert(S::CTAS == 1 || 2 * (1024 + S::BYTES + LENGTHS + (int)sizeof(Bars) + 1024) <= 233472, "two CTAs an SM");
   static gb::OncePerDevice configured;
   if (configured.needed()) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 1024 + S::BYTES + LENGTHS);
     if (e != cudaSuccess) return gb::fail(GB_CUDA_ERROR, "attention_f8_decode: %s", cudaGetErrorString(e));
     configured.done();
   }
-  const size_t smem = 1024 + S::RING + S::MERGE + (size_t)(p.R + 1) * 4;
-  return gb::check_pdl_launch(gb::launch_pdl(kernel, dim3((unsigned)grid), dim3(THREADS), smem, stream, dim3(1), km, vm, p, p.page < TK ? p.page : TK,
+  const int room = tc_host::sm_count() * S::CTAS;
+  const long long most = tiles_most / min_tiles + 1;
+  const size_t smem = 1024 + S::BYTES + (size_t)(4 * p.R + 3) * 4;
+  return gb::check_pdl_launch(gb::launch_pdl(kernel, dim3((unsigned)(most < room ? most : room)), dim3(THREADS), smem, stream, dim3(1), km, vm, p,
                                              min_tiles, (float*)parts, (int*)counters), "attention_f8_decode");
 }
 
 }  // namespace
 
-// Whether the kernel takes this shape: heads of 64 or 128, pages of 16, 32, 64 or 128 keys, up to sixteen query heads a group, up to 1,024 requests.
-GB_EXPORT int gb_f8_attention_decode_takes(int hd, int page, int g, int R) {
-  return (hd == 64 || hd == 128) && page >= 16 && page <= 128 && (page & (page - 1)) == 0 && g <= 16 && R <= MAX_REQUESTS && tc_host::encode_fn() != nullptr;
+// Whether the kernel takes this shape: heads of 64 or 128, pages of 16, 32, 64 or 128 keys, up to sixteen query heads a group.
+GB_EXPORT int gb_f8_attention_decode_takes(int hd, int page, int g) {
+  return (hd == 64 || hd == 128) && page >= 16 && page <= 128 && (page & (page - 1)) == 0 && g <= MAX_ROWS && tc_host::encode_fn() != nullptr;
 }
 // Rows (new tokens times heads of a group) up to which a request is its.
 GB_EXPORT int gb_f8_attention_decode_rows(int g) { return attn8::decode_rows(g); }
@@ -601,32 +764,34 @@ GB_EXPORT int gb_f8_attention_decode_rows(int g) { return attn8::decode_rows(g);
 // launch leaves them zero).
 GB_EXPORT long long gb_f8_attention_decode_scratch(int R, int Hkv, int hd, long long* counters) {
   *counters = ((long long)R * Hkv * 4 + 255) / 256 * 256;
-  return (long long)tc_host::sm_count() * CTAS * 2 * MAX_ROWS * (hd + 2) * 4;
+  return (long long)tc_host::sm_count() * 2 * 2 * MAX_ROWS * (hd + 2) * 4;
 }
 
 GB_EXPORT int gb_f8_attention_decode(const void* q, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale, const void* table,
                                      int table_width, const void* cu_q, const void* kv_lens, void* out, int R, long long pages, int Hq, int Hkv, int hd,
                                      float scale, int window, int page, int max_kv_len, void* parts, void* counters, void* stream) {
-  const int g = Hq / Hkv;
-  if (R <= 0 || Hkv <= 0 || Hq % Hkv || !gb_f8_attention_decode_takes(hd, page, g, R) || (uintptr_t)q % 8 || (uintptr_t)out % 4 || (uintptr_t)k_pool % 16 ||
-      (uintptr_t)v_pool % 16)
+  if (R <= 0 || Hkv <= 0 || Hq % Hkv || !gb_f8_attention_decode_takes(hd, page, Hq / Hkv) || (uintptr_t)q % 16 || (uintptr_t)out % 4 ||
+      (uintptr_t)k_pool % 16 || (uintptr_t)v_pool % 16)
     return gb::fail(GB_BAD_ARGUMENT, "attention_f8_decode: %d requests, heads %d / %d of %d, pages of %d", R, Hq, Hkv, hd, page);
-  Params p{(const __nv_bfloat16*)q, (const float*)k_scale, (const float*)v_scale, (__nv_bfloat16*)out, (const int32_t*)table, (const int32_t*)cu_q,
-           (const int32_t*)kv_lens, table_width, R, Hq, Hkv, g, window, page, attn8::decode_rows(g), scale * 1.4426950408889634f};
   CUtensorMap km, vm;
   int rc = pool_map(k_pool, page, Hkv, pages, hd, &km);
   if (rc) return rc;
   rc = pool_map(v_pool, page, Hkv, pages, hd, &vm);
   if (rc) return rc;
-  const int reach = window > 0 && window + 2 * TK < max_kv_len ? window + 2 * TK : max_kv_len;
-  // Four tiles a warp at least: a shorter stretch costs more in parts to merge than it saves (500 keys, 8 heads: 10.7 us from 4 tiles a CTA
-  // on, 8.6 from 16, 15.1 from 32).
-  const int min_tiles = 16;
-  const long long most = (long long)R * Hkv * ((reach + TK - 1) / TK + 1) / min_tiles + 1;
-  const int room = tc_host::sm_count() * CTAS, grid = (int)(most < room ? most : room);
-  const cudaStream_t st = (cudaStream_t)stream;
-  if (hd == 64) return g <= 8 ? launch<64, 1>(p, km, vm, grid, min_tiles, parts, counters, st) : launch<64, 2>(p, km, vm, grid, min_tiles, parts, counters, st);
-  return g <= 8 ? launch<128, 1>(p, km, vm, grid, min_tiles, parts, counters, st) : launch<128, 2>(p, km, vm, grid, min_tiles, parts, counters, st);
+  const int g = Hq / Hkv, reach = window > 0 && window + 2 * KT < max_kv_len ? window + 2 * KT : max_kv_len;
+  const int min_tiles = getenv("MINT") ? atoi(getenv("MINT")) : 4;
+  for (int r0 = 0; r0 < R && rc == GB_OK; r0 += MAX_REQUESTS) {
+    const int n = R - r0 < MAX_REQUESTS ? R - r0 : MAX_REQUESTS;
+    const Params p{(const __nv_bfloat16*)q, (const float*)k_scale, (const float*)v_scale, (__nv_bfloat16*)out,
+                   (const int32_t*)table + (size_t)r0 * table_width, (const int32_t*)cu_q + r0, (const int32_t*)kv_lens + r0, table_width, n, Hq,
+                   Hkv, g, window, page, scale * 1.4426950408889634f};
+    const long long tiles = (long long)n * Hkv * ((reach + KT - 1) / KT + 1);
+    int* count = (int*)counters + (size_t)r0 * Hkv;
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (hd == 64) rc = g <= 8 ? launch<64, 16>(p, km, vm, tiles, min_tiles, parts, count, st) : launch<64, 32>(p, km, vm, tiles, min_tiles, parts, count, st);
+    else rc = g <= 8 ? launch<128, 16>(p, km, vm, tiles, min_tiles, parts, count, st) : launch<128, 32>(p, km, vm, tiles, min_tiles, parts, count, st);
+  }
+  return rc;
 }
 
 GB_EXPORT int gb_f8_attention_decode_error_check() { return gb_err::fetch_and_clear(); }

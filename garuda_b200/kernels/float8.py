@@ -38,7 +38,7 @@ _FLOAT8_SIGNATURES = {
     "gb_f8_quantize_weight": [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_longlong, c_void_p, c_void_p],
     "gb_f8_append": [c_void_p, c_int, c_longlong, c_void_p, c_int] + [c_void_p] * 7 + [c_int] * 6 + [c_void_p, c_int, c_int, c_void_p],
     "gb_f8_attention_simple": [c_void_p, c_int] + [c_void_p] * 5 + [c_int] + [c_void_p] * 3 + [c_int] * 5 + [c_float, c_int, c_int, c_int, c_void_p],
-    "gb_f8_attention_decode_takes": [c_int] * 4,
+    "gb_f8_attention_decode_takes": [c_int] * 3,
     "gb_f8_attention_decode_rows": [c_int],
     "gb_f8_attention_decode": [c_void_p] * 6 + [c_int] + [c_void_p] * 3 + [c_int, c_longlong] + [c_int] * 3 + [c_float] + [c_int] * 3 + [c_void_p] * 3,
     "gb_f8_attention_decode_error_check": [],
@@ -203,7 +203,7 @@ class Float8Ops:
             return
         L, g, stream = self.float8_lib, Hq // Hkv, self._stream()
         above = -1             # requests of more rows (new tokens times heads of a group) than this are still to do
-        if q.dtype == torch.bfloat16 and L.gb_f8_attention_decode_takes(hd, int(page_size), g, R):
+        if q.dtype == torch.bfloat16 and q.data_ptr() % 16 == 0 and L.gb_f8_attention_decode_takes(hd, int(page_size), g):
             rows = L.gb_f8_attention_decode_rows(g)
             if min_q_len * g <= rows:
                 counter_bytes = c_longlong(0)
