@@ -216,39 +216,40 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
     if (threadIdx.x == THREADS - 1) bars.total = before;
     __syncthreads();
   }
-  // Stretches are equal in cost: a request's head is its tiles and SEGMENT behind them.
-  const long long tiles = (long long)cum[p.R] * p.Hkv, costs = (long long)cost[p.R] * p.Hkv;
-  const int workers = (int)max(1ll, min((long long)gridDim.x, tiles / min_tiles));          // each has min_tiles or so at least
+  // Stretches are equal in cost: a request's head is its tiles and SEGMENT behind them. (The host has seen that all of it fits 31 bits.)
+  const int tiles = cum[p.R] * p.Hkv, costs = cost[p.R] * p.Hkv;
+  const int workers = max(1, min((int)gridDim.x, tiles / min_tiles));          // each has min_tiles or so at least
+  const int stretch = max(1, (costs + workers - 1) / workers);
   const int cta = blockIdx.x;
-  auto find = [&](const int* sums, long long at) {     // the last request whose heads begin at or before it
+  auto find = [&](const int* sums, int at) {           // the last request whose heads begin at or before it
     int lo = 0, hi = p.R;
     while (hi - lo > 1) {              // (of requests without tiles at the same place the last one: it has some)
       const int mid = (lo + hi) >> 1;
-      if ((long long)sums[mid] * p.Hkv <= at) lo = mid;
+      if (sums[mid] * p.Hkv <= at) lo = mid;
       else hi = mid;
     }
     return lo;
   };
-  auto begins_at = [&](int w) -> long long {           // the first tile of worker w's stretch, in the row of all tiles
-    if (w >= workers) return tiles;
-    const long long c = costs * w / workers;
-    const int r = find(cost, c), n = cum[r + 1] - cum[r], rem = (int)(c - (long long)cost[r] * p.Hkv);
-    return (long long)cum[r] * p.Hkv + (long long)(rem / (n + SEGMENT)) * n + min(rem % (n + SEGMENT), n);
+  auto begins_at = [&](int w) {                        // the first tile of worker w's stretch, in the row of all tiles
+    const int c = w * stretch;
+    if (c >= costs) return tiles;
+    const int r = find(cost, c), n = cum[r + 1] - cum[r], rem = c - cost[r] * p.Hkv, head = rem / (n + SEGMENT);
+    return cum[r] * p.Hkv + head * n + min(rem - head * (n + SEGMENT), n);
   };
-  const long long a_begin = cta < workers && tiles > 0 ? begins_at(cta) : 0, a_end = cta < workers && tiles > 0 ? begins_at(cta + 1) : 0;
-  const int my_tiles = (int)(a_end - a_begin);
+  const int a_begin = cta < workers ? begins_at(cta) : tiles, a_end = cta < workers ? begins_at(cta + 1) : tiles;
+  const int my_tiles = a_end - a_begin;
 
   // A segment: one request's head, or this CTA's part of it: tiles first .. first + count of its n
   struct Segment {
     int r, kvh, first, n, count;
   };
-  auto segment_at = [&](long long a) {
+  auto segment_at = [&](int a) {
     Segment g;
     const int lo = find(cum, a);
     g.r = lo, g.n = cum[lo + 1] - cum[lo];
-    const int rem = (int)(a - (long long)cum[lo] * p.Hkv);
+    const int rem = a - cum[lo] * p.Hkv;
     g.kvh = rem / g.n, g.first = rem % g.n;
-    g.count = (int)min((long long)(g.n - g.first), a_end - a);
+    g.count = min(g.n - g.first, a_end - a);
     return g;
   };
   auto span_at = [&](int r) { return span_of(begin_s[r], begin_s[r + 1], len_s[r]); };
@@ -262,7 +263,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
     struct Lookup {
       int head, key, r, page;      // (r < 0: no tile)
       float ks, vs;
-    } now, ahead;
+    } now{}, ahead{};
     const int sub = lane & 7, per_page = p.page >> 4;        // sixteens of a page: 1 to 8
     auto look_pages = [&](Lookup& u, int t0) {
       u.r = -1, u.page = -1;
@@ -337,7 +338,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
     bool ok = true, ran_out = false;
     int s = 0, par = 0, sp = 0;            // the stage of S^T and its phase, the stage of P V
     int seg_s = 0, left_s = 0, seg_o = 0, left_o = 0;      // segments begun (by S^T, by P V), tiles left of them
-    long long a_s = a_begin, a_o = a_begin;
+    int a_s = a_begin, a_o = a_begin;
     for (int t = 0; t <= my_tiles && ok; ++t) {
       if (t < my_tiles) {
         if (left_s == 0) {
@@ -440,14 +441,13 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
     };
     // segments that other CTAs have a part of: the first and the last at most; merged at the end
     struct Shared {
-      long long seg0;
       Segment g;
       int nrows, q_begin;
     } shared[2];
     int n_shared = 0, t = 0, s = 0, par = 0;
     // the queries of a segment are put while the one in front is at work, and asked for one segment earlier still
     Segment now = segment_at(a_begin), next, later;
-    long long a = a_begin;
+    int a = a_begin;
     ask_queries(now);
     put_queries(0);
     sync_four();                      // the factors
@@ -615,7 +615,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
         mbar_arrive(smem_u32(&bars.o_free));
       }
       if (!whole) {
-        const Shared y = {a - g.first, g, w.nrows, w.q_begin};
+        const Shared y = {g, w.nrows, w.q_begin};
         if (n_shared == 0) shared[0] = y;
         else shared[1] = y;
         ++n_shared;
@@ -624,23 +624,16 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
       now = next, next = later;
     }
     // ---- segments of several CTAs: who counts the last arrival adds the parts up, in the CTAs' order
-    sync_four();                       // the parts are written
-    auto worker_of = [&](const Segment& g, int tile) {             // whose stretch holds this tile
-      const long long c = (long long)cost[g.r] * p.Hkv + (long long)g.kvh * (g.n + SEGMENT) + tile;
-      int w = (int)(c * workers / costs);
-      while (w + 1 < workers && costs * (w + 1) / workers <= c) ++w;
-      while (w > 0 && costs * w / workers > c) --w;
-      return w;
-    };
-    int c0[2], c1[2];
-    bool behind[2];                    // whether the first of them has another segment's end in front of its part
+    if (n_shared > 0) sync_four();     // the parts are written
+    int c0[2] = {0, 0}, c1[2] = {0, 0};
+    bool behind[2] = {false, false};   // whether the first of them has another segment's end in front of its part
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      c0[i] = c1[i] = 0, behind[i] = false;
-      if (i < n_shared) {
-        c0[i] = worker_of(shared[i].g, 0), c1[i] = worker_of(shared[i].g, shared[i].g.n - 1);
-        behind[i] = begins_at(c0[i]) < shared[i].seg0;
-      }
+      if (i >= n_shared) break;
+      const Segment& g = shared[i].g;
+      const int c = cost[g.r] * p.Hkv + g.kvh * (g.n + SEGMENT);
+      c0[i] = c / stretch, c1[i] = (c + g.n - 1) / stretch;
+      behind[i] = begins_at(c0[i]) < cum[g.r] * p.Hkv + g.kvh * g.n;
     }
     if (x < n_shared) {
       __threadfence();
@@ -651,7 +644,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
       bars.last[x] = last;
       __threadfence();
     }
-    sync_four();
+    if (n_shared > 0) sync_four();
     constexpr int LANES = 128 / ROWS, PER = HD / LANES / 2;          // threads of a row, pairs of channels of a thread
     const int row = x / LANES, sub = x % LANES;
 #pragma unroll
@@ -660,20 +653,30 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
       auto part_of = [&](int c) { return partials + ((size_t)c * 2 + (c == c0[i] && behind[i] ? 1 : 0)) * (MAX_ROWS * RS) + row * RS; };
       float mm = -INFINITY, ll = 0.f;
       float2 v[PER];
-#pragma unroll 4
-      for (int c = c0[i]; c <= c1[i]; ++c) mm = fmaxf(mm, __ldcg(part_of(c) + HD));
 #pragma unroll
       for (int e = 0; e < PER; ++e) v[e] = make_float2(0.f, 0.f);
-#pragma unroll 4
-      for (int c = c0[i]; c <= c1[i]; ++c) {
-        const float* part = part_of(c);
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + HD));
-        const float f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - mm);
-        ll += f > 0.f ? f * ml.y : ml.y == ml.y ? 0.f : ml.y;
+#pragma unroll 1
+      for (int c = c0[i]; c <= c1[i]; c += 4) {        // four parts' loads under way at once
+        float2 ml[4], y[4][PER];
 #pragma unroll
-        for (int e = 0; e < PER; ++e) {
-          const float2 y = __ldcg(reinterpret_cast<const float2*>(part + 2 * (sub + LANES * e)));
-          if (f > 0.f) v[e].x += f * y.x, v[e].y += f * y.y;
+        for (int k = 0; k < 4; ++k) {
+          const float* part = part_of(min(c + k, c1[i]));
+          ml[k] = __ldcg(reinterpret_cast<const float2*>(part + HD));
+#pragma unroll
+          for (int e = 0; e < PER; ++e) y[k][e] = __ldcg(reinterpret_cast<const float2*>(part + 2 * (sub + LANES * e)));
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (c + k > c1[i]) break;
+          const float m_new = fmaxf(mm, ml[k].x);
+          const float old = mm == -INFINITY ? 0.f : exp2_fast(mm - m_new), f = ml[k].x == -INFINITY ? 0.f : exp2_fast(ml[k].x - m_new);
+          mm = m_new;
+          ll = ll * old + (f > 0.f ? f * ml[k].y : ml[k].y == ml[k].y ? 0.f : ml[k].y);          // (a part without a key has nothing)
+#pragma unroll
+          for (int e = 0; e < PER; ++e) {
+            v[e].x = v[e].x * old + (f > 0.f ? f * y[k][e].x : 0.f);
+            v[e].y = v[e].y * old + (f > 0.f ? f * y[k][e].y : 0.f);
+          }
         }
       }
       const float inv = ll > 0.f ? 1.0f / ll : ll == ll ? 0.f : ll;
@@ -754,23 +757,16 @@ int launch(const Params& p, const CUtensorMap& km, const CUtensorMap& vm, long l
 
 }  // namespace
 
-// Whether the kernel takes this shape: heads of 64 or 128, pages of 16, 32, 64 or 128 keys, up to sixteen query heads a group.
-GB_EXPORT int gb_f8_attention_decode_takes(int hd, int page, int g) {
-  return (hd == 64 || hd == 128) && page >= 16 && page <= 128 && (page & (page - 1)) == 0 && g <= MAX_ROWS && tc_host::encode_fn() != nullptr;
-}
-// Rows (new tokens times heads of a group) up to which a request is its.
-GB_EXPORT int gb_f8_attention_decode_rows(int g) { return attn8::decode_rows(g); }
-// Bytes of the parts that CTAs leave to one another (no need to clear them) and of the counters (zero before the first launch; every
-// launch leaves them zero).
-GB_EXPORT long long gb_f8_attention_decode_scratch(int R, int Hkv, int hd, long long* counters) {
-  *counters = ((long long)R * Hkv * 4 + 255) / 256 * 256;
-  return (long long)tc_host::sm_count() * 2 * 2 * MAX_ROWS * (hd + 2) * 4;
-}
+// Bytes of the parts that CTAs leave to one another (no need to clear them). The counters are four bytes for each request and head, zero before the
+// first launch; every launch leaves them zero.
+GB_EXPORT long long gb_f8_attention_decode_part_bytes() { return (long long)tc_host::sm_count() * 2 * 2 * MAX_ROWS * (128 + 2) * 4; }
 
+// Heads of 64 or 128, pages of 16, 32, 64 or 128 keys, up to sixteen query heads a group; for requests of up to decode_rows(g) rows (new tokens
+// times heads of a group), the others are left.
 GB_EXPORT int gb_f8_attention_decode(const void* q, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale, const void* table,
                                      int table_width, const void* cu_q, const void* kv_lens, void* out, int R, long long pages, int Hq, int Hkv, int hd,
                                      float scale, int window, int page, int max_kv_len, void* parts, void* counters, void* stream) {
-  if (R <= 0 || Hkv <= 0 || Hq % Hkv || !gb_f8_attention_decode_takes(hd, page, Hq / Hkv) || (uintptr_t)q % 16 || (uintptr_t)out % 4 ||
+  if (R <= 0 || Hkv <= 0 || Hq % Hkv || (hd != 64 && hd != 128) || page < 16 || page > 128 || (page & (page - 1)) || Hq / Hkv > MAX_ROWS || (uintptr_t)q % 16 || (uintptr_t)out % 4 ||
       (uintptr_t)k_pool % 16 || (uintptr_t)v_pool % 16)
     return gb::fail(GB_BAD_ARGUMENT, "attention_f8_decode: %d requests, heads %d / %d of %d, pages of %d", R, Hq, Hkv, hd, page);
   CUtensorMap km, vm;
@@ -779,7 +775,9 @@ GB_EXPORT int gb_f8_attention_decode(const void* q, const void* k_pool, const vo
   rc = pool_map(v_pool, page, Hkv, pages, hd, &vm);
   if (rc) return rc;
   const int g = Hq / Hkv, reach = window > 0 && window + 2 * KT < max_kv_len ? window + 2 * KT : max_kv_len;
-  const int min_tiles = getenv("MINT") ? atoi(getenv("MINT")) : 4;
+  const int min_tiles = 4;
+  if (((long long)(reach + KT - 1) / KT + 4) * Hkv * (R < MAX_REQUESTS ? R : MAX_REQUESTS) > (1ll << 30))
+    return gb::fail(GB_UNSUPPORTED, "attention_f8_decode: %d requests of %d positions", R, reach);
   for (int r0 = 0; r0 < R && rc == GB_OK; r0 += MAX_REQUESTS) {
     const int n = R - r0 < MAX_REQUESTS ? R - r0 : MAX_REQUESTS;
     const Params p{(const __nv_bfloat16*)q, (const float*)k_scale, (const float*)v_scale, (__nv_bfloat16*)out,

@@ -338,7 +338,7 @@ GB_DEFINE_LAST_ERROR()
 
 // a [M, K] (rows lda apart) -> codes [M, pitch] (pitch a multiple of 16, at least K; the rest zeros) and scales
 // [ceil(K / 512)][M][4] as exponent bytes.
-GB_EXPORT int gb_f8_quantize_rows(const void* a, int tag, long long lda, int M, int K, void* codes, int pitch, void* scales, void* stream) {
+int gb_f8_quantize_rows(const void* a, int tag, long long lda, int M, int K, void* codes, int pitch, void* scales, cudaStream_t stream) {
   if (M < 0 || K <= 0 || pitch < K || pitch % 16 || (uintptr_t)codes % 16) return gb::fail(GB_BAD_ARGUMENT, "quantize_rows: %d x %d, pitch %d", M, K, pitch);
   if (M == 0) return GB_OK;
   const long long blocks = (long long)M * ((K + f8::BLOCK - 1) / f8::BLOCK);
@@ -347,7 +347,7 @@ GB_EXPORT int gb_f8_quantize_rows(const void* a, int tag, long long lda, int M, 
   return GB_DISPATCH_DTYPE(tag, T, [&]() -> int {
     const bool wide = (uintptr_t)a % 16 == 0 && lda * (long long)sizeof(T) % 16 == 0;
     auto* kernel = wide ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>;
-    return gb::check_pdl_launch(gb::launch_pdl(kernel, dim3((unsigned)grid), dim3(256), 0, (cudaStream_t)stream, dim3(1), (const T*)a, lda, M, K,
+    return gb::check_pdl_launch(gb::launch_pdl(kernel, dim3((unsigned)grid), dim3(256), 0, stream, dim3(1), (const T*)a, lda, M, K,
                                                (uint8_t*)codes, pitch, (uint8_t*)scales), "quantize_rows");
   });
 }

@@ -513,6 +513,8 @@ Plan make_plan(int M, int N, int K) {
   return q;
 }
 
+long long code_bytes(int M, int K) { return ((long long)M * ((K + 15) / 16 * 16) + 255) / 256 * 256; }
+long long scale_bytes(int M, int K) { return ((long long)(K + 4 * BK - 1) / (4 * BK) * M * 4 + 255) / 256 * 256; }
 long long part_bytes(const Plan& q) { return (long long)(q.share > 0 ? q.share : 1) * 2 * (q.pair ? 2 : 1) * q.nt * BM * 4; }
 long long counter_bytes(const Plan& q) { return ((long long)q.tiles_m * q.tiles_n * (q.pair ? 2 : 1) * 4 + 255) / 256 * 256; }
 
@@ -540,33 +542,41 @@ int launch_out(const Plan& q, const CUtensorMap& wm, const CUtensorMap& xm, cons
 
 }  // namespace
 
-// Bytes of scratch a product of this shape wants: counters (zero before the first launch; every launch leaves them zero) and parts.
-GB_EXPORT long long gb_f8_gemm_scratch_bytes(int M, int N, int K, long long* counters) {
+int gb_f8_quantize_rows(const void* a, int tag, long long lda, int M, int K, void* codes, int pitch, void* scales, cudaStream_t stream);
+
+// Bytes of scratch that a product of this shape wants (codes, scales and parts; no need to clear them), and of counters (zero before the
+// first launch; every launch leaves them zero).
+GB_EXPORT long long gb_f8_linear_scratch_bytes(int M, int N, int K, long long* counters) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   const Plan q = make_plan(M, N, K);
   *counters = counter_bytes(q);
-  return part_bytes(q);
+  return code_bytes(M, K) + scale_bytes(M, K) + part_bytes(q);
 }
 
-GB_EXPORT int gb_f8_gemm(const void* codes, int pitch, const void* xs, const void* w, long long w_pitch, const void* ws, void* out, int out_tag,
-                         int M, int N, int K, int accumulate, float alpha, void* counters, void* parts, void* stream) {
-  if (M < 0 || N < 0 || K <= 0) return gb::fail(GB_BAD_ARGUMENT, "gemm_f8: %d x %d x %d", M, N, K);
+// out [M, N] (+)= q(a) w^T: a [M, K] with rows lda apart, w [N, K] codes with rows w_pitch apart, ws its scales.
+GB_EXPORT int gb_f8_linear(const void* a, int a_tag, long long lda, const void* w, long long w_pitch, const void* ws, void* out, int out_tag, int M,
+                           int N, int K, int accumulate, float alpha, void* counters, void* scratch, void* stream) {
+  if (M < 0 || N < 0 || K <= 0) return gb::fail(GB_BAD_ARGUMENT, "linear_float8: %d x %d x %d", M, N, K);
   if (M == 0 || N == 0) return GB_OK;
-  if (w_pitch % 16 || w_pitch < K || (uintptr_t)w % 16 || (uintptr_t)codes % 16 || pitch % 16 || pitch < K)
-    return gb::fail(GB_BAD_ARGUMENT, "gemm_f8: rows of codes start on 16 bytes (pitches %d and %lld)", pitch, w_pitch);
-  if (accumulate && out_tag != GB_F32) return gb::fail(GB_BAD_ARGUMENT, "gemm_f8: accumulates into 32 bits only");
+  if (w_pitch % 16 || w_pitch < K || (uintptr_t)w % 16 || (uintptr_t)scratch % 256)
+    return gb::fail(GB_BAD_ARGUMENT, "linear_float8: rows of codes start on 16 bytes (pitch %lld)", w_pitch);
+  if (accumulate && out_tag != GB_F32) return gb::fail(GB_BAD_ARGUMENT, "linear_float8: accumulates into 32 bits only");
+  const cudaStream_t st = (cudaStream_t)stream;
+  const int pitch = (K + 15) / 16 * 16;
+  uint8_t* codes = (uint8_t*)scratch;
+  uint8_t* xs = codes + code_bytes(M, K);
+  int rc = gb_f8_quantize_rows(a, a_tag, lda, M, K, codes, pitch, xs, st);
+  if (rc) return rc;
   const Plan q = make_plan(M, N, K);
   const int ctas = q.pair ? 2 : 1;
   CUtensorMap wm, xm;
-  int rc = tensor_map(w, N, K, w_pitch, BM, &wm);
+  rc = tensor_map(w, N, K, w_pitch, BM, &wm);
   if (rc) return rc;
   rc = tensor_map(codes, M, pitch, pitch, q.nt / ctas, &xm);
   if (rc) return rc;
-  Args a{(const uint32_t*)xs, (const float*)ws, out, (float*)parts, (int*)counters, M, N, (K + BK - 1) / BK, q.nt, q.tiles_m, q.stages,
-         q.workers, q.rounds, q.units, q.share, accumulate ? alpha : 1.0f};
-  const cudaStream_t st = (cudaStream_t)stream;
-  const bool add = accumulate != 0;
-  return q.pair ? launch_out<true>(q, wm, xm, a, out_tag, add, st) : launch_out<false>(q, wm, xm, a, out_tag, add, st);
+  const Args args{(const uint32_t*)xs, (const float*)ws, out, (float*)(xs + scale_bytes(M, K)), (int*)counters, M, N, (K + BK - 1) / BK, q.nt,
+                  q.tiles_m, q.stages, q.workers, q.rounds, q.units, q.share, accumulate ? alpha : 1.0f};
+  return q.pair ? launch_out<true>(q, wm, xm, args, out_tag, accumulate != 0, st) : launch_out<false>(q, wm, xm, args, out_tag, accumulate != 0, st);
 }
 
 GB_EXPORT int gb_f8_gemm_error_check() { return gb_err::fetch_and_clear(); }

@@ -8,11 +8,12 @@ from __future__ import annotations
 
 import ctypes
 from ctypes import c_void_p, c_int, c_float, c_longlong
-from typing import NamedTuple, Optional
+from typing import NamedTuple
 
 import torch
 
 from ..csrc.build import load_kernel_lib
+from .checks import _TAG, KernelError, _need, _tag
 
 BLOCK = 128
 E4M3 = torch.float8_e4m3fn
@@ -34,17 +35,14 @@ class Float8Weight(NamedTuple):
 
 
 _FLOAT8_SIGNATURES = {
-    "gb_f8_quantize_rows": [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p],
     "gb_f8_quantize_weight": [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_longlong, c_void_p, c_void_p],
     "gb_f8_append": [c_void_p, c_int, c_longlong, c_void_p, c_int] + [c_void_p] * 7 + [c_int] * 6 + [c_void_p, c_int, c_int, c_void_p],
     "gb_f8_attention_simple": [c_void_p, c_int] + [c_void_p] * 5 + [c_int] + [c_void_p] * 3 + [c_int] * 5 + [c_float, c_int, c_int, c_int, c_void_p],
-    "gb_f8_attention_decode_takes": [c_int] * 3,
-    "gb_f8_attention_decode_rows": [c_int],
     "gb_f8_attention_decode": [c_void_p] * 6 + [c_int] + [c_void_p] * 3 + [c_int, c_longlong] + [c_int] * 3 + [c_float] + [c_int] * 3 + [c_void_p] * 3,
     "gb_f8_attention_decode_error_check": [],
     "gb_f8_attention_decode_set_error_sink": [c_void_p],
-    "gb_f8_gemm": [c_void_p, c_int, c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p,
-                   c_void_p, c_void_p],
+    "gb_f8_linear": [c_void_p, c_int, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p,
+                     c_void_p, c_void_p],
     "gb_f8_gemm_error_check": [],
     "gb_f8_gemm_set_error_sink": [c_void_p],
 }
@@ -63,20 +61,24 @@ class Float8Ops:
             for name, argtypes in _FLOAT8_SIGNATURES.items():
                 fn = getattr(L, name)
                 fn.argtypes, fn.restype = argtypes, c_int
-            L.gb_f8_gemm_scratch_bytes.argtypes = [c_int, c_int, c_int, ctypes.POINTER(c_longlong)]
-            L.gb_f8_gemm_scratch_bytes.restype = c_longlong
-            L.gb_f8_attention_decode_scratch.argtypes = [c_int, c_int, c_int, ctypes.POINTER(c_longlong)]
-            L.gb_f8_attention_decode_scratch.restype = c_longlong
+            L.gb_f8_linear_scratch_bytes.argtypes = [c_int, c_int, c_int, ctypes.POINTER(c_longlong)]
+            L.gb_f8_linear_scratch_bytes.restype = c_longlong
+            L.gb_f8_attention_decode_part_bytes.restype = c_longlong
+            self._float8_part_bytes = int(L.gb_f8_attention_decode_part_bytes())
+            self._float8_sizes, self._float8_scratch = {}, {}
             if L.gb_f8_gemm_set_error_sink(self.error_word.data_ptr()) or L.gb_f8_attention_decode_set_error_sink(self.error_word.data_ptr()):
                 _need(False, "the 8-bit library could not be given the host's error word")
             self._float8 = L
         return self._float8
 
-    def _scratch8(self, name, shape, dtype, ws, zero=False):
-        """Scratch of this name: the step's, or one per stream."""
-        if ws is not None:
-            return ws.get(name, shape, dtype, zero=zero)
-        return self.private_ws.get(f"{name}@{self._stream()}", shape, dtype, zero=zero)
+    def _scratch8(self, name, nbytes, ws, stream, zero=False):
+        """Scratch bytes of this name: the step's, or one per stream."""
+        if ws is None:
+            ws = self._float8_scratch.get(stream)
+            if ws is None:
+                from ..engine.batch import Workspace
+                ws = self._float8_scratch[stream] = Workspace(self.device)
+        return ws.get(name, (nbytes,), torch.uint8, zero=zero)
 
     def check_float8_errors(self) -> None:
         """Synchronises, and raises if an 8-bit kernel gave up on a wait since the last check."""
@@ -105,58 +107,64 @@ class Float8Ops:
         and float32 where ``accumulate`` adds ``alpha * product`` to what is there. A scale of the weights that is no positive power of two
         (``float8_weight`` makes none) turns the results of its 128 rows into NaN."""
         values, scales = w
-        self._on_device(a, values, scales, out)
+        _need(a.is_cuda and values.is_cuda and scales.is_cuda and out.is_cuda, "kernel operands must live on the CUDA device")
         _need(a.dim() == 2 and values.dim() == 2 and out.dim() == 2, "linear_float8: operands must be matrices")
         M, K = a.shape
-        N = values.shape[0]
-        if not (values.shape[1] == K and out.shape == (M, N)):
+        N, K_w = values.shape
+        a_row, w_row = a.stride(0), values.stride(0)
+        if not (K_w == K and out.shape == (M, N)):
             _need(False, f"linear_float8: shapes {tuple(a.shape)} x {tuple(values.shape)} -> {tuple(out.shape)}")
         _need(K > 0, "linear_float8: no channels")
-        _need(values.dtype == E4M3, "linear_float8: weights must be float8_e4m3fn")
-        _need(scales.dtype == torch.float32 and scales.is_contiguous()
-              and tuple(scales.shape) == ((N + BLOCK - 1) // BLOCK, (K + BLOCK - 1) // BLOCK),
+        _need(values.dtype is E4M3, "linear_float8: weights must be float8_e4m3fn")
+        _need(scales.dtype is torch.float32 and scales.is_contiguous() and scales.shape == ((N + 127) // 128, (K + 127) // 128),
               "linear_float8: one float32 scale per block of 128 x 128")
-        _need((values.stride(1) == 1 or K == 1) and (values.stride(0) % 16 == 0 or N <= 1) and values.data_ptr() % 16 == 0,
+        _need((values.stride(1) == 1 or K == 1) and (w_row % 16 == 0 or N <= 1) and values.data_ptr() % 16 == 0,
               "linear_float8: rows of codes must start on 16 bytes (float8_weight makes such)")
         _need(a.stride(1) == 1 or K == 1, "linear_float8: rows of a must have unit stride")
-        _need(out.is_contiguous() and out.dtype in (torch.float32, torch.bfloat16), "linear_float8: out must be contiguous, bfloat16 or float32")
-        _need(not accumulate or out.dtype == torch.float32, "linear_float8: accumulates into float32 only")
+        out_tag = _TAG.get(out.dtype)
+        _need(out_tag is not None and out.is_contiguous(), "linear_float8: out must be contiguous, bfloat16 or float32")
+        _need(not accumulate or out_tag == 0, "linear_float8: accumulates into float32 only")
         _need(accumulate or alpha == 1.0, "linear_float8: a multiplier goes with accumulation only")
         if M == 0 or N == 0:
             return
-        L = self.float8_lib
-        pitch = (K + 15) // 16 * 16
-        codes = self._scratch8("float8_codes", (M, pitch), torch.uint8, ws)
-        rows = self._scratch8("float8_scales", ((K + 4 * BLOCK - 1) // (4 * BLOCK), M, 4), torch.uint8, ws)
-        stream = self._stream()
-        self._check(L, L.gb_f8_quantize_rows(a.data_ptr(), _tag(a, "linear_float8 input"), a.stride(0), M, K, codes.data_ptr(), pitch,
-                                             rows.data_ptr(), stream), "quantize_rows")
-        counter_bytes = c_longlong(0)
-        part_bytes = int(L.gb_f8_gemm_scratch_bytes(M, N, K, ctypes.byref(counter_bytes)))
-        counters = self._scratch8("float8_counters", (int(counter_bytes.value),), torch.uint8, ws, zero=True)
-        parts = self._scratch8("float8_parts", (part_bytes,), torch.uint8, ws)
-        w_pitch = values.stride(0) if N > 1 else pitch
-        self._check(L, L.gb_f8_gemm(codes.data_ptr(), pitch, rows.data_ptr(), values.data_ptr(), w_pitch, scales.data_ptr(), out.data_ptr(),
-                                    _tag(out, "linear_float8 output"), M, N, K, int(accumulate), float(alpha), counters.data_ptr(),
-                                    parts.data_ptr(), stream), "linear_float8")
+        L, stream = self.float8_lib, self._stream()
+        sizes = self._float8_sizes.get((M, N, K))
+        if sizes is None:
+            counter_bytes = c_longlong(0)
+            scratch_bytes = int(L.gb_f8_linear_scratch_bytes(M, N, K, ctypes.byref(counter_bytes)))
+            if len(self._float8_sizes) > 4096:
+                self._float8_sizes.clear()
+            sizes = self._float8_sizes[M, N, K] = (scratch_bytes, int(counter_bytes.value))
+        scratch = self._scratch8("float8_linear", sizes[0], ws, stream)
+        counters = self._scratch8("float8_counters", sizes[1], ws, stream, zero=True)
+        self._check(L, L.gb_f8_linear(a.data_ptr(), _tag(a, "linear_float8 input"), a_row, values.data_ptr(), w_row if N > 1 else (K + 15) // 16 * 16,
+                                      scales.data_ptr(), out.data_ptr(), out_tag, M, N, K, accumulate, alpha, counters.data_ptr(),
+                                      scratch.data_ptr(), stream), "linear_float8", 2)
 
     # ------------------------------------------------------------------ the cache
-    def _check_pools(self, what, k_pool, v_pool, k_scale, v_scale, kv_heads, page_size, head_dim):
+    @staticmethod
+    def _check_cache(what, k_pool, v_pool, k_scale, v_scale, cu_q, kv_lens, block_table, kv_heads, page_size, head_dim):
+        """Shapes, types and layouts of the cache and the batch; the number of requests. (One condition, taken apart when it fails.)"""
+        pages, R = k_pool.shape[0], kv_lens.shape[0]
+        shape, rows = (pages, kv_heads, page_size, head_dim), (pages, kv_heads)
+        if (k_pool.shape == shape and v_pool.shape == shape and k_pool.dtype is E4M3 and v_pool.dtype is E4M3 and k_pool.is_contiguous()
+                and v_pool.is_contiguous() and k_scale.shape == rows and v_scale.shape == rows and k_scale.dtype is torch.float32
+                and v_scale.dtype is torch.float32 and k_scale.is_contiguous() and v_scale.is_contiguous()
+                and cu_q.dtype is torch.int32 and kv_lens.dtype is torch.int32 and block_table.dtype is torch.int32
+                and cu_q.is_contiguous() and kv_lens.is_contiguous() and block_table.is_contiguous()
+                and R > 0 and cu_q.shape == (R + 1,) and block_table.dim() == 2 and block_table.shape[0] >= R
+                and k_pool.is_cuda and v_pool.is_cuda and k_scale.is_cuda and v_scale.is_cuda and cu_q.is_cuda and kv_lens.is_cuda
+                and block_table.is_cuda and not (k_pool.data_ptr() | v_pool.data_ptr()) & 15):
+            return R
+        for t in (k_pool, v_pool, k_scale, v_scale, cu_q, kv_lens, block_table):
+            _need(t.is_cuda, "kernel operands must live on the CUDA device")
         for pool, scale in ((k_pool, k_scale), (v_pool, v_scale)):
-            _need(pool.dtype == E4M3 and pool.is_contiguous() and pool.dim() == 4
-                  and tuple(pool.shape[1:]) == (kv_heads, page_size, head_dim) and pool.data_ptr() % 16 == 0,
-                  f"{what}: pools must be float8_e4m3fn [pages, {kv_heads}, {page_size}, {head_dim}]")
-            _need(scale.dtype == torch.float32 and scale.is_contiguous() and tuple(scale.shape) == tuple(pool.shape[:2]),
-                  f"{what}: one float32 scale per page and head")
-        _need(k_pool.shape[0] == v_pool.shape[0], f"{what}: as many pages of keys as of values")
-
-    def _check_batch(self, what, cu_q, kv_lens, block_table):
-        R = kv_lens.shape[0]
+            _need(pool.dtype is E4M3 and pool.is_contiguous() and pool.shape == shape and pool.data_ptr() % 16 == 0,
+                  f"{what}: pools must be float8_e4m3fn {list(shape)}")
+            _need(scale.dtype is torch.float32 and scale.is_contiguous() and scale.shape == rows, f"{what}: one float32 scale per page and head")
         for t in (cu_q, kv_lens, block_table):
-            _need(t.dtype == torch.int32 and t.is_contiguous(), f"{what}: cu_q, kv_lens and the block table must be contiguous int32")
-        _need(R > 0 and cu_q.numel() == R + 1 and block_table.dim() == 2 and block_table.shape[0] >= R,
-              f"{what}: cu_q, kv_lens and the block table disagree on the number of requests")
-        return R
+            _need(t.dtype is torch.int32 and t.is_contiguous(), f"{what}: cu_q, kv_lens and the block table must be contiguous int32")
+        raise KernelError(f"{what}: cu_q, kv_lens and the block table disagree on the number of requests")
 
     def kv_append_float8(self, qkv, q_out, k_pool, v_pool, k_scale, v_scale, cu_q, kv_lens, block_table, heads, kv_heads, head_dim,
                          cos_sin, interleaved, page_size):
@@ -166,67 +174,55 @@ class Float8Ops:
         head_dim]`` with one scale per page and head ``[pages, kv_heads]``. Request r's tokens ``cu_q[r]`` to ``cu_q[r + 1]`` are its last
         positions of ``kv_lens[r]``; a page that held positions before them keeps these, in its new scale where that has grown."""
         what = "kv_append_float8"
-        self._on_device(qkv, q_out, k_pool, v_pool, k_scale, v_scale, cu_q, kv_lens, block_table, cos_sin)
-        T = qkv.shape[0]
-        R = self._check_batch(what, cu_q, kv_lens, block_table)
-        self._check_pools(what, k_pool, v_pool, k_scale, v_scale, kv_heads, page_size, head_dim)
-        _need(heads % kv_heads == 0 and head_dim % 16 == 0, f"{what}: heads in whole groups, of a multiple of 16 channels")
-        _need(qkv.dim() == 2 and qkv.shape[1] == (heads + 2 * kv_heads) * head_dim and qkv.stride(1) == 1 and qkv.stride(0) % 2 == 0
-              and qkv.data_ptr() % 8 == 0, f"{what}: qkv must be [T, (heads + 2 kv_heads) head_dim] with rows of unit stride, on 8 bytes")
-        _need(q_out.is_contiguous() and tuple(q_out.shape) == (T, heads, head_dim) and q_out.data_ptr() % 8 == 0, f"{what}: q_out shape")
-        _need(cos_sin is None or (cos_sin.dtype == torch.float32 and cos_sin.is_contiguous() and tuple(cos_sin.shape) == (T, head_dim // 2, 2)
-                                  and cos_sin.data_ptr() % 16 == 0), f"{what}: cos_sin must be float32 [T, head_dim / 2, 2]")
+        T, width = qkv.shape
+        R = self._check_cache(what, k_pool, v_pool, k_scale, v_scale, cu_q, kv_lens, block_table, kv_heads, page_size, head_dim)
+        _need(qkv.is_cuda and q_out.is_cuda and (cos_sin is None or cos_sin.is_cuda), "kernel operands must live on the CUDA device")
+        _need(heads % kv_heads == 0 and head_dim % 16 == 0, "kv_append_float8: heads in whole groups, of a multiple of 16 channels")
+        row = qkv.stride(0)
+        _need(width == (heads + 2 * kv_heads) * head_dim and qkv.stride(1) == 1 and row % 2 == 0 and qkv.data_ptr() % 8 == 0,
+              "kv_append_float8: qkv must be [T, (heads + 2 kv_heads) head_dim] with rows of unit stride, on 8 bytes")
+        _need(q_out.is_contiguous() and q_out.shape == (T, heads, head_dim) and q_out.data_ptr() % 8 == 0, "kv_append_float8: q_out shape")
+        _need(cos_sin is None or (cos_sin.dtype is torch.float32 and cos_sin.is_contiguous() and cos_sin.shape == (T, head_dim // 2, 2)
+                                  and cos_sin.data_ptr() % 16 == 0), "kv_append_float8: cos_sin must be float32 [T, head_dim / 2, 2]")
         L = self.float8_lib
         self._check(L, L.gb_f8_append(
-            qkv.data_ptr(), _tag(qkv, "qkv"), qkv.stride(0), q_out.data_ptr(), _tag(q_out, "q_out"), k_pool.data_ptr(), v_pool.data_ptr(),
+            qkv.data_ptr(), _tag(qkv, "qkv"), row, q_out.data_ptr(), _tag(q_out, "q_out"), k_pool.data_ptr(), v_pool.data_ptr(),
             k_scale.data_ptr(), v_scale.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(), block_table.shape[1], T, R,
-            heads, kv_heads, head_dim, None if cos_sin is None else cos_sin.data_ptr(), int(bool(interleaved)), int(page_size), self._stream()),
+            heads, kv_heads, head_dim, None if cos_sin is None else cos_sin.data_ptr(), bool(interleaved), page_size, self._stream()),
             what, 1 if T else 0)
 
     def paged_attention_float8(self, q, k_pool, v_pool, k_scale, v_scale, block_table, cu_q, kv_lens, out, scale, window, page_size,
                                num_requests, max_q_len, max_kv_len, ws=None, min_q_len: int = 1):
         """Causal grouped-query attention over pages of codes (``kv_append_float8``): ``q [T, Hq, hd]`` and ``out [T, Hq * hd]``
-        bfloat16 (or float32, on the plain kernel). ``window`` w > 0: a query reads the last w positions, itself included."""
+        bfloat16 (or float32, on the plain kernel). ``window`` w > 0: a query reads the last w positions, itself included. A query
+        without a key to read gets zeros."""
         what = "paged_attention_float8"
-        self._on_device(q, k_pool, v_pool, k_scale, v_scale, block_table, cu_q, kv_lens, out)
         T, Hq, hd = q.shape
         Hkv = k_pool.shape[1]
-        R = self._check_batch(what, cu_q, kv_lens, block_table)
-        _need(R == num_requests, f"{what}: as many lengths as requests")
-        self._check_pools(what, k_pool, v_pool, k_scale, v_scale, Hkv, page_size, hd)
-        _need(Hq % Hkv == 0 and hd % 16 == 0 and hd <= 256, f"{what}: heads in whole groups, of a multiple of 16 channels up to 256")
-        _need(q.is_contiguous() and out.is_contiguous() and tuple(out.shape) == (T, Hq * hd) and q.dtype == out.dtype, f"{what}: q/out shape")
-        _need(q.data_ptr() % 8 == 0 and out.data_ptr() % 8 == 0, f"{what}: q and out on 8 bytes")
-        _need(scale > 0, f"{what}: a positive scale")
-        _need(block_table.shape[1] * page_size >= max_kv_len, f"{what}: the block table is too narrow for {max_kv_len} positions")
+        R = self._check_cache(what, k_pool, v_pool, k_scale, v_scale, cu_q, kv_lens, block_table, Hkv, page_size, hd)
+        _need(q.is_cuda and out.is_cuda, "kernel operands must live on the CUDA device")
+        _need(R == num_requests, "paged_attention_float8: as many lengths as requests")
+        _need(Hq % Hkv == 0 and hd % 16 == 0 and hd <= 256, "paged_attention_float8: heads in whole groups, of a multiple of 16 channels up to 256")
+        _need(q.is_contiguous() and out.is_contiguous() and out.shape == (T, Hq * hd) and q.dtype is out.dtype, "paged_attention_float8: q/out shape")
+        q_ptr, out_ptr = q.data_ptr(), out.data_ptr()
+        _need(not (q_ptr | out_ptr) & 7, "paged_attention_float8: q and out on 8 bytes")
+        _need(scale > 0, "paged_attention_float8: a positive scale")
+        table_width = block_table.shape[1]
+        _need(table_width * page_size >= max_kv_len, "paged_attention_float8: the block table is too narrow for that many positions")
         if T == 0:
             return
         L, g, stream = self.float8_lib, Hq // Hkv, self._stream()
+        pools = (k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), table_width,
+                 cu_q.data_ptr(), kv_lens.data_ptr(), out_ptr)
         above = -1             # requests of more rows (new tokens times heads of a group) than this are still to do
-        if q.dtype == torch.bfloat16 and q.data_ptr() % 16 == 0 and L.gb_f8_attention_decode_takes(hd, int(page_size), g):
-            rows = L.gb_f8_attention_decode_rows(g)
-            if min_q_len * g <= rows:
-                counter_bytes = c_longlong(0)
-                parts = self._scratch8("float8_attention_parts", (int(L.gb_f8_attention_decode_scratch(R, Hkv, hd, ctypes.byref(counter_bytes))),),
-                                       torch.uint8, ws)
-                counters = self._scratch8("float8_attention_counters", (int(counter_bytes.value),), torch.uint8, ws, zero=True)
+        if (q.dtype is torch.bfloat16 and hd in (64, 128) and page_size in (16, 32, 64, 128) and g <= 16 and not q_ptr & 15):
+            above = 8 if g <= 8 else 16
+            if min_q_len * g <= above:
+                scratch = self._scratch8("float8_attention_parts", self._float8_part_bytes, ws, stream)
+                counters = self._scratch8("float8_attention_counters", 4 * R * Hkv, ws, stream, zero=True)
                 self._check(L, L.gb_f8_attention_decode(
-                    q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(),
-                    block_table.shape[1], cu_q.data_ptr(), kv_lens.data_ptr(), out.data_ptr(), R, k_pool.shape[0], Hq, Hkv, hd, float(scale),
-                    int(window), int(page_size), int(max_kv_len), parts.data_ptr(), counters.data_ptr(), stream), what)
-            above = rows
+                    q_ptr, *pools, R, k_pool.shape[0], Hq, Hkv, hd, scale, window, page_size, max_kv_len, scratch.data_ptr(),
+                    counters.data_ptr(), stream), what)
         if above < 0 or max_q_len * g > above:
-            self._check(L, L.gb_f8_attention_simple(
-                q.data_ptr(), _tag(q, "attention q"), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                block_table.data_ptr(), block_table.shape[1], cu_q.data_ptr(), kv_lens.data_ptr(), out.data_ptr(), T, R, Hq, Hkv, hd,
-                float(scale), int(window), int(page_size), above, stream), what)
-
-
-def _need(cond, msg):
-    from . import ops
-    ops._need(cond, msg)
-
-
-def _tag(t, what):
-    from . import ops
-    return ops._tag(t, what)
+            self._check(L, L.gb_f8_attention_simple(q_ptr, _tag(q, "attention q"), *pools, T, R, Hq, Hkv, hd, scale, window, page_size, above,
+                                                    stream), what)

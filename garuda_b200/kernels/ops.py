@@ -17,31 +17,8 @@ import numpy as np
 import torch
 
 from ..csrc.build import load_kernel_lib
+from .checks import GB_BF16, GB_F32, KernelError, _need, _ptr, _tag
 from .float8 import Float8Ops
-
-GB_F32, GB_BF16 = 0, 1
-_TAG = {torch.float32: GB_F32, torch.bfloat16: GB_BF16}
-
-
-class KernelError(RuntimeError):
-    pass
-
-
-def _tag(t: torch.Tensor, what: str) -> int:
-    try:
-        return _TAG[t.dtype]
-    except KeyError:
-        raise KernelError(f"{what}: dtype {t.dtype} is not supported (float32 or bfloat16)") from None
-
-
-def _need(cond: bool, msg: str) -> None:
-    if not cond:
-        raise KernelError(msg)
-
-
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
-
 
 _ERROR_WORD = None
 
@@ -95,6 +72,7 @@ class CudaOps(Float8Ops):
         if not torch.cuda.is_available():
             raise KernelError("garuda_b200 needs a CUDA device: there is no CPU path")
         self.device = torch.device(device)
+        self._device_index = self.device.index if self.device.index is not None else torch.cuda.current_device()
         self.core = load_kernel_lib("garuda_core")
         self._mixers = None
         self._state = None
@@ -356,7 +334,8 @@ class CudaOps(Float8Ops):
     def _stream(self):
         if self._held_stream is not None:
             return self._held_stream
-        return torch.cuda.current_stream(self.device).cuda_stream
+        # (what torch.cuda.current_stream(self.device).cuda_stream is, without making the object: 0.2 us against 1.5)
+        return torch._C._cuda_getCurrentRawStream(self._device_index)
 
     @contextlib.contextmanager
     def on_current_stream(self):
