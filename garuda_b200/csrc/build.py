@@ -48,7 +48,7 @@ KERNEL_LIBS: Dict[str, List[str]] = {
     # first needs them
     "garuda_memory": ["residual_norm.cu", "matrix_memory.cu", "attention_diff.cu"],
     # weights, tokens and cache pages in 8 bits: built when an engine first asks for them
-    "garuda_float8": ["float8.cu", "gemm_float8.cu", "attention_float8_decode.cu"],
+    "garuda_float8": ["float8.cu", "gemm_float8.cu", "attention_float8_decode.cu", "attention_float8_tile.cu"],
 }
 HOST_SOURCES = ["cache_manager.cpp", "scheduler.cpp", "step_batch.cpp", "bindings.cpp"]
 

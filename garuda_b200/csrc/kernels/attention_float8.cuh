@@ -6,7 +6,7 @@
 namespace attn8 {
 
 // A request with at most this many (token, head-of-group) rows is a decode request: each is two of a product's 16 (or 32) columns.
-inline int decode_rows(int g) { return g <= 8 ? 8 : 16; }
+__host__ __device__ inline int decode_rows(int g) { return g <= 8 ? 8 : g <= 16 ? 16 : 0; }
 
 struct Params {
   const __nv_bfloat16* q;        // [T, Hq, HD]

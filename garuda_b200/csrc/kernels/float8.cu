@@ -244,7 +244,6 @@ struct AttentionSimple {
   const int32_t *table, *cu_q, *kv_lens;
   void* out;
   int table_width, T, R, Hq, Hkv, hd, page, window;
-  int above;               // requests of at most this many (token, head-of-group) rows are another kernel's
   float scale_log2;
 };
 
@@ -264,7 +263,6 @@ __global__ void __launch_bounds__(128) attention_f8_simple_kernel(const Attentio
     if (p.cu_q[mid] <= t) lo = mid;
     else hi = mid;
   }
-  if ((p.cu_q[lo + 1] - p.cu_q[lo]) * (p.Hq / p.Hkv) <= p.above) return;
   const int r = lo, pos = p.kv_lens[r] - (p.cu_q[r + 1] - t);
   const int start = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
   const int32_t* table = p.table + (size_t)r * p.table_width;
@@ -384,12 +382,12 @@ GB_EXPORT int gb_f8_append(const void* qkv, int tag, long long qkv_stride, void*
 
 GB_EXPORT int gb_f8_attention_simple(const void* q, int tag, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale,
                                      const void* table, int table_width, const void* cu_q, const void* kv_lens, void* out, int T, int R,
-                                     int Hq, int Hkv, int hd, float scale, int window, int page, int above, void* stream) {
+                                     int Hq, int Hkv, int hd, float scale, int window, int page, void* stream) {
   if (T < 0 || R <= 0 || Hkv <= 0 || Hq % Hkv || hd % 16 || hd > MAX_HD || page <= 0)
     return gb::fail(GB_BAD_ARGUMENT, "f8_attention: %d tokens, %d requests, heads %d / %d of %d, pages of %d", T, R, Hq, Hkv, hd, page);
   if (T == 0) return GB_OK;
   AttentionSimple p{q, (const uint8_t*)k_pool, (const uint8_t*)v_pool, (const float*)k_scale, (const float*)v_scale, (const int32_t*)table,
-                    (const int32_t*)cu_q, (const int32_t*)kv_lens, out, table_width, T, R, Hq, Hkv, hd, page, window, above,
+                    (const int32_t*)cu_q, (const int32_t*)kv_lens, out, table_width, T, R, Hq, Hkv, hd, page, window,
                     scale * 1.4426950408889634f};
   const long long grid = ((long long)T * Hq + 3) / 4;
   if (grid > 0x7fffffff) return gb::fail(GB_UNSUPPORTED, "f8_attention: %lld rows", (long long)T * Hq);

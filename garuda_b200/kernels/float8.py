@@ -37,8 +37,11 @@ class Float8Weight(NamedTuple):
 _FLOAT8_SIGNATURES = {
     "gb_f8_quantize_weight": [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_longlong, c_void_p, c_void_p],
     "gb_f8_append": [c_void_p, c_int, c_longlong, c_void_p, c_int] + [c_void_p] * 7 + [c_int] * 6 + [c_void_p, c_int, c_int, c_void_p],
-    "gb_f8_attention_simple": [c_void_p, c_int] + [c_void_p] * 5 + [c_int] + [c_void_p] * 3 + [c_int] * 5 + [c_float, c_int, c_int, c_int, c_void_p],
+    "gb_f8_attention_simple": [c_void_p, c_int] + [c_void_p] * 5 + [c_int] + [c_void_p] * 3 + [c_int] * 5 + [c_float, c_int, c_int, c_void_p],
     "gb_f8_attention_decode": [c_void_p] * 6 + [c_int] + [c_void_p] * 3 + [c_int, c_longlong] + [c_int] * 3 + [c_float] + [c_int] * 3 + [c_void_p] * 3,
+    "gb_f8_attention_tile": [c_void_p] * 6 + [c_int] + [c_void_p] * 3 + [c_int, c_longlong] + [c_int] * 3 + [c_float] + [c_int] * 3 + [c_void_p],
+    "gb_f8_attention_tile_error_check": [],
+    "gb_f8_attention_tile_set_error_sink": [c_void_p],
     "gb_f8_attention_decode_error_check": [],
     "gb_f8_attention_decode_set_error_sink": [c_void_p],
     "gb_f8_linear": [c_void_p, c_int, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p,
@@ -66,7 +69,8 @@ class Float8Ops:
             L.gb_f8_attention_decode_part_bytes.restype = c_longlong
             self._float8_part_bytes = int(L.gb_f8_attention_decode_part_bytes())
             self._float8_sizes, self._float8_scratch = {}, {}
-            if L.gb_f8_gemm_set_error_sink(self.error_word.data_ptr()) or L.gb_f8_attention_decode_set_error_sink(self.error_word.data_ptr()):
+            sinks = (L.gb_f8_gemm_set_error_sink, L.gb_f8_attention_decode_set_error_sink, L.gb_f8_attention_tile_set_error_sink)
+            if any([sink(self.error_word.data_ptr()) for sink in sinks]):
                 _need(False, "the 8-bit library could not be given the host's error word")
             self._float8 = L
         return self._float8
@@ -84,7 +88,8 @@ class Float8Ops:
         """Synchronises, and raises if an 8-bit kernel gave up on a wait since the last check."""
         seen, self.error_word[0] = int(self.error_word[0]), 0
         L = self.float8_lib
-        code = L.gb_f8_gemm_error_check() or L.gb_f8_attention_decode_error_check() or seen
+        codes = [L.gb_f8_gemm_error_check(), L.gb_f8_attention_decode_error_check(), L.gb_f8_attention_tile_error_check(), seen]
+        code = next((c for c in codes if c), 0)
         _need(not code, f"an 8-bit kernel gave up waiting: code {code}")
 
     # ------------------------------------------------------------------ matrix products
@@ -214,15 +219,17 @@ class Float8Ops:
         L, g, stream = self.float8_lib, Hq // Hkv, self._stream()
         pools = (k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), table_width,
                  cu_q.data_ptr(), kv_lens.data_ptr(), out_ptr)
-        above = -1             # requests of more rows (new tokens times heads of a group) than this are still to do
-        if (q.dtype is torch.bfloat16 and hd in (64, 128) and page_size in (16, 32, 64, 128) and g <= 16 and not q_ptr & 15):
-            above = 8 if g <= 8 else 16
-            if min_q_len * g <= above:
+        if q.dtype is torch.bfloat16 and hd in (64, 128) and page_size in (16, 32, 64, 128) and g <= 128 and not (q_ptr | out_ptr) & 15:
+            # requests of a few rows (new tokens times heads of a group) go to one kernel, the others to the other
+            few = (8 if g <= 8 else 16) if g <= 16 else 0
+            if min_q_len * g <= few:
                 scratch = self._scratch8("float8_attention_parts", self._float8_part_bytes, ws, stream)
                 counters = self._scratch8("float8_attention_counters", 4 * R * Hkv, ws, stream, zero=True)
                 self._check(L, L.gb_f8_attention_decode(
                     q_ptr, *pools, R, k_pool.shape[0], Hq, Hkv, hd, scale, window, page_size, max_kv_len, scratch.data_ptr(),
                     counters.data_ptr(), stream), what)
-        if above < 0 or max_q_len * g > above:
-            self._check(L, L.gb_f8_attention_simple(q_ptr, _tag(q, "attention q"), *pools, T, R, Hq, Hkv, hd, scale, window, page_size, above,
-                                                    stream), what)
+            if max_q_len * g > few:
+                self._check(L, L.gb_f8_attention_tile(q_ptr, *pools, R, k_pool.shape[0], Hq, Hkv, hd, scale, window, page_size, max_q_len, stream),
+                            what)
+            return
+        self._check(L, L.gb_f8_attention_simple(q_ptr, _tag(q, "attention q"), *pools, T, R, Hq, Hkv, hd, scale, window, page_size, stream), what)
