@@ -36,6 +36,8 @@
 #include "tc_common.cuh"
 #include "tc_host.cuh"
 
+#include <algorithm>
+
 namespace {
 
 using namespace tc;
@@ -218,7 +220,8 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
   }
   // Stretches are equal in cost: a request's head is its tiles and SEGMENT behind them. (The host has seen that all of it fits 31 bits.)
   const int tiles = cum[p.R] * p.Hkv, costs = cost[p.R] * p.Hkv;
-  const int workers = max(1, min((int)gridDim.x, tiles / min_tiles));          // each has min_tiles or so at least
+  // as many workers as leave each min_tiles or so, and one for every head that has tiles
+  const int workers = max(1, min((int)gridDim.x, max(tiles / min_tiles, bars.total.y * p.Hkv)));
   const int stretch = max(1, (costs + workers - 1) / workers);
   const int cta = blockIdx.x;
   auto find = [&](const int* sums, int at) {           // the last request whose heads begin at or before it
@@ -749,7 +752,7 @@ int launch(const Params& p, const CUtensorMap& km, const CUtensorMap& vm, long l
     configured.done();
   }
   const int room = tc_host::sm_count() * S::CTAS;
-  const long long most = tiles_most / min_tiles + 1;
+  const long long most = std::max(tiles_most / min_tiles + 1, (long long)p.R * p.Hkv);
   const size_t smem = 1024 + S::BYTES + (size_t)(4 * p.R + 3) * 4;
   return gb::check_pdl_launch(gb::launch_pdl(kernel, dim3((unsigned)(most < room ? most : room)), dim3(THREADS), smem, stream, dim3(1), km, vm, p,
                                              min_tiles, (float*)parts, (int*)counters), "attention_f8_decode");

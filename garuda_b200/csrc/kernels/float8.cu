@@ -151,13 +151,17 @@ struct Append {
   bool interleaved;
 };
 
-constexpr int APPEND_THREADS = 256;
+constexpr int APPEND_THREADS = 256, APPEND_WARPS = APPEND_THREADS / 32;
+constexpr int KEPT = 4;         // rows of keys and of values that a thread keeps in registers between their maximum and their codes
 
-template <typename TI, typename TO>
-__global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const Append p) {
+// KEEP: a page's rows fit the block's registers (page * head size <= 4,096: 32 keys of 128 channels): read once; else they are read twice.
+// Lanes lie along a row (four channels each; short rows share a warp), warps take the rows in turn. The queries of a page's tokens have
+// blocks of their own (blockIdx.y from Hkv on, `QUERIES` heads each): they wait for no maximum.
+constexpr int QUERIES = 4;
+template <typename TI, typename TO, bool KEEP>
+__global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const Append p) {
   gb::pdl_launch_dependents();
-  __shared__ float part[2][APPEND_THREADS / 32];
-  const int kvh = blockIdx.y, g = p.Hq / p.Hkv;
+  __shared__ float part[2][APPEND_WARPS];
   // the request of this block: the last one that starts at or before it
   int lo = 0, hi = p.R;
   const int slot = blockIdx.x;
@@ -177,60 +181,96 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const Append p) 
 
   const int half = p.hd / 2, fours = p.hd / 4;
   const bool rotated = p.cos_sin != nullptr, split = rotated && !p.interleaved;
-  const TI* rows = reinterpret_cast<const TI*>(p.qkv);
-  auto k_row = [&](int t) { return rows + (tok0 + t) * p.qkv_stride + (size_t)(p.Hq + kvh) * p.hd; };
-  auto v_row = [&](int t) { return rows + (tok0 + t) * p.qkv_stride + (size_t)(p.Hq + p.Hkv + kvh) * p.hd; };
-  auto angles = [&](int t) { return p.cos_sin + (size_t)(tok0 + t) * p.hd; };
-  gb::pdl_wait();
-  if (at >= 0) {
-    float mk = 0.f, mv = 0.f;
-    for (int i = threadIdx.x; i < n * fours; i += APPEND_THREADS) {
-      const int t = i / fours, j = i % fours;
-      Four k = load_four(k_row(t), j, half, split);
-      if (rotated) rotate(k, angles(t), j, split);
-      mk = fmaxf(mk, largest_of(k));
-      mv = fmaxf(mv, largest_of(load_four(v_row(t), j, half, false)));
-    }
-    mk = gb::warp_max(mk), mv = gb::warp_max(mv);
-    if ((threadIdx.x & 31) == 0) part[0][threadIdx.x >> 5] = mk, part[1][threadIdx.x >> 5] = mv;
-    const size_t where = (size_t)at * p.Hkv + kvh;
-    const float old_k = held ? p.k_scale[where] : 0.f, old_v = held ? p.v_scale[where] : 0.f;
-    __syncthreads();
-    mk = part[0][0], mv = part[1][0];
-#pragma unroll
-    for (int w = 1; w < APPEND_THREADS / 32; ++w) mk = fmaxf(mk, part[0][w]), mv = fmaxf(mv, part[1][w]);
-    const float sk = fmaxf(old_k, power_of_two(scale_exponent(mk))), sv = fmaxf(old_v, power_of_two(scale_exponent(mv)));
-    if (threadIdx.x == 0) p.k_scale[where] = sk, p.v_scale[where] = sv;       // (every thread has read the old ones)
-    uint8_t* kp = p.k_pool + where * p.page * p.hd;
-    uint8_t* vp = p.v_pool + where * p.page * p.hd;
-    // the scale has grown: the rows that were there are encoded again
-    for (int which = 0; which < 2; ++which) {
-      const float s = which ? sv : sk, old = which ? old_v : old_k;
-      if (held == 0 || s == old) continue;
-      uint32_t* codes = reinterpret_cast<uint32_t*>(which ? vp : kp);
-      const float factor = old / s;
-      for (int i = threadIdx.x; i < held * fours; i += APPEND_THREADS) {
-        const float4 x = decode4(codes[i]);
-        codes[i] = encode4(x.x * factor, x.y * factor, x.z * factor, x.w * factor);
+  // this thread's place: row `row0` of every `step`, channels 4 j0 (and, in rows of more than 128, 4 (j0 + 32))
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int shared = fours == 16 ? 2 : fours == 8 ? 4 : fours == 4 ? 8 : 1;          // rows of a warp
+  const int row0 = warp * shared + (shared > 1 ? lane / fours : 0), step = APPEND_WARPS * shared;
+  const int j0 = shared > 1 ? lane % fours : lane;
+  const TI* rows = reinterpret_cast<const TI*>(p.qkv) + tok0 * p.qkv_stride;
+  const float* angles = p.cos_sin + (size_t)tok0 * p.hd;
+  if (blockIdx.y >= p.Hkv) {
+    const int h0 = ((int)blockIdx.y - p.Hkv) * QUERIES, heads = min(QUERIES, p.Hq - h0);
+    TO* const q_out = reinterpret_cast<TO*>(p.q_out) + ((size_t)tok0 * p.Hq + h0) * p.hd;
+    gb::pdl_wait();
+#pragma unroll 4
+    for (int i = row0; i < n * heads; i += step) {
+      const int t = i / heads, h = i - t * heads;
+      for (int j = j0; j < fours; j += 32) {
+        Four q = load_four(rows + t * p.qkv_stride + (size_t)(h0 + h) * p.hd, j, half, split);
+        if (rotated) rotate(q, angles + (size_t)t * p.hd, j, split);
+        TO* to = q_out + ((size_t)t * p.Hq + h) * p.hd;
+        gb::store_pair(to + (split ? 2 * j : 4 * j), q.a.x, q.a.y);
+        gb::store_pair(to + (split ? half + 2 * j : 4 * j + 2), q.b.x, q.b.y);
       }
     }
-    const float ik = 1.0f / sk, iv = 1.0f / sv;        // powers of two: exact
-    for (int i = threadIdx.x; i < n * fours; i += APPEND_THREADS) {
-      const int t = i / fours, j = i % fours;
-      Four k = load_four(k_row(t), j, half, split);
-      if (rotated) rotate(k, angles(t), j, split);
-      store_codes(kp + (size_t)(held + t) * p.hd, k, ik, j, half, split);
-      store_codes(vp + (size_t)(held + t) * p.hd, load_four(v_row(t), j, half, false), iv, j, half, false);
+    return;
+  }
+  const int kvh = blockIdx.y;
+  if (at < 0) return;
+  const TI* keys = rows + (size_t)(p.Hq + kvh) * p.hd;
+  const TI* values = keys + (size_t)p.Hkv * p.hd;
+  auto key = [&](int t, int j) {
+    Four k = load_four(keys + t * p.qkv_stride, j, half, split);
+    if (rotated) rotate(k, angles + (size_t)t * p.hd, j, split);
+    return k;
+  };
+  auto value = [&](int t, int j) { return load_four(values + t * p.qkv_stride, j, half, false); };
+  const size_t where = (size_t)at * p.Hkv + kvh;
+  gb::pdl_wait();
+  const float old_k = held ? p.k_scale[where] : 0.f, old_v = held ? p.v_scale[where] : 0.f;
+  float mk = 0.f, mv = 0.f;
+  Four ks[KEEP ? KEPT : 1], vs[KEEP ? KEPT : 1];
+  if (KEEP) {
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i) {
+      const int t = row0 + i * step;
+      if (t < n && j0 < fours) {
+        ks[i] = key(t, j0), vs[i] = value(t, j0);
+        mk = fmaxf(mk, largest_of(ks[i])), mv = fmaxf(mv, largest_of(vs[i]));
+      }
+    }
+  } else {
+    for (int t = row0; t < n; t += step)
+      for (int j = j0; j < fours; j += 32) mk = fmaxf(mk, largest_of(key(t, j))), mv = fmaxf(mv, largest_of(value(t, j)));
+  }
+  mk = gb::warp_max(mk), mv = gb::warp_max(mv);
+  if (lane == 0) part[0][warp] = mk, part[1][warp] = mv;
+  __syncthreads();
+  mk = part[0][0], mv = part[1][0];
+#pragma unroll
+  for (int w = 1; w < APPEND_WARPS; ++w) mk = fmaxf(mk, part[0][w]), mv = fmaxf(mv, part[1][w]);
+  const float sk = fmaxf(old_k, power_of_two(scale_exponent(mk))), sv = fmaxf(old_v, power_of_two(scale_exponent(mv)));
+  if (threadIdx.x == 0) p.k_scale[where] = sk, p.v_scale[where] = sv;       // (every thread has read the old ones)
+  uint8_t* kp = p.k_pool + where * p.page * p.hd;
+  uint8_t* vp = p.v_pool + where * p.page * p.hd;
+  // the scale has grown: the rows that were there are encoded again
+  for (int which = 0; which < 2; ++which) {
+    const float s = which ? sv : sk, old = which ? old_v : old_k;
+    if (held == 0 || s == old) continue;
+    uint32_t* codes = reinterpret_cast<uint32_t*>(which ? vp : kp);
+    const float factor = old / s;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < held * fours; i += APPEND_THREADS) {
+      const float4 x = decode4(codes[i]);
+      codes[i] = encode4(x.x * factor, x.y * factor, x.z * factor, x.w * factor);
     }
   }
-  // the queries of these tokens that read this head
-  for (int i = threadIdx.x; i < n * g * fours; i += APPEND_THREADS) {
-    const int t = i / (g * fours), h = kvh * g + i / fours % g, j = i % fours;
-    Four q = load_four(rows + (tok0 + t) * p.qkv_stride + (size_t)h * p.hd, j, half, split);
-    if (rotated) rotate(q, angles(t), j, split);
-    TO* to = reinterpret_cast<TO*>(p.q_out) + ((size_t)(tok0 + t) * p.Hq + h) * p.hd;
-    gb::store_pair(to + (split ? 2 * j : 4 * j), q.a.x, q.a.y);
-    gb::store_pair(to + (split ? half + 2 * j : 4 * j + 2), q.b.x, q.b.y);
+  const float ik = 1.0f / sk, iv = 1.0f / sv;        // powers of two: exact
+  if (KEEP) {
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i) {
+      const int t = row0 + i * step;
+      if (t < n && j0 < fours) {
+        store_codes(kp + (size_t)(held + t) * p.hd, ks[i], ik, j0, half, split);
+        store_codes(vp + (size_t)(held + t) * p.hd, vs[i], iv, j0, half, false);
+      }
+    }
+  } else {
+    for (int t = row0; t < n; t += step)
+      for (int j = j0; j < fours; j += 32) {
+        store_codes(kp + (size_t)(held + t) * p.hd, key(t, j), ik, j, half, split);
+        store_codes(vp + (size_t)(held + t) * p.hd, value(t, j), iv, j, half, false);
+      }
   }
 }
 
@@ -365,7 +405,7 @@ GB_EXPORT int gb_f8_quantize_weight(const void* w, int tag, long long ldw, int N
 GB_EXPORT int gb_f8_append(const void* qkv, int tag, long long qkv_stride, void* q_out, int q_tag, void* k_pool, void* v_pool, void* k_scale,
                            void* v_scale, const void* cu_q, const void* kv_lens, const void* table, int table_width, int T, int R, int Hq,
                            int Hkv, int hd, const void* cos_sin, int interleaved, int page, void* stream) {
-  if (T < 0 || R <= 0 || Hkv <= 0 || Hq % Hkv || hd % 16 || page <= 0 || Hkv > 65535)
+  if (T < 0 || R <= 0 || Hkv <= 0 || Hq % Hkv || hd % 16 || page <= 0 || Hq > 65535)
     return gb::fail(GB_BAD_ARGUMENT, "f8_append: %d tokens, %d requests, heads %d / %d of %d, pages of %d", T, R, Hq, Hkv, hd, page);
   if (T == 0) return GB_OK;
   Append p{qkv, qkv_stride, q_out, (uint8_t*)k_pool, (uint8_t*)v_pool, (float*)k_scale, (float*)v_scale, (const int32_t*)cu_q,
@@ -374,8 +414,10 @@ GB_EXPORT int gb_f8_append(const void* qkv, int tag, long long qkv_stride, void*
   if (slots > 0x7fffffff) return gb::fail(GB_UNSUPPORTED, "f8_append: %lld pages", slots);
   return GB_DISPATCH_DTYPE(tag, TI, [&]() -> int {
     return GB_DISPATCH_DTYPE(q_tag, TO, [&]() -> int {
-      return gb::check_pdl_launch(gb::launch_pdl(append_kernel<TI, TO>, dim3((unsigned)slots, (unsigned)Hkv), dim3(APPEND_THREADS), 0,
-                                                 (cudaStream_t)stream, dim3(1), p), "f8_append");
+      const int fours = hd / 4, shared = fours == 16 ? 2 : fours == 8 ? 4 : fours == 4 ? 8 : 1;
+      auto* kernel = fours <= 32 && page <= KEPT * APPEND_WARPS * shared ? append_kernel<TI, TO, true> : append_kernel<TI, TO, false>;
+      return gb::check_pdl_launch(gb::launch_pdl(kernel, dim3((unsigned)slots, (unsigned)(Hkv + (Hq + QUERIES - 1) / QUERIES)), dim3(APPEND_THREADS), 0, (cudaStream_t)stream, dim3(1), p),
+                                  "f8_append");
     });
   });
 }

@@ -21,7 +21,7 @@
 //   warp 0     TMA: a box of 128 bytes (128 channels) by 128 weight rows and one by the tokens, a ring of stages. Weights are asked for
 //              before the wait for the kernel in front, which makes the codes.
 //   warp 1     one elected lane: scales into tensor memory, four products a unit
-//   warp 2     the scales of four blocks into shared memory: row r's word at 16 (r % 32) + 4 (r / 32) of 512 bytes for 128 rows, as
+//   warps 2, 3 the scales of four blocks into shared memory: row r's word at 16 (r % 32) + 4 (r / 32) of 512 bytes for 128 rows, as
 //              the copy to tensor memory wants it (128 equal words for the weights, whose scale belongs to the block)
 //   warps 4-11 at a tile's end: write out, or write the part and perhaps add the parts up; the products go on in the
 //              other of two accumulators
@@ -42,9 +42,10 @@ constexpr int BM = 128;                         // weight rows per CTA
 constexpr int MAX_NT = 240;                     // tokens per tile: two accumulators leave room for the scales
 constexpr int THREADS = 128 + 256;
 constexpr int MAX_STAGES = 12;
-constexpr int SF_STAGES = 3, SF_BYTES = 3 * 512;        // the weights' words, the tokens' (up to 256)
+constexpr int SF_STAGES = 4, SF_BYTES = 3 * 512;        // the weights' words, the tokens' (up to 256)
 constexpr int SMEM_LIMIT = 232448, STATIC_BYTES = 1024;
-// tensor memory: accumulators at columns 0 and 256, scales in the gap behind the first
+// tensor memory: accumulators at columns 0 and 256, scales in the gaps behind them: two sets in turn, so that copying one set does not wait
+// for the products that read the other
 constexpr uint32_t ACC_STRIDE = 256, SFA_COL = 240, SFB_COL = 244;
 
 struct Args {
@@ -55,7 +56,8 @@ struct Args {
   int* counters;            // [tiles * CTAs of a worker], zero between launches
   int M, N, blocks;
   int nt, tiles_m;          // tokens per tile (a multiple of 16), tiles of tokens
-  int stages, workers, rounds;      // rounds: whole tiles for every worker
+  int stages, step;         // step: units of a stage (1 or 2)
+  int workers, rounds;      // rounds: whole tiles for every worker
   long long units;          // those of the tiles behind the rounds,
   int share;                // and the workers that share these
   float alpha;
@@ -119,7 +121,6 @@ struct Walk {
     tile = p.rounds > 0 ? worker : rest_tile, b = p.rounds > 0 ? 0 : rest_b;
   }
   __device__ __forceinline__ bool more() const { return i < n; }
-  __device__ __forceinline__ bool begins() const { return b == 0 || i == in_rounds; }          // a tile, or this worker's part of one
   __device__ __forceinline__ int left() const { return min(blocks - b, n - i); }               // units of it from here on
   __device__ __forceinline__ void advance(int k) {       // by up to left()
     i += k, b += k;
@@ -143,7 +144,7 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
   const uint32_t rank = PAIR ? cluster_ctarank() : 0;
   const int worker = blockIdx.x / CTAS;
   const int x_rows = p.nt / CTAS;                                  // rows of the tokens' box
-  const uint32_t stage_bytes = (uint32_t)(BM + x_rows) * BK;
+  const uint32_t unit_bytes = (uint32_t)(BM + x_rows) * BK, stage_bytes = unit_bytes * p.step;        // a stage: weights, then tokens
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const int stages = p.stages;
   const uint32_t sf_at = ring + stages * stage_bytes;              // behind the ring: the scales on their way
@@ -188,41 +189,65 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
 
   if (warp == 0) {
     // ---------------------------------------------------------------- producer
+    // What does not change within a tile is worked out once a tile, here and in the issuer: a division a step and a look at the abort flag
+    // made a step 650 cycles, whatever its width.
     const bool leader = elect_one();
-    bool go = true, ran_out;
-    auto load_w = [&](int s, const Walk& q) {
-      const uint32_t full = smem_u32(&full_bar[s]), bar = PAIR ? map_to_rank(full, 0) : full;
-      const int row = (q.tile / p.tiles_m * CTAS + (int)rank) * BM;
-      if (rank == 0) mbar_arrive_expect_tx(full, CTAS * stage_bytes);
-      if (PAIR) tma_load_2d_pair(ring + s * stage_bytes, &w_map, bar, q.b * BK, row);
-      else tma_load_2d(ring + s * stage_bytes, &w_map, bar, q.b * BK, row);
+    bool go = true;
+    struct Rows {
+      int w, x;              // the first weight row and token of the tile that this CTA fetches
     };
-    auto load_x = [&](int s, const Walk& q) {
-      const uint32_t full = smem_u32(&full_bar[s]), bar = PAIR ? map_to_rank(full, 0) : full;
-      const int row = q.tile % p.tiles_m * p.nt + (int)rank * x_rows;
-      if (PAIR) tma_load_2d_pair(ring + s * stage_bytes + BM * BK, &x_map, bar, q.b * BK, row);
-      else tma_load_2d(ring + s * stage_bytes + BM * BK, &x_map, bar, q.b * BK, row);
+    auto rows_of = [&](const Walk& at) {
+      const int n = at.tile / p.tiles_m;
+      return Rows{(n * CTAS + (int)rank) * BM, (at.tile - n * p.tiles_m) * p.nt + (int)rank * x_rows};
+    };
+    const int step = p.step;
+    auto load_w = [&](int s, int b, int n, int row) {          // n blocks
+      const uint32_t full = smem_u32(&full_bar[s]), bar = PAIR ? map_to_rank(full, 0) : full, to = ring + s * stage_bytes;
+      if (rank == 0) mbar_arrive_expect_tx(full, n * CTAS * unit_bytes);
+      for (int k = 0; k < n; ++k) {
+        if (PAIR) tma_load_2d_pair(to + k * (BM * BK), &w_map, bar, (b + k) * BK, row);
+        else tma_load_2d(to + k * (BM * BK), &w_map, bar, (b + k) * BK, row);
+      }
+    };
+    auto load_x = [&](int s, int b, int n, int row) {
+      const uint32_t full = smem_u32(&full_bar[s]), bar = PAIR ? map_to_rank(full, 0) : full, to = ring + s * stage_bytes + step * (BM * BK);
+      for (int k = 0; k < n; ++k) {
+        if (PAIR) tma_load_2d_pair(to + k * (x_rows * BK), &x_map, bar, (b + k) * BK, row);
+        else tma_load_2d(to + k * (x_rows * BK), &x_map, bar, (b + k) * BK, row);
+      }
     };
     // the first stages' weights before the wait for the kernel that makes the codes
-    const int early = min(stages, q.n);
     Walk ahead = q;
-    for (; ahead.i < early; ahead.advance(1))
-      if (leader) load_w(ahead.i, ahead);
+    for (int i = 0; i < stages && ahead.more(); ++i) {
+      const int n = min(step - (ahead.b & (step - 1)), ahead.left()), row = rows_of(ahead).w;
+      if (leader) load_w(i, ahead.b, n, row);
+      ahead.advance(n);
+    }
     __syncwarp();
     gb::pdl_wait();
-    for (; q.i < early; q.advance(1))
-      if (leader) load_x(q.i, q);
+    for (int i = 0; i < stages && q.more(); ++i) {
+      const int n = min(step - (q.b & (step - 1)), q.left()), row = rows_of(q).x;
+      if (leader) load_x(i, q.b, n, row);
+      q.advance(n);
+    }
     __syncwarp();
     int s = 0, par = 0;
-    for (; q.more() && go; q.advance(1)) {
-      if (!(go = mbar_wait_warp(smem_u32(&empty_bar[s]), par, aborted, ran_out))) {
-        if (ran_out) gb_err::report(ERR_WAIT_EMPTY), *aborted = 1;
-        break;
+    while (q.more() && go) {
+      const Rows row = rows_of(q);
+      const int all = q.left(), b_end = q.b + all;
+      for (int b = q.b; b < b_end;) {
+        const int n = min(step - (b & (step - 1)), b_end - b);
+        if (!(go = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty_bar[s]), par)))) {
+          gb_err::report(ERR_WAIT_EMPTY), *aborted = 1;
+          break;
+        }
+        if (leader) load_w(s, b, n, row.w), load_x(s, b, n, row.x);
+        if (++s == stages) s = 0, par ^= 1;
+        b += n;
       }
-      if (leader) load_w(s, q), load_x(s, q);
-      __syncwarp();
-      if (++s == stages) s = 0, par ^= 1;
+      q.advance(all);
     }
+    __syncwarp();
     if (leader && *aborted && q.n > 0) {
       // wind down: the copies in flight need microseconds to land; two milliseconds before the shared memory is given up
       const unsigned long long t0 = globaltimer_ns();
@@ -232,84 +257,96 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
     if (rank == 0) {
       // -------------------------------------------------------------- the products' issuer
       const uint32_t idesc0 = instr_desc_mxf8(CTAS * BM, p.nt, 0);
-      const uint64_t da0 = smem_desc_sw128(ring), db0 = smem_desc_sw128(ring + BM * BK), ds0 = smem_desc_rows16(sf_at);
-      const bool leader = elect_one();
-      bool go = true, ran_out;
-      int s = 0, par = 0, sf = 0, sf_par = 0, t = 0;         // t: tiles (or parts) begun
-      for (; q.more(); q.advance(1)) {
-        const int as = t & 1;
-        const bool begins = q.begins(), tile_ends = q.left() == 1;
-        if (begins) {                      // a tile begins: both epilogue groups have read this accumulator
-          if (!(go = mbar_wait_warp(smem_u32(&acc_empty[as]), ((t >> 1) & 1) ^ 1, aborted, ran_out))) {
-            if (ran_out) gb_err::report(ERR_WAIT_ACCUM), *aborted = 1;
-            break;
+      const uint64_t da0 = smem_desc_sw128(ring), db0 = smem_desc_sw128(ring + p.step * (BM * BK)), ds0 = smem_desc_rows16(sf_at);
+      const uint32_t stage_step = stage_bytes >> 4, x_step = (uint32_t)(x_rows * BK) >> 4;
+      const int step = p.step;
+      const bool leader = elect_one(), wide = p.nt > 128;
+      int s = 0, par = 0, sf = 0, sf_par = 0, failed = 0;
+      uint32_t set = ACC_STRIDE, at = 0;          // the set of scales; the stage, in units of the descriptors
+      for (int t = 0; q.more() && !failed; ++t) {      // tiles, or parts of them
+        const int as = t & 1, n = q.left(), b_end = q.b + n;
+        const uint32_t acc = tmem + as * ACC_STRIDE;
+        if (!mbar_wait(smem_u32(&acc_empty[as]), ((t >> 1) & 1) ^ 1)) failed = ERR_WAIT_ACCUM;        // both epilogue groups have read it
+        for (int b = q.b; b < b_end && !failed;) {
+          const int blocks = min(step - (b & (step - 1)), b_end - b);
+          if (b == q.b || (b & 3) == 0) {    // the scales of up to four blocks
+            if (!mbar_wait(smem_u32(&sf_full[sf]), sf_par)) failed = ERR_WAIT_FULL;
+            tc_fence_after_sync();
+            set ^= ACC_STRIDE;
+            if (leader && !failed) {
+              const uint64_t ds = ds0 + (uint64_t)(sf * (SF_BYTES >> 4));
+              copy_scales<PAIR>(tmem + set + SFA_COL, ds);
+              copy_scales<PAIR>(tmem + set + SFB_COL, ds + (512 >> 4));
+              if (wide) copy_scales<PAIR>(tmem + set + SFB_COL + 4, ds + (1024 >> 4));
+              if (PAIR) mma_commit_pair(smem_u32(&sf_empty[sf]), 3);
+              else mma_commit(smem_u32(&sf_empty[sf]));
+            }
+            if (++sf == SF_STAGES) sf = 0, sf_par ^= 1;
           }
-        }
-        if (begins || (q.b & 3) == 0) {    // the scales of up to four blocks
-          if (!(go = mbar_wait_warp(smem_u32(&sf_full[sf]), sf_par, aborted, ran_out))) {
-            if (ran_out) gb_err::report(ERR_WAIT_FULL), *aborted = 1;
-            break;
-          }
+          if (!mbar_wait(smem_u32(&full_bar[s]), par)) failed = ERR_WAIT_FULL;
           tc_fence_after_sync();
-          if (leader) {
-            const uint64_t ds = ds0 + (uint64_t)(sf * (SF_BYTES >> 4));
-            copy_scales<PAIR>(tmem + SFA_COL, ds);
-            copy_scales<PAIR>(tmem + SFB_COL, ds + (512 >> 4));
-            if (p.nt > 128) copy_scales<PAIR>(tmem + SFB_COL + 4, ds + (1024 >> 4));
-            if (PAIR) mma_commit_pair(smem_u32(&sf_empty[sf]), 3);
-            else mma_commit(smem_u32(&sf_empty[sf]));
-          }
-          __syncwarp();
-          if (++sf == SF_STAGES) sf = 0, sf_par ^= 1;
-        }
-        if (!(go = mbar_wait_warp(smem_u32(&full_bar[s]), par, aborted, ran_out))) {
-          if (ran_out) gb_err::report(ERR_WAIT_FULL), *aborted = 1;
-          break;
-        }
-        tc_fence_after_sync();
-        if (leader) {
-          const uint64_t da = da0 + (uint64_t)(s * (stage_bytes >> 4)), db = db0 + (uint64_t)(s * (stage_bytes >> 4));
-          const uint32_t id = (uint32_t)(q.b & 3), idesc = idesc0 | (id << 4) | (id << 29);
+          if (leader && !failed) {
+            uint64_t da = da0 + at, db = db0 + at;
+            for (int i = 0; i < blocks; ++i, da += (BM * BK) >> 4, db += x_step) {
+              const uint32_t id = (uint32_t)((b + i) & 3), idesc = idesc0 | (id << 4) | (id << 29);
 #pragma unroll
-          for (int k = 0; k < BK / 32; ++k)
-            mma_mxf8<PAIR>(tmem + as * ACC_STRIDE, da + 2 * k, db + 2 * k, idesc, tmem + SFA_COL, tmem + SFB_COL, !begins || k > 0);
-          if (PAIR) mma_commit_pair(smem_u32(&empty_bar[s]), 3);
-          else mma_commit(smem_u32(&empty_bar[s]));
-          if (tile_ends) {
-            if (PAIR) mma_commit_pair(smem_u32(&acc_full[as]), 3);
-            else mma_commit(smem_u32(&acc_full[as]));
+              for (int k = 0; k < BK / 32; ++k)
+                mma_mxf8<PAIR>(acc, da + 2 * k, db + 2 * k, idesc, tmem + set + SFA_COL, tmem + set + SFB_COL, b + i > q.b || k > 0);
+            }
+            if (PAIR) mma_commit_pair(smem_u32(&empty_bar[s]), 3);
+            else mma_commit(smem_u32(&empty_bar[s]));
           }
+          at += stage_step;
+          if (++s == stages) s = 0, par ^= 1, at = 0;
+          b += blocks;
+        }
+        if (leader && !failed) {
+          if (PAIR) mma_commit_pair(smem_u32(&acc_full[as]), 3);
+          else mma_commit(smem_u32(&acc_full[as]));
         }
         __syncwarp();
-        if (tile_ends) ++t;
-        if (++s == stages) s = 0, par ^= 1;
+        q.advance(n);
+      }
+      if (failed) {
+        gb_err::report(failed);
+        *aborted = 1;
       }
     }
-  } else if (warp == 2) {
+  } else if (warp == 2 || warp == 3) {
     // ---------------------------------------------------------------- scales
-    bool go = true, ran_out;
-    int sf = 0, sf_par = 1;
+    // Two warps, every second four blocks each. The next ones are asked for once the current ones have been handed over: the fence in front of
+    // that waits for loads under way. (One warp that asked for them before took 2,200 cycles for four blocks, more than their products.)
+    bool ran_out;
     gb::pdl_wait();          // the tokens' scales
-    while (q.more()) {
-      const int g = q.b >> 2, m0 = q.tile % p.tiles_m * p.nt, nb = q.tile / p.tiles_m * CTAS + (int)rank;
-      // this lane's tokens lane, 32 + lane, ...; lanes 0 to 3: the weights' blocks
-      uint32_t x[8];
+    uint32_t x[8];           // this lane's tokens lane, 32 + lane, ...
+    float w = 0.f;           // lanes 0 to 3: the weights' blocks
+    bool there = false;
+    auto ask = [&](const Walk& at) {
+      const int n = at.tile / p.tiles_m, m0 = (at.tile - n * p.tiles_m) * p.nt, nb = n * CTAS + (int)rank, g = at.b >> 2, wb = 4 * g + lane;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int n = j * 32 + lane;
-        x[j] = n < p.nt && m0 + n < p.M ? p.xs[(size_t)g * p.M + m0 + n] : 0u;
+        const int c = j * 32 + lane;
+        x[j] = c < p.nt && m0 + c < p.M ? p.xs[(size_t)g * p.M + m0 + c] : 0u;
       }
-      const int wb = 4 * g + lane;
-      uint32_t w = lane < 4 && wb < p.blocks && nb * BM < p.N ? scale_byte(p.ws[(size_t)nb * p.blocks + wb]) << (8 * lane) : 0u;
-      w |= __shfl_xor_sync(0xffffffffu, w, 1);
-      w |= __shfl_xor_sync(0xffffffffu, w, 2);
-      w = __shfl_sync(0xffffffffu, w, 0);
-      if (!(go = mbar_wait_warp(smem_u32(&sf_empty[sf]), sf_par, aborted, ran_out))) {
+      there = lane < 4 && wb < p.blocks && nb * BM < p.N;
+      w = there ? p.ws[(size_t)nb * p.blocks + wb] : 0.f;
+    };
+    auto next = [&]() { q.advance(min(4 - (q.b & 3), q.left())); };
+    int turn = 0;            // fours so far
+    if (warp == 3 && q.more()) next(), ++turn;
+    if (q.more()) ask(q);
+    while (q.more()) {
+      const int sf = turn % SF_STAGES;
+      uint32_t put_w = there ? scale_byte(w) << (8 * lane) : 0u;
+      put_w |= __shfl_xor_sync(0xffffffffu, put_w, 1);
+      put_w |= __shfl_xor_sync(0xffffffffu, put_w, 2);
+      put_w = __shfl_sync(0xffffffffu, put_w, 0);
+      if (!mbar_wait_warp(smem_u32(&sf_empty[sf]), (turn / SF_STAGES & 1) ^ 1, aborted, ran_out)) {
         if (ran_out) gb_err::report(ERR_WAIT_EMPTY), *aborted = 1;
         break;
       }
       uint4* to = reinterpret_cast<uint4*>(smem_raw + (sf_at - smem_u32(smem_raw)) + sf * SF_BYTES) + lane;
-      to[0] = make_uint4(w, w, w, w);
+      to[0] = make_uint4(put_w, put_w, put_w, put_w);
       to[32] = make_uint4(x[0], x[1], x[2], x[3]);
       to[64] = make_uint4(x[4], x[5], x[6], x[7]);
       fence_proxy_async();            // the tensor core reads them through the async proxy
@@ -318,8 +355,10 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
         if (rank == 0) mbar_arrive(smem_u32(&sf_full[sf]));
         else mbar_arrive_cluster(map_to_rank(smem_u32(&sf_full[sf]), 0));
       }
-      if (++sf == SF_STAGES) sf = 0, sf_par ^= 1;
-      q.advance(min(4 - (q.b & 3), q.left()));
+      next();
+      if (q.more()) next();
+      turn += 2;
+      if (q.more()) ask(q);
     }
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- results
@@ -475,42 +514,61 @@ int tensor_map(const void* ptr, long long rows, long long cols, long long pitch,
 
 struct Plan {
   bool pair;
-  int nt, stages, workers, rounds, share;
+  int nt, stages, step, workers, rounds, share;
   int tiles_m, tiles_n;
   long long units;          // of the tiles behind the rounds
 };
 
-Plan make_plan(int M, int N, int K) {
+// What a product of this shape would take, in microseconds, with `tiles` tiles of tokens, in pairs or not: the plan and its time, from what
+// was measured here. An SM takes in 115 KB a microsecond from L2, all together 11 MB, and 6.4 MB from memory; a step of a unit takes the issuing warp
+// 0.26 us (two units to a stage: 0.15 each), products of 256 tokens 0.27; a part of a tile costs its bytes once out and once in, and
+// 1.2 us each way; a pair of CTAs starts and ends 1.5 us later. The results of a tile's end overlap the next tile's products.
+Plan plan_of(int M, int N, int K, int tiles, bool pair, double* us_out) {
   Plan q;
-  q.pair = M > 512;
-  const int tiles = (M + MAX_NT - 1) / MAX_NT;
+  q.pair = pair;
   q.nt = ((M + tiles - 1) / tiles + 15) / 16 * 16;
   q.tiles_m = (M + q.nt - 1) / q.nt;
-  const int ctas = q.pair ? 2 : 1, blocks = (K + BK - 1) / BK;
+  const int ctas = pair ? 2 : 1, blocks = (K + BK - 1) / BK;
   q.tiles_n = (N + BM * ctas - 1) / (BM * ctas);
   const long long tiles_all = (long long)q.tiles_m * q.tiles_n, units = tiles_all * blocks;
-  const int stage = (BM + q.nt / ctas) * BK;
-  const int most = (SMEM_LIMIT - 1024 - STATIC_BYTES - SF_STAGES * SF_BYTES) / stage;
-  q.stages = most < MAX_STAGES ? most : MAX_STAGES;
+  const int unit = (BM + q.nt / ctas) * BK, room_bytes = SMEM_LIMIT - 1024 - STATIC_BYTES - SF_STAGES * SF_BYTES;
+  q.step = room_bytes / (2 * unit) >= 4 ? 2 : 1;           // two units to a stage where four such stages fit
+  q.stages = room_bytes / (q.step * unit) < MAX_STAGES ? room_bytes / (q.step * unit) : MAX_STAGES;
   const int room = tc_host::sm_count() / ctas;
   q.workers = (int)(units < room ? units : room);
   q.rounds = (int)(tiles_all / q.workers);
-  // The tiles that are left, each among c workers: c from a model of what they take. A worker takes in about 67 KB a microsecond from L2, all
-  // together 6.4 GB a millisecond from memory; a part of a tile costs its bytes once out and once in, and about 0.7 us each way.
+  const auto unit_us = [&](double active) {
+    const double fetch = fmax(unit / 115e3, active * ctas * unit / 11e6), memory = active * ctas * BM * BK / 6.4e6 / q.tiles_m;
+    return fmax(fmax(fetch, memory), fmax(q.step == 2 ? 0.15 : 0.26, 0.27 * q.nt / 256));
+  };
+  const double rounds_us = (double)q.rounds * blocks * unit_us(q.workers) + (pair ? 1.5 : 0.0);
+  // the tiles that are left, each among c workers
   const long long rest = tiles_all - (long long)q.rounds * q.workers;
   q.units = rest * blocks;
   q.share = 0;
-  double best = 1e30;
+  double best = rest > 0 ? 1e30 : 0;
   for (int c = 1; rest > 0 && c <= 16; ++c) {
-    const long long most = rest * c < q.workers ? rest * c : q.workers, share = most < q.units ? most : q.units;
+    const long long all = rest * c < q.workers ? rest * c : q.workers, share = all < q.units ? all : q.units;
     const double units_each = (double)((q.units + share - 1) / share);
-    const double unit = fmax(stage / 67e3, (double)share * ctas * BM * BK / 6.4e6);
     const double parts = share > rest ? (rest * c <= q.workers ? c : (double)share / rest + 1) + 1 : 0;
-    const double us = units_each * unit + parts * (0.7 + (double)(M < q.nt ? M : q.nt) * BM * 4 / 67e3);
+    const double us = units_each * unit_us((double)share) + parts * (1.2 + (double)(M < q.nt ? M : q.nt) * BM * 4 / 67e3);
     if (us < best) best = us, q.share = (int)share;
-    if (most == q.workers) break;
+    if (all == q.workers) break;
   }
+  *us_out = rounds_us + best;
   return q;
+}
+
+Plan make_plan(int M, int N, int K) {
+  const int least = (M + MAX_NT - 1) / MAX_NT;
+  double us, best = 1e30;
+  Plan plan{};
+  for (int pair = 0; pair < 2; ++pair)
+    for (int tiles = least; tiles <= least + 3 && tiles <= (M + 15) / 16; ++tiles) {
+      const Plan q = plan_of(M, N, K, tiles, pair != 0, &us);
+      if (us < best) best = us, plan = q;
+    }
+  return plan;
 }
 
 long long code_bytes(int M, int K) { return ((long long)M * ((K + 15) / 16 * 16) + 255) / 256 * 256; }
@@ -528,7 +586,7 @@ int launch(const Plan& q, const CUtensorMap& wm, const CUtensorMap& xm, const Ar
     configured.done();
   }
   const int ctas = PAIR ? 2 : 1;
-  const size_t smem = (size_t)q.stages * (BM + q.nt / ctas) * BK + SF_STAGES * SF_BYTES + 1024;
+  const size_t smem = (size_t)q.stages * q.step * (BM + q.nt / ctas) * BK + SF_STAGES * SF_BYTES + 1024;
   return gb::check_pdl_launch(gb::launch_pdl(kernel, dim3((unsigned)(q.workers * ctas)), dim3(THREADS), smem, stream, dim3(ctas), wm, xm, a),
                               "gemm_f8");
 }
@@ -575,7 +633,7 @@ GB_EXPORT int gb_f8_linear(const void* a, int a_tag, long long lda, const void* 
   rc = tensor_map(codes, M, pitch, pitch, q.nt / ctas, &xm);
   if (rc) return rc;
   const Args args{(const uint32_t*)xs, (const float*)ws, out, (float*)(xs + scale_bytes(M, K)), (int*)counters, M, N, (K + BK - 1) / BK, q.nt,
-                  q.tiles_m, q.stages, q.workers, q.rounds, q.units, q.share, accumulate ? alpha : 1.0f};
+                  q.tiles_m, q.stages, q.step, q.workers, q.rounds, q.units, q.share, accumulate ? alpha : 1.0f};
   return q.pair ? launch_out<true>(q, wm, xm, args, out_tag, accumulate != 0, st) : launch_out<false>(q, wm, xm, args, out_tag, accumulate != 0, st);
 }
 
