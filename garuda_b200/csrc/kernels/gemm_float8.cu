@@ -56,7 +56,7 @@ struct Args {
   int* counters;            // [tiles * CTAs of a worker], zero between launches
   int M, N, blocks;
   int nt, tiles_m;          // tokens per tile (a multiple of 16), tiles of tokens
-  int stages, step;         // step: units of a stage (1 or 2)
+  int stages;               // of one unit, or (STEP) two
   int workers, rounds;      // rounds: whole tiles for every worker
   long long units;          // those of the tiles behind the rounds,
   int share;                // and the workers that share these
@@ -131,7 +131,7 @@ struct Walk {
   }
 };
 
-template <bool PAIR, typename OT, bool ADD>
+template <bool PAIR, int STEP, typename OT, bool ADD>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const Args p) {
   constexpr int CTAS = PAIR ? 2 : 1;
@@ -144,7 +144,7 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
   const uint32_t rank = PAIR ? cluster_ctarank() : 0;
   const int worker = blockIdx.x / CTAS;
   const int x_rows = p.nt / CTAS;                                  // rows of the tokens' box
-  const uint32_t unit_bytes = (uint32_t)(BM + x_rows) * BK, stage_bytes = unit_bytes * p.step;        // a stage: weights, then tokens
+  const uint32_t unit_bytes = (uint32_t)(BM + x_rows) * BK, stage_bytes = unit_bytes * STEP;        // a stage: weights, then tokens
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const int stages = p.stages;
   const uint32_t sf_at = ring + stages * stage_bytes;              // behind the ring: the scales on their way
@@ -200,18 +200,21 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
       const int n = at.tile / p.tiles_m;
       return Rows{(n * CTAS + (int)rank) * BM, (at.tile - n * p.tiles_m) * p.nt + (int)rank * x_rows};
     };
-    const int step = p.step;
     auto load_w = [&](int s, int b, int n, int row) {          // n blocks
       const uint32_t full = smem_u32(&full_bar[s]), bar = PAIR ? map_to_rank(full, 0) : full, to = ring + s * stage_bytes;
       if (rank == 0) mbar_arrive_expect_tx(full, n * CTAS * unit_bytes);
-      for (int k = 0; k < n; ++k) {
+#pragma unroll
+      for (int k = 0; k < STEP; ++k) {
+        if (k >= n) break;
         if (PAIR) tma_load_2d_pair(to + k * (BM * BK), &w_map, bar, (b + k) * BK, row);
         else tma_load_2d(to + k * (BM * BK), &w_map, bar, (b + k) * BK, row);
       }
     };
     auto load_x = [&](int s, int b, int n, int row) {
-      const uint32_t full = smem_u32(&full_bar[s]), bar = PAIR ? map_to_rank(full, 0) : full, to = ring + s * stage_bytes + step * (BM * BK);
-      for (int k = 0; k < n; ++k) {
+      const uint32_t full = smem_u32(&full_bar[s]), bar = PAIR ? map_to_rank(full, 0) : full, to = ring + s * stage_bytes + STEP * (BM * BK);
+#pragma unroll
+      for (int k = 0; k < STEP; ++k) {
+        if (k >= n) break;
         if (PAIR) tma_load_2d_pair(to + k * (x_rows * BK), &x_map, bar, (b + k) * BK, row);
         else tma_load_2d(to + k * (x_rows * BK), &x_map, bar, (b + k) * BK, row);
       }
@@ -219,14 +222,14 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
     // the first stages' weights before the wait for the kernel that makes the codes
     Walk ahead = q;
     for (int i = 0; i < stages && ahead.more(); ++i) {
-      const int n = min(step - (ahead.b & (step - 1)), ahead.left()), row = rows_of(ahead).w;
+      const int n = min(STEP - (ahead.b & (STEP - 1)), ahead.left()), row = rows_of(ahead).w;
       if (leader) load_w(i, ahead.b, n, row);
       ahead.advance(n);
     }
     __syncwarp();
     gb::pdl_wait();
     for (int i = 0; i < stages && q.more(); ++i) {
-      const int n = min(step - (q.b & (step - 1)), q.left()), row = rows_of(q).x;
+      const int n = min(STEP - (q.b & (STEP - 1)), q.left()), row = rows_of(q).x;
       if (leader) load_x(i, q.b, n, row);
       q.advance(n);
     }
@@ -236,7 +239,7 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
       const Rows row = rows_of(q);
       const int all = q.left(), b_end = q.b + all;
       for (int b = q.b; b < b_end;) {
-        const int n = min(step - (b & (step - 1)), b_end - b);
+        const int n = min(STEP - (b & (STEP - 1)), b_end - b);
         if (!(go = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty_bar[s]), par)))) {
           gb_err::report(ERR_WAIT_EMPTY), *aborted = 1;
           break;
@@ -257,10 +260,9 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
     if (rank == 0) {
       // -------------------------------------------------------------- the products' issuer
       const uint32_t idesc0 = instr_desc_mxf8(CTAS * BM, p.nt, 0);
-      const uint64_t da0 = smem_desc_sw128(ring), db0 = smem_desc_sw128(ring + p.step * (BM * BK)), ds0 = smem_desc_rows16(sf_at);
+      const uint64_t da0 = smem_desc_sw128(ring), db0 = smem_desc_sw128(ring + STEP * (BM * BK)), ds0 = smem_desc_rows16(sf_at);
       const uint32_t stage_step = stage_bytes >> 4, x_step = (uint32_t)(x_rows * BK) >> 4;
-      const int step = p.step;
-      const bool leader = elect_one(), wide = p.nt > 128;
+        const bool leader = elect_one(), wide = p.nt > 128;
       int s = 0, par = 0, sf = 0, sf_par = 0, failed = 0;
       uint32_t set = ACC_STRIDE, at = 0;          // the set of scales; the stage, in units of the descriptors
       for (int t = 0; q.more() && !failed; ++t) {      // tiles, or parts of them
@@ -268,7 +270,7 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
         const uint32_t acc = tmem + as * ACC_STRIDE;
         if (!mbar_wait(smem_u32(&acc_empty[as]), ((t >> 1) & 1) ^ 1)) failed = ERR_WAIT_ACCUM;        // both epilogue groups have read it
         for (int b = q.b; b < b_end && !failed;) {
-          const int blocks = min(step - (b & (step - 1)), b_end - b);
+          const int blocks = min(STEP - (b & (STEP - 1)), b_end - b);
           if (b == q.b || (b & 3) == 0) {    // the scales of up to four blocks
             if (!mbar_wait(smem_u32(&sf_full[sf]), sf_par)) failed = ERR_WAIT_FULL;
             tc_fence_after_sync();
@@ -287,7 +289,9 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
           tc_fence_after_sync();
           if (leader && !failed) {
             uint64_t da = da0 + at, db = db0 + at;
-            for (int i = 0; i < blocks; ++i, da += (BM * BK) >> 4, db += x_step) {
+#pragma unroll
+            for (int i = 0; i < STEP; ++i, da += (BM * BK) >> 4, db += x_step) {
+              if (i >= blocks) break;
               const uint32_t id = (uint32_t)((b + i) & 3), idesc = idesc0 | (id << 4) | (id << 29);
 #pragma unroll
               for (int k = 0; k < BK / 32; ++k)
@@ -576,9 +580,9 @@ long long scale_bytes(int M, int K) { return ((long long)(K + 4 * BK - 1) / (4 *
 long long part_bytes(const Plan& q) { return (long long)(q.share > 0 ? q.share : 1) * 2 * (q.pair ? 2 : 1) * q.nt * BM * 4; }
 long long counter_bytes(const Plan& q) { return ((long long)q.tiles_m * q.tiles_n * (q.pair ? 2 : 1) * 4 + 255) / 256 * 256; }
 
-template <bool PAIR, typename OT, bool ADD>
+template <bool PAIR, int STEP, typename OT, bool ADD>
 int launch(const Plan& q, const CUtensorMap& wm, const CUtensorMap& xm, const Args& a, cudaStream_t stream) {
-  auto kernel = gemm_f8_kernel<PAIR, OT, ADD>;
+  auto kernel = gemm_f8_kernel<PAIR, STEP, OT, ADD>;
   static gb::OncePerDevice configured;
   if (configured.needed()) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT - STATIC_BYTES);
@@ -586,16 +590,16 @@ int launch(const Plan& q, const CUtensorMap& wm, const CUtensorMap& xm, const Ar
     configured.done();
   }
   const int ctas = PAIR ? 2 : 1;
-  const size_t smem = (size_t)q.stages * q.step * (BM + q.nt / ctas) * BK + SF_STAGES * SF_BYTES + 1024;
+  const size_t smem = (size_t)q.stages * STEP * (BM + q.nt / ctas) * BK + SF_STAGES * SF_BYTES + 1024;
   return gb::check_pdl_launch(gb::launch_pdl(kernel, dim3((unsigned)(q.workers * ctas)), dim3(THREADS), smem, stream, dim3(ctas), wm, xm, a),
                               "gemm_f8");
 }
 
-template <bool PAIR>
+template <bool PAIR, int STEP>
 int launch_out(const Plan& q, const CUtensorMap& wm, const CUtensorMap& xm, const Args& a, int out_tag, bool add, cudaStream_t stream) {
-  if (add) return launch<PAIR, float, true>(q, wm, xm, a, stream);
-  if (out_tag == GB_F32) return launch<PAIR, float, false>(q, wm, xm, a, stream);
-  return launch<PAIR, __nv_bfloat16, false>(q, wm, xm, a, stream);
+  if (add) return launch<PAIR, STEP, float, true>(q, wm, xm, a, stream);
+  if (out_tag == GB_F32) return launch<PAIR, STEP, float, false>(q, wm, xm, a, stream);
+  return launch<PAIR, STEP, __nv_bfloat16, false>(q, wm, xm, a, stream);
 }
 
 }  // namespace
@@ -633,8 +637,10 @@ GB_EXPORT int gb_f8_linear(const void* a, int a_tag, long long lda, const void* 
   rc = tensor_map(codes, M, pitch, pitch, q.nt / ctas, &xm);
   if (rc) return rc;
   const Args args{(const uint32_t*)xs, (const float*)ws, out, (float*)(xs + scale_bytes(M, K)), (int*)counters, M, N, (K + BK - 1) / BK, q.nt,
-                  q.tiles_m, q.stages, q.step, q.workers, q.rounds, q.units, q.share, accumulate ? alpha : 1.0f};
-  return q.pair ? launch_out<true>(q, wm, xm, args, out_tag, accumulate != 0, st) : launch_out<false>(q, wm, xm, args, out_tag, accumulate != 0, st);
+                  q.tiles_m, q.stages, q.workers, q.rounds, q.units, q.share, accumulate ? alpha : 1.0f};
+  const bool add = accumulate != 0;
+  if (q.pair) return q.step == 2 ? launch_out<true, 2>(q, wm, xm, args, out_tag, add, st) : launch_out<true, 1>(q, wm, xm, args, out_tag, add, st);
+  return q.step == 2 ? launch_out<false, 2>(q, wm, xm, args, out_tag, add, st) : launch_out<false, 1>(q, wm, xm, args, out_tag, add, st);
 }
 
 GB_EXPORT int gb_f8_gemm_error_check() { return gb_err::fetch_and_clear(); }
