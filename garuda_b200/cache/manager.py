@@ -29,12 +29,18 @@ class CacheConfig:
 
 
 class PagedCache:
-    def __init__(self, model, config: CacheConfig, dtype: torch.dtype, device, allocate: bool = True):
+    def __init__(self, model, config: CacheConfig, dtype: torch.dtype, device, allocate: bool = True, float8: bool = False):
+        """``float8``: the pages hold 8-bit numbers (E4M3) with a 32-bit scale per page and key/value head, ``k_scales`` and
+        ``v_scales`` ``[calls, num_pages, kv_heads]`` of every group; states of fixed size stay as they are."""
         host = load_host_module()
         self.host_module = host
         self.config = config
         self.model = model
         self.dtype, self.device = dtype, torch.device(device)
+        self.float8 = bool(float8)
+        if float8 and any(isinstance(g.need, PagedLatent) for g in model.cache_groups):
+            raise ValueError("pages in 8 bits hold keys and values, not latent rows")
+        page_dtype = torch.float8_e4m3fn if float8 else dtype
         ps = config.page_size
         if config.num_pages is not None:
             pages = int(config.num_pages)
@@ -52,6 +58,8 @@ class PagedCache:
         # device memory
         self.k_pools: List[torch.Tensor] = []
         self.v_pools: List[torch.Tensor] = []
+        self.k_scales: List[torch.Tensor] = []
+        self.v_scales: List[torch.Tensor] = []
         self.call_group: Dict[object, tuple] = {}
         for gi, g in enumerate(self.groups):
             if isinstance(g.need, PagedLatent):
@@ -64,8 +72,11 @@ class PagedCache:
                 shape = (len(g.calls), pages, g.need.kv_heads, ps, g.need.head_dim)
                 v_shape = shape[:-1] + (g.need.value_dim or g.need.head_dim,)
                 if allocate:
-                    self.k_pools.append(torch.zeros(shape, dtype=dtype, device=self.device))
-                    self.v_pools.append(torch.zeros(v_shape, dtype=dtype, device=self.device))
+                    self.k_pools.append(torch.zeros(shape, dtype=page_dtype, device=self.device))
+                    self.v_pools.append(torch.zeros(v_shape, dtype=page_dtype, device=self.device))
+                    if float8:
+                        self.k_scales.append(torch.zeros(shape[:3], dtype=torch.float32, device=self.device))
+                        self.v_scales.append(torch.zeros(shape[:3], dtype=torch.float32, device=self.device))
             for j, call in enumerate(g.calls):
                 self.call_group[call] = (gi, j)
         self.states: Dict[object, torch.Tensor] = {}
@@ -95,6 +106,9 @@ class PagedCache:
         self.manager.release(request)
 
     def bytes_per_position(self) -> int:
+        if self.float8:         # and a page's two scales a head
+            return sum(len(g.calls) * (g.need.kv_heads * (g.need.head_dim + (g.need.value_dim or g.need.head_dim))
+                                       + -(-8 * g.need.kv_heads // self.page_size)) for g in self.groups)
         item = self.dtype.itemsize
         return sum(len(g.calls) * (g.need.width if isinstance(g.need, PagedLatent)
                                    else g.need.kv_heads * (g.need.head_dim + (g.need.value_dim or g.need.head_dim)))
@@ -114,7 +128,9 @@ class PagedCache:
                 gi, j = self.call_group[key]
                 v_pool = self.v_pools[gi]
                 return LayerCache(need=need, k=self.k_pools[gi][j], v=None if v_pool is None else v_pool[j],
-                                  block_table=block_tables[gi], page_size=self.page_size, writes=writes)
+                                  block_table=block_tables[gi], page_size=self.page_size, writes=writes,
+                                  k_scale=self.k_scales[gi][j] if self.float8 else None,
+                                  v_scale=self.v_scales[gi][j] if self.float8 else None)
             return LayerCache(need=need, state=self.states[key], writes=writes)
 
         for i, call in enumerate(order):

@@ -52,6 +52,7 @@ def parse_size(s) -> int:
 class ModelSection:
     path: str = "./models"        # folder with config.json and model.safetensors
     dtype: str = "bfloat16"       # bfloat16 | float32
+    weight_dtype: str = ""        # "float8_e4m3": the layers' matrices in 8 bits; "": as dtype
     context: int = 4096           # context window; a model caps it at its own (server/mod.rs:419)
     sliding_window: int = 0       # attention window; 0 attends to the whole context
     seed: int = 0                 # random-weights mode: seed of `garuda init`
@@ -65,6 +66,7 @@ class MemorySection:
     kv_cache: str = "0"           # bytes for the paged cache, e.g. "8GB"; "0": size it from kv_tokens
     kv_tokens: int = 0            # positions the cache holds; 0: max_concurrent * context
     page_size: int = 32           # positions per page (garuda/src/llama/mod.rs:483)
+    cache_dtype: str = ""         # "float8_e4m3": keys and values in 8 bits, a scale per page and head; "": as model.dtype
 
 
 @dataclass
@@ -158,6 +160,12 @@ class EngineConfig:
             raise ConfigError("gpu = false, but this engine has no CPU path. Set gpu = true.")
         if self.model.dtype not in ("bfloat16", "float32"):
             raise ConfigError(f"model.dtype must be 'bfloat16' or 'float32', got '{self.model.dtype}'")
+        if self.model.weight_dtype not in ("", "float8_e4m3"):
+            raise ConfigError(f"model.weight_dtype must be 'float8_e4m3' or empty, got '{self.model.weight_dtype}'")
+        if self.model.weight_dtype and self.model.dtype != "bfloat16":
+            raise ConfigError("model.weight_dtype = 'float8_e4m3' goes with model.dtype = 'bfloat16'")
+        if self.memory.cache_dtype not in ("", "float8_e4m3"):
+            raise ConfigError(f"memory.cache_dtype must be 'float8_e4m3' or empty, got '{self.memory.cache_dtype}'")
         if self.model.context < 2:
             raise ConfigError("model.context must be at least 2")
         if self.model.sliding_window < 0:

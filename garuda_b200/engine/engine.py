@@ -54,14 +54,28 @@ class Engine:
                  queue_capacity: int = 256, max_batch_tokens: int = 2048, prefill_chunk: int = 2048,
                  cuda_graphs: bool = True, lookahead: bool = True, device: int = 0, ignore_eos: bool = False,
                  eos_token_id: Union[None, int, Sequence[int]] = None,
-                 request_timeout: Optional[float] = None, paced_prefill: bool = False, ops=None):
+                 request_timeout: Optional[float] = None, paced_prefill: bool = False, ops=None,
+                 weight_dtype: Optional[str] = None, cache_dtype: Optional[str] = None):
         """``request_timeout``: seconds from its submission after which a request, waiting or
         running, ends with the error "timeout" (garuda/src/scheduler/mod.rs:520); None: no limit.
         ``paced_prefill``: while something is decoding, prompts go in by portions that cost about
-        one decode step, sized from the measured times of the steps (garuda/src/scheduler/mod.rs:305-370)."""
+        one decode step, sized from the measured times of the steps (garuda/src/scheduler/mod.rs:305-370).
+        ``weight_dtype="float8_e4m3"``: the layers' matrices are held in 8 bits, with a scale per 128 x 128, and multiplied in 8 bits (tokens
+        are rounded with a scale per 128 channels); the embedding, the head and the norms stay as they are. ``cache_dtype=
+        "float8_e4m3"``: keys and values are, with a scale per page and head. For models whose layers know them (the Llama decoder)."""
         if dtype not in _DTYPES:
             raise ConfigError(f"dtype must be 'bfloat16' or 'float32', got {dtype!r}")
         self.dtype = _DTYPES[dtype]
+        for name, value in (("weight_dtype", weight_dtype), ("cache_dtype", cache_dtype)):
+            if value not in (None, "", "float8_e4m3"):
+                raise ConfigError(f"{name} must be 'float8_e4m3' or absent, got {value!r}")
+        weight_dtype, cache_dtype = weight_dtype or None, cache_dtype or None
+        if weight_dtype and self.dtype != torch.bfloat16:
+            raise ConfigError("weights in 8 bits go with dtype 'bfloat16'")
+        if ops is not None and weight_dtype != getattr(ops, "weight_dtype", None):
+            raise ConfigError(f"the kernel set that was given holds weights as {getattr(ops, 'weight_dtype', None)!r}, not as {weight_dtype!r}")
+        if ops is not None and cache_dtype and not hasattr(ops, "paged_attention_float8"):
+            raise ConfigError("the kernel set that was given has no attention over a cache in 8 bits")
         self.model_dir = model_dir
         if request_timeout is not None and not request_timeout > 0:
             raise ConfigError(f"request_timeout must be positive, got {request_timeout!r}")
@@ -74,11 +88,12 @@ class Engine:
             self.device = torch.device(f"cuda:{device}")
             torch.cuda.set_device(self.device)
             # the 32-bit path never touches a tensor core: true 32-bit multiply-adds throughout
-            ops = CudaOps(self.device, tensor_cores=self.dtype == torch.bfloat16)
+            ops = CudaOps(self.device, tensor_cores=self.dtype == torch.bfloat16, weight_dtype=weight_dtype)
         else:
             self.device = torch.device(getattr(ops, "device", "cpu"))
         self.ops = ops
         self.config, self.model = build_model(config_dict)
+        self._check_float8(bool(weight_dtype), bool(cache_dtype))
         load_weights(self.model, model_dir, ops, self.dtype, self.device)
 
         spec = self.model.spec
@@ -88,7 +103,7 @@ class Engine:
         probe = PagedCache(self.model, CacheConfig(page_size=page_size, num_pages=0,
                                                    max_requests=max_concurrent,
                                                    max_positions=self.max_context),
-                           self.dtype, self.device, allocate=False)
+                           self.dtype, self.device, allocate=False, float8=bool(cache_dtype))
         if kv_tokens:
             tokens = int(kv_tokens)
         elif kv_cache_bytes:
@@ -100,7 +115,7 @@ class Engine:
         self.cache = PagedCache(self.model, CacheConfig(page_size=page_size, num_pages=pages,
                                                         max_requests=max_concurrent,
                                                         max_positions=self.max_context),
-                                self.dtype, self.device)
+                                self.dtype, self.device, float8=bool(cache_dtype))
         self.runner = StepRunner(self.model, self.cache, ops, self.dtype, self.device)
         self.sampler = Sampler(ops, self.device)
         host = load_host_module()
@@ -132,6 +147,16 @@ class Engine:
             from .graph import DecodeGraphs
             self.runner.graphs = DecodeGraphs(self.runner, max_concurrent)
 
+    def _check_float8(self, weights: bool, cache: bool) -> None:
+        """Refuses 8 bits for a model with a part that does not know them."""
+        for block in self.model.blocks:
+            for part, _ in block.parts():
+                matrices = any(ts.role == "matrix" for ts in part.tensors().values())
+                if weights and matrices and not part.holds_matrices:
+                    raise ConfigError(f"weight_dtype: {type(part).__name__} does not hold its matrices in 8 bits")
+            if cache and block.mixer.cache_need() is not None and not block.mixer.takes_float8_cache:
+                raise ConfigError(f"cache_dtype: {type(block.mixer).__name__} does not keep its cache in 8 bits")
+
     @classmethod
     def from_config(cls, cfg: EngineConfig, **overrides) -> "Engine":
         kv_bytes = parse_size(cfg.memory.kv_cache)
@@ -143,6 +168,7 @@ class Engine:
             prefill_chunk=cfg.runtime.prefill_chunk, cuda_graphs=cfg.runtime.cuda_graphs,
             lookahead=cfg.runtime.lookahead, paced_prefill=cfg.runtime.paced_prefill,
             request_timeout=cfg.server.request_timeout_secs,
+            weight_dtype=cfg.model.weight_dtype or None, cache_dtype=cfg.memory.cache_dtype or None,
             device=cfg.runtime.device)
         kwargs.update(overrides)
         return cls(cfg.model.path, **kwargs)

@@ -78,6 +78,8 @@ def main(argv=None) -> int:
                     help="most tokens live requests hold at any time (each rounded up to 64)")
     ap.add_argument("--page-size", type=int, default=32)
     ap.add_argument("--max-requests", type=int, default=4)
+    ap.add_argument("--weight-dtype", choices=["float8_e4m3"], help="hold the layers' matrices in 8 bits")
+    ap.add_argument("--cache-dtype", choices=["float8_e4m3"], help="keep keys and values in 8 bits")
     ap.add_argument("--no-graphs", action="store_true", help="launch decode steps kernel by kernel")
     ap.add_argument("--plugin", action="append", default=[], metavar="MODULE",
                     help="import this module first (it registers an architecture or parts of its own)")
@@ -91,7 +93,8 @@ def main(argv=None) -> int:
     # with a shorter limit of its own keeps it)
     pool = max((args.max_tokens + args.page_size - 1) // args.page_size * args.page_size, 2 * args.page_size)
     engine = Engine(args.model, dtype=args.dtype, page_size=args.page_size, kv_tokens=args.max_tokens, context=pool,
-                    max_concurrent=args.max_requests, cuda_graphs=not args.no_graphs)
+                    max_concurrent=args.max_requests, cuda_graphs=not args.no_graphs, weight_dtype=args.weight_dtype,
+                    cache_dtype=args.cache_dtype)
     replay(engine, sys.stdin, args.out, report=_say_done)
     return 0
 

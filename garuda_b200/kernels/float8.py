@@ -6,6 +6,7 @@ page of one key/value head of the cache.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from ctypes import c_void_p, c_int, c_float, c_longlong
 from typing import NamedTuple
@@ -33,6 +34,14 @@ class Float8Weight(NamedTuple):
     def dtype(self):
         return self.values.dtype
 
+    @property
+    def is_cuda(self):
+        return self.values.is_cuda and self.scales.is_cuda
+
+    def first_rows(self, n: int) -> "Float8Weight":
+        """The first ``n`` rows, as a view."""
+        return Float8Weight(self.values[:n], self.scales[:(n + BLOCK - 1) // BLOCK])
+
 
 _FLOAT8_SIGNATURES = {
     "gb_f8_quantize_weight": [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_longlong, c_void_p, c_void_p],
@@ -55,6 +64,24 @@ class Float8Ops:
     """What ``CudaOps`` has of 8 bits. Everything is launched on torch's current stream; scratch memory belongs to the
     stream (or to ``ws``, a step's workspace), and results do not depend on the order in which blocks finish."""
 
+    #: the workspace of the step that is running (``scratch_from``): what a captured graph reads must be its own
+    step_ws = None
+    #: ``"float8_e4m3"``: ``hold`` keeps matrices in 8 bits
+    weight_dtype = None
+
+    @contextlib.contextmanager
+    def scratch_from(self, ws):
+        """Within the block, 8-bit calls that are given no workspace take their scratch memory from this one."""
+        outer, self.step_ws = self.step_ws, ws
+        try:
+            yield
+        finally:
+            self.step_ws = outer
+
+    def hold(self, w: torch.Tensor):
+        """A weight matrix as this kernel set keeps it: in 8 bits if it was asked to, else as it is. ``linear`` takes both."""
+        return self.float8_weight(w) if self.weight_dtype == "float8_e4m3" else w.contiguous()
+
     @property
     def float8_lib(self):
         """The library of the 8-bit kernels, compiled and loaded when a caller first needs it."""
@@ -76,7 +103,9 @@ class Float8Ops:
         return self._float8
 
     def _scratch8(self, name, nbytes, ws, stream, zero=False):
-        """Scratch bytes of this name: the step's, or one per stream."""
+        """Scratch bytes of this name: the call's workspace, the running step's, or one per stream."""
+        if ws is None:
+            ws = self.step_ws
         if ws is None:
             ws = self._float8_scratch.get(stream)
             if ws is None:
@@ -84,12 +113,18 @@ class Float8Ops:
                 ws = self._float8_scratch[stream] = Workspace(self.device)
         return ws.get(name, (nbytes,), torch.uint8, zero=zero)
 
+    def float8_error_code(self) -> int:
+        """The code of a wait that an 8-bit kernel gave up since the last check, or 0; synchronises and clears."""
+        if self._float8 is None:
+            return 0
+        L = self._float8
+        codes = [L.gb_f8_gemm_error_check(), L.gb_f8_attention_decode_error_check(), L.gb_f8_attention_tile_error_check()]
+        return next((c for c in codes if c), 0)
+
     def check_float8_errors(self) -> None:
         """Synchronises, and raises if an 8-bit kernel gave up on a wait since the last check."""
         seen, self.error_word[0] = int(self.error_word[0]), 0
-        L = self.float8_lib
-        codes = [L.gb_f8_gemm_error_check(), L.gb_f8_attention_decode_error_check(), L.gb_f8_attention_tile_error_check(), seen]
-        code = next((c for c in codes if c), 0)
+        code = self.float8_error_code() or seen
         _need(not code, f"an 8-bit kernel gave up waiting: code {code}")
 
     # ------------------------------------------------------------------ matrix products

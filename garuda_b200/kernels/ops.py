@@ -18,7 +18,7 @@ import torch
 
 from ..csrc.build import load_kernel_lib
 from .checks import GB_BF16, GB_F32, KernelError, _need, _ptr, _tag
-from .float8 import Float8Ops
+from .float8 import Float8Ops, Float8Weight
 
 _ERROR_WORD = None
 
@@ -68,11 +68,15 @@ class CudaOps(Float8Ops):
 
     name = "cuda"
 
-    def __init__(self, device="cuda:0", tensor_cores: bool = True):
+    def __init__(self, device="cuda:0", tensor_cores: bool = True, weight_dtype=None):
+        """``weight_dtype="float8_e4m3"``: the matrices that parts give to ``hold`` and ``pack_gate_up`` are kept in 8 bits."""
+        _need(weight_dtype in (None, "float8_e4m3"), f"weights are held as they are or as 'float8_e4m3', not as {weight_dtype!r}")
+        _need(weight_dtype is None or tensor_cores, "weights in 8 bits are multiplied on the tensor cores")
         if not torch.cuda.is_available():
             raise KernelError("garuda_b200 needs a CUDA device: there is no CPU path")
         self.device = torch.device(device)
         self._device_index = self.device.index if self.device.index is not None else torch.cuda.current_device()
+        self.weight_dtype = weight_dtype
         self.core = load_kernel_lib("garuda_core")
         self._mixers = None
         self._state = None
@@ -420,6 +424,9 @@ class CudaOps(Float8Ops):
         the kernel can, it folds that norm's first half into this product and returns a
         ``PendingNorm`` to hand to ``qkv_rope_append`` or ``linear_swiglu`` in place of the
         normed tensor; else it returns None and the norm runs as usual."""
+        if isinstance(w, Float8Weight):
+            self.linear_float8(a, w, out, accumulate, alpha)
+            return None
         self._on_device(a, w, out)
         _need(a.dim() == 2 and w.dim() == 2 and out.dim() == 2, "linear: operands must be matrices")
         M, K = a.shape
@@ -464,8 +471,10 @@ class CudaOps(Float8Ops):
         up rows packed in groups of 64 (rows ``[128 g, 128 g + 64)`` are gate rows
         ``64 g ..``, the next 64 the matching up rows, zero rows padding the last
         group), so that a 128-row tile holds both values of 64 features. Without
-        them: gate rows, then up rows."""
+        them, and with weights in 8 bits: gate rows, then up rows."""
         F, K = gate.shape
+        if self.weight_dtype is not None:
+            return self.hold(torch.cat([gate, up], dim=0))
         if self.tc is None or gate.dtype != torch.bfloat16:
             return torch.cat([gate, up], dim=0).contiguous()
         groups = (F + 63) // 64

@@ -82,6 +82,7 @@ class TensorCoreKernels:
             code = lib.gb_latent_attention_error_check() or code
         for lib in self._capped.values():
             code = lib.gb_capped_attention_error_check() or code
+        code = self.ops.float8_error_code() or code
         seen, self.ops.error_word[0] = int(self.ops.error_word[0]), 0
         code = code or seen
         if code:

@@ -172,6 +172,10 @@ class Decoder:
         logits ``[W, vocab]`` for the batch's ``logit_rows`` only: the final norm
         and the head touch no other row (garuda/src/llama/mod.rs:1110-1113)."""
         b, ops, s = ctx.batch, self.ops, self.spec
+        scratch_from = getattr(ops, "scratch_from", None)
+        if scratch_from is not None and ops.step_ws is not ctx.ws:
+            with scratch_from(ctx.ws):
+                return self.forward(ctx, layer_caches)
         if s.streams is not None:
             return self._forward_streams(ctx, layer_caches)
         x = ctx.ws.get("residual", (b.num_tokens, s.width), torch.float32)

@@ -19,7 +19,7 @@ from typing import Optional
 
 import torch
 
-from .base import (FixedState, Mixer, PagedKV, TensorSpec, PartSpec, build_part, register_mixer)
+from .base import (FixedState, Mixer, PagedKV, TensorSpec, PartSpec, build_part, hold_matrix, register_mixer)
 
 
 @register_mixer("paged_attention")
@@ -64,17 +64,38 @@ class PagedAttention(Mixer):
         super().load(tensors, ops, dtype)
         self.position.load({local: tensors["position." + local] for local in self.position.tensors()}, ops, dtype)
         if self.reads_shared_cache:
-            self.w_qkv = tensors["q_proj.weight"].contiguous()
+            self.w_qkv = hold_matrix(ops, tensors["q_proj.weight"])
         else:
-            self.w_qkv = torch.cat([tensors["q_proj.weight"], tensors["k_proj.weight"],
-                                    tensors["v_proj.weight"]], dim=0).contiguous()
-        self.w_o = tensors["o_proj.weight"].contiguous()
+            self.w_qkv = hold_matrix(ops, torch.cat([tensors["q_proj.weight"], tensors["k_proj.weight"],
+                                                     tensors["v_proj.weight"]], dim=0))
+        self.w_o = hold_matrix(ops, tensors["o_proj.weight"])
 
     # ---- one step ------------------------------------------------------------
     # ``h`` may be a norm that is half done (``CudaOps.qkv_rope_append`` takes it), and the output
     # product may fold in the first half of the norm that follows (``emit_norm``)
     takes_pending_norm = True
     emits_norm = True
+    holds_matrices = True
+    takes_float8_cache = True
+
+    def _write_float8(self, ctx, h, w_qkv, q, cache, writes):
+        """Queries to ``q``, keys and values into pages in 8 bits: the product in 32-bit, then one kernel that rotates, scales and stores."""
+        b, ops = ctx.batch, self.ops
+        qkv = ctx.ws.get("qkv", (h.shape[0], w_qkv.shape[0]), torch.float32)
+        ops.linear(ops.normed(ctx, h), w_qkv, qkv)
+        rotary = self.position.rotary
+        if rotary is None and self.position.changes_vectors:
+            qv = qkv[:, :self.q_dim].unflatten(1, (self.heads, self.head_dim))
+            kv = (qkv[:, self.q_dim:self.q_dim + self.kv_dim].unflatten(1, (self.kv_heads, self.head_dim))
+                  if writes else None)
+            self.position.apply(ctx, qv, kv, b.positions)
+        if not writes:         # queries only: nothing goes into a page
+            ops.rope_kv_append(qkv, q, None, None, b.positions, b.token_req, cache.block_table, self.heads, 0, self.head_dim, rotary,
+                               cache.page_size)
+            return
+        ops.kv_append_float8(qkv, q, cache.k, cache.v, cache.k_scale, cache.v_scale, b.cu_q, b.kv_lens, cache.block_table, self.heads,
+                             self.kv_heads, self.head_dim, None if rotary is None else ops.rope_table(ctx, b.positions, rotary),
+                             rotary is not None and rotary.interleaved, cache.page_size)
 
     def forward(self, ctx, h, cache, residual=None, emit_norm=None):
         b, ops, ws = ctx.batch, self.ops, ctx.ws
@@ -82,11 +103,16 @@ class PagedAttention(Mixer):
         writes = cache.writes and not self.reads_shared_cache
         cols = self.q_dim + (2 * self.kv_dim if writes else 0)
         # a call that reads another call's cache projects queries only (the first rows)
-        w_qkv = self.w_qkv if self.w_qkv.shape[0] == cols else self.w_qkv[:cols]
+        w_qkv = self.w_qkv
+        if w_qkv.shape[0] != cols:
+            w_qkv = w_qkv.first_rows(cols) if hasattr(w_qkv, "first_rows") else w_qkv[:cols]
         q = ws.get("q_heads", (T, self.heads, self.head_dim), self.dtype)
         rotary = self.position.rotary
         kv_heads = self.kv_heads if writes else 0
-        if rotary is not None or not self.position.changes_vectors:
+        float8 = cache.k_scale is not None
+        if float8:
+            self._write_float8(ctx, h, w_qkv, q, cache, writes)
+        elif rotary is not None or not self.position.changes_vectors:
             # the product, the rotation and the write into the pages, fused where the kernels allow
             ops.qkv_rope_append(ctx, h, w_qkv, q, cache.k if writes else None, cache.v if writes else None,
                                 b.positions, b.token_req, cache.block_table, self.heads, kv_heads,
@@ -105,9 +131,14 @@ class PagedAttention(Mixer):
                                b.positions, b.token_req, cache.block_table, self.heads, kv_heads,
                                self.head_dim, None, cache.page_size)
         out = ws.get("attn_ctx", (T, self.q_dim), self.dtype)
-        ops.paged_attention(q, cache.k, cache.v, cache.block_table, b.cu_q, b.kv_lens, b.token_req, out,
-                            self.scale, self.window or 0, cache.page_size,
-                            b.num_requests, b.max_q_len, b.max_kv_len, ws=ws, min_q_len=b.min_q_len)
+        if float8:
+            ops.paged_attention_float8(q, cache.k, cache.v, cache.k_scale, cache.v_scale, cache.block_table, b.cu_q, b.kv_lens, out,
+                                       self.scale, self.window or 0, cache.page_size, b.num_requests, b.max_q_len, b.max_kv_len, ws=ws,
+                                       min_q_len=b.min_q_len)
+        else:
+            ops.paged_attention(q, cache.k, cache.v, cache.block_table, b.cu_q, b.kv_lens, b.token_req, out,
+                                self.scale, self.window or 0, cache.page_size,
+                                b.num_requests, b.max_q_len, b.max_kv_len, ws=ws, min_q_len=b.min_q_len)
         if residual is not None:
             if emit_norm is None:
                 ops.linear(out, self.w_o, residual, accumulate=True)

@@ -102,6 +102,9 @@ class LayerCache:
     state: Optional[torch.Tensor] = None
     writes: bool = True
     parts: Optional[tuple] = None
+    #: of a cache in 8 bits (``k`` and ``v`` are float8_e4m3fn then): a scale per page and head, ``[num_pages, kv_heads]``
+    k_scale: Optional[torch.Tensor] = None
+    v_scale: Optional[torch.Tensor] = None
 
 
 # --------------------------------------------------------------------------
@@ -127,6 +130,10 @@ class Part:
     #: the row (scaled as the output is) in its own pass. Without ``defer_bias`` the part adds it itself.
     defers_bias = False
     output_bias = None
+    #: Whether the part gives all of its matrices to the kernel set to hold (``hold_matrix``), so that they may be held in 8 bits.
+    holds_matrices = False
+    #: Whether a mixer with a paged cache can read and write one in 8 bits (``LayerCache.k_scale``).
+    takes_float8_cache = False
 
     def tensors(self) -> Dict[str, TensorSpec]:
         return {}
@@ -246,6 +253,12 @@ class PartSpec:
     name: str
     params: dict = field(default_factory=dict)
     prefix: str = ""
+
+
+def hold_matrix(ops, w: torch.Tensor):
+    """A matrix as the kernel set keeps it for its products (``CudaOps.hold``)."""
+    hold = getattr(ops, "hold", None)
+    return w.contiguous() if hold is None else hold(w)
 
 
 def tensor_name(prefix: str, local: str) -> str:

@@ -10,12 +10,13 @@ from __future__ import annotations
 
 import torch
 
-from .base import FeedForward, TensorSpec, register_feed_forward
+from .base import FeedForward, TensorSpec, hold_matrix, register_feed_forward
 
 
 @register_feed_forward("swiglu")
 class SwiGLU(FeedForward):
     graph_safe = True
+    holds_matrices = True
 
     def __init__(self, width: int, inner: int, init_std: float = 0.02):
         self.width, self.inner = int(width), int(inner)
@@ -30,7 +31,7 @@ class SwiGLU(FeedForward):
     def load(self, tensors, ops, dtype):
         super().load(tensors, ops, dtype)
         self.w_gate_up = ops.pack_gate_up(tensors["gate_proj.weight"], tensors["up_proj.weight"])
-        self.w_down = tensors["down_proj.weight"].contiguous()
+        self.w_down = hold_matrix(ops, tensors["down_proj.weight"])
 
     # ``h`` may be a norm that is half done (``CudaOps.linear_swiglu`` takes it), and the last product
     # may fold in the first half of the norm that follows (``emit_norm``)
