@@ -37,6 +37,7 @@
 #include "tc_host.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -46,21 +47,24 @@ using attn8::Params;
 constexpr int KT = 128;                 // keys per tile
 constexpr int THREADS = 192;
 constexpr int MAX_ROWS = 16;
-constexpr int SEGMENT = 2;              // what a request's head costs beside its tiles, in tiles
+constexpr int MAX_CLUSTER = 8;
+constexpr int SEGMENT = 4;              // what a request's head costs beside its tiles, in tiles
 constexpr uint32_t O_COL = 64, TMEM_COLS = 256;          // tensor memory: two buffers of S^T, then O
 
-template <int HD, int N>
+template <int HD, int N, bool CLUSTER>
 struct Shape {
   static constexpr int ROWS = N / 2;                                    // query rows
   static constexpr int OPERAND = KT * HD, STAGE = 2 * OPERAND;          // bytes: keys, values
-  static constexpr int CTAS = N == 16 ? 2 : 1;                          // per SM
-  static constexpr int STAGES = 192 * 1024 / CTAS / STAGE;              // 3 (6) of 32 KB, 6 (12) of 16 KB
+  static constexpr int CTAS = N == 16 && !CLUSTER ? 2 : 1;              // per SM
+  static constexpr int STAGES = (CLUSTER ? 128 : 192 / CTAS) * 1024 / STAGE;        // 3 (6, 4) of 32 KB, 6 (12, 8) of 16 KB
   static constexpr int PARTS = N == 16 ? 3 : 2;                         // codes of a weight
   // weights go to 2^GROWTH of the reference and are multiplied by 2^UP: codes go to 448
   static constexpr float GROWTH = PARTS == 3 ? 3.f : 0.f, UP = PARTS == 3 ? 5.f : 8.f;
   static constexpr int P_BYTES = PARTS * ROWS * KT, Q_BYTES = N * 128;
   static constexpr int RING_AT = 2 * P_BYTES + 2 * Q_BYTES;
-  static constexpr int BYTES = RING_AT + STAGES * STAGE;
+  // CLUSTER: behind the ring the rows' sums, maxima and denominators of the cluster's CTAs, in its first
+  static constexpr int RC = HD + 4, PARTS_AT = RING_AT + STAGES * STAGE;
+  static constexpr int BYTES = PARTS_AT + (CLUSTER ? MAX_CLUSTER * ROWS * RC * 4 : 0);
   static constexpr int RS = HD + 2;                                     // a row's sums, maximum, denominator: a part in scratch memory
   static_assert(RING_AT % 1024 == 0 && P_BYTES + KT * 128 <= BYTES, "swizzled tiles; P's 128 rows end inside");
 };
@@ -122,10 +126,15 @@ __device__ __forceinline__ bool any_of_four(bool mine) {
       : "=r"(r) : "r"((uint32_t)mine) : "memory");
   return r != 0;
 }
+__device__ __forceinline__ void st_async_v4(uint32_t addr, uint32_t bar, float a, float b, float c, float d) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%2, %3, %4, %5}, [%1];"
+               ::"r"(addr), "r"(bar), "r"(__float_as_uint(a)), "r"(__float_as_uint(b)), "r"(__float_as_uint(c)), "r"(__float_as_uint(d))
+               : "memory");
+}
 __device__ __forceinline__ void sync_four() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
 
 struct Bars {
-  uint64_t full[12], empty[12], s_ready[2], p_ready[2], pv_done[2], q_ready[2], o_free;
+  uint64_t full[12], empty[12], s_ready[2], p_ready[2], pv_done[2], q_ready[2], o_free, part;
   uint32_t tmem_base;
   int abort, last[2];
   int2 total, scan[6];
@@ -134,11 +143,13 @@ struct Bars {
   float top[4][MAX_ROWS], corr[MAX_ROWS], vtop[4], lsum[4][MAX_ROWS];
 };
 
-template <int HD, int N>
-__global__ void __launch_bounds__(THREADS, Shape<HD, N>::CTAS)
+// CLUSTER: one request's head per thread-block cluster, its CTAs share the tiles and merge through distributed shared memory.
+template <int HD, int N, bool CLUSTER>
+__global__ void __launch_bounds__(THREADS, Shape<HD, N, CLUSTER>::CTAS)
 attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const Params p,
-                           const int min_tiles, float* __restrict__ partials, int* __restrict__ counters) {
-  using S = Shape<HD, N>;
+                           const int min_tiles,        // (CLUSTER: CTAs of a cluster)
+                           float* __restrict__ partials, int* __restrict__ counters) {
+  using S = Shape<HD, N, CLUSTER>;
   constexpr int RS = S::RS, ROWS = S::ROWS, STAGES = S::STAGES;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bars;
@@ -159,6 +170,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
       mbar_init(smem_u32(&bars.q_ready[b]), 128);
     }
     mbar_init(smem_u32(&bars.o_free), 32);
+    mbar_init(smem_u32(&bars.part), 1);
     bars.abort = 0, bars.total = make_int2(0, 0);
     fence_barrier_init();
     fence_proxy_async();
@@ -175,6 +187,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
   const uint32_t tmem = bars.tmem_base;
   volatile int* aborted = &bars.abort;
   gb::pdl_launch_dependents();
+  if (CLUSTER) cluster_arrive_wait();      // every barrier is there before another CTA's sums are sent to it
 
   // ---- every request's tiles (the batch's lengths are there before the step's first kernel)
   struct Span {
@@ -187,7 +200,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
     s.hi = kv_len - 1;
     return s;
   };
-  for (int r0 = 0; r0 < p.R; r0 += THREADS) {
+  for (int r0 = 0; !CLUSTER && r0 < p.R; r0 += THREADS) {
     const int r = r0 + threadIdx.x;
     int n = 0;
     if (r < p.R) {
@@ -219,7 +232,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
     __syncthreads();
   }
   // Stretches are equal in cost: a request's head is its tiles and SEGMENT behind them. (The host has seen that all of it fits 31 bits.)
-  const int tiles = cum[p.R] * p.Hkv, costs = cost[p.R] * p.Hkv;
+  const int tiles = CLUSTER ? 0 : cum[p.R] * p.Hkv, costs = CLUSTER ? 0 : cost[p.R] * p.Hkv;
   // as many workers as leave each min_tiles or so, and one for every head that has tiles
   const int workers = max(1, min((int)gridDim.x, max(tiles / min_tiles, bars.total.y * p.Hkv)));
   const int stretch = max(1, (costs + workers - 1) / workers);
@@ -239,7 +252,18 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
     const int r = find(cost, c), n = cum[r + 1] - cum[r], rem = c - cost[r] * p.Hkv, head = rem / (n + SEGMENT);
     return cum[r] * p.Hkv + head * n + min(rem - head * (n + SEGMENT), n);
   };
-  const int a_begin = cta < workers ? begins_at(cta) : tiles, a_end = cta < workers ? begins_at(cta + 1) : tiles;
+  // CLUSTER: this CTA's head, its request's keys, and the CTA's part of them
+  const int head = cta / min_tiles, rank = cta % min_tiles, own_r = head / p.Hkv;
+  Span own{};
+  int own_n = 0, own_per = 0;
+  if (CLUSTER) {
+    own = span_of(p.cu_q[own_r], p.cu_q[own_r + 1], p.kv_lens[own_r]);
+    if (own.nrows > 0 && own.nrows <= ROWS && own.hi >= own.lo) own_n = own.hi / KT - own.lo / KT + 1;
+    own_per = (own_n + min_tiles - 1) / min_tiles;
+  }
+  const int own_first = min(own_n, rank * own_per), own_end = min(own_n, own_first + own_per);
+  const int a_begin = CLUSTER ? own_first : cta < workers ? begins_at(cta) : tiles;
+  const int a_end = CLUSTER ? own_end : cta < workers ? begins_at(cta + 1) : tiles;
   const int my_tiles = a_end - a_begin;
 
   // A segment: one request's head, or this CTA's part of it: tiles first .. first + count of its n
@@ -248,6 +272,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
   };
   auto segment_at = [&](int a) {
     Segment g;
+    if (CLUSTER) return Segment{own_r, head % p.Hkv, a, own_n, a_end - a};
     const int lo = find(cum, a);
     g.r = lo, g.n = cum[lo + 1] - cum[lo];
     const int rem = a - cum[lo] * p.Hkv;
@@ -255,7 +280,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
     g.count = min(g.n - g.first, a_end - a);
     return g;
   };
-  auto span_at = [&](int r) { return span_of(begin_s[r], begin_s[r + 1], len_s[r]); };
+  auto span_at = [&](int r) { return CLUSTER ? own : span_of(begin_s[r], begin_s[r + 1], len_s[r]); };
 
   // Everything else comes from the kernels in front, the pages among it: a page that this step writes is encoded again.
   gb::pdl_wait();
@@ -591,6 +616,8 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
         const float f = whole ? unit * inv : unit;
         __nv_bfloat16* const dst = p.out + ((size_t)(w.q_begin + r / p.g) * p.Hq + g.kvh * p.g + r % p.g) * HD;
         float* const part = partials + ((size_t)cta * 2 + (a == a_begin ? 0 : 1)) * (MAX_ROWS * RS) + r * RS;
+        float* const own_part = reinterpret_cast<float*>(base + S::PARTS_AT) + (rank * ROWS + r) * S::RC;
+        const uint32_t to = CLUSTER ? map_to_rank(smem_u32(own_part), 0) : 0, to_bar = CLUSTER ? map_to_rank(smem_u32(&bars.part), 0) : 0;
 #pragma unroll
         for (int h = 0; h < HD / 16; ++h) {
           uint32_t o[16];
@@ -605,7 +632,13 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
             // (nothing seen: the sums mean nothing)
             y[c] = mr == -INFINITY && ll == ll ? 0.f : fmaf(lo, 0.03125f, hi) * f;
           }
-          if (mine) {
+          if (CLUSTER && mine && !whole) {
+#pragma unroll
+            for (int c = 0; c < 16; c += 4) {
+              if (rank == 0) *reinterpret_cast<float4*>(own_part + h * 16 + c) = make_float4(y[c], y[c + 1], y[c + 2], y[c + 3]);
+              else st_async_v4(to + (h * 16 + c) * 4, to_bar, y[c], y[c + 1], y[c + 2], y[c + 3]);
+            }
+          } else if (mine) {
 #pragma unroll
             for (int c = 0; c < 16; c += 2) {
               if (whole) gb::store_pair(dst + h * 16 + c, y[c], y[c + 1]);
@@ -613,7 +646,12 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
             }
           }
         }
-        if (mine && !whole) __stcg(reinterpret_cast<float2*>(part + HD), make_float2(mr, ll));
+        if (CLUSTER && mine && !whole) {
+          if (rank == 0) *reinterpret_cast<float4*>(own_part + HD) = make_float4(mr, ll, 0.f, 0.f);
+          else st_async_v4(to + HD * 4, to_bar, mr, ll, 0.f, 0.f);
+        } else if (mine && !whole) {
+          __stcg(reinterpret_cast<float2*>(part + HD), make_float2(mr, ll));
+        }
         tc_fence_before_sync();
         mbar_arrive(smem_u32(&bars.o_free));
       }
@@ -627,18 +665,24 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
       now = next, next = later;
     }
     // ---- segments of several CTAs: who counts the last arrival adds the parts up, in the CTAs' order
+    if (CLUSTER && rank != 0) n_shared = 0;
     if (n_shared > 0) sync_four();     // the parts are written
     int c0[2] = {0, 0}, c1[2] = {0, 0};
     bool behind[2] = {false, false};   // whether the first of them has another segment's end in front of its part
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      if (i >= n_shared) break;
+      if (CLUSTER) c1[i] = (own_n + own_per - 1) / max(own_per, 1) - 1;
+      if (CLUSTER || i >= n_shared) break;
       const Segment& g = shared[i].g;
       const int c = cost[g.r] * p.Hkv + g.kvh * (g.n + SEGMENT);
       c0[i] = c / stretch, c1[i] = (c + g.n - 1) / stretch;
       behind[i] = begins_at(c0[i]) < cum[g.r] * p.Hkv + g.kvh * g.n;
     }
-    if (x < n_shared) {
+    if (CLUSTER && n_shared > 0) {         // the others' rows
+      if (x == 0) mbar_arrive_expect_tx(smem_u32(&bars.part), c1[0] * shared[0].nrows * S::RC * 4);
+      wait(bars.part, 0);
+    }
+    if (!CLUSTER && x < n_shared) {
       __threadfence();
       const Segment& g = x == 0 ? shared[0].g : shared[1].g;
       int* counter = counters + (size_t)g.r * p.Hkv + g.kvh;
@@ -652,8 +696,12 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
     const int row = x / LANES, sub = x % LANES;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      if (i >= n_shared || !bars.last[i] || row >= shared[i].nrows || !ok) continue;
-      auto part_of = [&](int c) { return partials + ((size_t)c * 2 + (c == c0[i] && behind[i] ? 1 : 0)) * (MAX_ROWS * RS) + row * RS; };
+      if (i >= n_shared || (!CLUSTER && !bars.last[i]) || row >= shared[i].nrows || !ok) continue;
+      auto part_of = [&](int c) -> const float* {
+        if (CLUSTER) return reinterpret_cast<const float*>(base + S::PARTS_AT) + (c * ROWS + row) * S::RC;
+        return partials + ((size_t)c * 2 + (c == c0[i] && behind[i] ? 1 : 0)) * (MAX_ROWS * RS) + row * RS;
+      };
+      auto read2 = [&](const float* from) { return CLUSTER ? *reinterpret_cast<const float2*>(from) : __ldcg(reinterpret_cast<const float2*>(from)); };
       float mm = -INFINITY, ll = 0.f;
       float2 v[PER];
 #pragma unroll
@@ -664,9 +712,9 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float* part = part_of(min(c + k, c1[i]));
-          ml[k] = __ldcg(reinterpret_cast<const float2*>(part + HD));
+          ml[k] = read2(part + HD);
 #pragma unroll
-          for (int e = 0; e < PER; ++e) y[k][e] = __ldcg(reinterpret_cast<const float2*>(part + 2 * (sub + LANES * e)));
+          for (int e = 0; e < PER; ++e) y[k][e] = read2(part + 2 * (sub + LANES * e));
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -691,6 +739,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
   }
   tc_fence_before_sync();
   __syncthreads();
+  if (CLUSTER) cluster_arrive_wait();      // nobody sends to a CTA that has left
   if (warp == 1) tmem_dealloc(tmem, TMEM_COLS);
 }
 
@@ -736,14 +785,16 @@ int pool_map(const void* ptr, int page, int heads, long long pages, int hd, CUte
   return GB_OK;
 }
 
+constexpr int CLUSTER_TILES = 16;
 constexpr int MAX_REQUESTS = 256;    // of one launch: their lengths lie in shared memory
 
-template <int HD, int N>
+template <int HD, int N, bool CLUSTER>
 int launch(const Params& p, const CUtensorMap& km, const CUtensorMap& vm, long long tiles_most, int min_tiles, void* parts, void* counters,
            cudaStream_t stream) {
-  using S = Shape<HD, N>;
-  auto kernel = attention_f8_decode_kernel<HD, N>;
+  using S = Shape<HD, N, CLUSTER>;
+  auto kernel = attention_f8_decode_kernel<HD, N, CLUSTER>;
   constexpr int LENGTHS = (4 * MAX_REQUESTS + 3) * 4;
+  static_assert(1024 + S::BYTES + LENGTHS + (int)sizeof(Bars) + 1024 <= 232448, "one CTA");
   static_assert(S::CTAS == 1 || 2 * (1024 + S::BYTES + LENGTHS + (int)sizeof(Bars) + 1024) <= 233472, "two CTAs an SM");
   static gb::OncePerDevice configured;
   if (configured.needed()) {
@@ -754,8 +805,8 @@ int launch(const Params& p, const CUtensorMap& km, const CUtensorMap& vm, long l
   const int room = tc_host::sm_count() * S::CTAS;
   const long long most = std::max(tiles_most / min_tiles + 1, (long long)p.R * p.Hkv);
   const size_t smem = 1024 + S::BYTES + (size_t)(4 * p.R + 3) * 4;
-  return gb::check_pdl_launch(gb::launch_pdl(kernel, dim3((unsigned)(most < room ? most : room)), dim3(THREADS), smem, stream, dim3(1), km, vm, p,
-                                             min_tiles, (float*)parts, (int*)counters), "attention_f8_decode");
+  const unsigned grid = CLUSTER ? (unsigned)(p.R * p.Hkv * min_tiles) : (unsigned)(most < room ? most : room);
+  return gb::check_pdl_launch(gb::launch_pdl(kernel, dim3(grid), dim3(THREADS), smem, stream, dim3(CLUSTER ? (unsigned)min_tiles : 1u), km, vm, p, min_tiles, (float*)parts, (int*)counters), "attention_f8_decode");
 }
 
 }  // namespace
@@ -786,11 +837,26 @@ GB_EXPORT int gb_f8_attention_decode(const void* q, const void* k_pool, const vo
     const Params p{(const __nv_bfloat16*)q, (const float*)k_scale, (const float*)v_scale, (__nv_bfloat16*)out,
                    (const int32_t*)table + (size_t)r0 * table_width, (const int32_t*)cu_q + r0, (const int32_t*)kv_lens + r0, table_width, n, Hq,
                    Hkv, g, window, page, scale * 1.4426950408889634f};
-    const long long tiles = (long long)n * Hkv * ((reach + KT - 1) / KT + 1);
+    const int reach_tiles = (reach + KT - 1) / KT;
+    const long long tiles = (long long)n * Hkv * (reach_tiles + 1);
     int* count = (int*)counters + (size_t)r0 * Hkv;
     const cudaStream_t st = (cudaStream_t)stream;
-    if (hd == 64) rc = g <= 8 ? launch<64, 16>(p, km, vm, tiles, min_tiles, parts, count, st) : launch<64, 32>(p, km, vm, tiles, min_tiles, parts, count, st);
-    else rc = g <= 8 ? launch<128, 16>(p, km, vm, tiles, min_tiles, parts, count, st) : launch<128, 32>(p, km, vm, tiles, min_tiles, parts, count, st);
+    // Few heads with little work: a cluster for each, which merges through shared memory and sums no lengths up: eight CTAs, or as many as let all
+    // clusters run at once (the GPU holds 15 of eight, 22 of six, 33 of four, one CTA an SM; with three CTAs for 48 heads a third of them
+    // waited: 19 us for 10.6 with two). Heads of 128, eight of them, us with and without clusters: 500 keys 8.5 / 12.9, 2,048 10.7 / 19.6, 16,384
+    // 24.3 / 25.4; 64 heads: 500 keys 10.9 / 14.3, 2,048 18.5 / 25.7, 4,096 25.0 / 31.8. Not where a CTA gets more than
+    // CLUSTER_TILES tiles: requests of unequal length are not evened out here.
+    const int heads = n * Hkv;
+    int c = heads <= 15 ? 8 : heads <= 22 ? 6 : heads <= 33 ? 4 : heads <= tc_host::sm_count() / 2 ? 2 : heads <= tc_host::sm_count() ? 1 : 0;
+    c = std::min(std::min(c, MAX_CLUSTER), reach_tiles);
+    const bool cluster = c >= 1 && (reach_tiles + c - 1) / c <= CLUSTER_TILES;
+    const auto go = [&](auto hd_c, auto n_c) {
+      constexpr int HD = decltype(hd_c)::value, N = decltype(n_c)::value;
+      return cluster ? launch<HD, N, true>(p, km, vm, tiles, c, parts, count, st) : launch<HD, N, false>(p, km, vm, tiles, min_tiles, parts, count, st);
+    };
+    using std::integral_constant;
+    if (hd == 64) rc = g <= 8 ? go(integral_constant<int, 64>(), integral_constant<int, 16>()) : go(integral_constant<int, 64>(), integral_constant<int, 32>());
+    else rc = g <= 8 ? go(integral_constant<int, 128>(), integral_constant<int, 16>()) : go(integral_constant<int, 128>(), integral_constant<int, 32>());
   }
   return rc;
 }
