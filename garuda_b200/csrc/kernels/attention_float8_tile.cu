@@ -3,22 +3,29 @@
 //   s_j = (q . k8_j) * ks(page of j) * scale over keys [start, pos];  out = sum_j softmax(s)_j vs(page of j) v8_j
 // (garuda/src/llama/mod.rs:793-818; the window garuda/src/cache/mod.rs:333-338; query head h reads key/value head h / g).
 //
-// Laid out as the bfloat16 kernel (attention_tcgen05.cu): 128 query rows a piece of work, tiles of 128 keys, persistent CTAs, S = Q K^T two
-// tiles ahead of O += P V, two softmax groups of 128 threads with 64 keys of every tile each and an accumulator of their own,
-// probabilities through tensor memory, a reference maximum that moves when it has been outgrown by 2^8. What the codes change:
+// A piece of work is 256 query rows, (token, head-of-group) pairs of one kv head of one request, in two halves of 128; its keys are walked in
+// tiles of 128. The kernel is persistent: one CTA per SM takes pieces until none are left (rounds of gridDim.x pieces, walked forth and
+// back so that long and short ones mix). Per half: S = Q K^T into tensor memory, a softmax in registers (a thread has a row and all 128 keys
+// of the tile), P back over S, O += P V; while one half's softmax runs, the tensor cores work for the other. Products run in the order of
+// their issue, so a half's next S, which overwrites P, is issued right behind the P V that reads it, and the end of an S product says that
+// the P V in front has ended too: the accumulator may be rescaled without another wait.
+// (The bfloat16 kernel's arrangement, 128 rows whose tiles two groups share and S two tiles ahead, took 70 us for 2,048 tokens of 32 heads of 128
+// and 105 us for two portions of 509 over a window of 4,096; this one takes 55 and 79, that kernel itself 59 and 92.) A tile takes 4,000
+// clocks: 2,200 of them the softmax of a half, of which 1,500 for its 128 exponentials a row (1,024 at the rate of their pipe), the
+// rest the products between its weights and its next scores, behind one another: the chain, not a unit, sets the pace.
 //   * S is a product of codes as they lie (tcgen05.mma kind f8f6f4): a query row, scaled by a power of two to a largest of at most 448, is the
 //     sum of two E4M3 rows (a bfloat16's eight bits are four and four; what is 2^-11 of the row's largest and below loses bits
 //     that the sum does not see), so S = Qhi K^T + Qlo K^T at twice the rate of bfloat16: the same time, half of the keys' bytes.
 //   * Values become halves (exactly: every E4M3 number is one) in shared memory, a conversion for two of them, by four warps of
-//     their own: 128 keys of 128 channels are 256 conversions and 1,024 shared-memory accesses of 16 bytes a warp lane row, for 128 rows'
-//     worth of products. (Splitting P into codes instead would cost the softmax warps, which set the pace, two instructions a score.)
+//     their own, for 256 rows' worth of products. (Splitting P into codes instead would cost the softmax warps two instructions a score.)
 //   * A page's ks goes into the factor of the exponent's multiply-add, its vs (as a power of two) into the constant; the denominator takes it
 //     out again per sixteen keys. The accumulators are in units of the largest vs so far. P in halves: eleven bits.
+//   * The reference maximum follows the running one only when it has been outgrown by 2^8 for some row of a warp.
 //   warp 0      TMA: keys and values, a box a page, into rings of their own; looks up pages and scales four tiles at a time, two steps ahead
 //   warp 1      one elected lane issues the products
-//   warps 4-11  softmax
+//   warps 4-11  softmax, four warps a half
 //   warps 12-15 the queries of the next piece as codes, the values of the next tile as halves (rows that no query reads as zeros)
-// Registers are shared out by need (setmaxnreg). Every wait is bounded.
+// Registers are shared out by need (setmaxnreg; with 184 for the softmax some went to memory, and it took 60 us). Every wait is bounded.
 #include "attention_float8.cuh"
 #include "error_word.cuh"
 #include "tc_common.cuh"
@@ -29,20 +36,18 @@ namespace {
 using namespace tc;
 using attn8::Params;
 
-constexpr int QROWS = 128;          // query rows per CTA
+constexpr int QROWS = 256;          // query rows per CTA
+constexpr int HALF = 128;           // of a half
 constexpr int KT = 128;             // keys per tile
-constexpr int GROUPS = 2;           // softmax groups: each walks its own half of every key tile
-constexpr int GK = KT / GROUPS;     // keys per group and tile
 constexpr int BLOCK_BYTES = 128 * 128;              // 128 values' rows of one block of 64 channels in halves
 constexpr int TMEM_COLS = 512;
-constexpr int S_BUFS = 2;                           // S buffers: the S products run this many tiles ahead
-constexpr int O_COL0 = S_BUFS * KT;                 // behind the S buffers
+constexpr int O_COL0 = 2 * KT;                      // behind the halves' S
 constexpr int THREADS = 512;
 constexpr float RESCALE_ABOVE = 8.f;                // in powers of two
 constexpr float UP = 6.f;                           // probabilities are multiplied by 2^6: halves go to 65,504, and down to 2^-30 of the reference
 constexpr int SLOTS = 16;                            // tiles' scales in flight
 // registers a thread of the warpgroups: copies and products, softmax (two), conversions; 128 a thread at launch
-constexpr int REGS_ISSUE = 56, REGS_SOFTMAX = 176, REGS_CONVERT = 104;
+constexpr int REGS_ISSUE = 56, REGS_SOFTMAX = 200, REGS_CONVERT = 56;
 static_assert(REGS_ISSUE + 2 * REGS_SOFTMAX + REGS_CONVERT <= 4 * 128, "no more registers than at launch");
 
 template <int HD>
@@ -50,23 +55,20 @@ struct Shape {
   static constexpr int BLOCKS = HD / 64;                              // blocks of 64 channels of values in halves
   static constexpr int Q_BYTES = 2 * QROWS * HD, CODE_BYTES = KT * HD, H_BYTES = BLOCKS * BLOCK_BYTES;
   static constexpr int K_STAGES = HD == 64 ? 4 : 3, V_STAGES = HD == 64 ? 4 : 2, H_STAGES = HD == 64 ? 3 : 2;
-  static constexpr int K_AT = 2 * Q_BYTES, V_AT = K_AT + K_STAGES * CODE_BYTES, H_AT = V_AT + V_STAGES * CODE_BYTES;
+  static constexpr int K_AT = Q_BYTES, V_AT = K_AT + K_STAGES * CODE_BYTES, H_AT = V_AT + V_STAGES * CODE_BYTES;
   static constexpr int TILE_BYTES = H_AT + H_STAGES * H_BYTES;
-  static constexpr int CH = HD / GROUPS;                              // channels that a group writes out in the merge
-  static_assert(O_COL0 + GROUPS * HD <= TMEM_COLS && GK == 64, "tensor memory layout");
+  static_assert(O_COL0 + 2 * HD <= TMEM_COLS, "tensor memory layout");
   static_assert(K_STAGES + 5 <= SLOTS, "a tile's scales outlive its keys");
 };
 
 // Barriers and the like, behind the tiles in dynamic shared memory.
 struct Misc {
-  uint64_t q_full[2], q_empty[2], k_full[6], k_empty[6], v_full[4], v_empty[4], h_full[3], h_empty[3];
-  uint64_t s_ready[S_BUFS], p_ready[S_BUFS], o_ready;
+  uint64_t q_full[2], k_full[6], k_empty[6], v_full[4], v_empty[4], h_full[3], h_empty[3];
+  uint64_t s_ready[2], p_ready[2][2], o_ready[2], o_free[2];
   uint32_t tmem_base;
   int abort;
   float2 scales[SLOTS][8];              // a tile's ks of each sixteen keys (negative: no page there) and log2 of vs
-  float factor[2][QROWS];               // per query row: 2^e * scale * log2(e)
-  float2 ml[GROUPS][QROWS];             // the groups' reference maxima and denominators, for the merge
-  float vref[GROUPS];
+  float factor[QROWS];                  // per query row: 2^e * scale * log2(e)
 };
 
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -82,6 +84,20 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
+}
+// Two at a time.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 // The largest of three in one instruction.
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -112,11 +128,17 @@ __device__ __forceinline__ uint32_t swizzled(int row, int c) {
   return HD == 128 ? (uint32_t)(row * 128 + ((c ^ (row & 7)) << 4)) : (uint32_t)(row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
 }
 
-// One piece of work: 128 query rows of one request and kv head.
+// One piece of work: 256 query rows of one request and kv head.
 struct Item {
   bool valid;
   int kvh, q_begin, tok0, nrows, pos0, lo, hi, tile_begin, n_tiles;
   const int32_t* table;
+  // tiles of a half: the first rows of a piece see fewer keys than the last
+  __device__ __forceinline__ int tiles_of(int half, int g) const {
+    const int rows = min(HALF, nrows - half * HALF);
+    if (rows <= 0) return 0;
+    return max(1, (pos0 + (half * HALF + rows - 1) / g) / KT + 1 - tile_begin);
+  }
 };
 
 // Items are numbered request by request, the tiles of a request from its end (the longest first), the
@@ -132,7 +154,6 @@ __device__ __forceinline__ Item decode_item(const Params& p, int q_tiles, int it
   const int q_len = p.cu_q[r + 1] - w.q_begin;
   const int tokens_per_tile = QROWS / p.g;
   w.tok0 = qt * tokens_per_tile;
-  w.valid = q_len * p.g > attn8::decode_rows(p.g) && w.tok0 < q_len;      // else a decode request, or past its end
   const int kv_len = p.kv_lens[r];
   const int ntok = min(tokens_per_tile, q_len - w.tok0);
   w.nrows = ntok * p.g;
@@ -140,12 +161,12 @@ __device__ __forceinline__ Item decode_item(const Params& p, int q_tiles, int it
   w.lo = p.window > 0 ? max(0, w.pos0 + 1 - p.window) : 0;          // first key any row reads
   w.hi = w.pos0 + ntok - 1;                                         // last key any row reads
   w.tile_begin = w.lo / KT;
+  w.valid = q_len * p.g > attn8::decode_rows(p.g) && w.tok0 < q_len && w.hi >= w.lo;      // else a decode request, or past its end
   w.n_tiles = w.valid ? w.hi / KT + 1 - w.tile_begin : 0;
   w.table = p.block_table + (size_t)r * p.table_width;
   return w;
 }
 
-// Walks this CTA's items tile by tile.
 // The k-th item of this CTA: rounds of gridDim.x items, walked forth and back in turn, so that the
 // CTA that got the longest item of one round gets the shortest of the next.
 __device__ __forceinline__ int cta_item(int k) {
@@ -153,10 +174,11 @@ __device__ __forceinline__ int cta_item(int k) {
   return k * g + ((k & 1) ? g - 1 - b : b);
 }
 
+// Walks this CTA's items.
 struct Cursor {
   int item, total, step, q_tiles, round;
   int it;          // valid items before this one
-  int j;           // tile within the item
+  int j;           // tile within the item (for who walks tiles)
   Item w;
   bool done;
   __device__ __forceinline__ void seek(const Params& p) {
@@ -181,48 +203,39 @@ struct Cursor {
 };
 
 // The same walk for the warp that issues the matrix products: it needs nothing of an item but its
-// number of tiles, and everything it executes delays the tensor cores. Its lanes decode 32 items at
+// halves' tiles, and everything it executes delays the tensor cores. Its lanes decode 32 items at
 // a time, one each; the walk then only shuffles the counts out.
-struct TileWalk {
+struct CountWalk {
   int base;        // this CTA's items before the batch
-  int my_n;        // tiles of this lane's item of the batch (0: none, or not a valid item)
-  int lane_i;      // the current item's lane
-  int n, j;        // the current item's tiles, the current tile
-  int it;          // valid items before the current one
-  bool done;
+  int my_n[2];     // tiles of the halves of this lane's item of the batch (0: none, or not a valid item)
+  int lane_i;      // the next item's lane
+  int n[2];
   __device__ __forceinline__ void load(const Params& p, int q_tiles, int total) {
     const int k = base + (int)(threadIdx.x & 31);
     const long long item = (long long)k * gridDim.x < total ? cta_item(k) : total;
-    my_n = item < total ? decode_item(p, q_tiles, (int)item).n_tiles : 0;
-  }
-  __device__ __forceinline__ void seek(const Params& p, int q_tiles, int total) {
-    for (;;) {
-      // the next lane of the batch with tiles, if any
-      const unsigned have = __ballot_sync(0xffffffffu, my_n > 0) & (0xffffffffu << lane_i);
-      if (lane_i < 32 && have != 0) {
-        lane_i = __ffs(have) - 1;
-        n = __shfl_sync(0xffffffffu, my_n, lane_i);
-        return;
-      }
-      base += 32;
-      lane_i = 0;
-      if ((long long)base * gridDim.x >= total) {
-        done = true;
-        return;
-      }
-      load(p, q_tiles, total);
+    my_n[0] = my_n[1] = 0;
+    if (item < total) {
+      const Item w = decode_item(p, q_tiles, (int)item);
+      if (w.valid) my_n[0] = w.tiles_of(0, p.g), my_n[1] = w.tiles_of(1, p.g);
     }
   }
   __device__ __forceinline__ void start(const Params& p, int q_tiles, int total) {
-    base = 0, lane_i = 0, j = 0, it = 0, n = 0, done = false;
+    base = 0, lane_i = 0;
     load(p, q_tiles, total);
-    seek(p, q_tiles, total);
   }
-  __device__ __forceinline__ void next_tile(const Params& p, int q_tiles, int total) {
-    if (++j >= n) {
-      j = 0, ++it, ++lane_i;
-      if (lane_i >= 32) lane_i = 32;
-      seek(p, q_tiles, total);
+  // The next item's counts; false: there is none.
+  __device__ __forceinline__ bool next(const Params& p, int q_tiles, int total) {
+    for (;;) {
+      const unsigned have = lane_i < 32 ? __ballot_sync(0xffffffffu, my_n[0] > 0) & (0xffffffffu << lane_i) : 0u;
+      if (have != 0) {
+        const int l = __ffs(have) - 1;
+        n[0] = __shfl_sync(0xffffffffu, my_n[0], l), n[1] = __shfl_sync(0xffffffffu, my_n[1], l);
+        lane_i = l + 1;
+        return true;
+      }
+      base += 32, lane_i = 0;
+      if ((long long)base * gridDim.x >= total) return false;
+      load(p, q_tiles, total);
     }
   }
 };
@@ -240,7 +253,7 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
   Misc& mc = *reinterpret_cast<Misc*>(smem_raw + S::TILE_BYTES);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t q_s = smem_u32(smem_raw);                         // two buffers: the rows' codes, then what they leave
+  const uint32_t q_s = smem_u32(smem_raw);                         // the rows' codes, then what they leave
   const uint32_t k_s = q_s + S::K_AT, v_s = q_s + S::V_AT, h_s = q_s + S::H_AT;
   if ((q_s & 1023u) != 0) {                                        // the swizzle needs it; never seen
     if (threadIdx.x == 0) gb_err::report(ERR_WAIT_DRAIN);
@@ -250,11 +263,11 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
   if (threadIdx.x == 0) {
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&mc.q_full[b]), 128);
-      mbar_init(smem_u32(&mc.q_empty[b]), 1);
-    }
-    for (int b = 0; b < S_BUFS; ++b) {
-      mbar_init(smem_u32(&mc.s_ready[b]), 1);
-      mbar_init(smem_u32(&mc.p_ready[b]), GROUPS * 128);
+      mbar_init(smem_u32(&mc.s_ready[b]), 2);       // the product's end; the issuing thread, who has seen the keys' scales arrive
+      mbar_init(smem_u32(&mc.p_ready[b][0]), 128);
+      mbar_init(smem_u32(&mc.p_ready[b][1]), 128);
+      mbar_init(smem_u32(&mc.o_ready[b]), 1);
+      mbar_init(smem_u32(&mc.o_free[b]), 128);
     }
     for (int s = 0; s < K_STAGES; ++s) {
       mbar_init(smem_u32(&mc.k_full[s]), 1);
@@ -268,7 +281,6 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
       mbar_init(smem_u32(&mc.h_full[s]), 128);
       mbar_init(smem_u32(&mc.h_empty[s]), 1);
     }
-    mbar_init(smem_u32(&mc.o_ready), 1);
     mc.abort = 0;
     fence_barrier_init();
     fence_proxy_async();
@@ -285,8 +297,8 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
   const uint32_t tmem_base = mc.tmem_base;
   volatile int* abort_s = &mc.abort;
   gb::pdl_launch_dependents();
-  gb::pdl_wait();      // queries and this step's keys and values come from the kernel in front
-
+  // Queries, scales and this step's keys and values come from the kernel in front (pdl_wait below); the batch's lengths and block tables were
+  // there before the step's first kernel.
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ISSUE));
     if (warp == 0) {
@@ -320,6 +332,7 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         u.vs = u.page >= 0 ? p.v_scale[where] : 1.f;
       };
       look_pages(now);
+      gb::pdl_wait();
       look_scales(now);
       int gt = 0, ks = 0, kpar = 1, vs = 0, vpar = 1;       // tiles so far; the stages to fill and the phases of their "empty" barriers
       bool ok = true, ran_out;
@@ -364,136 +377,87 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
       }
     } else if (warp == 1) {
       // -------------------------------------------------------------------- MMA issuer
-      // The S products run two tiles ahead of the P V products, across the items' borders. After a tile's softmax its P V goes first: it
-      // reads the probabilities from the S buffer that the S product two tiles ahead then overwrites (products run in the order of
-      // their issue).
       const bool leader = elect_one();
-      constexpr uint32_t idesc_s = instr_desc(QROWS, KT), idesc_o = instr_desc(QROWS, HD) | INSTR_B_MN_MAJOR;
+      constexpr uint32_t idesc_s = instr_desc(HALF, KT), idesc_o = instr_desc(HALF, HD) | INSTR_B_MN_MAJOR;
       const uint64_t dq0 = smem_desc_rows<HD>(q_s), dk0 = smem_desc_rows<HD>(k_s), dv0 = smem_desc_sw128_mn(h_s, BLOCKS > 1 ? BLOCK_BYTES : 16);
       bool ok = true;
-      TileWalk ws, wp;               // the S products' tile, the P V products' tile
-      ws.start(p, q_tiles, total_items);
-      wp = ws;
-      int k_stage = 0, k_par = 0;                    // key stage (and its phase) of the S tile
-      int h_stage = 0, h_par = 0;                    // value stage of the P V tile
-      int s_buf = 0;                                 // S buffer of the S tile
-      int p_buf = 0, p_par = 0;                      // buffer of the P V tile and its phase
-      auto issue_s = [&]() {      // S = (Qhi + Qlo) K^T of the S tile into S buffer s_buf (both groups' columns)
-        const int qb = ws.it & 1;
-        if (ws.j == 0 && !mbar_wait(smem_u32(&mc.q_full[qb]), (ws.it >> 1) & 1)) ok = false;
-        if (ok && !mbar_wait(smem_u32(&mc.k_full[k_stage]), k_par)) ok = false;
-        if (!ok) {
-          if (lane == 0) gb_err::report(ERR_WAIT_FULL);
-          return;
-        }
-        tc_fence_after_sync();
-        if (leader) {
-          const uint64_t dq = dq0 + (uint64_t)(qb * (S::Q_BYTES >> 4)), dk = dk0 + (uint64_t)(k_stage * (S::CODE_BYTES >> 4));
-#pragma unroll
-          for (int part = 0; part < 2; ++part)
-#pragma unroll
-            for (int k = 0; k < HD / 32; ++k)
-              mma_f8(tmem_base + s_buf * KT, dq + (uint64_t)(part * (QROWS * HD >> 4) + 2 * k), dk + 2 * k, idesc_s, part > 0 || k > 0);
-          mma_commit(smem_u32(&mc.s_ready[s_buf]));      // the softmax warps pass it on to the keys' and the queries' "empty" barriers
-        }
-        __syncwarp();
-        if (++k_stage == K_STAGES) k_stage = 0, k_par ^= 1;
-        if (++s_buf == S_BUFS) s_buf = 0;
-        ws.next_tile(p, q_tiles, total_items);
+      int ks = 0, kpar = 0, hs = 0, hpar = 0;       // stages (and phases) of the keys and values in use
+      int sp[2] = {0, 0}, used[2] = {0, 0};                  // phases of p_ready, items so far, a half each
+      auto wait = [&](uint64_t& bar, int par, int code) {
+        if (!ok) return;
+        const bool came = mbar_wait(smem_u32(&bar), par);
+        if (!came) gb_err::report(code);
+        ok = __all_sync(0xffffffffu, came);
       };
-#pragma unroll 1
-      for (int b = 0; b < S_BUFS; ++b)
-        if (ok && !ws.done) issue_s();
-      while (ok && !wp.done) {
-        if (*abort_s) break;
-        if (ok && !mbar_wait(smem_u32(&mc.h_full[h_stage]), h_par)) {
-          if (lane == 0) gb_err::report(ERR_WAIT_FULL);
-          ok = false;
-        }
-        if (ok && !mbar_wait(smem_u32(&mc.p_ready[p_buf]), p_par)) {
-          if (lane == 0) gb_err::report(ERR_WAIT_ACCUM);
-          ok = false;
-        }
-        if (!ok) break;
-        tc_fence_after_sync();
-        if (leader) {
+      CountWalk w;
+      w.start(p, q_tiles, total_items);
+      while (ok && w.next(p, q_tiles, total_items)) {
+        const int n0 = w.n[0], n1 = w.n[1], n = max(n0, n1);
+        auto issue_s = [&](int h, int j) {       // S = (Qhi + Qlo) K^T of tile j
+          const bool first = h == 0, last = h == 1 || j >= n1;       // of the halves that read these keys
+          if (first || j >= n0) wait(mc.k_full[ks], kpar, ERR_WAIT_FULL);
+          tc_fence_after_sync();
+          if (leader && ok) {
+            const uint64_t dq = dq0 + (uint64_t)(h * HALF * HD >> 4), dk = dk0 + (uint64_t)(ks * (S::CODE_BYTES >> 4));
 #pragma unroll
-          for (int g = 0; g < GROUPS; ++g)
-            mma_bf16_ts<GK / 16>(tmem_base + O_COL0 + g * HD, tmem_base + p_buf * KT + g * GK,
-                                 dv0 + (uint64_t)(h_stage * (S::H_BYTES >> 4) + g * (GK * 128 >> 4)), idesc_o, 16 * 128 >> 4, wp.j > 0);
-          mma_commit(smem_u32(&mc.o_ready));             // the softmax warps pass it on to the values' "empty" barrier
+            for (int part = 0; part < 2; ++part)
+#pragma unroll
+              for (int k = 0; k < HD / 32; ++k)
+                mma_f8(tmem_base + h * KT, dq + (uint64_t)(part * (QROWS * HD >> 4) + 2 * k), dk + 2 * k, idesc_s, part > 0 || k > 0);
+            mbar_arrive(smem_u32(&mc.s_ready[h]));
+            mma_commit(smem_u32(&mc.s_ready[h]));
+            if (last) mma_commit(smem_u32(&mc.k_empty[ks]));
+          }
+          __syncwarp();
+          if (last && ++ks == K_STAGES) ks = 0, kpar ^= 1;
+        };
+        wait(mc.q_full[0], used[0] & 1, ERR_WAIT_FULL);
+        issue_s(0, 0);
+        if (n1 > 0) {
+          wait(mc.q_full[1], used[1] & 1, ERR_WAIT_FULL);
+          issue_s(1, 0);
         }
-        __syncwarp();
-        // both groups have read this S buffer in full, and the products above read their P from it
-        // before the next one writes: the S product two tiles ahead takes the buffer over
-        if (!ws.done) issue_s();
-        if (!ok) break;
-        if (++h_stage == H_STAGES) h_stage = 0, h_par ^= 1;
-        if (++p_buf == S_BUFS) p_buf = 0, p_par ^= 1;
-        wp.next_tile(p, q_tiles, total_items);
+        for (int j = 0; j < n && ok; ++j) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int mine = h == 0 ? n0 : n1;
+            if (j >= mine) continue;
+            const bool last = h == 1 || j >= n1;                     // of the halves that read these values
+            if (j == 0 && used[h] > 0) wait(mc.o_free[h], (used[h] - 1) & 1, ERR_WAIT_ACCUM);        // the item in front has been written out
+            if (j == 0) ++used[h];
+            if (h == 0 || j >= n0) wait(mc.h_full[hs], hpar, ERR_WAIT_FULL);
+            const uint64_t dv = dv0 + (uint64_t)(hs * (S::H_BYTES >> 4));
+#pragma unroll
+            for (int k = 0; k < KT / 64; ++k) {              // 64 keys' weights at a time, while the softmax is at the next
+              wait(mc.p_ready[h][k], sp[h], ERR_WAIT_ACCUM);
+              tc_fence_after_sync();
+              if (leader && ok)
+                mma_bf16_ts<4>(tmem_base + O_COL0 + h * HD, tmem_base + h * KT + k * 32, dv + (uint64_t)(k * (64 * 128 >> 4)), idesc_o,
+                               16 * 128 >> 4, j > 0 || k > 0);
+              __syncwarp();
+            }
+            sp[h] ^= 1;
+            if (leader && ok) {
+              if (last) mma_commit(smem_u32(&mc.h_empty[hs]));
+              if (j == mine - 1) mma_commit(smem_u32(&mc.o_ready[h]));
+            }
+            __syncwarp();
+            if (last && ++hs == H_STAGES) hs = 0, hpar ^= 1;
+            if (j + 1 < mine) issue_s(h, j + 1);
+          }
+        }
       }
       if (!ok) *abort_s = 1;
     }
   } else if (warp >= 12) {
     // -------------------------------------------------------------------- conversions
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_CONVERT));
-    const int x = threadIdx.x - 384;             // a query row, a key
+    const int x = threadIdx.x - 384;             // a key
     bool ok = true;
     int gt = 0, vs = 0, vpar = 0, hs = 0, hpar = 1;
-    // the queries of an item: this thread's row
-    auto put_queries = [&](const Cursor& c) {
+    Cursor c;
+    for (c.start(p, q_tiles, total_items); !c.done && ok; c.next_item(p)) {
       const Item& w = c.w;
-      const int qb = c.it & 1;
-      if (c.it >= 2 && ok && (!mbar_wait(smem_u32(&mc.q_empty[qb]), ((c.it >> 1) & 1) ^ 1) || *abort_s)) {
-        if (!*abort_s) gb_err::report(ERR_WAIT_EMPTY);
-        ok = false, *abort_s = 1;
-      }
-      if (!ok) return;
-      const bool there = x < w.nrows;
-      const uint4* src = reinterpret_cast<const uint4*>(
-          p.q + ((size_t)(w.q_begin + w.tok0 + (there ? x / p.g : 0)) * p.Hq + w.kvh * p.g + (there ? x % p.g : 0)) * HD);
-      // (read twice, the second time from L1, rather than kept in 64 registers)
-      float largest = 0.f;
-#pragma unroll 4
-      for (int i = 0; i < HD / 8; ++i) {
-        const uint4 two = there ? src[i] : make_uint4(0u, 0u, 0u, 0u);
-        const uint32_t u[4] = {two.x, two.y, two.z, two.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) largest = max3(largest, fabsf(__uint_as_float(u[e] << 16)), fabsf(__uint_as_float(u[e] & 0xFFFF0000u)));
-      }
-      const int e2 = f8::scale_exponent(largest);
-      const float inv = f8::power_of_two(-e2);
-      uint8_t* to = smem_raw + qb * S::Q_BYTES;
-#pragma unroll 2
-      for (int i = 0; i < HD / 16; ++i) {
-        const uint4 r0 = there ? src[2 * i] : make_uint4(0u, 0u, 0u, 0u), r1 = there ? src[2 * i + 1] : make_uint4(0u, 0u, 0u, 0u);
-        const uint32_t u[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float a = __uint_as_float(u[2 * e] << 16) * inv, b = __uint_as_float(u[2 * e] & 0xFFFF0000u) * inv;
-          const float d = __uint_as_float(u[2 * e + 1] << 16) * inv, f = __uint_as_float(u[2 * e + 1] & 0xFFFF0000u) * inv;
-          hi[e] = f8::encode4(a, b, d, f);
-          const float4 back = f8::decode4(hi[e]);
-          lo[e] = f8::encode4(a - back.x, b - back.y, d - back.z, f - back.w);
-        }
-        *reinterpret_cast<uint4*>(to + swizzled<HD>(x, i)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(to + QROWS * HD + swizzled<HD>(x, i)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      }
-      mc.factor[qb][x] = f8::power_of_two(e2) * p.scale_log2;
-      fence_proxy_async();              // the tensor core reads them through the async proxy
-      mbar_arrive(smem_u32(&mc.q_full[qb]));
-    };
-    Cursor c, next;
-    c.start(p, q_tiles, total_items);
-    next = c;
-    if (!c.done) {
-      put_queries(next);
-      next.next_item(p);
-    }
-    for (; !c.done && ok; c.next_item(p)) {
-      const Item& w = c.w;
-      bool asked = !next.done;
       for (int j = 0; j < w.n_tiles && ok; ++j, ++gt) {
         if (!mbar_wait(smem_u32(&mc.v_full[vs]), vpar) || (ok && !mbar_wait(smem_u32(&mc.h_empty[hs]), hpar)) || *abort_s) {
           if (!*abort_s) gb_err::report(ERR_WAIT_FULL);
@@ -506,12 +470,11 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         const bool readable = key >= w.lo && key <= w.hi && mc.scales[gt % SLOTS][x >> 4].x >= 0.f;
         const uint8_t* from = smem_raw + S::V_AT + vs * S::CODE_BYTES;
         uint8_t* to = smem_raw + S::H_AT + hs * S::H_BYTES;
-        uint4 code[HD / 16];
-#pragma unroll
-        for (int i = 0; i < HD / 16; ++i) code[i] = *reinterpret_cast<const uint4*>(from + swizzled<HD>(x, i));
-#pragma unroll
+        const uint32_t keep = readable ? 0xffffffffu : 0u;
+#pragma unroll 2
         for (int i = 0; i < HD / 16; ++i) {          // sixteen channels: two chunks of halves
-          const uint32_t u[4] = {readable ? code[i].x : 0u, readable ? code[i].y : 0u, readable ? code[i].z : 0u, readable ? code[i].w : 0u};
+          const uint4 code = *reinterpret_cast<const uint4*>(from + swizzled<HD>(x, i));
+          const uint32_t u[4] = {code.x & keep, code.y & keep, code.z & keep, code.w & keep};
           uint32_t h[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) h[2 * e] = f8::decode2_f16(u[e] & 0xFFFFu), h[2 * e + 1] = f8::decode2_f16(u[e] >> 16);
@@ -524,205 +487,92 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         mbar_arrive(smem_u32(&mc.h_full[hs]));
         if (++vs == V_STAGES) vs = 0, vpar ^= 1;
         if (++hs == H_STAGES) hs = 0, hpar ^= 1;
-        if (asked && (j == 1 || j + 1 == w.n_tiles)) {
-          put_queries(next);
-          next.next_item(p);
-          asked = false;
-        }
       }
     }
   } else {
     // -------------------------------------------------------------------- softmax warps
-    // Group g takes keys [g * 64, g * 64 + 64) of every tile: an attention stream of its own
-    // (reference maximum, denominator, accumulator), merged with the other group's at the end.
-    // Two groups put two warps on every scheduler, so that one computes while the other waits
-    // for tensor memory.
+    // Warps 4-7 have the first half's rows, 8-11 the second's: a thread a row.
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
-    const int grp = (warp - 4) >> 2;
+    const int half = (warp - 4) >> 2;
     const int quarter = warp & 3;                        // the TMEM lanes this warp may read
-    const int row = quarter * 32 + lane;
+    const int row = half * HALF + quarter * 32 + lane;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t o_mine = lane_addr + O_COL0 + grp * HD;
-    bool ok = true;       // false: this thread only keeps the others company at the barriers
-    int gt = 0;           // tiles so far, over all items
-    int sb = 0, sph = 0;          // the current tile's S buffer and the phase of its barriers
-    int kstage = 0;               // the current tile's stage of keys
-    int kpar = 0;
-    int hprev = 0, hstage = 0;    // the values' stages of the tile before and of the current one
-    const bool passes_on = threadIdx.x == 128;     // one thread tells the TMA warp what the tensor core has finished with
-    Cursor c;
-    for (c.start(p, q_tiles, total_items); !c.done; c.next_item(p)) {
-      const Item& w = c.w;
-      const int row_pos = row < w.nrows ? w.pos0 + row / p.g : -1;       // no key is valid for a padding row
-      const int row_start = (row < w.nrows && p.window > 0) ? max(0, row_pos + 1 - p.window) : 0;
-      float m = -INFINITY, l = 0.f;      // m: the reference maximum, in powers of two
-      float vref = -200.f;               // log2 of the vs in whose units the sums are
-      float factor = 0.f;
-
-      // waits until the P V products of the tile counted t have ended
-      auto wait_o = [&](int t) {
-        if (!mbar_wait(smem_u32(&mc.o_ready), t & 1)) {
-          if (lane == 0) gb_err::report(ERR_WAIT_ACCUM);
-          ok = false;
-          *abort_s = 1;
+    const uint32_t s_addr = lane_addr + half * KT, o_addr = lane_addr + O_COL0 + half * HD;
+    bool ok = true;
+    int gt = 0, sph = 0, oph = 0;          // tiles so far (all items' and both halves'), phases of s_ready and o_ready
+    bool ran_out = false;
+    // The queries of an item as codes: this warp's 32 rows, eight channels a lane. (Nobody reads the old ones any more: the product of the
+    // half's last tile has been waited for.)
+    auto put_queries = [&](const Cursor& at) {
+      const Item& w = at.w;
+      if (at.done || w.nrows <= half * HALF) return;
+      constexpr int LANES = HD / 8, ROWS = 32 / LANES, BATCH = 8;          // lanes of a row, rows of a load
+      const int sub = lane % LANES, row0 = half * HALF + quarter * 32 + lane / LANES;
+      const int own_row = (w.q_begin + w.tok0 + row / p.g) * p.Hq + w.kvh * p.g + row % p.g;          // of `q`
+#pragma unroll 1
+      for (int i0 = 0; i0 < 32 / ROWS; i0 += BATCH) {
+        uint4 raw[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+          const int from = __shfl_sync(0xffffffffu, own_row, (i0 + i) * ROWS + lane / LANES);
+          raw[i] = row0 + (i0 + i) * ROWS < w.nrows ? *reinterpret_cast<const uint4*>(p.q + (size_t)from * HD + sub * 8) : make_uint4(0u, 0u, 0u, 0u);
         }
-        tc_fence_after_sync();
-      };
-
-      for (int j = 0; j < w.n_tiles && ok; ++j, ++gt) {
-        if (*abort_s) { ok = false; break; }
-        if (!mbar_wait(smem_u32(&mc.s_ready[sb]), sph)) {
-          if (lane == 0) gb_err::report(ERR_WAIT_ACCUM);
-          ok = false;
-          *abort_s = 1;
-          break;
-        }
-        mbar_wait(smem_u32(&mc.k_full[kstage]), kpar);        // (over already: the scales were written before it)
-        tc_fence_after_sync();
-        const uint32_t s_addr = lane_addr + sb * KT + grp * GK;
-        // the row's 64 scores of this group, one wait for the two loads
-        uint32_t sv[GK / 32][32];
 #pragma unroll
-        for (int h = 0; h < GK / 32; ++h) tmem_ld_32(s_addr + h * 32, sv[h]);
-        if (j == 0) factor = mc.factor[c.it & 1][row];
-        float f[4], ev[4];            // of each sixteen keys: the scores' factor, log2 of vs
-        bool pages = true;
+        for (int i = 0; i < BATCH; ++i) {
+          const int qr = row0 + (i0 + i) * ROWS;
+          const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+          float v[8], largest = 0.f;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const float2 two = mc.scales[gt % SLOTS][grp * 4 + b];
-          f[b] = two.x * factor, ev[b] = two.x >= 0.f ? two.y : -200.f;
-          pages = pages && two.x >= 0.f;
-        }
-        const int hcur = hstage;
-        if (++hstage == H_STAGES) hstage = 0;
-        const int tile_key0 = (w.tile_begin + j) * KT;
-        tmem_ld_wait();
-        if (passes_on) {      // S of this tile is complete: its keys have been read, and after an item's last tile its queries
-          mbar_arrive(smem_u32(&mc.k_empty[kstage]));
-          if (j == w.n_tiles - 1) mbar_arrive(smem_u32(&mc.q_empty[c.it & 1]));
-        }
-        if (++kstage == K_STAGES) kstage = 0, kpar ^= 1;
-        auto sc = [&](int ch) -> float& { return reinterpret_cast<float&>(sv[ch >> 5][ch & 31]); };
-        const int key0 = tile_key0 + grp * GK;
-        // the keys need no mask if they lie wholly before the first row's position and inside the
-        // last row's window
-        const bool full = pages && key0 + GK - 1 <= w.pos0 && (p.window <= 0 || key0 >= w.hi + 1 - p.window);
-        if (!full) {
-#pragma unroll
-          for (int ch = 0; ch < GK; ++ch)
-            if (!(key0 + ch >= row_start && key0 + ch <= row_pos && f[ch >> 4] >= 0.f)) sc(ch) = -INFINITY;
-          // (a factor must not turn a masked score's sign)
-#pragma unroll
-          for (int b = 0; b < 4; ++b) f[b] = fmaxf(f[b], 0x1p-126f);
-        }
-        // the maximum of each sixteen keys' raw products, times their factor
-        float m_new = m;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          float mx = max3(sc(16 * b), sc(16 * b + 1), sc(16 * b + 2));
-#pragma unroll
-          for (int ch = 3; ch < 15; ch += 2) mx = max3(mx, sc(16 * b + ch), sc(16 * b + ch + 1));
-          mx = fmaxf(mx, sc(16 * b + 15));
-          m_new = fmaxf(m_new, mx * f[b]);
-        }
-        const float ev_top = fmaxf(fmaxf(ev[0], ev[1]), fmaxf(ev[2], ev[3]));
-        // The reference maximum moves only if some row of the warp has outgrown it by more than
-        // 2^8; then the warp rescales what it has accumulated (the loads and stores of tensor
-        // memory are the whole warp's). A row that has seen no valid key yet has nothing to rescale.
-        const bool grown = (m != -INFINITY && m_new - m > RESCALE_ABOVE) || ev_top > vref;
-        bool waited = false;
-        if (j > 0 && __any_sync(0xffffffffu, grown)) {
-          wait_o(gt - 1);
-          waited = true;
-          if (!ok) break;
-          const float own = m == -INFINITY ? 1.f : fast_exp2(m - m_new);
-          const float v_new = fmaxf(vref, ev_top), corr = own * fast_exp2(vref - v_new);
-          vref = v_new;
-#pragma unroll
-          for (int h = 0; h < HD / 32; ++h) {
-            uint32_t v[32];
-            tmem_ld_32(o_mine + h * 32, v);
-            tmem_ld_wait();
-#pragma unroll
-            for (int ch = 0; ch < 32; ++ch) v[ch] = __float_as_uint(__uint_as_float(v[ch]) * corr);
-            tmem_st_32(o_mine + h * 32, v);
+          for (int e = 0; e < 4; ++e) {
+            v[2 * e] = __uint_as_float(u[e] << 16), v[2 * e + 1] = __uint_as_float(u[e] & 0xFFFF0000u);
+            largest = max3(largest, fabsf(v[2 * e]), fabsf(v[2 * e + 1]));
           }
-          l *= own;
-          m = m_new;
-        } else {
-          if (m == -INFINITY) m = m_new;
-          vref = fmaxf(vref, ev_top);          // (j > 0: it is the larger one already)
-        }
-        const float neg_m = m == -INFINITY ? 0.f : -m;       // nothing valid yet: avoid inf - inf
-        // All exponentials first, in place (the unit that computes them takes a warp's instruction
-        // every eight cycles; the multiply-adds in front fit in between), then sums and packing.
-        // (2^-100 of the largest vs is nothing; and where nothing is read the probabilities are zeros.)
-        float up[4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) up[b] = UP + fminf(fmaxf(ev[b] - vref, -100.f), 0.f);
+          for (int o = LANES / 2; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+          const int e2 = f8::scale_exponent(largest);
+          const float inv = f8::power_of_two(-e2);
+          uint32_t hi[2], lo[2];
 #pragma unroll
-        for (int ch = 0; ch < GK; ++ch) sc(ch) = fast_exp2(fmaf(sc(ch), f[ch >> 4], neg_m + up[ch >> 4]));   // exp2(-inf) = 0 for masked keys
-        uint32_t pk[GK / 2];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          float ls[2] = {0.f, 0.f};
-#pragma unroll
-          for (int ch = 16 * b; ch < 16 * b + 16; ch += 2) {
-            ls[(ch >> 1) & 1] += sc(ch) + sc(ch + 1);
-            pk[ch >> 1] = pack_f16(sc(ch), sc(ch + 1));
+          for (int e = 0; e < 2; ++e) {
+            const float a = v[4 * e] * inv, b = v[4 * e + 1] * inv, d = v[4 * e + 2] * inv, f = v[4 * e + 3] * inv;
+            hi[e] = f8::encode4(a, b, d, f);
+            const float4 back = f8::decode4(hi[e]);
+            lo[e] = f8::encode4(a - back.x, b - back.y, d - back.z, f - back.w);
           }
-          l = fmaf(ls[0] + ls[1], fast_exp2(-up[b]), l);          // without vs
+          uint8_t* to = smem_raw + swizzled<HD>(qr, sub >> 1) + (sub & 1) * 8;
+          *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
+          *reinterpret_cast<uint2*>(to + QROWS * HD) = make_uint2(lo[0], lo[1]);
+          if (sub == 0) mc.factor[qr] = f8::power_of_two(e2) * p.scale_log2;
         }
-        tmem_st(s_addr, pk);            // over the first half of the scores just read
-        tmem_st_wait();
-        if (j > 0 && !waited) wait_o(gt - 1);      // every phase of the barrier is seen, in order
-        tc_fence_before_sync();         // this thread's accesses to tensor memory are over
-        mbar_arrive(smem_u32(&mc.p_ready[sb]));
-        if (passes_on && j > 0) mbar_arrive(smem_u32(&mc.h_empty[hprev]));      // the tile before: its P V has ended
-        hprev = hcur;
-        if (++sb == S_BUFS) sb = 0, sph ^= 1;
       }
-      if (ok && w.n_tiles > 0) {
-        wait_o(gt - 1);
-        if (passes_on && ok) mbar_arrive(smem_u32(&mc.h_empty[hprev]));
-      }
-      // ---- merge the groups: each writes its share of the channels, summed over all accumulators
-      mc.ml[grp][row] = make_float2(m, l);
-      if (row == 0) mc.vref[grp] = vref;
-      tc_fence_before_sync();
-      asm volatile("bar.sync 1, %0;" ::"n"(GROUPS * 128) : "memory");
-      tc_fence_after_sync();
-      if (ok && !*abort_s) {
-        float a[GROUPS];
-        float mt = -INFINITY, lt = 0.f;
-#pragma unroll
-        for (int g = 0; g < GROUPS; ++g) mt = fmaxf(mt, mc.ml[g][row].x);
-#pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-          const float2 x = mc.ml[g][row];
-          const float own = x.x == -INFINITY ? 0.f : fast_exp2(x.x - mt);
-          lt += own > 0.f || x.y != x.y ? x.y * own : 0.f;        // (a score that is no number stays one)
-          a[g] = own * fast_exp2(mc.vref[g] - UP);
-        }
-        const float inv = lt > 0.f ? 1.0f / lt : lt == lt ? 0.f : lt;
-        __nv_bfloat16* dst = p.out + ((size_t)(w.q_begin + w.tok0 + row / p.g) * p.Hq + w.kvh * p.g + row % p.g) * HD + grp * S::CH;
-#pragma unroll
-        for (int h = 0; h < S::CH / 16; ++h) {
+      fence_proxy_async();              // the tensor core reads them through the async proxy
+      mbar_arrive(smem_u32(&mc.q_full[half]));
+      __syncwarp();
+    };
+    Cursor next;                           // the item after the current one
+    next.start(p, q_tiles, total_items);
+    gb::pdl_wait();
+    Item w{};                              // the current one
+    int n = 0;                             // its tiles of this half
+    float m = -INFINITY, l = 0.f;          // the reference maximum, in powers of two; the denominator
+    float vref = -200.f;                   // log2 of the vs in whose units the sums are
+    while (ok) {
+      put_queries(next);
+      // ---- write the current one out
+      if (n > 0) {
+        if (!(ok = mbar_wait_warp(smem_u32(&mc.o_ready[half]), oph, abort_s, ran_out))) break;
+        oph ^= 1;
+        tc_fence_after_sync();
+        const float inv = l > 0.f ? fast_exp2(vref - UP) / l : l == l ? 0.f : l;        // (a score that is no number stays one)
+        __nv_bfloat16* dst = p.out + ((size_t)(w.q_begin + w.tok0 + row / p.g) * p.Hq + w.kvh * p.g + row % p.g) * HD;
+#pragma unroll 2
+        for (int h = 0; h < HD / 16; ++h) {
+          uint32_t v[16];
+          tmem_ld_16(o_addr + h * 16, v);
+          tmem_ld_wait();
           float t[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) t[e] = lt == lt ? 0.f : lt;
-#pragma unroll
-          for (int g = 0; g < GROUPS; g += 2) {      // two accumulators at a time (registers)
-            uint32_t v[2][16];
-            tmem_ld_16(lane_addr + O_COL0 + g * HD + grp * S::CH + h * 16, v[0]);
-            tmem_ld_16(lane_addr + O_COL0 + (g + 1) * HD + grp * S::CH + h * 16, v[1]);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {      // a stream without a valid key has an accumulator that means nothing
-              t[e] += a[g] > 0.f ? __uint_as_float(v[0][e]) * (a[g] * inv) : 0.f;
-              t[e] += a[g + 1] > 0.f ? __uint_as_float(v[1][e]) * (a[g + 1] * inv) : 0.f;
-            }
-          }
+          for (int e = 0; e < 16; ++e) t[e] = __uint_as_float(v[e]) * inv;
           if (row < w.nrows) {
             uint4 w0, w1;
             w0.x = pack_bf16(t[0], t[1]), w0.y = pack_bf16(t[2], t[3]), w0.z = pack_bf16(t[4], t[5]), w0.w = pack_bf16(t[6], t[7]);
@@ -731,12 +581,123 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
             *reinterpret_cast<uint4*>(dst + h * 16 + 8) = w1;
           }
         }
+        tc_fence_before_sync();
+        mbar_arrive(smem_u32(&mc.o_free[half]));
       }
-      // The next item's first P V overwrites the accumulators; it is issued only after all groups
-      // have arrived for that tile, that is after all are through here. A
-      // group must not write the next item's values while another still reads these.
-      asm volatile("bar.sync 1, %0;" ::"n"(GROUPS * 128) : "memory");
-      tc_fence_before_sync();
+      if (next.done) break;
+      w = next.w, n = w.tiles_of(half, p.g);
+      next.next_item(p);
+      m = -INFINITY, l = 0.f, vref = -200.f;
+      const int row_pos = row < w.nrows ? w.pos0 + row / p.g : -1;       // no key is valid for a padding row
+      const int row_start = (row < w.nrows && p.window > 0) ? max(0, row_pos + 1 - p.window) : 0;
+      // what all rows of this half read: up to the first row's position, from the last row's window on
+      const int half_lo = w.pos0 + half * HALF / p.g, half_hi = w.pos0 + (min(w.nrows, half * HALF + HALF) - 1) / p.g;
+      float factor = 0.f;
+      for (int j = 0; j < w.n_tiles; ++j, ++gt) {
+        if (j >= n) continue;            // keys that only the other half reads
+        if (!(ok = mbar_wait_warp(smem_u32(&mc.s_ready[half]), sph, abort_s, ran_out))) break;
+        sph ^= 1;
+        tc_fence_after_sync();
+        if (j == 0) factor = mc.factor[row];
+        uint32_t sv[KT / 32][32];
+#pragma unroll
+        for (int h = 0; h < KT / 32; ++h) tmem_ld_32(s_addr + h * 32, sv[h]);
+        float f[8], ev[8], ev_top = -200.f;            // of each sixteen keys: the scores' factor, log2 of vs
+        bool pages = true;
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+          const float2 two = mc.scales[gt % SLOTS][b];
+          f[b] = two.x * factor, ev[b] = two.x >= 0.f ? two.y : -200.f;
+          pages = pages && two.x >= 0.f;
+          ev_top = fmaxf(ev_top, ev[b]);
+        }
+        tmem_ld_wait();
+        auto sc = [&](int ch) -> float& { return reinterpret_cast<float&>(sv[ch >> 5][ch & 31]); };
+        const int key0 = (w.tile_begin + j) * KT;
+        // the keys need no mask if they lie wholly before the first row's position and inside the last row's window
+        const bool full = pages && key0 + KT - 1 <= half_lo && (p.window <= 0 || key0 >= half_hi + 1 - p.window);
+        if (!full) {
+#pragma unroll
+          for (int h = 0; h < KT / 32; ++h) {          // 32 keys: an interval of bits, less the pages that are not there
+            const int first = max(row_start - key0 - 32 * h, 0), end = min(row_pos + 1 - key0 - 32 * h, 32);
+            uint32_t bits = end > first ? (0xffffffffu >> (32 - end)) & (0xffffffffu << first) : 0u;
+            if (f[2 * h] < 0.f) bits &= 0xffff0000u;
+            if (f[2 * h + 1] < 0.f) bits &= 0x0000ffffu;
+#pragma unroll
+            for (int ch = 0; ch < 32; ++ch)
+              if (!(bits >> ch & 1)) sv[h][ch] = 0xff800000u;          // -inf
+          }
+          // (a factor must not turn a masked score's sign)
+#pragma unroll
+          for (int b = 0; b < 8; ++b) f[b] = fmaxf(f[b], 0x1p-126f);
+        }
+        // the maximum of each sixteen keys' raw products, times their factor
+        float m_new = m;
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+          float mx = max3(sc(16 * b), sc(16 * b + 1), sc(16 * b + 2));
+#pragma unroll
+          for (int ch = 3; ch < 15; ch += 2) mx = max3(mx, sc(16 * b + ch), sc(16 * b + ch + 1));
+          mx = fmaxf(mx, sc(16 * b + 15));
+          m_new = fmaxf(m_new, mx * f[b]);
+        }
+        // The reference maximum moves only if some row of the warp has outgrown it by more than 2^8; then the warp rescales what it has
+        // accumulated (the loads and stores of tensor memory are the whole warp's). A row that has seen no valid key yet has
+        // nothing to rescale.
+        const bool grown = (m != -INFINITY && m_new - m > RESCALE_ABOVE) || ev_top > vref;
+        if (j > 0 && __any_sync(0xffffffffu, grown)) {
+          const float own = m == -INFINITY ? 1.f : fast_exp2(m - m_new);
+          const float v_new = fmaxf(vref, ev_top), corr = own * fast_exp2(vref - v_new);
+          vref = v_new;
+#pragma unroll 1
+          for (int h = 0; h < HD / 16; ++h) {
+            uint32_t v[16];
+            tmem_ld_16(o_addr + h * 16, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int ch = 0; ch < 16; ++ch) v[ch] = __float_as_uint(__uint_as_float(v[ch]) * corr);
+            tmem_st_16(o_addr + h * 16, v);
+          }
+          l *= own;
+          m = m_new;
+        } else {
+          if (m == -INFINITY) m = m_new;
+          vref = fmaxf(vref, ev_top);          // (j > 0: it is the larger one already)
+        }
+        const float neg_m = m == -INFINITY ? 0.f : -m;       // nothing valid yet: avoid inf - inf
+        // (2^-100 of the largest vs is nothing; and where nothing is read the probabilities are zeros.)
+#pragma unroll
+        for (int h = 0; h < KT / 32; ++h) {                  // 32 keys: 16 columns of P, over scores that have been read
+          uint32_t pk[16];
+#pragma unroll
+          for (int b = 2 * h; b < 2 * h + 2; ++b) {
+            const float up = UP + fminf(fmaxf(ev[b] - vref, -100.f), 0.f), off = neg_m + up;
+            const float2 f2 = make_float2(f[b], f[b]), off2 = make_float2(off, off);
+            float2 ls = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int ch = 16 * b; ch < 16 * b + 16; ch += 2) {
+              float2 y = fma2(make_float2(sc(ch), sc(ch + 1)), f2, off2);
+              y.x = fast_exp2(y.x), y.y = fast_exp2(y.y);                     // exp2(-inf) = 0 for masked keys
+              ls = add2(ls, y);
+              pk[(ch >> 1) - 16 * h] = pack_f16(y.x, y.y);
+            }
+            l = fmaf(ls.x + ls.y, fast_exp2(-up), l);          // without vs
+          }
+          tmem_st_16(s_addr + h * 16, pk);
+          if (h == 1) {
+            tmem_st_wait();
+            tc_fence_before_sync();       // this thread's accesses to tensor memory are over
+            mbar_arrive(smem_u32(&mc.p_ready[half][0]));
+          }
+        }
+        tmem_st_wait();
+        tc_fence_before_sync();
+        mbar_arrive(smem_u32(&mc.p_ready[half][1]));
+      }
+    }
+    if (!ok) {
+      if (ran_out) gb_err::report(ERR_WAIT_ACCUM);
+      *abort_s = 1;
     }
   }
   tc_fence_before_sync();
@@ -804,7 +765,7 @@ int launch(const Params& p, const CUtensorMap& km, const CUtensorMap& vm, int q_
 
 }  // namespace
 
-// Heads of 64 or 128, pages of 16, 32, 64 or 128 keys, up to 128 query heads a group; for requests of more than decode_rows(g) rows (new tokens
+// Heads of 64 or 128, pages of 16, 32, 64 or 128 keys, up to 256 query heads a group; for requests of more than decode_rows(g) rows (new tokens
 // times heads of a group), the others are left.
 GB_EXPORT int gb_f8_attention_tile(const void* q, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale, const void* table,
                                    int table_width, const void* cu_q, const void* kv_lens, void* out, int R, long long pages, int Hq, int Hkv, int hd,
