@@ -151,24 +151,29 @@ struct Append {
   bool interleaved;
 };
 
-constexpr int APPEND_THREADS = 256, APPEND_WARPS = APPEND_THREADS / 32;
+constexpr int APPEND_THREADS = 256;
 constexpr int KEPT = 4;         // rows of keys and of values that a thread keeps in registers between their maximum and their codes
+constexpr int QUERIES = 4;      // heads of a piece of queries
 
-// KEEP: a page's rows fit the block's registers (page * head size <= 4,096: 32 keys of 128 channels): read once; else they are read twice.
-// Lanes lie along a row (four channels each; short rows share a warp), warps take the rows in turn. The queries of a page's tokens have
-// blocks of their own (blockIdx.y from Hkv on, `QUERIES` heads each): they wait for no maximum.
-constexpr int QUERIES = 4;
-template <typename TI, typename TO, bool KEEP>
-__global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const Append p) {
+// A piece of work is one head of a page's keys and values, or QUERIES heads of its tokens' queries (they wait for no maximum); WARPS of a
+// block have one. Lanes lie along a row (four channels each; short rows share a warp), a piece's warps take the rows in turn. KEEP: a
+// thread's first KEPT rows are read once, and with eight warps these are all (page * head size <= 4,096: 32 keys of 128 channels; else,
+// and what a single warp has beyond them, is read twice).
+template <typename TI, typename TO, bool KEEP, int WARPS>
+__global__ void __launch_bounds__(APPEND_THREADS, WARPS == 1 ? 2 : 4) append_kernel(const Append p) {
   gb::pdl_launch_dependents();
-  __shared__ float part[2][APPEND_WARPS];
-  // the request of this block: the last one that starts at or before it
-  int lo = 0, hi = p.R;
+  __shared__ float part[2][WARPS];
+  const int lane = threadIdx.x & 31, warp = WARPS == 1 ? 0 : threadIdx.x >> 5, thread = WARPS == 1 ? lane : threadIdx.x;       // of the piece
+  const int piece = WARPS == 1 ? blockIdx.y * (APPEND_THREADS / 32) + (threadIdx.x >> 5) : blockIdx.y;
+  if (piece >= p.Hkv + (p.Hq + QUERIES - 1) / QUERIES) return;
+  // the request of this page: the last one that starts at or before it, found by 32 lanes at a time
+  int lo = 0;
   const int slot = blockIdx.x;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.cu_q[mid] / p.page + 2 * mid <= slot) lo = mid;
-    else hi = mid;
+  for (int left = p.R; left > 1;) {
+    const int apart = (left + 31) / 32, i = lo + lane * apart;
+    const bool before = lane * apart < left && p.cu_q[i] / p.page + 2 * i <= slot;
+    const int skip = max(__popc(__ballot_sync(0xffffffffu, before)) - 1, 0) * apart;
+    lo += skip, left = min(apart, left - skip);
   }
   const int r = lo, begin = p.cu_q[r], q_len = p.cu_q[r + 1] - begin;
   const int pos0 = p.kv_lens[r] - q_len;
@@ -182,14 +187,13 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const Append 
   const int half = p.hd / 2, fours = p.hd / 4;
   const bool rotated = p.cos_sin != nullptr, split = rotated && !p.interleaved;
   // this thread's place: row `row0` of every `step`, channels 4 j0 (and, in rows of more than 128, 4 (j0 + 32))
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int shared = fours == 16 ? 2 : fours == 8 ? 4 : fours == 4 ? 8 : 1;          // rows of a warp
-  const int row0 = warp * shared + (shared > 1 ? lane / fours : 0), step = APPEND_WARPS * shared;
+  const int row0 = warp * shared + (shared > 1 ? lane / fours : 0), step = WARPS * shared;
   const int j0 = shared > 1 ? lane % fours : lane;
   const TI* rows = reinterpret_cast<const TI*>(p.qkv) + tok0 * p.qkv_stride;
   const float* angles = p.cos_sin + (size_t)tok0 * p.hd;
-  if (blockIdx.y >= p.Hkv) {
-    const int h0 = ((int)blockIdx.y - p.Hkv) * QUERIES, heads = min(QUERIES, p.Hq - h0);
+  if (piece >= p.Hkv) {
+    const int h0 = (piece - p.Hkv) * QUERIES, heads = min(QUERIES, p.Hq - h0);
     TO* const q_out = reinterpret_cast<TO*>(p.q_out) + ((size_t)tok0 * p.Hq + h0) * p.hd;
     gb::pdl_wait();
 #pragma unroll 4
@@ -205,7 +209,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const Append 
     }
     return;
   }
-  const int kvh = blockIdx.y;
+  const int kvh = piece;
   if (at < 0) return;
   const TI* keys = rows + (size_t)(p.Hq + kvh) * p.hd;
   const TI* values = keys + (size_t)p.Hkv * p.hd;
@@ -229,18 +233,24 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const Append 
         mk = fmaxf(mk, largest_of(ks[i])), mv = fmaxf(mv, largest_of(vs[i]));
       }
     }
-  } else {
-    for (int t = row0; t < n; t += step)
+  }
+  const int again = KEEP ? row0 + KEPT * step : row0;          // the first row that is read twice
+  if (!KEEP || WARPS == 1) {
+    for (int t = again; t < n; t += step)
       for (int j = j0; j < fours; j += 32) mk = fmaxf(mk, largest_of(key(t, j))), mv = fmaxf(mv, largest_of(value(t, j)));
   }
   mk = gb::warp_max(mk), mv = gb::warp_max(mv);
-  if (lane == 0) part[0][warp] = mk, part[1][warp] = mv;
-  __syncthreads();
-  mk = part[0][0], mv = part[1][0];
+  if (WARPS > 1) {
+    if (lane == 0) part[0][warp] = mk, part[1][warp] = mv;
+    __syncthreads();
+    mk = part[0][0], mv = part[1][0];
 #pragma unroll
-  for (int w = 1; w < APPEND_WARPS; ++w) mk = fmaxf(mk, part[0][w]), mv = fmaxf(mv, part[1][w]);
+    for (int w = 1; w < WARPS; ++w) mk = fmaxf(mk, part[0][w]), mv = fmaxf(mv, part[1][w]);
+  } else {
+    __syncwarp();          // (every lane has read the old scales)
+  }
   const float sk = fmaxf(old_k, power_of_two(scale_exponent(mk))), sv = fmaxf(old_v, power_of_two(scale_exponent(mv)));
-  if (threadIdx.x == 0) p.k_scale[where] = sk, p.v_scale[where] = sv;       // (every thread has read the old ones)
+  if (thread == 0) p.k_scale[where] = sk, p.v_scale[where] = sv;       // (every thread has read the old ones)
   uint8_t* kp = p.k_pool + where * p.page * p.hd;
   uint8_t* vp = p.v_pool + where * p.page * p.hd;
   // the scale has grown: the rows that were there are encoded again
@@ -250,7 +260,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const Append 
     uint32_t* codes = reinterpret_cast<uint32_t*>(which ? vp : kp);
     const float factor = old / s;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < held * fours; i += APPEND_THREADS) {
+    for (int i = thread; i < held * fours; i += 32 * WARPS) {
       const float4 x = decode4(codes[i]);
       codes[i] = encode4(x.x * factor, x.y * factor, x.z * factor, x.w * factor);
     }
@@ -265,8 +275,9 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const Append 
         store_codes(vp + (size_t)(held + t) * p.hd, vs[i], iv, j0, half, false);
       }
     }
-  } else {
-    for (int t = row0; t < n; t += step)
+  }
+  if (!KEEP || WARPS == 1) {
+    for (int t = again; t < n; t += step)
       for (int j = j0; j < fours; j += 32) {
         store_codes(kp + (size_t)(held + t) * p.hd, key(t, j), ik, j, half, split);
         store_codes(vp + (size_t)(held + t) * p.hd, value(t, j), iv, j, half, false);
@@ -414,9 +425,14 @@ GB_EXPORT int gb_f8_append(const void* qkv, int tag, long long qkv_stride, void*
   if (slots > 0x7fffffff) return gb::fail(GB_UNSUPPORTED, "f8_append: %lld pages", slots);
   return GB_DISPATCH_DTYPE(tag, TI, [&]() -> int {
     return GB_DISPATCH_DTYPE(q_tag, TO, [&]() -> int {
-      const int fours = hd / 4, shared = fours == 16 ? 2 : fours == 8 ? 4 : fours == 4 ? 8 : 1;
-      auto* kernel = fours <= 32 && page <= KEPT * APPEND_WARPS * shared ? append_kernel<TI, TO, true> : append_kernel<TI, TO, false>;
-      return gb::check_pdl_launch(gb::launch_pdl(kernel, dim3((unsigned)slots, (unsigned)(Hkv + (Hq + QUERIES - 1) / QUERIES)), dim3(APPEND_THREADS), 0, (cudaStream_t)stream, dim3(1), p),
+      // Single tokens leave a page one row: a warp a piece (64 tokens of 32 + 8 heads of 128: 3.0 us; eight warps, seven of them idle, 7.6).
+      // Else eight (2,047 tokens: 24 us).
+      const int pieces = Hkv + (Hq + QUERIES - 1) / QUERIES, fours = hd / 4, shared = fours == 16 ? 2 : fours == 8 ? 4 : fours == 4 ? 8 : 1;
+      const bool few = T <= R, fits = hd <= 128 && page <= KEPT * (APPEND_THREADS / 32) * shared;
+      auto* kernel = few ? (hd <= 128 ? append_kernel<TI, TO, true, 1> : append_kernel<TI, TO, false, 1>)
+                         : (fits ? append_kernel<TI, TO, true, APPEND_THREADS / 32> : append_kernel<TI, TO, false, APPEND_THREADS / 32>);
+      const dim3 grid((unsigned)slots, few ? (unsigned)(pieces + APPEND_THREADS / 32 - 1) / (APPEND_THREADS / 32) : (unsigned)pieces);
+      return gb::check_pdl_launch(gb::launch_pdl(kernel, grid, dim3(APPEND_THREADS), 0, (cudaStream_t)stream, dim3(1), p),
                                   "f8_append");
     });
   });
