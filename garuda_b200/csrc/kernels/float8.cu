@@ -116,8 +116,8 @@ __device__ __forceinline__ Four load_four(const T* x, int j, int half, bool spli
   f.b = load2(x + (split ? half + 2 * j : 4 * j + 2));
   return f;
 }
-__device__ __forceinline__ void rotate(Four& f, const float* cs, int j, bool split) {
-  const float4 t = *reinterpret_cast<const float4*>(cs + 4 * j);       // cos, sin of pair 2 j, cos, sin of pair 2 j + 1
+// (t: cos, sin of pair 2 j, cos, sin of pair 2 j + 1)
+__device__ __forceinline__ void rotate(Four& f, float4 t, bool split) {
   float& x0 = f.a.x;
   float& y0 = split ? f.b.x : f.a.y;
   float& x1 = split ? f.a.y : f.b.x;
@@ -196,15 +196,23 @@ __global__ void __launch_bounds__(APPEND_THREADS, WARPS == 1 ? 2 : 4) append_ker
     const int h0 = (piece - p.Hkv) * QUERIES, heads = min(QUERIES, p.Hq - h0);
     TO* const q_out = reinterpret_cast<TO*>(p.q_out) + ((size_t)tok0 * p.Hq + h0) * p.hd;
     gb::pdl_wait();
-#pragma unroll 4
-    for (int i = row0; i < n * heads; i += step) {
-      const int t = i / heads, h = i - t * heads;
+#pragma unroll 1
+    for (int t = row0; t < n; t += step) {
       for (int j = j0; j < fours; j += 32) {
-        Four q = load_four(rows + t * p.qkv_stride + (size_t)(h0 + h) * p.hd, j, half, split);
-        if (rotated) rotate(q, angles + (size_t)t * p.hd, j, split);
-        TO* to = q_out + ((size_t)t * p.Hq + h) * p.hd;
-        gb::store_pair(to + (split ? 2 * j : 4 * j), q.a.x, q.a.y);
-        gb::store_pair(to + (split ? half + 2 * j : 4 * j + 2), q.b.x, q.b.y);
+        float4 turn{};          // the heads' one rotation
+        if (rotated) turn = *reinterpret_cast<const float4*>(angles + (size_t)t * p.hd + 4 * j);
+        Four q[QUERIES];
+#pragma unroll
+        for (int h = 0; h < QUERIES; ++h)
+          if (h < heads) q[h] = load_four(rows + t * p.qkv_stride + (size_t)(h0 + h) * p.hd, j, half, split);
+#pragma unroll
+        for (int h = 0; h < QUERIES; ++h) {
+          if (h >= heads) break;
+          if (rotated) rotate(q[h], turn, split);
+          TO* to = q_out + ((size_t)t * p.Hq + h) * p.hd;
+          gb::store_pair(to + (split ? 2 * j : 4 * j), q[h].a.x, q[h].a.y);
+          gb::store_pair(to + (split ? half + 2 * j : 4 * j + 2), q[h].b.x, q[h].b.y);
+        }
       }
     }
     return;
@@ -215,7 +223,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, WARPS == 1 ? 2 : 4) append_ker
   const TI* values = keys + (size_t)p.Hkv * p.hd;
   auto key = [&](int t, int j) {
     Four k = load_four(keys + t * p.qkv_stride, j, half, split);
-    if (rotated) rotate(k, angles + (size_t)t * p.hd, j, split);
+    if (rotated) rotate(k, *reinterpret_cast<const float4*>(angles + (size_t)t * p.hd + 4 * j), split);
     return k;
   };
   auto value = [&](int t, int j) { return load_four(values + t * p.qkv_stride, j, half, false); };
@@ -425,8 +433,8 @@ GB_EXPORT int gb_f8_append(const void* qkv, int tag, long long qkv_stride, void*
   if (slots > 0x7fffffff) return gb::fail(GB_UNSUPPORTED, "f8_append: %lld pages", slots);
   return GB_DISPATCH_DTYPE(tag, TI, [&]() -> int {
     return GB_DISPATCH_DTYPE(q_tag, TO, [&]() -> int {
-      // Single tokens leave a page one row: a warp a piece (64 tokens of 32 + 8 heads of 128: 3.0 us; eight warps, seven of them idle, 7.6).
-      // Else eight (2,047 tokens: 24 us).
+      // Single tokens leave a page one row: a warp a piece (64 tokens of 32 + 8 heads of 128: 2.3 us; eight warps, seven of them idle, 7.6).
+      // Else eight (2,047 tokens: 17 us).
       const int pieces = Hkv + (Hq + QUERIES - 1) / QUERIES, fours = hd / 4, shared = fours == 16 ? 2 : fours == 8 ? 4 : fours == 4 ? 8 : 1;
       const bool few = T <= R, fits = hd <= 128 && page <= KEPT * (APPEND_THREADS / 32) * shared;
       auto* kernel = few ? (hd <= 128 ? append_kernel<TI, TO, true, 1> : append_kernel<TI, TO, false, 1>)
