@@ -126,15 +126,20 @@ __device__ __forceinline__ bool any_of_four(bool mine) {
       : "=r"(r) : "r"((uint32_t)mine) : "memory");
   return r != 0;
 }
-__device__ __forceinline__ void st_async_v4(uint32_t addr, uint32_t bar, float a, float b, float c, float d) {
-  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%2, %3, %4, %5}, [%1];"
-               ::"r"(addr), "r"(bar), "r"(__float_as_uint(a)), "r"(__float_as_uint(b)), "r"(__float_as_uint(c)), "r"(__float_as_uint(d))
-               : "memory");
+// Into another CTA of the cluster.
+__device__ __forceinline__ void st_cluster_v4(uint32_t addr, float a, float b, float c, float d) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+// The largest of a warp's (of those that are numbers).
+__device__ __forceinline__ float redux_max(float x) {
+  float y;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ void sync_four() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
 
 struct Bars {
-  uint64_t full[12], empty[12], s_ready[2], p_ready[2], pv_done[2], q_ready[2], o_free, part;
+  uint64_t full[12], empty[12], s_ready[2], p_ready[2], pv_done[2], q_ready[2], o_free;
   uint32_t tmem_base;
   int abort, last[2];
   int2 total, scan[6];
@@ -170,7 +175,6 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
       mbar_init(smem_u32(&bars.q_ready[b]), 128);
     }
     mbar_init(smem_u32(&bars.o_free), 32);
-    mbar_init(smem_u32(&bars.part), 1);
     bars.abort = 0, bars.total = make_int2(0, 0);
     fence_barrier_init();
     fence_proxy_async();
@@ -187,7 +191,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
   const uint32_t tmem = bars.tmem_base;
   volatile int* aborted = &bars.abort;
   gb::pdl_launch_dependents();
-  if (CLUSTER) cluster_arrive_wait();      // every barrier is there before another CTA's sums are sent to it
+  if (CLUSTER) cluster_arrive_wait();      // the first CTA is there before sums are sent to it
 
   // ---- every request's tiles (the batch's lengths are there before the step's first kernel)
   struct Span {
@@ -331,12 +335,14 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&bars.full[s]));          // (after what the other lanes wrote)
     };
-    // the first tiles' copies do not wait for their scales
+    // (a tile's copies take a third of a microsecond to ask for, their scales twice that to arrive: the first two tiles', then those)
     const int early = min(min(my_tiles, STAGES), 4);
     look_pages(now, 0);
-    for (int i = 0; i < early; ++i) copy(i, i);
     look_scales(now);
-    for (int i = 0; i < early; ++i) write_scales(i, i);
+    for (int i = 0; i <= early; ++i) {
+      if (i < early) copy(i, i);
+      if (i > 0) write_scales(i - 1, i - 1);
+    }
     look_pages(ahead, 4);
     int s = early % STAGES, par = early == STAGES ? 0 : 1, t = early;
     if (early == 4) look_scales(ahead);
@@ -524,17 +530,17 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
         for (int r = 0; r < ROWS; ++r)
           if (r < w.nrows) more = more || !(v[r] <= m[r] + S::GROWTH);          // (a score that is no number stays one)
         // a score far above the reference (rare after a request's first tiles), or a larger vs: everything is brought to it
-        if (any_of_four(more)) {
+        if (j == 0 || any_of_four(more)) {
           if (j > 0) {
             wait(bars.pv_done[(t - 1) & 1], (t - 1) >> 1);
             tc_fence_after_sync();
           }
-          const float vt = gb::warp_max(ev);
+          const float vt = redux_max(ev);
           if (lane == 0) bars.vtop[sw] = vt;
 #pragma unroll
           for (int r = 0; r < ROWS; ++r)
             if (r < w.nrows) {
-              const float top = gb::warp_max(v[r]);
+              const float top = redux_max(v[r]);
               if (lane == 0) bars.top[sw][r] = top;
             }
           sync_four();
@@ -550,7 +556,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
             l[r] *= corr;
             if (x == r) bars.corr[r] = corr * v_corr;
           }
-          sync_four();
+          sync_four();               // (before the maxima's place is used again, too)
           if (quarter == 0 && j > 0) {             // the sums' rows lie in its lanes: r, r + ROWS, r + 2 ROWS
             const float corr = lane < S::PARTS * ROWS && lane % ROWS < w.nrows ? bars.corr[lane % ROWS] : 1.f;
 #pragma unroll
@@ -617,7 +623,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
         __nv_bfloat16* const dst = p.out + ((size_t)(w.q_begin + r / p.g) * p.Hq + g.kvh * p.g + r % p.g) * HD;
         float* const part = partials + ((size_t)cta * 2 + (a == a_begin ? 0 : 1)) * (MAX_ROWS * RS) + r * RS;
         float* const own_part = reinterpret_cast<float*>(base + S::PARTS_AT) + (rank * ROWS + r) * S::RC;
-        const uint32_t to = CLUSTER ? map_to_rank(smem_u32(own_part), 0) : 0, to_bar = CLUSTER ? map_to_rank(smem_u32(&bars.part), 0) : 0;
+        const uint32_t to = CLUSTER ? map_to_rank(smem_u32(own_part), 0) : 0;
 #pragma unroll
         for (int h = 0; h < HD / 16; ++h) {
           uint32_t o[16];
@@ -634,10 +640,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
           }
           if (CLUSTER && mine && !whole) {
 #pragma unroll
-            for (int c = 0; c < 16; c += 4) {
-              if (rank == 0) *reinterpret_cast<float4*>(own_part + h * 16 + c) = make_float4(y[c], y[c + 1], y[c + 2], y[c + 3]);
-              else st_async_v4(to + (h * 16 + c) * 4, to_bar, y[c], y[c + 1], y[c + 2], y[c + 3]);
-            }
+            for (int c = 0; c < 16; c += 4) st_cluster_v4(to + (h * 16 + c) * 4, y[c], y[c + 1], y[c + 2], y[c + 3]);
           } else if (mine) {
 #pragma unroll
             for (int c = 0; c < 16; c += 2) {
@@ -647,8 +650,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
           }
         }
         if (CLUSTER && mine && !whole) {
-          if (rank == 0) *reinterpret_cast<float4*>(own_part + HD) = make_float4(mr, ll, 0.f, 0.f);
-          else st_async_v4(to + HD * 4, to_bar, mr, ll, 0.f, 0.f);
+          st_cluster_v4(to + HD * 4, mr, ll, 0.f, 0.f);
         } else if (mine && !whole) {
           __stcg(reinterpret_cast<float2*>(part + HD), make_float2(mr, ll));
         }
@@ -665,8 +667,13 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
       now = next, next = later;
     }
     // ---- segments of several CTAs: who counts the last arrival adds the parts up, in the CTAs' order
-    if (CLUSTER && rank != 0) n_shared = 0;
-    if (n_shared > 0) sync_four();     // the parts are written
+    if (CLUSTER) {
+      __syncwarp();
+      cluster_arrive_wait();           // (every thread of the cluster once, the others at the kernel's end; every wait in front of it is bounded)
+      if (rank != 0) n_shared = 0;
+    } else if (n_shared > 0) {
+      sync_four();                     // the parts are written
+    }
     int c0[2] = {0, 0}, c1[2] = {0, 0};
     bool behind[2] = {false, false};   // whether the first of them has another segment's end in front of its part
 #pragma unroll
@@ -678,10 +685,6 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
       c0[i] = c / stretch, c1[i] = (c + g.n - 1) / stretch;
       behind[i] = begins_at(c0[i]) < cum[g.r] * p.Hkv + g.kvh * g.n;
     }
-    if (CLUSTER && n_shared > 0) {         // the others' rows
-      if (x == 0) mbar_arrive_expect_tx(smem_u32(&bars.part), c1[0] * shared[0].nrows * S::RC * 4);
-      wait(bars.part, 0);
-    }
     if (!CLUSTER && x < n_shared) {
       __threadfence();
       const Segment& g = x == 0 ? shared[0].g : shared[1].g;
@@ -691,7 +694,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
       bars.last[x] = last;
       __threadfence();
     }
-    if (n_shared > 0) sync_four();
+    if (!CLUSTER && n_shared > 0) sync_four();
     constexpr int LANES = 128 / ROWS, PER = HD / LANES / 2;          // threads of a row, pairs of channels of a thread
     const int row = x / LANES, sub = x % LANES;
 #pragma unroll
@@ -737,9 +740,12 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
       for (int e = 0; e < PER; ++e) gb::store_pair(dst + 2 * (sub + LANES * e), v[e].x * inv, v[e].y * inv);
     }
   }
+  if (CLUSTER && (my_tiles == 0 || warp < 2)) {
+    __syncwarp();
+    cluster_arrive_wait();
+  }
   tc_fence_before_sync();
   __syncthreads();
-  if (CLUSTER) cluster_arrive_wait();      // nobody sends to a CTA that has left
   if (warp == 1) tmem_dealloc(tmem, TMEM_COLS);
 }
 
