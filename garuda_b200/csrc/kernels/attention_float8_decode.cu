@@ -48,7 +48,7 @@ constexpr int KT = 128;                 // keys per tile
 constexpr int THREADS = 192;
 constexpr int MAX_ROWS = 16;
 constexpr int MAX_CLUSTER = 8;
-constexpr int SEGMENT = 4;              // what a request's head costs beside its tiles, in tiles
+constexpr int SEGMENT = 4;              // what a request's head costs beside its tiles, in tiles (64 ragged requests: 2 129 us, 3 114, 4 109)
 constexpr uint32_t O_COL = 64, TMEM_COLS = 256;          // tensor memory: two buffers of S^T, then O
 
 template <int HD, int N, bool CLUSTER>
@@ -849,9 +849,9 @@ GB_EXPORT int gb_f8_attention_decode(const void* q, const void* k_pool, const vo
     const cudaStream_t st = (cudaStream_t)stream;
     // Few heads with little work: a cluster for each, which merges through shared memory and sums no lengths up: eight CTAs, or as many as let all
     // clusters run at once (the GPU holds 15 of eight, 22 of six, 33 of four, one CTA an SM; with three CTAs for 48 heads a third of them
-    // waited: 19 us for 10.6 with two). Heads of 128, eight of them, us with and without clusters: 500 keys 8.5 / 12.9, 2,048 10.7 / 19.6, 16,384
-    // 24.3 / 25.4; 64 heads: 500 keys 10.9 / 14.3, 2,048 18.5 / 25.7, 4,096 25.0 / 31.8. Not where a CTA gets more than
-    // CLUSTER_TILES tiles: requests of unequal length are not evened out here.
+    // waited: 19 us for 10.6 with two). Heads of 128, eight of them, us with and without clusters: 500 keys 7.6 / 11.8, 2,048 9.5 / 15.7, 8,192
+    // 14.9 / 18.5, 16,384 22.0 / 23.8; 64 heads: 500 keys 9.5 / 12.8, 2,048 15.6 / 20.1, 4,096 22.5 / 25.6. Not where a CTA gets more
+    // than CLUSTER_TILES tiles (22 of them: 27.2 / 27.0): requests of unequal length are not evened out here.
     const int heads = n * Hkv;
     int c = heads <= 15 ? 8 : heads <= 22 ? 6 : heads <= 33 ? 4 : heads <= tc_host::sm_count() / 2 ? 2 : heads <= tc_host::sm_count() ? 1 : 0;
     c = std::min(std::min(c, MAX_CLUSTER), reach_tiles);

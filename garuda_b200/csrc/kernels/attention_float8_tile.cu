@@ -11,8 +11,9 @@
 // the P V in front has ended too: the accumulator may be rescaled without another wait.
 // (The bfloat16 kernel's arrangement, 128 rows whose tiles two groups share and S two tiles ahead, took 70 us for 2,048 tokens of 32 heads of 128
 // and 105 us for two portions of 509 over a window of 4,096; this one takes 55 and 79, that kernel itself 59 and 92.) A tile takes 4,000
-// clocks: 2,200 of them the softmax of a half, of which 1,500 for its 128 exponentials a row (1,024 at the rate of their pipe), the
-// rest the products between its weights and its next scores, behind one another: the chain, not a unit, sets the pace.
+// clocks: a half's softmax is 2,200 of them, 1,500 for the exponentials (1,024 at their pipe's rate), and 1,900 pass from its weights to
+// its next scores (1,024 of products at the tensor cores' rate): the halves' chains, not a unit, set the pace. Two threads a row, sixteen
+// softmax warps, took 61 and 96; 32 scores at a time in a loop 63 and 94; a quarter of the exponentials as polynomials 63 and 85.
 //   * S is a product of codes as they lie (tcgen05.mma kind f8f6f4): a query row, scaled by a power of two to a largest of at most 448, is the
 //     sum of two E4M3 rows (a bfloat16's eight bits are four and four; what is 2^-11 of the row's largest and below loses bits
 //     that the sum does not see), so S = Qhi K^T + Qlo K^T at twice the rate of bfloat16: the same time, half of the keys' bytes.
@@ -23,8 +24,8 @@
 //   * The reference maximum follows the running one only when it has been outgrown by 2^8 for some row of a warp.
 //   warp 0      TMA: keys and values, a box a page, into rings of their own; looks up pages and scales four tiles at a time, two steps ahead
 //   warp 1      one elected lane issues the products
-//   warps 4-11  softmax, four warps a half
-//   warps 12-15 the queries of the next piece as codes, the values of the next tile as halves (rows that no query reads as zeros)
+//   warps 4-11  softmax, four warps a half; their half's queries of the next piece as codes; results
+//   warps 12-15 the values of the next tile as halves (rows that no query reads as zeros)
 // Registers are shared out by need (setmaxnreg; with 184 for the softmax some went to memory, and it took 60 us). Every wait is bounded.
 #include "attention_float8.cuh"
 #include "error_word.cuh"
