@@ -559,7 +559,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
           sync_four();               // (before the maxima's place is used again, too)
           if (quarter == 0 && j > 0) {             // the sums' rows lie in its lanes: r, r + ROWS, r + 2 ROWS
             const float corr = lane < S::PARTS * ROWS && lane % ROWS < w.nrows ? bars.corr[lane % ROWS] : 1.f;
-#pragma unroll
+#pragma unroll 1                           // (unrolled, registers of the whole tile's turn went to memory: 4 x 65,536 keys 100 us for 90)
             for (int h = 0; h < HD / 32; ++h) {
               uint32_t o[32];
               tmem_ld_32(lane_addr + O_COL + h * 32, o);
@@ -624,7 +624,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
         float* const part = partials + ((size_t)cta * 2 + (a == a_begin ? 0 : 1)) * (MAX_ROWS * RS) + r * RS;
         float* const own_part = reinterpret_cast<float*>(base + S::PARTS_AT) + (rank * ROWS + r) * S::RC;
         const uint32_t to = CLUSTER ? map_to_rank(smem_u32(own_part), 0) : 0;
-#pragma unroll
+#pragma unroll 1
         for (int h = 0; h < HD / 16; ++h) {
           uint32_t o[16];
           tmem_ld_16(lane_addr + O_COL + h * 16, o);

@@ -221,6 +221,14 @@ def test_append(ops, heads, kv_heads, hd, page, lens, mode, dtype, q_dtype):
         assert torch.equal(got.cpu().double(), want)
 
 
+@pytest.mark.parametrize("heads,kv_heads,hd,page", [(8, 2, 128, 32), (12, 3, 64, 16), (40, 8, 64, 32), (2, 1, 256, 32), (3, 3, 16, 5), (4, 1, 128, 128)])
+@pytest.mark.parametrize("lens", [[(1, 1 + 13 * i) for i in range(33)], [(40, 100)] + [(0, 5)] * 60 + [(1, 33), (0, 0), (3, 65)],
+                                  [(0, 9)] * 70 + [(66, 70)]])
+def test_append_of_fewer_tokens_than_requests(ops, heads, kv_heads, hd, page, lens):
+    test_append(ops, heads, kv_heads, hd, page, lens, "half", torch.float32, torch.bfloat16)
+    test_append(ops, heads, kv_heads, hd, page, lens, "interleaved", torch.bfloat16, torch.bfloat16)
+
+
 def test_append_token_by_token_is_append_at_once_but_for_the_smallest(ops):
     """A page filled token by token has the scale that it gets when filled at once; its codes differ by the second rounding of
     subnormals at most (half a step of 2^-9 of the scale more)."""
@@ -313,6 +321,20 @@ def test_attention_of_single_tokens(ops, heads, kv_heads, hd, page, case):
     check_attention(ops, heads, kv_heads, hd, page, SINGLES[case], seed=case)
 
 
+@pytest.mark.parametrize("requests", [1, 2, 3, 4, 5, 9, 10, 18, 19])       # 8 heads each: on either side of every number of CTAs that share a head
+@pytest.mark.parametrize("heads,hd,page", [(32, 128, 32), (8, 64, 16), (128, 64, 32)])
+def test_attention_of_single_tokens_of_few_and_many_heads(ops, requests, heads, hd, page):
+    lens = [(1, max(1, 1100 - 61 * i * i % 1093)) for i in range(requests)]
+    check_attention(ops, heads, 8, hd, page, lens, seed=requests)
+    check_attention(ops, heads, 8, hd, page, lens[:-1] + [(0, 40)] if requests > 1 else [(1, 40)], window=300, seed=requests)
+
+
+@pytest.mark.parametrize("length", [8191, 8193, 16384, 16385, 20000])         # on either side of the longest that a cluster takes
+@pytest.mark.parametrize("heads,kv_heads,hd", [(4, 1, 128), (16, 8, 64)])
+def test_attention_of_a_long_context(ops, length, heads, kv_heads, hd):
+    check_attention(ops, heads, kv_heads, hd, 32, [(1, length)], seed=length)
+
+
 @pytest.mark.parametrize("window", [1, 20, 33, 100])
 @pytest.mark.parametrize("heads,kv_heads,hd,page", SHAPES[:6])
 def test_attention_of_single_tokens_in_a_window(ops, heads, kv_heads, hd, page, window):
@@ -327,6 +349,13 @@ PROMPTS = [[(2, 2)], [(3, 70), (1, 40)], [(130, 130)], [(129, 400), (1, 300), (1
 @pytest.mark.parametrize("window", [0, 50])
 def test_attention_of_portions(ops, heads, kv_heads, hd, page, case, window):
     check_attention(ops, heads, kv_heads, hd, page, PROMPTS[case], window=window, seed=case)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,page", [(32, 32, 64, 32), (40, 40, 128, 16), (96, 32, 64, 128), (64, 32, 128, 64)])
+@pytest.mark.parametrize("window", [0, 200])
+def test_attention_of_more_portions_than_multiprocessors(ops, heads, kv_heads, hd, page, window):
+    """Several pieces of 256 rows to a CTA, some of them with rows in their first half only, long and short in turn."""
+    check_attention(ops, heads, kv_heads, hd, page, [(300, 520), (1, 77), (129, 129), (0, 3), (200, 200), (128, 640)], window=window)
 
 
 @pytest.mark.parametrize("heads,kv_heads,hd,page", [(4, 2, 64, 32), (8, 2, 128, 32), (3, 1, 48, 8)])
