@@ -34,7 +34,8 @@ __device__ __forceinline__ void load8(const T* src, int have, float (&x)[8]) {
   }
 }
 
-template <typename T, bool WIDE>
+// GATED: rows are [gate | up], K channels each, and silu(gate) * up is what becomes codes, from 32 bits at once.
+template <typename T, bool WIDE, bool GATED>
 __global__ void __launch_bounds__(256)
 quantize_rows_kernel(const T* __restrict__ a, long long lda, int M, int K, uint8_t* __restrict__ codes, int pitch,
                      uint8_t* __restrict__ scales) {
@@ -48,6 +49,12 @@ quantize_rows_kernel(const T* __restrict__ a, long long lda, int M, int K, uint8
   const int k = b * BLOCK + (threadIdx.x & 15) * 8;
   float x[8];
   load8<T, WIDE>(a + row * lda + k, mine ? K - k : 0, x);
+  if (GATED) {
+    float up[8];
+    load8<T, WIDE>(a + row * lda + K + k, mine ? K - k : 0, up);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = x[i] / (1.0f + expf(-x[i])) * up[i];
+  }
   float largest = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fabsf(x[i]));
@@ -393,17 +400,18 @@ __global__ void __launch_bounds__(128) attention_f8_simple_kernel(const Attentio
 
 GB_DEFINE_LAST_ERROR()
 
-// a [M, K] (rows lda apart) -> codes [M, pitch] (pitch a multiple of 16, at least K; the rest zeros) and scales
+// a [M, K] (rows lda apart; gated: [M, 2 K]) -> codes [M, pitch] (pitch a multiple of 16, at least K; the rest zeros) and scales
 // [ceil(K / 512)][M][4] as exponent bytes.
-int gb_f8_quantize_rows(const void* a, int tag, long long lda, int M, int K, void* codes, int pitch, void* scales, cudaStream_t stream) {
+int gb_f8_quantize_rows(const void* a, int tag, long long lda, int gated, int M, int K, void* codes, int pitch, void* scales, cudaStream_t stream) {
   if (M < 0 || K <= 0 || pitch < K || pitch % 16 || (uintptr_t)codes % 16) return gb::fail(GB_BAD_ARGUMENT, "quantize_rows: %d x %d, pitch %d", M, K, pitch);
   if (M == 0) return GB_OK;
   const long long blocks = (long long)M * ((K + f8::BLOCK - 1) / f8::BLOCK);
   const long long grid = (blocks * 16 + 255) / 256;
   if (grid > 0x7fffffff) return gb::fail(GB_UNSUPPORTED, "quantize_rows: %lld blocks", blocks);
   return GB_DISPATCH_DTYPE(tag, T, [&]() -> int {
-    const bool wide = (uintptr_t)a % 16 == 0 && lda * (long long)sizeof(T) % 16 == 0;
-    auto* kernel = wide ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>;
+    const bool wide = (uintptr_t)a % 16 == 0 && lda * (long long)sizeof(T) % 16 == 0 && (!gated || K * (long long)sizeof(T) % 16 == 0);
+    auto* kernel = gated ? (wide ? quantize_rows_kernel<T, true, true> : quantize_rows_kernel<T, false, true>)
+                         : (wide ? quantize_rows_kernel<T, true, false> : quantize_rows_kernel<T, false, false>);
     return gb::check_pdl_launch(gb::launch_pdl(kernel, dim3((unsigned)grid), dim3(256), 0, stream, dim3(1), (const T*)a, lda, M, K,
                                                (uint8_t*)codes, pitch, (uint8_t*)scales), "quantize_rows");
   });

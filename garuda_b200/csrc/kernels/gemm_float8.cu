@@ -604,7 +604,7 @@ int launch_out(const Plan& q, const CUtensorMap& wm, const CUtensorMap& xm, cons
 
 }  // namespace
 
-int gb_f8_quantize_rows(const void* a, int tag, long long lda, int M, int K, void* codes, int pitch, void* scales, cudaStream_t stream);
+int gb_f8_quantize_rows(const void* a, int tag, long long lda, int gated, int M, int K, void* codes, int pitch, void* scales, cudaStream_t stream);
 
 // Bytes of scratch that a product of this shape wants (codes, scales and parts; no need to clear them), and of counters (zero before the
 // first launch; every launch leaves them zero).
@@ -615,9 +615,9 @@ GB_EXPORT long long gb_f8_linear_scratch_bytes(int M, int N, int K, long long* c
   return code_bytes(M, K) + scale_bytes(M, K) + part_bytes(q);
 }
 
-// out [M, N] (+)= q(a) w^T: a [M, K] with rows lda apart, w [N, K] codes with rows w_pitch apart, ws its scales.
+// out [M, N] (+)= q(a) w^T: a [M, K] with rows lda apart (gated: [M, 2 K], rows [gate | up], multiplied as silu(gate) * up), w [N, K] codes with rows w_pitch apart, ws its scales.
 GB_EXPORT int gb_f8_linear(const void* a, int a_tag, long long lda, const void* w, long long w_pitch, const void* ws, void* out, int out_tag, int M,
-                           int N, int K, int accumulate, float alpha, void* counters, void* scratch, void* stream) {
+                           int N, int K, int accumulate, float alpha, int gated, void* counters, void* scratch, void* stream) {
   if (M < 0 || N < 0 || K <= 0) return gb::fail(GB_BAD_ARGUMENT, "linear_float8: %d x %d x %d", M, N, K);
   if (M == 0 || N == 0) return GB_OK;
   if (w_pitch % 16 || w_pitch < K || (uintptr_t)w % 16 || (uintptr_t)scratch % 256)
@@ -627,7 +627,7 @@ GB_EXPORT int gb_f8_linear(const void* a, int a_tag, long long lda, const void* 
   const int pitch = (K + 15) / 16 * 16;
   uint8_t* codes = (uint8_t*)scratch;
   uint8_t* xs = codes + code_bytes(M, K);
-  int rc = gb_f8_quantize_rows(a, a_tag, lda, M, K, codes, pitch, xs, st);
+  int rc = gb_f8_quantize_rows(a, a_tag, lda, gated, M, K, codes, pitch, xs, st);
   if (rc) return rc;
   const Plan q = make_plan(M, N, K);
   const int ctas = q.pair ? 2 : 1;

@@ -53,7 +53,7 @@ _FLOAT8_SIGNATURES = {
     "gb_f8_attention_tile_set_error_sink": [c_void_p],
     "gb_f8_attention_decode_error_check": [],
     "gb_f8_attention_decode_set_error_sink": [c_void_p],
-    "gb_f8_linear": [c_void_p, c_int, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p,
+    "gb_f8_linear": [c_void_p, c_int, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p,
                      c_void_p, c_void_p],
     "gb_f8_gemm_error_check": [],
     "gb_f8_gemm_set_error_sink": [c_void_p],
@@ -141,18 +141,19 @@ class Float8Ops:
             "float8_weight")
         return Float8Weight(codes[:, :K], scales)
 
-    def linear_float8(self, a, w, out, accumulate: bool = False, alpha: float = 1.0, ws=None):
+    def linear_float8(self, a, w, out, accumulate: bool = False, alpha: float = 1.0, ws=None, gated: bool = False):
         """``out[M, N] (+)= q(a) @ w^T``: ``w`` a ``Float8Weight`` (or a pair of its two tensors), ``a [M, K]`` bfloat16 or float32, its
         rows rounded to 8 bits with a scale per token and 128 channels (``q``). Sums are 32-bit; ``out`` is bfloat16 or float32,
         and float32 where ``accumulate`` adds ``alpha * product`` to what is there. A scale of the weights that is no positive power of two
-        (``float8_weight`` makes none) turns the results of its 128 rows into NaN."""
+        (``float8_weight`` makes none) turns the results of its 128 rows into NaN. ``gated``: ``a [M, 2 K]`` has rows ``[gate | up]``, and
+        ``silu(gate) * up`` is rounded to 8 bits, from 32, and multiplied."""
         values, scales = w
         _need(a.is_cuda and values.is_cuda and scales.is_cuda and out.is_cuda, "kernel operands must live on the CUDA device")
         _need(a.dim() == 2 and values.dim() == 2 and out.dim() == 2, "linear_float8: operands must be matrices")
-        M, K = a.shape
-        N, K_w = values.shape
+        M, width = a.shape
+        N, K = values.shape
         a_row, w_row = a.stride(0), values.stride(0)
-        if not (K_w == K and out.shape == (M, N)):
+        if not (width == (2 * K if gated else K) and out.shape == (M, N)):
             _need(False, f"linear_float8: shapes {tuple(a.shape)} x {tuple(values.shape)} -> {tuple(out.shape)}")
         _need(K > 0, "linear_float8: no channels")
         _need(values.dtype is E4M3, "linear_float8: weights must be float8_e4m3fn")
@@ -178,8 +179,15 @@ class Float8Ops:
         scratch = self._scratch8("float8_linear", sizes[0], ws, stream)
         counters = self._scratch8("float8_counters", sizes[1], ws, stream, zero=True)
         self._check(L, L.gb_f8_linear(a.data_ptr(), _tag(a, "linear_float8 input"), a_row, values.data_ptr(), w_row if N > 1 else (K + 15) // 16 * 16,
-                                      scales.data_ptr(), out.data_ptr(), out_tag, M, N, K, accumulate, alpha, counters.data_ptr(),
+                                      scales.data_ptr(), out.data_ptr(), out_tag, M, N, K, accumulate, alpha, bool(gated), counters.data_ptr(),
                                       scratch.data_ptr(), stream), "linear_float8", 2)
+
+    def swiglu_float8(self, ctx, h, w_gate_up, w_down, out, accumulate: bool = False):
+        """``out (+)= q(silu(g) * u) @ w_down^T`` with ``[g | u] = q(h) @ w_gate_up^T``, both weights ``Float8Weight``. Gate and up are kept
+        in bfloat16 between the products: half the bytes, and 2^-9 of a number that keeps four bits behind the gate."""
+        gate_up = ctx.ws.get("gate_up", (h.shape[0], w_gate_up.values.shape[0]), torch.bfloat16)
+        self.linear_float8(h, w_gate_up, gate_up)
+        self.linear_float8(gate_up, w_down, out, accumulate, gated=True)
 
     # ------------------------------------------------------------------ the cache
     @staticmethod

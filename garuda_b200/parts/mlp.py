@@ -32,6 +32,7 @@ class SwiGLU(FeedForward):
         super().load(tensors, ops, dtype)
         self.w_gate_up = ops.pack_gate_up(tensors["gate_proj.weight"], tensors["up_proj.weight"])
         self.w_down = hold_matrix(ops, tensors["down_proj.weight"])
+        self.in_8_bits = getattr(ops, "weight_dtype", None) is not None
 
     # ``h`` may be a norm that is half done (``CudaOps.linear_swiglu`` takes it), and the last product
     # may fold in the first half of the norm that follows (``emit_norm``)
@@ -40,6 +41,10 @@ class SwiGLU(FeedForward):
 
     def forward(self, ctx, h, residual=None, emit_norm=None):
         T = h.shape[0]
+        if self.in_8_bits:
+            y = residual if residual is not None else ctx.ws.get("ffn_out", (T, self.width), torch.float32)
+            self.ops.swiglu_float8(ctx, self.ops.normed(ctx, h), self.w_gate_up, self.w_down, y, accumulate=residual is not None)
+            return None if residual is not None else y
         act = ctx.ws.get("ffn_act", (T, self.inner), self.dtype)
         self.ops.linear_swiglu(ctx, h, self.w_gate_up, act)
         if residual is not None:

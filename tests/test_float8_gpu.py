@@ -139,6 +139,38 @@ def test_a_token_that_is_not_a_number_spoils_its_own_row_only(ops):
     check_product(out[keep], a[keep], w8)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 64, 16), (1, 256, 5632), (3, 130, 100), (17, 200, 392), (150, 300, 272), (260, 128, 1376)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_products_of_a_gated_pair(ops, M, N, K, dtype):
+    """silu(gate) * up is 32-bit: the exponential (2 units), a sum, a quotient and a product, 2^-20 of it at most in all. Where the exact
+    value lies nearer than 2^-19 of itself to the middle of two codes, the code may be the other one: a step, 2^-3 of the value
+    (2^-9 of the scale below the normal numbers)."""
+    g = gen(M + N + K)
+    pair = (torch.randn(M, 2 * K, generator=g) * 3).to(dtype)
+    w = torch.randn(N, K, generator=g) * 0.05
+    w8 = ops.float8_weight(w.cuda())
+    gate, up = pair.double().split(K, 1)
+    a = gate / (1 + torch.exp(-gate)) * up
+    want, mag = plain.linear(a, w8.values.cpu().double(), w8.scales.cpu())
+    blocks = -(-K // 128)
+    padded = torch.nn.functional.pad(a, (0, blocks * 128 - K))
+    scale = plain.scales_of(padded.view(M, blocks, 128).abs().amax(-1)).repeat_interleave(128, 1)[:, :K]
+    low, high = plain.encode(a * (1 - 2.0 ** -19) / scale), plain.encode(a * (1 + 2.0 ** -19) / scale)
+    dense = w8.values.cpu().double() * w8.scales.cpu().double().repeat_interleave(128, 0)[:N].repeat_interleave(128, 1)[:, :K]
+    flips = torch.where(low != high, a.abs() * 2.0 ** -3 + scale * 2.0 ** -9, 0.0) @ dense.abs().t()
+    out = torch.full((M, N), math.nan, device="cuda")
+    ops.linear_float8(pair.cuda(), w8, out, gated=True)
+    err = (out.cpu().double() - want).abs()
+    assert (err <= 2.0 ** -22 * want.abs() + 2.0 ** -13 * mag + flips + 1e-30).all()
+    summed = torch.ones(M, N, device="cuda")
+    ops.linear_float8(pair.cuda(), w8, summed, accumulate=True, gated=True)
+    assert (summed.cpu().double() - 1 - want).abs().le(2.0 ** -22 * (1 + want.abs()) + 2.0 ** -13 * mag + flips).all()
+    from garuda_b200.kernels.ops import KernelError
+    for bad in (pair[:, :K], pair[:, 1:]):
+        with pytest.raises(KernelError):
+            ops.linear_float8(bad.cuda(), w8, out, gated=True)
+
+
 def test_products_refuse(ops):
     from garuda_b200.kernels.ops import KernelError
     a, w = operands(4, 256, 256, torch.bfloat16)
