@@ -31,6 +31,9 @@
 //   warp 1     one elected lane issues the products: S^T of a tile, then O += P V of the tile before
 //   warps 2-5  scores, maxima, weights; the next head's queries as codes; results
 // Two CTAs an SM (N = 16; one with N = 32). Every wait is bounded.
+// Few short heads (CLUSTER): one head to a thread-block cluster, whose CTAs share its tiles and store their rows of sums into the shared
+// memory of the first, which adds them up in the CTAs' order behind a barrier of the cluster. (Asynchronous stores counted on a barrier in
+// memory took 2 us for 400 of them.) 4 requests of 65,536 positions, 8 heads of 128: 5.9 TB/s; one of 500: 6.9 us; 8 of 2,048, 4 of 64: 11.2.
 #include "attention_float8.cuh"
 #include "error_word.cuh"
 #include "tc_common.cuh"
@@ -812,7 +815,8 @@ int launch(const Params& p, const CUtensorMap& km, const CUtensorMap& vm, long l
   const long long most = std::max(tiles_most / min_tiles + 1, (long long)p.R * p.Hkv);
   const size_t smem = 1024 + S::BYTES + (size_t)(4 * p.R + 3) * 4;
   const unsigned grid = CLUSTER ? (unsigned)(p.R * p.Hkv * min_tiles) : (unsigned)(most < room ? most : room);
-  return gb::check_pdl_launch(gb::launch_pdl(kernel, dim3(grid), dim3(THREADS), smem, stream, dim3(CLUSTER ? (unsigned)min_tiles : 1u), km, vm, p, min_tiles, (float*)parts, (int*)counters), "attention_f8_decode");
+  return gb::check_pdl_launch(gb::launch_pdl(kernel, dim3(grid), dim3(THREADS), smem, stream, dim3(CLUSTER ? (unsigned)min_tiles : 1u), km, vm, p,
+                                             min_tiles, (float*)parts, (int*)counters), "attention_f8_decode");
 }
 
 }  // namespace
@@ -826,7 +830,8 @@ GB_EXPORT long long gb_f8_attention_decode_part_bytes() { return (long long)tc_h
 GB_EXPORT int gb_f8_attention_decode(const void* q, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale, const void* table,
                                      int table_width, const void* cu_q, const void* kv_lens, void* out, int R, long long pages, int Hq, int Hkv, int hd,
                                      float scale, int window, int page, int max_kv_len, void* parts, void* counters, void* stream) {
-  if (R <= 0 || Hkv <= 0 || Hq % Hkv || (hd != 64 && hd != 128) || page < 16 || page > 128 || (page & (page - 1)) || Hq / Hkv > MAX_ROWS || (uintptr_t)q % 16 || (uintptr_t)out % 4 ||
+  if (R <= 0 || Hkv <= 0 || Hq % Hkv || (hd != 64 && hd != 128) || page < 16 || page > 128 || (page & (page - 1)) ||
+      Hq / Hkv > MAX_ROWS || (uintptr_t)q % 16 || (uintptr_t)out % 4 ||
       (uintptr_t)k_pool % 16 || (uintptr_t)v_pool % 16)
     return gb::fail(GB_BAD_ARGUMENT, "attention_f8_decode: %d requests, heads %d / %d of %d, pages of %d", R, Hq, Hkv, hd, page);
   CUtensorMap km, vm;

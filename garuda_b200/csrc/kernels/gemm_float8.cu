@@ -629,7 +629,8 @@ GB_EXPORT long long gb_f8_linear_scratch_bytes(int M, int N, int K, long long* c
   return code_bytes(M, K) + scale_bytes(M, K) + part_bytes(q);
 }
 
-// out [M, N] (+)= q(a) w^T: a [M, K] with rows lda apart (gated: [M, 2 K], rows [gate | up], multiplied as silu(gate) * up), w [N, K] codes with rows w_pitch apart, ws its scales.
+// out [M, N] (+)= q(a) w^T: a [M, K] with rows lda apart (gated: [M, 2 K], rows [gate | up], multiplied as silu(gate) * up), w [N, K] codes
+// with rows w_pitch apart, ws its scales.
 GB_EXPORT int gb_f8_linear(const void* a, int a_tag, long long lda, const void* w, long long w_pitch, const void* ws, void* out, int out_tag, int M,
                            int N, int K, int accumulate, float alpha, int gated, void* counters, void* scratch, void* stream) {
   if (M < 0 || N < 0 || K <= 0) return gb::fail(GB_BAD_ARGUMENT, "linear_float8: %d x %d x %d", M, N, K);
