@@ -262,7 +262,7 @@ gemm_f8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
       const uint32_t idesc0 = instr_desc_mxf8(CTAS * BM, p.nt, 0);
       const uint64_t da0 = smem_desc_sw128(ring), db0 = smem_desc_sw128(ring + STEP * (BM * BK)), ds0 = smem_desc_rows16(sf_at);
       const uint32_t stage_step = stage_bytes >> 4, x_step = (uint32_t)(x_rows * BK) >> 4;
-        const bool leader = elect_one(), wide = p.nt > 128;
+      const bool leader = elect_one(), wide = p.nt > 128;
       int s = 0, par = 0, sf = 0, sf_par = 0, failed = 0;
       uint32_t set = ACC_STRIDE, at = 0;          // the set of scales; the stage, in units of the descriptors
       for (int t = 0; q.more() && !failed; ++t) {      // tiles, or parts of them

@@ -17,6 +17,7 @@ from .base import FeedForward, TensorSpec, hold_matrix, register_feed_forward
 class SwiGLU(FeedForward):
     graph_safe = True
     holds_matrices = True
+    in_8_bits = False         # (set where the kernel set holds weights so)
 
     def __init__(self, width: int, inner: int, init_std: float = 0.02):
         self.width, self.inner = int(width), int(inner)
