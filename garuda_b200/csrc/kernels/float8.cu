@@ -40,12 +40,12 @@ __global__ void __launch_bounds__(256)
 quantize_rows_kernel(const T* __restrict__ a, long long lda, int M, int K, uint8_t* __restrict__ codes, int pitch,
                      uint8_t* __restrict__ scales) {
   gb::pdl_launch_dependents();
-  const int kb = (K + BLOCK - 1) / BLOCK;
-  const long long block = ((long long)blockIdx.x * 256 + threadIdx.x) >> 4;       // of all rows'
+  const uint32_t kb = (uint32_t)(K + BLOCK - 1) / BLOCK, all = (uint32_t)M * kb;
+  const uint32_t block = blockIdx.x * 16 + (threadIdx.x >> 4);       // of all rows'; the host has seen that they fit 31 bits
+  if (block - (threadIdx.x & 16 ? 1 : 0) >= all) return;             // the warp's first block lies behind the last
+  const bool mine = block < all;
+  const int row = mine ? (int)(block / kb) : 0, b = mine ? (int)(block - (uint32_t)row * kb) : 0;
   gb::pdl_wait();
-  if (block - (threadIdx.x & 16 ? 1 : 0) >= (long long)M * kb) return;            // the warp's first block lies behind the last
-  const bool mine = block < (long long)M * kb;
-  const int row = mine ? (int)(block / kb) : 0, b = mine ? (int)(block % kb) : 0;
   const int k = b * BLOCK + (threadIdx.x & 15) * 8;
   float x[8];
   load8<T, WIDE>(a + row * lda + k, mine ? K - k : 0, x);
@@ -407,7 +407,7 @@ int gb_f8_quantize_rows(const void* a, int tag, long long lda, int gated, int M,
   if (M == 0) return GB_OK;
   const long long blocks = (long long)M * ((K + f8::BLOCK - 1) / f8::BLOCK);
   const long long grid = (blocks * 16 + 255) / 256;
-  if (grid > 0x7fffffff) return gb::fail(GB_UNSUPPORTED, "quantize_rows: %lld blocks", blocks);
+  if (blocks > 0x7fffffff) return gb::fail(GB_UNSUPPORTED, "quantize_rows: %lld blocks", blocks);
   return GB_DISPATCH_DTYPE(tag, T, [&]() -> int {
     const bool wide = (uintptr_t)a % 16 == 0 && lda * (long long)sizeof(T) % 16 == 0 && (!gated || K * (long long)sizeof(T) % 16 == 0);
     auto* kernel = gated ? (wide ? quantize_rows_kernel<T, true, true> : quantize_rows_kernel<T, false, true>)
