@@ -263,9 +263,10 @@ class Float8Ops:
         pools = (k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), table_width,
                  cu_q.data_ptr(), kv_lens.data_ptr(), out_ptr)
         if q.dtype is torch.bfloat16 and hd in (64, 128) and page_size in (16, 32, 64, 128) and g <= 128 and not (q_ptr | out_ptr) & 15:
-            # requests of a few rows (new tokens times heads of a group) go to one kernel, the others to the other
+            # requests of a few rows (new tokens times heads of a group) go to one kernel, the others to the other; groups of more than
+            # sixteen heads have none of a few (a request without tokens is nobody's)
             few = (8 if g <= 8 else 16) if g <= 16 else 0
-            if min_q_len * g <= few:
+            if few and min_q_len * g <= few:
                 scratch = self._scratch8("float8_attention_parts", self._float8_part_bytes, ws, stream)
                 counters = self._scratch8("float8_attention_counters", 4 * R * Hkv, ws, stream, zero=True)
                 self._check(L, L.gb_f8_attention_decode(
