@@ -6,9 +6,9 @@
 // Bound by the stream of codes, 2 * HD bytes a key and head, so they go from shared memory into the matrix instructions as they are
 // (tcgen05.mma kind f8f6f4, 32-bit sums), and what has more than four bits is split instead: a query row, scaled by a power of two to a largest
 // of at most 448, is the sum of two E4M3 rows (a bfloat16's eight bits are four and four; what is 2^-11 of the row's largest and below
-// loses bits that the sum does not see), and a weight exp(s - m) is three codes, the second and third in units of 1/32 and 1/1024: twelve
+// loses bits that the sum does not see), and a weight exp(s) * vs is three codes, the second and third in units of 1/32 and 1/1024: twelve
 // bits, down to 2^-24 of the reference. (Groups of more than eight heads: two codes, nine bits, down to 2^-22, and a reference that
-// follows every larger score.) Products of one tile of 128 keys:
+// follows every larger one.) Products of one tile of 128 keys:
 //   S^T [128 keys, N] = K [128, HD] * Q [N, HD]^T         N = 16 (or 32): the rows' codes, then what these leave
 //   O [rows, HD]     += P [rows, 128] * V [128, HD]       P's rows: the weights' first codes, then the others; V as it lies, keys along its
 //                                                         rows. The products' other rows (128 in all) read whatever lies behind P, and
@@ -18,10 +18,12 @@
 // such product and converts; with the codes converted to halves by hand 700; both were bound by instructions at 5.0 TB/s and below. Here
 // 128 keys take some 500.) Maxima and denominators are 32-bit.
 //
-// The maximum that weights refer to is common to the tile's 128 keys. It follows the running maximum only when some score exceeds it by more
-// than 2^3 (a vote a tile; following at once cost 0.8 us a time, some 14 times in 60 tiles), and then the sums in tensor
-// memory are brought to it. Scales cost nothing per key: ks goes into the score's factor, vs, as a power of two, into the
-// exponent, and the denominator takes it out again. The sums are in units of the largest vs so far.
+// Scales cost nothing per key: ks goes into the score's factor, vs, as a power of two, is added to the score, and the denominator takes it out
+// again. So what weights refer to is a row's own largest exp(s) * vs: a page that a row may not read, or whose keys have no weight,
+// takes no bits from the others however large its values are (with the largest vs of all pages in the reference, weights of pages
+// 2^-20 below it were off by several per cent, below 2^-25 gone). The reference is common to the tile's 128 keys. It follows the
+// running maximum only when some key exceeds it by more than 2^3 (a vote a tile; following at once cost 0.8 us a time, some 14 times in 60
+// tiles), and then the sums in tensor memory are brought to it.
 //
 // Work: the tiles of all requests and heads in a row, an equal stretch to every CTA, so that requests of unequal length do not wait for
 // the longest; a request that falls to several CTAs is merged by the one that finishes last, in their order, from scratch memory, so
@@ -107,6 +109,11 @@ __device__ __forceinline__ void tmem_load<16>(uint32_t addr, uint32_t (&r)[16]) 
 template <>
 __device__ __forceinline__ void tmem_load<32>(uint32_t addr, uint32_t (&r)[32]) { tmem_ld_32(addr, r); }
 
+// x * 2^d, d <= 0, where 2^d by itself may be too small for a number in 32 bits.
+__device__ __forceinline__ float times_power(float x, float d) {
+  const float most = fmaxf(d, -120.f);
+  return x * exp2_fast(most) * exp2_fast(d - most);
+}
 // Two weights as a code, 32 times what that leaves as a code, and (PARTS 3) 32 times what that leaves; in the low byte the first's.
 template <int PARTS>
 __device__ __forceinline__ void split(float a, float b, uint32_t (&code)[PARTS]) {
@@ -334,7 +341,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
       }
     };
     auto write_scales = [&](int t, int s) {
-      if ((lane >> 3) == (t & 3)) bars.scales[s][sub] = make_float2(now.ks, log2f(now.vs));
+      if ((lane >> 3) == (t & 3)) bars.scales[s][sub] = make_float2(now.ks, fmaxf(log2f(now.vs), -100.f));
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&bars.full[s]));          // (after what the other lanes wrote)
     };
@@ -493,9 +500,11 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
       const Segment g = now;
       const Span w = span_at(g.r);
       bool asked = a + g.count < a_end;
-      float m[ROWS], l[ROWS], vref = -200.f;       // vref: log2 of the vs in whose units the sums are
+      // per row: the reference, in powers of two, and the denominator, the sum of 2^(s - ref); of the keys up to the last change of references
+      // the largest vs
+      float ref[ROWS], l[ROWS], vtop = -200.f;
 #pragma unroll
-      for (int r = 0; r < ROWS; ++r) m[r] = -INFINITY, l[r] = 0.f;
+      for (int r = 0; r < ROWS; ++r) ref[r] = -INFINITY, l[r] = 0.f;
 
       for (int j = 0; j < g.count; ++j, ++t) {
         wait(bars.s_ready[t & 1], t >> 1);
@@ -506,19 +515,20 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
         const bool readable = key >= w.lo && key <= w.hi && sc.x >= 0.f;
         // no mask for a tile that lies before the first row's position, inside the last row's window, on pages that are there
         const bool full = key0 + KT - 1 <= w.pos0 && (p.window <= 0 || key0 >= w.hi + 1 - p.window) && sc.x >= 0.f;
-        float v[ROWS];
+        float u[ROWS];                             // log2 of exp(s) * vs
         {
           uint32_t raw_s[N];
           tmem_load<N>(lane_addr + (t & 1) * 32, raw_s);
           tmem_ld_wait();
 #pragma unroll
-          for (int r = 0; r < ROWS; ++r) v[r] = (__uint_as_float(raw_s[r]) + __uint_as_float(raw_s[r + ROWS])) * (bars.factor[seg & 1][r] * sc.x);
+          for (int r = 0; r < ROWS; ++r)
+            u[r] = fmaf(__uint_as_float(raw_s[r]) + __uint_as_float(raw_s[r + ROWS]), bars.factor[seg & 1][r] * sc.x, sc.y);
         }
         if (!full) {
 #pragma unroll
           for (int r = 0; r < ROWS; ++r) {
             const int pos = w.pos0 + r / p.g;
-            if (!readable || key > pos || (p.window > 0 && key + p.window <= pos)) v[r] = -INFINITY;
+            if (!readable || key > pos || (p.window > 0 && key + p.window <= pos)) u[r] = -INFINITY;
           }
           // A value row that nobody reads is cleared: a weight of zero times a code that is no number would spoil a sum.
           if (!readable) {
@@ -528,11 +538,11 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
           }
         }
         const float ev = readable ? sc.y : -200.f;
-        bool more = ev > vref;
+        bool more = false;
 #pragma unroll
         for (int r = 0; r < ROWS; ++r)
-          if (r < w.nrows) more = more || !(v[r] <= m[r] + S::GROWTH);          // (a score that is no number stays one)
-        // a score far above the reference (rare after a request's first tiles), or a larger vs: everything is brought to it
+          if (r < w.nrows) more = more || !(u[r] <= ref[r] + S::GROWTH);          // (a score that is no number stays one)
+        // a key far above the reference (rare after a request's first tiles): everything is brought to it
         if (j == 0 || any_of_four(more)) {
           if (j > 0) {
             wait(bars.pv_done[(t - 1) & 1], (t - 1) >> 1);
@@ -543,21 +553,19 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
 #pragma unroll
           for (int r = 0; r < ROWS; ++r)
             if (r < w.nrows) {
-              const float top = redux_max(v[r]);
+              const float top = redux_max(u[r]);
               if (lane == 0) bars.top[sw][r] = top;
             }
           sync_four();
-          const float v_new = fmaxf(vref, fmaxf(fmaxf(bars.vtop[0], bars.vtop[1]), fmaxf(bars.vtop[2], bars.vtop[3])));
-          const float v_corr = exp2_fast(vref - v_new);
-          vref = v_new;
+          vtop = fmaxf(vtop, fmaxf(fmaxf(bars.vtop[0], bars.vtop[1]), fmaxf(bars.vtop[2], bars.vtop[3])));
 #pragma unroll
           for (int r = 0; r < ROWS; ++r) {
             if (r >= w.nrows) continue;
-            const float m_new = fmaxf(m[r], fmaxf(fmaxf(bars.top[0][r], bars.top[1][r]), fmaxf(bars.top[2][r], bars.top[3][r])));
-            const float corr = m[r] == -INFINITY ? 0.f : exp2_fast(m[r] - m_new);
-            m[r] = m_new;
-            l[r] *= corr;
-            if (x == r) bars.corr[r] = corr * v_corr;
+            const float top = fmaxf(ref[r], fmaxf(fmaxf(bars.top[0][r], bars.top[1][r]), fmaxf(bars.top[2][r], bars.top[3][r])));
+            const float corr = ref[r] == -INFINITY ? 0.f : exp2_fast(ref[r] - top);
+            l[r] = ref[r] == -INFINITY ? l[r] : times_power(l[r], ref[r] - top);
+            ref[r] = top;
+            if (x == r) bars.corr[r] = corr;
           }
           sync_four();               // (before the maxima's place is used again, too)
           if (quarter == 0 && j > 0) {             // the sums' rows lie in its lanes: r, r + ROWS, r + 2 ROWS
@@ -575,15 +583,21 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
           }
         }
         if (t >= 2) wait(bars.pv_done[t & 1], (t - 2) >> 1);       // P's buffer is free
-        // weights * 2^UP * vs / 2^vref as two codes each, the denominator without vs. (2^-100 of the largest vs is nothing; and where
-        // nothing is read the weights are zeros.)
-        const float up = S::UP + fminf(fmaxf(sc.y - vref, -100.f), 0.f), down = exp2_fast(-up);
+        // Weights times vs, in units of 2^(ref - UP), as codes; the denominator takes vs out again. Only where this key's vs is 2^-90 of another's may
+        // its weight be too small a number for that, and count all the same: the denominator gets an exponential of its own.
+        const bool far = sc.y < vtop - 90.f;
+        if (far) {
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r)
+            if (r < w.nrows) l[r] += exp2_fast(u[r] - sc.y - (ref[r] == -INFINITY ? 0.f : ref[r]));
+        }
+        const float down = far ? 0.f : exp2_fast(-S::UP - sc.y);
         const uint32_t p_base = p_at + (t & 1) * S::P_BYTES + (key_i & 15), chunk = (uint32_t)key_i >> 4;
 #pragma unroll
         for (int r = 0; r < ROWS; r += 2) {
           if (r >= w.nrows) break;
-          const float wa = exp2_fast(v[r] + (up - (m[r] == -INFINITY ? 0.f : m[r])));
-          const float wb = exp2_fast(v[r + 1] + (up - (m[r + 1] == -INFINITY ? 0.f : m[r + 1])));
+          const float wa = exp2_fast(u[r] + (S::UP - (ref[r] == -INFINITY ? 0.f : ref[r])));
+          const float wb = exp2_fast(u[r + 1] + (S::UP - (ref[r + 1] == -INFINITY ? 0.f : ref[r + 1])));
           l[r] = fmaf(wa, down, l[r]), l[r + 1] = fmaf(wb, down, l[r + 1]);
           uint32_t code[S::PARTS];
           split<S::PARTS>(wa, wb, code);
@@ -616,12 +630,12 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
       if (quarter == 0) {
         const int r = lane % ROWS;
         const bool mine = lane < w.nrows && ok;
-        float mr = -INFINITY;
+        float mine_ref = -INFINITY;
 #pragma unroll
         for (int i = 0; i < ROWS; ++i)
-          if (i == r) mr = m[i];
+          if (i == r) mine_ref = ref[i];
         const float ll = (bars.lsum[0][r] + bars.lsum[1][r]) + (bars.lsum[2][r] + bars.lsum[3][r]);
-        const float unit = exp2_fast(vref - S::UP), inv = ll > 0.f ? 1.0f / ll : ll == ll ? 0.f : ll;
+        const float unit = exp2_fast(-S::UP), inv = ll > 0.f ? 1.0f / ll : ll == ll ? 0.f : ll;
         const float f = whole ? unit * inv : unit;
         __nv_bfloat16* const dst = p.out + ((size_t)(w.q_begin + r / p.g) * p.Hq + g.kvh * p.g + r % p.g) * HD;
         float* const part = partials + ((size_t)cta * 2 + (a == a_begin ? 0 : 1)) * (MAX_ROWS * RS) + r * RS;
@@ -639,7 +653,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
             float lo = __shfl_sync(0xffffffffu, hi, (lane + ROWS) & 31);
             if (S::PARTS == 3) lo = fmaf(__shfl_sync(0xffffffffu, hi, (lane + 2 * ROWS) & 31), 0.03125f, lo);
             // (nothing seen: the sums mean nothing)
-            y[c] = mr == -INFINITY && ll == ll ? 0.f : fmaf(lo, 0.03125f, hi) * f;
+            y[c] = mine_ref == -INFINITY && ll == ll ? 0.f : fmaf(lo, 0.03125f, hi) * f;
           }
           if (CLUSTER && mine && !whole) {
 #pragma unroll
@@ -653,9 +667,9 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
           }
         }
         if (CLUSTER && mine && !whole) {
-          st_cluster_v4(to + HD * 4, mr, ll, 0.f, 0.f);
+          st_cluster_v4(to + HD * 4, mine_ref, ll, 0.f, 0.f);
         } else if (mine && !whole) {
-          __stcg(reinterpret_cast<float2*>(part + HD), make_float2(mr, ll));
+          __stcg(reinterpret_cast<float2*>(part + HD), make_float2(mine_ref, ll));
         }
         tc_fence_before_sync();
         mbar_arrive(smem_u32(&bars.o_free));
@@ -708,7 +722,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
         return partials + ((size_t)c * 2 + (c == c0[i] && behind[i] ? 1 : 0)) * (MAX_ROWS * RS) + row * RS;
       };
       auto read2 = [&](const float* from) { return CLUSTER ? *reinterpret_cast<const float2*>(from) : __ldcg(reinterpret_cast<const float2*>(from)); };
-      float mm = -INFINITY, ll = 0.f;
+      float top = -INFINITY, ll = 0.f;
       float2 v[PER];
 #pragma unroll
       for (int e = 0; e < PER; ++e) v[e] = make_float2(0.f, 0.f);
@@ -725,10 +739,11 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           if (c + k > c1[i]) break;
-          const float m_new = fmaxf(mm, ml[k].x);
-          const float old = mm == -INFINITY ? 0.f : exp2_fast(mm - m_new), f = ml[k].x == -INFINITY ? 0.f : exp2_fast(ml[k].x - m_new);
-          mm = m_new;
-          ll = ll * old + (f > 0.f ? f * ml[k].y : ml[k].y == ml[k].y ? 0.f : ml[k].y);          // (a part without a key has nothing)
+          const float top_new = fmaxf(top, ml[k].x);
+          const float old = top == -INFINITY ? 0.f : exp2_fast(top - top_new), f = ml[k].x == -INFINITY ? 0.f : exp2_fast(ml[k].x - top_new);
+          if (top != -INFINITY) ll = times_power(ll, top - top_new);
+          ll += ml[k].x == -INFINITY ? (ml[k].y == ml[k].y ? 0.f : ml[k].y) : times_power(ml[k].y, ml[k].x - top_new);          // (a part without a key has nothing)
+          top = top_new;
 #pragma unroll
           for (int e = 0; e < PER; ++e) {
             v[e].x = v[e].x * old + (f > 0.f ? f * y[k][e].x : 0.f);

@@ -20,8 +20,9 @@
 //   * Values become halves (exactly: every E4M3 number is one) in shared memory, a conversion for two of them, by four warps of
 //     their own, for 256 rows' worth of products. (Splitting P into codes instead would cost the softmax warps two instructions a score.)
 //   * A page's ks goes into the factor of the exponent's multiply-add, its vs (as a power of two) into the constant; the denominator takes it
-//     out again per sixteen keys. The accumulators are in units of the largest vs so far. P in halves: eleven bits.
-//   * The reference maximum follows the running one only when it has been outgrown by 2^8 for some row of a warp.
+//     out again per sixteen keys. P in halves: eleven bits, down to 2^-30 of what a row refers to, its own largest weight times vs: a
+//     page that a row may not read, or whose keys have no weight, takes no bits from the others however large its values are.
+//   * The references follow the running maxima only when one has been outgrown by 2^8 for some row of a warp.
 //   warp 0      TMA: keys and values, a box a page, into rings of their own; looks up pages and scales four tiles at a time, two steps ahead
 //   warp 1      one elected lane issues the products
 //   warps 4-11  softmax, four warps a half; their half's queries of the next piece as codes; results
@@ -348,7 +349,7 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
           const bool mine = (lane >> 3) == (gt & 3), there = mine && now.page >= 0 && sub % per_page == 0;
           const int pages = __popc(__ballot_sync(0xffffffffu, there));
           if (!(ok = mbar_wait_warp(smem_u32(&mc.k_empty[ks]), kpar, abort_s, ran_out))) break;
-          if (mine) mc.scales[gt % SLOTS][sub] = make_float2(now.ks, log2f(now.vs));
+          if (mine) mc.scales[gt % SLOTS][sub] = make_float2(now.ks, fmaxf(log2f(now.vs), -100.f));
           __syncwarp();
           if (lane == 0) {           // (after what the other lanes wrote)
             if (pages == 0) mbar_arrive(smem_u32(&mc.k_full[ks]));
@@ -555,8 +556,8 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
     gb::pdl_wait();
     Item w{};                              // the current one
     int n = 0;                             // its tiles of this half
-    float m = -INFINITY, l = 0.f;          // the reference maximum, in powers of two; the denominator
-    float vref = -200.f;                   // log2 of the vs in whose units the sums are
+    // the references, in powers of two: of scores (the denominator's unit), of weights times vs (the accumulators')
+    float m = -INFINITY, c = -INFINITY, l = 0.f;
     while (ok) {
       put_queries(next);
       // ---- write the current one out
@@ -564,7 +565,7 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         if (!(ok = mbar_wait_warp(smem_u32(&mc.o_ready[half]), oph, abort_s, ran_out))) break;
         oph ^= 1;
         tc_fence_after_sync();
-        const float inv = l > 0.f ? fast_exp2(vref - UP) / l : l == l ? 0.f : l;        // (a score that is no number stays one)
+        const float inv = l > 0.f ? fast_exp2(c - m - UP) / l : l == l ? 0.f : l;        // (a score that is no number stays one)
         __nv_bfloat16* dst = p.out + ((size_t)(w.q_begin + w.tok0 + row / p.g) * p.Hq + w.kvh * p.g + row % p.g) * HD;
 #pragma unroll 2
         for (int h = 0; h < HD / 16; ++h) {
@@ -588,7 +589,7 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
       if (next.done) break;
       w = next.w, n = w.tiles_of(half, p.g);
       next.next_item(p);
-      m = -INFINITY, l = 0.f, vref = -200.f;
+      m = c = -INFINITY, l = 0.f;
       const int row_pos = row < w.nrows ? w.pos0 + row / p.g : -1;       // no key is valid for a padding row
       const int row_start = (row < w.nrows && p.window > 0) ? max(0, row_pos + 1 - p.window) : 0;
       // what all rows of this half read: up to the first row's position, from the last row's window on
@@ -603,14 +604,13 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         uint32_t sv[KT / 32][32];
 #pragma unroll
         for (int h = 0; h < KT / 32; ++h) tmem_ld_32(s_addr + h * 32, sv[h]);
-        float f[8], ev[8], ev_top = -200.f;            // of each sixteen keys: the scores' factor, log2 of vs
+        float f[8], ev[8];            // of each sixteen keys: the scores' factor, log2 of vs
         bool pages = true;
 #pragma unroll
         for (int b = 0; b < 8; ++b) {
           const float2 two = mc.scales[gt % SLOTS][b];
-          f[b] = two.x * factor, ev[b] = two.x >= 0.f ? two.y : -200.f;
+          f[b] = two.x * factor, ev[b] = two.y;
           pages = pages && two.x >= 0.f;
-          ev_top = fmaxf(ev_top, ev[b]);
         }
         tmem_ld_wait();
         auto sc = [&](int ch) -> float& { return reinterpret_cast<float&>(sv[ch >> 5][ch & 31]); };
@@ -632,24 +632,22 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
 #pragma unroll
           for (int b = 0; b < 8; ++b) f[b] = fmaxf(f[b], 0x1p-126f);
         }
-        // the maximum of each sixteen keys' raw products, times their factor
-        float m_new = m;
+        // the maximum of each sixteen keys' raw products, times their factor, and with vs
+        float m_new = m, c_new = c;
 #pragma unroll
         for (int b = 0; b < 8; ++b) {
           float mx = max3(sc(16 * b), sc(16 * b + 1), sc(16 * b + 2));
 #pragma unroll
           for (int ch = 3; ch < 15; ch += 2) mx = max3(mx, sc(16 * b + ch), sc(16 * b + ch + 1));
           mx = fmaxf(mx, sc(16 * b + 15));
-          m_new = fmaxf(m_new, mx * f[b]);
+          m_new = fmaxf(m_new, mx * f[b]), c_new = fmaxf(c_new, fmaf(mx, f[b], ev[b]));
         }
-        // The reference maximum moves only if some row of the warp has outgrown it by more than 2^8; then the warp rescales what it has
+        // The references move only if some row of the warp has outgrown one by more than 2^8; then the warp rescales what it has
         // accumulated (the loads and stores of tensor memory are the whole warp's). A row that has seen no valid key yet has
         // nothing to rescale.
-        const bool grown = (m != -INFINITY && m_new - m > RESCALE_ABOVE) || ev_top > vref;
+        const bool grown = m != -INFINITY && fmaxf(m_new - m, c_new - c) > RESCALE_ABOVE;
         if (j > 0 && __any_sync(0xffffffffu, grown)) {
-          const float own = m == -INFINITY ? 1.f : fast_exp2(m - m_new);
-          const float v_new = fmaxf(vref, ev_top), corr = own * fast_exp2(vref - v_new);
-          vref = v_new;
+          const float own = m == -INFINITY ? 1.f : fast_exp2(m - m_new), corr = m == -INFINITY ? 1.f : fast_exp2(c - c_new);
 #pragma unroll 1
           for (int h = 0; h < HD / 16; ++h) {
             uint32_t v[16];
@@ -660,19 +658,19 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
             tmem_st_16(o_addr + h * 16, v);
           }
           l *= own;
-          m = m_new;
-        } else {
-          if (m == -INFINITY) m = m_new;
-          vref = fmaxf(vref, ev_top);          // (j > 0: it is the larger one already)
+          m = m_new, c = c_new;
+        } else if (m == -INFINITY) {
+          m = m_new, c = c_new;
         }
-        const float neg_m = m == -INFINITY ? 0.f : -m;       // nothing valid yet: avoid inf - inf
-        // (2^-100 of the largest vs is nothing; and where nothing is read the probabilities are zeros.)
+        const float neg_m = m == -INFINITY ? 0.f : -m, vref = m == -INFINITY ? 0.f : c - m;       // nothing valid yet: avoid inf - inf
+        // (A page's vs counts as 2^-100 of vref at least, which is nothing, so that its keys have numbers for the denominator. Where nothing is
+        // read the probabilities are zeros.)
 #pragma unroll
         for (int h = 0; h < KT / 32; ++h) {                  // 32 keys: 16 columns of P, over scores that have been read
           uint32_t pk[16];
 #pragma unroll
           for (int b = 2 * h; b < 2 * h + 2; ++b) {
-            const float up = UP + fminf(fmaxf(ev[b] - vref, -100.f), 0.f), off = neg_m + up;
+            const float up = UP + fmaxf(ev[b] - vref, -100.f), off = neg_m + up;
             const float2 f2 = make_float2(f[b], f[b]), off2 = make_float2(off, off);
             float2 ls = make_float2(0.f, 0.f);
 #pragma unroll

@@ -49,6 +49,71 @@ SHAPES = [(4, 1, 64, 32), (32, 8, 128, 32), (16, 1, 128, 32), (12, 1, 64, 16), (
 FAR = [10, 20, 30, 40, 127]            # powers of two (of pages whose other scales are 2^-7; 2^120 is the largest there is)
 
 
+@pytest.mark.parametrize("heads,kv_heads,hd,page", SHAPES)
+@pytest.mark.parametrize("far", FAR)
+@pytest.mark.parametrize("lens", [[(1, 200), (1, 70)], [(1, 2600), (1, 900)], [(130, 200), (1, 70), (40, 100)]])
+def test_a_page_of_large_values_without_weight(ops, heads, kv_heads, hd, page, far, lens):  # noqa: F811
+    """Scores of the page lie more than 280 powers of two below the others: whatever its values, they count for nothing."""
+    cu, kv, table, q, k, v, ks, vs, scale = case(heads, kv_heads, hd, page, lens, far + hd)
+    for r in range(len(lens)):
+        at = table[r, 1].long()
+        k[at, :, :, 0] = -448.0
+        vs[at] = 2.0 ** (far - 7)
+    q[..., 0] = 300 * math.log(2) / (scale * 448 * 2.0 ** -7)
+    q, k8, v8 = q.to(torch.bfloat16), k.to(E4M3), v.to(E4M3)
+    args = (q, k8, v8, ks, vs, table, cu, kv, scale, 0, page)
+    check(attend(ops, *args, lens), *args)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,page", [(4, 1, 64, 32), (2, 1, 128, 32), (2, 2, 64, 16), (6, 2, 48, 32), (40, 2, 64, 32)])
+@pytest.mark.parametrize("far", FAR)
+@pytest.mark.parametrize("lens", [[(2, 33)], [(4, 130), (1, 33)], [(140, 161)], [(300, 321), (40, 65)]])
+def test_a_page_of_large_values_behind_a_row(ops, heads, kv_heads, hd, page, far, lens):  # noqa: F811
+    """The last page belongs to the last tokens: earlier rows of the same tile may not read it and know nothing of its scale."""
+    cu, kv, table, q, k, v, ks, vs, scale = case(heads, kv_heads, hd, page, lens, far + hd)
+    for r, (_, n) in enumerate(lens):
+        vs[table[r, (n - 1) // page].long()] = 2.0 ** (far - 7)
+    q, k8, v8 = q.to(torch.bfloat16), k.to(E4M3), v.to(E4M3)
+    args = (q, k8, v8, ks, vs, table, cu, kv, scale, 0, page)
+    if far == 127:                      # rows that read the page overflow: they are left out
+        out, (want, mag) = attend(ops, *args, lens), plain.attention(*args)
+        rows = (want.abs().amax(1) < 2.0 ** 60)
+        assert rows.sum() >= len(lens)
+        assert ((out.double() - want).abs() <= 2.0 ** -8 * (want.abs() + 1.5 * mag) + 2.0 ** -20)[rows].all()
+    else:
+        check(attend(ops, *args, lens), *args)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,page", SHAPES)
+@pytest.mark.parametrize("lens", [[(1, 150), (1, 40)], [(1, 5000)], [(1, 300 + 170 * i) for i in range(24)], [(5, 640), (200, 700)]])
+@pytest.mark.parametrize("window", [0, 100])
+def test_pages_of_every_size(ops, heads, kv_heads, hd, page, lens, window):  # noqa: F811
+    """Scales of values from 2^-40 to 2^40, of keys from 2^-10 to 2^-6, in any order: parts of a request have references of their own."""
+    cu, kv, table, q, k, v, ks, vs, scale = case(heads, kv_heads, hd, page, lens, hd + len(lens))
+    g = gen(hd)
+    vs = torch.pow(2.0, torch.randint(-40, 41, vs.shape, generator=g).float())
+    ks = torch.pow(2.0, torch.randint(-10, -5, ks.shape, generator=g).float())
+    q, k8, v8 = q.to(torch.bfloat16), k.to(E4M3), v.to(E4M3)
+    args = (q, k8, v8, ks, vs, table, cu, kv, scale, window, page)
+    check(attend(ops, *args, lens), *args)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,page", SHAPES)
+@pytest.mark.parametrize("lens", [[(1, 96), (1, 70)], [(1, 3000)], [(130, 200), (40, 100)]])
+@pytest.mark.parametrize("size", [-100, 8, 40])
+def test_pages_of_zeros_count_in_the_denominator(ops, heads, kv_heads, hd, page, lens, size):  # noqa: F811
+    """Pages of zeros have the smallest scale there is, 2^-100: their weight is in the sum of weights, next to values of any size."""
+    cu, kv, table, q, k, v, ks, vs, scale = case(heads, kv_heads, hd, page, lens, hd)
+    vs.fill_(2.0 ** size)
+    for r, (_, n) in enumerate(lens):
+        for j in range(0, -(-n // page), 2):
+            at = table[r, j].long()
+            v[at], vs[at] = 0.0, 2.0 ** -100
+    q, k8, v8 = q.to(torch.bfloat16), k.to(E4M3), v.to(E4M3)
+    args = (q, k8, v8, ks, vs, table, cu, kv, scale, 0, page)
+    check(attend(ops, *args, lens), *args)
+
+
 @pytest.mark.parametrize("heads,kv_heads,hd", [(40, 2, 64), (34, 2, 128), (128, 1, 64), (16, 1, 64)])
 def test_groups_of_many_heads_beside_requests_without_tokens(ops, heads, kv_heads, hd):  # noqa: F811
     lens = [(0, 7), (1, 90), (0, 0), (3, 33)]
