@@ -458,9 +458,12 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
     };
     auto put_queries = [&](int seg) {
       const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
-      float largest = 0.f;
+      float v[16], largest = 0.f;             // (scores with an infinite channel are infinite or no numbers, and their softmax is no number)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xFFFF0000u))));
+      for (int i = 0; i < 8; ++i) {
+        v[2 * i] = f8::spoil_infinity(__uint_as_float(w[i] << 16)), v[2 * i + 1] = f8::spoil_infinity(__uint_as_float(w[i] & 0xFFFF0000u));
+        largest = fmaxf(largest, fmaxf(fabsf(v[2 * i]), fabsf(v[2 * i + 1])));
+      }
 #pragma unroll
       for (int o = HD / 32; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
       const int e2 = f8::scale_exponent(largest);
@@ -468,8 +471,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float a = __uint_as_float(w[2 * i] << 16) * inv, b = __uint_as_float(w[2 * i] & 0xFFFF0000u) * inv;
-        const float c = __uint_as_float(w[2 * i + 1] << 16) * inv, d = __uint_as_float(w[2 * i + 1] & 0xFFFF0000u) * inv;
+        const float a = v[4 * i] * inv, b = v[4 * i + 1] * inv, c = v[4 * i + 2] * inv, d = v[4 * i + 3] * inv;
         hi[i] = f8::encode4(a, b, c, d);
         const float4 back = f8::decode4(hi[i]);
         lo[i] = f8::encode4(a - back.x, b - back.y, c - back.z, d - back.w);

@@ -526,7 +526,8 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
           float v[8], largest = 0.f;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            v[2 * e] = __uint_as_float(u[e] << 16), v[2 * e + 1] = __uint_as_float(u[e] & 0xFFFF0000u);
+            // (scores with an infinite channel are infinite or no numbers, and their softmax is no number)
+            v[2 * e] = f8::spoil_infinity(__uint_as_float(u[e] << 16)), v[2 * e + 1] = f8::spoil_infinity(__uint_as_float(u[e] & 0xFFFF0000u));
             largest = max3(largest, fabsf(v[2 * e]), fabsf(v[2 * e + 1]));
           }
 #pragma unroll

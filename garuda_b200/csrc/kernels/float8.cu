@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(128) attention_f8_simple_kernel(const Attentio
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int c = 128 * i + 4 * lane + e;
-      qv[i][e] = c < p.hd ? gb::to_float(q[c]) : 0.f;
+      qv[i][e] = c < p.hd ? spoil_infinity(gb::to_float(q[c])) : 0.f;      // (a softmax of infinite scores is no number)
       o[i][e] = 0.f;
     }
   float m = -INFINITY, l = 0.f;
@@ -369,7 +369,8 @@ __global__ void __launch_bounds__(128) attention_f8_simple_kernel(const Attentio
       }
       s = gb::warp_sum(s) * ks;
       const float m_new = fmaxf(m, s);
-      const float corr = m == m_new ? 1.f : exp2f(m - m_new), w = m_new == -INFINITY ? 0.f : exp2f(s - m_new);
+      // (a score that is no number stays one)
+      const float corr = m == m_new ? 1.f : exp2f(m - m_new), w = m_new == -INFINITY ? (s == s ? 0.f : s) : exp2f(s - m_new);
       m = m_new;
       l = l * corr + w;
       const float wv = w * vs;

@@ -114,6 +114,25 @@ def test_pages_of_zeros_count_in_the_denominator(ops, heads, kv_heads, hd, page,
     check(attend(ops, *args, lens), *args)
 
 
+@pytest.mark.parametrize("heads,kv_heads,hd,page", SHAPES + [(40, 2, 64, 32)])
+@pytest.mark.parametrize("lens", [[(1, 90), (1, 300)], [(1, 5000)], [(150, 200), (3, 40)]])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_a_query_that_is_not_finite_spoils_its_own_row_only(ops, heads, kv_heads, hd, page, lens, bad):  # noqa: F811
+    """An infinite channel makes scores that are infinite or no numbers, and a softmax of these is no number."""
+    cu, kv, table, q, k, v, ks, vs, scale = case(heads, kv_heads, hd, page, lens, hd)
+    q, k8, v8 = q.to(torch.bfloat16), k.to(E4M3), v.to(E4M3)
+    args = (k8, v8, ks, vs, table, cu, kv, scale, 0, page)
+    spoilt = q.clone()
+    spoilt[0, 1, 5] = bad
+    out = attend(ops, spoilt, *args, lens).view(q.shape)
+    assert torch.isnan(out[0, 1]).all()
+    want, mag = (t.view(q.shape) for t in plain.attention(q, *args))
+    keep = torch.ones(q.shape[:2], dtype=torch.bool)
+    keep[0, 1] = False
+    err = (out.double() - want).abs()
+    assert (err <= 2.0 ** -8 * (want.abs() + 1.5 * mag) + 1e-30)[keep].all()
+
+
 @pytest.mark.parametrize("heads,kv_heads,hd", [(40, 2, 64), (34, 2, 128), (128, 1, 64), (16, 1, 64)])
 def test_groups_of_many_heads_beside_requests_without_tokens(ops, heads, kv_heads, hd):  # noqa: F811
     lens = [(0, 7), (1, 90), (0, 0), (3, 33)]
