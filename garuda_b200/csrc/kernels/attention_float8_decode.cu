@@ -5,8 +5,8 @@
 //
 // Bound by the stream of codes, 2 * HD bytes a key and head, so they go from shared memory into the matrix instructions as they are
 // (tcgen05.mma kind f8f6f4, 32-bit sums), and what has more than four bits is split instead: a query row, scaled by a power of two to a largest
-// of at most 448, is the sum of two E4M3 rows (a bfloat16's eight bits are four and four; what is 2^-11 of the row's largest and below
-// loses bits that the sum does not see), and a weight exp(s) * vs is three codes, the second and third in units of 1/32 and 1/1024: twelve
+// of at most 448, is the sum of an E4M3 row and 1/16 of another (a bfloat16's eight bits are four and four: exact down to 2^-13 of the
+// row's largest; what is below that loses bits, and is gone below 2^-21), and a weight exp(s) * vs is three codes, the second and third in units of 1/32 and 1/1024: twelve
 // bits, down to 2^-24 of the reference. (Groups of more than eight heads: two codes, nine bits, down to 2^-22, and a reference that
 // follows every larger one.) Products of one tile of 128 keys:
 //   S^T [128 keys, N] = K [128, HD] * Q [N, HD]^T         N = 16 (or 32): the rows' codes, then what these leave
@@ -474,7 +474,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
         const float a = v[4 * i] * inv, b = v[4 * i + 1] * inv, c = v[4 * i + 2] * inv, d = v[4 * i + 3] * inv;
         hi[i] = f8::encode4(a, b, c, d);
         const float4 back = f8::decode4(hi[i]);
-        lo[i] = f8::encode4(a - back.x, b - back.y, c - back.z, d - back.w);
+        lo[i] = f8::encode4(16.f * (a - back.x), 16.f * (b - back.y), 16.f * (c - back.z), 16.f * (d - back.w));      // up to 16 * 16
       }
       if (qrow < ROWS) {
         uint8_t* to = base + 2 * S::P_BYTES + (seg & 1) * S::Q_BYTES;
@@ -524,7 +524,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
           tmem_ld_wait();
 #pragma unroll
           for (int r = 0; r < ROWS; ++r)
-            u[r] = fmaf(__uint_as_float(raw_s[r]) + __uint_as_float(raw_s[r + ROWS]), bars.factor[seg & 1][r] * sc.x, sc.y);
+            u[r] = fmaf(fmaf(__uint_as_float(raw_s[r + ROWS]), 0.0625f, __uint_as_float(raw_s[r])), bars.factor[seg & 1][r] * sc.x, sc.y);
         }
         if (!full) {
 #pragma unroll

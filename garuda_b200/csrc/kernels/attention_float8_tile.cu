@@ -15,8 +15,9 @@
 // its next scores (1,024 of products at the tensor cores' rate): the halves' chains, not a unit, set the pace. Two threads a row, sixteen
 // softmax warps, took 61 and 96; 32 scores at a time in a loop 63 and 94; a quarter of the exponentials as polynomials 63 and 85.
 //   * S is a product of codes as they lie (tcgen05.mma kind f8f6f4): a query row, scaled by a power of two to a largest of at most 448, is the
-//     sum of two E4M3 rows (a bfloat16's eight bits are four and four; what is 2^-11 of the row's largest and below loses bits
-//     that the sum does not see), so S = Qhi K^T + Qlo K^T at twice the rate of bfloat16: the same time, half of the keys' bytes.
+//     sum of two E4M3 rows (a bfloat16's eight bits are four and four: exact down to 2^-9 of the row's largest; what is below that
+//     loses bits, and is gone below 2^-17: both products add to the same sums, so the second row cannot have a finer unit), so
+//     S = Qhi K^T + Qlo K^T at twice the rate of bfloat16: the same time, half of the keys' bytes.
 //   * Values become halves (exactly: every E4M3 number is one) in shared memory, a conversion for two of them, by four warps of
 //     their own, for 256 rows' worth of products. (Splitting P into codes instead would cost the softmax warps two instructions a score.)
 //   * A page's ks goes into the factor of the exponent's multiply-add, its vs (as a power of two) into the constant; the denominator takes it

@@ -133,6 +133,40 @@ def test_a_query_that_is_not_finite_spoils_its_own_row_only(ops, heads, kv_heads
     assert (err <= 2.0 ** -8 * (want.abs() + 1.5 * mag) + 1e-30)[keep].all()
 
 
+@pytest.mark.parametrize("heads,kv_heads,hd,page", SHAPES[:4])
+@pytest.mark.parametrize("lens", [[(1, 90), (1, 30)], [(1, 2500)]])
+def test_single_tokens_with_a_channel_far_above_the_others(ops, heads, kv_heads, hd, page, lens):  # noqa: F811
+    """The keys have nothing in the large channel: the others, down to 2^-14 of it, make the scores, and are exact (bfloat16's eight bits are
+    the four of a code and the four of what it leaves, in units of 1/16)."""
+    cu, kv, table, q, k, v, ks, vs, scale = case(heads, kv_heads, hd, page, lens, hd)
+    g = gen(3)
+    q = torch.pow(2.0, -14 * torch.rand(q.shape, generator=g)) * torch.where(torch.rand(q.shape, generator=g) < 0.5, -1.0, 1.0) * 2.0 ** 14
+    low = torch.rand(q.shape[:2] + (hd // 2,), generator=g) + 1           # half of them between 1 and 2: the smallest
+    q[..., hd // 2:] = low
+    q[..., 0] = 2.0 ** 14 * 1.75
+    k[..., :hd // 2] = 0.0
+    ks = torch.full_like(ks, 2.0 ** -8)
+    q, k8, v8 = q.to(torch.bfloat16), k.to(E4M3), v.to(E4M3)
+    args = (q, k8, v8, ks, vs, table, cu, kv, 4.0, 0, page)
+    check(attend(ops, *args, lens), *args)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,page", [(4, 1, 64, 32), (4, 4, 128, 32)])
+@pytest.mark.parametrize("above", [8, 12])
+def test_portions_with_a_channel_far_above_the_others(ops, heads, kv_heads, hd, page, above):  # noqa: F811
+    """Both of a query's codes are in the unit of the first, 2^-9 of the scale at least: a channel is off by 2^-10 of it, and a score by as much for
+    every channel of the key."""
+    lens = [(130, 200), (40, 100)]
+    cu, kv, table, q, k, v, ks, vs, scale = case(heads, kv_heads, hd, page, lens, hd)
+    q[..., 0] = 1.75 * 2.0 ** above                                       # 448 times 2^(above - 8)
+    q[..., 1:] = q[..., 1:].clamp(-3, 3)
+    q, k8, v8 = q.to(torch.bfloat16), k.to(E4M3), v.to(E4M3)
+    args = (q, k8, v8, ks, vs, table, cu, kv, scale, 0, page)
+    out, (want, mag) = attend(ops, *args, lens), plain.attention(*args)
+    score_off = 2.0 ** (above - 18) * float(k8.float().abs().sum(-1).max()) * 2.0 ** -7 * scale
+    assert ((out.double() - want).abs() <= 2.0 ** -8 * (want.abs() + 1.5 * mag) + math.expm1(2 * score_off) * mag).all()
+
+
 @pytest.mark.parametrize("heads,kv_heads,hd", [(40, 2, 64), (34, 2, 128), (128, 1, 64), (16, 1, 64)])
 def test_groups_of_many_heads_beside_requests_without_tokens(ops, heads, kv_heads, hd):  # noqa: F811
     lens = [(0, 7), (1, 90), (0, 0), (3, 33)]
