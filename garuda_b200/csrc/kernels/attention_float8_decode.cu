@@ -458,16 +458,17 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
     };
     auto put_queries = [&](int seg) {
       const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
-      float v[16], largest = 0.f;             // (scores with an infinite channel are infinite or no numbers, and their softmax is no number)
+      float v[16], largest = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        v[2 * i] = f8::spoil_infinity(__uint_as_float(w[i] << 16)), v[2 * i + 1] = f8::spoil_infinity(__uint_as_float(w[i] & 0xFFFF0000u));
+        v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
         largest = fmaxf(largest, fmaxf(fabsf(v[2 * i]), fabsf(v[2 * i + 1])));
       }
 #pragma unroll
       for (int o = HD / 32; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
       const int e2 = f8::scale_exponent(largest);
-      const float inv = f8::power_of_two(-e2);
+      // (scores with an infinite channel are infinite or no numbers, and their softmax is no number)
+      const float inv = largest < INFINITY ? f8::power_of_two(-e2) : NAN;
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {

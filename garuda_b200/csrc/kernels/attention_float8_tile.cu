@@ -527,14 +527,14 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
           float v[8], largest = 0.f;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            // (scores with an infinite channel are infinite or no numbers, and their softmax is no number)
-            v[2 * e] = f8::spoil_infinity(__uint_as_float(u[e] << 16)), v[2 * e + 1] = f8::spoil_infinity(__uint_as_float(u[e] & 0xFFFF0000u));
+            v[2 * e] = __uint_as_float(u[e] << 16), v[2 * e + 1] = __uint_as_float(u[e] & 0xFFFF0000u);
             largest = max3(largest, fabsf(v[2 * e]), fabsf(v[2 * e + 1]));
           }
 #pragma unroll
           for (int o = LANES / 2; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
           const int e2 = f8::scale_exponent(largest);
-          const float inv = f8::power_of_two(-e2);
+          // (scores with an infinite channel are infinite or no numbers, and their softmax is no number)
+          const float inv = largest < INFINITY ? f8::power_of_two(-e2) : NAN;
           uint32_t hi[2], lo[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {

@@ -340,7 +340,8 @@ __global__ void __launch_bounds__(128) attention_f8_simple_kernel(const Attentio
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int c = 128 * i + 4 * lane + e;
-      qv[i][e] = c < p.hd ? spoil_infinity(gb::to_float(q[c])) : 0.f;      // (a softmax of infinite scores is no number)
+      const float x = c < p.hd ? gb::to_float(q[c]) : 0.f;
+      qv[i][e] = x + (x - x);      // (NaN for an infinity: a softmax of infinite scores is no number)
       o[i][e] = 0.f;
     }
   float m = -INFINITY, l = 0.f;

@@ -23,9 +23,6 @@ __device__ __forceinline__ int scale_exponent(float largest) {
 // 2^e for e from -126 to 127
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// x, but NaN for an infinity: where an infinite number is to spoil what is made of it (a code would make 448 of it).
-__device__ __forceinline__ float spoil_infinity(float x) { return x + (x - x); }
-
 // Two values as codes, the first in the lower byte; beyond 448 (infinity too) 448, NaN stays NaN.
 __device__ __forceinline__ uint16_t encode2(float first, float second) {
   uint16_t r;
