@@ -148,14 +148,15 @@ class Engine:
             self.runner.graphs = DecodeGraphs(self.runner, max_concurrent)
 
     def _check_float8(self, weights: bool, cache: bool) -> None:
-        """Refuses 8 bits for a model with a part that does not know them."""
+        """Refuses 8 bits for a model with a part that does not know them, or not at its head size."""
         for block in self.model.blocks:
             for part, _ in block.parts():
                 matrices = any(ts.role == "matrix" for ts in part.tensors().values())
                 if weights and matrices and not part.holds_matrices:
                     raise ConfigError(f"weight_dtype: {type(part).__name__} does not hold its matrices in 8 bits")
             if cache and block.mixer.cache_need() is not None and not block.mixer.takes_float8_cache:
-                raise ConfigError(f"cache_dtype: {type(block.mixer).__name__} does not keep its cache in 8 bits")
+                heads = f" with heads of {block.mixer.head_dim} channels" if hasattr(block.mixer, "head_dim") else ""
+                raise ConfigError(f"cache_dtype: {type(block.mixer).__name__}{heads} does not keep its cache in 8 bits")
 
     @classmethod
     def from_config(cls, cfg: EngineConfig, **overrides) -> "Engine":

@@ -76,7 +76,11 @@ class PagedAttention(Mixer):
     takes_pending_norm = True
     emits_norm = True
     holds_matrices = True
-    takes_float8_cache = True
+
+    @property
+    def takes_float8_cache(self):
+        """Heads of a multiple of 16 channels, up to 256, as the kernels over pages of codes take them."""
+        return self.head_dim % 16 == 0 and self.head_dim <= 256
 
     def _write_float8(self, ctx, h, w_qkv, q, cache, writes):
         """Queries to ``q``, keys and values into pages in 8 bits: the product in 32-bit, then one kernel that rotates, scales and stores."""

@@ -132,7 +132,7 @@ class Part:
     output_bias = None
     #: Whether the part gives all of its matrices to the kernel set to hold (``hold_matrix``), so that they may be held in 8 bits.
     holds_matrices = False
-    #: Whether a mixer with a paged cache can read and write one in 8 bits (``LayerCache.k_scale``).
+    #: Whether a mixer with a paged cache, of its head size, can read and write one in 8 bits (``LayerCache.k_scale``).
     takes_float8_cache = False
 
     def tensors(self) -> Dict[str, TensorSpec]:

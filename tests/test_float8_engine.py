@@ -59,3 +59,20 @@ def test_pages_in_8_bits():
     for cache in small.layer_caches(tables):
         assert cache.k_scale.shape == cache.v_scale.shape == cache.k.shape[:2]
     assert all(c.k_scale is None for c in plain.layer_caches(tables))
+
+
+@pytest.mark.parametrize("head_dim,taken", [(16, True), (80, True), (256, True), (8, False), (20, False), (100, False), (272, False)])
+def test_head_sizes_that_no_8_bit_kernel_takes_are_refused_when_the_engine_is_made(head_dim, taken):
+    from garuda_b200.config.registry import build_model
+    from garuda_b200.engine.engine import Engine
+
+    class Half:
+        _check_float8 = Engine._check_float8
+    half = Half()
+    _, half.model = build_model(dict(TINY["A"][0], head_dim=head_dim))
+    half._check_float8(True, False)              # the weights know no heads
+    if taken:
+        half._check_float8(False, True)
+    else:
+        with pytest.raises(ConfigError, match=f"heads of {head_dim} channels"):
+            half._check_float8(False, True)
