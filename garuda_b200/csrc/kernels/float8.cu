@@ -186,8 +186,8 @@ __global__ void __launch_bounds__(APPEND_THREADS, WARPS == 1 ? 2 : 4) append_ker
   const int pos0 = p.kv_lens[r] - q_len;
   const int page_index = pos0 / p.page + (slot - (begin / p.page + 2 * r));
   const int first = max(pos0, page_index * p.page), last = min(p.kv_lens[r], (page_index + 1) * p.page);
-  if (q_len <= 0 || first >= last || page_index >= p.table_width) return;
-  const int at = p.table[(size_t)r * p.table_width + page_index];
+  if (q_len <= 0 || first >= last) return;
+  const int at = page_index < p.table_width ? p.table[(size_t)r * p.table_width + page_index] : -1;       // (no page: the queries are written all the same)
   const int n = last - first, held = first - page_index * p.page;
   const int tok0 = begin + first - pos0;
 

@@ -220,7 +220,8 @@ class Float8Ops:
         (``CudaOps.rope_table``; None: leave them; ``interleaved``: pairs (2i, 2i + 1) in place of (i, i + head_dim / 2)), write the
         queries to ``q_out [T, heads, head_dim]``, and keys and values in 8 bits into their pages ``[pages, kv_heads, page_size,
         head_dim]`` with one scale per page and head ``[pages, kv_heads]``. Request r's tokens ``cu_q[r]`` to ``cu_q[r + 1]`` are its last
-        positions of ``kv_lens[r]``; a page that held positions before them keeps these, in its new scale where that has grown."""
+        positions of ``kv_lens[r]``; a page that held positions before them keeps these, in its new scale where that has grown. Where the
+        block table has no page (-1, or beyond its width) keys and values go nowhere."""
         what = "kv_append_float8"
         T, width = qkv.shape
         R = self._check_cache(what, k_pool, v_pool, k_scale, v_scale, cu_q, kv_lens, block_table, kv_heads, page_size, head_dim)
