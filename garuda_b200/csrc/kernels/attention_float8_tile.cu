@@ -766,12 +766,12 @@ int launch(const Params& p, const CUtensorMap& km, const CUtensorMap& vm, int q_
 
 }  // namespace
 
-// Heads of 64 or 128, pages of 16, 32, 64 or 128 keys, up to 256 query heads a group; for requests of more than decode_rows(g) rows (new tokens
+// Heads of 64 or 128, pages of 16, 32, 64 or 128 keys, up to 128 query heads a group; for requests of more than decode_rows(g) rows (new tokens
 // times heads of a group), the others are left.
 GB_EXPORT int gb_f8_attention_tile(const void* q, const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale, const void* table,
                                    int table_width, const void* cu_q, const void* kv_lens, void* out, int R, long long pages, int Hq, int Hkv, int hd,
                                    float scale, int window, int page, int max_q_len, void* stream) {
-  if (R <= 0 || Hkv <= 0 || Hq % Hkv || (hd != 64 && hd != 128) || page < 16 || page > 128 || (page & (page - 1)) || Hq / Hkv > QROWS ||
+  if (R <= 0 || Hkv <= 0 || Hq % Hkv || (hd != 64 && hd != 128) || page < 16 || page > 128 || (page & (page - 1)) || Hq / Hkv > HALF ||
       (uintptr_t)q % 16 || (uintptr_t)out % 16 || (uintptr_t)k_pool % 16 || (uintptr_t)v_pool % 16)
     return gb::fail(GB_BAD_ARGUMENT, "attention_f8_tile: %d requests, heads %d / %d of %d, pages of %d", R, Hq, Hkv, hd, page);
   CUtensorMap km, vm;

@@ -537,6 +537,11 @@ struct Plan {
   long long units;          // of the tiles behind the rounds
 };
 
+// Shared memory for the stages. Three of two units fit for every pair of CTAs, whose units hold half of the tokens: pairs come with two
+// units to a stage only.
+constexpr int ROOM_BYTES = SMEM_LIMIT - 1024 - STATIC_BYTES - SF_STAGES * SF_BYTES;
+static_assert(3 * 2 * (BM + MAX_NT / 2) * BK <= ROOM_BYTES, "a pair's stages");
+
 // What a product of this shape would take, in microseconds, with `tiles` tiles of tokens, in pairs or not: the plan and its time, from what
 // was measured here. An SM takes in 115 KB a microsecond from L2, all together 11 MB, and 6.4 MB from memory; a step of a unit takes the issuing warp
 // 0.26 us (two units to a stage: 0.15 each), products of 256 tokens 0.27; a part of a tile costs its bytes once out and once in, and
@@ -549,9 +554,9 @@ Plan plan_of(int M, int N, int K, int tiles, bool pair, double* us_out) {
   const int ctas = pair ? 2 : 1, blocks = (K + BK - 1) / BK;
   q.tiles_n = (N + BM * ctas - 1) / (BM * ctas);
   const long long tiles_all = (long long)q.tiles_m * q.tiles_n, units = tiles_all * blocks;
-  const int unit = (BM + q.nt / ctas) * BK, room_bytes = SMEM_LIMIT - 1024 - STATIC_BYTES - SF_STAGES * SF_BYTES;
-  q.step = room_bytes / (2 * unit) >= 3 ? 2 : 1;           // two units to a stage where three such stages fit (4096 x 28672 x 4096: 354 us against 386)
-  q.stages = room_bytes / (q.step * unit) < MAX_STAGES ? room_bytes / (q.step * unit) : MAX_STAGES;
+  const int unit = (BM + q.nt / ctas) * BK;
+  q.step = ROOM_BYTES / (2 * unit) >= 3 ? 2 : 1;           // two units to a stage where three such stages fit (4096 x 28672 x 4096: 354 us against 386)
+  q.stages = ROOM_BYTES / (q.step * unit) < MAX_STAGES ? ROOM_BYTES / (q.step * unit) : MAX_STAGES;
   const int room = tc_host::sm_count() / ctas;
   q.workers = (int)(units < room ? units : room);
   q.rounds = (int)(tiles_all / q.workers);
@@ -654,7 +659,7 @@ GB_EXPORT int gb_f8_linear(const void* a, int a_tag, long long lda, const void* 
   const Args args{(const uint32_t*)xs, (const float*)ws, out, (float*)(xs + scale_bytes(M, K)), (int*)counters, M, N, (K + BK - 1) / BK, q.nt,
                   q.tiles_m, q.stages, q.workers, q.rounds, q.units, q.share, accumulate ? alpha : 1.0f};
   const bool add = accumulate != 0;
-  if (q.pair) return q.step == 2 ? launch_out<true, 2>(q, wm, xm, args, out_tag, add, st) : launch_out<true, 1>(q, wm, xm, args, out_tag, add, st);
+  if (q.pair) return launch_out<true, 2>(q, wm, xm, args, out_tag, add, st);
   return q.step == 2 ? launch_out<false, 2>(q, wm, xm, args, out_tag, add, st) : launch_out<false, 1>(q, wm, xm, args, out_tag, add, st);
 }
 
