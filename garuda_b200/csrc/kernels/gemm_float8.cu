@@ -634,6 +634,16 @@ GB_EXPORT long long gb_f8_linear_scratch_bytes(int M, int N, int K, long long* c
   return code_bytes(M, K) + scale_bytes(M, K) + part_bytes(q);
 }
 
+// How a product of this shape is cut: CTAs of a worker, units of a stage, tokens of a tile, tiles, workers, rounds of whole tiles, and of the tiles
+// behind these the workers that share them.
+GB_EXPORT int gb_f8_linear_plan(int M, int N, int K, int* out) {
+  if (M <= 0 || N <= 0 || K <= 0) return gb::fail(GB_BAD_ARGUMENT, "linear_float8_plan: %d x %d x %d", M, N, K);
+  const Plan q = make_plan(M, N, K);
+  const int values[7] = {q.pair ? 2 : 1, q.step, q.nt, q.tiles_m * q.tiles_n, q.workers, q.rounds, q.share};
+  for (int i = 0; i < 7; ++i) out[i] = values[i];
+  return GB_OK;
+}
+
 // out [M, N] (+)= q(a) w^T: a [M, K] with rows lda apart (gated: [M, 2 K], rows [gate | up], multiplied as silu(gate) * up), w [N, K] codes
 // with rows w_pitch apart, ws its scales.
 GB_EXPORT int gb_f8_linear(const void* a, int a_tag, long long lda, const void* w, long long w_pitch, const void* ws, void* out, int out_tag, int M,

@@ -55,6 +55,7 @@ _FLOAT8_SIGNATURES = {
     "gb_f8_attention_decode_set_error_sink": [c_void_p],
     "gb_f8_linear": [c_void_p, c_int, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p,
                      c_void_p, c_void_p],
+    "gb_f8_linear_plan": [c_int, c_int, c_int, c_void_p],
     "gb_f8_gemm_error_check": [],
     "gb_f8_gemm_set_error_sink": [c_void_p],
 }
@@ -181,6 +182,13 @@ class Float8Ops:
         self._check(L, L.gb_f8_linear(a.data_ptr(), _tag(a, "linear_float8 input"), a_row, values.data_ptr(), w_row if N > 1 else (K + 15) // 16 * 16,
                                       scales.data_ptr(), out.data_ptr(), out_tag, M, N, K, accumulate, alpha, bool(gated), counters.data_ptr(),
                                       scratch.data_ptr(), stream), "linear_float8", 2)
+
+    def linear_float8_plan(self, M: int, N: int, K: int) -> dict:
+        """How ``linear_float8`` cuts a product of this shape: ``ctas`` that work on a tile together, channel ``blocks`` (of 128) to a stage,
+        ``tokens`` of a tile, ``tiles``, ``workers``, ``rounds`` in which every worker has a whole tile, and how many ``share`` the rest."""
+        values = (c_int * 7)()
+        self._check(self.float8_lib, self.float8_lib.gb_f8_linear_plan(M, N, K, values), "linear_float8_plan", 0)
+        return dict(zip(("ctas", "blocks", "tokens", "tiles", "workers", "rounds", "share"), values))
 
     def swiglu_float8(self, ctx, h, w_gate_up, w_down, out, accumulate: bool = False):
         """``out (+)= q(silu(g) * u) @ w_down^T`` with ``[g | u] = q(h) @ w_gate_up^T``, both weights ``Float8Weight``. Gate and up are kept
