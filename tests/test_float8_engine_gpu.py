@@ -121,3 +121,30 @@ def test_replay_from_the_command_line(tmp_path):
     for step, row in ((0, 32), (1, 33)):
         got = np.fromfile(next(str(p) for p in tmp_path.iterdir() if p.name.startswith(f"{step}.")), dtype=np.float32)
         assert off(got, held[row]) <= BOTH_OFF
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+def test_preemption_over_a_cache_in_8_bits(graphs):
+    """A pool too small for all requests: some are sent back and start again, in pages that others have used. What pages held and what scales they
+    had counts for nothing (codes that are no numbers and scales of 2^60 to begin with). A request that starts again goes in at once with
+    what it had got token by token, whose codes may differ; so every chosen token is held against the plain model: its logit is the
+    largest but for what the cache's codes move two logits by."""
+    from garuda_b200 import Engine, SamplingParams
+    prompts = [random_tokens("A", 20, 70 + i) for i in range(3)]
+    tight = Engine(model_dir("A", torch.bfloat16), dtype="bfloat16", page_size=8, kv_tokens=96, max_concurrent=3, cuda_graphs=graphs,
+                   cache_dtype="float8_e4m3")
+    for pool, scales in zip(tight.cache.k_pools + tight.cache.v_pools, tight.cache.k_scales + tight.cache.v_scales):
+        pool.view(torch.uint8).fill_(0x7F)
+        scales.fill_(2.0 ** 60)
+    got = tight.generate(prompts, SamplingParams.greedy(max_tokens=24))
+    st = tight.stats()
+    assert st["preemptions"] > 0 and st["completed"] == len(prompts) and st["pages_free"] == st["pages_total"]
+    cfg = TINY["A"][0]
+    w = folder_weights(model_dir("A", torch.bfloat16))
+    for prompt, r in zip(prompts, got):
+        assert len(r.tokens) == 24
+        want = llama_plain.forward(cfg, w, prompt + r.tokens[:-1])
+        assert off(logits_of(tight, prompt + r.tokens[:-1], [20, 20] + [1] * 3), want) <= CACHE_OFF        # in the same pages, once more
+        rows = want[len(prompt) - 1:]
+        assert (rows.max(1) - rows[np.arange(24), r.tokens] <= 2 * CACHE_OFF * np.linalg.norm(rows, axis=1)).all()
+    tight.check_errors()

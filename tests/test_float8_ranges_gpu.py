@@ -22,7 +22,7 @@ def attend(ops, q, k8, v8, ks, vs, table, cu, kv, scale, window, page, lens):
 
 
 def check(out, q, k8, v8, ks, vs, table, cu, kv, scale, window, page):
-    """A result in bfloat16 is off by 2^-9 of itself, and by the weights' roundings: 2^-8 of the magnitudes' sum at most (two codes; three and
+    """A result in bfloat16 is off by 2^-8 of itself, and by the weights' roundings: 2^-8 of the magnitudes' sum at most (two codes; three and
     halves less). What is 2^-22 of the row's largest weight times its scale or less may be gone, times a code of 448 a key."""
     want, mag = plain.attention(q, k8, v8, ks, vs, table, cu, kv, scale, window, page)
     ones = torch.ones(v8.shape, dtype=torch.float32).to(E4M3)
@@ -165,6 +165,28 @@ def test_portions_with_a_channel_far_above_the_others(ops, heads, kv_heads, hd, 
     out, (want, mag) = attend(ops, *args, lens), plain.attention(*args)
     score_off = 2.0 ** (above - 18) * float(k8.float().abs().sum(-1).max()) * 2.0 ** -7 * scale
     assert ((out.double() - want).abs() <= 2.0 ** -8 * (want.abs() + 1.5 * mag) + math.expm1(2 * score_off) * mag).all()
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,page,new", [(32, 4, 64, 32, 1), (64, 8, 128, 32, 1), (64, 4, 128, 32, 1), (8, 8, 64, 32, 40), (8, 8, 128, 32, 40),
+                                                        (6, 2, 48, 32, 40)])
+def test_the_weights_last_bits(ops, heads, kv_heads, hd, page, new):  # noqa: F811
+    """Few keys whose values cancel but for the weights' differences, so that the result's own rounding hides little; and that rounding is allowed for
+    exactly: the result lies between the exact one, less and more what weights may be off by, each rounded to bfloat16. A weight is off
+    by 2^-12 of itself (three codes of four bits; halves 2^-11; two codes, for groups of more than eight heads, 2^-8), its exponential by
+    2^-21 and, through the score's roundings, by 2^-20 of the score; the queries are exact."""
+    group = heads // kv_heads
+    lens = [(new, max(new, 2 + i % 5)) for i in range(24)]
+    cu, kv, table, q, k, v, ks, vs, _ = case(heads, kv_heads, hd, page, lens, hd)
+    q = (torch.randint(-64, 65, q.shape, generator=gen(1)) / 32.0)                      # seven bits, every channel above 2^-11 of the largest or zero
+    v = torch.where(torch.rand(v.shape, generator=gen(2)) < 0.5, -256.0, 256.0)
+    q, k8, v8 = q.to(torch.bfloat16), k.to(E4M3), v.to(E4M3)
+    args = (q, k8, v8, ks, vs, table, cu, kv, 0.1, 0, page)
+    out = attend(ops, *args, lens)
+    want, mag = plain.attention(*args)
+    unit = 2.0 ** -11 if new > 1 else 2.0 ** -12 if group <= 8 else 2.0 ** -8
+    off = (unit + 2.0 ** -15) * mag
+    low, high = ((want + sign * off).to(torch.float32).to(torch.bfloat16) for sign in (-1, 1))
+    assert ((low <= out) & (out <= high)).all()
 
 
 @pytest.mark.parametrize("heads,kv_heads,hd", [(40, 2, 64), (34, 2, 128), (128, 1, 64), (16, 1, 64)])
