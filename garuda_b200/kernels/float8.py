@@ -18,6 +18,8 @@ from .checks import _TAG, KernelError, _need, _tag
 
 BLOCK = 128
 E4M3 = torch.float8_e4m3fn
+# (what torch.cuda.is_current_stream_capturing is, without the call around it)
+_capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
 class Float8Weight(NamedTuple):
@@ -103,16 +105,21 @@ class Float8Ops:
             self._float8 = L
         return self._float8
 
-    def _scratch8(self, name, nbytes, ws, stream, zero=False):
-        """Scratch bytes of this name: the call's workspace, the running step's, or one per stream."""
+    def _scratch8(self, name, nbytes, counters, counter_bytes, ws, stream):
+        """Scratch bytes and counters (cleared when they are made) of these names: from the call's workspace, the running step's, or one per
+        stream. A call that is captured without a workspace has memory of its graph's own, cleared in the graph: what the set keeps may
+        never have been cleared, if the graph that it was made in does not run."""
         if ws is None:
             ws = self.step_ws
         if ws is None:
+            if _capturing():
+                return (torch.empty(nbytes, dtype=torch.uint8, device=self.device),
+                        torch.zeros(counter_bytes, dtype=torch.uint8, device=self.device))
             ws = self._float8_scratch.get(stream)
             if ws is None:
                 from ..engine.batch import Workspace
                 ws = self._float8_scratch[stream] = Workspace(self.device)
-        return ws.get(name, (nbytes,), torch.uint8, zero=zero)
+        return ws.get(name, (nbytes,), torch.uint8), ws.get(counters, (counter_bytes,), torch.uint8, zero=True)
 
     def float8_error_code(self) -> int:
         """The code of a wait that an 8-bit kernel gave up since the last check, or 0; synchronises and clears."""
@@ -149,24 +156,30 @@ class Float8Ops:
         (``float8_weight`` makes none) turns the results of its 128 rows into NaN. ``gated``: ``a [M, 2 K]`` has rows ``[gate | up]``, and
         ``silu(gate) * up`` is rounded to 8 bits, from 32, and multiplied."""
         values, scales = w
-        _need(a.is_cuda and values.is_cuda and scales.is_cuda and out.is_cuda, "kernel operands must live on the CUDA device")
-        _need(a.dim() == 2 and values.dim() == 2 and out.dim() == 2, "linear_float8: operands must be matrices")
+        # (one condition, taken apart when it fails)
+        out_tag = _TAG.get(out.dtype)
+        if not (a.is_cuda and values.is_cuda and scales.is_cuda and out.is_cuda and a.dim() == 2 and values.dim() == 2 and out.dim() == 2):
+            _need(a.is_cuda and values.is_cuda and scales.is_cuda and out.is_cuda, "kernel operands must live on the CUDA device")
+            raise KernelError("linear_float8: operands must be matrices")
         M, width = a.shape
         N, K = values.shape
         a_row, w_row = a.stride(0), values.stride(0)
-        if not (width == (2 * K if gated else K) and out.shape == (M, N)):
-            _need(False, f"linear_float8: shapes {tuple(a.shape)} x {tuple(values.shape)} -> {tuple(out.shape)}")
-        _need(K > 0, "linear_float8: no channels")
-        _need(values.dtype is E4M3, "linear_float8: weights must be float8_e4m3fn")
-        _need(scales.dtype is torch.float32 and scales.is_contiguous() and scales.shape == ((N + 127) // 128, (K + 127) // 128),
-              "linear_float8: one float32 scale per block of 128 x 128")
-        _need((values.stride(1) == 1 or K == 1) and (w_row % 16 == 0 or N <= 1) and values.data_ptr() % 16 == 0,
-              "linear_float8: rows of codes must start on 16 bytes (float8_weight makes such)")
-        _need(a.stride(1) == 1 or K == 1, "linear_float8: rows of a must have unit stride")
-        out_tag = _TAG.get(out.dtype)
-        _need(out_tag is not None and out.is_contiguous(), "linear_float8: out must be contiguous, bfloat16 or float32")
-        _need(not accumulate or out_tag == 0, "linear_float8: accumulates into float32 only")
-        _need(accumulate or alpha == 1.0, "linear_float8: a multiplier goes with accumulation only")
+        if not (width == (2 * K if gated else K) and out.shape == (M, N) and K > 0 and values.dtype is E4M3 and scales.dtype is torch.float32
+                and scales.is_contiguous() and scales.shape == ((N + 127) // 128, (K + 127) // 128) and (values.stride(1) == 1 or K == 1)
+                and (w_row % 16 == 0 or N <= 1) and values.data_ptr() % 16 == 0 and (a.stride(1) == 1 or K == 1) and out_tag is not None
+                and out.is_contiguous() and (out_tag == 0 if accumulate else alpha == 1.0)):
+            _need(width == (2 * K if gated else K) and out.shape == (M, N),
+                  f"linear_float8: shapes {tuple(a.shape)} x {tuple(values.shape)} -> {tuple(out.shape)}")
+            _need(K > 0, "linear_float8: no channels")
+            _need(values.dtype is E4M3, "linear_float8: weights must be float8_e4m3fn")
+            _need(scales.dtype is torch.float32 and scales.is_contiguous() and scales.shape == ((N + 127) // 128, (K + 127) // 128),
+                  "linear_float8: one float32 scale per block of 128 x 128")
+            _need((values.stride(1) == 1 or K == 1) and (w_row % 16 == 0 or N <= 1) and values.data_ptr() % 16 == 0,
+                  "linear_float8: rows of codes must start on 16 bytes (float8_weight makes such)")
+            _need(a.stride(1) == 1 or K == 1, "linear_float8: rows of a must have unit stride")
+            _need(out_tag is not None and out.is_contiguous(), "linear_float8: out must be contiguous, bfloat16 or float32")
+            _need(not accumulate or out_tag == 0, "linear_float8: accumulates into float32 only")
+            raise KernelError("linear_float8: a multiplier goes with accumulation only")
         if M == 0 or N == 0:
             return
         L, stream = self.float8_lib, self._stream()
@@ -177,8 +190,7 @@ class Float8Ops:
             if len(self._float8_sizes) > 4096:
                 self._float8_sizes.clear()
             sizes = self._float8_sizes[M, N, K] = (scratch_bytes, int(counter_bytes.value))
-        scratch = self._scratch8("float8_linear", sizes[0], ws, stream)
-        counters = self._scratch8("float8_counters", sizes[1], ws, stream, zero=True)
+        scratch, counters = self._scratch8("float8_linear", sizes[0], "float8_counters", sizes[1], ws, stream)
         self._check(L, L.gb_f8_linear(a.data_ptr(), _tag(a, "linear_float8 input"), a_row, values.data_ptr(), w_row if N > 1 else (K + 15) // 16 * 16,
                                       scales.data_ptr(), out.data_ptr(), out_tag, M, N, K, accumulate, alpha, bool(gated), counters.data_ptr(),
                                       scratch.data_ptr(), stream), "linear_float8", 2)
@@ -257,15 +269,17 @@ class Float8Ops:
         T, Hq, hd = q.shape
         Hkv = k_pool.shape[1]
         R = self._check_cache(what, k_pool, v_pool, k_scale, v_scale, cu_q, kv_lens, block_table, Hkv, page_size, hd)
-        _need(q.is_cuda and out.is_cuda, "kernel operands must live on the CUDA device")
-        _need(R == num_requests, "paged_attention_float8: as many lengths as requests")
-        _need(Hq % Hkv == 0 and hd % 16 == 0 and hd <= 256, "paged_attention_float8: heads in whole groups, of a multiple of 16 channels up to 256")
-        _need(q.is_contiguous() and out.is_contiguous() and out.shape == (T, Hq * hd) and q.dtype is out.dtype, "paged_attention_float8: q/out shape")
-        q_ptr, out_ptr = q.data_ptr(), out.data_ptr()
-        _need(not (q_ptr | out_ptr) & 7, "paged_attention_float8: q and out on 8 bytes")
-        _need(scale > 0, "paged_attention_float8: a positive scale")
-        table_width = block_table.shape[1]
-        _need(table_width * page_size >= max_kv_len, "paged_attention_float8: the block table is too narrow for that many positions")
+        q_ptr, out_ptr, table_width = q.data_ptr(), out.data_ptr(), block_table.shape[1]
+        if not (q.is_cuda and out.is_cuda and R == num_requests and Hq % Hkv == 0 and hd % 16 == 0 and hd <= 256 and q.is_contiguous()
+                and out.is_contiguous() and out.shape == (T, Hq * hd) and q.dtype is out.dtype and not (q_ptr | out_ptr) & 7 and scale > 0
+                and table_width * page_size >= max_kv_len):          # (one condition, taken apart when it fails)
+            _need(q.is_cuda and out.is_cuda, "kernel operands must live on the CUDA device")
+            _need(R == num_requests, f"{what}: as many lengths as requests")
+            _need(Hq % Hkv == 0 and hd % 16 == 0 and hd <= 256, f"{what}: heads in whole groups, of a multiple of 16 channels up to 256")
+            _need(q.is_contiguous() and out.is_contiguous() and out.shape == (T, Hq * hd) and q.dtype is out.dtype, f"{what}: q/out shape")
+            _need(not (q_ptr | out_ptr) & 7, f"{what}: q and out on 8 bytes")
+            _need(scale > 0, f"{what}: a positive scale")
+            raise KernelError(f"{what}: the block table is too narrow for that many positions")
         if T == 0:
             return
         L, g, stream = self.float8_lib, Hq // Hkv, self._stream()
@@ -276,8 +290,8 @@ class Float8Ops:
             # sixteen heads have none of a few (a request without tokens is nobody's)
             few = (8 if g <= 8 else 16) if g <= 16 else 0
             if few and min_q_len * g <= few:
-                scratch = self._scratch8("float8_attention_parts", self._float8_part_bytes, ws, stream)
-                counters = self._scratch8("float8_attention_counters", 4 * R * Hkv, ws, stream, zero=True)
+                scratch, counters = self._scratch8("float8_attention_parts", self._float8_part_bytes, "float8_attention_counters", 4 * R * Hkv, ws,
+                                                   stream)
                 self._check(L, L.gb_f8_attention_decode(
                     q_ptr, *pools, R, k_pool.shape[0], Hq, Hkv, hd, scale, window, page_size, max_kv_len, scratch.data_ptr(),
                     counters.data_ptr(), stream), what)
