@@ -566,7 +566,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
             if (r >= w.nrows) continue;
             const float top = fmaxf(ref[r], fmaxf(fmaxf(bars.top[0][r], bars.top[1][r]), fmaxf(bars.top[2][r], bars.top[3][r])));
             const float corr = ref[r] == -INFINITY ? 0.f : exp2_fast(ref[r] - top);
-            l[r] = ref[r] == -INFINITY ? l[r] : times_power(l[r], ref[r] - top);
+            if (j > 0 && ref[r] != -INFINITY) l[r] = times_power(l[r], ref[r] - top);
             ref[r] = top;
             if (x == r) bars.corr[r] = corr;
           }
