@@ -35,7 +35,7 @@
 // Two CTAs an SM (N = 16; one with N = 32). Every wait is bounded.
 // Few short heads (CLUSTER): one head to a thread-block cluster, whose CTAs share its tiles and store their rows of sums into the shared
 // memory of the first, which adds them up in the CTAs' order behind a barrier of the cluster. (Asynchronous stores counted on a barrier in
-// memory took 2 us for 400 of them.) 4 requests of 65,536 positions, 8 heads of 128: 5.9 TB/s; one of 500: 6.9 us; 8 of 2,048, 4 of 64: 11.2.
+// memory took 2 us for 400 of them.) 4 requests of 65,536 positions, 8 heads of 128: 5.9 TB/s from a graph (5.4 a call from Python); one of 500: 7.1 us; 8 of 2,048, 4 of 64: 11.0.
 #include "attention_float8.cuh"
 #include "error_word.cuh"
 #include "tc_common.cuh"

@@ -62,7 +62,8 @@ class Engine:
         one decode step, sized from the measured times of the steps (garuda/src/scheduler/mod.rs:305-370).
         ``weight_dtype="float8_e4m3"``: the layers' matrices are held in 8 bits, with a scale per 128 x 128, and multiplied in 8 bits (tokens
         are rounded with a scale per 128 channels); the embedding, the head and the norms stay as they are. ``cache_dtype=
-        "float8_e4m3"``: keys and values are, with a scale per page and head. For models whose layers know them (the Llama decoder)."""
+        "float8_e4m3"``: keys and values are, with a scale per page and head. For models whose layers know them (the Llama decoder); a cache
+        in 8 bits for heads of a multiple of 16 channels up to 256, of which those of 64 and 128 have kernels on the tensor cores."""
         if dtype not in _DTYPES:
             raise ConfigError(f"dtype must be 'bfloat16' or 'float32', got {dtype!r}")
         self.dtype = _DTYPES[dtype]

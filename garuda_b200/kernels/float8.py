@@ -64,8 +64,18 @@ _FLOAT8_SIGNATURES = {
 
 
 class Float8Ops:
-    """What ``CudaOps`` has of 8 bits. Everything is launched on torch's current stream; scratch memory belongs to the
-    stream (or to ``ws``, a step's workspace), and results do not depend on the order in which blocks finish."""
+    """What ``CudaOps`` has of 8 bits. Everything is launched on torch's current stream, and results do not depend on the order in which
+    blocks finish.
+
+    Scratch memory is the call's ``ws``, else that of the step that is running (``scratch_from``), else one that the set keeps for the stream, at
+    the largest size that was asked for, as long as the set lives; a call that is captured into a graph without ``ws`` has memory of its
+    graph's own (and clears its counters in every replay: give a captured step a ``ws`` that it ran with once). ``scratch_from`` is a
+    state of the set, so a set is one thread's.
+
+    A kernel may start while the one in front of it in the stream still runs, if that one lets it (programmatic dependent launch; the framework's
+    do, torch's and copies do not). Before it waits for that one it reads what a step has from the host or from load time: lengths
+    (``cu_q``, ``kv_lens``), block tables and weights. A kernel of the caller's own that lets its dependents start early must not write these
+    right in front of a call; everything else may come from it."""
 
     #: the workspace of the step that is running (``scratch_from``): what a captured graph reads must be its own
     step_ws = None
@@ -151,8 +161,8 @@ class Float8Ops:
 
     def linear_float8(self, a, w, out, accumulate: bool = False, alpha: float = 1.0, ws=None, gated: bool = False):
         """``out[M, N] (+)= q(a) @ w^T``: ``w`` a ``Float8Weight`` (or a pair of its two tensors), ``a [M, K]`` bfloat16 or float32, its
-        rows rounded to 8 bits with a scale per token and 128 channels (``q``). Sums are 32-bit; ``out`` is bfloat16 or float32,
-        and float32 where ``accumulate`` adds ``alpha * product`` to what is there. A scale of the weights that is no positive power of two
+        rows rounded to 8 bits with a scale per token and 128 channels (``q``; an infinity counts as 448 * 2^120, next to which the rest of its
+        128 channels is nothing). Sums are 32-bit; ``out`` is bfloat16 or float32, and float32 where ``accumulate`` adds ``alpha * product`` to what is there. A scale of the weights that is no positive power of two
         (``float8_weight`` makes none) turns the results of its 128 rows into NaN. ``gated``: ``a [M, 2 K]`` has rows ``[gate | up]``, and
         ``silu(gate) * up`` is rounded to 8 bits, from 32, and multiplied."""
         values, scales = w
@@ -264,7 +274,12 @@ class Float8Ops:
                                num_requests, max_q_len, max_kv_len, ws=None, min_q_len: int = 1):
         """Causal grouped-query attention over pages of codes (``kv_append_float8``): ``q [T, Hq, hd]`` and ``out [T, Hq * hd]``
         bfloat16 (or float32, on the plain kernel). ``window`` w > 0: a query reads the last w positions, itself included. A query
-        without a key to read gets zeros."""
+        without a key to read gets zeros, one that is not finite no numbers.
+
+        On the tensor cores (bfloat16, heads of 64 and 128, pages of 16, 32, 64 or 128) a query's channels count down to 2^-21 of its largest
+        for requests of a few rows, 2^-17 for longer portions, and weights times their page's scale down to 2^-24 (2^-22 in groups of more
+        than eight heads) of the row's largest. A value that is no number spoils the rows that read it and may spoil others of its request.
+        Other shapes go to a kernel of one warp a row, right but up to eighty times slower."""
         what = "paged_attention_float8"
         T, Hq, hd = q.shape
         Hkv = k_pool.shape[1]
