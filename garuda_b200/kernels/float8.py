@@ -162,8 +162,9 @@ class Float8Ops:
     def linear_float8(self, a, w, out, accumulate: bool = False, alpha: float = 1.0, ws=None, gated: bool = False):
         """``out[M, N] (+)= q(a) @ w^T``: ``w`` a ``Float8Weight`` (or a pair of its two tensors), ``a [M, K]`` bfloat16 or float32, its
         rows rounded to 8 bits with a scale per token and 128 channels (``q``; an infinity counts as 448 * 2^120, next to which the rest of its
-        128 channels is nothing). Sums are 32-bit; ``out`` is bfloat16 or float32, and float32 where ``accumulate`` adds ``alpha * product`` to what is there. A scale of the weights that is no positive power of two
-        (``float8_weight`` makes none) turns the results of its 128 rows into NaN. ``gated``: ``a [M, 2 K]`` has rows ``[gate | up]``, and
+        128 channels is nothing). Sums are 32-bit; ``out`` is bfloat16 or float32, and float32 where ``accumulate`` adds ``alpha *
+        product`` to what is there. A scale of the weights that is no positive power of two (``float8_weight`` makes none) turns the results
+        of its 128 rows into NaN. ``gated``: ``a [M, 2 K]`` has rows ``[gate | up]``, and
         ``silu(gate) * up`` is rounded to 8 bits, from 32, and multiplied."""
         values, scales = w
         # (one condition, taken apart when it fails)
