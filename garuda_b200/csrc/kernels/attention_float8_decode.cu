@@ -47,7 +47,7 @@
 namespace {
 
 using namespace tc;
-using attn8::Params;
+using namespace attn8;
 
 constexpr int KT = 128;                 // keys per tile
 constexpr int THREADS = 192;
@@ -74,34 +74,6 @@ struct Shape {
   static_assert(RING_AT % 1024 == 0 && P_BYTES + KT * 128 <= BYTES, "swizzled tiles; P's 128 rows end inside");
 };
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-      : "memory");
-}
-// Sums in 32 bits, both operands E4M3.
-__device__ __forceinline__ constexpr uint32_t instr_desc_e4m3(int m, int n) {
-  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
-}
-// Rows of 128 bytes (or of 64) as TMA swizzles them, eight to a group; for keys and queries the contraction lies along the row, for
-// values the rows are the contraction.
-template <int HD>
-__device__ __forceinline__ uint64_t smem_desc_rows(uint32_t addr) {
-  if (HD == 128) return smem_desc_sw128(addr);
-  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(512 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)4 << 61);
-}
-// Byte offset of 16-byte chunk `c` of row `row` in such a tile.
-template <int HD>
-__device__ __forceinline__ uint32_t swizzled(int row, int c) {
-  return HD == 128 ? (uint32_t)(row * 128 + ((c ^ (row & 7)) << 4)) : (uint32_t)(row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
-}
 template <int N>
 __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[N]);
 template <>
@@ -375,7 +347,7 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
     }
   } else if (my_tiles > 0 && warp == 1) {
     // ---------------------------------------------------------------- products
-    constexpr uint32_t idesc_s = instr_desc_e4m3(KT, N), idesc_o = instr_desc_e4m3(KT, HD) | INSTR_B_MN_MAJOR;
+    constexpr uint32_t idesc_s = instr_desc(KT, N), idesc_o = instr_desc(KT, HD) | INSTR_B_MN_MAJOR;
     const uint64_t dk0 = smem_desc_rows<HD>(ring), dq0 = smem_desc_rows<HD>(q_at), dv0 = smem_desc_rows<HD>(ring + S::OPERAND),
                    dp0 = smem_desc_sw128(p_at);
     const bool leader = elect_one();
@@ -458,30 +430,13 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
     };
     auto put_queries = [&](int seg) {
       const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
-      float v[16], largest = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        largest = fmaxf(largest, fmaxf(fabsf(v[2 * i]), fabsf(v[2 * i + 1])));
-      }
-#pragma unroll
-      for (int o = HD / 32; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-      const int e2 = f8::scale_exponent(largest);
-      // (scores with an infinite channel are infinite or no numbers, and their softmax is no number)
-      const float inv = largest < INFINITY ? f8::power_of_two(-e2) : NAN;
       uint32_t hi[4], lo[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float a = v[4 * i] * inv, b = v[4 * i + 1] * inv, c = v[4 * i + 2] * inv, d = v[4 * i + 3] * inv;
-        hi[i] = f8::encode4(a, b, c, d);
-        const float4 back = f8::decode4(hi[i]);
-        lo[i] = f8::encode4(16.f * (a - back.x), 16.f * (b - back.y), 16.f * (c - back.z), 16.f * (d - back.w));      // up to 16 * 16
-      }
+      const float unit = split_query<HD / 16>(w, 16.f, hi, lo);
       if (qrow < ROWS) {
         uint8_t* to = base + 2 * S::P_BYTES + (seg & 1) * S::Q_BYTES;
         *reinterpret_cast<uint4*>(to + swizzled<HD>(qrow, qc)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         *reinterpret_cast<uint4*>(to + swizzled<HD>(qrow + ROWS, qc)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        if (qc == 0) bars.factor[seg & 1][qrow] = f8::power_of_two(e2) * p.scale_log2;
+        if (qc == 0) bars.factor[seg & 1][qrow] = unit * p.scale_log2;
       }
       fence_proxy_async();            // the tensor core reads them through the async proxy
       mbar_arrive(smem_u32(&bars.q_ready[seg & 1]));
@@ -771,47 +726,6 @@ attention_f8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __gr
 }
 
 // ------------------------------------------------------------------ host side
-struct MapKey {
-  const void* ptr;
-  long long page, heads, pages;
-  int hd;
-  bool operator==(const MapKey& o) const { return ptr == o.ptr && page == o.page && heads == o.heads && pages == o.pages && hd == o.hd; }
-};
-struct MapKeyHash {
-  size_t operator()(const MapKey& k) const {
-    return std::hash<const void*>()(k.ptr) ^ (std::hash<long long>()(k.page) * 31) ^ (std::hash<long long>()(k.heads) * 131) ^
-           (std::hash<long long>()(k.pages) * 521) ^ (size_t)k.hd * 7919;
-  }
-};
-
-// Pools [pages][heads][page][hd] of bytes through boxes [1][1][page][hd], swizzled over the rows' width.
-int pool_map(const void* ptr, int page, int heads, long long pages, int hd, CUtensorMap* out) {
-  static std::mutex mu;
-  static std::unordered_map<MapKey, CUtensorMap, MapKeyHash> cache;
-  const MapKey key{ptr, page, heads, pages, hd};
-  std::lock_guard<std::mutex> lock(mu);
-  auto it = cache.find(key);
-  if (it != cache.end()) {
-    *out = it->second;
-    return GB_OK;
-  }
-  tc_host::EncodeTiledFn fn = tc_host::encode_fn();
-  if (!fn) return gb::fail(GB_CUDA_ERROR, "cuTensorMapEncodeTiled is not available from this driver");
-  cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)page, (cuuint64_t)heads, (cuuint64_t)pages};
-  cuuint64_t strides[3] = {(cuuint64_t)hd, (cuuint64_t)hd * page, (cuuint64_t)hd * page * heads};
-  cuuint32_t box[4] = {(cuuint32_t)hd, (cuuint32_t)page, 1, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUtensorMap m;
-  const CUresult r = fn(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        hd == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return gb::fail(GB_CUDA_ERROR, "cuTensorMapEncodeTiled failed with code %d for a pool of codes", (int)r);
-  if (cache.size() >= 1024) cache.clear();
-  cache.emplace(key, m);
-  *out = m;
-  return GB_OK;
-}
-
 constexpr int CLUSTER_TILES = 16;
 constexpr int MAX_REQUESTS = 256;    // of one launch: their lengths lie in shared memory
 
@@ -842,6 +756,9 @@ int launch(const Params& p, const CUtensorMap& km, const CUtensorMap& vm, long l
 // Bytes of the parts that CTAs leave to one another (no need to clear them). The counters are four bytes for each request and head, zero before the
 // first launch; every launch leaves them zero.
 GB_EXPORT long long gb_f8_attention_decode_part_bytes() { return (long long)tc_host::sm_count() * 2 * 2 * MAX_ROWS * (128 + 2) * 4; }
+
+// The most rows (new tokens times heads of a group) of a request that the next entry takes, in groups of g heads; 0: it takes none.
+GB_EXPORT int gb_f8_attention_decode_rows(int g) { return decode_rows(g); }
 
 // Heads of 64 or 128, pages of 16, 32, 64 or 128 keys, up to sixteen query heads a group; for requests of up to decode_rows(g) rows (new tokens
 // times heads of a group), the others are left.

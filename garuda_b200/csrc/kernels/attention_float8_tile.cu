@@ -37,7 +37,7 @@
 namespace {
 
 using namespace tc;
-using attn8::Params;
+using namespace attn8;
 
 constexpr int QROWS = 256;          // query rows per CTA
 constexpr int HALF = 128;           // of a half
@@ -74,11 +74,6 @@ struct Misc {
   float factor[QROWS];                  // per query row: 2^e * scale * log2(e)
 };
 
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -101,34 +96,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
       : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
-}
-// The largest of three in one instruction.
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-      : "memory");
-}
-// Sums in 32 bits; E4M3 operands, or (the same bits) halves.
-__device__ __forceinline__ constexpr uint32_t instr_desc(int m, int n) {
-  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
-}
-// Rows of 128 bytes (or of 64) as TMA swizzles them, eight to a group.
-template <int HD>
-__device__ __forceinline__ uint64_t smem_desc_rows(uint32_t addr) {
-  if (HD == 128) return smem_desc_sw128(addr);
-  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(512 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)4 << 61);
-}
-// Byte offset of 16-byte chunk `c` of row `row` in such a tile.
-template <int HD>
-__device__ __forceinline__ uint32_t swizzled(int row, int c) {
-  return HD == 128 ? (uint32_t)(row * 128 + ((c ^ (row & 7)) << 4)) : (uint32_t)(row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
 }
 
 // One piece of work: 256 query rows of one request and kv head.
@@ -164,7 +131,7 @@ __device__ __forceinline__ Item decode_item(const Params& p, int q_tiles, int it
   w.lo = p.window > 0 ? max(0, w.pos0 + 1 - p.window) : 0;          // first key any row reads
   w.hi = w.pos0 + ntok - 1;                                         // last key any row reads
   w.tile_begin = w.lo / KT;
-  w.valid = q_len * p.g > attn8::decode_rows(p.g) && w.tok0 < q_len && w.hi >= w.lo;      // else a decode request, or past its end
+  w.valid = q_len * p.g > decode_rows(p.g) && w.tok0 < q_len && w.hi >= w.lo;      // else a decode request, or past its end
   w.n_tiles = w.valid ? w.hi / KT + 1 - w.tile_begin : 0;
   w.table = p.block_table + (size_t)r * p.table_width;
   return w;
@@ -524,29 +491,12 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         for (int i = 0; i < BATCH; ++i) {
           const int qr = row0 + (i0 + i) * ROWS;
           const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-          float v[8], largest = 0.f;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            v[2 * e] = __uint_as_float(u[e] << 16), v[2 * e + 1] = __uint_as_float(u[e] & 0xFFFF0000u);
-            largest = max3(largest, fabsf(v[2 * e]), fabsf(v[2 * e + 1]));
-          }
-#pragma unroll
-          for (int o = LANES / 2; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-          const int e2 = f8::scale_exponent(largest);
-          // (scores with an infinite channel are infinite or no numbers, and their softmax is no number)
-          const float inv = largest < INFINITY ? f8::power_of_two(-e2) : NAN;
           uint32_t hi[2], lo[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float a = v[4 * e] * inv, b = v[4 * e + 1] * inv, d = v[4 * e + 2] * inv, f = v[4 * e + 3] * inv;
-            hi[e] = f8::encode4(a, b, d, f);
-            const float4 back = f8::decode4(hi[e]);
-            lo[e] = f8::encode4(a - back.x, b - back.y, d - back.z, f - back.w);
-          }
+          const float unit = split_query<LANES>(u, 1.f, hi, lo);
           uint8_t* to = smem_raw + swizzled<HD>(qr, sub >> 1) + (sub & 1) * 8;
           *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
           *reinterpret_cast<uint2*>(to + QROWS * HD) = make_uint2(lo[0], lo[1]);
-          if (sub == 0) mc.factor[qr] = f8::power_of_two(e2) * p.scale_log2;
+          if (sub == 0) mc.factor[qr] = unit * p.scale_log2;
         }
       }
       fence_proxy_async();              // the tensor core reads them through the async proxy
@@ -567,7 +517,7 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         if (!(ok = mbar_wait_warp(smem_u32(&mc.o_ready[half]), oph, abort_s, ran_out))) break;
         oph ^= 1;
         tc_fence_after_sync();
-        const float inv = l > 0.f ? fast_exp2(c - m - UP) / l : l == l ? 0.f : l;        // (a score that is no number stays one)
+        const float inv = l > 0.f ? exp2_fast(c - m - UP) / l : l == l ? 0.f : l;        // (a score that is no number stays one)
         __nv_bfloat16* dst = p.out + ((size_t)(w.q_begin + w.tok0 + row / p.g) * p.Hq + w.kvh * p.g + row % p.g) * HD;
 #pragma unroll 2
         for (int h = 0; h < HD / 16; ++h) {
@@ -649,7 +599,7 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         // nothing to rescale.
         const bool grown = m != -INFINITY && fmaxf(m_new - m, c_new - c) > RESCALE_ABOVE;
         if (j > 0 && __any_sync(0xffffffffu, grown)) {
-          const float own = m == -INFINITY ? 1.f : fast_exp2(m - m_new), corr = m == -INFINITY ? 1.f : fast_exp2(c - c_new);
+          const float own = m == -INFINITY ? 1.f : exp2_fast(m - m_new), corr = m == -INFINITY ? 1.f : exp2_fast(c - c_new);
 #pragma unroll 1
           for (int h = 0; h < HD / 16; ++h) {
             uint32_t v[16];
@@ -678,11 +628,11 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
 #pragma unroll
             for (int ch = 16 * b; ch < 16 * b + 16; ch += 2) {
               float2 y = fma2(make_float2(sc(ch), sc(ch + 1)), f2, off2);
-              y.x = fast_exp2(y.x), y.y = fast_exp2(y.y);                     // exp2(-inf) = 0 for masked keys
+              y.x = exp2_fast(y.x), y.y = exp2_fast(y.y);                     // exp2(-inf) = 0 for masked keys
               ls = add2(ls, y);
               pk[(ch >> 1) - 16 * h] = pack_f16(y.x, y.y);
             }
-            l = fmaf(ls.x + ls.y, fast_exp2(-up), l);          // without vs
+            l = fmaf(ls.x + ls.y, exp2_fast(-up), l);          // without vs
           }
           tmem_st_16(s_addr + h * 16, pk);
           if (h == 1) {
@@ -707,47 +657,6 @@ attention_f8_tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
 }
 
 // ------------------------------------------------------------------ host side
-struct MapKey {
-  const void* ptr;
-  long long page, heads, pages;
-  int hd;
-  bool operator==(const MapKey& o) const { return ptr == o.ptr && page == o.page && heads == o.heads && pages == o.pages && hd == o.hd; }
-};
-struct MapKeyHash {
-  size_t operator()(const MapKey& k) const {
-    return std::hash<const void*>()(k.ptr) ^ (std::hash<long long>()(k.page) * 31) ^ (std::hash<long long>()(k.heads) * 131) ^
-           (std::hash<long long>()(k.pages) * 521) ^ (size_t)k.hd * 7919;
-  }
-};
-
-// Pools [pages][heads][page][hd] of bytes through boxes [1][1][page][hd], swizzled over the rows' width.
-int pool_map(const void* ptr, int page, int heads, long long pages, int hd, CUtensorMap* out) {
-  static std::mutex mu;
-  static std::unordered_map<MapKey, CUtensorMap, MapKeyHash> cache;
-  const MapKey key{ptr, page, heads, pages, hd};
-  std::lock_guard<std::mutex> lock(mu);
-  auto it = cache.find(key);
-  if (it != cache.end()) {
-    *out = it->second;
-    return GB_OK;
-  }
-  tc_host::EncodeTiledFn fn = tc_host::encode_fn();
-  if (!fn) return gb::fail(GB_CUDA_ERROR, "cuTensorMapEncodeTiled is not available from this driver");
-  cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)page, (cuuint64_t)heads, (cuuint64_t)pages};
-  cuuint64_t strides[3] = {(cuuint64_t)hd, (cuuint64_t)hd * page, (cuuint64_t)hd * page * heads};
-  cuuint32_t box[4] = {(cuuint32_t)hd, (cuuint32_t)page, 1, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUtensorMap m;
-  const CUresult r = fn(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        hd == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return gb::fail(GB_CUDA_ERROR, "cuTensorMapEncodeTiled failed with code %d for a pool of codes", (int)r);
-  if (cache.size() >= 1024) cache.clear();
-  cache.emplace(key, m);
-  *out = m;
-  return GB_OK;
-}
-
 template <int HD>
 int launch(const Params& p, const CUtensorMap& km, const CUtensorMap& vm, int q_tiles, int total, cudaStream_t stream) {
   auto kernel = attention_f8_tile_kernel<HD>;

@@ -51,6 +51,7 @@ _FLOAT8_SIGNATURES = {
     "gb_f8_attention_simple": [c_void_p, c_int] + [c_void_p] * 5 + [c_int] + [c_void_p] * 3 + [c_int] * 5 + [c_float, c_int, c_int, c_void_p],
     "gb_f8_attention_decode": [c_void_p] * 6 + [c_int] + [c_void_p] * 3 + [c_int, c_longlong] + [c_int] * 3 + [c_float] + [c_int] * 3 + [c_void_p] * 3,
     "gb_f8_attention_tile": [c_void_p] * 6 + [c_int] + [c_void_p] * 3 + [c_int, c_longlong] + [c_int] * 3 + [c_float] + [c_int] * 3 + [c_void_p],
+    "gb_f8_attention_decode_rows": [c_int],
     "gb_f8_attention_tile_error_check": [],
     "gb_f8_attention_tile_set_error_sink": [c_void_p],
     "gb_f8_attention_decode_error_check": [],
@@ -108,7 +109,7 @@ class Float8Ops:
             L.gb_f8_linear_scratch_bytes.restype = c_longlong
             L.gb_f8_attention_decode_part_bytes.restype = c_longlong
             self._float8_part_bytes = int(L.gb_f8_attention_decode_part_bytes())
-            self._float8_sizes, self._float8_scratch = {}, {}
+            self._float8_sizes, self._float8_scratch, self._float8_few = {}, {}, {}
             sinks = (L.gb_f8_gemm_set_error_sink, L.gb_f8_attention_decode_set_error_sink, L.gb_f8_attention_tile_set_error_sink)
             if any([sink(self.error_word.data_ptr()) for sink in sinks]):
                 _need(False, "the 8-bit library could not be given the host's error word")
@@ -304,7 +305,9 @@ class Float8Ops:
         if q.dtype is torch.bfloat16 and hd in (64, 128) and page_size in (16, 32, 64, 128) and g <= 128 and not (q_ptr | out_ptr) & 15:
             # requests of a few rows (new tokens times heads of a group) go to one kernel, the others to the other; groups of more than
             # sixteen heads have none of a few (a request without tokens is nobody's)
-            few = (8 if g <= 8 else 16) if g <= 16 else 0
+            few = self._float8_few.get(g)
+            if few is None:
+                few = self._float8_few[g] = L.gb_f8_attention_decode_rows(g)
             if few and min_q_len * g <= few:
                 scratch, counters = self._scratch8("float8_attention_parts", self._float8_part_bytes, "float8_attention_counters", 4 * R * Hkv, ws,
                                                    stream)
