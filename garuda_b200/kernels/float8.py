@@ -178,7 +178,7 @@ class Float8Ops:
         a_row, w_row = a.stride(0), values.stride(0)
         if not (width == (2 * K if gated else K) and out.shape == (M, N) and K > 0 and values.dtype is E4M3 and scales.dtype is torch.float32
                 and scales.is_contiguous() and scales.shape == ((N + 127) // 128, (K + 127) // 128) and (values.stride(1) == 1 or K == 1)
-                and (w_row % 16 == 0 or N <= 1) and values.data_ptr() % 16 == 0 and (a.stride(1) == 1 or K == 1) and out_tag is not None
+                and (w_row % 16 == 0 or N <= 1) and values.data_ptr() % 16 == 0 and (a.stride(1) == 1 or width == 1) and out_tag is not None
                 and out.is_contiguous() and (out_tag == 0 if accumulate else alpha == 1.0)):
             _need(width == (2 * K if gated else K) and out.shape == (M, N),
                   f"linear_float8: shapes {tuple(a.shape)} x {tuple(values.shape)} -> {tuple(out.shape)}")
@@ -188,7 +188,7 @@ class Float8Ops:
                   "linear_float8: one float32 scale per block of 128 x 128")
             _need((values.stride(1) == 1 or K == 1) and (w_row % 16 == 0 or N <= 1) and values.data_ptr() % 16 == 0,
                   "linear_float8: rows of codes must start on 16 bytes (float8_weight makes such)")
-            _need(a.stride(1) == 1 or K == 1, "linear_float8: rows of a must have unit stride")
+            _need(a.stride(1) == 1 or width == 1, "linear_float8: rows of a must have unit stride")
             _need(out_tag is not None and out.is_contiguous(), "linear_float8: out must be contiguous, bfloat16 or float32")
             _need(not accumulate or out_tag == 0, "linear_float8: accumulates into float32 only")
             raise KernelError("linear_float8: a multiplier goes with accumulation only")

@@ -133,6 +133,20 @@ def test_products_on_streams_of_their_own(ops):  # noqa: F811
     ops.check_float8_errors()
 
 
+def test_gated_pairs_of_one_channel_need_unit_stride(ops):  # noqa: F811
+    """Rows of two numbers, whatever lies between them, and the same rows closed up."""
+    from garuda_b200.kernels.ops import KernelError
+    g = gen(4)
+    apart = torch.randn(5, 2, 3, generator=g).cuda()[:, :, 0]
+    w8, out = ops.float8_weight(torch.randn(7, 1, generator=g).cuda()), torch.zeros(5, 7, device="cuda")
+    with pytest.raises(KernelError):
+        ops.linear_float8(apart, w8, out, gated=True)
+    ops.linear_float8(apart.contiguous(), w8, out, gated=True)
+    gate, up = apart.double().unbind(1)
+    act = gate / (1 + torch.exp(-gate)) * up
+    assert torch.allclose(out.double(), act[:, None] * dense(w8)[None, :, 0], rtol=2.0 ** -4, atol=0.0)
+
+
 @pytest.mark.parametrize("size", [0.05, 40.0])
 @pytest.mark.parametrize("M,N,K", [(5, 200, 400), (300, 257, 1000)])
 @pytest.mark.parametrize("bad", [math.inf, -math.inf])
