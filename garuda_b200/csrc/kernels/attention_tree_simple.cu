@@ -1,0 +1,285 @@
+// Attention of drafted trees over the paged cache in 32-bit arithmetic throughout: the true 32-bit path, and bfloat16 where the kernel on
+// the tensor cores does not apply (head sizes other than 64 and 128, pages of other sizes). The same formula, see attention_tree_tcgen05.cu.
+//
+// Bound by the multiply-adds (32-bit ones run on the ordinary pipes): a block takes 32 query rows, (token, head-of-group) pairs of
+// one key/value head of one request, and walks its keys 32 at a time, so that a number from shared memory is used eight times in each
+// product. Its 128 threads are 16 pairs of rows by 8: a thread has two rows' scores with four keys, and of the sums two rows' every eighth four
+// channels. A row's eight threads are neighbours of one warp: maxima and sums are three shuffles, and the weights need no barrier.
+// Where the blocks of rows are fewer than the device runs at once, a request's keys are cut into parts that blocks of their own
+// take; the block that counts the last of them joins them in the order of the keys. Masked keys are skipped: nothing of them reaches a sum.
+#include "branches.h"
+
+namespace {
+
+using branches::TreeParams;
+
+constexpr int ROWS = 32, KEYS = 32, THREADS = 128;
+constexpr int P_LD = KEYS + 4;
+
+template <int HDMAX>
+struct Shape {
+  static constexpr int MOST = HDMAX / 32;      // fours of channels that a thread sums
+};
+__host__ __device__ constexpr int row_floats(int hd) { return hd + 4; }        // (eight rows' 16 bytes on different banks where hd is a multiple of 32)
+__host__ __device__ constexpr int smem_floats(int hd) { return (ROWS + 2 * KEYS) * row_floats(hd) + ROWS * P_LD; }
+
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p);
+template <>
+__device__ __forceinline__ float4 load4<float>(const float* p) { return *reinterpret_cast<const float4*>(p); }
+template <>
+__device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
+  return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xFFFF0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xFFFF0000u));
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float4 v) {
+  gb::store_pair(p, v.x, v.y);
+  gb::store_pair(p + 2, v.z, v.w);
+}
+// exp of a difference; -inf gives 0
+__device__ __forceinline__ float weight_of(float s, float m) { return m == -INFINITY ? 0.f : expf(s - m); }
+
+template <typename T, int HDMAX>
+__global__ void __launch_bounds__(THREADS)
+attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts, float* __restrict__ scratch, int* __restrict__ counters) {
+  constexpr int MOST = Shape<HDMAX>::MOST;
+  extern __shared__ __align__(16) float smem[];
+  __shared__ int last_s;
+  const int ld = row_floats(hd);
+  float* const qs = smem;
+  float* const ks = qs + ROWS * ld;
+  float* const vs = ks + KEYS * ld;
+  float* const ps = vs + KEYS * ld;
+  gb::pdl_launch_dependents();
+  gb::pdl_wait();
+  const int r = blockIdx.z, kvh = blockIdx.y % p.Hkv, block = blockIdx.y / p.Hkv, part = blockIdx.x;
+  const int q_begin = p.cu_q[r], q_len = p.cu_q[r + 1] - q_begin, row0 = block * ROWS, nrows = min(ROWS, q_len * p.g - row0);
+  const int kv_len = p.kv_lens[r], ctx = max(0, kv_len - q_len);
+  if (nrows <= 0 || kv_len <= 0) return;
+  const int lo = (p.window > 0 ? max(0, ctx + 1 - p.window) : 0) / KEYS, tiles = (kv_len - 1) / KEYS + 1 - lo;
+  const int per = (tiles + parts - 1) / parts, busy = (tiles + per - 1) / per;      // parts that have keys
+  if (part >= busy) return;
+  const int tile_begin = lo + part * per, tile_end = min(lo + tiles, tile_begin + per);
+  const int32_t* table = p.block_table + (size_t)r * p.table_width;
+
+  const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3, c4 = hd / 4;
+  const T* q = reinterpret_cast<const T*>(p.q);
+  for (int x = threadIdx.x; x < ROWS * c4; x += THREADS) {
+    const int row = x / c4, c = x % c4, at = row0 + row;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row < nrows) v = load4(q + ((size_t)(q_begin + at / p.g) * p.Hq + kvh * p.g + at % p.g) * hd + c * 4);
+    *reinterpret_cast<float4*>(qs + row * ld + c * 4) = v;
+  }
+  // this thread's two rows
+  int token[2], start[2];
+  bool there[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = 2 * ty + i;
+    there[i] = row < nrows;
+    token[i] = q_begin + (there[i] ? (row0 + row) / p.g : 0);
+    start[i] = p.window > 0 ? p.positions[token[i]] + 1 - p.window : 0;
+  }
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float4 o[2][MOST];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int c = 0; c < MOST; ++c) o[i][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+
+  for (int tile = tile_begin; tile < tile_end; ++tile) {
+    const int key0 = tile * KEYS;
+    __syncthreads();
+    for (int x = threadIdx.x; x < KEYS * c4; x += THREADS) {
+      const int key = x / c4, c = x % c4, at = key0 + key, slot = at / p.page_size;
+      const int page = at < kv_len && slot < p.table_width ? table[slot] : -1;
+      float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+      if (page >= 0 && page < p.pages) {
+        const size_t where = (((size_t)page * p.Hkv + kvh) * p.page_size + at % p.page_size) * hd + c * 4;
+        k = load4(reinterpret_cast<const T*>(p.k_pool) + where);
+        v = load4(reinterpret_cast<const T*>(p.v_pool) + where);
+      }
+      *reinterpret_cast<float4*>(ks + key * ld + c * 4) = k;
+      *reinterpret_cast<float4*>(vs + key * ld + c * 4) = v;
+    }
+    __syncthreads();
+    // ---- scores of two rows with keys tx, tx + 8, tx + 16, tx + 24
+    float s[2][4] = {};
+    for (int c = 0; c < c4; ++c) {
+      float4 a[2], b[4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) a[i] = *reinterpret_cast<const float4*>(qs + (2 * ty + i) * ld + c * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b[e] = *reinterpret_cast<const float4*>(ks + (tx + 8 * e) * ld + c * 4);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[i][e] = fmaf(a[i].x, b[e].x, s[i][e]);
+          s[i][e] = fmaf(a[i].y, b[e].y, s[i][e]);
+          s[i][e] = fmaf(a[i].z, b[e].z, s[i][e]);
+          s[i][e] = fmaf(a[i].w, b[e].w, s[i][e]);
+        }
+    }
+    // ---- the keys that a row does not read, then the softmax's running maximum and sum
+    const bool edge = key0 + KEYS > ctx || p.window > 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float top = m[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[i][e] *= p.scale;
+        if (edge) {
+          const int key = key0 + tx + 8 * e, j = key - ctx;
+          bool sees = there[i] && key < kv_len;
+          if (j < 0) sees = sees && key >= start[i];
+          else sees = sees && (j >> 5) < p.mask_words && (p.mask[(size_t)token[i] * p.mask_words + (j >> 5)] >> (j & 31) & 1u);
+          if (!sees) s[i][e] = -INFINITY;
+        }
+        top = fmaxf(top, s[i][e]);
+      }
+#pragma unroll
+      for (int d = 1; d < 8; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const float keep = weight_of(m[i], top);
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        // (a masked key's weight is nothing, whatever the maximum is; a score that is no number stays none)
+        const float w = s[i][e] == -INFINITY ? 0.f : expf(s[i][e] - (top == -INFINITY ? 0.f : top));
+        sum += w;
+        ps[(2 * ty + i) * P_LD + tx + 8 * e] = w;
+      }
+      l[i] = l[i] * (m[i] == -INFINITY ? 1.f : keep) + sum;          // this thread's share
+      if (m[i] != -INFINITY && keep != 1.f) {
+#pragma unroll
+        for (int c = 0; c < MOST; ++c) o[i][c].x *= keep, o[i][c].y *= keep, o[i][c].z *= keep, o[i][c].w *= keep;
+      }
+      m[i] = top;
+    }
+    __syncwarp();
+    // ---- sums of two rows' channels 4 tx + 32 c
+    for (int key = 0; key < KEYS; ++key) {
+      const float w0 = ps[2 * ty * P_LD + key], w1 = ps[(2 * ty + 1) * P_LD + key];
+#pragma unroll
+      for (int c = 0; c < MOST; ++c) {
+        if (4 * tx + 32 * c >= hd) break;
+        const float4 v = *reinterpret_cast<const float4*>(vs + key * ld + 4 * tx + 32 * c);
+        if (!edge || w0 != 0.f)
+          o[0][c].x = fmaf(w0, v.x, o[0][c].x), o[0][c].y = fmaf(w0, v.y, o[0][c].y), o[0][c].z = fmaf(w0, v.z, o[0][c].z), o[0][c].w = fmaf(w0, v.w, o[0][c].w);
+        if (!edge || w1 != 0.f)
+          o[1][c].x = fmaf(w1, v.x, o[1][c].x), o[1][c].y = fmaf(w1, v.y, o[1][c].y), o[1][c].z = fmaf(w1, v.z, o[1][c].z), o[1][c].w = fmaf(w1, v.w, o[1][c].w);
+      }
+    }
+    __syncwarp();
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], d);
+  T* const out = reinterpret_cast<T*>(p.out);
+  auto place = [&](int row) { return out + ((size_t)(q_begin + (row0 + row) / p.g) * p.Hq + kvh * p.g + (row0 + row) % p.g) * hd; };
+  if (busy == 1) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float inv = l[i] == 0.f ? 0.f : 1.0f / l[i];
+#pragma unroll
+      for (int c = 0; c < MOST; ++c)
+        if (there[i] && 4 * tx + 32 * c < hd)
+          store4(place(2 * ty + i) + 4 * tx + 32 * c, make_float4(o[i][c].x * inv, o[i][c].y * inv, o[i][c].z * inv, o[i][c].w * inv));
+    }
+    return;
+  }
+  // ---- parts: sums, maximum and denominator of every row to scratch memory; the last block joins them
+  const int rs = hd + 4, unit = r * gridDim.y + blockIdx.y;
+  float* const all = scratch + (size_t)unit * parts * ROWS * rs;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (!there[i]) continue;
+    float* to = all + (size_t)(part * ROWS + 2 * ty + i) * rs;
+#pragma unroll
+    for (int c = 0; c < MOST; ++c)
+      if (4 * tx + 32 * c < hd) *reinterpret_cast<float4*>(to + 4 * tx + 32 * c) = o[i][c];
+    if (tx == 0) to[hd] = m[i], to[hd + 1] = l[i];
+  }
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int seen = atomicAdd(&counters[unit], 1);
+    last_s = seen == busy - 1;
+    if (last_s) counters[unit] = 0;           // as the next launch expects it
+  }
+  __syncthreads();
+  if (!last_s) return;
+  __threadfence();
+  for (int x = threadIdx.x; x < nrows * c4; x += THREADS) {
+    const int row = x / c4, c = x % c4;
+    float mt = -INFINITY, lt = 0.f;
+    float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < busy; ++i) {
+      const float* from = all + (size_t)(i * ROWS + row) * rs;
+      const float mi = __ldcg(from + hd), li = __ldcg(from + hd + 1);
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(from + c * 4));
+      if (mi == -INFINITY && li == 0.f) continue;        // no key of this part
+      const float top = fmaxf(mt, mi), keep = mt == -INFINITY ? 1.f : weight_of(mt, top), add = mi == -INFINITY ? 1.f : weight_of(mi, top);
+      t.x = t.x * keep + v.x * add, t.y = t.y * keep + v.y * add, t.z = t.z * keep + v.z * add, t.w = t.w * keep + v.w * add;
+      lt = lt * keep + li * add, mt = top;
+    }
+    const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+    store4(place(row) + c * 4, make_float4(t.x * inv, t.y * inv, t.z * inv, t.w * inv));
+  }
+}
+
+struct Cut {
+  int blocks, parts;
+};
+// Parts of a request's keys: as many as fill the device four times over, each of at least four tiles
+Cut cut_of(int R, int max_q_len, int g, int Hkv, int max_kv_len) {
+  const int blocks = (max_q_len * g + ROWS - 1) / ROWS, tiles = (max_kv_len + KEYS - 1) / KEYS;
+  const long long units = (long long)R * blocks * Hkv;
+  long long parts = 4ll * gb::sm_count() / (units < 1 ? 1 : units);
+  if (parts > (tiles + 3) / 4) parts = (tiles + 3) / 4;
+  return {blocks, parts < 1 ? 1 : (int)parts};
+}
+
+template <typename T, int HDMAX>
+int launch(const TreeParams& p, int hd, Cut cut, float* scratch, int* counters, cudaStream_t stream) {
+  static gb::OncePerDevice configured;
+  if (configured.needed()) {
+    const cudaError_t e = cudaFuncSetAttribute(attention_tree_simple_kernel<T, HDMAX>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               4 * smem_floats(HDMAX));
+    if (e != cudaSuccess) return gb::fail(GB_CUDA_ERROR, "tree_attention: %s", cudaGetErrorString(e));
+    configured.done();
+  }
+  return gb::check_pdl_launch(gb::launch_pdl(attention_tree_simple_kernel<T, HDMAX>, dim3(cut.parts, cut.blocks * p.Hkv, p.R), dim3(THREADS),
+                                             4 * smem_floats(hd), stream, dim3(1), p, hd, cut.parts, scratch, counters), "tree_attention");
+}
+
+}  // namespace
+
+// Bytes of scratch memory of a call, of which the counters' are zero before the first one and after every one.
+GB_EXPORT long long gb_tree_attention_simple_scratch_bytes(int R, int max_q_len, int Hq, int Hkv, int head_dim, int max_kv_len,
+                                                           long long* counter_bytes) {
+  const Cut cut = cut_of(R, max_q_len, Hq / Hkv, Hkv, max_kv_len);
+  const long long units = (long long)R * cut.blocks * Hkv;
+  *counter_bytes = cut.parts > 1 ? (4 * units + 15) / 16 * 16 : 16;
+  return cut.parts > 1 ? units * cut.parts * ROWS * (head_dim + 4) * 4 : 16;
+}
+
+GB_EXPORT int gb_tree_attention_simple(const void* q, int dtype, const void* k_pool, const void* v_pool, const int32_t* block_table, int table_width,
+                                       const int32_t* cu_q, const int32_t* kv_lens, const int32_t* positions, const int32_t* mask, int mask_words,
+                                       void* out, int T, int R, long long pages, int Hq, int Hkv, int head_dim, float scale, int window,
+                                       int page_size, int max_q_len, int max_kv_len, void* counters, void* scratch, void* stream) {
+  const TreeParams p{q, k_pool, v_pool, out, block_table, cu_q, kv_lens, positions, reinterpret_cast<const uint32_t*>(mask), pages,
+                     table_width, mask_words, Hq, Hkv, Hq / Hkv, window, page_size, T, R, scale};
+  const Cut cut = cut_of(R, max_q_len, p.g, Hkv, max_kv_len);
+  if (head_dim % 4 != 0 || head_dim > 256) return gb::fail(GB_UNSUPPORTED, "tree_attention: heads of %d channels", head_dim);
+  if (R > 65535 || (long long)cut.blocks * Hkv > 65535) return gb::fail(GB_UNSUPPORTED, "tree_attention: %d requests, %d blocks of rows", R, cut.blocks * Hkv);
+  return GB_DISPATCH_DTYPE(dtype, E, [&]() -> int {
+    float* parts = reinterpret_cast<float*>(scratch);
+    int* counts = reinterpret_cast<int*>(counters);
+    if (head_dim <= 64) return launch<E, 64>(p, head_dim, cut, parts, counts, (cudaStream_t)stream);
+    if (head_dim <= 128) return launch<E, 128>(p, head_dim, cut, parts, counts, (cudaStream_t)stream);
+    return launch<E, 256>(p, head_dim, cut, parts, counts, (cudaStream_t)stream);
+  });
+}

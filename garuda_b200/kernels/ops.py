@@ -17,6 +17,7 @@ import numpy as np
 import torch
 
 from ..csrc.build import load_kernel_lib
+from .branches import BranchOps
 from .checks import GB_BF16, GB_F32, KernelError, _need, _ptr, _tag
 from .float8 import Float8Ops, Float8Weight
 
@@ -61,7 +62,7 @@ class ExpertRows:
         self.rows, self.pair_row, self.weights, self.identity, self.base = rows, pair_row, weights, identity, base
 
 
-class CudaOps(Float8Ops):
+class CudaOps(Float8Ops, BranchOps):
     """Hand-written sm_100a kernels. ``tensor_cores=False`` keeps every matrix
     product and the attention on the plain 32-bit-arithmetic kernels (the true
     32-bit path uses them in any case)."""
@@ -84,6 +85,7 @@ class CudaOps(Float8Ops):
         self._ssd = None
         self._memory = None
         self._float8 = None
+        self._branches = None
         self._declare_core()
         # A word of pinned host memory that a kernel whose bounded wait ran out writes its code to (the
         # device reaches pinned host memory directly); ``failed_wait`` reads it without a copy.
