@@ -32,6 +32,8 @@ _SIGNATURES = {
     "gb_copy_entries": [c_int] + [c_void_p] * 6 + [c_int, c_void_p],
     "gb_tree_attention_error_check": [],
     "gb_tree_attention_set_error_sink": [c_void_p],
+    "gb_beam_select_error_check": [],
+    "gb_beam_select_set_error_sink": [c_void_p],
     "gb_branches_error_check": [],
     "gb_branches_set_error_sink": [c_void_p],
 }
@@ -65,7 +67,8 @@ class BranchOps:
                 fn = getattr(L, name)
                 fn.argtypes, fn.restype = argtypes, c_longlong
             self._branch_sizes, self._branch_scratch = {}, {}
-            if any([sink(self.error_word.data_ptr()) for sink in (L.gb_tree_attention_set_error_sink, L.gb_branches_set_error_sink)]):
+            if any([sink(self.error_word.data_ptr()) for sink in (L.gb_tree_attention_set_error_sink, L.gb_beam_select_set_error_sink,
+                                                                     L.gb_branches_set_error_sink)]):
                 _need(False, "the library of branches could not be given the host's error word")
             self._branches = L
         return self._branches
@@ -97,7 +100,7 @@ class BranchOps:
         if self._branches is None:
             return 0
         L = self._branches
-        codes = [L.gb_tree_attention_error_check(), L.gb_branches_error_check()]
+        codes = [L.gb_tree_attention_error_check(), L.gb_beam_select_error_check(), L.gb_branches_error_check()]
         return next((c for c in codes if c), 0)
 
     def check_branch_errors(self) -> None:
