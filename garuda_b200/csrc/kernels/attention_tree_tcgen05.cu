@@ -45,6 +45,7 @@ constexpr int TMEM_COLS = 512;
 constexpr int S_BUFS = 2;           // S buffers: the S products run this many tiles ahead
 constexpr int O_COL0 = S_BUFS * KT;
 constexpr float RESCALE_ABOVE = 8.f;                // in powers of two
+constexpr int BLOCK_COST = 2;                       // what a block of rows costs beside its tiles, in tiles
 constexpr int MAX_REQUESTS = 2048;                  // of one launch (their places are in shared memory)
 constexpr int COUNTERS = 1024;                      // one per CTA, and so no more CTAs
 
@@ -64,7 +65,7 @@ struct Shape {
 
 struct Misc {
   uint64_t q_full, q_empty, k_full[4], k_empty[4], v_full[5], v_empty[5];
-  uint64_t s_ready[S_BUFS], p_ready[S_BUFS], o_ready, looked[GROUPS];
+  uint64_t s_ready[S_BUFS], p_ready[S_BUFS], o_ready[2], looked[GROUPS];
   uint32_t tmem_base;
   int abort, last, total, scan[THREADS / 32];
   uint32_t bad[2][GROUPS][2];             // keys of a masked tile whose values are not finite, a bit each, two such tiles in turn
@@ -96,23 +97,25 @@ __device__ __forceinline__ void clear_shared_v4(uint32_t addr) {
 // whether one of two bfloat16 is an infinity or NaN
 __device__ __forceinline__ bool not_finite(uint32_t w) { return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u; }
 
-// A piece: tiles first .. first + count of the n of one request's block of rows and head.
+// A piece: tiles first .. first + count of the n of one request's block of rows and head. The row of all blocks' costs, a tile each and
+// BLOCK_COST for a block, is what is cut into stretches.
 struct Piece {
   int r, kvh, tok0, nrows, q_begin, ctx, kv_len;      // of the request: its first token, its context and all its keys
   int lo, tile0, first, n, count;                     // first key that any row reads; the tile that it lies in
+  int at, next;                                       // in the row of costs: the block's place, and what comes behind the piece
 };
 
 template <int HD>
 __global__ void __launch_bounds__(THREADS, 1)
 attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
-                         const __grid_constant__ CUtensorMap v_map, const TreeParams p, const int box_tokens, const int min_tiles,
+                         const __grid_constant__ CUtensorMap v_map, const TreeParams p, const int box_tokens, const int min_stretch,
                          float* __restrict__ parts, int* __restrict__ counters) {
   using S = Shape<HD>;
   constexpr int BLOCKS = S::BLOCKS, K_STAGES = S::K_STAGES, V_STAGES = S::V_STAGES, CH = S::CH;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Misc& mc = *reinterpret_cast<Misc*>(smem_raw + S::TILE_BYTES);
-  int* const cum = reinterpret_cast<int*>(smem_raw + S::TILE_BYTES + sizeof(Misc));      // [R + 1]: tiles of the requests in front
-  int* const begin_s = cum + p.R + 1;                                                    // [R + 1]: cu_q
+  int* const cost = reinterpret_cast<int*>(smem_raw + S::TILE_BYTES + sizeof(Misc));     // [R + 1]: of the requests in front
+  int* const begin_s = cost + p.R + 1;                                                   // [R + 1]: cu_q
   int* const len_s = begin_s + p.R + 1;                                                  // [R]: kv_lens
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -130,7 +133,8 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
     }
     for (int s = 0; s < K_STAGES; ++s) mbar_init(smem_u32(&mc.k_full[s]), 1), mbar_init(smem_u32(&mc.k_empty[s]), 1);
     for (int s = 0; s < V_STAGES; ++s) mbar_init(smem_u32(&mc.v_full[s]), 1), mbar_init(smem_u32(&mc.v_empty[s]), 1);
-    mbar_init(smem_u32(&mc.o_ready), 1);
+    mbar_init(smem_u32(&mc.o_ready[0]), 1);
+    mbar_init(smem_u32(&mc.o_ready[1]), 1);
     for (int g = 0; g < GROUPS; ++g) mbar_init(smem_u32(&mc.looked[g]), 2);
     mc.abort = 0, mc.total = 0;
     fence_barrier_init();
@@ -165,7 +169,8 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
       const int q0 = p.cu_q[r], q1 = p.cu_q[r + 1], kv = p.kv_lens[r];
       begin_s[r] = q0, len_s[r] = kv;
       if (r + 1 == p.R) begin_s[r + 1] = q1;
-      n = tiles_of(q1 - q0, kv) * ((q1 - q0 + tokens_per_block - 1) / tokens_per_block) * p.Hkv;
+      n = tiles_of(q1 - q0, kv);
+      if (n > 0) n = (n + BLOCK_COST) * ((q1 - q0 + tokens_per_block - 1) / tokens_per_block) * p.Hkv;
     }
     int inc = n;
 #pragma unroll
@@ -179,40 +184,50 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
     for (int w = 0; w < warp; ++w) before += mc.scan[w];
     before += inc;
     if (r < p.R) {
-      cum[r] = before - n;
-      if (r + 1 == p.R) cum[r + 1] = before;
+      cost[r] = before - n;
+      if (r + 1 == p.R) cost[r + 1] = before;
     }
     __syncthreads();
     if (threadIdx.x == THREADS - 1) mc.total = before;
     __syncthreads();
   }
-  const int total = cum[p.R];
-  const int stretch = max(min_tiles, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+  const int total = cost[p.R];
+  const int stretch = max(min_stretch, (total + (int)gridDim.x - 1) / (int)gridDim.x);
   const int a_begin = (int)min((long long)total, (long long)blockIdx.x * stretch), a_end = min(total, a_begin + stretch);
 
-  auto piece_at = [&](int a) {
-    int lo = 0, hi = p.R;                  // the last request whose tiles begin at or before `a` (of several at the same place it has some)
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (cum[mid] <= a) lo = mid;
-      else hi = mid;
-    }
+  auto piece_at = [&](int a) {             // the piece that begins there or behind; count 0: the stretch has no more
     Piece w;
-    w.r = lo, w.q_begin = begin_s[lo], w.kv_len = len_s[lo];
-    const int q_len = begin_s[lo + 1] - w.q_begin, blocks = (q_len + tokens_per_block - 1) / tokens_per_block;
-    w.ctx = max(0, w.kv_len - q_len);
-    w.lo = low_of(w.ctx), w.tile0 = w.lo / KT;
-    w.n = tiles_of(q_len, w.kv_len);
-    const int rem = a - cum[lo], unit = rem / w.n;
-    w.first = rem % w.n;
-    w.kvh = unit / blocks;                 // (a head's blocks of rows one behind the other: they read the same keys)
-    w.tok0 = unit % blocks * tokens_per_block;
-    w.nrows = min(tokens_per_block, q_len - w.tok0) * p.g;
-    w.count = min(w.n - w.first, a_end - a);
+    w.count = 0;
+    while (a < a_end) {
+      int lo = 0, hi = p.R;                // the last request that begins at or before `a` (of several at the same place it has tiles)
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (cost[mid] <= a) lo = mid;
+        else hi = mid;
+      }
+      w.r = lo, w.q_begin = begin_s[lo], w.kv_len = len_s[lo];
+      const int q_len = begin_s[lo + 1] - w.q_begin, blocks = (q_len + tokens_per_block - 1) / tokens_per_block;
+      w.ctx = max(0, w.kv_len - q_len);
+      w.lo = low_of(w.ctx), w.tile0 = w.lo / KT;
+      w.n = tiles_of(q_len, w.kv_len);
+      const int per = w.n + BLOCK_COST, rem = a - cost[lo], unit = rem / per;
+      w.first = rem - unit * per;
+      w.at = a - w.first;
+      if (w.first >= w.n) {                // what the block costs beside its tiles
+        a = w.at + per;
+        continue;
+      }
+      w.kvh = unit / blocks;               // (a head's blocks of rows one behind the other: they read the same keys)
+      w.tok0 = unit % blocks * tokens_per_block;
+      w.nrows = min(tokens_per_block, q_len - w.tok0) * p.g;
+      w.count = min(w.n - w.first, a_end - a);
+      w.next = a + w.count;
+      break;
+    }
     return w;
   };
 
-  if (a_begin < a_end && warp == 0) {
+  if (warp == 0) {
     // ------------------------------------------------------------------ TMA
     // The lanes look up the pages of several tiles in one round trip; for a tile, lane i issues its i-th page's copies.
     const int page_shift = __ffs(p.page_size) - 1;         // pages are a power of two of keys, 8 to 128
@@ -221,9 +236,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
     int gt = 0, it = 0;               // tiles and pieces so far
     int ks = 0, kpar = 1, vs = 0, vpar = 1;         // the stages to fill and the phases of their "empty" barriers
     bool ok = true, ran_out = false;
-    for (int a = a_begin; a < a_end && ok; ++it) {
-      const Piece w = piece_at(a);
-      a += w.count;
+    for (Piece w = piece_at(a_begin); w.count > 0 && ok; w = piece_at(w.next), ++it) {
       if (it > 0) ok = mbar_wait_warp(smem_u32(&mc.q_empty), (it - 1) & 1, abort_s, ran_out);
       if (!ok) break;
       if (lane == 0) {
@@ -273,7 +286,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
         while (globaltimer_ns() - t0 < 2000000ull) {}
       }
     }
-  } else if (a_begin < a_end && warp == 1) {
+  } else if (warp == 1) {
     // -------------------------------------------------------------------- MMA issuer
     // The S products run two tiles ahead of the P V products, across the pieces' borders. After a tile's softmax its P V goes first: it
     // reads the weights from the S buffer that the S product two tiles ahead then overwrites (products run in the order of their issue).
@@ -281,18 +294,18 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
     constexpr uint32_t idesc_s = instr_desc_bf16(QROWS, KT), idesc_o = instr_desc_bf16(QROWS, HD) | INSTR_B_MN_MAJOR;
     const uint64_t dq0 = smem_desc_sw128(q_s), dk0 = smem_desc_sw128(k_s), dv0 = smem_desc_sw128_mn(v_s, BLOCKS > 1 ? BLOCK_BYTES : 16);
     bool ok = true, ran_out = false;
-    int a_s = a_begin, left_s = 0, pieces_s = 0, a_o = a_begin, left_o = 0;
+    Piece ws = piece_at(a_begin), wo = ws;           // of the S products, of the P V products
+    int left_s = ws.count, left_o = ws.count, pieces_s = 0;
     int ks = 0, kpar = 0, vs = 0, vpar = 0, sb = 0, pb = 0, ppar = 0;
-    auto issue_s = [&]() {
-      if (left_s == 0) {
-        left_s = piece_at(a_s).count;
-        a_s += left_s;
+    // (a wait costs near two hundred clocks even when there is nothing to wait for: those for keys and values go in front of the one for the weights)
+    auto wait_s = [&]() {
+      if (left_s == ws.count) {
         ok = mbar_wait_warp(smem_u32(&mc.q_full), pieces_s & 1, abort_s, ran_out);
         ++pieces_s;
       }
       if (ok) ok = mbar_wait_warp(smem_u32(&mc.k_full[ks]), kpar, abort_s, ran_out);
-      if (!ok) return;
-      tc_fence_after_sync();
+    };
+    auto issue_s = [&]() {
       if (leader) {
 #pragma unroll
         for (int h = 0; h < BLOCKS; ++h)
@@ -302,41 +315,48 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
         if (S::KEYS_FREED_BY_COMMIT) mma_commit(smem_u32(&mc.k_empty[ks]));
       }
       __syncwarp();
-      --left_s;
       if (++ks == K_STAGES) ks = 0, kpar ^= 1;
       if (++sb == S_BUFS) sb = 0;
+      if (--left_s == 0) ws = piece_at(ws.next), left_s = ws.count;
     };
 #pragma unroll 1
     for (int b = 0; b < S_BUFS; ++b)
-      if (ok && (left_s > 0 || a_s < a_end)) issue_s();
-    while (ok && (left_o > 0 || a_o < a_end)) {
-      bool first = false;
-      if (left_o == 0) {
-        const Piece w = piece_at(a_o);
-        left_o = w.count, a_o += w.count, first = true;
+      if (ok && left_s > 0) {
+        wait_s();
+        tc_fence_after_sync();
+        if (ok) issue_s();
       }
-      ok = mbar_wait_warp(smem_u32(&mc.p_ready[pb]), ppar, abort_s, ran_out);
+    while (ok && left_o > 0) {
+      // (not for another piece's queries: their place is free when the softmax has got to this piece's last tile, which these products let it)
+      const bool more = left_s > 0, early = more && left_s != ws.count;
+      if (early) wait_s();
       if (ok) ok = mbar_wait_warp(smem_u32(&mc.v_full[vs]), vpar, abort_s, ran_out);
+      if (ok) ok = mbar_wait_warp(smem_u32(&mc.p_ready[pb]), ppar, abort_s, ran_out);
       if (!ok) break;
       tc_fence_after_sync();
       if (leader) {
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g)
           mma_bf16_ts<GK / 16>(tmem_base + O_COL0 + g * HD, tmem_base + pb * KT + g * GK,
-                               dv0 + (uint64_t)(vs * (S::BYTES >> 4) + g * (GK * ROW_BYTES >> 4)), idesc_o, 16 * ROW_BYTES >> 4, !first);
-        mma_commit(smem_u32(&mc.o_ready));
+                               dv0 + (uint64_t)(vs * (S::BYTES >> 4) + g * (GK * ROW_BYTES >> 4)), idesc_o, 16 * ROW_BYTES >> 4, left_o != wo.count);
+        mma_commit(smem_u32(&mc.o_ready[pb]));
       }
       __syncwarp();
-      --left_o;
-      if (left_s > 0 || a_s < a_end) issue_s();
+      if (more && !early) {
+        wait_s();
+        if (!ok) break;
+        tc_fence_after_sync();
+      }
+      if (more) issue_s();
       if (++vs == V_STAGES) vs = 0, vpar ^= 1;
       if (++pb == S_BUFS) pb = 0, ppar ^= 1;
+      if (--left_o == 0) wo = piece_at(wo.next), left_o = wo.count;
     }
     if (!ok) {
       if (ran_out) gb_err::report(ERR_WAIT_FULL);
       *abort_s = 1;
     }
-  } else if (a_begin < a_end) {
+  } else {
     // -------------------------------------------------------------------- softmax warps
     const int grp = (warp - 2) >> 2;
     const int quarter = warp & 3;                        // the TMEM lanes this warp may read
@@ -346,8 +366,10 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
     const float scale_log2 = p.scale * 1.4426950408889634f;
     bool ok = true;               // false: this thread only keeps the others company at the barriers
     int gt = 0, it = 0, et = 0;   // tiles, pieces and masked tiles so far
-    int sb = 0, sph = 0, kstage = 0, vstage = 0, vpar = 0, vprev = 0;
+    int sb = 0, sph = 0, kstage = 0, vstage = 0, vpar = 0, vfree = 0;       // (vfree: the stage of values to give back next)
+    int freed = 0;                // tiles whose values have been given back
     const bool passes_on = threadIdx.x == 64;      // one thread tells the TMA warp what the tensor core has finished with
+    auto again = [] { asm volatile("" ::: "memory"); };           // what is looked up behind it is looked up again, not kept
     auto wait = [&](uint64_t& bar, int parity, int code) {       // the whole warp's: it stays together
       bool ran_out;
       if (!mbar_wait_warp(smem_u32(&bar), parity, abort_s, ran_out)) {
@@ -356,28 +378,39 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
         *abort_s = 1;
       }
     };
-    auto wait_o = [&](int t) {                     // until the P V products of the tile counted t have ended
-      wait(mc.o_ready, t & 1, ERR_WAIT_ACCUM);
+    // Until the P V products of the tile counted t have ended. (Not asked for every tile: those of t - 2, the barrier's phase in front, have ended since the
+    // scores of t were there, those of t + 2 wait for this warp.)
+    auto wait_o = [&](int t) {
+      wait(mc.o_ready[t & 1], t >> 1 & 1, ERR_WAIT_ACCUM);
       tc_fence_after_sync();
     };
-    for (int a = a_begin; a < a_end; ++it) {
-      const Piece w = piece_at(a);
-      a += w.count;
+    for (int at = a_begin;; ++it) {
+      int count;                     // (few of a piece's numbers are kept over its tiles: registers are short)
+      const int piece = at;
+      Piece w = piece_at(at);
+      if ((count = w.count) == 0) break;
+      at = w.next;
       const bool there = row < w.nrows;
       const bool active = quarter * 32 < w.nrows;        // this warp has a row
-      const int token = w.q_begin + w.tok0 + (there ? row / p.g : 0);
       // tiles from here on, and up to there, hold keys that some row does not read
-      const int edge_from = w.ctx, edge_to = p.window > 0 ? w.kv_len - p.window : w.lo;
+      const int edge_from = w.ctx, edge_to = p.window > 0 ? w.kv_len - p.window : 0, first_key = (w.tile0 + w.first) * KT;
       float m = -INFINITY, l = 0.f;      // m: the reference maximum of the raw dot products
       bool spoiled = false;              // this row reads a value that is not finite
 
-      for (int j = 0; j < w.count && ok; ++j, ++gt) {
+      for (int j = 0; j < count && ok; ++j, ++gt) {
         wait(mc.s_ready[sb], sph, ERR_WAIT_ACCUM);
         if (!ok) break;
         tc_fence_after_sync();
-        if (passes_on) {      // S of this tile is complete: its keys have been read, and after a piece's last tile its queries
+        // S of this tile is complete: its keys have been read, after a piece's last tile its queries, and the values of the tile two in front
+        // (products run in the order of their issue)
+        if (passes_on) {
+          if (freed < gt - 1) {
+            mbar_arrive(smem_u32(&mc.v_empty[vfree]));
+            if (++vfree == V_STAGES) vfree = 0;
+            ++freed;
+          }
           if (!S::KEYS_FREED_BY_COMMIT) mbar_arrive(smem_u32(&mc.k_empty[kstage]));
-          if (j == w.count - 1) mbar_arrive(smem_u32(&mc.q_empty));
+          if (j == count - 1) mbar_arrive(smem_u32(&mc.q_empty));
         }
         if (++kstage == K_STAGES) kstage = 0;
         const uint32_t s_addr = lane_addr + sb * KT + grp * GK;
@@ -386,10 +419,13 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
 #pragma unroll
           for (int h = 0; h < GK / 32; ++h) tmem_ld_32(s_addr + h * 32, sv[h]);
         }
-        const int tile_key0 = (w.tile0 + w.first + j) * KT, key0 = tile_key0 + grp * GK;
+        const int tile_key0 = first_key + j * KT, key0 = tile_key0 + grp * GK;
         const bool edge = tile_key0 + KT > edge_from || tile_key0 < edge_to;
         unsigned long long sees = ~0ull;
         if (edge) {
+          again();
+          const Piece w = piece_at(piece);
+          const int token = w.q_begin + w.tok0 + (there ? row / p.g : 0);
           wait(mc.v_full[vstage], vpar, ERR_WAIT_FULL);
           bool bad = false;
           if (ok && row < GK) {               // (a row of values to each of half of the group's threads)
@@ -443,10 +479,8 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
           }
           spoiled = spoiled || (sees & spoils) != 0;
         }
-        const int vcur = vstage;
         if (++vstage == V_STAGES) vstage = 0, vpar ^= 1;
         if (!ok) break;
-        bool waited = false;
         if (active) {
           tmem_ld_wait();
           auto sc = [&](int ch) -> float& { return reinterpret_cast<float&>(sv[ch >> 5][ch & 31]); };
@@ -468,7 +502,6 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
           const bool grown = there && m != -INFINITY && (m_new - m) * scale_log2 > RESCALE_ABOVE;
           if (j > 0 && __any_sync(0xffffffffu, grown)) {
             wait_o(gt - 1);
-            waited = true;
             if (ok) {
               const float corr = m == -INFINITY ? 1.f : fast_exp2((m - m_new) * scale_log2);
 #pragma unroll
@@ -502,17 +535,20 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
           tmem_st(s_addr, pk);            // over the first half of the scores just read
           tmem_st_wait();
         }
-        if (j > 0 && !waited) wait_o(gt - 1);      // every phase of the barrier is seen, in order
         tc_fence_before_sync();
         mbar_arrive(smem_u32(&mc.p_ready[sb]));
-        if (passes_on && j > 0) mbar_arrive(smem_u32(&mc.v_empty[vprev]));      // the tile before: its P V has ended
-        vprev = vcur;
         if (++sb == S_BUFS) sb = 0, sph ^= 1;
       }
       if (ok) {
         wait_o(gt - 1);
-        if (passes_on && ok) mbar_arrive(smem_u32(&mc.v_empty[vprev]));
+        for (; passes_on && ok && freed < gt; ++freed) {
+          mbar_arrive(smem_u32(&mc.v_empty[vfree]));
+          if (++vfree == V_STAGES) vfree = 0;
+        }
       }
+      again();
+      w = piece_at(piece);
+      const int token = w.q_begin + w.tok0 + (there ? row / p.g : 0);
       // ---- merge the groups: each has its share of the channels, summed over both accumulators
       const int mb = it & 1;
       if (spoiled) l = NAN;
@@ -521,8 +557,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
       asm volatile("bar.sync 1, %0;" ::"n"(GROUPS * 128) : "memory");
       tc_fence_after_sync();
       const bool whole = w.count == w.n;
-      // the block's pieces: its first tile is worker c0's, its last worker c1's
-      const int first_tile = a - w.count - w.first, c0 = first_tile / stretch, c1 = (first_tile + w.n - 1) / stretch;
+      const int c0 = w.at / stretch, c1 = (w.at + w.n - 1) / stretch;           // the CTAs that have the block's first and last tile
       float* const part = parts + ((size_t)blockIdx.x * 2 + ((int)blockIdx.x == c0 ? 1 : 0)) * S::PART_FLOATS;
       if (ok && !*abort_s && active) {
         float mt = -INFINITY, lt = 0.f, f[GROUPS];
@@ -538,7 +573,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
         const float inv = whole ? (lt == 0.f ? 0.f : 1.0f / lt) : 1.f;
         __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) +
                              ((size_t)token * p.Hq + w.kvh * p.g + (there ? row % p.g : 0)) * HD + grp * CH;
-        float* pdst = part + row * HD + grp * CH;
+        float4* pdst = reinterpret_cast<float4*>(part) + grp * (CH / 4) * QROWS + row;        // [HD / 4][rows]: neighbouring lanes side by side
 #pragma unroll
         for (int h = 0; h < CH / 16; ++h) {
           float t[16];
@@ -560,7 +595,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
               *reinterpret_cast<uint4*>(dst + h * 16 + 8) = w1;
             } else {
 #pragma unroll
-              for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(pdst + h * 16 + e) = make_float4(t[e], t[e + 1], t[e + 2], t[e + 3]);
+              for (int e = 0; e < 4; ++e) pdst[(h * 4 + e) * QROWS] = make_float4(t[4 * e], t[4 * e + 1], t[4 * e + 2], t[4 * e + 3]);
             }
           }
         }
@@ -571,38 +606,62 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
       if (!whole) {
         // ---- the CTA that counts the last of the block's pieces joins them, in the order of the keys. (A CTA that gave up counts too: the
         // error word says that the results are not to be trusted.)
-        __threadfence();
+        // (The barrier orders what the CTA has written in front of the count, which is a release, and behind it what it reads of the others'.)
         asm volatile("bar.sync 1, %0;" ::"n"(GROUPS * 128) : "memory");
         if (threadIdx.x == 64) {
-          const int seen = atomicAdd(&counters[c0], 1);
+          int seen;
+          asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(seen) : "l"(counters + c0) : "memory");
           mc.last = seen == c1 - c0;
           if (seen == c1 - c0) counters[c0] = 0;         // as the next launch expects it
         }
         asm volatile("bar.sync 1, %0;" ::"n"(GROUPS * 128) : "memory");
         if (mc.last) {
-          __threadfence();
-          // HD / 4 threads a row, four channels each
-          constexpr int PER = HD / 4;
-          const int x = threadIdx.x - 64, c = x % PER;
+          // a thread has a row and a share of the channels, FOURS times four at a time, of four pieces at a time: that many loads are on their way
+          constexpr int FOURS = 2;
+          const int x = threadIdx.x - 64, rows = (w.nrows + 31) & ~31, shares = GROUPS * 128 / rows, row2 = x % rows, share = x / rows;
+          const int mine = HD / 4 / shares;                              // fours of channels
           auto part_of = [&](int cta) { return parts + ((size_t)cta * 2 + (cta == c0 ? 1 : 0)) * S::PART_FLOATS; };
-          for (int row2 = x / PER; row2 < w.nrows; row2 += GROUPS * 128 / PER) {
-            float mt = -INFINITY, lt = 0.f;
-            float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int cta = c0; cta <= c1; ++cta) {
-              const float* from = part_of(cta);
-              const float2 ml = __ldcg(reinterpret_cast<const float2*>(from + QROWS * HD + row2 * 2));
-              const float4 v = __ldcg(reinterpret_cast<const float4*>(from + row2 * HD + c * 4));
-              if (ml.x == -INFINITY && ml.y == 0.f) continue;       // no key of this piece
-              const float top = fmaxf(mt, ml.x);
-              const float keep = mt == -INFINITY ? (lt == 0.f ? 0.f : NAN) : fast_exp2(mt - top);
-              const float add = ml.x == -INFINITY ? NAN : fast_exp2(ml.x - top);
-              t.x = t.x * keep + v.x * add, t.y = t.y * keep + v.y * add, t.z = t.z * keep + v.z * add, t.w = t.w * keep + v.w * add;
-              lt = lt * keep + ml.y * add, mt = top;
-            }
-            const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+          if (share < shares && row2 < w.nrows) {
             __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) +
-                                 ((size_t)(w.q_begin + w.tok0 + row2 / p.g) * p.Hq + w.kvh * p.g + row2 % p.g) * HD + c * 4;
-            *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(t.x * inv, t.y * inv), pack_bf16(t.z * inv, t.w * inv));
+                                 ((size_t)(w.q_begin + w.tok0 + row2 / p.g) * p.Hq + w.kvh * p.g + row2 % p.g) * HD;
+#pragma unroll 1
+            for (int f0 = share * mine; f0 < (share + 1) * mine; f0 += FOURS) {
+              float mt = -INFINITY, lt = 0.f;
+              float4 t[FOURS];
+#pragma unroll
+              for (int i = 0; i < FOURS; ++i) t[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+              for (int cta = c0; cta <= c1; cta += 4) {
+                float2 ml[4];
+                float4 v[4][FOURS];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                  const float* from = part_of(min(cta + u, c1));
+                  ml[u] = __ldcg(reinterpret_cast<const float2*>(from + QROWS * HD + row2 * 2));
+#pragma unroll
+                  for (int i = 0; i < FOURS; ++i) v[u][i] = __ldcg(reinterpret_cast<const float4*>(from) + (f0 + i) * QROWS + row2);
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                  if (cta + u > c1 || (ml[u].x == -INFINITY && ml[u].y == 0.f)) continue;       // no key of this piece
+                  const float top = fmaxf(mt, ml[u].x);
+                  const float keep = mt == -INFINITY ? (lt == 0.f ? 0.f : NAN) : fast_exp2(mt - top);
+                  const float add = ml[u].x == -INFINITY ? NAN : fast_exp2(ml[u].x - top);
+#pragma unroll
+                  for (int i = 0; i < FOURS; ++i) {
+                    t[i].x = t[i].x * keep + v[u][i].x * add, t[i].y = t[i].y * keep + v[u][i].y * add;
+                    t[i].z = t[i].z * keep + v[u][i].z * add, t[i].w = t[i].w * keep + v[u][i].w * add;
+                  }
+                  lt = lt * keep + ml[u].y * add, mt = top;
+                }
+              }
+              const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+#pragma unroll
+              for (int i = 0; i < FOURS; i += 2)
+                *reinterpret_cast<uint4*>(dst + (f0 + i) * 4) =
+                    make_uint4(pack_bf16(t[i].x * inv, t[i].y * inv), pack_bf16(t[i].z * inv, t[i].w * inv),
+                               pack_bf16(t[i + 1].x * inv, t[i + 1].y * inv), pack_bf16(t[i + 1].z * inv, t[i + 1].w * inv));
+            }
           }
         }
       }
