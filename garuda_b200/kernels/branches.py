@@ -25,7 +25,7 @@ _SIGNATURES = {
     "gb_tree_layout": [c_void_p] * 5 + [c_int] * 4 + [c_void_p],
     "gb_tree_accept": [c_void_p] * 6 + [c_int] + [c_void_p] * 2 + [c_int] + [c_void_p] * 4 + [c_longlong, c_void_p] + [c_int] * 4 + [c_void_p],
     "gb_tree_attention_tc": [c_void_p] * 4 + [c_int] + [c_void_p] * 4 + [c_int, c_void_p, c_int, c_int, c_longlong] + [c_int] * 3 + [c_float]
-    + [c_int] * 3 + [c_void_p] * 3,
+    + [c_int] * 4 + [c_void_p] * 3,
     "gb_tree_attention_simple": [c_void_p, c_int] + [c_void_p] * 3 + [c_int] + [c_void_p] * 4 + [c_int, c_void_p, c_int, c_int, c_longlong]
     + [c_int] * 3 + [c_float] + [c_int] * 4 + [c_void_p] * 3,
     "gb_beam_select": [c_void_p, c_longlong, c_void_p] + [c_int] * 4 + [c_void_p] * 6,
@@ -199,7 +199,7 @@ class BranchOps:
             scratch, counters = self._branch_memory("tree_attention", L.gb_tree_attention_scratch_bytes, (hd,), ws, stream)
             self._check(L, L.gb_tree_attention_tc(q_ptr, k_ptr, v_ptr, block_table.data_ptr(), width, cu_q.data_ptr(), kv_lens.data_ptr(),
                                                   positions.data_ptr(), mask.data_ptr(), words, out_ptr, T, R, pages, Hq, Hkv, hd, scale, window,
-                                                  page_size, max_q_len, counters.data_ptr(), scratch.data_ptr(), stream), what,
+                                                  page_size, max_q_len, max_kv_len, counters.data_ptr(), scratch.data_ptr(), stream), what,
                         (R + 2047) // 2048)
             return
         _need(hd % 4 == 0 and hd <= 256, f"{what}: heads of a multiple of 4 channels up to 256")
