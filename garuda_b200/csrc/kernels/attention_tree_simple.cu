@@ -5,9 +5,10 @@
 // one key/value head of one request, and walks its keys 32 at a time, so that a number from shared memory is used eight times in each
 // product. Its 128 threads are 16 pairs of rows by 8: a thread has two rows' scores with four keys, and of the sums two rows' every eighth four
 // channels. A row's eight threads are neighbours of one warp: maxima and sums are three shuffles, and the weights need no barrier.
-// Where the blocks of rows are fewer than the device runs at once, a request's keys are cut into parts that blocks of their own
-// take; the block that counts the last of them joins them in the order of the keys. Masked keys are skipped: nothing of them reaches a sum.
+// Where the blocks of rows are fewer than the device runs at once, a request's keys are shared by the blocks of a thread-block cluster, which join their
+// sums, in the order of the keys, from one another's shared memory. Masked keys are skipped: nothing of them reaches a sum.
 #include "branches.h"
+#include "tc_common.cuh"
 
 namespace {
 
@@ -15,13 +16,10 @@ using branches::TreeParams;
 
 constexpr int ROWS = 32, KEYS = 32, THREADS = 128;
 constexpr int P_LD = KEYS + 4;
+constexpr int MOST_PARTS = 8;
 
-template <int HDMAX>
-struct Shape {
-  static constexpr int MOST = HDMAX / 32;      // fours of channels that a thread sums
-};
 __host__ __device__ constexpr int row_floats(int hd) { return hd + 4; }        // (eight rows' 16 bytes on different banks where hd is a multiple of 32)
-__host__ __device__ constexpr int smem_floats(int hd) { return (ROWS + 2 * KEYS) * row_floats(hd) + ROWS * P_LD; }
+__host__ __device__ constexpr int smem_floats(int hd) { return (ROWS + 4 * KEYS) * row_floats(hd) + ROWS * P_LD; }
 
 template <typename T>
 __device__ __forceinline__ float4 load4(const T* p);
@@ -40,31 +38,59 @@ __device__ __forceinline__ void store4(T* p, float4 v) {
 // exp of a difference; -inf gives 0
 __device__ __forceinline__ float weight_of(float s, float m) { return m == -INFINITY ? 0.f : expf(s - m); }
 
+__device__ __forceinline__ void copy_async_16(float* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+
 template <typename T, int HDMAX>
 __global__ void __launch_bounds__(THREADS)
-attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts, float* __restrict__ scratch, int* __restrict__ counters) {
-  constexpr int MOST = Shape<HDMAX>::MOST;
+attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts) {
+  constexpr int MOST = HDMAX / 32;             // fours of channels that a thread sums
   extern __shared__ __align__(16) float smem[];
-  __shared__ int last_s;
-  const int ld = row_floats(hd);
+  __shared__ long long where[2][KEYS];         // two tiles' keys: their rows' places in the pools, -1: no page
+  const int ld = row_floats(hd), c4 = hd / 4;
   float* const qs = smem;
-  float* const ks = qs + ROWS * ld;
-  float* const vs = ks + KEYS * ld;
-  float* const ps = vs + KEYS * ld;
+  float* const ring = qs + ROWS * ld;          // two tiles: keys, then values
+  float* const ps = ring + 4 * KEYS * ld;
   gb::pdl_launch_dependents();
   gb::pdl_wait();
   const int r = blockIdx.z, kvh = blockIdx.y % p.Hkv, block = blockIdx.y / p.Hkv, part = blockIdx.x;
   const int q_begin = p.cu_q[r], q_len = p.cu_q[r + 1] - q_begin, row0 = block * ROWS, nrows = min(ROWS, q_len * p.g - row0);
   const int kv_len = p.kv_lens[r], ctx = max(0, kv_len - q_len);
-  if (nrows <= 0 || kv_len <= 0) return;
+  if (nrows <= 0 || kv_len <= 0) return;       // (the whole cluster's)
   const int lo = (p.window > 0 ? max(0, ctx + 1 - p.window) : 0) / KEYS, tiles = (kv_len - 1) / KEYS + 1 - lo;
-  const int per = (tiles + parts - 1) / parts, busy = (tiles + per - 1) / per;      // parts that have keys
-  if (part >= busy) return;
-  const int tile_begin = lo + part * per, tile_end = min(lo + tiles, tile_begin + per);
+  const int per = (tiles + parts - 1) / parts, tile_begin = lo + part * per, tile_end = min(lo + tiles, tile_begin + per);
   const int32_t* table = p.block_table + (size_t)r * p.table_width;
 
-  const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3, c4 = hd / 4;
+  const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
+  auto place_keys = [&](int tile) {            // by the first warp
+    if (threadIdx.x < KEYS && tile < tile_end) {
+      const int at = tile * KEYS + threadIdx.x, slot = at / p.page_size;
+      const int page = at < kv_len && slot < p.table_width ? table[slot] : -1;
+      where[tile & 1][threadIdx.x] =
+          page >= 0 && page < p.pages ? (((long long)page * p.Hkv + kvh) * p.page_size + at % p.page_size) * hd : -1;
+    }
+  };
+  // A tile's keys and values: 32-bit ones on their way to shared memory while the tile in front is at work, others by way of registers
+  auto fetch = [&](int tile) {
+    float* const ks = ring + (tile & 1) * 2 * KEYS * ld;
+#pragma unroll 4
+    for (int x = threadIdx.x; x < 2 * KEYS * c4; x += THREADS) {
+      const int half = x >= KEYS * c4, y = x - half * KEYS * c4, key = y / c4, c = y % c4;
+      const long long at = where[tile & 1][key];
+      float* const to = ks + (half * KEYS + key) * ld + c * 4;
+      const T* const from = reinterpret_cast<const T*>(half ? p.v_pool : p.k_pool) + at + c * 4;
+      if (at < 0) *reinterpret_cast<float4*>(to) = make_float4(0.f, 0.f, 0.f, 0.f);
+      else if (sizeof(T) == 4) copy_async_16(to, from);
+      else *reinterpret_cast<float4*>(to) = load4(from);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
   const T* q = reinterpret_cast<const T*>(p.q);
+  place_keys(tile_begin);
+  place_keys(tile_begin + 1);
+  __syncthreads();
+  if (tile_begin < tile_end) fetch(tile_begin);
   for (int x = threadIdx.x; x < ROWS * c4; x += THREADS) {
     const int row = x / c4, c = x % c4, at = row0 + row;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -90,22 +116,15 @@ attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts, 
 
   for (int tile = tile_begin; tile < tile_end; ++tile) {
     const int key0 = tile * KEYS;
-    __syncthreads();
-    for (int x = threadIdx.x; x < KEYS * c4; x += THREADS) {
-      const int key = x / c4, c = x % c4, at = key0 + key, slot = at / p.page_size;
-      const int page = at < kv_len && slot < p.table_width ? table[slot] : -1;
-      float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
-      if (page >= 0 && page < p.pages) {
-        const size_t where = (((size_t)page * p.Hkv + kvh) * p.page_size + at % p.page_size) * hd + c * 4;
-        k = load4(reinterpret_cast<const T*>(p.k_pool) + where);
-        v = load4(reinterpret_cast<const T*>(p.v_pool) + where);
-      }
-      *reinterpret_cast<float4*>(ks + key * ld + c * 4) = k;
-      *reinterpret_cast<float4*>(vs + key * ld + c * 4) = v;
-    }
-    __syncthreads();
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();                           // the tile is there, and all are done with the one in front
+    if (tile + 1 < tile_end) fetch(tile + 1);
+    place_keys(tile + 2);
+    const float* const ks = ring + (tile & 1) * 2 * KEYS * ld;
+    const float* const vs = ks + KEYS * ld;
     // ---- scores of two rows with keys tx, tx + 8, tx + 16, tx + 24
     float s[2][4] = {};
+#pragma unroll 4
     for (int c = 0; c < c4; ++c) {
       float4 a[2], b[4];
 #pragma unroll
@@ -159,16 +178,21 @@ attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts, 
     }
     __syncwarp();
     // ---- sums of two rows' channels 4 tx + 32 c
-    for (int key = 0; key < KEYS; ++key) {
-      const float w0 = ps[2 * ty * P_LD + key], w1 = ps[(2 * ty + 1) * P_LD + key];
+#pragma unroll 2
+    for (int key = 0; key < KEYS; key += 4) {
+      const float4 w0 = *reinterpret_cast<const float4*>(ps + 2 * ty * P_LD + key), w1 = *reinterpret_cast<const float4*>(ps + (2 * ty + 1) * P_LD + key);
 #pragma unroll
-      for (int c = 0; c < MOST; ++c) {
-        if (4 * tx + 32 * c >= hd) break;
-        const float4 v = *reinterpret_cast<const float4*>(vs + key * ld + 4 * tx + 32 * c);
-        if (!edge || w0 != 0.f)
-          o[0][c].x = fmaf(w0, v.x, o[0][c].x), o[0][c].y = fmaf(w0, v.y, o[0][c].y), o[0][c].z = fmaf(w0, v.z, o[0][c].z), o[0][c].w = fmaf(w0, v.w, o[0][c].w);
-        if (!edge || w1 != 0.f)
-          o[1][c].x = fmaf(w1, v.x, o[1][c].x), o[1][c].y = fmaf(w1, v.y, o[1][c].y), o[1][c].z = fmaf(w1, v.z, o[1][c].z), o[1][c].w = fmaf(w1, v.w, o[1][c].w);
+      for (int e = 0; e < 4; ++e) {
+        const float u0 = e == 0 ? w0.x : e == 1 ? w0.y : e == 2 ? w0.z : w0.w, u1 = e == 0 ? w1.x : e == 1 ? w1.y : e == 2 ? w1.z : w1.w;
+#pragma unroll
+        for (int c = 0; c < MOST; ++c) {
+          if (4 * tx + 32 * c >= hd) break;
+          const float4 v = *reinterpret_cast<const float4*>(vs + (key + e) * ld + 4 * tx + 32 * c);
+          if (!edge || u0 != 0.f)
+            o[0][c].x = fmaf(u0, v.x, o[0][c].x), o[0][c].y = fmaf(u0, v.y, o[0][c].y), o[0][c].z = fmaf(u0, v.z, o[0][c].z), o[0][c].w = fmaf(u0, v.w, o[0][c].w);
+          if (!edge || u1 != 0.f)
+            o[1][c].x = fmaf(u1, v.x, o[1][c].x), o[1][c].y = fmaf(u1, v.y, o[1][c].y), o[1][c].z = fmaf(u1, v.z, o[1][c].z), o[1][c].w = fmaf(u1, v.w, o[1][c].w);
+        }
       }
     }
     __syncwarp();
@@ -179,7 +203,7 @@ attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts, 
     for (int d = 1; d < 8; d <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], d);
   T* const out = reinterpret_cast<T*>(p.out);
   auto place = [&](int row) { return out + ((size_t)(q_begin + (row0 + row) / p.g) * p.Hq + kvh * p.g + (row0 + row) % p.g) * hd; };
-  if (busy == 1) {
+  if (parts == 1) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const float inv = l[i] == 0.f ? 0.f : 1.0f / l[i];
@@ -190,60 +214,53 @@ attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts, 
     }
     return;
   }
-  // ---- parts: sums, maximum and denominator of every row to scratch memory; the last block joins them
-  const int rs = hd + 4, unit = r * gridDim.y + blockIdx.y;
-  float* const all = scratch + (size_t)unit * parts * ROWS * rs;
+  // ---- the cluster's parts: every row's sums, maximum and denominator where the tiles were, then each block joins its share of the rows
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    if (!there[i]) continue;
-    float* to = all + (size_t)(part * ROWS + 2 * ty + i) * rs;
+    float* to = ring + (2 * ty + i) * ld;
 #pragma unroll
     for (int c = 0; c < MOST; ++c)
       if (4 * tx + 32 * c < hd) *reinterpret_cast<float4*>(to + 4 * tx + 32 * c) = o[i][c];
     if (tx == 0) to[hd] = m[i], to[hd + 1] = l[i];
   }
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const int seen = atomicAdd(&counters[unit], 1);
-    last_s = seen == busy - 1;
-    if (last_s) counters[unit] = 0;           // as the next launch expects it
-  }
-  __syncthreads();
-  if (!last_s) return;
-  __threadfence();
-  for (int x = threadIdx.x; x < nrows * c4; x += THREADS) {
+  tc::cluster_arrive_wait();
+  for (int x = part * THREADS + threadIdx.x; x < nrows * c4; x += parts * THREADS) {
     const int row = x / c4, c = x % c4;
+    const uint32_t v_at = tc::smem_u32(ring + row * ld + c * 4), ml_at = tc::smem_u32(ring + row * ld + hd);
+    float2 ml[MOST_PARTS];
+    float4 v[MOST_PARTS];
+#pragma unroll
+    for (int i = 0; i < MOST_PARTS; ++i) {
+      const uint32_t from = min(i, parts - 1), a = tc::map_to_rank(ml_at, from), b = tc::map_to_rank(v_at, from);
+      asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml[i].x), "=f"(ml[i].y) : "r"(a) : "memory");
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[i].x), "=f"(v[i].y), "=f"(v[i].z), "=f"(v[i].w) : "r"(b) : "memory");
+    }
     float mt = -INFINITY, lt = 0.f;
     float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = 0; i < busy; ++i) {
-      const float* from = all + (size_t)(i * ROWS + row) * rs;
-      const float mi = __ldcg(from + hd), li = __ldcg(from + hd + 1);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(from + c * 4));
-      if (mi == -INFINITY && li == 0.f) continue;        // no key of this part
-      const float top = fmaxf(mt, mi), keep = mt == -INFINITY ? 1.f : weight_of(mt, top), add = mi == -INFINITY ? 1.f : weight_of(mi, top);
-      t.x = t.x * keep + v.x * add, t.y = t.y * keep + v.y * add, t.z = t.z * keep + v.z * add, t.w = t.w * keep + v.w * add;
-      lt = lt * keep + li * add, mt = top;
+#pragma unroll
+    for (int i = 0; i < MOST_PARTS; ++i) {
+      if (i >= parts || (ml[i].x == -INFINITY && ml[i].y == 0.f)) continue;        // no key of this part
+      const float top = fmaxf(mt, ml[i].x), keep = mt == -INFINITY ? 1.f : weight_of(mt, top), add = ml[i].x == -INFINITY ? 1.f : weight_of(ml[i].x, top);
+      t.x = t.x * keep + v[i].x * add, t.y = t.y * keep + v[i].y * add, t.z = t.z * keep + v[i].z * add, t.w = t.w * keep + v[i].w * add;
+      lt = lt * keep + ml[i].y * add, mt = top;
     }
     const float inv = lt == 0.f ? 0.f : 1.0f / lt;
     store4(place(row) + c * 4, make_float4(t.x * inv, t.y * inv, t.z * inv, t.w * inv));
   }
+  tc::cluster_arrive_wait();                   // nobody leaves while another reads
 }
 
-struct Cut {
-  int blocks, parts;
-};
-// Parts of a request's keys: as many as fill the device four times over, each of at least four tiles
-Cut cut_of(int R, int max_q_len, int g, int Hkv, int max_kv_len) {
-  const int blocks = (max_q_len * g + ROWS - 1) / ROWS, tiles = (max_kv_len + KEYS - 1) / KEYS;
-  const long long units = (long long)R * blocks * Hkv;
-  long long parts = 4ll * gb::sm_count() / (units < 1 ? 1 : units);
-  if (parts > (tiles + 3) / 4) parts = (tiles + 3) / 4;
-  return {blocks, parts < 1 ? 1 : (int)parts};
+// Parts of a request's keys, a power of two: as many as fill the device four times over, each of two tiles at least.
+int parts_of(long long units, int max_kv_len) {
+  const int tiles = (max_kv_len + KEYS - 1) / KEYS;
+  int parts = 1;
+  while (parts < MOST_PARTS && 2 * parts * units <= 4ll * gb::sm_count() && 4 * parts <= tiles) parts *= 2;
+  return parts;
 }
 
 template <typename T, int HDMAX>
-int launch(const TreeParams& p, int hd, Cut cut, float* scratch, int* counters, cudaStream_t stream) {
+int launch(const TreeParams& p, int hd, int blocks, int parts, cudaStream_t stream) {
   static gb::OncePerDevice configured;
   if (configured.needed()) {
     const cudaError_t e = cudaFuncSetAttribute(attention_tree_simple_kernel<T, HDMAX>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -251,35 +268,25 @@ int launch(const TreeParams& p, int hd, Cut cut, float* scratch, int* counters, 
     if (e != cudaSuccess) return gb::fail(GB_CUDA_ERROR, "tree_attention: %s", cudaGetErrorString(e));
     configured.done();
   }
-  return gb::check_pdl_launch(gb::launch_pdl(attention_tree_simple_kernel<T, HDMAX>, dim3(cut.parts, cut.blocks * p.Hkv, p.R), dim3(THREADS),
-                                             4 * smem_floats(hd), stream, dim3(1), p, hd, cut.parts, scratch, counters), "tree_attention");
+  return gb::check_pdl_launch(gb::launch_pdl(attention_tree_simple_kernel<T, HDMAX>, dim3(parts, blocks * p.Hkv, p.R), dim3(THREADS),
+                                             4 * smem_floats(hd), stream, dim3(parts), p, hd, parts), "tree_attention");
 }
 
 }  // namespace
 
-// Bytes of scratch memory of a call, of which the counters' are zero before the first one and after every one.
-GB_EXPORT long long gb_tree_attention_simple_scratch_bytes(int R, int max_q_len, int Hq, int Hkv, int head_dim, int max_kv_len,
-                                                           long long* counter_bytes) {
-  const Cut cut = cut_of(R, max_q_len, Hq / Hkv, Hkv, max_kv_len);
-  const long long units = (long long)R * cut.blocks * Hkv;
-  *counter_bytes = cut.parts > 1 ? (4 * units + 15) / 16 * 16 : 16;
-  return cut.parts > 1 ? units * cut.parts * ROWS * (head_dim + 4) * 4 : 16;
-}
-
 GB_EXPORT int gb_tree_attention_simple(const void* q, int dtype, const void* k_pool, const void* v_pool, const int32_t* block_table, int table_width,
                                        const int32_t* cu_q, const int32_t* kv_lens, const int32_t* positions, const int32_t* mask, int mask_words,
                                        void* out, int T, int R, long long pages, int Hq, int Hkv, int head_dim, float scale, int window,
-                                       int page_size, int max_q_len, int max_kv_len, void* counters, void* scratch, void* stream) {
+                                       int page_size, int max_q_len, int max_kv_len, void* stream) {
   const TreeParams p{q, k_pool, v_pool, out, block_table, cu_q, kv_lens, positions, reinterpret_cast<const uint32_t*>(mask), pages,
                      table_width, mask_words, Hq, Hkv, Hq / Hkv, window, page_size, T, R, scale};
-  const Cut cut = cut_of(R, max_q_len, p.g, Hkv, max_kv_len);
+  const long long blocks = ((long long)max_q_len * p.g + ROWS - 1) / ROWS;
   if (head_dim % 4 != 0 || head_dim > 256) return gb::fail(GB_UNSUPPORTED, "tree_attention: heads of %d channels", head_dim);
-  if (R > 65535 || (long long)cut.blocks * Hkv > 65535) return gb::fail(GB_UNSUPPORTED, "tree_attention: %d requests, %d blocks of rows", R, cut.blocks * Hkv);
+  if (R > 65535 || blocks * Hkv > 65535) return gb::fail(GB_UNSUPPORTED, "tree_attention: %d requests, %lld blocks of rows", R, blocks * Hkv);
+  const int parts = parts_of(R * blocks * Hkv, max_kv_len);
   return GB_DISPATCH_DTYPE(dtype, E, [&]() -> int {
-    float* parts = reinterpret_cast<float*>(scratch);
-    int* counts = reinterpret_cast<int*>(counters);
-    if (head_dim <= 64) return launch<E, 64>(p, head_dim, cut, parts, counts, (cudaStream_t)stream);
-    if (head_dim <= 128) return launch<E, 128>(p, head_dim, cut, parts, counts, (cudaStream_t)stream);
-    return launch<E, 256>(p, head_dim, cut, parts, counts, (cudaStream_t)stream);
+    if (head_dim <= 64) return launch<E, 64>(p, head_dim, (int)blocks, parts, (cudaStream_t)stream);
+    if (head_dim <= 128) return launch<E, 128>(p, head_dim, (int)blocks, parts, (cudaStream_t)stream);
+    return launch<E, 256>(p, head_dim, (int)blocks, parts, (cudaStream_t)stream);
   });
 }

@@ -27,7 +27,7 @@ _SIGNATURES = {
     "gb_tree_attention_tc": [c_void_p] * 4 + [c_int] + [c_void_p] * 4 + [c_int, c_void_p, c_int, c_int, c_longlong] + [c_int] * 3 + [c_float]
     + [c_int] * 4 + [c_void_p] * 3,
     "gb_tree_attention_simple": [c_void_p, c_int] + [c_void_p] * 3 + [c_int] + [c_void_p] * 4 + [c_int, c_void_p, c_int, c_int, c_longlong]
-    + [c_int] * 3 + [c_float] + [c_int] * 4 + [c_void_p] * 3,
+    + [c_int] * 3 + [c_float] + [c_int] * 4 + [c_void_p],
     "gb_beam_select": [c_void_p, c_longlong, c_void_p] + [c_int] * 4 + [c_void_p] * 6,
     "gb_copy_entries": [c_int] + [c_void_p] * 6 + [c_int, c_void_p],
     "gb_tree_attention_error_check": [],
@@ -61,7 +61,6 @@ class BranchOps:
                 fn = getattr(L, name)
                 fn.argtypes, fn.restype = argtypes, c_int
             sizes = {"gb_tree_attention_scratch_bytes": [c_int, ctypes.POINTER(c_longlong)],
-                     "gb_tree_attention_simple_scratch_bytes": [c_int] * 6 + [ctypes.POINTER(c_longlong)],
                      "gb_beam_select_scratch_bytes": [c_int] * 4 + [ctypes.POINTER(c_longlong)]}
             for name, argtypes in sizes.items():
                 fn = getattr(L, name)
@@ -204,11 +203,9 @@ class BranchOps:
             return
         _need(hd % 4 == 0 and hd <= 256, f"{what}: heads of a multiple of 4 channels up to 256")
         _need(not (q_ptr | k_ptr | v_ptr | out_ptr) & (15 if dtype is torch.float32 else 7), f"{what}: operands on 16 bytes (bfloat16: 8)")
-        scratch, counters = self._branch_memory("tree_attention_simple", L.gb_tree_attention_simple_scratch_bytes,
-                                                (R, max_q_len, Hq, Hkv, hd, max_kv_len), ws, stream)
         self._check(L, L.gb_tree_attention_simple(q_ptr, _TAG[dtype], k_ptr, v_ptr, block_table.data_ptr(), width, cu_q.data_ptr(), kv_lens.data_ptr(),
                                                   positions.data_ptr(), mask.data_ptr(), words, out_ptr, T, R, pages, Hq, Hkv, hd, scale, window,
-                                                  page_size, max_q_len, max_kv_len, counters.data_ptr(), scratch.data_ptr(), stream), what)
+                                                  page_size, max_q_len, max_kv_len, stream), what)
 
     def tree_accept(self, tokens, targets, parents, cu_q, kv_lens, path, kept, next_tokens, max_q_len: int, pools=(), block_table=None,
                     page_size: int = 0):

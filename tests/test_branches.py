@@ -24,7 +24,7 @@ class Recorder(BranchOps):
 
         self._branches = types.SimpleNamespace(**{n: entry(n) for n in (
             "gb_tree_layout", "gb_tree_accept", "gb_tree_attention_tc", "gb_tree_attention_simple", "gb_beam_select", "gb_copy_entries",
-            "gb_tree_attention_scratch_bytes", "gb_tree_attention_simple_scratch_bytes", "gb_beam_select_scratch_bytes")})
+            "gb_tree_attention_scratch_bytes", "gb_beam_select_scratch_bytes")})
 
     def _stream(self):
         return 0
