@@ -274,19 +274,16 @@ int launch(const TreeParams& p, int hd, int blocks, int parts, cudaStream_t stre
 
 }  // namespace
 
-GB_EXPORT int gb_tree_attention_simple(const void* q, int dtype, const void* k_pool, const void* v_pool, const int32_t* block_table, int table_width,
-                                       const int32_t* cu_q, const int32_t* kv_lens, const int32_t* positions, const int32_t* mask, int mask_words,
-                                       void* out, int T, int R, long long pages, int Hq, int Hkv, int head_dim, float scale, int window,
-                                       int page_size, int max_q_len, int max_kv_len, void* stream) {
-  const TreeParams p{q, k_pool, v_pool, out, block_table, cu_q, kv_lens, positions, reinterpret_cast<const uint32_t*>(mask), pages,
-                     table_width, mask_words, Hq, Hkv, Hq / Hkv, window, page_size, T, R, scale};
-  const long long blocks = ((long long)max_q_len * p.g + ROWS - 1) / ROWS;
+GB_EXPORT int gb_tree_attention_simple(const branches::TreeCall* call) {
+  const TreeParams p = call->params();
+  const int R = p.R, Hkv = p.Hkv, head_dim = (int)call->head_dim;
+  const long long blocks = (call->max_q_len * p.g + ROWS - 1) / ROWS;
   if (head_dim % 4 != 0 || head_dim > 256) return gb::fail(GB_UNSUPPORTED, "tree_attention: heads of %d channels", head_dim);
   if (R > 65535 || blocks * Hkv > 65535) return gb::fail(GB_UNSUPPORTED, "tree_attention: %d requests, %lld blocks of rows", R, blocks * Hkv);
-  const int parts = parts_of(R * blocks * Hkv, max_kv_len);
-  return GB_DISPATCH_DTYPE(dtype, E, [&]() -> int {
-    if (head_dim <= 64) return launch<E, 64>(p, head_dim, (int)blocks, parts, (cudaStream_t)stream);
-    if (head_dim <= 128) return launch<E, 128>(p, head_dim, (int)blocks, parts, (cudaStream_t)stream);
-    return launch<E, 256>(p, head_dim, (int)blocks, parts, (cudaStream_t)stream);
+  const int parts = parts_of(R * blocks * Hkv, (int)call->max_kv_len);
+  return GB_DISPATCH_DTYPE(call->dtype, E, [&]() -> int {
+    if (head_dim <= 64) return launch<E, 64>(p, head_dim, (int)blocks, parts, (cudaStream_t)call->stream);
+    if (head_dim <= 128) return launch<E, 128>(p, head_dim, (int)blocks, parts, (cudaStream_t)call->stream);
+    return launch<E, 256>(p, head_dim, (int)blocks, parts, (cudaStream_t)call->stream);
   });
 }

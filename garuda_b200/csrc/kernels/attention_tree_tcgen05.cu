@@ -854,17 +854,14 @@ GB_EXPORT long long gb_tree_attention_scratch_bytes(int head_dim, long long* cou
   return 2ll * tc_host::sm_count() * QROWS * (head_dim + 2) * 4;
 }
 
-GB_EXPORT int gb_tree_attention_tc(const void* q, const void* k_pool, const void* v_pool, const int32_t* block_table, int table_width,
-                                   const int32_t* cu_q, const int32_t* kv_lens, const int32_t* positions, const int32_t* mask, int mask_words,
-                                   void* out, int T, int R, long long pages, int Hq, int Hkv, int head_dim, float scale, int window, int page_size,
-                                   int max_q_len, int max_kv_len, void* counters, void* scratch, void* stream) {
-  TreeParams p{q, k_pool, v_pool, out, block_table, cu_q, kv_lens, positions, reinterpret_cast<const uint32_t*>(mask), pages,
-               table_width, mask_words, Hq, Hkv, Hq / Hkv, window, page_size, T, R, scale};
-  int* counts = reinterpret_cast<int*>(counters);
-  float* parts = reinterpret_cast<float*>(scratch);
-  if (head_dim == 64) return launch<64>(p, max_q_len, max_kv_len, counts, parts, (cudaStream_t)stream);
-  if (head_dim == 128) return launch<128>(p, max_q_len, max_kv_len, counts, parts, (cudaStream_t)stream);
-  return gb::fail(GB_UNSUPPORTED, "tree_attention: head size %d", head_dim);
+GB_EXPORT int gb_tree_attention_tc(const branches::TreeCall* call) {
+  const TreeParams p = call->params();
+  int* counters = reinterpret_cast<int*>(call->counters);
+  float* parts = reinterpret_cast<float*>(call->scratch);
+  const int max_q_len = (int)call->max_q_len, max_kv_len = (int)call->max_kv_len;
+  if (call->head_dim == 64) return launch<64>(p, max_q_len, max_kv_len, counters, parts, (cudaStream_t)call->stream);
+  if (call->head_dim == 128) return launch<128>(p, max_q_len, max_kv_len, counters, parts, (cudaStream_t)call->stream);
+  return gb::fail(GB_UNSUPPORTED, "tree_attention: head size %lld", call->head_dim);
 }
 
 GB_EXPORT int gb_tree_attention_error_check() { return gb_err::fetch_and_clear(); }

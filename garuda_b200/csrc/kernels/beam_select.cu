@@ -479,13 +479,21 @@ GB_EXPORT long long gb_beam_select_scratch_bytes(int items, int beams, int V, in
   return rows * chunks * (long long)(sizeof(Part) + K * sizeof(Key));
 }
 
-GB_EXPORT int gb_beam_select(const float* logits, long long ld, const float* scores, int items, int beams, int V, int K, float* best, int32_t* parents,
-                             int32_t* tokens, void* counters, void* scratch, void* stream) {
+// What the caller packs, eight bytes each.
+struct BeamCall {
+  const float *logits, *scores;
+  float* best;
+  int32_t *parents, *tokens;
+  void *counters, *scratch, *stream;
+  long long ld, items, beams, V, K;
+};
+GB_EXPORT int gb_beam_select(const BeamCall* call) {
+  const int items = (int)call->items, beams = (int)call->beams, V = (int)call->V, K = (int)call->K;
   if (K > MOST || beams > MOST) return gb::fail(GB_UNSUPPORTED, "beam_select: %d of %d beams (at most %d)", K, beams, MOST);
   const int rows = items * beams;
   if (rows > 65535) return gb::fail(GB_UNSUPPORTED, "beam_select: %d rows of logits", rows);
   const Cut cut = cut_of(rows, V);
-  Part* parts = reinterpret_cast<Part*>(scratch);
+  Part* parts = reinterpret_cast<Part*>(call->scratch);
   Key* lists = reinterpret_cast<Key*>(parts + (long long)rows * cut.chunks);
   auto launch = [&](auto values) {
     constexpr int VALUES = decltype(values)::value, RING = STAGES * THREADS * VALUES * 4, SMEM = RING > (int)sizeof(Joined) ? RING : (int)sizeof(Joined);
@@ -495,9 +503,9 @@ GB_EXPORT int gb_beam_select(const float* logits, long long ld, const float* sco
       if (e != cudaSuccess) return gb::fail(GB_CUDA_ERROR, "beam_select: %s", cudaGetErrorString(e));
       configured.done();
     }
-    return gb::check_pdl_launch(gb::launch_pdl(beam_select_kernel<VALUES>, dim3(cut.chunks, rows), dim3(THREADS), SMEM, (cudaStream_t)stream, dim3(1),
-                                               logits, ld, scores, V, beams, K, cut.per_block, best, parents, tokens, parts, lists,
-                                               reinterpret_cast<int*>(counters)), "beam_select");
+    return gb::check_pdl_launch(gb::launch_pdl(beam_select_kernel<VALUES>, dim3(cut.chunks, rows), dim3(THREADS), SMEM, (cudaStream_t)call->stream, dim3(1),
+                                               call->logits, call->ld, call->scores, V, beams, K, cut.per_block, call->best, call->parents, call->tokens, parts,
+                                               lists, reinterpret_cast<int*>(call->counters)), "beam_select");
   };
   return cut.small ? launch(std::integral_constant<int, 4>{}) : launch(std::integral_constant<int, MANY>{});
 }

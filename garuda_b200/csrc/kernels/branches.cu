@@ -77,7 +77,7 @@ constexpr int AHEAD = 8;
 struct Arrays {
   static constexpr int MOST = 64;
   uint8_t* at[MOST];          // [calls, pages, heads, page_size, row] each
-  int calls[MOST], heads[MOST], row_bytes[MOST];
+  int heads[MOST], row_bytes[MOST];
   int first[MOST + 1];        // calls of the arrays in front
   int n;
 };
@@ -270,11 +270,17 @@ GB_EXPORT int gb_tree_layout(const int32_t* parents, const int32_t* cu_q, const 
                               "tree_layout");
 }
 
-// arrays: n of them, [calls, pages, heads, page_size, row bytes] each
-GB_EXPORT int gb_tree_accept(const int32_t* tokens, const int32_t* targets, const int32_t* parents, const int32_t* cu_q, const int32_t* kv_lens,
-                             int32_t* path, int path_width, int32_t* kept, int32_t* next_tokens, int n, void* const* at, const int32_t* calls,
-                             const int32_t* heads, const int32_t* row_bytes, long long pages, const int32_t* block_table, int table_width,
-                             int page_size, int R, int max_q_len, void* stream) {
+// What the caller packs, eight bytes each (see TreeCall).
+struct AcceptCall {
+  const int32_t *tokens, *targets, *parents, *cu_q, *kv_lens;
+  int32_t *path, *kept, *next_tokens;
+  const int32_t* block_table;
+  const long long* pools;          // n times {address, calls, heads, bytes of a row}: arrays [calls, pages, heads, page_size, row bytes]
+  void* stream;
+  long long n, pages, path_width, table_width, page_size, R, max_q_len;
+};
+GB_EXPORT int gb_tree_accept(const AcceptCall* call) {
+  const int n = (int)call->n, R = (int)call->R, max_q_len = (int)call->max_q_len;
   if (n > Arrays::MOST) return gb::fail(GB_UNSUPPORTED, "tree_accept: %d pools (at most %d)", n, Arrays::MOST);
   if (max_q_len > ACCEPT_TOKENS) return gb::fail(GB_UNSUPPORTED, "tree_accept: %d drafted tokens of one request (at most %d)", max_q_len, ACCEPT_TOKENS);
   if (R <= 0) return GB_OK;
@@ -282,9 +288,10 @@ GB_EXPORT int gb_tree_accept(const int32_t* tokens, const int32_t* targets, cons
   a.n = n;
   uintptr_t all = 0;
   for (int k = 0; k < n; ++k) {
-    a.at[k] = (uint8_t*)at[k], a.calls[k] = calls[k], a.heads[k] = heads[k], a.row_bytes[k] = row_bytes[k];
-    a.first[k + 1] = a.first[k] + calls[k];
-    all |= (uintptr_t)at[k] | (uintptr_t)row_bytes[k];
+    const long long* pool = call->pools + 4 * k;
+    a.at[k] = (uint8_t*)pool[0], a.heads[k] = (int)pool[2], a.row_bytes[k] = (int)pool[3];
+    a.first[k + 1] = a.first[k] + (int)pool[1];
+    all |= (uintptr_t)pool[0] | (uintptr_t)pool[3];
   }
   const int rows = a.first[n];
   // as many blocks as run at once (eight of 256 threads an SM), and no more walks than that
@@ -299,18 +306,24 @@ GB_EXPORT int gb_tree_accept(const int32_t* tokens, const int32_t* targets, cons
       if (e != cudaSuccess) return gb::fail(GB_CUDA_ERROR, "tree_accept: %s", cudaGetErrorString(e));
       configured.done();
     }
-    return gb::check_pdl_launch(gb::launch_pdl(kernel, dim3(blocks, R), dim3(ACCEPT_THREADS), smem, (cudaStream_t)stream, dim3(1), tokens, targets,
-                                               parents, cu_q, kv_lens, path, path_width, kept, next_tokens, a, pages, block_table, table_width,
-                                               page_size, max_q_len, per_block), "tree_accept");
+    return gb::check_pdl_launch(gb::launch_pdl(kernel, dim3(blocks, R), dim3(ACCEPT_THREADS), smem, (cudaStream_t)call->stream, dim3(1), call->tokens,
+                                               call->targets, call->parents, call->cu_q, call->kv_lens, call->path, (int)call->path_width, call->kept,
+                                               call->next_tokens, a, call->pages, call->block_table, (int)call->table_width, (int)call->page_size, max_q_len,
+                                               per_block), "tree_accept");
   };
   if (all % 16 == 0) return launch(uint4{});
   if (all % 4 == 0) return launch(uint32_t{});
   return launch(uint16_t{});
 }
 
-// arrays: n of them, [outer, entries, bytes] each; no more than MOST_COPIES copies
-GB_EXPORT int gb_copy_entries(int n, void* const* at, const int32_t* outer, const int32_t* entries, const long long* bytes, const int32_t* source,
-                              const int32_t* target, int copies, void* stream) {
+struct CopyCall {
+  const int32_t *source, *target;
+  const long long* arrays;         // n times {address, outer, entries, bytes}
+  void* stream;
+  long long n, copies;
+};
+GB_EXPORT int gb_copy_entries(const CopyCall* call) {
+  const int n = (int)call->n, copies = (int)call->copies;
   if (copies > MOST_COPIES) return gb::fail(GB_UNSUPPORTED, "copy_entries: %d copies (at most %d)", copies, MOST_COPIES);
   if (copies <= 0) return GB_OK;
   // Shared memory for one column of every copy: a quarter of an SM's, as long as that gives columns of 512 bytes, else more.
@@ -319,9 +332,10 @@ GB_EXPORT int gb_copy_entries(int n, void* const* at, const int32_t* outer, cons
     uintptr_t all = 0;
     long long widest = 0;
     for (int k = k0; k < n && a.n < CopyArrays::MOST; ++k, ++a.n) {
-      a.at[a.n] = (uint8_t*)at[k], a.outer[a.n] = outer[k], a.entries[a.n] = entries[k], a.bytes[a.n] = bytes[k];
-      all |= (uintptr_t)at[k] | (uintptr_t)bytes[k];
-      widest = widest > bytes[k] ? widest : bytes[k];
+      const long long* array = call->arrays + 4 * k;
+      a.at[a.n] = (uint8_t*)array[0], a.outer[a.n] = (int)array[1], a.entries[a.n] = (int)array[2], a.bytes[a.n] = array[3];
+      all |= (uintptr_t)array[0] | (uintptr_t)array[3];
+      widest = widest > array[3] ? widest : array[3];
     }
     constexpr int QUARTER = 40 * 1024, WHOLE = 200 * 1024;
     long long column = QUARTER / copies >= 512 ? QUARTER / copies : WHOLE / copies < 512 ? WHOLE / copies : 512;
@@ -341,8 +355,8 @@ GB_EXPORT int gb_copy_entries(int n, void* const* at, const int32_t* outer, cons
         if (e != cudaSuccess) return gb::fail(GB_CUDA_ERROR, "copy_entries: %s", cudaGetErrorString(e));
         configured.done();
       }
-      return gb::check_pdl_launch(gb::launch_pdl(kernel, dim3((unsigned)(pieces < room ? pieces : room)), dim3(COPY_THREADS), smem, (cudaStream_t)stream,
-                                                 dim3(1), a, source, target, copies, (int)column), "copy_entries");
+      return gb::check_pdl_launch(gb::launch_pdl(kernel, dim3((unsigned)(pieces < room ? pieces : room)), dim3(COPY_THREADS), smem, (cudaStream_t)call->stream,
+                                                 dim3(1), a, call->source, call->target, copies, (int)column), "copy_entries");
     };
     const int rc = all % 16 == 0 ? launch(uint4{}) : all % 4 == 0 ? launch(uint32_t{}) : launch(uint8_t{});
     if (rc) return rc;

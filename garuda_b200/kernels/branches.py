@@ -12,7 +12,10 @@ ways a copy of its last page and of its states (``PagedCache.fork`` says which).
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_void_p, c_int, c_float, c_longlong
+import math
+import struct
+from array import array
+from ctypes import c_char_p, c_int, c_longlong, c_void_p
 
 import torch
 
@@ -23,13 +26,11 @@ _capturing = torch._C._cuda_isCurrentStreamCapturing
 
 _SIGNATURES = {
     "gb_tree_layout": [c_void_p] * 5 + [c_int] * 4 + [c_void_p],
-    "gb_tree_accept": [c_void_p] * 6 + [c_int] + [c_void_p] * 2 + [c_int] + [c_void_p] * 4 + [c_longlong, c_void_p] + [c_int] * 4 + [c_void_p],
-    "gb_tree_attention_tc": [c_void_p] * 4 + [c_int] + [c_void_p] * 4 + [c_int, c_void_p, c_int, c_int, c_longlong] + [c_int] * 3 + [c_float]
-    + [c_int] * 4 + [c_void_p] * 3,
-    "gb_tree_attention_simple": [c_void_p, c_int] + [c_void_p] * 3 + [c_int] + [c_void_p] * 4 + [c_int, c_void_p, c_int, c_int, c_longlong]
-    + [c_int] * 3 + [c_float] + [c_int] * 4 + [c_void_p],
-    "gb_beam_select": [c_void_p, c_longlong, c_void_p] + [c_int] * 4 + [c_void_p] * 6,
-    "gb_copy_entries": [c_int] + [c_void_p] * 6 + [c_int, c_void_p],
+    "gb_tree_accept": [c_char_p],
+    "gb_tree_attention_tc": [c_char_p],
+    "gb_tree_attention_simple": [c_char_p],
+    "gb_beam_select": [c_char_p],
+    "gb_copy_entries": [c_char_p],
     "gb_tree_attention_error_check": [],
     "gb_tree_attention_set_error_sink": [c_void_p],
     "gb_beam_select_error_check": [],
@@ -37,12 +38,16 @@ _SIGNATURES = {
     "gb_branches_error_check": [],
     "gb_branches_set_error_sink": [c_void_p],
 }
+# What the entry points of one argument take: the fields of their structures in order, eight bytes each (a call of two dozen arguments takes three
+# microseconds, packing them half of one)
+_TREE_CALL, _ACCEPT_CALL, _BEAM_CALL, _COPY_CALL = (struct.Struct(f) for f in ("=12Q13qd", "=11Q7q", "=8Q5q", "=4Q2q"))
 
 
 class BranchOps:
     """What ``CudaOps`` has of branches. Everything is launched on torch's current stream; results do not depend on the order in which blocks
     finish. Scratch memory is the call's ``ws``, else that of the step that is running (``scratch_from``), else one that the set
-    keeps for the stream; a call captured into a graph without ``ws`` has memory of its graph's own. One ``ws`` is for one stream at a time."""
+    keeps for the stream; a call captured into a graph without ``ws`` has memory of its graph's own (and clears its counters in every replay). One
+    ``ws`` is for one stream at a time, and not to be used on after a call that gave up a wait."""
 
     #: ``tree_layout`` and ``tree_accept`` take trees of up to this many tokens
     MOST_DRAFTED = 8192
@@ -73,7 +78,8 @@ class BranchOps:
         return self._branches
 
     def _branch_memory(self, name, sizes, key, ws, stream):
-        """Scratch and counters (zero when they are made) of a call; ``sizes`` is the library's function that gives their bytes."""
+        """Addresses of a call's scratch and counters (zero when they are made), and what keeps them; ``sizes`` is the library's function that
+        gives their bytes."""
         known = self._branch_sizes.get((name, key))
         if known is None:
             if len(self._branch_sizes) > 4096:
@@ -84,15 +90,19 @@ class BranchOps:
         nbytes, counter_bytes = known
         if ws is None:
             ws = self.step_ws
-        if ws is None:
-            if _capturing():
-                return (torch.empty(nbytes, dtype=torch.uint8, device=self.device),
-                        torch.zeros(counter_bytes, dtype=torch.uint8, device=self.device))
-            ws = self._branch_scratch.get(stream)
-            if ws is None:
-                from ..engine.batch import Workspace
-                ws = self._branch_scratch[stream] = Workspace(self.device)
-        return ws.get(name, (nbytes,), torch.uint8), ws.get(name + "_counters", (counter_bytes,), torch.uint8, zero=True)
+        if ws is not None:
+            held = ws.get(name, (nbytes,), torch.uint8), ws.get(name + "_counters", (counter_bytes,), torch.uint8, zero=True)
+        elif _capturing():
+            held = torch.empty(nbytes, dtype=torch.uint8, device=self.device), torch.zeros(counter_bytes, dtype=torch.uint8, device=self.device)
+        else:
+            kept = self._branch_scratch.get((name, stream))
+            if kept is None or kept[0] < nbytes or kept[1] < counter_bytes:
+                if kept is not None:
+                    nbytes, counter_bytes = max(nbytes, kept[0]), max(counter_bytes, kept[1])
+                held = torch.empty(nbytes, dtype=torch.uint8, device=self.device), torch.zeros(counter_bytes, dtype=torch.uint8, device=self.device)
+                kept = self._branch_scratch[name, stream] = (nbytes, counter_bytes, held[0].data_ptr(), held[1].data_ptr(), held)
+            return kept[2:]
+        return held[0].data_ptr(), held[1].data_ptr(), held
 
     def branch_error_code(self) -> int:
         """The code of a wait that one of these kernels gave up since the last check, or 0; synchronises and clears."""
@@ -100,7 +110,10 @@ class BranchOps:
             return 0
         L = self._branches
         codes = [L.gb_tree_attention_error_check(), L.gb_beam_select_error_check(), L.gb_branches_error_check()]
-        return next((c for c in codes if c), 0)
+        code = next((c for c in codes if c), 0)
+        if code:                # (counters that a kernel which gave up left behind are not zero)
+            self._branch_scratch.clear()
+        return code
 
     def check_branch_errors(self) -> None:
         """Synchronises, and raises if one of these kernels gave up on a wait since the last check."""
@@ -113,7 +126,7 @@ class BranchOps:
             _need(t.get_device() == self._device_index, "kernel operands must live on the kernel set's CUDA device")
 
     @staticmethod
-    def _check_requests(what, T, cu_q, kv_lens):
+    def _check_requests(what, cu_q, kv_lens):
         for t in (cu_q, kv_lens):
             _need(t.dtype is torch.int32 and t.is_contiguous() and t.dim() == 1, f"{what}: cu_q and kv_lens must be contiguous int32")
         R = kv_lens.shape[0]
@@ -131,7 +144,7 @@ class BranchOps:
         what = "tree_layout"
         self._here(parents, cu_q, kv_lens, positions, mask)
         T = parents.shape[0]
-        R = self._check_requests(what, T, cu_q, kv_lens)
+        R = self._check_requests(what, cu_q, kv_lens)
         for t in (parents, positions):
             _need(t.dtype is torch.int32 and t.is_contiguous() and t.shape == (T,), f"{what}: parents and positions must be contiguous int32 [T]")
         _need(mask.dtype is torch.int32 and mask.is_contiguous() and mask.dim() == 2 and mask.shape[0] == T, f"{what}: mask must be contiguous int32 [T, words]")
@@ -156,56 +169,65 @@ class BranchOps:
 
         On the tensor cores for bfloat16, heads of 64 and 128 and pages of 8 to 128 (a power of two), with weights rounded to bfloat16; other shapes (heads of a
         multiple of 4 channels up to 256) and float32 in 32-bit arithmetic throughout."""
-        what = "tree_attention"
         T, Hq, hd = q.shape
-        pages, Hkv = k_pool.shape[0], k_pool.shape[1]
-        R, dev, width, words = kv_lens.shape[0], self._device_index, block_table.shape[1], mask.shape[1]
+        pool = k_pool.shape
+        pages, Hkv = pool[0], pool[1]
+        table = block_table.shape
+        rows, words = mask.shape
+        R, dev, width = kv_lens.shape[0], self._device_index, table[1]
         dtype, i32 = q.dtype, torch.int32
-        shape = (pages, Hkv, page_size, hd)
         # (one condition, taken apart when it fails)
         if not (q.is_contiguous() and out.is_contiguous() and out.shape == (T, Hq * hd) and dtype is out.dtype and dtype is k_pool.dtype
-                and dtype is v_pool.dtype and dtype in _TAG and k_pool.shape == shape and v_pool.shape == shape and k_pool.is_contiguous()
+                and dtype is v_pool.dtype and dtype in _TAG and pool == (pages, Hkv, page_size, hd) and v_pool.shape == pool and k_pool.is_contiguous()
                 and v_pool.is_contiguous() and Hkv > 0 and Hq % Hkv == 0 and block_table.dtype is i32 and cu_q.dtype is i32 and kv_lens.dtype is i32
                 and positions.dtype is i32 and mask.dtype is i32 and block_table.is_contiguous() and cu_q.is_contiguous() and kv_lens.is_contiguous()
-                and positions.is_contiguous() and mask.is_contiguous() and cu_q.shape == (R + 1,) and kv_lens.dim() == 1 and block_table.shape[0] >= R
-                and positions.shape == (T,) and mask.shape[0] == T and 32 * words >= max_q_len and max_q_len > 0 and scale > 0 and window >= 0
+                and positions.is_contiguous() and mask.is_contiguous() and cu_q.shape == (R + 1,) and kv_lens.dim() == 1 and table[0] >= R
+                and positions.shape == (T,) and rows == T and 32 * words >= max_q_len > 0 and scale > 0 and window >= 0
                 and width * page_size >= max_kv_len and q.get_device() == dev and k_pool.get_device() == dev and v_pool.get_device() == dev
                 and out.get_device() == dev and block_table.get_device() == dev and cu_q.get_device() == dev and kv_lens.get_device() == dev
                 and positions.get_device() == dev and mask.get_device() == dev):
-            self._here(q, k_pool, v_pool, out, block_table, cu_q, kv_lens, positions, mask)
-            _need(q.is_contiguous() and out.is_contiguous() and out.shape == (T, Hq * hd), f"{what}: q/out shape")
-            _need(dtype is out.dtype and dtype is k_pool.dtype and dtype is v_pool.dtype and dtype in _TAG,
-                  f"{what}: one dtype, bfloat16 or float32, for q, cache and out")
-            _need(k_pool.shape == shape and v_pool.shape == shape and k_pool.is_contiguous() and v_pool.is_contiguous(),
-                  f"{what}: pools must be contiguous {list(shape)}")
-            _need(Hkv > 0 and Hq % Hkv == 0, f"{what}: heads in whole groups")
-            self._check_requests(what, T, cu_q, kv_lens)
-            for t in (block_table, positions, mask):
-                _need(t.dtype is i32 and t.is_contiguous(), f"{what}: block table, positions and mask must be contiguous int32")
-            _need(block_table.shape[0] >= R, f"{what}: a row of the block table for every request")
-            _need(positions.shape == (T,) and mask.shape[0] == T, f"{what}: a position and a row of the mask for every token")
-            _need(max_q_len > 0 and 32 * words >= max_q_len, f"{what}: the mask is too narrow for that many tokens")
-            _need(scale > 0 and window >= 0, f"{what}: a positive scale, a window that is not negative")
-            raise KernelError(f"{what}: the block table is too narrow for that many positions")
+            self._refuse_attention(q, k_pool, v_pool, block_table, cu_q, kv_lens, positions, mask, out, scale, window, page_size, max_q_len)
         if T == 0 or R == 0:
             return
         L, g, stream = self.branch_lib, Hq // Hkv, self._stream()
         q_ptr, k_ptr, v_ptr, out_ptr = q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr()
+        low_bits = q_ptr | k_ptr | v_ptr | out_ptr
         if (dtype is torch.bfloat16 and self.tc is not None and (hd == 64 or hd == 128) and page_size in (8, 16, 32, 64, 128) and g <= 128 and pages > 0
-                and not (q_ptr | k_ptr | v_ptr | out_ptr) & 15):
+                and not low_bits & 15):
             # the row of all tiles is counted in 31 bits
-            _need(R * Hkv * (max_q_len * g // 64 + 1) * (max_kv_len // 128 + 2) < 1 << 31, f"{what}: more tiles than fit 31 bits")
-            scratch, counters = self._branch_memory("tree_attention", L.gb_tree_attention_scratch_bytes, (hd,), ws, stream)
-            self._check(L, L.gb_tree_attention_tc(q_ptr, k_ptr, v_ptr, block_table.data_ptr(), width, cu_q.data_ptr(), kv_lens.data_ptr(),
-                                                  positions.data_ptr(), mask.data_ptr(), words, out_ptr, T, R, pages, Hq, Hkv, hd, scale, window,
-                                                  page_size, max_q_len, max_kv_len, counters.data_ptr(), scratch.data_ptr(), stream), what,
-                        (R + 2047) // 2048)
-            return
-        _need(hd % 4 == 0 and hd <= 256, f"{what}: heads of a multiple of 4 channels up to 256")
-        _need(not (q_ptr | k_ptr | v_ptr | out_ptr) & (15 if dtype is torch.float32 else 7), f"{what}: operands on 16 bytes (bfloat16: 8)")
-        self._check(L, L.gb_tree_attention_simple(q_ptr, _TAG[dtype], k_ptr, v_ptr, block_table.data_ptr(), width, cu_q.data_ptr(), kv_lens.data_ptr(),
-                                                  positions.data_ptr(), mask.data_ptr(), words, out_ptr, T, R, pages, Hq, Hkv, hd, scale, window,
-                                                  page_size, max_q_len, max_kv_len, stream), what)
+            if R * Hkv * (max_q_len * g // 64 + 1) * (max_kv_len // 128 + 4) >= 1 << 31:
+                raise KernelError("tree_attention: more tiles than fit 31 bits")
+            scratch, counters, _held = self._branch_memory("tree_attention", L.gb_tree_attention_scratch_bytes, (hd,), ws, stream)
+            entry, launches = L.gb_tree_attention_tc, (R + 2047) // 2048
+        else:
+            _need(hd % 4 == 0 and hd <= 256, "tree_attention: heads of a multiple of 4 channels up to 256")
+            _need(not low_bits & (15 if dtype is torch.float32 else 7), "tree_attention: operands on 16 bytes (bfloat16: 8)")
+            entry, counters, scratch, launches = L.gb_tree_attention_simple, 0, 0, 1
+        self._check(L, entry(_TREE_CALL.pack(
+            q_ptr, k_ptr, v_ptr, out_ptr, block_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), positions.data_ptr(), mask.data_ptr(), counters,
+            scratch, stream, width, words, T, R, pages, Hq, Hkv, hd, window, page_size, max_q_len, max_kv_len, _TAG[dtype], scale)),
+            "tree_attention", launches)
+
+    def _refuse_attention(self, q, k_pool, v_pool, block_table, cu_q, kv_lens, positions, mask, out, scale, window, page_size, max_q_len):
+        what = "tree_attention"
+        T, Hq, hd = q.shape
+        Hkv, R = k_pool.shape[1], kv_lens.shape[0]
+        shape = (k_pool.shape[0], Hkv, page_size, hd)
+        self._here(q, k_pool, v_pool, out, block_table, cu_q, kv_lens, positions, mask)
+        _need(q.is_contiguous() and out.is_contiguous() and out.shape == (T, Hq * hd), f"{what}: q/out shape")
+        _need(q.dtype is out.dtype and q.dtype is k_pool.dtype and q.dtype is v_pool.dtype and q.dtype in _TAG,
+              f"{what}: one dtype, bfloat16 or float32, for q, cache and out")
+        _need(k_pool.shape == shape and v_pool.shape == shape and k_pool.is_contiguous() and v_pool.is_contiguous(),
+              f"{what}: pools must be contiguous {list(shape)}")
+        _need(Hkv > 0 and Hq % Hkv == 0, f"{what}: heads in whole groups")
+        self._check_requests(what, cu_q, kv_lens)
+        for t in (block_table, positions, mask):
+            _need(t.dtype is torch.int32 and t.is_contiguous(), f"{what}: block table, positions and mask must be contiguous int32")
+        _need(block_table.shape[0] >= R, f"{what}: a row of the block table for every request")
+        _need(positions.shape == (T,) and mask.shape[0] == T, f"{what}: a position and a row of the mask for every token")
+        _need(0 < max_q_len <= 32 * mask.shape[1], f"{what}: the mask is too narrow for that many tokens")
+        _need(scale > 0 and window >= 0, f"{what}: a positive scale, a window that is not negative")
+        raise KernelError(f"{what}: the block table is too narrow for that many positions")
 
     def tree_accept(self, tokens, targets, parents, cu_q, kv_lens, path, kept, next_tokens, max_q_len: int, pools=(), block_table=None,
                     page_size: int = 0):
@@ -219,44 +241,54 @@ class BranchOps:
         every call. Rows behind them, and where the block table has no page, are left as they are. The request's length is then its context plus
         ``kept[r]``. (A chosen token may come from any rule, a drawn one too: a token is its parent's target or is not kept.)"""
         what = "tree_accept"
-        T = tokens.shape[0]
-        self._here(tokens, targets, parents, cu_q, kv_lens, path, kept, next_tokens)
-        R = self._check_requests(what, T, cu_q, kv_lens)
-        for t in (tokens, targets, parents):
-            _need(t.dtype is torch.int32 and t.is_contiguous() and t.shape == (T,), f"{what}: tokens, targets and parents must be contiguous int32 [T]")
-        for t in (kept, next_tokens):
-            _need(t.dtype is torch.int32 and t.is_contiguous() and t.shape == (R,), f"{what}: kept and next_tokens must be contiguous int32 [R]")
-        _need(path.dtype is torch.int32 and path.is_contiguous() and path.dim() == 2 and path.shape[0] == R, f"{what}: path must be contiguous int32 [R, width]")
-        _need(0 < max_q_len <= self.MOST_DRAFTED, f"{what}: 1 to {self.MOST_DRAFTED} drafted tokens of a request")
-        _need(path.shape[1] >= max_q_len, f"{what}: a path as wide as the largest tree")
-        _need(R <= 65535, f"{what}: at most 65,535 requests")
-        n, pages, table, width = len(pools), 0, None, 0
-        at, calls, heads, rows = [], [], [], []
-        if n:
-            _need(block_table is not None, f"{what}: pools come with a block table")
-            self._here(block_table, *pools)
-            _need(block_table.dtype is torch.int32 and block_table.is_contiguous() and block_table.dim() == 2 and block_table.shape[0] >= R,
-                  f"{what}: the block table must be contiguous int32, a row for every request")
+        tokens_shape, i32, dev = tokens.shape, torch.int32, self._device_index
+        path_shape, R = path.shape, kv_lens.shape[0]
+        # (one condition, taken apart when it fails)
+        if not (tokens.dtype is i32 and targets.dtype is i32 and parents.dtype is i32 and cu_q.dtype is i32 and kv_lens.dtype is i32 and path.dtype is i32
+                and kept.dtype is i32 and next_tokens.dtype is i32 and tokens.is_contiguous() and targets.is_contiguous() and parents.is_contiguous()
+                and cu_q.is_contiguous() and kv_lens.is_contiguous() and path.is_contiguous() and kept.is_contiguous() and next_tokens.is_contiguous()
+                and len(tokens_shape) == 1 and targets.shape == tokens_shape and parents.shape == tokens_shape and cu_q.shape == (R + 1,)
+                and kept.shape == (R,) and next_tokens.shape == (R,) and kv_lens.dim() == 1 and len(path_shape) == 2 and path_shape[0] == R
+                and 0 < max_q_len <= self.MOST_DRAFTED and path_shape[1] >= max_q_len and R <= 65535 and tokens.get_device() == dev
+                and targets.get_device() == dev and parents.get_device() == dev and cu_q.get_device() == dev and kv_lens.get_device() == dev
+                and path.get_device() == dev and kept.get_device() == dev and next_tokens.get_device() == dev):
+            self._here(tokens, targets, parents, cu_q, kv_lens, path, kept, next_tokens)
+            self._check_requests(what, cu_q, kv_lens)
+            for t in (tokens, targets, parents):
+                _need(t.dtype is i32 and t.is_contiguous() and t.dim() == 1 and t.shape == tokens_shape,
+                      f"{what}: tokens, targets and parents must be contiguous int32 [T]")
+            for t in (kept, next_tokens):
+                _need(t.dtype is i32 and t.is_contiguous() and t.shape == (R,), f"{what}: kept and next_tokens must be contiguous int32 [R]")
+            _need(path.dtype is i32 and path.is_contiguous() and path.dim() == 2 and path_shape[0] == R, f"{what}: path must be contiguous int32 [R, width]")
+            _need(0 < max_q_len <= self.MOST_DRAFTED, f"{what}: 1 to {self.MOST_DRAFTED} drafted tokens of a request")
+            _need(path_shape[1] >= max_q_len, f"{what}: a path as wide as the largest tree")
+            raise KernelError(f"{what}: at most 65,535 requests")
+        pages, table, width, flat = 0, 0, 0, array("q")
+        if pools:
+            if not (block_table is not None and block_table.dtype is i32 and block_table.is_contiguous() and block_table.dim() == 2
+                    and block_table.get_device() == dev and block_table.shape[0] >= R):
+                _need(block_table is not None, f"{what}: pools come with a block table")
+                self._here(block_table)
+                raise KernelError(f"{what}: the block table must be contiguous int32, a row for every request")
             table, width = block_table.data_ptr(), block_table.shape[1]
+            pages = pools[0].shape[-4] if pools[0].dim() >= 4 else 0
             for pool in pools:
-                shape = tuple(pool.shape) if pool.dim() == 5 else (1,) + tuple(pool.shape)
-                _need(len(shape) == 5 and pool.is_contiguous() and shape[3] == page_size and page_size > 0,
-                      f"{what}: pools must be contiguous [calls, pages, heads, page_size, width]")
-                _need(pool.dtype.itemsize in (2, 4), f"{what}: rows of two or four bytes a number (pages in 8 bits have a scale for all their rows)")
-                _need(not at or shape[1] == pages, f"{what}: pools of one block table have the same number of pages")
-                pages = shape[1]
-                if pool.numel():
-                    at.append(pool.data_ptr())
-                    calls.append(shape[0])
-                    heads.append(shape[2])
-                    rows.append(shape[4] * pool.dtype.itemsize)
-            n = len(at)
+                shape, item = pool.shape, pool.dtype.itemsize
+                if not (len(shape) in (4, 5) and pool.is_contiguous() and shape[-2] == page_size > 0 and (item == 2 or item == 4) and shape[-4] == pages
+                        and pool.get_device() == dev):
+                    self._here(pool)
+                    _need(len(shape) in (4, 5) and pool.is_contiguous() and shape[-2] == page_size > 0,
+                          f"{what}: pools must be contiguous [calls, pages, heads, page_size, width]")
+                    _need(item in (2, 4), f"{what}: rows of two or four bytes a number (pages in 8 bits have a scale for all their rows)")
+                    raise KernelError(f"{what}: pools of one block table have the same number of pages")
+                flat.extend((pool.data_ptr(), shape[0] if len(shape) == 5 else 1, shape[-3], shape[-1] * item))
         if R == 0:
             return
-        L, ints = self.branch_lib, c_int * max(n, 1)
-        self._check(L, L.gb_tree_accept(tokens.data_ptr(), targets.data_ptr(), parents.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), path.data_ptr(),
-                                        path.shape[1], kept.data_ptr(), next_tokens.data_ptr(), n, (c_void_p * max(n, 1))(*at), ints(*calls), ints(*heads),
-                                        ints(*rows), pages, table, width, page_size, R, max_q_len, self._stream()), what)
+        L = self.branch_lib
+        self._check(L, L.gb_tree_accept(_ACCEPT_CALL.pack(
+            tokens.data_ptr(), targets.data_ptr(), parents.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), path.data_ptr(), kept.data_ptr(),
+            next_tokens.data_ptr(), table, flat.buffer_info()[0], self._stream(), len(flat) // 4 if pages else 0, pages, path_shape[1], width, page_size, R,
+            max_q_len)), what)
 
     # ------------------------------------------------------------------ beams
     def beam_select(self, logits, scores, best, parents, tokens, ws=None):
@@ -269,10 +301,11 @@ class BranchOps:
         items, beams = scores.shape
         rows, V = logits.shape
         n, dev, f32, i32 = best.shape[1], self._device_index, torch.float32, torch.int32
+        chosen = best.shape
         if not (rows == items * beams and logits.dtype is f32 and (logits.stride(1) == 1 or V == 1) and scores.dtype is f32 and scores.is_contiguous()
                 and best.dtype is f32 and best.is_contiguous() and parents.dtype is i32 and parents.is_contiguous() and tokens.dtype is i32
-                and tokens.is_contiguous() and best.shape == (items, n) and parents.shape == best.shape and tokens.shape == best.shape
-                and 0 < n <= min(self.MOST_BEAMS, beams * V) and beams <= self.MOST_BEAMS and rows <= 65535 and V <= 1 << 30
+                and tokens.is_contiguous() and chosen == (items, n) and parents.shape == chosen and tokens.shape == chosen
+                and 0 < n <= self.MOST_BEAMS and n <= beams * V and beams <= self.MOST_BEAMS and rows <= 65535 and V <= 1 << 30
                 and logits.get_device() == dev and scores.get_device() == dev and best.get_device() == dev and parents.get_device() == dev
                 and tokens.get_device() == dev):
             self._here(logits, scores, best, parents, tokens)
@@ -287,9 +320,10 @@ class BranchOps:
         if rows == 0:
             return
         L, stream = self.branch_lib, self._stream()
-        scratch, counters = self._branch_memory("beam_select", L.gb_beam_select_scratch_bytes, (items, beams, V, n), ws, stream)
-        self._check(L, L.gb_beam_select(logits.data_ptr(), logits.stride(0), scores.data_ptr(), items, beams, V, n, best.data_ptr(), parents.data_ptr(),
-                                        tokens.data_ptr(), counters.data_ptr(), scratch.data_ptr(), stream), what)
+        scratch, counters, _held = self._branch_memory("beam_select", L.gb_beam_select_scratch_bytes, (items, beams, V, n), ws, stream)
+        self._check(L, L.gb_beam_select(_BEAM_CALL.pack(
+            logits.data_ptr(), scores.data_ptr(), best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), counters, scratch, stream,
+            logits.stride(0), items, beams, V, n)), what)
 
     def copy_entries(self, arrays, source, target, dim: int = 0):
         """In every one of ``arrays`` (contiguous, of any type, none of them twice): entry ``source[i]`` along ``dim`` is copied to entry
@@ -297,26 +331,28 @@ class BranchOps:
         states ``[slots, ...]`` with 0. ``source`` and ``target``: int32, up to 1,024. A copy with a source or target that the array does not
         have (-1) is left out; of several to one target the last one counts."""
         what = "copy_entries"
-        self._here(source, target, *arrays)
-        n = source.shape[0]
-        for t in (source, target):
-            _need(t.dtype is torch.int32 and t.is_contiguous() and t.shape == (n,), f"{what}: source and target must be contiguous int32 of one length")
-        _need(n <= self.MOST_COPIES, f"{what}: {n} copies (at most {self.MOST_COPIES})")
-        at, outer, entries, nbytes = [], [], [], []
+        copies, i32, dev = source.shape, torch.int32, self._device_index
+        if not (source.dtype is i32 and target.dtype is i32 and source.is_contiguous() and target.is_contiguous() and len(copies) == 1
+                and target.shape == copies and copies[0] <= self.MOST_COPIES and source.get_device() == dev and target.get_device() == dev):
+            self._here(source, target)
+            for t in (source, target):
+                _need(t.dtype is i32 and t.is_contiguous() and t.dim() == 1 and t.shape == copies,
+                      f"{what}: source and target must be contiguous int32 of one length")
+            raise KernelError(f"{what}: {copies[0]} copies (at most {self.MOST_COPIES})")
+        flat, of_shape, of_dtype = array("q"), None, None
         for a in arrays:
-            _need(a.is_contiguous() and 0 <= dim < a.dim(), f"{what}: arrays must be contiguous and have dimension {dim}")
-            size, count = a.numel() * a.dtype.itemsize, a.shape[dim]
-            if size:
-                above = 1
-                for d in a.shape[:dim]:
-                    above *= d
-                at.append(a.data_ptr())
-                outer.append(above)
-                entries.append(count)
-                nbytes.append(size // (above * count))
-        if n == 0 or not at:
+            shape, dtype = a.shape, a.dtype
+            if not (a.is_contiguous() and a.get_device() == dev):
+                self._here(a)
+                raise KernelError(f"{what}: arrays must be contiguous and have dimension {dim}")
+            if shape != of_shape or dtype is not of_dtype:           # (layers' arrays are alike)
+                _need(0 <= dim < len(shape), f"{what}: arrays must be contiguous and have dimension {dim}")
+                of_shape, of_dtype, entries = shape, dtype, shape[dim]
+                outer, inner = math.prod(shape[:dim]), math.prod(shape[dim + 1:]) * dtype.itemsize
+            if outer and entries and inner:
+                flat.extend((a.data_ptr(), outer, entries, inner))
+        if not flat or copies[0] == 0:
             return
-        k = len(at)
-        L, ints = self.branch_lib, c_int * k
-        self._check(L, L.gb_copy_entries(k, (c_void_p * k)(*at), ints(*outer), ints(*entries), (c_longlong * k)(*nbytes), source.data_ptr(),
-                                         target.data_ptr(), n, self._stream()), what, (k + 95) // 96)
+        L, k = self.branch_lib, len(flat) // 4
+        self._check(L, L.gb_copy_entries(_COPY_CALL.pack(source.data_ptr(), target.data_ptr(), flat.buffer_info()[0], self._stream(), k, copies[0])), what,
+                    (k + 95) // 96)

@@ -1,4 +1,6 @@
 """Decoding along branches, what needs no GPU: what the wrappers refuse and what they hand on."""
+import ctypes
+import struct
 import types
 
 import pytest
@@ -20,7 +22,13 @@ class Recorder(BranchOps):
         self._branch_sizes, self._branch_scratch = {}, {}
 
         def entry(name):
-            return lambda *args: self.calls.append((name, args)) or 0
+            def call(*args):
+                self.calls.append((name, args))
+                if name == "gb_copy_entries":          # (what it points to lives as long as the call)
+                    at, n = struct.unpack("=4Q2q", args[0])[2], struct.unpack("=4Q2q", args[0])[4]
+                    self.arrays = [list((ctypes.c_longlong * 4).from_address(at + 32 * i))[1:] for i in range(n)]
+                return 0
+            return call
 
         self._branches = types.SimpleNamespace(**{n: entry(n) for n in (
             "gb_tree_layout", "gb_tree_accept", "gb_tree_attention_tc", "gb_tree_attention_simple", "gb_beam_select", "gb_copy_entries",
@@ -147,9 +155,9 @@ def test_copies_refuse(change, match):
 def test_copies_hand_on_shapes_and_leave_out_empty_arrays():
     ops = Recorder()
     ops.copy_entries([zeros(3, 7, 2, 4), zeros(3, 0, 2), zeros(2, 5, dtype=torch.uint8)], zeros(2), zeros(2), 1)
-    (name, args), = ops.calls
-    assert name == "gb_copy_entries" and args[0] == 2
-    assert [list(x) for x in args[2:5]] == [[3, 2], [7, 5], [32, 1]]
+    (name, (packed,)), = ops.calls
+    assert name == "gb_copy_entries" and struct.unpack("=4Q2q", packed)[4:] == (2, 2)
+    assert ops.arrays == [[3, 7, 32], [2, 5, 1]]
     ops.copy_entries([zeros(3, 7)], zeros(0), zeros(0))
     ops.copy_entries([], zeros(2), zeros(2))
     assert len(ops.calls) == 1
