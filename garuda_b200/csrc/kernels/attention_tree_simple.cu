@@ -1,25 +1,46 @@
 // Attention of drafted trees over the paged cache in 32-bit arithmetic throughout: the true 32-bit path, and bfloat16 where the kernel on
 // the tensor cores does not apply (head sizes other than 64 and 128, pages of other sizes). The same formula, see attention_tree_tcgen05.cu.
 //
-// Bound by the multiply-adds (32-bit ones run on the ordinary pipes): a block takes 32 query rows, (token, head-of-group) pairs of
-// one key/value head of one request, and walks its keys 32 at a time, so that a number from shared memory is used eight times in each
-// product. Its 128 threads are 16 pairs of rows by 8: a thread has two rows' scores with four keys, and of the sums two rows' every eighth four
-// channels. A row's eight threads are neighbours of one warp: maxima and sums are three shuffles, and the weights need no barrier.
-// Where the blocks of rows are fewer than the device runs at once, a request's keys are shared by the blocks of a thread-block cluster, which join their
-// sums, in the order of the keys, from one another's shared memory. Masked keys are skipped: nothing of them reaches a sum.
+// Bound by the multiply-adds (32-bit ones run on the ordinary pipes) and by what shared memory feeds them, so what counts is how many products a thread makes of
+// what it loads, and that no product waits for the one in front. A block takes up to 64 query rows, (token, head-of-group) pairs of one key/value head of one
+// request, and walks its keys 128 at a time; its 128 threads are 8 by 16: a thread has eight rows' scores with eight keys (16 loads to 256 multiply-adds), then
+// eight rows' sums of eight channels. Between them the scores lie in shared memory, where the softmax walks a row with two lanes. Where the blocks
+// of rows are fewer than the device runs at once, a request's keys are shared by the blocks of a thread-block cluster, which join their sums, in the order of the
+// keys, from one another's shared memory. Masked keys are skipped: nothing of them reaches a sum.
+// Four trees of 12 over up to 1,024 keys of heads of 64: 29 us, a step of 128 keys 12: scores 4 (1.9 clocks a multiply-add of a warp), softmax 4, sums 4.
+// (Two rows by four keys a thread: 33 us, 352 where this takes 182, 64 rows over 8,000 keys of 8 heads of 128. Sixteen rows a warp, a lane a key: 47. Products of
+// pairs, fma.rn.f32x2: 35.)
 #include "branches.h"
 #include "tc_common.cuh"
+
+#include <type_traits>
 
 namespace {
 
 using branches::TreeParams;
 
-constexpr int ROWS = 32, KEYS = 32, THREADS = 128;
-constexpr int P_LD = KEYS + 4;
+constexpr int THREADS = 128, ACROSS = 16;       // threads of a block, and of a row
 constexpr int MOST_PARTS = 8;
 
-__host__ __device__ constexpr int row_floats(int hd) { return hd + 4; }        // (eight rows' 16 bytes on different banks where hd is a multiple of 32)
-__host__ __device__ constexpr int smem_floats(int hd) { return (ROWS + 4 * KEYS) * row_floats(hd) + ROWS * P_LD; }
+// What a head size takes: rows of a block and keys of a step, rows and keys of a thread; in the second product how many threads share a row's keys, and the fours of
+// channels of each (eight rows by eight channels, so that loads and multiply-adds take as long).
+template <int HDMAX, int R>
+struct Shape {
+  static constexpr int ROWS = R * (THREADS / ACROSS), KEYS = HDMAX > 128 ? 64 : 128, K = KEYS / ACROSS, SPLIT = HDMAX > 64 ? 1 : 2, WIDE = ACROSS / SPLIT, FOURS = HDMAX / (4 * WIDE);
+  static constexpr int WARP_ROWS = ROWS / (THREADS / 32), SHARE = 32 / WARP_ROWS;         // a warp's rows, and lanes of a row in the softmax
+  static constexpr int P_LD = ROWS + 4;         // floats of a key's weights
+};
+// floats of a row of channels: an odd number of 16 bytes, so that eight lanes' rows lie on different banks
+__host__ __device__ constexpr int row_floats(int hd) { return hd + (hd / 4 % 2 == 0 ? 4 : 8); }
+// queries; keys, then weights; values
+template <typename S>
+__host__ __device__ constexpr int key_floats(int hd) {
+  return S::KEYS * (row_floats(hd) > S::P_LD ? row_floats(hd) : S::P_LD);
+}
+template <typename S>
+__host__ __device__ constexpr int smem_floats(int hd) {
+  return S::ROWS * row_floats(hd) + key_floats<S>(hd) + S::KEYS * row_floats(hd);
+}
 
 template <typename T>
 __device__ __forceinline__ float4 load4(const T* p);
@@ -42,192 +63,235 @@ __device__ __forceinline__ void copy_async_16(float* to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
 }
 
-template <typename T, int HDMAX>
+template <typename T, int HDMAX, int R>
 __global__ void __launch_bounds__(THREADS)
 attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts) {
-  constexpr int MOST = HDMAX / 32;             // fours of channels that a thread sums
+  using S = Shape<HDMAX, R>;
+  constexpr int ROWS = S::ROWS, KEYS = S::KEYS, K = S::K, FOURS = S::FOURS, WIDE = S::WIDE, P_LD = S::P_LD, WARP_ROWS = S::WARP_ROWS;
   extern __shared__ __align__(16) float smem[];
-  __shared__ long long where[2][KEYS];         // two tiles' keys: their rows' places in the pools, -1: no page
+  __shared__ long long where[KEYS];            // the step's keys: their rows' places in the pools, -1: no page
+  __shared__ float keep_s[ROWS];               // by what a row's sums are multiplied for a new maximum
   const int ld = row_floats(hd), c4 = hd / 4;
   float* const qs = smem;
-  float* const ring = qs + ROWS * ld;          // two tiles: keys, then values
-  float* const ps = ring + 4 * KEYS * ld;
+  float* const ks = qs + ROWS * ld;            // keys, then the weights, a key's rows side by side
+  float* const vs = ks + key_floats<S>(hd);
   gb::pdl_launch_dependents();
   gb::pdl_wait();
   const int r = blockIdx.z, kvh = blockIdx.y % p.Hkv, block = blockIdx.y / p.Hkv, part = blockIdx.x;
   const int q_begin = p.cu_q[r], q_len = p.cu_q[r + 1] - q_begin, row0 = block * ROWS, nrows = min(ROWS, q_len * p.g - row0);
   const int kv_len = p.kv_lens[r], ctx = max(0, kv_len - q_len);
   if (nrows <= 0 || kv_len <= 0) return;       // (the whole cluster's)
-  const int lo = (p.window > 0 ? max(0, ctx + 1 - p.window) : 0) / KEYS, tiles = (kv_len - 1) / KEYS + 1 - lo;
-  const int per = (tiles + parts - 1) / parts, tile_begin = lo + part * per, tile_end = min(lo + tiles, tile_begin + per);
+  const int lo = (p.window > 0 ? max(0, ctx + 1 - p.window) : 0) / KEYS, steps = (kv_len - 1) / KEYS + 1 - lo;
+  const int per = (steps + parts - 1) / parts, begin = lo + part * per, end = min(lo + steps, begin + per);
   const int32_t* table = p.block_table + (size_t)r * p.table_width;
 
-  const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
-  auto place_keys = [&](int tile) {            // by the first warp
-    if (threadIdx.x < KEYS && tile < tile_end) {
-      const int at = tile * KEYS + threadIdx.x, slot = at / p.page_size;
-      const int page = at < kv_len && slot < p.table_width ? table[slot] : -1;
-      where[tile & 1][threadIdx.x] =
-          page >= 0 && page < p.pages ? (((long long)page * p.Hkv + kvh) * p.page_size + at % p.page_size) * hd : -1;
-    }
-  };
-  // A tile's keys and values: 32-bit ones on their way to shared memory while the tile in front is at work, others by way of registers
-  auto fetch = [&](int tile) {
-    float* const ks = ring + (tile & 1) * 2 * KEYS * ld;
-#pragma unroll 4
-    for (int x = threadIdx.x; x < 2 * KEYS * c4; x += THREADS) {
-      const int half = x >= KEYS * c4, y = x - half * KEYS * c4, key = y / c4, c = y % c4;
-      const long long at = where[tile & 1][key];
-      float* const to = ks + (half * KEYS + key) * ld + c * 4;
-      const T* const from = reinterpret_cast<const T*>(half ? p.v_pool : p.k_pool) + at + c * 4;
-      if (at < 0) *reinterpret_cast<float4*>(to) = make_float4(0.f, 0.f, 0.f, 0.f);
-      else if (sizeof(T) == 4) copy_async_16(to, from);
-      else *reinterpret_cast<float4*>(to) = load4(from);
+  const int tx = threadIdx.x % ACROSS, first_row = threadIdx.x / ACROSS * R, channel0 = 4 * (tx % WIDE), split = tx / WIDE;
+  const int lane = threadIdx.x & 31, soft_row = threadIdx.x / 32 * WARP_ROWS + lane % WARP_ROWS, soft_share = lane / WARP_ROWS;      // this lane's row
+  const bool there = soft_row < nrows;
+  const int token = q_begin + (there ? (row0 + soft_row) / p.g : 0), start = p.window > 0 ? p.positions[token] + 1 - p.window : 0;
+  const uint32_t* const bits = p.mask + (size_t)token * p.mask_words;
+  // Rows to shared memory, eight threads a row at a time: 32-bit ones by asynchronous copies, others by way of registers
+  auto fetch = [&](const void* pool, float* to) {
+    for (int x = threadIdx.x / 8; x < KEYS; x += THREADS / 8) {
+      const long long at = where[x];
+      const T* const from = reinterpret_cast<const T*>(pool) + at;
+#pragma unroll 2
+      for (int c = threadIdx.x % 8; c < c4; c += 8) {
+        float* const there = to + x * ld + c * 4;
+        if (at < 0) *reinterpret_cast<float4*>(there) = make_float4(0.f, 0.f, 0.f, 0.f);
+        else if (sizeof(T) == 4) copy_async_16(there, from + c * 4);
+        else *reinterpret_cast<float4*>(there) = load4(from + c * 4);
+      }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   const T* q = reinterpret_cast<const T*>(p.q);
-  place_keys(tile_begin);
-  place_keys(tile_begin + 1);
-  __syncthreads();
-  if (tile_begin < tile_end) fetch(tile_begin);
-  for (int x = threadIdx.x; x < ROWS * c4; x += THREADS) {
-    const int row = x / c4, c = x % c4, at = row0 + row;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (row < nrows) v = load4(q + ((size_t)(q_begin + at / p.g) * p.Hq + kvh * p.g + at % p.g) * hd + c * 4);
-    *reinterpret_cast<float4*>(qs + row * ld + c * 4) = v;
+  for (int x = threadIdx.x / 8; x < ROWS; x += THREADS / 8) {
+    const int at = row0 + x;
+    const T* const from = q + ((size_t)(q_begin + at / p.g) * p.Hq + kvh * p.g + at % p.g) * hd;
+    for (int c = threadIdx.x % 8; c < c4; c += 8)
+      *reinterpret_cast<float4*>(qs + x * ld + c * 4) = x < nrows ? load4(from + c * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  // this thread's two rows
-  int token[2], start[2];
-  bool there[2];
+  float m = -INFINITY, l = 0.f;                // of this lane's row; the denominator: of its share of the keys
+  float4 o[R][FOURS];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row = 2 * ty + i;
-    there[i] = row < nrows;
-    token[i] = q_begin + (there[i] ? (row0 + row) / p.g : 0);
-    start[i] = p.window > 0 ? p.positions[token[i]] + 1 - p.window : 0;
-  }
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  float4 o[2][MOST];
+  for (int i = 0; i < R; ++i)
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int c = 0; c < MOST; ++c) o[i][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = 0; c < FOURS; ++c) o[i][c] = make_float4(0.f, 0.f, 0.f, 0.f);
 
-  for (int tile = tile_begin; tile < tile_end; ++tile) {
-    const int key0 = tile * KEYS;
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();                           // the tile is there, and all are done with the one in front
-    if (tile + 1 < tile_end) fetch(tile + 1);
-    place_keys(tile + 2);
-    const float* const ks = ring + (tile & 1) * 2 * KEYS * ld;
-    const float* const vs = ks + KEYS * ld;
-    // ---- scores of two rows with keys tx, tx + 8, tx + 16, tx + 24
-    float s[2][4] = {};
-#pragma unroll 4
+  for (int step = begin; step < end; ++step) {
+    const int key0 = step * KEYS;
+    __syncthreads();                           // all are done with the step in front
+    if (threadIdx.x < KEYS) {
+      const int at = key0 + threadIdx.x, slot = at / p.page_size;
+      const int page = at < kv_len && slot < p.table_width ? table[slot] : -1;
+      where[threadIdx.x] = page >= 0 && page < p.pages ? (((long long)page * p.Hkv + kvh) * p.page_size + at % p.page_size) * hd : -1;
+    }
+    __syncthreads();
+    fetch(p.k_pool, ks);
+    fetch(p.v_pool, vs);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncthreads();                           // the keys are there
+    // ---- scores of this thread's rows with keys tx, tx + 16, ...
+    float s[R][K];
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int e = 0; e < K; ++e) s[i][e] = 0.f;
+#pragma unroll 1
     for (int c = 0; c < c4; ++c) {
-      float4 a[2], b[4];
+      float4 a[R], b[K];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) a[i] = *reinterpret_cast<const float4*>(qs + (2 * ty + i) * ld + c * 4);
+      for (int i = 0; i < R; ++i) a[i] = *reinterpret_cast<const float4*>(qs + (first_row + i) * ld + c * 4);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) b[e] = *reinterpret_cast<const float4*>(ks + (tx + 8 * e) * ld + c * 4);
+      for (int e = 0; e < K; ++e) b[e] = *reinterpret_cast<const float4*>(ks + (tx + ACROSS * e) * ld + c * 4);
+      // (channel by channel: a sum's next addition is 64 others later)
+      auto add = [&](auto channel) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < R; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[i][e] = fmaf(a[i].x, b[e].x, s[i][e]);
-          s[i][e] = fmaf(a[i].y, b[e].y, s[i][e]);
-          s[i][e] = fmaf(a[i].z, b[e].z, s[i][e]);
-          s[i][e] = fmaf(a[i].w, b[e].w, s[i][e]);
-        }
+          for (int e = 0; e < K; ++e) s[i][e] = fmaf(channel(a[i]), channel(b[e]), s[i][e]);
+      };
+      add([](const float4& v) { return v.x; });
+      add([](const float4& v) { return v.y; });
+      add([](const float4& v) { return v.z; });
+      add([](const float4& v) { return v.w; });
     }
-    // ---- the keys that a row does not read, then the softmax's running maximum and sum
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();                           // all have read the keys, and the values are there
+#pragma unroll
+    for (int e = 0; e < K; ++e)
+#pragma unroll
+      for (int i = 0; i < R; i += 2)
+        *reinterpret_cast<float2*>(ks + (tx + ACROSS * e) * P_LD + first_row + i) = make_float2(s[i][e], s[i + 1][e]);
+    __syncwarp();                              // (a warp's rows are its own)
+    // ---- the softmax, a row to one, two or four lanes, in loops: laid out over a thread's 64 scores it took six times as long, its instructions on their way
     const bool edge = key0 + KEYS > ctx || p.window > 0;
+    float* const mine = ks + soft_row;
+    float top = m;
+    constexpr int BATCH = 8;                   // (all read before one is written: nothing waits for the one in front)
+#pragma unroll 1
+    for (int k0 = soft_share; k0 < KEYS; k0 += BATCH * S::SHARE) {
+      float x[BATCH];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float top = m[i];
+      for (int u = 0; u < BATCH; ++u) x[u] = mine[(k0 + u * S::SHARE) * P_LD] * p.scale;
+      if (edge) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[i][e] *= p.scale;
-        if (edge) {
-          const int key = key0 + tx + 8 * e, j = key - ctx;
-          bool sees = there[i] && key < kv_len;
-          if (j < 0) sees = sees && key >= start[i];
-          else sees = sees && (j >> 5) < p.mask_words && (p.mask[(size_t)token[i] * p.mask_words + (j >> 5)] >> (j & 31) & 1u);
-          if (!sees) s[i][e] = -INFINITY;
-        }
-        top = fmaxf(top, s[i][e]);
-      }
-#pragma unroll
-      for (int d = 1; d < 8; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-      const float keep = weight_of(m[i], top);
-      float sum = 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        // (a masked key's weight is nothing, whatever the maximum is; a score that is no number stays none)
-        const float w = s[i][e] == -INFINITY ? 0.f : expf(s[i][e] - (top == -INFINITY ? 0.f : top));
-        sum += w;
-        ps[(2 * ty + i) * P_LD + tx + 8 * e] = w;
-      }
-      l[i] = l[i] * (m[i] == -INFINITY ? 1.f : keep) + sum;          // this thread's share
-      if (m[i] != -INFINITY && keep != 1.f) {
-#pragma unroll
-        for (int c = 0; c < MOST; ++c) o[i][c].x *= keep, o[i][c].y *= keep, o[i][c].z *= keep, o[i][c].w *= keep;
-      }
-      m[i] = top;
-    }
-    __syncwarp();
-    // ---- sums of two rows' channels 4 tx + 32 c
-#pragma unroll 2
-    for (int key = 0; key < KEYS; key += 4) {
-      const float4 w0 = *reinterpret_cast<const float4*>(ps + 2 * ty * P_LD + key), w1 = *reinterpret_cast<const float4*>(ps + (2 * ty + 1) * P_LD + key);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float u0 = e == 0 ? w0.x : e == 1 ? w0.y : e == 2 ? w0.z : w0.w, u1 = e == 0 ? w1.x : e == 1 ? w1.y : e == 2 ? w1.z : w1.w;
-#pragma unroll
-        for (int c = 0; c < MOST; ++c) {
-          if (4 * tx + 32 * c >= hd) break;
-          const float4 v = *reinterpret_cast<const float4*>(vs + (key + e) * ld + 4 * tx + 32 * c);
-          if (!edge || u0 != 0.f)
-            o[0][c].x = fmaf(u0, v.x, o[0][c].x), o[0][c].y = fmaf(u0, v.y, o[0][c].y), o[0][c].z = fmaf(u0, v.z, o[0][c].z), o[0][c].w = fmaf(u0, v.w, o[0][c].w);
-          if (!edge || u1 != 0.f)
-            o[1][c].x = fmaf(u1, v.x, o[1][c].x), o[1][c].y = fmaf(u1, v.y, o[1][c].y), o[1][c].z = fmaf(u1, v.z, o[1][c].z), o[1][c].w = fmaf(u1, v.w, o[1][c].w);
+        for (int u = 0; u < BATCH; ++u) {
+          const int k = k0 + u * S::SHARE, key = key0 + k, j = key - ctx;
+          bool sees = there && key < kv_len;
+          if (j < 0) sees = sees && key >= start;
+          else sees = sees && (j >> 5) < p.mask_words && (bits[j >> 5] >> (j & 31) & 1u);
+          if (!sees) x[u] = -INFINITY;
         }
       }
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        mine[(k0 + u * S::SHARE) * P_LD] = x[u];
+        top = fmaxf(top, x[u]);
+      }
     }
+#pragma unroll
+    for (int d = WARP_ROWS; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const float keep = m == -INFINITY ? 1.f : weight_of(m, top), less = top == -INFINITY ? 0.f : top;        // (of nothing, or of what is no number and stays none)
+    float sum = 0.f;
+#pragma unroll 1
+    for (int k0 = soft_share; k0 < KEYS; k0 += BATCH * S::SHARE) {
+      float x[BATCH];
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) x[u] = mine[(k0 + u * S::SHARE) * P_LD];
+      // (a masked key's weight is nothing, whatever the maximum is; a score that is no number stays none)
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) x[u] = x[u] == -INFINITY ? 0.f : expf(x[u] - less);
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        sum += x[u];
+        mine[(k0 + u * S::SHARE) * P_LD] = x[u];
+      }
+    }
+    l = l * keep + sum, m = top;
+    if (soft_share == 0) keep_s[soft_row] = keep;
     __syncwarp();
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const float less_now = keep_s[first_row + i];
+      if (less_now != 1.f) {
+#pragma unroll
+        for (int c = 0; c < FOURS; ++c) o[i][c].x *= less_now, o[i][c].y *= less_now, o[i][c].z *= less_now, o[i][c].w *= less_now;
+      }
+    }
+    // ---- sums of this thread's rows' channels, over its share of the keys. Without masked keys a weight of nothing does no harm; else it is left out
+    auto sums = [&](auto masked) {
+      // (the next key's weights and values are on their way while this one's are multiplied: there may be no other warp to fill the wait)
+      float w[2][R];
+      float4 v[2][FOURS];
+      auto load = [&](int key, float (&w)[R], float4 (&v)[FOURS]) {
+#pragma unroll
+        for (int i = 0; i < R; i += 2) {
+          const float2 w2 = *reinterpret_cast<const float2*>(ks + key * P_LD + first_row + i);
+          w[i] = w2.x, w[i + 1] = w2.y;
+        }
+#pragma unroll
+        for (int c = 0; c < FOURS; ++c)
+          v[c] = channel0 + 4 * WIDE * c < hd ? *reinterpret_cast<const float4*>(vs + key * ld + channel0 + 4 * WIDE * c) : make_float4(0.f, 0.f, 0.f, 0.f);
+      };
+      auto add = [&](const float (&w)[R], const float4 (&v)[FOURS]) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          if (decltype(masked)::value && w[i] == 0.f) continue;
+#pragma unroll
+          for (int c = 0; c < FOURS; ++c) {
+            o[i][c].x = fmaf(w[i], v[c].x, o[i][c].x), o[i][c].y = fmaf(w[i], v[c].y, o[i][c].y);
+            o[i][c].z = fmaf(w[i], v[c].z, o[i][c].z), o[i][c].w = fmaf(w[i], v[c].w, o[i][c].w);
+          }
+        }
+      };
+      // an even number of keys a thread, those behind the last masked or (without masks) there; their rows are in shared memory in any case
+      load(split, w[0], v[0]);
+#pragma unroll 1
+      for (int key = split; key < KEYS; key += 2 * S::SPLIT) {
+        load(key + S::SPLIT, w[1], v[1]);
+        add(w[0], v[0]);
+        if (key + 2 * S::SPLIT < KEYS) load(key + 2 * S::SPLIT, w[0], v[0]);
+        add(w[1], v[1]);
+      }
+    };
+    if (edge) sums(std::true_type{});
+    else sums(std::false_type{});
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int d = WARP_ROWS; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+  // ---- every row's sums, maximum and denominator where the queries were; then the cluster's blocks join their shares of the rows
+  __syncthreads();
 #pragma unroll
-    for (int d = 1; d < 8; d <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], d);
+  for (int i = 0; i < R; ++i) {
+    float* const to = qs + (first_row + i) * ld;
+#pragma unroll
+    for (int c = 0; c < FOURS; ++c) {
+      if (S::SPLIT == 2) {
+        o[i][c].x += __shfl_xor_sync(0xffffffffu, o[i][c].x, WIDE), o[i][c].y += __shfl_xor_sync(0xffffffffu, o[i][c].y, WIDE);
+        o[i][c].z += __shfl_xor_sync(0xffffffffu, o[i][c].z, WIDE), o[i][c].w += __shfl_xor_sync(0xffffffffu, o[i][c].w, WIDE);
+      }
+      if (split == 0 && channel0 + 4 * WIDE * c < hd) *reinterpret_cast<float4*>(to + channel0 + 4 * WIDE * c) = o[i][c];
+    }
+  }
+  if (soft_share == 0) *reinterpret_cast<float2*>(qs + soft_row * ld + hd) = make_float2(m, l);
   T* const out = reinterpret_cast<T*>(p.out);
   auto place = [&](int row) { return out + ((size_t)(q_begin + (row0 + row) / p.g) * p.Hq + kvh * p.g + (row0 + row) % p.g) * hd; };
   if (parts == 1) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float inv = l[i] == 0.f ? 0.f : 1.0f / l[i];
-#pragma unroll
-      for (int c = 0; c < MOST; ++c)
-        if (there[i] && 4 * tx + 32 * c < hd)
-          store4(place(2 * ty + i) + 4 * tx + 32 * c, make_float4(o[i][c].x * inv, o[i][c].y * inv, o[i][c].z * inv, o[i][c].w * inv));
+    __syncthreads();
+    for (int x = threadIdx.x; x < nrows * c4; x += THREADS) {
+      const int row = x / c4, c = x % c4;
+      const float den = qs[row * ld + hd + 1], inv = den == 0.f ? 0.f : 1.0f / den;
+      const float4 v = *reinterpret_cast<const float4*>(qs + row * ld + c * 4);
+      store4(place(row) + c * 4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
     }
     return;
-  }
-  // ---- the cluster's parts: every row's sums, maximum and denominator where the tiles were, then each block joins its share of the rows
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    float* to = ring + (2 * ty + i) * ld;
-#pragma unroll
-    for (int c = 0; c < MOST; ++c)
-      if (4 * tx + 32 * c < hd) *reinterpret_cast<float4*>(to + 4 * tx + 32 * c) = o[i][c];
-    if (tx == 0) to[hd] = m[i], to[hd + 1] = l[i];
   }
   tc::cluster_arrive_wait();
   for (int x = part * THREADS + threadIdx.x; x < nrows * c4; x += parts * THREADS) {
     const int row = x / c4, c = x % c4;
-    const uint32_t v_at = tc::smem_u32(ring + row * ld + c * 4), ml_at = tc::smem_u32(ring + row * ld + hd);
+    const uint32_t v_at = tc::smem_u32(qs + row * ld + c * 4), ml_at = tc::smem_u32(qs + row * ld + hd);
     float2 ml[MOST_PARTS];
     float4 v[MOST_PARTS];
 #pragma unroll
@@ -251,39 +315,52 @@ attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts) 
   tc::cluster_arrive_wait();                   // nobody leaves while another reads
 }
 
-// Parts of a request's keys, a power of two: as many as fill the device four times over, each of two tiles at least.
-int parts_of(long long units, int max_kv_len) {
-  const int tiles = (max_kv_len + KEYS - 1) / KEYS;
+// Parts of a request's keys, a power of two: as long as all blocks run at once (of clusters of eight blocks with an SM each, 15), and of a step at least.
+int parts_of(long long units, int steps, int at_once) {
   int parts = 1;
-  while (parts < MOST_PARTS && 2 * parts * units <= 4ll * gb::sm_count() && 4 * parts <= tiles) parts *= 2;
+  while (parts < MOST_PARTS && 2 * parts * units <= at_once && 2 * parts <= steps) parts *= 2;
   return parts;
 }
 
-template <typename T, int HDMAX>
-int launch(const TreeParams& p, int hd, int blocks, int parts, cudaStream_t stream) {
+template <typename T, int HDMAX, int R>
+int launch(const TreeParams& p, int hd, int max_q_len, int max_kv_len, cudaStream_t stream) {
+  using S = Shape<HDMAX, R>;
+  const long long blocks = ((long long)max_q_len * p.g + S::ROWS - 1) / S::ROWS;
+  if (p.R > 65535 || blocks * p.Hkv > 65535) return gb::fail(GB_UNSUPPORTED, "tree_attention: %d requests, %lld blocks of rows", p.R, blocks * p.Hkv);
   static gb::OncePerDevice configured;
   if (configured.needed()) {
-    const cudaError_t e = cudaFuncSetAttribute(attention_tree_simple_kernel<T, HDMAX>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               4 * smem_floats(HDMAX));
+    const cudaError_t e = cudaFuncSetAttribute(attention_tree_simple_kernel<T, HDMAX, R>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               4 * smem_floats<S>(HDMAX));
     if (e != cudaSuccess) return gb::fail(GB_CUDA_ERROR, "tree_attention: %s", cudaGetErrorString(e));
     configured.done();
   }
-  return gb::check_pdl_launch(gb::launch_pdl(attention_tree_simple_kernel<T, HDMAX>, dim3(parts, blocks * p.Hkv, p.R), dim3(THREADS),
-                                             4 * smem_floats(hd), stream, dim3(parts), p, hd, parts), "tree_attention");
+  const int parts = parts_of(p.R * blocks * p.Hkv, (max_kv_len + S::KEYS - 1) / S::KEYS, HDMAX <= 64 ? 2 * gb::sm_count() : 3 * gb::sm_count() / 4);
+  return gb::check_pdl_launch(gb::launch_pdl(attention_tree_simple_kernel<T, HDMAX, R>, dim3(parts, (unsigned)(blocks * p.Hkv), p.R), dim3(THREADS),
+                                             4 * smem_floats<S>(hd), stream, dim3(parts), p, hd, parts), "tree_attention");
+}
+
+// Blocks of 64 rows (heads of more than 128 channels: 32); of 32 or 16 where no request has more (5 tokens, no shared heads, 500 keys of heads of 128: 53 us with
+// 64, 30 with 16), or where the device would be half empty with as many blocks as can share a request's keys (32 rows, 4 heads of 64, 3,000 keys: 35 us with 32,
+// 28 with 16).
+template <typename T, int HDMAX>
+int by_rows(const TreeParams& p, int hd, int max_q_len, int max_kv_len, cudaStream_t stream) {
+  const long long rows = (long long)max_q_len * p.g, steps = (max_kv_len + 127) / 128, parts = steps < MOST_PARTS ? steps : MOST_PARTS;
+  int most = HDMAX > 128 ? 32 : 64;
+  while (most > 16 && (rows <= most / 2 || 8 * ((rows + most - 1) / most) * p.R * p.Hkv * parts <= 3 * gb::sm_count())) most /= 2;
+  if (most == 16) return launch<T, HDMAX, 2>(p, hd, max_q_len, max_kv_len, stream);
+  if (most == 32) return launch<T, HDMAX, 4>(p, hd, max_q_len, max_kv_len, stream);
+  return launch<T, HDMAX, (HDMAX > 128 ? 4 : 8)>(p, hd, max_q_len, max_kv_len, stream);
 }
 
 }  // namespace
 
 GB_EXPORT int gb_tree_attention_simple(const branches::TreeCall* call) {
   const TreeParams p = call->params();
-  const int R = p.R, Hkv = p.Hkv, head_dim = (int)call->head_dim;
-  const long long blocks = (call->max_q_len * p.g + ROWS - 1) / ROWS;
+  const int head_dim = (int)call->head_dim, max_q_len = (int)call->max_q_len, max_kv_len = (int)call->max_kv_len;
   if (head_dim % 4 != 0 || head_dim > 256) return gb::fail(GB_UNSUPPORTED, "tree_attention: heads of %d channels", head_dim);
-  if (R > 65535 || blocks * Hkv > 65535) return gb::fail(GB_UNSUPPORTED, "tree_attention: %d requests, %lld blocks of rows", R, blocks * Hkv);
-  const int parts = parts_of(R * blocks * Hkv, (int)call->max_kv_len);
   return GB_DISPATCH_DTYPE(call->dtype, E, [&]() -> int {
-    if (head_dim <= 64) return launch<E, 64>(p, head_dim, (int)blocks, parts, (cudaStream_t)call->stream);
-    if (head_dim <= 128) return launch<E, 128>(p, head_dim, (int)blocks, parts, (cudaStream_t)call->stream);
-    return launch<E, 256>(p, head_dim, (int)blocks, parts, (cudaStream_t)call->stream);
+    if (head_dim <= 64) return by_rows<E, 64>(p, head_dim, max_q_len, max_kv_len, (cudaStream_t)call->stream);
+    if (head_dim <= 128) return by_rows<E, 128>(p, head_dim, max_q_len, max_kv_len, (cudaStream_t)call->stream);
+    return by_rows<E, 256>(p, head_dim, max_q_len, max_kv_len, (cudaStream_t)call->stream);
   });
 }
