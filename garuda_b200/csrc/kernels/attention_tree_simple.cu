@@ -315,10 +315,12 @@ attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts) 
   tc::cluster_arrive_wait();                   // nobody leaves while another reads
 }
 
-// Parts of a request's keys, a power of two: as long as all blocks run at once (of clusters of eight blocks with an SM each, 15), and of a step at least.
-int parts_of(long long units, int steps, int at_once) {
+// Parts of a request's keys, a power of two: as long as all clusters run at once, and of a step at least. Of 148 SMs 74 clusters of two blocks, 33 of four, 15
+// of eight run at once; with two blocks an SM twice as many (and two more of eight, which wait a little: 29 us, parts of twice as many keys 46).
+int parts_of(long long units, int steps, int per_sm) {
+  const int sms = gb::sm_count(), at_once[3] = {per_sm * sms / 2, per_sm * sms * 2 / 9, per_sm > 1 ? sms * 2 / 9 : sms / 10};
   int parts = 1;
-  while (parts < MOST_PARTS && 2 * parts * units <= at_once && 2 * parts <= steps) parts *= 2;
+  for (int i = 0; i < 3 && units <= at_once[i] && 2 * parts <= steps; ++i) parts *= 2;
   return parts;
 }
 
@@ -334,7 +336,7 @@ int launch(const TreeParams& p, int hd, int max_q_len, int max_kv_len, cudaStrea
     if (e != cudaSuccess) return gb::fail(GB_CUDA_ERROR, "tree_attention: %s", cudaGetErrorString(e));
     configured.done();
   }
-  const int parts = parts_of(p.R * blocks * p.Hkv, (max_kv_len + S::KEYS - 1) / S::KEYS, HDMAX <= 64 ? 2 * gb::sm_count() : 3 * gb::sm_count() / 4);
+  const int parts = parts_of(p.R * blocks * p.Hkv, (max_kv_len + S::KEYS - 1) / S::KEYS, HDMAX <= 64 ? 2 : 1);
   return gb::check_pdl_launch(gb::launch_pdl(attention_tree_simple_kernel<T, HDMAX, R>, dim3(parts, (unsigned)(blocks * p.Hkv), p.R), dim3(THREADS),
                                              4 * smem_floats<S>(hd), stream, dim3(parts), p, hd, parts), "tree_attention");
 }
