@@ -105,6 +105,33 @@ class PagedCache:
     def release(self, request: int) -> None:
         self.manager.release(request)
 
+    def fork(self, pairs: Sequence[tuple], ops) -> None:
+        """For every ``(parent, child)``: ``child`` becomes a request that goes on where ``parent`` is. It holds the parent's full pages together
+        with it, and gets a copy of its last page, where that is not full, and of its fixed-size states, in every layer call (on the
+        current stream, behind what the parent's last step wrote). All or nothing; a child is nobody's parent in the same call."""
+        if {p for p, _ in pairs} & {c for _, c in pairs}:
+            raise ValueError("a request that is forked in this call cannot be forked in it again")
+        done, copies = [], []
+        try:
+            for parent, child in pairs:
+                copies += self.manager.fork(parent, child)
+                done.append(child)
+        except self.host_module.CacheError:
+            for child in done:
+                self.manager.release(child)
+            raise
+
+        def copy(arrays, moves, dim):
+            for i in range(0, len(moves), ops.MOST_COPIES):          # (targets are new: no copy's source is another's target)
+                both = torch.tensor(moves[i:i + ops.MOST_COPIES], dtype=torch.int32).t().contiguous().to(self.device)
+                ops.copy_entries(arrays, both[0], both[1], dim)
+
+        for g in range(len(self.groups)):
+            arrays = [self.k_pools[g], self.v_pools[g]] + ([self.k_scales[g], self.v_scales[g]] if self.float8 else [])
+            copy([a for a in arrays if a is not None], [(a, b) for group, a, b in copies if group == g], 1)
+        if self.states:
+            copy(list(self.states.values()), [(self.manager.slot(a), self.manager.slot(b)) for a, b in pairs], 0)
+
     def bytes_per_position(self) -> int:
         if self.float8:         # and a page's two scales a head
             return sum(len(g.calls) * (g.need.kv_heads * (g.need.head_dim + (g.need.value_dim or g.need.head_dim))

@@ -76,6 +76,12 @@ PYBIND11_MODULE(_garuda_host, m) {
       .def("reserve", &CacheManager::reserve)
       .def("commit", &CacheManager::commit)
       .def("release", &CacheManager::release)
+      .def("fork",
+           [](CacheManager& c, int64_t parent, int64_t child) {
+             std::vector<std::tuple<int, int, int>> out;
+             for (const auto& copy : c.fork(parent, child)) out.emplace_back(copy.group, copy.from, copy.to);
+             return out;
+           })
       .def("known", &CacheManager::known)
       .def("length", &CacheManager::length)
       .def("slot", &CacheManager::slot)

@@ -26,6 +26,7 @@ CacheManager::CacheManager(std::vector<GroupConfig> groups, int page_size, int m
     // Highest id at the bottom, so that page 0 is handed out first.
     for (int p = g.num_pages - 1; p >= 0; --p) pool.free.push_back(p);
     pool.used_before.assign(g.num_pages, 0);
+    pool.holders.assign(g.num_pages, 0);
     pools_.push_back(std::move(pool));
   }
   for (int s = max_requests_ - 1; s >= 0; --s) free_slots_.push_back(s);
@@ -104,15 +105,9 @@ void CacheManager::reserve(int64_t request, int new_len) {
   }
   const int last = (new_len + page_size_ - 1) / page_size_;
   for (size_t g = 0; g < groups_.size(); ++g) {
-    Pool& pool = pools_[g];
     for (int p = first_live_page(static_cast<int>(g), r.len); p < last; ++p) {
       if (r.tables[g][p] >= 0) continue;
-      const int32_t page = pool.free.back();
-      pool.free.pop_back();
-      r.tables[g][p] = page;
-      ++pages_handed_out_;
-      if (pool.used_before[page]) ++pages_reused_;
-      pool.used_before[page] = 1;
+      r.tables[g][p] = new_page(static_cast<int>(g));
     }
   }
   r.reserved = std::max(r.reserved, new_len);
@@ -130,7 +125,7 @@ void CacheManager::commit(int64_t request, int new_len) {
     const int first = first_live_page(static_cast<int>(g), r.len);
     for (int p = kept_pages(static_cast<int>(g)); p < first && p < max_pages_; ++p) {
       if (r.tables[g][p] >= 0) {
-        pools_[g].free.push_back(r.tables[g][p]);
+        pools_[g].give_back(r.tables[g][p]);
         r.tables[g][p] = -1;
       }
     }
@@ -141,9 +136,57 @@ void CacheManager::release(int64_t request) {
   Request& r = get(request);
   for (size_t g = 0; g < groups_.size(); ++g)
     for (int p = 0; p < max_pages_; ++p)
-      if (r.tables[g][p] >= 0) pools_[g].free.push_back(r.tables[g][p]);
+      if (r.tables[g][p] >= 0) pools_[g].give_back(r.tables[g][p]);
   free_slots_.push_back(r.slot);
   requests_.erase(request);
+}
+
+int32_t CacheManager::new_page(int group) {
+  Pool& pool = pools_[group];
+  const int32_t page = pool.free.back();
+  pool.free.pop_back();
+  pool.holders[page] = 1;
+  ++pages_handed_out_;
+  if (pool.used_before[page]) ++pages_reused_;
+  pool.used_before[page] = 1;
+  return page;
+}
+
+void CacheManager::Pool::give_back(int32_t page) {
+  if (--holders[page] == 0) free.push_back(page);
+}
+
+std::vector<CacheManager::Copy> CacheManager::fork(int64_t parent, int64_t child) {
+  const Request& from = get(parent);
+  if (requests_.count(child)) throw CacheError("request " + std::to_string(child) + " already holds a slot");
+  if (free_slots_.empty()) throw CacheError("no request slot is free");
+  // The page that holds the next position, where it is not that page's first and the request's groups still read it
+  const int open = from.len % page_size_ != 0 ? from.len / page_size_ : -1;
+  for (size_t g = 0; g < groups_.size(); ++g)
+    if (open >= 0 && from.tables[g][open] >= 0 && pools_[g].free.empty())
+      throw OutOfPages("request " + std::to_string(child) + " needs a page of group " + std::to_string(g) + " to go on from request " +
+                       std::to_string(parent) + ", but none is free");
+  Request r;
+  r.slot = free_slots_.back();
+  free_slots_.pop_back();
+  r.len = from.len;
+  r.reserved = from.len;
+  r.tables.assign(groups_.size(), std::vector<int32_t>(max_pages_, -1));
+  std::vector<Copy> copies;
+  const int full = from.len / page_size_;
+  for (size_t g = 0; g < groups_.size(); ++g) {
+    for (int p = 0; p < full; ++p) {
+      if (from.tables[g][p] < 0) continue;
+      r.tables[g][p] = from.tables[g][p];
+      ++pools_[g].holders[from.tables[g][p]];
+    }
+    if (open >= 0 && from.tables[g][open] >= 0) {
+      r.tables[g][open] = new_page(static_cast<int>(g));
+      copies.push_back(Copy{static_cast<int>(g), from.tables[g][open], r.tables[g][open]});
+    }
+  }
+  requests_.emplace(child, std::move(r));
+  return copies;
 }
 
 void CacheManager::block_table_row(int64_t request, int group, int32_t* out, int width) const {
@@ -161,19 +204,24 @@ void CacheManager::check_invariants() const {
         throw CacheError("group " + std::to_string(g) + ": free list holds page id out of range");
       if (seen[p]++) throw CacheError("group " + std::to_string(g) + ": page " + std::to_string(p) + " is free twice");
     }
+    std::vector<int32_t> holders(groups_[g].num_pages, 0);
     for (const auto& kv : requests_) {
       for (int32_t p : kv.second.tables[g]) {
         if (p < 0) continue;
         if (p >= groups_[g].num_pages)
           throw CacheError("group " + std::to_string(g) + ": a table holds page id out of range");
-        if (seen[p]++)
-          throw CacheError("group " + std::to_string(g) + ": page " + std::to_string(p) +
-                           " is held twice (or held and free)");
+        if (seen[p])
+          throw CacheError("group " + std::to_string(g) + ": page " + std::to_string(p) + " is held and free");
+        ++holders[p];
       }
     }
-    for (int p = 0; p < groups_[g].num_pages; ++p)
-      if (seen[p] != 1)
+    for (int p = 0; p < groups_[g].num_pages; ++p) {
+      if (holders[p] != pools_[g].holders[p])
+        throw CacheError("group " + std::to_string(g) + ": page " + std::to_string(p) + " is held " + std::to_string(holders[p]) +
+                         " times, but " + std::to_string(pools_[g].holders[p]) + " are counted");
+      if (seen[p] == 0 && holders[p] == 0)
         throw CacheError("group " + std::to_string(g) + ": page " + std::to_string(p) + " is lost");
+    }
   }
   std::vector<int> slot_seen(max_requests_, 0);
   for (int s : free_slots_) {

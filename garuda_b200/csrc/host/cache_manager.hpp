@@ -58,8 +58,20 @@ class CacheManager {
   // later query's window has passed go back to their pool.
   void commit(int64_t request, int new_len);
   // Everything the request holds goes back: pages (most recently used first,
-  // so that they are handed out again at once) and the slot.
+  // so that they are handed out again at once) and the slot. A page that other
+  // requests hold as well stays theirs.
   void release(int64_t request);
+  // A new request that goes on where another one is: it takes a slot and holds the
+  // other's full pages together with it. What its next position would be written into,
+  // a page that is not full, it gets of its own, to be filled with a copy of the other's:
+  // (group, the other's page, its page) for each. (Positions are only ever written behind
+  // a request's length, so that a page which two requests hold is never written again.)
+  // All or nothing: throws if an id is known or not, no slot is free, or (OutOfPages) no page.
+  struct Copy {
+    int group;
+    int32_t from, to;
+  };
+  std::vector<Copy> fork(int64_t parent, int64_t child);
 
   // ---- queries -------------------------------------------------------------
   bool known(int64_t request) const { return requests_.count(request) != 0; }
@@ -81,7 +93,7 @@ class CacheManager {
   // First position that a query at position `len` (the next token) still reads.
   int first_live_position(int group, int len) const;
   // Throws CacheError naming the first violated invariant: every page is either
-  // free or held by exactly one (request, group, index); no page is free twice.
+  // free or held, by one (request, group, index) or by as many as have forked; no page is free twice.
   void check_invariants() const;
   uint64_t pages_handed_out() const { return pages_handed_out_; }
   uint64_t pages_reused() const { return pages_reused_; }
@@ -97,7 +109,10 @@ class CacheManager {
   struct Pool {
     std::vector<int32_t> free;        // stack: back() is handed out next
     std::vector<uint8_t> used_before; // page id -> has been handed out at least once
+    std::vector<int32_t> holders;     // page id -> requests that hold it (0: it is free)
+    void give_back(int32_t page);     // by one holder
   };
+  int32_t new_page(int group);        // the next free one; there is one
 
   const Request& get(int64_t request) const;
   Request& get(int64_t request);

@@ -137,6 +137,8 @@ class Engine:
         else:
             eos = tuple(int(t) for t in eos_token_id)
         sc.eos_token_ids = list(eos)
+        self.eos_ids = frozenset() if ignore_eos else frozenset(eos)
+        self.prefill_chunk = int(prefill_chunk)
         sc.ignore_eos = bool(ignore_eos)
         sc.paced_prefill = bool(paced_prefill)
         self.paced_prefill = bool(paced_prefill)
@@ -187,7 +189,10 @@ class Engine:
         results. ``generate`` and ``replay`` do."""
         failed = getattr(self.ops, "failed_wait", None)
         if failed is not None and failed():
-            self.ops.tc.check_errors()       # synchronises, clears, raises with the code's meaning
+            if self.ops.tc is not None:
+                self.ops.tc.check_errors()       # synchronises, clears, raises with the code's meaning
+            else:
+                self.ops.check_branch_errors()
 
     def replay(self, trace, out_dir: str, report=None) -> int:
         """Trace replay through this engine's step function: ``trace`` is a path of a file of
@@ -259,6 +264,16 @@ class Engine:
         if len(priorities) != len(prompts):
             raise ConfigError(f"{len(priorities)} priorities for {len(prompts)} prompts")
         return self._events(prompts, sampling, float(timeout or 0.0), priorities)
+
+    def beam_search(self, prompts: Sequence[Sequence[int]], beams: int = 4, max_tokens: int = 64, length_penalty: float = 1.0):
+        """The ``beams`` best continuations of every prompt: a list of ``Hypothesis`` (``tokens``, ``score``, ``finish_reason``) for each, best first by
+        ``score / length ** length_penalty``, where the score is the sum of the tokens' log-probabilities and the length counts an end token. Each step
+        chooses the best of all beams' continuations (``beam_select``); those among the first ``beams`` that end the text are set aside, and the search
+        is over when ``beams`` have been and no other can overtake them, at ``max_tokens`` tokens, or where the context is full. Beams are
+        requests that share pages (``PagedCache.fork``): ``beams`` of the engine's slots for every prompt that runs, and pages for their
+        continuations; where pages run out, ``OutOfPages``. Not for while a ``stream`` of this engine is being read."""
+        from .beams import beam_search
+        return beam_search(self, prompts, int(beams), int(max_tokens), float(length_penalty))
 
     def _events(self, prompts, sampling, timeout: float, priorities):
         index_of: Dict[int, int] = {}

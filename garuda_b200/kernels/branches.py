@@ -1,10 +1,10 @@
 """Decoding along several branches: the checking wrappers of its kernels.
 
 A step may bring a *tree* of drafted tokens per request instead of a stretch: token 0 is the request's last one, which the cache does not hold
-yet, and ``parents`` names for every other the token of the same request that it continues. The tokens' keys and values are in the cache,
-behind the request's context in the order of the tokens' numbers (``rope_kv_append`` with those places as positions and the rotation's table
-made from ``tree_layout``'s). A step with trees goes: ``tree_layout`` once, ``tree_attention`` in every layer, and behind the logits
-``tree_accept``, which keeps the tokens that the model would have chosen itself and moves what they left in the cache together.
+yet, and ``parents`` names for every other the token of the same request that it continues. A step with trees goes: ``tree_layout`` once; in every
+layer the projections' queries and keys are turned by its positions (``CudaOps.rope_inplace``), keys and values go behind the request's context in the
+order of the tokens' numbers (``rope_kv_append`` with those places and no rotation of its own), and ``tree_attention`` reads them; behind the logits
+``tree_accept`` keeps the tokens that the model would have chosen itself and moves what they left in the cache together.
 
 *Beams* are requests of their own over shared pages: ``beam_select`` chooses how they go on, ``copy_entries`` gives a beam that goes on in several
 ways a copy of its last page and of its states (``PagedCache.fork`` says which).

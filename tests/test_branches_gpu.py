@@ -386,6 +386,85 @@ def test_a_tree_that_is_kept_is_the_context_of_the_next_step(ops):
                 assert torch.equal(a[0, table[r, at // page], :, at % page], b[0, table[r, at // page], :, at % page])
 
 
+@pytest.mark.parametrize("dtype, hd, window", [(torch.bfloat16, 64, 0), (torch.float32, 16, 0), (torch.bfloat16, 128, 6)])
+def test_a_layer_of_a_tree_step(ops, dtype, hd, window):
+    """A step's projections, rotated by the tree's positions and written to their places, are read as the same tokens one behind the other are."""
+    from garuda_b200.parts.rotary import RotaryParams
+    rotary = RotaryParams(10000.0, hd, False)
+    g = torch.Generator(device="cuda").manual_seed(hd)
+    heads, kv_heads, page, ctx, parents = 4, 2, 8, 13, [-1, 0, 0, 2, 1, 3]
+    before, now = (torch.randn(n, (heads + 2 * kv_heads) * hd, generator=g, device="cuda") for n in (ctx, 6))
+    pools = [torch.zeros(4, kv_heads, page, hd, dtype=dtype, device="cuda") for _ in range(2)]
+    table, zero, scale = ints([[2, 0, 3]]), ints([0] * 13), hd ** -0.5
+    ops.rope_kv_append(before, torch.empty(ctx, heads, hd, dtype=dtype, device="cuda"), *pools, ints(list(range(ctx))), zero, table, heads, kv_heads, hd, rotary, page)
+    kept = [p.clone() for p in pools]
+    positions, mask = ints([0] * 6), ints([[0]] * 6)
+    ops.tree_layout(ints(parents), ints([0, 6]), ints([ctx + 6]), positions, mask, 6, window)
+    assert positions.tolist() == [13, 14, 14, 15, 15, 16]
+    turned, q = now.clone(), torch.empty(6, heads, hd, dtype=dtype, device="cuda")
+    ops.rope_inplace(turned[:, :(heads + kv_heads) * hd].view(6, heads + kv_heads, hd), positions, rotary)
+    ops.rope_kv_append(turned, q, *pools, ints([ctx + i for i in range(6)]), zero[:6], table, heads, kv_heads, hd, None, page)
+    out = torch.empty(6, heads * hd, dtype=dtype, device="cuda")
+    ops.tree_attention(q, *pools, table, ints([0, 6]), ints([ctx + 6]), positions, mask, out, scale, window, page, 6, ctx + 6)
+    for branch in ([0, 1, 4], [0, 2, 3, 5]):
+        n = len(branch)
+        straight, at = [p.clone() for p in kept], ints(list(range(ctx, ctx + n)))
+        q2, again = torch.empty(n, heads, hd, dtype=dtype, device="cuda"), torch.empty(n, heads * hd, dtype=dtype, device="cuda")
+        ops.rope_kv_append(now[branch].contiguous(), q2, *straight, at, zero[:n], table, heads, kv_heads, hd, rotary, page)
+        ops.paged_attention(q2, *straight, table, ints([0, n]), ints([ctx + n]), zero[:n], again, scale, window, page, 1, n, ctx + n)
+        # (weights are rounded to bfloat16 on both sides)
+        tol = 4 * U16 if dtype is torch.bfloat16 else 64 * U32
+        torch.testing.assert_close(out[branch].float(), again.float(), rtol=tol, atol=tol)
+
+
+@pytest.mark.parametrize("name, dtype, graphs", [("A", "float32", True), ("B", "float32", False), ("D", "bfloat16", True)])
+def test_beam_search(name, dtype, graphs):
+    """The engine's search against the plain one, which runs every beam's whole sequence anew; in bfloat16 by the scores that the plain model gives
+    the tokens."""
+    from garuda_b200 import Engine
+    from tests.helpers import TINY, TOL, folder_weights, model_dir, random_tokens
+    from tests.plain import llama_plain
+    from tests.test_beams import plain_search
+    cfg, folder = TINY[name][0], model_dir(name, torch.bfloat16 if dtype == "bfloat16" else torch.float32)
+    w = folder_weights(folder)
+    prompts = [random_tokens(name, n, n) for n in (30, 1, 17)]
+    e = Engine(folder, dtype=dtype, page_size=8, kv_tokens=1024, max_concurrent=8, cuda_graphs=graphs, eos_token_id=())
+    got = e.beam_search(prompts, beams=4, max_tokens=6)
+    for p, hypotheses in zip(prompts, got):
+        if dtype == "float32":
+            want = plain_search(cfg, w, p, 4, 6, 1.0, set(), e.max_context)
+            assert [h.tokens for h in hypotheses] == [t for t, *_ in want]
+        assert [h.score for h in hypotheses] == sorted((h.score for h in hypotheses), reverse=True) and len({tuple(h.tokens) for h in hypotheses}) == 4
+        for h in hypotheses:
+            x = llama_plain.forward(cfg, w, p + h.tokens)[len(p) - 1:-1].astype(np.float64)
+            lse = x.max(axis=1) + np.log(np.exp(x - x.max(axis=1, keepdims=True)).sum(axis=1))
+            score = sum(row[t] - n for row, t, n in zip(x, h.tokens, lse))
+            # a logit is off by the tolerance times the largest one, a sum of logarithms by as much: twice that a token
+            assert abs(h.score - score) <= 2 * 6 * TOL[dtype] * np.abs(x).max()
+    assert e.cache.manager.live_requests == 0
+    e.cache.manager.check_invariants()
+
+
+def test_forked_states_on_the_device():
+    from garuda_b200 import Engine
+    from tests.test_beams import fork_a_model_with_states
+    from tests.test_extensibility import toy_dir
+    fork_a_model_with_states(Engine(toy_dir(), dtype="float32", page_size=8, max_concurrent=4))
+
+
+def test_forked_pages_in_8_bits(ops):
+    """Codes and their scales go together."""
+    from garuda_b200 import Engine
+    from tests.helpers import model_dir, random_tokens
+    e = Engine(model_dir("D", torch.bfloat16), dtype="bfloat16", cache_dtype="float8_e4m3", page_size=16, kv_tokens=512, max_concurrent=4)
+    from garuda_b200 import StepEntry
+    toks = random_tokens("D", 37, 1)
+    e.step([StepEntry(1, toks, ())])
+    e.cache.fork([(1, 2), (1, 3)], e.ops)
+    rows = e.step([StepEntry(r, [11], [0]) for r in (1, 2, 3)])
+    assert torch.equal(rows[0], rows[1]) and torch.equal(rows[0], rows[2])
+
+
 def test_captured_and_replayed(ops):
     """All of it in one graph, with new inputs in the same places; without a workspace and with one; beside eager calls."""
     from garuda_b200.engine.batch import Workspace
