@@ -312,7 +312,7 @@ attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts) 
     const float inv = lt == 0.f ? 0.f : 1.0f / lt;
     store4(place(row) + c * 4, make_float4(t.x * inv, t.y * inv, t.z * inv, t.w * inv));
   }
-  tc::cluster_arrive_wait();                   // nobody leaves while another reads
+  tc::cluster_read_wait();                     // nobody leaves while another reads
 }
 
 // Parts of a request's keys, a power of two: as long as all clusters run at once, and of a step at least. Of 148 SMs 74 clusters of two blocks, 33 of four, 15

@@ -508,32 +508,37 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
       bool spoiled = false;              // this row reads a value that is not finite
 
       for (int j = 0; j < count && ok; ++j, ++gt) {
-        wait(mc.s_ready[sb], sph, ERR_WAIT_ACCUM);
-        if (!ok) break;
-        tc_fence_after_sync();
-        // S of this tile is complete: its keys have been read, after a piece's last tile its queries (every warp says so: it is done with the piece in
-        // front), and the values of the tile two in front (products run in the order of their issue)
-        if (j == count - 1 && lane == 0) mbar_arrive(smem_u32(&mc.q_empty));
-        if (passes_on) {
-          if (freed < gt - 1) {
-            mbar_arrive(smem_u32(&mc.v_empty[vfree]));
-            if (++vfree == V_STAGES) vfree = 0;
-            ++freed;
-          }
-          if (!S::KEYS_FREED_BY_COMMIT) mbar_arrive(smem_u32(&mc.k_empty[kstage]));
-        }
-        if (++kstage == K_STAGES) kstage = 0;
-        const uint32_t s_addr = lane_addr + sb * KT + grp * GK;
-        uint32_t sv[GK / 32][32];
-        if (active) {
-#pragma unroll
-          for (int h = 0; h < GK / 32; ++h) tmem_ld_32(s_addr + h * 32, sv[h]);
-        }
+        // (What an edge asks of the row is read while the scores are made.)
         const int tile_key0 = first_key + j * KT, key0 = tile_key0 + grp * GK;
         const bool edge = tile_key0 + KT > edge_from || tile_key0 < edge_to;
         unsigned long long sees = ~0ull;
         if (edge) {
           const int token = w.q_begin + w.tok0 + (there ? row / p.g : 0);
+          // the keys of these 64 that the row reads: context, then drafted tokens by their bits
+          const int c = w.ctx - key0;
+          sees = 0;
+          if (there) {
+            const uint32_t* bits = p.mask + (size_t)token * p.mask_words;
+            if (c > 0) {
+              const int row_start = p.window > 0 ? max(0, p.positions[token] + 1 - p.window) : 0;
+              sees = c >= 64 ? ~0ull : (1ull << c) - 1;
+              const int s0 = row_start - key0;
+              if (s0 > 0) sees &= s0 >= 64 ? 0ull : ~0ull << s0;
+            }
+            if (c < 64) {
+              const int from = max(0, -c), word = from >> 5;
+              auto at = [&](int i) -> unsigned long long { return i < p.mask_words ? bits[i] : 0u; };
+              unsigned long long b = at(word) | (at(word + 1) << 32);
+              if (from & 31) b = (b >> (from & 31)) | (at(word + 2) << (64 - (from & 31)));
+              const int left = w.kv_len - key0 - max(0, c);         // drafted tokens from there on
+              b &= left >= 64 ? ~0ull : left > 0 ? (1ull << left) - 1 : 0ull;
+              sees |= c > 0 ? b << c : b;
+            }
+          }
+        }
+        // The values of a tile at an edge: rows that nobody may read are cleared, those that are not finite noted.
+        auto look = [&]() {
+          if (!edge) return;
           wait(mc.v_full[vstage], vpar, ERR_WAIT_FULL);
           bool bad = false;
           if (ok && row < GK) {               // (a row of values to each of half of the group's threads)
@@ -564,29 +569,33 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
           wait(mc.looked[grp], et & 1, ERR_WAIT_FULL);
           const unsigned long long spoils = mc.bad[et & 1][grp][0] | ((unsigned long long)mc.bad[et & 1][grp][1] << 32);
           ++et;
-          // the keys of these 64 that the row reads: context, then drafted tokens by their bits
-          const int c = w.ctx - key0;
-          sees = 0;
-          if (there) {
-            const uint32_t* bits = p.mask + (size_t)token * p.mask_words;
-            if (c > 0) {
-              const int row_start = p.window > 0 ? max(0, p.positions[token] + 1 - p.window) : 0;
-              sees = c >= 64 ? ~0ull : (1ull << c) - 1;
-              const int s0 = row_start - key0;
-              if (s0 > 0) sees &= s0 >= 64 ? 0ull : ~0ull << s0;
-            }
-            if (c < 64) {
-              const int from = max(0, -c), word = from >> 5;
-              auto at = [&](int i) -> unsigned long long { return i < p.mask_words ? bits[i] : 0u; };
-              unsigned long long b = at(word) | (at(word + 1) << 32);
-              if (from & 31) b = (b >> (from & 31)) | (at(word + 2) << (64 - (from & 31)));
-              const int left = w.kv_len - key0 - max(0, c);         // drafted tokens from there on
-              b &= left >= 64 ? ~0ull : left > 0 ? (1ull << left) - 1 : 0ull;
-              sees |= c > 0 ? b << c : b;
-            }
-          }
           spoiled = spoiled || (sees & spoils) != 0;
+        };
+        // (In front of the scores if the tile is one of few: then the values come no later than the keys. Their stage was given back before the scores in
+        // front were used, so that they come whatever this warp waits for.)
+        if (CLUSTER) look();
+        wait(mc.s_ready[sb], sph, ERR_WAIT_ACCUM);
+        if (!ok) break;
+        tc_fence_after_sync();
+        // S of this tile is complete: its keys have been read, after a piece's last tile its queries (every warp says so: it is done with the piece in
+        // front), and the values of the tile two in front (products run in the order of their issue)
+        if (j == count - 1 && lane == 0) mbar_arrive(smem_u32(&mc.q_empty));
+        if (passes_on) {
+          if (freed < gt - 1) {
+            mbar_arrive(smem_u32(&mc.v_empty[vfree]));
+            if (++vfree == V_STAGES) vfree = 0;
+            ++freed;
+          }
+          if (!S::KEYS_FREED_BY_COMMIT) mbar_arrive(smem_u32(&mc.k_empty[kstage]));
         }
+        if (++kstage == K_STAGES) kstage = 0;
+        const uint32_t s_addr = lane_addr + sb * KT + grp * GK;
+        uint32_t sv[GK / 32][32];
+        if (active) {
+#pragma unroll
+          for (int h = 0; h < GK / 32; ++h) tmem_ld_32(s_addr + h * 32, sv[h]);
+        }
+        if (!CLUSTER) look();
         if (++vstage == V_STAGES) vstage = 0, vpar ^= 1;
         if (!ok) break;
         if (active) {
@@ -738,8 +747,8 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
     if (w.count == 0)
       for (int i = threadIdx.x; i < QROWS; i += THREADS) reinterpret_cast<float2*>(part + QROWS * HD)[i] = make_float2(-INFINITY, 0.f);
     cluster_arrive_wait();
-    const int items = w.nrows * (HD / 8);              // eight channels of a row
-    for (int i = rank * THREADS + threadIdx.x; i < items && !*abort_s; i += ranks * THREADS) {
+    const int items = w.nrows * (HD / 8), mine = (items + ranks - 1) / ranks;          // eight channels of a row
+    for (int i = rank * mine + threadIdx.x; i < min(items, (rank + 1) * mine) && !*abort_s; i += THREADS) {
       const int row = i % w.nrows, f0 = i / w.nrows * 2;
       const uint32_t ml_at = smem_u32(part + QROWS * HD + row * 2), v_at = smem_u32(part) + (uint32_t)(f0 * QROWS + row) * 16;
       Join join;
@@ -761,7 +770,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
       join.store(reinterpret_cast<__nv_bfloat16*>(p.out) +
                  ((size_t)(w.q_begin + w.tok0 + row / p.g) * p.Hq + w.kvh * p.g + row % p.g) * HD + f0 * 4);
     }
-    cluster_arrive_wait();                             // nobody leaves while another reads
+    cluster_read_wait();                               // nobody leaves while another reads
   }
   if (warp == 1) tmem_dealloc(tmem_base, TMEM_COLS);
 }
@@ -783,7 +792,7 @@ int tensor_map(const void* ptr, int hd, long long d1, long long d2, long long d3
 }
 
 // CTAs of a cluster that share the keys of each of `units` blocks of rows, or 0: stretches. Clusters need no scratch memory, no scan of the lengths, and
-// join faster (a request of 8 tokens, 8 heads of 128, 500 keys: 10.6 us against 13.3; 8,000 keys: 18 against 22), but they are of 2, 4 or 8 CTAs (16 took
+// join faster (a request of 8 tokens, 8 heads of 128, 500 keys: 9.6 us against 13.3; 8,000 keys: 17.4 against 22), but they are of 2, 4 or 8 CTAs (16 took
 // twice as long: hardly any run at once), so that SMs stay idle, and wait for the longest request (32,000 keys: 46 against 38). In microseconds, with what both
 // have in common left out: a tile takes 1.1, a piece of a stretch 0.4 to join.
 template <int HD>

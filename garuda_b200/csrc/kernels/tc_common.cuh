@@ -127,6 +127,11 @@ __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
 __device__ __forceinline__ void cluster_arrive_wait() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The same where nobody reads what another has written from here on: what a thread has read of the others it has used, so that nothing of it is
+// on its way, and its own writes need not have arrived.
+__device__ __forceinline__ void cluster_read_wait() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
 // The address, in the cluster's shared window, of `local` in the CTA of rank `rank`.
 __device__ __forceinline__ uint32_t map_to_rank(uint32_t local, uint32_t rank) {
   uint32_t r;
