@@ -68,11 +68,13 @@ tree_layout_kernel(const int32_t* __restrict__ parents, const int32_t* __restric
 // then -1; kept[r]: how many; next_tokens[r] = targets of the last. Row ctx + path[i] of every array's pages goes to row ctx + i.
 //
 // Every block of a request makes the same walk (a few microseconds' worth of waiting at most, and no block waits for another), then moves its
-// share of the rows. A thread has its vectors of every row to itself and path is ascending, path[i] >= i: read in that order, eight rows at a time before
-// any of them is written, no row is overwritten before it has been read.
+// share of the rows. A thread has its vectors of every row to itself and path is ascending, path[i] >= i: read in that order, some rows at a time before
+// any of them is written, no row is overwritten before it has been read. (Four: 64 requests of 64 tokens, 43 MB of rows read and written, take 13.0 us; eight, for
+// which registers leave fewer blocks on an SM, 15.9, two 13.4.) Bound by the way to the rows (lengths, then the tree and its pages, then the rows: 3 us for
+// one small tree) and by their pieces of 256 bytes, which lie apart: 3.3 TB/s.
 constexpr int ACCEPT_THREADS = 256;
 constexpr int ACCEPT_TOKENS = 8192;
-constexpr int AHEAD = 8;
+constexpr int AHEAD = 4;
 
 struct Arrays {
   static constexpr int MOST = 64;
@@ -91,39 +93,43 @@ tree_accept_kernel(const int32_t* __restrict__ tokens, const int32_t* __restrict
   extern __shared__ int2 smem[];
   int2* const from = smem;                      // [most]: page and line of the rows (page -1: no move)
   int2* const to = from + most;
-  int32_t* const follow = reinterpret_cast<int32_t*>(to + most);        // [most]: the token accepted behind each
-  int32_t* const walk = follow + most;          // [most]
-  __shared__ int kept_s;
+  int32_t* const walk = reinterpret_cast<int32_t*>(to + most);          // [most]
+  int32_t* const pages_s = walk + most;         // [most + 1]: from the context's end on
+  int32_t* const follow = reinterpret_cast<int32_t*>(from);             // [most]: the token accepted behind each (until the rows are known)
+  int32_t* const wanted = reinterpret_cast<int32_t*>(to);               // [most]: targets (likewise)
+  __shared__ int kept_s, moved_s;
   gb::pdl_launch_dependents();
   gb::pdl_wait();
   const int r = blockIdx.y, first = cu_q[r], q_len = min(cu_q[r + 1] - first, most), ctx = kv_lens[r] - (cu_q[r + 1] - first);
-  for (int i = threadIdx.x; i < q_len; i += ACCEPT_THREADS) follow[i] = INT_MAX;
-  __syncthreads();
-  for (int i = threadIdx.x; i < q_len; i += ACCEPT_THREADS) {
-    const int above = parents[first + i];
-    if (above >= 0 && above < i && tokens[first + i] == targets[first + above]) atomicMin(&follow[above], i);
+  const bool moves = arrays.n > 0 && ctx >= 0;
+  const int first_entry = moves ? ctx / page_size : 0, last_entry = moves ? min(table_width, (ctx + q_len - 1) / page_size + 1) : 0;
+  for (int i = threadIdx.x; i < q_len; i += ACCEPT_THREADS) follow[i] = INT_MAX, wanted[i] = targets[first + i];
+  for (int i = first_entry + threadIdx.x; i < last_entry; i += ACCEPT_THREADS) pages_s[i - first_entry] = block_table[(size_t)r * table_width + i];
+  for (int i0 = 0; i0 < q_len; i0 += ACCEPT_THREADS) {
+    const int i = i0 + threadIdx.x, above = i < q_len ? parents[first + i] : -1, token = i < q_len ? tokens[first + i] : 0;
+    if (i0 == 0) __syncthreads();               // (behind the loads, which are on their way together)
+    if (above >= 0 && above < i && token == wanted[above]) atomicMin(&follow[above], i);
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    int n = 0;
-    for (int at = 0; at < q_len; at = follow[at]) walk[n++] = at;
-    kept_s = n;
+    int n = 0, in_place = 0;                    // (the first tokens of a path may be where they belong, none behind one that is not)
+    for (int at = 0; at < q_len; at = follow[at]) in_place += at == n, walk[n++] = at;
+    kept_s = n, moved_s = in_place;
   }
   __syncthreads();
-  const int n = kept_s;
+  const int n = kept_s, moved = moved_s;
   if (blockIdx.x == 0) {
     for (int i = threadIdx.x; i < path_width; i += ACCEPT_THREADS) path[(size_t)r * path_width + i] = i < n ? walk[i] : -1;
     if (threadIdx.x == 0) kept[r] = n, next_tokens[r] = n > 0 ? targets[first + walk[n - 1]] : -1;
   }
-  if (arrays.n == 0 || ctx < 0) return;
-  for (int i = threadIdx.x; i < n; i += ACCEPT_THREADS) {
+  if (!moves || moved == n) return;
+  for (int i = moved + threadIdx.x; i < n; i += ACCEPT_THREADS) {
     auto line = [&](int slot) {
-      const int entry = slot / page_size;
-      const int page = entry < table_width ? block_table[(size_t)r * table_width + entry] : -1;
+      const int entry = slot / page_size, page = entry < last_entry ? pages_s[entry - first_entry] : -1;
       return make_int2(page < pages ? page : -1, slot % page_size);
     };
     const int2 a = line(ctx + walk[i]), b = line(ctx + i);
-    from[i] = make_int2(walk[i] != i && b.x >= 0 ? a.x : -1, a.y), to[i] = b;
+    from[i] = make_int2(b.x >= 0 ? a.x : -1, a.y), to[i] = b;
   }
   __syncthreads();
   // this block's calls, of all arrays in a row; its threads have (call, head, vector) places
@@ -139,7 +145,7 @@ tree_accept_kernel(const int32_t* __restrict__ tokens, const int32_t* __restrict
       uint8_t* const base = arrays.at[k] + (size_t)(call - arrays.first[k] + x / per_call) * pages * page_bytes + head * head_bytes +
                             vector * sizeof(V);
       auto place = [&](int2 where) { return reinterpret_cast<V*>(base + where.x * page_bytes + where.y * line_bytes); };
-      for (int i0 = 0; i0 < n; i0 += AHEAD) {
+      for (int i0 = moved; i0 < n; i0 += AHEAD) {
         V v[AHEAD];
 #pragma unroll
         for (int e = 0; e < AHEAD; ++e)
@@ -294,15 +300,15 @@ GB_EXPORT int gb_tree_accept(const AcceptCall* call) {
     all |= (uintptr_t)pool[0] | (uintptr_t)pool[3];
   }
   const int rows = a.first[n];
-  // as many blocks as run at once (eight of 256 threads an SM), and no more walks than that
+  // a few more blocks than run at once (six of 256 threads an SM; exactly as many 13.8 us, twice as many 17): each walks its request's tree
   const int room = 8 * gb::sm_count();
   const int per_block = rows > 0 ? (int)(((long long)rows * R + room - 1) / room) : 1, blocks = rows > 0 ? (rows + per_block - 1) / per_block : 1;
-  const size_t smem = 24 * (size_t)max_q_len;
+  const size_t smem = 24 * (size_t)max_q_len + 4;
   auto launch = [&](auto vector) {
     const auto kernel = tree_accept_kernel<decltype(vector)>;
     static gb::OncePerDevice configured;          // (one per type)
     if (configured.needed()) {
-      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 24 * ACCEPT_TOKENS);
+      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 24 * ACCEPT_TOKENS + 4);
       if (e != cudaSuccess) return gb::fail(GB_CUDA_ERROR, "tree_accept: %s", cudaGetErrorString(e));
       configured.done();
     }
