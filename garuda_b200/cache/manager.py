@@ -112,25 +112,25 @@ class PagedCache:
         if {p for p, _ in pairs} & {c for _, c in pairs}:
             raise ValueError("a request that is forked in this call cannot be forked in it again")
         done, copies = [], []
-        try:
-            for parent, child in pairs:
-                copies += self.manager.fork(parent, child)
-                done.append(child)
-        except self.host_module.CacheError:
-            for child in done:
-                self.manager.release(child)
-            raise
 
         def copy(arrays, moves, dim):
             for i in range(0, len(moves), ops.MOST_COPIES):          # (targets are new: no copy's source is another's target)
                 both = torch.tensor(moves[i:i + ops.MOST_COPIES], dtype=torch.int32).t().contiguous().to(self.device)
                 ops.copy_entries(arrays, both[0], both[1], dim)
 
-        for g in range(len(self.groups)):
-            arrays = [self.k_pools[g], self.v_pools[g]] + ([self.k_scales[g], self.v_scales[g]] if self.float8 else [])
-            copy([a for a in arrays if a is not None], [(a, b) for group, a, b in copies if group == g], 1)
-        if self.states:
-            copy(list(self.states.values()), [(self.manager.slot(a), self.manager.slot(b)) for a, b in pairs], 0)
+        try:
+            for parent, child in pairs:
+                copies += self.manager.fork(parent, child)
+                done.append(child)
+            for g in range(len(self.groups)):
+                arrays = [self.k_pools[g], self.v_pools[g]] + ([self.k_scales[g], self.v_scales[g]] if self.float8 else [])
+                copy([a for a in arrays if a is not None], [(a, b) for group, a, b in copies if group == g], 1)
+            if self.states:
+                copy(list(self.states.values()), [(self.manager.slot(a), self.manager.slot(b)) for a, b in pairs], 0)
+        except Exception:
+            for child in done:
+                self.manager.release(child)
+            raise
 
     def bytes_per_position(self) -> int:
         if self.float8:         # and a page's two scales a head

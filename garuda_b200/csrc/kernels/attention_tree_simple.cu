@@ -79,9 +79,9 @@ attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts) 
   gb::pdl_wait();
   const int r = blockIdx.z, kvh = blockIdx.y % p.Hkv, block = blockIdx.y / p.Hkv, part = blockIdx.x;
   const int q_begin = p.cu_q[r], q_len = p.cu_q[r + 1] - q_begin, row0 = block * ROWS, nrows = min(ROWS, q_len * p.g - row0);
-  const int kv_len = p.kv_lens[r], ctx = max(0, kv_len - q_len);
-  if (nrows <= 0 || kv_len <= 0) return;       // (the whole cluster's)
-  const int lo = (p.window > 0 ? max(0, ctx + 1 - p.window) : 0) / KEYS, steps = (kv_len - 1) / KEYS + 1 - lo;
+  const int kv_len = max(0, p.kv_lens[r]), ctx = max(0, kv_len - q_len);
+  if (nrows <= 0) return;                      // (the whole cluster's)
+  const int lo = (p.window > 0 ? max(0, ctx + 1 - p.window) : 0) / KEYS, steps = (kv_len - 1) / KEYS + 1 - lo;       // (one at least, without keys too)
   const int per = (steps + parts - 1) / parts, begin = lo + part * per, end = min(lo + steps, begin + per);
   const int32_t* table = p.block_table + (size_t)r * p.table_width;
 

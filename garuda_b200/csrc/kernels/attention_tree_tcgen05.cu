@@ -232,9 +232,9 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
   // ---- the tiles of every request
   const int tokens_per_block = QROWS / p.g;
   auto low_of = [&](int ctx) { return p.window > 0 ? max(0, ctx + 1 - p.window) : 0; };
-  auto tiles_of = [&](int q_len, int kv_len) {       // of one head and block of rows
-    if (q_len <= 0 || kv_len <= 0) return 0;
-    return (kv_len - 1) / KT + 1 - low_of(max(0, kv_len - q_len)) / KT;
+  auto tiles_of = [&](int q_len, int kv_len) {       // of one head and block of rows: one at least, without keys too
+    if (q_len <= 0) return 0;
+    return (max(1, kv_len) - 1) / KT + 1 - low_of(max(0, kv_len - q_len)) / KT;
   };
   for (int r0 = 0; !CLUSTER && r0 < p.R; r0 += THREADS) {
     const int r = r0 + threadIdx.x;

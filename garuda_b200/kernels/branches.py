@@ -51,6 +51,8 @@ class BranchOps:
 
     #: ``tree_layout`` and ``tree_accept`` take trees of up to this many tokens
     MOST_DRAFTED = 8192
+    #: ``tree_attention`` reads requests of up to this many positions
+    MOST_POSITIONS = 1 << 30
     #: ``copy_entries`` makes up to this many copies
     MOST_COPIES = 1024
     #: ``beam_select`` takes up to this many beams and chooses up to this many candidates
@@ -150,7 +152,7 @@ class BranchOps:
         _need(mask.dtype is torch.int32 and mask.is_contiguous() and mask.dim() == 2 and mask.shape[0] == T, f"{what}: mask must be contiguous int32 [T, words]")
         _need(0 <= max_q_len <= min(32 * mask.shape[1], self.MOST_DRAFTED), f"{what}: at most {self.MOST_DRAFTED} drafted tokens of a request, and 32 to a word")
         _need(mask.shape[1] * 32 <= self.MOST_DRAFTED, f"{what}: a mask of more than {self.MOST_DRAFTED} bits")
-        _need(window >= 0, f"{what}: a window cannot be negative")
+        _need(0 <= window < 1 << 31, f"{what}: a window of 31 bits")
         if T == 0 or R == 0:
             return
         L = self.branch_lib
@@ -182,11 +184,12 @@ class BranchOps:
                 and v_pool.is_contiguous() and Hkv > 0 and Hq % Hkv == 0 and block_table.dtype is i32 and cu_q.dtype is i32 and kv_lens.dtype is i32
                 and positions.dtype is i32 and mask.dtype is i32 and block_table.is_contiguous() and cu_q.is_contiguous() and kv_lens.is_contiguous()
                 and positions.is_contiguous() and mask.is_contiguous() and cu_q.shape == (R + 1,) and kv_lens.dim() == 1 and table[0] >= R
-                and positions.shape == (T,) and rows == T and 32 * words >= max_q_len > 0 and scale > 0 and window >= 0
-                and width * page_size >= max_kv_len and q.get_device() == dev and k_pool.get_device() == dev and v_pool.get_device() == dev
+                and positions.shape == (T,) and rows == T and 32 * words >= max_q_len > 0 and scale > 0
+                and 0 <= window < 1 << 31 and width * page_size >= max_kv_len <= self.MOST_POSITIONS and q.get_device() == dev and k_pool.get_device() == dev and v_pool.get_device() == dev
                 and out.get_device() == dev and block_table.get_device() == dev and cu_q.get_device() == dev and kv_lens.get_device() == dev
                 and positions.get_device() == dev and mask.get_device() == dev):
-            self._refuse_attention(q, k_pool, v_pool, block_table, cu_q, kv_lens, positions, mask, out, scale, window, page_size, max_q_len)
+            self._refuse_attention(q, k_pool, v_pool, block_table, cu_q, kv_lens, positions, mask, out, scale, window, page_size, max_q_len,
+                                   max_kv_len)
         if T == 0 or R == 0:
             return
         L, g, stream = self.branch_lib, Hq // Hkv, self._stream()
@@ -208,7 +211,7 @@ class BranchOps:
             scratch, stream, width, words, T, R, pages, Hq, Hkv, hd, window, page_size, max_q_len, max_kv_len, _TAG[dtype], scale)),
             "tree_attention", launches)
 
-    def _refuse_attention(self, q, k_pool, v_pool, block_table, cu_q, kv_lens, positions, mask, out, scale, window, page_size, max_q_len):
+    def _refuse_attention(self, q, k_pool, v_pool, block_table, cu_q, kv_lens, positions, mask, out, scale, window, page_size, max_q_len, max_kv_len):
         what = "tree_attention"
         T, Hq, hd = q.shape
         Hkv, R = k_pool.shape[1], kv_lens.shape[0]
@@ -226,7 +229,8 @@ class BranchOps:
         _need(block_table.shape[0] >= R, f"{what}: a row of the block table for every request")
         _need(positions.shape == (T,) and mask.shape[0] == T, f"{what}: a position and a row of the mask for every token")
         _need(0 < max_q_len <= 32 * mask.shape[1], f"{what}: the mask is too narrow for that many tokens")
-        _need(scale > 0 and window >= 0, f"{what}: a positive scale, a window that is not negative")
+        _need(scale > 0 and 0 <= window < 1 << 31, f"{what}: a positive scale, a window that is not negative (and fits 31 bits)")
+        _need(max_kv_len <= self.MOST_POSITIONS, f"{what}: at most {self.MOST_POSITIONS} positions of a request")
         raise KernelError(f"{what}: the block table is too narrow for that many positions")
 
     def tree_accept(self, tokens, targets, parents, cu_q, kv_lens, path, kept, next_tokens, max_q_len: int, pools=(), block_table=None,
@@ -236,7 +240,7 @@ class BranchOps:
         continue the last one and are its target is kept, until there is none. ``path [R, width]`` (int32) becomes the kept tokens' numbers, then
         -1, ``kept [R]`` how many they are (0: a request without tokens), ``next_tokens [R]`` the last one's target (-1).
 
-        ``pools`` (each ``[calls, pages, heads, page_size, width]`` or without ``calls``; two or four bytes a number) share ``block_table``: the
+        ``pools`` (each ``[calls, pages, heads, page_size, width]`` or without ``calls``; two or four bytes a number; none twice) share ``block_table``: the
         rows of kept tokens, at ``kv_lens[r]`` less the tree's size plus their numbers, go to the places right behind the context, in
         every call. Rows behind them, and where the block table has no page, are left as they are. The request's length is then its context plus
         ``kept[r]``. (A chosen token may come from any rule, a drawn one too: a token is its parent's target or is not kept.)"""
@@ -282,6 +286,9 @@ class BranchOps:
                     _need(item in (2, 4), f"{what}: rows of two or four bytes a number (pages in 8 bits have a scale for all their rows)")
                     raise KernelError(f"{what}: pools of one block table have the same number of pages")
                 flat.extend((pool.data_ptr(), shape[0] if len(shape) == 5 else 1, shape[-3], shape[-1] * item))
+            if len(set(flat[::4])) != len(pools):
+                at = [a for a in flat[::4] if a]               # (empty ones have no address)
+                _need(len(set(at)) == len(at), f"{what}: a pool is given twice")
         if R == 0:
             return
         L = self.branch_lib
@@ -354,5 +361,6 @@ class BranchOps:
         if not flat or copies[0] == 0:
             return
         L, k = self.branch_lib, len(flat) // 4
+        _need(len(set(flat[::4])) == k, f"{what}: an array is given twice")
         self._check(L, L.gb_copy_entries(_COPY_CALL.pack(source.data_ptr(), target.data_ptr(), flat.buffer_info()[0], self._stream(), k, copies[0])), what,
                     (k + 95) // 96)

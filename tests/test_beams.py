@@ -178,6 +178,22 @@ def test_fork_takes_everything_back_when_pages_run_out():
 
 
 # ------------------------------------------------------------------ the search
+def test_fork_takes_everything_back_when_a_copy_is_refused():
+    e = engine("A")
+    e.step([StepEntry(1, random_tokens("A", 11, 1), ())])
+    free = [e.cache.manager.free_pages(g) for g in range(len(e.cache.groups))]
+
+    def refuse(*args):
+        raise RuntimeError("refused")
+
+    e.ops.copy_entries = refuse
+    with pytest.raises(RuntimeError, match="refused"):
+        e.cache.fork([(1, 2), (1, 3)], e.ops)
+    assert not e.cache.manager.known(2) and not e.cache.manager.known(3)
+    assert [e.cache.manager.free_pages(g) for g in range(len(e.cache.groups))] == free
+    e.cache.manager.check_invariants()
+
+
 def plain_search(cfg, weights, prompt, beams, max_tokens, penalty, eos, context):
     """The same search with the whole sequence run anew for every beam."""
     live, done = [([], 0.0)], []

@@ -161,3 +161,33 @@ def test_copies_hand_on_shapes_and_leave_out_empty_arrays():
     ops.copy_entries([zeros(3, 7)], zeros(0), zeros(0))
     ops.copy_entries([], zeros(2), zeros(2))
     assert len(ops.calls) == 1
+
+
+def test_what_would_not_fit_the_kernels_numbers_is_refused():
+    ops = Recorder()
+    for window in (1 << 31, (1 << 32) + 5):
+        with pytest.raises(KernelError, match="31 bits"):
+            ops.tree_attention(**attention_args(window=window))
+        with pytest.raises(KernelError, match="31 bits"):
+            ops.tree_layout(zeros(5), zeros(3), zeros(2), zeros(5), zeros(5, 1), 3, window)
+    wide = zeros(2, ((1 << 30) + 128) // 128)
+    with pytest.raises(KernelError, match="positions of a request"):
+        ops.tree_attention(**attention_args(page=128, block_table=wide, max_kv_len=(1 << 30) + 1))
+    assert not ops.names()
+    ops.tree_attention(**attention_args(page=128, block_table=wide, max_kv_len=1 << 30, window=(1 << 31) - 1))
+    assert len(ops.names()) == 1
+
+
+def test_an_array_given_twice_is_refused():
+    ops = Recorder()
+    pool, empty = zeros(2, 4, 2, 32, 64, dtype=BF16), zeros(0, 4, 2, 32, 64, dtype=BF16)
+    accept = dict(tokens=zeros(5), targets=zeros(5), parents=zeros(5), cu_q=zeros(3), kv_lens=zeros(2), path=zeros(2, 3), kept=zeros(2), next_tokens=zeros(2),
+                  max_q_len=3, block_table=zeros(2, 3), page_size=32)
+    with pytest.raises(KernelError, match="given twice"):
+        ops.tree_accept(pools=[pool, empty, empty, pool.view(2, 4, 2, 32, 64)], **accept)
+    with pytest.raises(KernelError, match="given twice"):
+        ops.copy_entries([pool, pool.clone(), pool.view(2, 4, -1)], zeros(2), zeros(2), 1)
+    assert not ops.names()
+    ops.tree_accept(pools=[pool, empty, empty, pool.clone()], **accept)
+    ops.copy_entries([pool, empty, empty, pool.clone()], zeros(2), zeros(2), 1)
+    assert len(ops.names()) == 2

@@ -182,6 +182,19 @@ def test_rows_behind_the_last_request_and_absent_pages(ops):
 
 
 # ------------------------------------------------------------------ trees
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("requests", [3, 90])
+def test_a_length_of_zero_reads_nothing(ops, dtype, requests):
+    """(Of a padded batch, say: tokens, but no key at all.) Their rows are zeros, the others' what they were."""
+    step = Step(requests, [(40 + 9 * (r % 5), 1 + r % 4) for r in range(requests)], 4, 2, 64, 32, dtype, 30 * (requests > 3))
+    want = step.run(ops)
+    step.kv = [0 if r % 3 == 1 else n for r, n in enumerate(step.kv)]
+    for r in range(1, requests, 3):
+        want[step.cu[r]:step.cu[r + 1]] = 0
+    assert torch.equal(step.run(ops), want)
+    ops.check_branch_errors()
+
+
 @pytest.mark.parametrize("window", [0, 1, 5, 40])
 def test_layout(ops, window):
     rng = random.Random(window)
