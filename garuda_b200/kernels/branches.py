@@ -144,19 +144,26 @@ class BranchOps:
         ancestor; with a ``window`` w those of its last w positions. A token whose parents do not lead to -1 gets no bits
         and the context's length as position."""
         what = "tree_layout"
-        self._here(parents, cu_q, kv_lens, positions, mask)
-        T = parents.shape[0]
-        R = self._check_requests(what, cu_q, kv_lens)
-        for t in (parents, positions):
-            _need(t.dtype is torch.int32 and t.is_contiguous() and t.shape == (T,), f"{what}: parents and positions must be contiguous int32 [T]")
-        _need(mask.dtype is torch.int32 and mask.is_contiguous() and mask.dim() == 2 and mask.shape[0] == T, f"{what}: mask must be contiguous int32 [T, words]")
-        _need(0 <= max_q_len <= min(32 * mask.shape[1], self.MOST_DRAFTED), f"{what}: at most {self.MOST_DRAFTED} drafted tokens of a request, and 32 to a word")
-        _need(mask.shape[1] * 32 <= self.MOST_DRAFTED, f"{what}: a mask of more than {self.MOST_DRAFTED} bits")
-        _need(0 <= window < 1 << 31, f"{what}: a window of 31 bits")
+        i32, dev, T, R = torch.int32, self._device_index, parents.shape[0], kv_lens.shape[0]
+        rows, words = mask.shape if mask.dim() == 2 else (-1, 0)
+        # (one condition, taken apart when it fails)
+        if not (parents.dtype is i32 and cu_q.dtype is i32 and kv_lens.dtype is i32 and positions.dtype is i32 and mask.dtype is i32 and parents.is_contiguous()
+                and cu_q.is_contiguous() and kv_lens.is_contiguous() and positions.is_contiguous() and mask.is_contiguous() and parents.shape == (T,)
+                and positions.shape == (T,) and rows == T and kv_lens.dim() == 1 and cu_q.shape == (R + 1,) and 0 <= max_q_len <= 32 * words <= self.MOST_DRAFTED
+                and 0 <= window < 1 << 31 and parents.get_device() == dev and cu_q.get_device() == dev and kv_lens.get_device() == dev
+                and positions.get_device() == dev and mask.get_device() == dev):
+            self._here(parents, cu_q, kv_lens, positions, mask)
+            self._check_requests(what, cu_q, kv_lens)
+            for t in (parents, positions):
+                _need(t.dtype is i32 and t.is_contiguous() and t.shape == (T,), f"{what}: parents and positions must be contiguous int32 [T]")
+            _need(mask.dtype is i32 and mask.is_contiguous() and rows == T, f"{what}: mask must be contiguous int32 [T, words]")
+            _need(0 <= max_q_len <= min(32 * words, self.MOST_DRAFTED), f"{what}: at most {self.MOST_DRAFTED} drafted tokens of a request, and 32 to a word")
+            _need(32 * words <= self.MOST_DRAFTED, f"{what}: a mask of more than {self.MOST_DRAFTED} bits")
+            raise KernelError(f"{what}: a window of 31 bits")
         if T == 0 or R == 0:
             return
         L = self.branch_lib
-        self._check(L, L.gb_tree_layout(parents.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), positions.data_ptr(), mask.data_ptr(), mask.shape[1],
+        self._check(L, L.gb_tree_layout(parents.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), positions.data_ptr(), mask.data_ptr(), words,
                                         window, R, max_q_len, self._stream()), what)
 
     def tree_attention(self, q, k_pool, v_pool, block_table, cu_q, kv_lens, positions, mask, out, scale, window, page_size, max_q_len, max_kv_len,
@@ -267,7 +274,7 @@ class BranchOps:
             _need(0 < max_q_len <= self.MOST_DRAFTED, f"{what}: 1 to {self.MOST_DRAFTED} drafted tokens of a request")
             _need(path_shape[1] >= max_q_len, f"{what}: a path as wide as the largest tree")
             raise KernelError(f"{what}: at most 65,535 requests")
-        pages, table, width, flat = 0, 0, 0, array("q")
+        pages, table, width, flat = 0, 0, 0, []
         if pools:
             if not (block_table is not None and block_table.dtype is i32 and block_table.is_contiguous() and block_table.dim() == 2
                     and block_table.get_device() == dev and block_table.shape[0] >= R):
@@ -277,7 +284,7 @@ class BranchOps:
             table, width = block_table.data_ptr(), block_table.shape[1]
             pages = pools[0].shape[-4] if pools[0].dim() >= 4 else 0
             for pool in pools:
-                shape, item = pool.shape, pool.dtype.itemsize
+                shape, item = pool.shape, pool.itemsize
                 if not (len(shape) in (4, 5) and pool.is_contiguous() and shape[-2] == page_size > 0 and (item == 2 or item == 4) and shape[-4] == pages
                         and pool.get_device() == dev):
                     self._here(pool)
@@ -285,16 +292,16 @@ class BranchOps:
                           f"{what}: pools must be contiguous [calls, pages, heads, page_size, width]")
                     _need(item in (2, 4), f"{what}: rows of two or four bytes a number (pages in 8 bits have a scale for all their rows)")
                     raise KernelError(f"{what}: pools of one block table have the same number of pages")
-                flat.extend((pool.data_ptr(), shape[0] if len(shape) == 5 else 1, shape[-3], shape[-1] * item))
-            if len(set(flat[::4])) != len(pools):
+                flat += pool.data_ptr(), shape[0] if len(shape) == 5 else 1, shape[-3], shape[-1] * item
+            if len({*flat[::4]}) != len(pools):
                 at = [a for a in flat[::4] if a]               # (empty ones have no address)
                 _need(len(set(at)) == len(at), f"{what}: a pool is given twice")
         if R == 0:
             return
-        L = self.branch_lib
+        L, packed = self.branch_lib, array("q", flat)
         self._check(L, L.gb_tree_accept(_ACCEPT_CALL.pack(
             tokens.data_ptr(), targets.data_ptr(), parents.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), path.data_ptr(), kept.data_ptr(),
-            next_tokens.data_ptr(), table, flat.buffer_info()[0], self._stream(), len(flat) // 4 if pages else 0, pages, path_shape[1], width, page_size, R,
+            next_tokens.data_ptr(), table, packed.buffer_info()[0], self._stream(), len(flat) // 4 if pages else 0, pages, path_shape[1], width, page_size, R,
             max_q_len)), what)
 
     # ------------------------------------------------------------------ beams
@@ -346,7 +353,7 @@ class BranchOps:
                 _need(t.dtype is i32 and t.is_contiguous() and t.dim() == 1 and t.shape == copies,
                       f"{what}: source and target must be contiguous int32 of one length")
             raise KernelError(f"{what}: {copies[0]} copies (at most {self.MOST_COPIES})")
-        flat, of_shape, of_dtype = array("q"), None, None
+        flat, of_shape, of_dtype = [], None, None
         for a in arrays:
             shape, dtype = a.shape, a.dtype
             if not (a.is_contiguous() and a.get_device() == dev):
@@ -354,13 +361,14 @@ class BranchOps:
                 raise KernelError(f"{what}: arrays must be contiguous and have dimension {dim}")
             if shape != of_shape or dtype is not of_dtype:           # (layers' arrays are alike)
                 _need(0 <= dim < len(shape), f"{what}: arrays must be contiguous and have dimension {dim}")
-                of_shape, of_dtype, entries = shape, dtype, shape[dim]
-                outer, inner = math.prod(shape[:dim]), math.prod(shape[dim + 1:]) * dtype.itemsize
-            if outer and entries and inner:
-                flat.extend((a.data_ptr(), outer, entries, inner))
+                of_shape, of_dtype, entries, nbytes = shape, dtype, shape[dim], a.nbytes
+                outer = 1 if dim == 0 else shape[0] if dim == 1 else math.prod(shape[:dim])
+            if nbytes:
+                flat += a.data_ptr(), outer, entries, nbytes // (outer * entries)
         if not flat or copies[0] == 0:
             return
-        L, k = self.branch_lib, len(flat) // 4
-        _need(len(set(flat[::4])) == k, f"{what}: an array is given twice")
-        self._check(L, L.gb_copy_entries(_COPY_CALL.pack(source.data_ptr(), target.data_ptr(), flat.buffer_info()[0], self._stream(), k, copies[0])), what,
+        L, k, packed = self.branch_lib, len(flat) // 4, array("q", flat)
+        if k > 1:
+            _need(len({*flat[::4]}) == k, f"{what}: an array is given twice")
+        self._check(L, L.gb_copy_entries(_COPY_CALL.pack(source.data_ptr(), target.data_ptr(), packed.buffer_info()[0], self._stream(), k, copies[0])), what,
                     (k + 95) // 96)
