@@ -2,14 +2,14 @@
 // the tensor cores does not apply (head sizes other than 64 and 128, pages of other sizes). The same formula, see attention_tree_tcgen05.cu.
 //
 // Bound by the multiply-adds (32-bit ones run on the ordinary pipes) and by what shared memory feeds them, so what counts is how many products a thread makes of
-// what it loads, and that no product waits for the one in front. A block takes up to 64 query rows, (token, head-of-group) pairs of one key/value head of one
-// request, and walks its keys 128 at a time; its 128 threads are 8 by 16: a thread has eight rows' scores with eight keys (16 loads to 256 multiply-adds), then
-// eight rows' sums of eight channels. Between them the scores lie in shared memory, where the softmax walks a row with two lanes. Where the blocks
-// of rows are fewer than the device runs at once, a request's keys are shared by the blocks of a thread-block cluster, which join their sums, in the order of the
-// keys, from one another's shared memory. Masked keys are skipped: nothing of them reaches a sum.
-// Four trees of 12 over up to 1,024 keys of heads of 64: 29 us, a step of 128 keys 12: scores 4 (1.9 clocks a multiply-add of a warp), softmax 4, sums 4.
-// (Two rows by four keys a thread: 33 us, 352 where this takes 182, 64 rows over 8,000 keys of 8 heads of 128. Sixteen rows a warp, a lane a key: 47. Products of
-// pairs, fma.rn.f32x2: 35.)
+// what it loads, how many places a load asks for, and that no product waits for the one in front. A block takes up to 64 query rows, (token, head-of-group) pairs
+// of one key/value head of one request, and walks its keys 128 at a time. Its 256 threads are two halves, which share the keys, of 8 by 16: a thread has up to
+// eight rows' scores with four keys (12 loads to 128 multiply-adds), then eight rows' sums of eight channels. Between them the scores lie in shared memory, where
+// the softmax walks a row with four lanes. Where the blocks of rows are fewer than the device runs at once, a request's keys are shared by the blocks
+// of a thread-block cluster, which join their sums, in the order of the keys, from one another's shared memory. Masked keys are skipped: nothing of them reaches a sum.
+// Four trees of 12 over up to 1,024 keys of heads of 64: 26 us (128 threads, eight rows by eight keys each: 29; a half's lanes in two runs of sixteen instead of
+// pairs: 27; copies of the next step's keys under this one's products: 27.5). 64 rows over 8,000 keys of 8 heads of 128: 120 (182, 134, 133.5).
+// (Sixteen rows a warp, a lane a key: 47 for the former. Products of pairs, fma.rn.f32x2: 35.)
 #include "branches.h"
 #include "tc_common.cuh"
 
@@ -19,15 +19,17 @@ namespace {
 
 using branches::TreeParams;
 
-constexpr int THREADS = 128, ACROSS = 16;       // threads of a block, and of a row
+constexpr int HALF = 128, THREADS = 2 * HALF;   // threads of a block: two halves, which share a row's keys
+constexpr int ACROSS = 16;                      // threads of a row in each
 constexpr int MOST_PARTS = 8;
 
 // What a head size takes: rows of a block and keys of a step, rows and keys of a thread; in the second product how many threads share a row's keys, and the fours of
 // channels of each (eight rows by eight channels, so that loads and multiply-adds take as long).
 template <int HDMAX, int R>
 struct Shape {
-  static constexpr int ROWS = R * (THREADS / ACROSS), KEYS = HDMAX > 128 ? 64 : 128, K = KEYS / ACROSS, SPLIT = HDMAX > 64 ? 1 : 2, WIDE = ACROSS / SPLIT, FOURS = HDMAX / (4 * WIDE);
-  static constexpr int WARP_ROWS = ROWS / (THREADS / 32), SHARE = 32 / WARP_ROWS;         // a warp's rows, and lanes of a row in the softmax
+  static constexpr int ROWS = R * (HALF / ACROSS), KEYS = HDMAX > 128 ? 64 : 128, K = KEYS / (2 * ACROSS), WIDE = HDMAX > 64 ? ACROSS : ACROSS / 2;
+  static constexpr int SPLIT = 2 * ACROSS / WIDE, FOURS = HDMAX / (4 * WIDE);
+  static constexpr int SHARE = 32 / R, BATCH = KEYS / SHARE < 8 ? KEYS / SHARE : 8;       // lanes of a row in the softmax (a warp has R rows), and scores they have at a time
   static constexpr int P_LD = ROWS + 4;         // floats of a key's weights
 };
 // floats of a row of channels: an odd number of 16 bytes, so that eight lanes' rows lie on different banks
@@ -64,10 +66,10 @@ __device__ __forceinline__ void copy_async_16(float* to, const void* from) {
 }
 
 template <typename T, int HDMAX, int R>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, HDMAX <= 64 && R < 8 ? 2 : 1)
 attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts) {
   using S = Shape<HDMAX, R>;
-  constexpr int ROWS = S::ROWS, KEYS = S::KEYS, K = S::K, FOURS = S::FOURS, WIDE = S::WIDE, P_LD = S::P_LD, WARP_ROWS = S::WARP_ROWS;
+  constexpr int ROWS = S::ROWS, KEYS = S::KEYS, K = S::K, FOURS = S::FOURS, WIDE = S::WIDE, P_LD = S::P_LD, BATCH = S::BATCH;
   extern __shared__ __align__(16) float smem[];
   __shared__ long long where[KEYS];            // the step's keys: their rows' places in the pools, -1: no page
   __shared__ float keep_s[ROWS];               // by what a row's sums are multiplied for a new maximum
@@ -85,8 +87,12 @@ attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts) 
   const int per = (steps + parts - 1) / parts, begin = lo + part * per, end = min(lo + steps, begin + per);
   const int32_t* table = p.block_table + (size_t)r * p.table_width;
 
-  const int tx = threadIdx.x % ACROSS, first_row = threadIdx.x / ACROSS * R, channel0 = 4 * (tx % WIDE), split = tx / WIDE;
-  const int lane = threadIdx.x & 31, soft_row = threadIdx.x / 32 * WARP_ROWS + lane % WARP_ROWS, soft_share = lane / WARP_ROWS;      // this lane's row
+  const int half = threadIdx.x / HALF, pair = threadIdx.x % HALF / 32;         // a warp of each half makes a pair: it has 2 R rows
+  // Neighbouring lanes have two groups of rows, pairs of lanes the keys or channels: of a 16-byte load a quad of lanes asks for two places at most, for which
+  // shared memory takes two clocks; with more it takes four.
+  const int lane = threadIdx.x & 31, tx = lane / 2, first_row = (2 * pair + lane % 2) * R, channel0 = 4 * (tx % WIDE), split = half * (ACROSS / WIDE) + tx / WIDE;
+  const int soft_row = (2 * pair + half) * R + lane % R, soft_share = lane / R;      // this lane's row in the softmax
+  auto meet_pair = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + pair) : "memory"); };
   const bool there = soft_row < nrows;
   const int token = q_begin + (there ? (row0 + soft_row) / p.g : 0), start = p.window > 0 ? p.positions[token] + 1 - p.window : 0;
   const uint32_t* const bits = p.mask + (size_t)token * p.mask_words;
@@ -112,6 +118,9 @@ attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts) 
     for (int c = threadIdx.x % 8; c < c4; c += 8)
       *reinterpret_cast<float4*>(qs + x * ld + c * 4) = x < nrows ? load4(from + c * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
+  int channel[FOURS];                          // this thread's fours of channels; those that the head does not have read another and are not stored
+#pragma unroll
+  for (int c = 0; c < FOURS; ++c) channel[c] = channel0 + 4 * WIDE * c < hd ? channel0 + 4 * WIDE * c : 0;
   float m = -INFINITY, l = 0.f;                // of this lane's row; the denominator: of its share of the keys
   float4 o[R][FOURS];
 #pragma unroll
@@ -138,13 +147,13 @@ attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts) 
     for (int i = 0; i < R; ++i)
 #pragma unroll
       for (int e = 0; e < K; ++e) s[i][e] = 0.f;
-#pragma unroll 1
+#pragma unroll 2
     for (int c = 0; c < c4; ++c) {
       float4 a[R], b[K];
 #pragma unroll
       for (int i = 0; i < R; ++i) a[i] = *reinterpret_cast<const float4*>(qs + (first_row + i) * ld + c * 4);
 #pragma unroll
-      for (int e = 0; e < K; ++e) b[e] = *reinterpret_cast<const float4*>(ks + (tx + ACROSS * e) * ld + c * 4);
+      for (int e = 0; e < K; ++e) b[e] = *reinterpret_cast<const float4*>(ks + (tx + ACROSS * (half * K + e)) * ld + c * 4);
       // (channel by channel: a sum's next addition is 64 others later)
       auto add = [&](auto channel) {
 #pragma unroll
@@ -163,13 +172,12 @@ attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts) 
     for (int e = 0; e < K; ++e)
 #pragma unroll
       for (int i = 0; i < R; i += 2)
-        *reinterpret_cast<float2*>(ks + (tx + ACROSS * e) * P_LD + first_row + i) = make_float2(s[i][e], s[i + 1][e]);
-    __syncwarp();                              // (a warp's rows are its own)
+        *reinterpret_cast<float2*>(ks + (tx + ACROSS * (half * K + e)) * P_LD + first_row + i) = make_float2(s[i][e], s[i + 1][e]);
+    meet_pair();                               // (a pair's rows are its own)
     // ---- the softmax, a row to one, two or four lanes, in loops: laid out over a thread's 64 scores it took six times as long, its instructions on their way
     const bool edge = key0 + KEYS > ctx || p.window > 0;
     float* const mine = ks + soft_row;
     float top = m;
-    constexpr int BATCH = 8;                   // (all read before one is written: nothing waits for the one in front)
 #pragma unroll 1
     for (int k0 = soft_share; k0 < KEYS; k0 += BATCH * S::SHARE) {
       float x[BATCH];
@@ -192,7 +200,7 @@ attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts) 
       }
     }
 #pragma unroll
-    for (int d = WARP_ROWS; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    for (int d = R; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
     const float keep = m == -INFINITY ? 1.f : weight_of(m, top), less = top == -INFINITY ? 0.f : top;        // (of nothing, or of what is no number and stays none)
     float sum = 0.f;
 #pragma unroll 1
@@ -211,7 +219,7 @@ attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts) 
     }
     l = l * keep + sum, m = top;
     if (soft_share == 0) keep_s[soft_row] = keep;
-    __syncwarp();
+    meet_pair();
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const float less_now = keep_s[first_row + i];
@@ -226,14 +234,19 @@ attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts) 
       float w[2][R];
       float4 v[2][FOURS];
       auto load = [&](int key, float (&w)[R], float4 (&v)[FOURS]) {
+        const float* const from = ks + key * P_LD + first_row;
+        if constexpr (R % 4 == 0) {
 #pragma unroll
-        for (int i = 0; i < R; i += 2) {
-          const float2 w2 = *reinterpret_cast<const float2*>(ks + key * P_LD + first_row + i);
-          w[i] = w2.x, w[i + 1] = w2.y;
+          for (int i = 0; i < R; i += 4) {
+            const float4 w4 = *reinterpret_cast<const float4*>(from + i);
+            w[i] = w4.x, w[i + 1] = w4.y, w[i + 2] = w4.z, w[i + 3] = w4.w;
+          }
+        } else {
+          const float2 w2 = *reinterpret_cast<const float2*>(from);
+          w[0] = w2.x, w[1] = w2.y;
         }
 #pragma unroll
-        for (int c = 0; c < FOURS; ++c)
-          v[c] = channel0 + 4 * WIDE * c < hd ? *reinterpret_cast<const float4*>(vs + key * ld + channel0 + 4 * WIDE * c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; c < FOURS; ++c) v[c] = *reinterpret_cast<const float4*>(vs + key * ld + channel[c]);
       };
       auto add = [&](const float (&w)[R], const float4 (&v)[FOURS]) {
 #pragma unroll
@@ -260,21 +273,35 @@ attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts) 
     else sums(std::false_type{});
   }
 #pragma unroll
-  for (int d = WARP_ROWS; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+  for (int d = R; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
   // ---- every row's sums, maximum and denominator where the queries were; then the cluster's blocks join their shares of the rows
   __syncthreads();
+  auto sums_to = [&](float* rows, bool add) {
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    float* const to = qs + (first_row + i) * ld;
+    for (int i = 0; i < R; ++i)
 #pragma unroll
-    for (int c = 0; c < FOURS; ++c) {
-      if (S::SPLIT == 2) {
-        o[i][c].x += __shfl_xor_sync(0xffffffffu, o[i][c].x, WIDE), o[i][c].y += __shfl_xor_sync(0xffffffffu, o[i][c].y, WIDE);
-        o[i][c].z += __shfl_xor_sync(0xffffffffu, o[i][c].z, WIDE), o[i][c].w += __shfl_xor_sync(0xffffffffu, o[i][c].w, WIDE);
+      for (int c = 0; c < FOURS; ++c) {
+        float4* const to = reinterpret_cast<float4*>(rows + (first_row + i) * ld + channel0 + 4 * WIDE * c);
+        const bool mine = tx < WIDE && channel0 + 4 * WIDE * c < hd;
+        if (add && mine) {
+          const float4 other = *reinterpret_cast<const float4*>(ks + (first_row + i) * ld + channel0 + 4 * WIDE * c);
+          o[i][c].x += other.x, o[i][c].y += other.y, o[i][c].z += other.z, o[i][c].w += other.w;
+        }
+        if (mine) *to = o[i][c];
       }
-      if (split == 0 && channel0 + 4 * WIDE * c < hd) *reinterpret_cast<float4*>(to + channel0 + 4 * WIDE * c) = o[i][c];
-    }
+  };
+  if (WIDE < ACROSS) {
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int c = 0; c < FOURS; ++c) {
+        o[i][c].x += __shfl_xor_sync(0xffffffffu, o[i][c].x, 2 * WIDE), o[i][c].y += __shfl_xor_sync(0xffffffffu, o[i][c].y, 2 * WIDE);
+        o[i][c].z += __shfl_xor_sync(0xffffffffu, o[i][c].z, 2 * WIDE), o[i][c].w += __shfl_xor_sync(0xffffffffu, o[i][c].w, 2 * WIDE);
+      }
   }
+  if (half == 1) sums_to(ks, false);                     // (where keys and weights were)
+  __syncthreads();
+  if (half == 0) sums_to(qs, true);
   if (soft_share == 0) *reinterpret_cast<float2*>(qs + soft_row * ld + hd) = make_float2(m, l);
   T* const out = reinterpret_cast<T*>(p.out);
   auto place = [&](int row) { return out + ((size_t)(q_begin + (row0 + row) / p.g) * p.Hq + kvh * p.g + (row0 + row) % p.g) * hd; };
@@ -315,43 +342,81 @@ attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts) 
   tc::cluster_read_wait();                     // nobody leaves while another reads
 }
 
-// Parts of a request's keys, a power of two: as long as all clusters run at once, and of a step at least. Of 148 SMs 74 clusters of two blocks, 33 of four, 15
-// of eight run at once; with two blocks an SM twice as many (and two more of eight, which wait a little: 29 us, parts of twice as many keys 46).
-int parts_of(long long units, int steps, int per_sm) {
-  const int sms = gb::sm_count(), at_once[3] = {per_sm * sms / 2, per_sm * sms * 2 / 9, per_sm > 1 ? sms * 2 / 9 : sms / 10};
-  int parts = 1;
-  for (int i = 0; i < 3 && units <= at_once[i] && 2 * parts <= steps; ++i) parts *= 2;
-  return parts;
+// How a call is cut: the rows of a block (8 r), and the parts of a request's keys.
+struct Plan {
+  int r, parts;
+  float time;
+};
+
+// Clusters of `parts` blocks that run at once (of the device that was current first).
+template <typename T, int HDMAX, int R>
+int at_once(int parts) {
+  static int known[MOST_PARTS + 1] = {};       // (one more than that; 0: not asked for yet)
+  if (known[parts] == 0) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(parts), config.blockDim = dim3(THREADS), config.dynamicSmemBytes = 4 * smem_floats<Shape<HDMAX, R>>(HDMAX);
+    cudaLaunchAttribute shape;
+    shape.id = cudaLaunchAttributeClusterDimension;
+    shape.val.clusterDim.x = parts, shape.val.clusterDim.y = shape.val.clusterDim.z = 1;
+    config.attrs = &shape, config.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, attention_tree_simple_kernel<T, HDMAX, R>, &config) != cudaSuccess) n = 0, cudaGetLastError();
+    known[parts] = n + 1;
+  }
+  return known[parts] - 1;
 }
 
 template <typename T, int HDMAX, int R>
-int launch(const TreeParams& p, int hd, int max_q_len, int max_kv_len, cudaStream_t stream) {
-  using S = Shape<HDMAX, R>;
-  const long long blocks = ((long long)max_q_len * p.g + S::ROWS - 1) / S::ROWS;
-  if (p.R > 65535 || blocks * p.Hkv > 65535) return gb::fail(GB_UNSUPPORTED, "tree_attention: %d requests, %lld blocks of rows", p.R, blocks * p.Hkv);
+int configure() {
   static gb::OncePerDevice configured;
   if (configured.needed()) {
     const cudaError_t e = cudaFuncSetAttribute(attention_tree_simple_kernel<T, HDMAX, R>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               4 * smem_floats<S>(HDMAX));
+                                               4 * smem_floats<Shape<HDMAX, R>>(HDMAX));
     if (e != cudaSuccess) return gb::fail(GB_CUDA_ERROR, "tree_attention: %s", cudaGetErrorString(e));
     configured.done();
   }
-  const int parts = parts_of(p.R * blocks * p.Hkv, (max_kv_len + S::KEYS - 1) / S::KEYS, HDMAX <= 64 ? 2 : 1);
+  return GB_OK;
+}
+
+template <typename T, int HDMAX, int R>
+int consider(const TreeParams& p, int max_q_len, int max_kv_len, float start, float step, Plan& best) {
+  using S = Shape<HDMAX, R>;
+  const int rc = configure<T, HDMAX, R>();
+  const long long units = ((long long)max_q_len * p.g + S::ROWS - 1) / S::ROWS * p.Hkv * p.R;
+  const int steps = (max_kv_len + S::KEYS - 1) / S::KEYS;
+  for (int parts = 1; !rc && parts <= MOST_PARTS && (parts == 1 || parts <= steps); ++parts) {
+    const int room = at_once<T, HDMAX, R>(parts);
+    if (room == 0) continue;
+    const float time = (float)((units + room - 1) / room) * (start + step * (float)((steps + parts - 1) / parts));
+    if (time < best.time) best = Plan{R, parts, time};
+  }
+  return rc;
+}
+
+template <typename T, int HDMAX, int R>
+int launch(const TreeParams& p, int hd, int max_q_len, int parts, cudaStream_t stream) {
+  using S = Shape<HDMAX, R>;
+  const long long blocks = ((long long)max_q_len * p.g + S::ROWS - 1) / S::ROWS;
+  if (p.R > 65535 || blocks * p.Hkv > 65535) return gb::fail(GB_UNSUPPORTED, "tree_attention: %d requests, %lld blocks of rows", p.R, blocks * p.Hkv);
   return gb::check_pdl_launch(gb::launch_pdl(attention_tree_simple_kernel<T, HDMAX, R>, dim3(parts, (unsigned)(blocks * p.Hkv), p.R), dim3(THREADS),
                                              4 * smem_floats<S>(hd), stream, dim3(parts), p, hd, parts), "tree_attention");
 }
 
-// Blocks of 64 rows (heads of more than 128 channels: 32); of 32 or 16 where no request has more (5 tokens, no shared heads, 500 keys of heads of 128: 53 us with
-// 64, 30 with 16), or where the device would be half empty with as many blocks as can share a request's keys (32 rows, 4 heads of 64, 3,000 keys: 35 us with 32,
-// 28 with 16).
+// What takes least: all blocks in as many rounds as the device needs for them, each as long as a start and its steps. The figures are microseconds, measured with
+// one block an SM (heads of 64 and, of 128 and 256 alike, 128 keys of 128 channels or 64 of 256). So 5 tokens without shared heads over 500 keys have blocks
+// of 16 rows, two a request (20 us; 64 rows in one or two parts 80 and 43), 64 rows over 8,000 keys two blocks of 32 in six parts (120; 64 in
+// eight parts, of which 15 run at once, 159).
 template <typename T, int HDMAX>
 int by_rows(const TreeParams& p, int hd, int max_q_len, int max_kv_len, cudaStream_t stream) {
-  const long long rows = (long long)max_q_len * p.g, steps = (max_kv_len + 127) / 128, parts = steps < MOST_PARTS ? steps : MOST_PARTS;
-  int most = HDMAX > 128 ? 32 : 64;
-  while (most > 16 && (rows <= most / 2 || 8 * ((rows + most - 1) / most) * p.R * p.Hkv * parts <= 3 * gb::sm_count())) most /= 2;
-  if (most == 16) return launch<T, HDMAX, 2>(p, hd, max_q_len, max_kv_len, stream);
-  if (most == 32) return launch<T, HDMAX, 4>(p, hd, max_q_len, max_kv_len, stream);
-  return launch<T, HDMAX, (HDMAX > 128 ? 4 : 8)>(p, hd, max_q_len, max_kv_len, stream);
+  Plan best{0, 1, INFINITY};
+  constexpr bool SMALL = HDMAX <= 64;
+  int rc = consider<T, HDMAX, 2>(p, max_q_len, max_kv_len, SMALL ? 7.f : 8.f, SMALL ? 5.f : 9.f, best);
+  if (!rc) rc = consider<T, HDMAX, 4>(p, max_q_len, max_kv_len, SMALL ? 7.f : 8.5f, SMALL ? 7.f : 12.f, best);
+  if (!rc && HDMAX <= 128) rc = consider<T, HDMAX, (HDMAX > 128 ? 4 : 8)>(p, max_q_len, max_kv_len, SMALL ? 7.5f : 11.5f, SMALL ? 10.5f : 18.5f, best);
+  if (rc) return rc;
+  if (best.r == 2) return launch<T, HDMAX, 2>(p, hd, max_q_len, best.parts, stream);
+  if (best.r == 8) return launch<T, HDMAX, (HDMAX > 128 ? 4 : 8)>(p, hd, max_q_len, best.parts, stream);
+  return launch<T, HDMAX, 4>(p, hd, max_q_len, best.parts, stream);
 }
 
 }  // namespace
