@@ -9,7 +9,7 @@
 // of a thread-block cluster, which join their sums, in the order of the keys, from one another's shared memory. Masked keys are skipped: nothing of them reaches a sum.
 // Four trees of 12 over up to 1,024 keys of heads of 64: 26 us (128 threads, eight rows by eight keys each: 29; a half's lanes in two runs of sixteen instead of
 // pairs: 27; copies of the next step's keys under this one's products: 27.5). 64 rows over 8,000 keys of 8 heads of 128: 120 (182, 134, 133.5).
-// (Sixteen rows a warp, a lane a key: 47 for the former. Products of pairs, fma.rn.f32x2: 35.)
+// (Sixteen rows a warp, a lane a key: 47 for the former. Sums by products of pairs, fma.rn.f32x2: 28, and 127 for the latter.)
 #include "branches.h"
 #include "tc_common.cuh"
 
