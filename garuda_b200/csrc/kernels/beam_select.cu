@@ -5,10 +5,11 @@
 //
 // Bound by the one pass over the logits. Within a beam candidates lie as their logits do, so a block walks a stretch of a row, 4,096 (few: 1,024)
 // logits at a time, and leaves its K largest and what the stretch adds to the row's sum in scratch memory; the block that counts the last
-// of an item's stretches joins them. Rows of beams that are over are not read. Tiles come by bulk copies, one ahead (registers for that were
-// spilled: 150 us against 57 for 512 rows of 128,256, whose bytes take 40); a thread's sixteen logits cost one comparison as long as none is above the
-// bound. Of those 57 us the stream itself takes 38 to 41; starting, the first tile and joining the last rows are the others. A small call is a chain of
-// waits: 4 rows of 32,000 take 8 us, one for the first tile, one for its bound, one and a half for the count, three and a half to join.
+// of an item's stretches joins them. Of rows of beams that are over only the first tiles are read. Tiles come by bulk copies, one ahead (registers for that were
+// spilled: 150 us against 56 for 512 rows of 128,256, whose bytes take 40); a thread's sixteen logits cost one comparison as long as none is above the
+// bound. SMs with three rows are through with the stream some fifteen before those with four, and joining the last item takes five. A small
+// call is a chain of waits: 4 rows of 32,000 take 8 us, half a one for the first tile, one for its bound, one for the list in order, one for the count, three
+// and a half to join.
 //   * The K largest: a list in shared memory of the logits above a bound. The first bound is the K-th largest of 64 maxima of groups of four
 //     threads, which is no larger than the K-th largest logit; the list is cut to K, and its last entry becomes the bound, whenever it has grown. A tile
 //     that runs the list over (many equal logits) enters by its own K-th key, found bit by bit.
@@ -143,24 +144,40 @@ beam_select_kernel(const float* __restrict__ logits, const long long ld, const f
   __syncthreads();
   gb::pdl_launch_dependents();
   gb::pdl_wait();
-  if (is_finite(scores[row])) {
-    // ---- a stretch of the row, in 16-byte vectors: places count from the 16 bytes in which the row begins
-    const float* const x_row = logits + row * ld;
-    const int shift = (int)((uintptr_t)x_row >> 2 & 3);
-    const int tile0 = chunk * tiles_per_block, tiles = min(tiles_per_block, (V + shift + TILE - 1) / TILE - tile0);
-    auto place = [&](int tile, int i) { return (tile0 + tile) * TILE + (i >> 2) * THREADS * 4 + (int)threadIdx.x * 4 + (i & 3) - shift; };
-    auto fetch = [&](int tile) {           // the tile's whole vectors: those of the row's ends are read where they are used
-      const int start = (tile0 + tile) * TILE - shift, from = start < 0 ? start + 4 : start;
-      const int vectors = max(0, min(start + TILE, V) - from) / 4;
-      const uint32_t bar = smem_u32(&sh.full[tile % STAGES]);
-      if (vectors == 0) {
-        mbar_arrive(bar);
-        return;
-      }
-      mbar_arrive_expect_tx(bar, vectors * 16);
-      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                       smem_u32(ring + tile % STAGES * TILE + (from - start))), "l"(x_row + from), "r"(vectors * 16), "r"(bar) : "memory");
-    };
+  // a stretch of the row, in 16-byte vectors: places count from the 16 bytes in which the row begins
+  const float* const x_row = logits + row * ld;
+  const int shift = (int)((uintptr_t)x_row >> 2 & 3);
+  const int tile0 = chunk * tiles_per_block, tiles = min(tiles_per_block, (V + shift + TILE - 1) / TILE - tile0);
+  auto place = [&](int tile, int i) { return (tile0 + tile) * TILE + (i >> 2) * THREADS * 4 + (int)threadIdx.x * 4 + (i & 3) - shift; };
+  auto fetch = [&](int tile) {           // the tile's whole vectors: those of the row's ends are read where they are used
+    const int start = (tile0 + tile) * TILE - shift, from = start < 0 ? start + 4 : start;
+    const int vectors = max(0, min(start + TILE, V) - from) / 4;
+    const uint32_t bar = smem_u32(&sh.full[tile % STAGES]);
+    if (vectors == 0) {
+      mbar_arrive(bar);
+      return;
+    }
+    mbar_arrive_expect_tx(bar, vectors * 16);
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_u32(ring + tile % STAGES * TILE + (from - start))), "l"(x_row + from), "r"(vectors * 16), "r"(bar) : "memory");
+  };
+  // (the first tiles are asked for before it is known whether the beam is over)
+  if (threadIdx.x == 0)
+    for (int tile = 0; tile < min(STAGES, tiles); ++tile) fetch(tile);
+  if (threadIdx.x < beams) sh.score[threadIdx.x] = scores[(long long)item * beams + threadIdx.x];
+  __syncthreads();
+  bool ok = true;
+  auto gave_up = [&]() {                 // a copy that never came: others in flight need microseconds to land
+    gb_err::report(ERR_WAIT_FULL);
+    const unsigned long long t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 2000000ull) {}
+  };
+  if (!is_finite(sh.score[blockIdx.y % beams])) {
+    if (threadIdx.x == 0) {
+      for (int tile = 0; tile < min(STAGES, tiles); ++tile) ok = mbar_wait(smem_u32(&sh.full[tile]), 0) && ok;
+      if (!ok) gave_up();
+    }
+  } else {
     float x[VALUES];
     auto read = [&](int tile) {
       const float* const from = ring + tile % STAGES * TILE + threadIdx.x * 4;
@@ -222,9 +239,6 @@ beam_select_kernel(const float* __restrict__ logits, const long long ld, const f
       if (threadIdx.x == 0) sh.n = n;
       __syncthreads();
     };
-    if (threadIdx.x == 0)
-      for (int tile = 0; tile < min(STAGES, tiles); ++tile) fetch(tile);
-    bool ok = true;
     for (int tile = 0; tile < tiles && ok; ++tile) {
       ok = mbar_wait(smem_u32(&sh.full[tile % STAGES]), tile / STAGES & 1);
       int taken = 0;
@@ -320,13 +334,8 @@ beam_select_kernel(const float* __restrict__ logits, const long long ld, const f
     n = sh.n;
     __syncthreads();
     if (!ok) {
-      // a copy that never came: the stretch counts as no numbers. Others in flight need microseconds to land
-      if (threadIdx.x == 0) {
-        gb_err::report(ERR_WAIT_FULL);
-        const unsigned long long t0 = globaltimer_ns();
-        while (globaltimer_ns() - t0 < 2000000ull) {}
-      }
-      n = 0, sum = NAN;
+      if (threadIdx.x == 0) gave_up();
+      n = 0, sum = NAN;                  // the stretch counts as no numbers
     }
     cut(true);
     Key* const list = lists + (row * chunks + chunk) * K;
@@ -362,14 +371,13 @@ beam_select_kernel(const float* __restrict__ logits, const long long ld, const f
     for (int j = 0; j < 4; ++j) {
       const int e = e0 + j * THREADS + threadIdx.x;
       beam[j] = e < entries ? e / per_row : 0;
-      mine[j] = e < entries && is_finite(scores[row0 + beam[j]]) ? __ldcg(all + e) : 0;
+      mine[j] = e < entries && is_finite(sh.score[beam[j]]) ? __ldcg(all + e) : 0;
     }
   };
   ask(0);
   for (int w = warp; w < beams; w += WARPS) {
-    const float score = scores[row0 + w];
     double lse = NAN;
-    if (is_finite(score)) {
+    if (is_finite(sh.score[w])) {
       const Part* const row_parts = parts + (row0 + w) * chunks;
       Part first{-INFINITY, 0.};
       if (lane < chunks) first.ref = __ldcg(&row_parts[lane].ref), first.sum = __ldcg(&row_parts[lane].sum);
@@ -381,7 +389,7 @@ beam_select_kernel(const float* __restrict__ logits, const long long ld, const f
       for (int c = lane + 32; c < chunks; c += 32) part += __ldcg(&row_parts[c].sum) * exp_of(__ldcg(&row_parts[c].ref) - top);
       lse = log(warp_sum(part)) + top;
     }
-    if (lane == 0) sh.score[w] = score, sh.lse[w] = isfinite(lse) ? lse : NAN;
+    if (lane == 0) sh.lse[w] = isfinite(lse) ? lse : NAN;
   }
   __syncthreads();
   Joined& join = *reinterpret_cast<Joined*>(ring);
@@ -453,7 +461,7 @@ beam_select_kernel(const float* __restrict__ logits, const long long ld, const f
 
 // How rows are cut. A small call, of less than a tile of 4,096 an SM, goes by tiles of 1,024. Then as many blocks as run at once, each with its share
 // of a row: a block pays for its first bound and its last cut, and the bound rises with the tiles that it has seen. Where there are more rows than that, four
-// times as many, so that the last ones do not keep the device waiting. (512 rows of 128,256: a block a row 57 us, two 64, three 70, eight 86.)
+// times as many, so that the last ones do not keep the device waiting. (512 rows of 128,256: a block a row 56 us, two 64, three 70, eight 86.)
 struct Cut {
   bool small;
   int per_block, chunks;
