@@ -313,10 +313,10 @@ class BranchOps:
         distribution: their candidates, like tokens of logit -inf, have the score -inf and come last. Up to 64 beams and 64 candidates."""
         what = "beam_select"
         items, beams = scores.shape
-        rows, V = logits.shape
+        (rows, V), (ld, unit) = logits.shape, logits.stride()
         n, dev, f32, i32 = best.shape[1], self._device_index, torch.float32, torch.int32
         chosen = best.shape
-        if not (rows == items * beams and logits.dtype is f32 and (logits.stride(1) == 1 or V == 1) and scores.dtype is f32 and scores.is_contiguous()
+        if not (rows == items * beams and logits.dtype is f32 and (unit == 1 or V == 1) and scores.dtype is f32 and scores.is_contiguous()
                 and best.dtype is f32 and best.is_contiguous() and parents.dtype is i32 and parents.is_contiguous() and tokens.dtype is i32
                 and tokens.is_contiguous() and chosen == (items, n) and parents.shape == chosen and tokens.shape == chosen
                 and 0 < n <= self.MOST_BEAMS and n <= beams * V and beams <= self.MOST_BEAMS and rows <= 65535 and V <= 1 << 30
@@ -324,7 +324,7 @@ class BranchOps:
                 and tokens.get_device() == dev):
             self._here(logits, scores, best, parents, tokens)
             _need(rows == items * beams, f"{what}: {rows} rows of logits for {items} items of {beams} beams")
-            _need(logits.dtype is f32 and (logits.stride(1) == 1 or V == 1), f"{what}: float32 logits with rows of unit stride")
+            _need(logits.dtype is f32 and (unit == 1 or V == 1), f"{what}: float32 logits with rows of unit stride")
             _need(scores.dtype is f32 and scores.is_contiguous(), f"{what}: contiguous float32 scores")
             for t, dtype in ((best, f32), (parents, i32), (tokens, i32)):
                 _need(t.dtype is dtype and t.is_contiguous() and t.shape == (items, n), f"{what}: best (float32), parents and tokens (int32) [items, n], contiguous")
@@ -337,7 +337,7 @@ class BranchOps:
         scratch, counters, _held = self._branch_memory("beam_select", L.gb_beam_select_scratch_bytes, (items, beams, V, n), ws, stream)
         self._check(L, L.gb_beam_select(_BEAM_CALL.pack(
             logits.data_ptr(), scores.data_ptr(), best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), counters, scratch, stream,
-            logits.stride(0), items, beams, V, n)), what)
+            ld, items, beams, V, n)), what)
 
     def copy_entries(self, arrays, source, target, dim: int = 0):
         """In every one of ``arrays`` (contiguous, of any type, none of them twice): entry ``source[i]`` along ``dim`` is copied to entry
