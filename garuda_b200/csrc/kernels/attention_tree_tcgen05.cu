@@ -19,8 +19,11 @@
 //   warp 1     one elected lane issues the products: S = Q K^T two tiles ahead, O += P V (P from tensor memory)
 //   warps 2-9  two groups of 128 threads; a thread has a row and 64 keys of every tile: an attention stream of its own, whose reference
 //              maximum follows the running one when that has grown by 2^8. Warps whose rows are all behind the last only keep count
-// A tile takes 2,900 to 3,000 clocks of a stretch, what its bytes take at the memory's rate: 2,100 are a warp's softmax, 1,100 the products, which run beside the
-// other tile's. 32 requests of 4,096 keys, 24 tokens: 107 us, of which the bytes are 84; lengths from 256 to 8,191: 111 (equal numbers of tiles: 153).
+// A tile takes 2,900 to 3,000 clocks of a stretch, what its bytes take at the memory's rate: 2,000 are a warp's softmax (of which 1,024 the exponentials, sixteen a
+// clock and SM), 1,100 the products, which run beside the other tile's. 32 requests of 4,096 keys, 24 tokens: 104 us, of which the bytes are 84; lengths from
+// 256 to 8,191: 106 (equal numbers of tiles: 153). Call behind call the power limit takes the clock from 1,965 to 1,690 MHz, and the latter 117: there the softmax
+// is what a tile waits for, and fewer instructions are a higher clock too (scores and sums one by one, not two at a time: 120.5; a quarter of the
+// exponentials as polynomials on the other pipes: 133).
 // Tiles that hold a key which some row does not read are masked by 64 bits a thread, made of the row's bits and limits. Their values
 // are looked at: a row of values that no query may read is cleared (it holds whatever was there), and one with an infinity or NaN
 // is cleared too and told to the rows, of which those that read it become NaN and the others are left alone (0 * inf would
@@ -49,7 +52,7 @@ constexpr int S_BUFS = 2;           // S buffers: the S products run this many t
 constexpr int O_COL0 = S_BUFS * KT;
 constexpr float RESCALE_ABOVE = 8.f;                // in powers of two
 constexpr int MIN_STRETCH = 4;                      // of shorter ones the joining takes longer than the tiles
-constexpr int BLOCK_COST = 2;                       // what a block of rows costs beside its tiles, in tiles
+constexpr int BLOCK_COST = 4;                       // what a block of rows costs beside its tiles, in tiles (two: 113 us for 110, 130 for 123 at the lower clock)
 constexpr int MAX_REQUESTS = 2048;                  // of one launch (their places are in shared memory)
 constexpr int COUNTERS = 1024;                      // one per CTA, and so no more CTAs
 
@@ -90,6 +93,27 @@ __device__ __forceinline__ float fast_exp2(float x) {      // about 2^-22 relati
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+typedef unsigned long long Two;            // two floats, for one instruction
+__device__ __forceinline__ Two two(float a, float b) {
+  Two d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float2 apart(Two a) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(a));
+  return d;
+}
+__device__ __forceinline__ Two fma_two(Two a, Two b, Two c) {
+  Two d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ Two add_two(Two a, Two b) {
+  Two d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
@@ -123,16 +147,17 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t at) {
 }
 
 // A row's result of several pieces: their sums with weights 2^(m - the largest m), over the denominators' sum. m is in powers of two.
+template <int FOURS>               // of channels
 struct Join {
   float m = -INFINITY, l = 0.f;
-  float4 t[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-  __device__ __forceinline__ void add(float2 ml, const float4 (&v)[2]) {
+  float4 t[FOURS] = {};
+  __device__ __forceinline__ void add(float2 ml, const float4 (&v)[FOURS]) {
     if (ml.x == -INFINITY && ml.y == 0.f) return;               // no key of this piece
     const float top = fmaxf(m, ml.x);
     // (without a reference there is nothing yet, or what is no number)
     const float keep = m == -INFINITY ? (l == 0.f ? 0.f : NAN) : fast_exp2(m - top), more = ml.x == -INFINITY ? NAN : fast_exp2(ml.x - top);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < FOURS; ++i) {
       t[i].x = t[i].x * keep + v[i].x * more, t[i].y = t[i].y * keep + v[i].y * more;
       t[i].z = t[i].z * keep + v[i].z * more, t[i].w = t[i].w * keep + v[i].w * more;
     }
@@ -140,34 +165,35 @@ struct Join {
   }
   __device__ __forceinline__ void store(__nv_bfloat16* to) const {
     const float inv = l == 0.f ? 0.f : 1.0f / l;
-    *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16(t[0].x * inv, t[0].y * inv), pack_bf16(t[0].z * inv, t[0].w * inv),
-                                               pack_bf16(t[1].x * inv, t[1].y * inv), pack_bf16(t[1].z * inv, t[1].w * inv));
+#pragma unroll
+    for (int i = 0; i < FOURS; i += 2)
+      *reinterpret_cast<uint4*>(to + 4 * i) = make_uint4(pack_bf16(t[i].x * inv, t[i].y * inv), pack_bf16(t[i].z * inv, t[i].w * inv),
+                                                         pack_bf16(t[i + 1].x * inv, t[i + 1].y * inv), pack_bf16(t[i + 1].z * inv, t[i + 1].w * inv));
   }
 };
 
 // Joins a block's pieces, of the CTAs c0 to c1, in this order: by the 256 threads of the softmax warps. (A function of its own: its registers are
-// not the tiles' loop's.) A thread has a row and a share of the channels, eight of AT_ONCE pieces at a time: that many loads are on their way.
-template <int HD>
-__device__ __noinline__ void join_pieces(const float* __restrict__ parts, int c0, int c1, int nrows, __nv_bfloat16* __restrict__ out, int g, int Hq) {
-  constexpr int AT_ONCE = 4;                                     // (with eight the whole kernel runs short of registers)
+// not the tiles' loop's.) A thread has a row and a share of the channels, so many fours of so many pieces at a time: that many loads are on their way.
+template <int HD, int AT_ONCE, int FOURS>
+__device__ __forceinline__ void join_by(const float* __restrict__ parts, int c0, int c1, int nrows, __nv_bfloat16* __restrict__ out, int g, int Hq) {
   const int x = threadIdx.x - 64, rows = (nrows + 31) & ~31, shares = GROUPS * 128 / rows, row = x % rows, share = x / rows;
   const int mine = HD / 4 / shares;                              // fours of channels
   if (share >= shares || row >= nrows) return;
   auto part_of = [&](int cta) { return parts + ((size_t)cta * 2 + (cta == c0 ? 1 : 0)) * Shape<HD>::PART_FLOATS; };
   __nv_bfloat16* const to = out + ((size_t)(row / g) * Hq + row % g) * HD;
 #pragma unroll 1
-  for (int f0 = share * mine; f0 < (share + 1) * mine; f0 += 2) {
-    Join join;
+  for (int f0 = share * mine; f0 < (share + 1) * mine; f0 += FOURS) {
+    Join<FOURS> join;
 #pragma unroll 1
     for (int cta = c0; cta <= c1; cta += AT_ONCE) {
       float2 ml[AT_ONCE];
-      float4 v[AT_ONCE][2];
+      float4 v[AT_ONCE][FOURS];
 #pragma unroll
       for (int u = 0; u < AT_ONCE; ++u) {
         const float* from = part_of(min(cta + u, c1));
         ml[u] = __ldcg(reinterpret_cast<const float2*>(from + QROWS * HD + row * 2));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) v[u][i] = __ldcg(reinterpret_cast<const float4*>(from) + (f0 + i) * QROWS + row);
+        for (int i = 0; i < FOURS; ++i) v[u][i] = __ldcg(reinterpret_cast<const float4*>(from) + (f0 + i) * QROWS + row);
       }
 #pragma unroll
       for (int u = 0; u < AT_ONCE; ++u)
@@ -175,6 +201,12 @@ __device__ __noinline__ void join_pieces(const float* __restrict__ parts, int c0
     }
     join.store(to + f0 * 4);
   }
+}
+template <int HD>
+__device__ __noinline__ void join_pieces(const float* __restrict__ parts, int c0, int c1, int nrows, __nv_bfloat16* __restrict__ out, int g, int Hq) {
+  // (more loads at once: the whole kernel runs short of registers)
+  if (c1 - c0 == 1 && nrows > 32) join_by<HD, 2, 4>(parts, c0, c1, nrows, out, g, Hq);          // (up to 32 rows: a thread has two or four fours)
+  else join_by<HD, 4, 2>(parts, c0, c1, nrows, out, g, Hq);
 }
 
 // CLUSTER: a block of rows and a head is a thread-block cluster's, of `ranks` CTAs, which share its keys; else CTAs have stretches.
@@ -637,18 +669,20 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
             m = m_new;
           }
           const float neg_m = m == -INFINITY ? 0.f : -m * scale_log2;       // nothing valid yet: avoid inf - inf
-#pragma unroll
-          for (int ch = 0; ch < GK; ++ch) sc(ch) = fast_exp2(fmaf(sc(ch), scale_log2, neg_m));
-          float ls[4] = {0.f, 0.f, 0.f, 0.f};
+          const Two scale_two = two(scale_log2, scale_log2), neg_m_two = two(neg_m, neg_m);
+          Two ls[4] = {two(0.f, 0.f), two(0.f, 0.f), two(0.f, 0.f), two(0.f, 0.f)};
           uint32_t pk[GK / 2];
 #pragma unroll
           for (int ch = 0; ch < GK; ch += 2) {
-            ls[(ch >> 1) & 3] += sc(ch) + sc(ch + 1);
+            const float2 x = apart(fma_two(two(sc(ch), sc(ch + 1)), scale_two, neg_m_two));
+            const float wx = fast_exp2(x.x), wy = fast_exp2(x.y);
+            ls[(ch >> 1) & 3] = add_two(ls[(ch >> 1) & 3], two(wx, wy));
             // Weights are rounded to bfloat16, the type of the values that they multiply: half a step of 2^-8 each, averaged out by the
             // sum over keys; the denominator takes them as they are.
-            pk[ch >> 1] = pack_bf16(sc(ch), sc(ch + 1));
+            pk[ch >> 1] = pack_bf16(wx, wy);
           }
-          l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+          const float2 sums = apart(add_two(add_two(ls[0], ls[1]), add_two(ls[2], ls[3])));
+          l += sums.x + sums.y;
           tmem_st(s_addr, pk);            // over the first half of the scores just read
           tmem_st_wait();
         }
@@ -751,7 +785,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
     for (int i = rank * mine + threadIdx.x; i < min(items, (rank + 1) * mine) && !*abort_s; i += THREADS) {
       const int row = i % w.nrows, f0 = i / w.nrows * 2;
       const uint32_t ml_at = smem_u32(part + QROWS * HD + row * 2), v_at = smem_u32(part) + (uint32_t)(f0 * QROWS + row) * 16;
-      Join join;
+      Join<2> join;
 #pragma unroll 1
       for (int q = 0; q < ranks; q += 4) {
         float2 ml[4];
@@ -792,7 +826,7 @@ int tensor_map(const void* ptr, int hd, long long d1, long long d2, long long d3
 }
 
 // CTAs of a cluster that share the keys of each of `units` blocks of rows, or 0: stretches. Clusters need no scratch memory, no scan of the lengths, and
-// join faster (a request of 8 tokens, 8 heads of 128, 500 keys: 9.6 us against 13.3; 8,000 keys: 17.4 against 22), but they are of 2, 4 or 8 CTAs (16 took
+// join faster (a request of 8 tokens, 8 heads of 128, 500 keys: 9.2 us against 13.3; 8,000 keys: 16.5 against 22), but they are of 2, 4 or 8 CTAs (16 took
 // twice as long: hardly any run at once), so that SMs stay idle, and wait for the longest request (32,000 keys: 46 against 38). In microseconds, with what both
 // have in common left out: a tile takes 1.1, a piece of a stretch 0.4 to join.
 template <int HD>
