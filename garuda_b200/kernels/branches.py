@@ -204,8 +204,8 @@ class BranchOps:
         low_bits = q_ptr | k_ptr | v_ptr | out_ptr
         if (dtype is torch.bfloat16 and self.tc is not None and (hd == 64 or hd == 128) and page_size in (8, 16, 32, 64, 128) and g <= 128 and pages > 0
                 and not low_bits & 15):
-            # the row of all tiles is counted in 31 bits
-            if R * Hkv * (max_q_len * g // 64 + 1) * (max_kv_len // 128 + 4) >= 1 << 31:
+            # the row of all tiles, with four more for every block of rows, is counted in 31 bits
+            if R * Hkv * (max_q_len * g // 64 + 1) * (max_kv_len // 128 + 6) >= 1 << 31:
                 raise KernelError("tree_attention: more tiles than fit 31 bits")
             scratch, counters, _held = self._branch_memory("tree_attention", L.gb_tree_attention_scratch_bytes, (hd,), ws, stream)
             entry, launches = L.gb_tree_attention_tc, (R + 2047) // 2048
