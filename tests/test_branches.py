@@ -196,10 +196,11 @@ def test_an_array_given_twice_is_refused():
 def test_more_tiles_than_fit_the_row_of_costs_are_refused():
     # 2^12 requests of 2^10 key/value heads, one token, one key: 2^22 blocks of rows; a tile and four more each fit, 511 tiles and as many do not
     R, Hkv = 1 << 12, 1 << 10
-    args = dict(q=zeros(R, Hkv, 64, dtype=BF16), k_pool=zeros(1, Hkv, 8, 64, dtype=BF16), v_pool=zeros(1, Hkv, 8, 64, dtype=BF16), cu_q=zeros(R + 1), kv_lens=zeros(R),
-                positions=zeros(R), mask=zeros(R, 1), out=torch.zeros(R, Hkv * 64, dtype=BF16), scale=0.1, window=0, page_size=8, max_q_len=1)
+    args = dict(q=zeros(1, Hkv, 64, dtype=BF16), k_pool=zeros(1, Hkv, 128, 64, dtype=BF16), v_pool=zeros(1, Hkv, 128, 64, dtype=BF16), cu_q=zeros(R + 1),
+                kv_lens=zeros(R), positions=zeros(1), mask=zeros(1, 1), out=zeros(1, Hkv * 64, dtype=BF16), block_table=zeros(R, 507), scale=0.1, window=0,
+                page_size=128, max_q_len=1)
     ops = Recorder()
-    ops.tree_attention(block_table=zeros(R, 1), max_kv_len=1, **args)
+    ops.tree_attention(max_kv_len=1, **args)
     assert ops.names() == ["gb_tree_attention_tc"]
     with pytest.raises(KernelError, match="31 bits"):
-        ops.tree_attention(block_table=zeros(R, 8192), max_kv_len=507 * 128, **args)
+        ops.tree_attention(max_kv_len=507 * 128, **args)
