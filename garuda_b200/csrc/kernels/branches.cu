@@ -242,7 +242,11 @@ copy_entries_kernel(const __grid_constant__ CopyArrays arrays, const int32_t* __
         phase ^= 1;
         if (!came) gb_err::report(ERR_WAIT_FULL);
         ok = __syncthreads_and(came);
-        if (!ok) break;
+        if (!ok) {                    // what is still in flight needs microseconds to land
+          const unsigned long long t0 = globaltimer_ns();
+          while (globaltimer_ns() - t0 < 2000000ull) {}
+          break;
+        }
         for (int i = threadIdx.x; i < n; i += COPY_THREADS)
           asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(row + sh.target[i] * bytes), "r"(base + i * column),
                        "r"(size) : "memory");
