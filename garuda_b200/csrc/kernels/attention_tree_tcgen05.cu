@@ -21,9 +21,9 @@
 //              maximum follows the running one when that has grown by 2^8. Warps whose rows are all behind the last only keep count
 // A tile takes 2,900 to 3,000 clocks of a stretch, what its bytes take at the memory's rate: 2,000 are a warp's softmax (of which 1,024 the exponentials, sixteen a
 // clock and SM), 1,100 the products, which run beside the other tile's. 32 requests of 4,096 keys, 24 tokens: 104 us, of which the bytes are 84; lengths from
-// 256 to 8,191: 106 (equal numbers of tiles: 153). Call behind call the power limit takes the clock from 1,965 to 1,690 MHz, and the latter 117: there the softmax
-// is what a tile waits for, and fewer instructions are a higher clock too (scores and sums one by one, not two at a time: 120.5; a quarter of the
-// exponentials as polynomials on the other pipes: 133).
+// 256 to 8,191: 106 (equal numbers of tiles: 153). Call behind call the power limit takes the clock from 1,965 to 1,690 MHz, and the latter 117:
+// fewer instructions are a higher clock (scores and sums one by one, not two at a time: 120.5; a quarter of the
+// exponentials as polynomials on the other pipes: 133; the groups on alternate tiles instead of halves, each with a row's 128 keys in two walks: 109 and 122.5).
 // Tiles that hold a key which some row does not read are masked by 64 bits a thread, made of the row's bits and limits. Their values
 // are looked at: a row of values that no query may read is cleared (it holds whatever was there), and one with an infinity or NaN
 // is cleared too and told to the rows, of which those that read it become NaN and the others are left alone (0 * inf would
