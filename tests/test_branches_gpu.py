@@ -182,6 +182,33 @@ def test_rows_behind_the_last_request_and_absent_pages(ops):
 
 
 # ------------------------------------------------------------------ trees
+@pytest.mark.parametrize("dtype, page", [(torch.bfloat16, 32), (torch.bfloat16, 24), (torch.float32, 32)])
+def test_pages_behind_two_thousand_million_numbers(ops, dtype, page):
+    """The far end of a large pool: attention, moved rows and copied pages are those of a small one, bit for bit."""
+    step = Step(3, [(700, 12), (90, 3)], 8, 4, 128, page, dtype)
+    want, small = step.run(ops), step.k.cuda()
+    pages = 2 ** 31 // (4 * page * 128) + 50
+    shift = pages - small.shape[0]
+    k, v = (torch.zeros(pages, 4, page, 128, dtype=dtype, device="cuda") for _ in range(2))
+    k[shift:], v[shift:] = small, step.v.cuda()
+    table = torch.from_numpy(np.where(step.table >= 0, step.table + shift, -1).astype(np.int32)).cuda()
+    out = torch.full_like(want, 7.0)
+    ops.tree_attention(step.q.cuda(), k, v, table, ints(step.cu), ints(step.kv), ints(step.positions), step.words_of, out, step.scale, 0, page, step.max_q, step.max_kv)
+    assert torch.equal(out, want)
+    drafted = ints([5, 6, 7, 6]), ints([7, 8, 1, 2]), ints([-1, 0, 0, 1]), ints([0, 4]), ints([10])
+    for pool, last in ((k, pages - 1), (small, small.shape[0] - 1)):
+        path, kept, after = ints([[9] * 4]), ints([9]), ints([9])
+        ops.tree_accept(*drafted, path, kept, after, 4, [pool], ints([[last]]), page)
+        assert path.tolist() == [[0, 2, -1, -1]]
+    ops.copy_entries([k], ints([pages - 1, 0]), ints([pages - 2, pages - 3]))
+    ops.copy_entries([small], ints([small.shape[0] - 1]), ints([small.shape[0] - 2]))
+    small[-3] = 0
+    assert torch.equal(k[shift:].view(torch.uint8), small.view(torch.uint8))          # (there are NaN in them)
+    ops.check_branch_errors()
+    del k, v
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("requests", [3, 90])
 def test_a_length_of_zero_reads_nothing(ops, dtype, requests):
@@ -315,6 +342,17 @@ def test_beam_of_rows_that_lie_apart(ops):
     wide = torch.randn(8, 6007, generator=g)
     for first, V in ((1, 6000), (2, 4099), (3, 17), (0, 6007)):
         check_beam(ops, wide[:, first:first + V].contiguous(), torch.zeros(2, 4), 5, device=wide.cuda()[:, first:first + V])
+
+
+def test_beam_of_rows_that_lie_far_apart(ops):
+    g = torch.Generator().manual_seed(6)
+    wide, row = torch.zeros(8, 2 ** 29 + 4, device="cuda")[:, :9001], 2 * torch.randn(9001, generator=g)
+    wide[7] = row.cuda()
+    logits = torch.zeros(1, 8, 9001)
+    logits[0, 7] = row
+    check_beam(ops, logits, torch.full((1, 8), -1.0), 12, device=wide)
+    del wide
+    torch.cuda.empty_cache()
 
 
 def test_beams_as_near_as_64_bits_tell(ops):
