@@ -461,7 +461,8 @@ beam_select_kernel(const float* __restrict__ logits, const long long ld, const f
 
 // How rows are cut. A small call, of less than a tile of 4,096 an SM, goes by tiles of 1,024. Then as many blocks as run at once, each with its share
 // of a row: a block pays for its first bound and its last cut, and the bound rises with the tiles that it has seen. Where there are more rows than that, four
-// times as many, so that the last ones do not keep the device waiting. (512 rows of 128,256: a block a row 56 us, two 64, three 70, eight 86.)
+// times as many, so that the last ones do not keep the device waiting. (512 rows of 128,256: a block a row 56 us, two 64, three 70, eight 86; equal stretches, which begin
+// and end inside rows, 70: pieces of two rows, and too few registers for what tells them apart.)
 struct Cut {
   bool small;
   int per_block, chunks;
