@@ -192,8 +192,8 @@ class BranchOps:
                 and positions.dtype is i32 and mask.dtype is i32 and block_table.is_contiguous() and cu_q.is_contiguous() and kv_lens.is_contiguous()
                 and positions.is_contiguous() and mask.is_contiguous() and cu_q.shape == (R + 1,) and kv_lens.dim() == 1 and table[0] >= R
                 and positions.shape == (T,) and rows == T and 32 * words >= max_q_len > 0 and scale > 0
-                and 0 <= window < 1 << 31 and width * page_size >= max_kv_len <= self.MOST_POSITIONS and q.get_device() == dev and k_pool.get_device() == dev and v_pool.get_device() == dev
-                and out.get_device() == dev and block_table.get_device() == dev and cu_q.get_device() == dev and kv_lens.get_device() == dev
+                and 0 <= window < 1 << 31 and width * page_size >= max_kv_len <= self.MOST_POSITIONS and q.get_device() == dev
+                and k_pool.get_device() == dev and v_pool.get_device() == dev and out.get_device() == dev and block_table.get_device() == dev and cu_q.get_device() == dev and kv_lens.get_device() == dev
                 and positions.get_device() == dev and mask.get_device() == dev):
             self._refuse_attention(q, k_pool, v_pool, block_table, cu_q, kv_lens, positions, mask, out, scale, window, page_size, max_q_len,
                                    max_kv_len)
