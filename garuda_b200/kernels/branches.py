@@ -192,9 +192,9 @@ class BranchOps:
                 and positions.dtype is i32 and mask.dtype is i32 and block_table.is_contiguous() and cu_q.is_contiguous() and kv_lens.is_contiguous()
                 and positions.is_contiguous() and mask.is_contiguous() and cu_q.shape == (R + 1,) and kv_lens.dim() == 1 and table[0] >= R
                 and positions.shape == (T,) and rows == T and 32 * words >= max_q_len > 0 and scale > 0
-                and 0 <= window < 1 << 31 and width * page_size >= max_kv_len <= self.MOST_POSITIONS and q.get_device() == dev
-                and k_pool.get_device() == dev and v_pool.get_device() == dev and out.get_device() == dev and block_table.get_device() == dev and cu_q.get_device() == dev and kv_lens.get_device() == dev
-                and positions.get_device() == dev and mask.get_device() == dev):
+                and 0 <= window < 1 << 31 and page_size > 0 and width * page_size >= max_kv_len >= 0 and max_kv_len <= self.MOST_POSITIONS
+                and q.get_device() == dev and k_pool.get_device() == dev and v_pool.get_device() == dev and out.get_device() == dev
+                and block_table.get_device() == dev and cu_q.get_device() == dev and kv_lens.get_device() == dev and positions.get_device() == dev and mask.get_device() == dev):
             self._refuse_attention(q, k_pool, v_pool, block_table, cu_q, kv_lens, positions, mask, out, scale, window, page_size, max_q_len,
                                    max_kv_len)
         if T == 0 or R == 0:
@@ -230,6 +230,7 @@ class BranchOps:
         _need(k_pool.shape == shape and v_pool.shape == shape and k_pool.is_contiguous() and v_pool.is_contiguous(),
               f"{what}: pools must be contiguous {list(shape)}")
         _need(Hkv > 0 and Hq % Hkv == 0, f"{what}: heads in whole groups")
+        _need(page_size > 0, f"{what}: pages of at least one position")
         self._check_requests(what, cu_q, kv_lens)
         for t in (block_table, positions, mask):
             _need(t.dtype is torch.int32 and t.is_contiguous(), f"{what}: block table, positions and mask must be contiguous int32")
@@ -237,7 +238,7 @@ class BranchOps:
         _need(positions.shape == (T,) and mask.shape[0] == T, f"{what}: a position and a row of the mask for every token")
         _need(0 < max_q_len <= 32 * mask.shape[1], f"{what}: the mask is too narrow for that many tokens")
         _need(scale > 0 and 0 <= window < 1 << 31, f"{what}: a positive scale, a window that is not negative (and fits 31 bits)")
-        _need(max_kv_len <= self.MOST_POSITIONS, f"{what}: at most {self.MOST_POSITIONS} positions of a request")
+        _need(0 <= max_kv_len <= self.MOST_POSITIONS, f"{what}: at most {self.MOST_POSITIONS} positions of a request")
         raise KernelError(f"{what}: the block table is too narrow for that many positions")
 
     def tree_accept(self, tokens, targets, parents, cu_q, kv_lens, path, kept, next_tokens, max_q_len: int, pools=(), block_table=None,

@@ -204,3 +204,13 @@ def test_more_tiles_than_fit_the_row_of_costs_are_refused():
     assert ops.names() == ["gb_tree_attention_tc"]
     with pytest.raises(KernelError, match="31 bits"):
         ops.tree_attention(max_kv_len=507 * 128, **args)
+
+
+def test_pages_without_a_position_and_negative_lengths_are_refused():
+    ops = Recorder()
+    pool = zeros(4, 2, 0, 64, dtype=BF16)
+    with pytest.raises(KernelError, match="at least one position"):
+        ops.tree_attention(**attention_args(k_pool=pool, v_pool=pool, page_size=0, max_kv_len=0))
+    with pytest.raises(KernelError, match="positions of a request"):
+        ops.tree_attention(**attention_args(max_kv_len=-1))
+    assert not ops.names()
