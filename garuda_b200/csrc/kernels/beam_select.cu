@@ -15,7 +15,8 @@
 //     that runs the list over (many equal logits) enters by its own K-th key, found bit by bit.
 //   * Two candidates of different beams may be as near as 1e-7, so sums and scores are in 64 bits where it matters: exponentials of what is on the
 //     list at last, the largest ones, and the sum over tiles and threads; a thread's other exponentials of a tile and their sum are 32-bit:
-//     their errors are those of single terms, each smaller than K others, and average out.
+//     their errors are those of single terms, each smaller than K others and near the reference if it counts, and average out (4e-8 at most in 600 draws of
+//     rows in four orders; with references up to 30 below the largest logit 4e-7 on ascending rows).
 #include <climits>
 #include <type_traits>
 
@@ -34,7 +35,7 @@ constexpr int BLOCKS_PER_SM = 4;
 constexpr int MOST = 64;             // candidates that are chosen, and beams
 constexpr int LIST = 512;            // entries of a list
 constexpr int JOINED = 1024 + 64;    // of the list of all beams' candidates
-constexpr float CLOSE = 30.f;        // a reference may stay this far below the largest logit
+constexpr float CLOSE = 1.f;         // a reference may stay this far below the largest logit (its distance is what a term's exponent is rounded by)
 
 typedef unsigned long long Key;      // the larger logit first, then the smaller number: a block's keys all differ
 
@@ -207,7 +208,7 @@ beam_select_kernel(const float* __restrict__ logits, const long long ld, const f
     int n = 0, side = 0;               // the list's entries when it was last looked at, and which of the two lists it is
     const int limit = 2 * K + 32;      // entries at which the list is cut
     auto refer_to = [&](float to) {
-      if (to > ref + CLOSE) {          // (of the first tile's largest by as much: hardly ever)
+      if (to > ref + CLOSE) {          // (of the first tile's largest by as much: once or twice a row)
         sum *= exp_of((double)ref - (double)to);
         ref = to;
       }

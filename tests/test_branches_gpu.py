@@ -364,6 +364,15 @@ def test_beams_as_near_as_64_bits_tell(ops):
     check_beam(ops, logits, scores, 24)
 
 
+@pytest.mark.parametrize("n", [1, 2, 16])
+def test_beam_of_rows_in_order(ops, n):
+    """Every tile's logits are larger than those in front, or smaller: sums are as good as those of rows in no order."""
+    g = torch.Generator().manual_seed(n)
+    rows = (5 * torch.randn(40, 3, 32000, generator=g)).sort(-1)[0]
+    check_beam(ops, rows, -3 * torch.rand(40, 3, generator=g), n)
+    check_beam(ops, rows.flip(-1).contiguous(), -3 * torch.rand(40, 3, generator=g), n)
+
+
 # ------------------------------------------------------------------ copies
 @pytest.mark.parametrize("shapes, dim, dtype", [
     ([(3, 40, 2, 16, 64)] * 2, 1, torch.bfloat16), ([(40, 4, 32, 32), (40, 7), (40, 1)], 0, torch.float32), ([(5, 40, 3)], 1, torch.bfloat16),
