@@ -373,6 +373,22 @@ def test_beam_of_rows_in_order(ops, n):
     check_beam(ops, rows.flip(-1).contiguous(), -3 * torch.rand(40, 3, generator=g), n)
 
 
+def test_beam_of_rows_that_are_mostly_equal(ops):
+    """One logit, and all others d below: the exponentials' errors are one and the same, and do not average out."""
+    for V in (1000, 128256):
+        d = torch.linspace(0.01, 14, 60)
+        rows = (-d[:, None]).repeat(1, V)
+        rows[:, 7] = 0
+        best, parents, tokens = torch.empty(60, 1, device="cuda"), ints([[9]] * 60), ints([[9]] * 60)
+        ops.beam_select(rows.cuda(), torch.zeros(60, 1, device="cuda"), best, parents, tokens)
+        exact = -rows.double().logsumexp(-1)
+        outside = 1 - exact.exp()
+        # 2^-22 of an exponential; half a step each of the difference and of its product (d and d log2(e) ln 2), log2(e)'s 1.3e-8; the result's half step
+        bound = outside * (2.0 ** -22 + d * (2 * U32 + 1.4e-8)) + U32 * exact.abs()
+        assert tokens.flatten().tolist() == [7] * 60
+        assert ((best.flatten().cpu().double() - exact).abs() <= 1.01 * bound).all()
+
+
 # ------------------------------------------------------------------ copies
 @pytest.mark.parametrize("shapes, dim, dtype", [
     ([(3, 40, 2, 16, 64)] * 2, 1, torch.bfloat16), ([(40, 4, 32, 32), (40, 7), (40, 1)], 0, torch.float32), ([(5, 40, 3)], 1, torch.bfloat16),
