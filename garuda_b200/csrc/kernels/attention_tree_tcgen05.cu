@@ -241,7 +241,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
     for (int s = 0; s < V_STAGES; ++s) mbar_init(smem_u32(&mc.v_full[s]), 1), mbar_init(smem_u32(&mc.v_empty[s]), 1);
     mbar_init(smem_u32(&mc.o_ready[0]), 1);
     mbar_init(smem_u32(&mc.o_ready[1]), 1);
-    for (int g = 0; g < GROUPS; ++g) mbar_init(smem_u32(&mc.looked[g]), 2);
+    for (int g = 0; g < GROUPS; ++g) mbar_init(smem_u32(&mc.looked[g]), 4);
     mc.abort = 0, mc.total = 0;
     fence_barrier_init();
     fence_proxy_async();
@@ -594,10 +594,10 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
             fence_proxy_async();            // the tensor core reads the values through the async proxy
           }
           const uint32_t bads = __ballot_sync(0xffffffffu, bad);
-          if (quarter < 2 && lane == 0) {
-            mc.bad[et & 1][grp][quarter] = bads;
-            mbar_arrive(smem_u32(&mc.looked[grp]));
-          }
+          if (quarter < 2 && lane == 0) mc.bad[et & 1][grp][quarter] = bads;
+          // (All four warps arrive, those too that look at no value: so none is two such tiles in front of another, whose wait would take the phase after
+          // the next for its own, and whose notes would be written over.)
+          if (lane == 0) mbar_arrive(smem_u32(&mc.looked[grp]));
           wait(mc.looked[grp], et & 1, ERR_WAIT_FULL);
           const unsigned long long spoils = mc.bad[et & 1][grp][0] | ((unsigned long long)mc.bad[et & 1][grp][1] << 32);
           ++et;

@@ -1,0 +1,36 @@
+"""Decoding along branches on the device where calls are large, long or odd: many tiles that some rows must not read, many requests, wide groups, long trees."""
+import numpy as np
+import pytest
+import torch
+
+from tests.plain import branches_plain as plain
+from tests.test_branches_gpu import Step, ints, ops  # noqa: F401 (a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("heads, kv_heads, hd, copies", [(1, 1, 64, 1), (1, 1, 128, 1), (4, 2, 128, 1), (4, 4, 64, 4), (8, 4, 128, 4)])
+def test_values_that_are_not_finite_in_many_tiles_in_a_row(ops, heads, kv_heads, hd, copies):
+    """Eight tiles of drafted tokens behind one another, each with values that a few rows read and the others must not notice: one request, whose blocks of rows
+    have a cluster each, and many. (Marks of a tile that came too late, or from another tile, would change which rows are no numbers.)"""
+    clean = Step(hd, [(50, 1000)] * copies, heads, kv_heads, hd, 32, torch.bfloat16, reads=True)
+    spoilt = Step(hd, [(50, 1000)] * copies, heads, kv_heads, hd, 32, torch.bfloat16, reads=True)
+    bad = [j for j in range(1000) if j % 41 in (3, 7)]
+    for step in (clean, spoilt):
+        for t, reads in enumerate(step.reads):
+            for j in bad:
+                reads.discard(j)
+                if (7 * t + j) % 60 == 0:
+                    reads.add(j)
+    for r in range(copies):
+        for j in bad:
+            page, line = spoilt.table[r, (50 + j) // 32], (50 + j) % 32
+            spoilt.v[page, :, line, j % hd] = (float("nan"), float("inf"), float("-inf"))[j % 3]
+    want, got = (s.run(ops).view(s.T, heads, hd) for s in (clean, spoilt))
+    reads_bad = torch.tensor([not reads.isdisjoint(bad) for reads in spoilt.reads], device="cuda")
+    assert 0 < int(reads_bad.sum()) < len(reads_bad)
+    assert got[reads_bad].isnan().all()
+    assert torch.equal(got[~reads_bad], want[~reads_bad]) and not want.isnan().any()
+    for _ in range(3):
+        assert torch.equal(spoilt.run(ops).view(torch.int16), got.reshape(spoilt.T, -1).view(torch.int16))
+    ops.check_branch_errors()
