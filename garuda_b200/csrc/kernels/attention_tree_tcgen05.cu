@@ -231,7 +231,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
   }
   if (threadIdx.x == 0) {
     mbar_init(smem_u32(&mc.q_full), 1);
-    mbar_init(smem_u32(&mc.q_empty), GROUPS * 4);
+    mbar_init(smem_u32(&mc.q_empty), GROUPS * 4 + 1);
     mbar_init(smem_u32(&mc.met), GROUPS * 4);
     for (int b = 0; b < S_BUFS; ++b) {
       mbar_init(smem_u32(&mc.s_ready[b]), 1);
@@ -424,6 +424,10 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
       if (!(ok = mbar_wait_warp(smem_u32(&mc.q_full), it & 1, abort_s, ran_out))) break;
       const Piece w = mc.piece[it & 1];
       if (w.count == 0) break;
+      // (The piece has been seen, and that its queries came. The softmax warps alone do not say so: a piece of one or two tiles has all its scores before any
+      // of its values, and the barrier could be through the next piece's phase by the time that this warp looks at it.)
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&mc.q_empty));
       Lookup u{look(w, 0), -1};
       for (int j = 0; j < w.count; ++j) {
         if (!(ok = mbar_wait_warp(smem_u32(&mc.v_empty[vs]), vpar, abort_s, ran_out))) break;
@@ -609,8 +613,8 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
         wait(mc.s_ready[sb], sph, ERR_WAIT_ACCUM);
         if (!ok) break;
         tc_fence_after_sync();
-        // S of this tile is complete: its keys have been read, after a piece's last tile its queries (every warp says so: it is done with the piece in
-        // front), and the values of the tile two in front (products run in the order of their issue)
+        // S of this tile is complete: its keys have been read, after a piece's last tile its queries (every warp says so, and the values' once it has seen the
+        // piece: it is done with the piece in front), and the values of the tile two in front (products run in the order of their issue)
         if (j == count - 1 && lane == 0) mbar_arrive(smem_u32(&mc.q_empty));
         if (passes_on) {
           if (freed < gt - 1) {

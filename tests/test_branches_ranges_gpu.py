@@ -34,3 +34,14 @@ def test_values_that_are_not_finite_in_many_tiles_in_a_row(ops, heads, kv_heads,
     for _ in range(3):
         assert torch.equal(spoilt.run(ops).view(torch.int16), got.reshape(spoilt.T, -1).view(torch.int16))
     ops.check_branch_errors()
+
+
+@pytest.mark.parametrize("heads, kv_heads, hd", [(2, 2, 64), (4, 2, 128)])
+def test_many_pieces_of_one_and_two_tiles(ops, heads, kv_heads, hd):
+    """Requests of one to three tiles each, several to a stretch: the warps that bring queries, keys and values go from piece to piece side by side."""
+    step = Step(hd, [(64 * (i % 6) + i % 5, 1 + i % 4) for i in range(500)], heads, kv_heads, hd, 32, torch.bfloat16)
+    first = step.run(ops)
+    step.check(first, True)
+    for _ in range(20):
+        assert torch.equal(step.run(ops), first)
+    ops.check_branch_errors()
