@@ -188,7 +188,7 @@ class BranchOps:
         # (one condition, taken apart when it fails)
         if not (q.is_contiguous() and out.is_contiguous() and out.shape == (T, Hq * hd) and dtype is out.dtype and dtype is k_pool.dtype
                 and dtype is v_pool.dtype and dtype in _TAG and pool == (pages, Hkv, page_size, hd) and v_pool.shape == pool and k_pool.is_contiguous()
-                and v_pool.is_contiguous() and Hkv > 0 and Hq % Hkv == 0 and block_table.dtype is i32 and cu_q.dtype is i32 and kv_lens.dtype is i32
+                and v_pool.is_contiguous() and Hkv > 0 and Hq > 0 and Hq % Hkv == 0 and hd > 0 and block_table.dtype is i32 and cu_q.dtype is i32 and kv_lens.dtype is i32
                 and positions.dtype is i32 and mask.dtype is i32 and block_table.is_contiguous() and cu_q.is_contiguous() and kv_lens.is_contiguous()
                 and positions.is_contiguous() and mask.is_contiguous() and cu_q.shape == (R + 1,) and kv_lens.dim() == 1 and table[0] >= R
                 and positions.shape == (T,) and rows == T and 32 * words >= max_q_len > 0 and scale > 0
@@ -229,7 +229,8 @@ class BranchOps:
               f"{what}: one dtype, bfloat16 or float32, for q, cache and out")
         _need(k_pool.shape == shape and v_pool.shape == shape and k_pool.is_contiguous() and v_pool.is_contiguous(),
               f"{what}: pools must be contiguous {list(shape)}")
-        _need(Hkv > 0 and Hq % Hkv == 0, f"{what}: heads in whole groups")
+        _need(Hkv > 0 and Hq > 0 and Hq % Hkv == 0, f"{what}: heads in whole groups")
+        _need(hd > 0, f"{what}: heads of at least four channels")
         _need(page_size > 0, f"{what}: pages of at least one position")
         self._check_requests(what, cu_q, kv_lens)
         for t in (block_table, positions, mask):

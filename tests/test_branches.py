@@ -214,3 +214,16 @@ def test_pages_without_a_position_and_negative_lengths_are_refused():
     with pytest.raises(KernelError, match="positions of a request"):
         ops.tree_attention(**attention_args(max_kv_len=-1))
     assert not ops.names()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 48])
+def test_attention_without_heads_or_channels_is_refused(hd):
+    """(The kernels divide by the heads of a group.)"""
+    ops = Recorder()
+    for heads in (0, 2):
+        none = zeros(4, heads, 32, hd, dtype=BF16)
+        with pytest.raises(KernelError, match="whole groups"):
+            ops.tree_attention(**attention_args(q=zeros(5, 0, hd, dtype=BF16), k_pool=none, v_pool=none, out=zeros(5, 0, dtype=BF16)))
+    with pytest.raises(KernelError, match="channels"):
+        ops.tree_attention(**attention_args(hd=0))
+    assert not ops.names()
