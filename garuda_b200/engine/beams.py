@@ -42,13 +42,13 @@ class _Item:
 def beam_search(engine, prompts: Sequence[Sequence[int]], beams: int, max_tokens: int, length_penalty: float) -> List[List[Hypothesis]]:
     ops, cache = engine.ops, engine.cache
     vocab = engine.model.spec.vocab_size
-    # as many candidates as leave enough that do not end the text, whichever do
-    candidates = min(beams * (1 + len(engine.eos_ids)), vocab)
+    # as many candidates as leave enough that do not end the text, whichever do (a step may have fewer)
+    candidates = beams * (1 + len(engine.eos_ids))
     most = getattr(ops, "MOST_BEAMS", 64)
     if beams < 1 or max_tokens < 1:
         raise ConfigError(f"beam search needs at least one beam and one token, not {beams} and {max_tokens}")
     if candidates > most or beams > vocab:
-        raise ConfigError(f"{beams} beams of a model with {len(engine.eos_ids)} end tokens need {beams * (1 + len(engine.eos_ids))} candidates "
+        raise ConfigError(f"{beams} beams of a model with {len(engine.eos_ids)} end tokens need {candidates} candidates "
                           f"(at most {most}, and no more beams than the vocabulary's {vocab} tokens)")
     if beams > cache.config.max_requests:
         raise ConfigError(f"{beams} beams need as many slots, the engine has {cache.config.max_requests} (max_concurrent)")

@@ -268,3 +268,27 @@ def test_what_the_search_refuses_and_what_it_leaves_behind():
     assert e.cache.manager.live_requests == 0 and e.stats()["pages_free"] == [5]
     e.cache.manager.check_invariants()
     assert len(e.beam_search([[3, 4]], beams=3, max_tokens=2)[0]) == 3
+
+
+def small_vocabulary(vocab, seed):
+    """A folder of a model with few tokens, and its configuration."""
+    import tempfile
+    from garuda_b200.weights import write_random_model
+    cfg = dict(TINY["A"][0], vocab_size=vocab)
+    folder = tempfile.mkdtemp(prefix="garuda_few_tokens_")
+    write_random_model(folder, cfg, seed, scale={"q_proj": 8.0, "k_proj": 8.0, "lm_head": 8.0})
+    return cfg, folder
+
+
+@pytest.mark.parametrize("vocab, beams, ends, seed", [(6, 4, 2, 0), (5, 5, 1, 1), (12, 4, 3, 2), (9, 8, 2, 3)])
+def test_search_in_a_vocabulary_smaller_than_its_candidates(vocab, beams, ends, seed):
+    """A step has every live beam's continuations to choose from, more than the vocabulary has tokens: end tokens of many beams do not crowd the others out."""
+    cfg, folder = small_vocabulary(vocab, seed)
+    w, prompt = folder_weights(folder), [1, 3, 2, 4]
+    x = llama_plain.forward(cfg, w, prompt)[-1]
+    eos = tuple(int(t) for t in np.argsort(-x)[:ends])
+    e = Engine(folder, dtype="float32", ops=BranchCpuOps(), cuda_graphs=False, page_size=8, kv_tokens=512, max_concurrent=8, eos_token_id=eos)
+    got = e.beam_search([prompt], beams=beams, max_tokens=5, length_penalty=1.0)[0]
+    want = plain_search(cfg, w, prompt, beams, 5, 1.0, set(eos), e.max_context)
+    assert [(h.tokens, h.finish_reason) for h in got] == [(t, why) for t, _, _, why in want]
+    assert np.allclose([h.score for h in got], [s for _, s, *_ in want], rtol=1e-4, atol=1e-4)
