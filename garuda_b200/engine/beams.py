@@ -21,7 +21,8 @@ _REQUESTS = itertools.count(1 << 40)        # ids that no scheduler hands out
 @dataclass
 class Hypothesis:
     """A continuation of a prompt: its tokens (without the token that ended it), the sum of their log-probabilities (with that token's), and why it
-    ended: "eos", "length" or "context_full"."""
+    ended: "eos", "length" or "context_full"; or "error": the model gave none of its beams a distribution (logits with an infinity or NaN), and these are
+    the tokens in front of that."""
     tokens: List[int] = field(default_factory=list)
     score: float = 0.0
     finish_reason: str = ""
@@ -70,7 +71,8 @@ def beam_search(engine, prompts: Sequence[Sequence[int]], beams: int, max_tokens
             _step(engine, [item for _, item in running], candidates, max_tokens, length_penalty)
             for i, item in running:
                 if not item.live:
-                    order = sorted(item.done, key=lambda h: -item.penalised(h, length_penalty))          # (stable: equal ones as they ended)
+                    # (stable: equal ones as they ended; those that have not ended come last, one behind the other by their scores)
+                    order = sorted(item.done, key=lambda h: (1, -h.score) if h.finish_reason == "error" else (0, -item.penalised(h, length_penalty)))
                     out[i] = order[:beams]
             running = [(i, item) for i, item in running if item.live]
     finally:
@@ -140,6 +142,8 @@ def _choose(engine, item, candidates, max_tokens, length_penalty) -> None:
         live.append(h)
         parents.append(parent)
     ended = [h for h in live if h.finish_reason]           # (all of them or none: beams are of one length)
+    if candidates[0][0] == float("-inf"):
+        item.done += [Hypothesis(h.tokens, h.score, "error") for h in item.live]
     if ended or not live:
         item.done += ended
         live = []

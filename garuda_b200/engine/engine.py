@@ -269,7 +269,8 @@ class Engine:
         """The ``beams`` best continuations of every prompt: a list of ``Hypothesis`` (``tokens``, ``score``, ``finish_reason``) for each, best first by
         ``score / length ** length_penalty``, where the score is the sum of the tokens' log-probabilities and the length counts an end token. Each step
         chooses the best of all beams' continuations (``beam_select``); those among the first ``beams`` that end the text are set aside, and the search
-        is over when ``beams`` have been and no other can overtake them, at ``max_tokens`` tokens, or where the context is full. Beams are
+        is over when ``beams`` have been and no other can overtake them, at ``max_tokens`` tokens, or where the context is full; where the model's logits
+        hold no distribution (an infinity or NaN) for any beam, what there is comes back with the reason "error", behind those that have ended. Beams are
         requests that share pages (``PagedCache.fork``): ``beams`` of the engine's slots for every prompt that runs, and pages for their
         continuations; where pages run out, ``OutOfPages``. Not for while a ``stream`` of this engine is being read."""
         from .beams import beam_search

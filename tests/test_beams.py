@@ -292,3 +292,38 @@ def test_search_in_a_vocabulary_smaller_than_its_candidates(vocab, beams, ends, 
     want = plain_search(cfg, w, prompt, beams, 5, 1.0, set(eos), e.max_context)
     assert [(h.tokens, h.finish_reason) for h in got] == [(t, why) for t, _, _, why in want]
     assert np.allclose([h.score for h in got], [s for _, s, *_ in want], rtol=1e-4, atol=1e-4)
+
+
+@pytest.mark.parametrize("after, eos", [(0, ()), (2, ()), (2, "likely")])
+def test_search_keeps_what_it_has_where_the_model_gives_no_distribution(after, eos):
+    """Logits that hold NaN in every beam: the hypotheses so far come back, marked, behind those that have ended; other prompts' are what they were."""
+    prompts = [random_tokens("A", 11, 1), random_tokens("A", 7, 2)]
+    if eos:
+        x = llama_plain.forward(TINY["A"][0], folder_weights(model_dir("A")), prompts[1])[-1]
+        eos = (int(np.argmax(x)),)
+    want = engine("A", eos_token_id=eos).beam_search(prompts, beams=2, max_tokens=4)
+    until = engine("A", eos_token_id=eos).beam_search(prompts[1:], beams=2, max_tokens=after)[0] if after else None
+    e = engine("A", eos_token_id=eos)
+    run, steps = e.runner.run, []
+
+    def spoilt(entries, **kw):
+        logits = run(entries, **kw)
+        if entries[0].want:
+            steps.append(len(entries))
+            if len(steps) == after + 1:
+                logits = logits.clone()
+                logits[2 if after else 1:, 5] = float("nan")          # the second prompt's beams
+        return logits
+
+    e.runner.run = spoilt
+    got = e.beam_search(prompts, beams=2, max_tokens=4)
+    key = [[(h.tokens, h.finish_reason, h.score) for h in hypotheses] for hypotheses in (got[0], want[0])]
+    assert key[0] == key[1]
+    ended = [h for h in got[1] if h.finish_reason == "eos"]
+    cut = [h for h in got[1] if h.finish_reason == "error"]
+    assert got[1] == ended + cut and cut and bool(ended) == bool(eos)
+    if after:
+        assert [(h.tokens, h.score) for h in cut] == [(h.tokens, h.score) for h in until if h.finish_reason == "length"][:len(cut)]
+    else:
+        assert [(h.tokens, h.score) for h in cut] == [([], 0.0)]
+    assert e.cache.manager.live_requests == 0 and e.stats()["pages_free"] == e.stats()["pages_total"]
