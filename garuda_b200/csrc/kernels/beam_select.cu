@@ -1,7 +1,8 @@
 // Selection over beams and vocabulary: of an item's candidates (beam w, token v) with the scores
 //   s_w + (x_wv - log sum_u exp x_wu)
-// the K best, equal ones in the order of w * V + v. A beam whose score is not finite is over, one whose logits hold an infinity or
-// NaN (or nothing but -inf) has no distribution: all their candidates count as -inf, as a token of logit -inf does.
+// the K best, equal ones in the order of w * V + v (beams of the same logits and score have the same ones, to the last bit). A beam whose score
+// is not finite is over, one whose logits hold an infinity or NaN (or nothing but -inf) has no distribution: all their candidates count as -inf,
+// as a token of logit -inf does.
 //
 // Bound by the one pass over the logits. Within a beam candidates lie as their logits do, so a block walks a stretch of a row, 4,096 (few: 1,024)
 // logits at a time, and leaves its K largest and what the stretch adds to the row's sum in scratch memory; the block that counts the last
@@ -131,8 +132,8 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM)
 beam_select_kernel(const float* __restrict__ logits, const long long ld, const float* __restrict__ scores, const int V, const int beams, const int K,
                    const int tiles_per_block, float* __restrict__ best, int32_t* __restrict__ parents, int32_t* __restrict__ tokens,
                    Part* __restrict__ parts, Key* __restrict__ lists, int* __restrict__ counters) {
-  constexpr int TILE = THREADS * VALUES;
-  extern __shared__ __align__(16) float ring[];            // [STAGES][TILE]
+  constexpr int TILE = THREADS * VALUES, STAGE = TILE + 4;
+  extern __shared__ __align__(16) float ring[];            // [STAGES][STAGE]
   __shared__ Shared sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int chunk = blockIdx.x, chunks = gridDim.x, item = blockIdx.y / beams;
@@ -146,14 +147,16 @@ beam_select_kernel(const float* __restrict__ logits, const long long ld, const f
   __syncthreads();
   gb::pdl_launch_dependents();
   gb::pdl_wait();
-  // a stretch of the row, in 16-byte vectors: places count from the 16 bytes in which the row begins
+  // A stretch of the row: tiles count from the row's first logit, wherever that lies, and a thread has every 256th logit of a tile, so that rows of the same logits
+  // have the same sums. (Four neighbouring ones a thread, a load from shared memory instead of four, tie a row's tiles to its place within 16 bytes, and were no faster:
+  // 512 rows of 128,256 58.6 and 57.9 us.) Copies are of 16-byte vectors; the row's ends, in front of `head` and from `tail` on, are read where they are used.
   const float* const x_row = logits + row * ld;
-  const int shift = (int)((uintptr_t)x_row >> 2 & 3);
-  const int tile0 = chunk * tiles_per_block, tiles = min(tiles_per_block, (V + shift + TILE - 1) / TILE - tile0);
-  auto place = [&](int tile, int i) { return (tile0 + tile) * TILE + (i >> 2) * THREADS * 4 + (int)threadIdx.x * 4 + (i & 3) - shift; };
-  auto fetch = [&](int tile) {           // the tile's whole vectors: those of the row's ends are read where they are used
-    const int start = (tile0 + tile) * TILE - shift, from = start < 0 ? start + 4 : start;
-    const int vectors = max(0, min(start + TILE, V) - from) / 4;
+  const int shift = (int)((uintptr_t)x_row >> 2 & 3), head = (4 - shift) & 3, tail = V - (V + shift & 3);
+  const int tile0 = chunk * tiles_per_block, tiles = min(tiles_per_block, (V + TILE - 1) / TILE - tile0);
+  auto place = [&](int tile, int i) { return (tile0 + tile) * TILE + i * THREADS + (int)threadIdx.x; };
+  auto fetch = [&](int tile) {           // the vectors that hold the tile's logits
+    const int start = (tile0 + tile) * TILE, from = start == 0 ? head : start - shift;
+    const int vectors = max(0, min(start + TILE + head, tail) - from) / 4;
     const uint32_t bar = smem_u32(&sh.full[tile % STAGES]);
     if (vectors == 0) {
       mbar_arrive(bar);
@@ -161,7 +164,7 @@ beam_select_kernel(const float* __restrict__ logits, const long long ld, const f
     }
     mbar_arrive_expect_tx(bar, vectors * 16);
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                     smem_u32(ring + tile % STAGES * TILE + (from - start))), "l"(x_row + from), "r"(vectors * 16), "r"(bar) : "memory");
+                     smem_u32(ring + tile % STAGES * STAGE + (from + shift - start))), "l"(x_row + from), "r"(vectors * 16), "r"(bar) : "memory");
   };
   // (the first tiles are asked for before it is known whether the beam is over)
   if (threadIdx.x == 0)
@@ -182,18 +185,16 @@ beam_select_kernel(const float* __restrict__ logits, const long long ld, const f
   } else {
     float x[VALUES];
     auto read = [&](int tile) {
-      const float* const from = ring + tile % STAGES * TILE + threadIdx.x * 4;
-      const int start = (tile0 + tile) * TILE - shift;
-      const bool inside = start >= 0 && start + TILE <= V;
+      const float* const from = ring + tile % STAGES * STAGE + shift + threadIdx.x;
+      const int start = (tile0 + tile) * TILE;
+      if (start >= head && start + TILE <= tail) {
 #pragma unroll
-      for (int j = 0; j < VALUES / 4; ++j) {
-        const int at = place(tile, 4 * j);
-        if (inside || (at >= 0 && at + 3 < V)) {
-          const float4 v = *reinterpret_cast<const float4*>(from + j * THREADS * 4);
-          x[4 * j] = v.x, x[4 * j + 1] = v.y, x[4 * j + 2] = v.z, x[4 * j + 3] = v.w;
-        } else {
+        for (int i = 0; i < VALUES; ++i) x[i] = from[i * THREADS];
+      } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[4 * j + e] = at + e >= 0 && at + e < V ? x_row[at + e] : -INFINITY;
+        for (int i = 0; i < VALUES; ++i) {
+          const int at = place(tile, i);
+          x[i] = at >= V ? -INFINITY : at >= head && at < tail ? from[i * THREADS] : x_row[at];
         }
       }
     };
@@ -214,7 +215,7 @@ beam_select_kernel(const float* __restrict__ logits, const long long ld, const f
         ref = to;
       }
     };
-    // The list becomes its K largest in order. What leaves it goes into the sum, at last all of it.
+    // The list becomes its K largest in order (the others behind them, until new ones come). What leaves it goes into the sum, at last all of it.
     auto cut = [&](bool last) {
       const Key* const from = sh.list[side];
       Key* const to = sh.list[side ^ 1];
@@ -224,17 +225,17 @@ beam_select_kernel(const float* __restrict__ logits, const long long ld, const f
         int rank = 0;
         for (int j = threadIdx.x % 4; j < n; j += 4) rank += from[j] > mine;
         rank = sum_of_four(rank);
-        if (rank < K && i < n) to[rank] = mine;
+        if (i < n) to[rank] = mine;
       }
       __syncthreads();
       const int kept = min(n, K);
       if (n > 0) {
         refer_to(logit_of(to[0]));
-        const Key least = to[kept - 1];
+        // (in order: places on the list go to whoever is first)
         for (int i = threadIdx.x; i < n; i += THREADS)
-          if (last) sum += exp_of((double)logit_of(from[i]) - (double)ref);
-          else if (from[i] < least) sum += (double)fast_exp2((logit_of(from[i]) - ref) * 1.4426950408889634f);
-        if (kept == K) bound = logit_of(least);          // (a later logit as large has a larger number)
+          if (last) sum += exp_of((double)logit_of(to[i]) - (double)ref);
+          else if (i >= kept) sum += (double)fast_exp2((logit_of(to[i]) - ref) * 1.4426950408889634f);
+        if (kept == K) bound = logit_of(to[kept - 1]);          // (a later logit as large has a larger number)
       }
       side ^= 1;
       n = kept;
@@ -253,10 +254,10 @@ beam_select_kernel(const float* __restrict__ logits, const long long ld, const f
           for (int i = 0; i < VALUES; ++i)
             if (x[i] > bound && (exactly == 0 || key_of(x[i], place(tile, i)) >= exactly)) above |= 1u << i, x[i] = -INFINITY;
           while (above) {
-            const int i = __ffs(above) - 1, first = place(tile, i & ~3), at = first + (i & 3);
+            const int i = __ffs(above) - 1, at = place(tile, i);
             above &= above - 1;
             taken = atomicAdd(&sh.n, 1);
-            const float value = first >= 0 && first + 3 < V ? ring[tile % STAGES * TILE + at + shift - (tile0 + tile) * TILE] : x_row[at];
+            const float value = at >= head && at < tail ? ring[tile % STAGES * STAGE + at + shift - (tile0 + tile) * TILE] : x_row[at];
             if (taken < LIST) sh.list[side][taken] = key_of(value, at);
           }
         }
@@ -299,7 +300,7 @@ beam_select_kernel(const float* __restrict__ logits, const long long ld, const f
         __syncthreads();
         for (int i = threadIdx.x; i < LIST; i += THREADS) {
           const Key k = sh.list[side][i];
-          if (index_of(k) < (tile0 + tile) * TILE - shift) sh.list[side ^ 1][atomicAdd(&sh.n, 1)] = k;
+          if (index_of(k) < (tile0 + tile) * TILE) sh.list[side ^ 1][atomicAdd(&sh.n, 1)] = k;
         }
         __syncthreads();
         n = sh.n;
@@ -473,7 +474,7 @@ Cut cut_of(int rows, int V) {
   const long long room = (long long)BLOCKS_PER_SM * gb::sm_count();
   Cut c;
   c.small = (long long)rows * V < (long long)gb::sm_count() * THREADS * MANY;
-  const int tile = THREADS * (c.small ? 4 : MANY), tiles = (V + 3 + tile - 1) / tile;
+  const int tile = THREADS * (c.small ? 4 : MANY), tiles = (V + tile - 1) / tile;
   const long long blocks = rows > room ? (4 * room + rows - 1) / rows : room / rows;           // of a row
   c.per_block = (int)((tiles + blocks - 1) / blocks);
   c.chunks = (tiles + c.per_block - 1) / c.per_block;
@@ -507,7 +508,7 @@ GB_EXPORT int gb_beam_select(const BeamCall* call) {
   Part* parts = reinterpret_cast<Part*>(call->scratch);
   Key* lists = reinterpret_cast<Key*>(parts + (long long)rows * cut.chunks);
   auto launch = [&](auto values) {
-    constexpr int VALUES = decltype(values)::value, RING = STAGES * THREADS * VALUES * 4, SMEM = RING > (int)sizeof(Joined) ? RING : (int)sizeof(Joined);
+    constexpr int VALUES = decltype(values)::value, RING = STAGES * (THREADS * VALUES + 4) * 4, SMEM = RING > (int)sizeof(Joined) ? RING : (int)sizeof(Joined);
     static gb::OncePerDevice configured;
     if (configured.needed()) {
       const cudaError_t e = cudaFuncSetAttribute(beam_select_kernel<VALUES>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);

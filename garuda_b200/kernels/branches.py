@@ -311,7 +311,8 @@ class BranchOps:
         """The best continuations of every item over its beams and the vocabulary: candidates (beam w, token v) have the score ``scores[i, w] +
         log_softmax(logits[i * beams + w])[v]``, with sums and what counts most in 64 bits, other exponentials in 32 (off by 4e-8 as a rule, by up to
         1e-6 where most of a row are equal logits far below its largest); ``best``, ``parents``, ``tokens`` (float32, int32, int32 ``[items, n]``)
-        become the n best ones' scores, beams and tokens, equal ones in the order of (w, v). ``logits [items * beams, V]`` float32 with rows of unit stride,
+        become the n best ones' scores, beams and tokens, equal ones in the order of (w, v); beams of the same logits and score have
+        equal ones, wherever their rows lie. ``logits [items * beams, V]`` float32 with rows of unit stride,
         ``scores [items, beams]`` float32. A beam whose score is not finite is over, one whose logits hold an infinity or NaN has no
         distribution: their candidates, like tokens of logit -inf, have the score -inf and come last. Up to 64 beams and 64 candidates."""
         what = "beam_select"

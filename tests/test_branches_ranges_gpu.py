@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from tests.plain import branches_plain as plain
-from tests.test_branches_gpu import Step, ints, ops  # noqa: F401 (a fixture)
+from tests.test_branches_gpu import Step, check_beam, ints, ops  # noqa: F401 (a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +45,30 @@ def test_many_pieces_of_one_and_two_tiles(ops, heads, kv_heads, hd):
     for _ in range(20):
         assert torch.equal(step.run(ops), first)
     ops.check_branch_errors()
+
+
+# ------------------------------------------------------------------ beams
+@pytest.mark.parametrize("V", [3, 1237, 5001, 16387, 50257])
+@pytest.mark.parametrize("first", [0, 1])
+def test_alike_beams_wherever_their_rows_begin(ops, V, first):
+    """Rows of the same logits that begin on different four bytes: their candidates' scores are equal, and come in the order of the beams."""
+    items = 12
+    g = torch.Generator().manual_seed(V)
+    logits = 4 * torch.randn(items, 1, V, generator=g).expand(items, 3, V)
+    wide = torch.empty(items * 3, V + (V % 2 == 0) + 2 * first)
+    wide[:, first:first + V] = logits.reshape(-1, V)
+    device = wide.cuda()[:, first:first + V]
+    assert len({device[i].data_ptr() % 16 for i in range(36)}) == 4
+    check_beam(ops, logits.contiguous(), torch.full((items, 3), -1.25), min(3 * V, 13), device=device)
+
+
+def test_beam_repeats_itself(ops):
+    """Results do not depend on which of a block's threads come first: sums in 64 bits of rising rows, whose lists are cut often."""
+    g = torch.Generator().manual_seed(8)
+    logits = torch.cat([3 * torch.randn(30, 50257, generator=g), (3 * torch.randn(30, 50257, generator=g)).sort(-1)[0]]).cuda()
+    scores, outs = -torch.rand(12, 5, generator=g).cuda(), []
+    for _ in range(20):
+        outs.append((torch.empty(12, 40, device="cuda"), ints([[9] * 40] * 12), ints([[9] * 40] * 12)))
+        ops.beam_select(logits, scores, *outs[-1])
+    for out in outs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(out, outs[0]))
