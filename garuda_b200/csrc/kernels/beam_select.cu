@@ -16,9 +16,10 @@
 //     that runs the list over (many equal logits) enters by its own K-th key, found bit by bit.
 //   * Two candidates of different beams may be as near as 1e-7, so sums and scores are in 64 bits where it matters: exponentials of what is on the
 //     list at last, the largest ones, and the sum over tiles and threads; a thread's other exponentials of a tile and their sum are 32-bit:
-//     their errors are those of single terms, each smaller than K others and near the reference if it counts, and average out (4e-8 at most in 600 draws of
-//     rows in four orders; with references up to 30 below the largest logit 4e-7 on ascending rows). Where most of a row are equal they do not: a term that lies d below
-//     is off by up to 2^-22 + 1.35e-7 d (the difference's and its product's roundings, log2(e)'s), which came to 5e-7 for d = 11.
+//     a term that lies d below the largest logit is off by up to 2^-22 + 1.35e-7 d of itself (the exponential's error; the difference's and its product's roundings, log2(e)'s).
+//     Errors of different terms average out (4e-8 at most in 600 draws of rows in four orders; with references up to 30 below the largest logit 4e-7 on ascending
+//     rows). Those of equal ones do not: a row of one large logit and others d below is off by as much, and two roundings of a thread's sum, times their share of
+//     the sum: below 2^-21 + 1.35e-7 d (5e-7 seen at d = 11 for 128,256 of them).
 #include <climits>
 #include <type_traits>
 
@@ -205,7 +206,7 @@ beam_select_kernel(const float* __restrict__ logits, const long long ld, const f
       return top;
     };
     float bound = -INFINITY;           // what is no larger is not on the list
-    float ref = -INFINITY;             // exponentials are of x - ref, of which none is above 2^CLOSE times
+    float ref = -INFINITY;             // exponentials are of x - ref, none above e^CLOSE
     double sum = 0.;
     int n = 0, side = 0;               // the list's entries when it was last looked at, and which of the two lists it is
     const int limit = 2 * K + 32;      // entries at which the list is cut

@@ -309,8 +309,8 @@ class BranchOps:
     # ------------------------------------------------------------------ beams
     def beam_select(self, logits, scores, best, parents, tokens, ws=None):
         """The best continuations of every item over its beams and the vocabulary: candidates (beam w, token v) have the score ``scores[i, w] +
-        log_softmax(logits[i * beams + w])[v]``, with sums and what counts most in 64 bits, other exponentials in 32 (off by 4e-8 as a rule, by up to
-        1e-6 where most of a row are equal logits far below its largest); ``best``, ``parents``, ``tokens`` (float32, int32, int32 ``[items, n]``)
+        log_softmax(logits[i * beams + w])[v]``, with sums and what counts most in 64 bits, other exponentials in 32: off by 4e-8 as a rule, and
+        where most of a row's sum are equal logits d below its largest by up to 2^-21 + 1.35e-7 d (2.1e-6 at d = 12); ``best``, ``parents``, ``tokens`` (float32, int32, int32 ``[items, n]``)
         become the n best ones' scores, beams and tokens, equal ones in the order of (w, v); beams of the same logits and score have
         equal ones, wherever their rows lie. ``logits [items * beams, V]`` float32 with rows of unit stride,
         ``scores [items, beams]`` float32. A beam whose score is not finite is over, one whose logits hold an infinity or NaN has no

@@ -72,3 +72,18 @@ def test_beam_repeats_itself(ops):
         ops.beam_select(logits, scores, *outs[-1])
     for out in outs[1:]:
         assert all(torch.equal(a, b) for a, b in zip(out, outs[0]))
+
+
+@pytest.mark.parametrize("V", [1 << 17, 1 << 20, 1 << 22])
+def test_beam_of_equal_logits_far_below_the_largest(ops, V):
+    """What the wrapper states for rows of one logit and others d below, in vocabularies where these are most of the sum although they lie far below."""
+    d = torch.linspace(float(np.log(V)) - 4, float(np.log(V)) + 4, 30)
+    rows = (-d[:, None]).repeat(1, V)
+    rows[:, V // 3] = 0
+    best, parents, tokens = torch.empty(30, 1, device="cuda"), ints([[9]] * 30), ints([[9]] * 30)
+    ops.beam_select(rows.cuda(), torch.zeros(30, 1, device="cuda"), best, parents, tokens)
+    exact = -torch.log1p((V - 1) * torch.exp(-d.double()))
+    assert tokens.flatten().tolist() == [V // 3] * 30
+    # an exponential's 2^-22, 2^-24 each of the difference, its product with log2(e) and, of four equal terms, the third's and the fourth's sum, log2(e)'s 1.3e-8; and half
+    # a step of the result
+    assert ((best.flatten().cpu().double() - exact).abs() <= 1.01 * (2.0 ** -21 + 1.35e-7 * d + 2.0 ** -24 * exact.abs())).all()
