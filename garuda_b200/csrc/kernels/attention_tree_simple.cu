@@ -58,6 +58,10 @@ __device__ __forceinline__ void store4(T* p, float4 v) {
   gb::store_pair(p, v.x, v.y);
   gb::store_pair(p + 2, v.z, v.w);
 }
+// What stands for a masked key's score and weight: a NaN that no arithmetic gives (its results' are 0x7FFFFFFF), so that a key that is read counts whatever
+// its score is: a weight of nothing times a value that is not finite is none.
+constexpr uint32_t MASKED = 0xFFFFFFFFu;
+__device__ __forceinline__ bool is_masked(float x) { return __float_as_uint(x) == MASKED; }
 // exp of a difference; -inf gives 0
 __device__ __forceinline__ float weight_of(float s, float m) { return m == -INFINITY ? 0.f : expf(s - m); }
 
@@ -190,13 +194,13 @@ attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts) 
           bool sees = there && key < kv_len;
           if (j < 0) sees = sees && key >= start;
           else sees = sees && (j >> 5) < p.mask_words && (bits[j >> 5] >> (j & 31) & 1u);
-          if (!sees) x[u] = -INFINITY;
+          if (!sees) x[u] = __uint_as_float(MASKED);
         }
       }
 #pragma unroll
       for (int u = 0; u < BATCH; ++u) {
         mine[(k0 + u * S::SHARE) * P_LD] = x[u];
-        top = fmaxf(top, x[u]);
+        top = fmaxf(top, x[u]);                // (of a number and a NaN the number)
       }
     }
 #pragma unroll
@@ -208,12 +212,12 @@ attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts) 
       float x[BATCH];
 #pragma unroll
       for (int u = 0; u < BATCH; ++u) x[u] = mine[(k0 + u * S::SHARE) * P_LD];
-      // (a masked key's weight is nothing, whatever the maximum is; a score that is no number stays none)
+      // (a score that is no number stays none)
 #pragma unroll
-      for (int u = 0; u < BATCH; ++u) x[u] = x[u] == -INFINITY ? 0.f : expf(x[u] - less);
+      for (int u = 0; u < BATCH; ++u) x[u] = is_masked(x[u]) ? x[u] : expf(x[u] - less);
 #pragma unroll
       for (int u = 0; u < BATCH; ++u) {
-        sum += x[u];
+        sum += is_masked(x[u]) ? 0.f : x[u];
         mine[(k0 + u * S::SHARE) * P_LD] = x[u];
       }
     }
@@ -228,7 +232,7 @@ attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts) 
         for (int c = 0; c < FOURS; ++c) o[i][c].x *= less_now, o[i][c].y *= less_now, o[i][c].z *= less_now, o[i][c].w *= less_now;
       }
     }
-    // ---- sums of this thread's rows' channels, over its share of the keys. Without masked keys a weight of nothing does no harm; else it is left out
+    // ---- sums of this thread's rows' channels, over its share of the keys, masked ones left out
     auto sums = [&](auto masked) {
       // (the next key's weights and values are on their way while this one's are multiplied: there may be no other warp to fill the wait)
       float w[2][R];
@@ -251,7 +255,7 @@ attention_tree_simple_kernel(const TreeParams p, const int hd, const int parts) 
       auto add = [&](const float (&w)[R], const float4 (&v)[FOURS]) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-          if (decltype(masked)::value && w[i] == 0.f) continue;
+          if (decltype(masked)::value && is_masked(w[i])) continue;
 #pragma unroll
           for (int c = 0; c < FOURS; ++c) {
             o[i][c].x = fmaf(w[i], v[c].x, o[i][c].x), o[i][c].y = fmaf(w[i], v[c].y, o[i][c].y);

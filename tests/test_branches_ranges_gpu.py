@@ -87,3 +87,30 @@ def test_beam_of_equal_logits_far_below_the_largest(ops, V):
     # an exponential's 2^-22, 2^-24 each of the difference, its product with log2(e) and, of four equal terms, the third's and the fourth's sum, log2(e)'s 1.3e-8; and half
     # a step of the result
     assert ((best.flatten().cpu().double() - exact).abs() <= 1.01 * (2.0 ** -21 + 1.35e-7 * d + 2.0 ** -24 * exact.abs())).all()
+
+
+# ------------------------------------------------------------------ values that are not finite
+@pytest.mark.parametrize("dtype, hd", [(torch.float32, 64), (torch.float32, 128), (torch.bfloat16, 96)])
+@pytest.mark.parametrize("ctx, window, at, large", [(700, 0, 100, None), (700, 650, 100, None), (700, 0, 100, 600), (700, 0, 600, 100), (700, 650, 70, 130), (700, 650, 200, 600),
+                                                    (700, 0, 70, 10), (700, 0, 705, 100), (700, 0, 702, 704), (9000, 0, 100, 8900), (9000, 8990, 8000, 200), (100, 0, 60, 99)])
+def test_a_value_that_is_read_and_not_finite_shows(ops, dtype, hd, ctx, window, at, large):
+    """Wherever its key lies, in a tile that all rows read or at an edge, and if its weight is nothing beside a much larger one's."""
+    clean, spoilt = (Step(ctx + hd, [(ctx, 9), (40, 3)], 4, 2, hd, 32, dtype, window) for _ in range(2))
+    for step in (clean, spoilt):
+        step.q = step.q.abs() + 0.5
+        for reads in step.reads[:9]:
+            reads.update({2, 4, 5})
+        if large is not None:
+            step.k[step.table[0, large // 32], :, large % 32] = 40.0
+    for i, bad in enumerate((float("inf"), float("nan"), float("-inf"))):
+        spoilt.v[spoilt.table[0, at // 32], 0, at % 32, 3 + i] = bad
+    want, got = (s.run(ops).view(s.T, 4, hd).float() for s in (clean, spoilt))
+    assert want.isfinite().all()
+    assert not got[:9, :2, 3:6].isfinite().any()
+    assert torch.equal(got[:, 2:], want[:, 2:]) and torch.equal(got[9:], want[9:])
+    rest = [c for c in range(hd) if c not in (3, 4, 5)]
+    if dtype is torch.float32 or hd == 96:
+        assert torch.equal(got[..., rest], want[..., rest])
+    else:
+        assert (got[:9, :2].isnan() | (got == want)[:9, :2])[..., rest].all()
+    ops.check_branch_errors()
