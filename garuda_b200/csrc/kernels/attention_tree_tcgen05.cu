@@ -720,8 +720,9 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
         for (int g = 0; g < GROUPS; ++g) x[g] = mc.ml[mb][g][row], mt = fmaxf(mt, x[g].x);
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
-          // (a stream without a key: its accumulator means nothing; without a number: it has no reference)
-          f[g] = x[g].x == -INFINITY ? (x[g].y == 0.f ? 0.f : NAN) : fast_exp2((x[g].x - mt) * scale_log2);
+          // (a stream without a key: its accumulator means nothing, -inf stands for that; without a number: it has no reference. One whose weights are nothing beside
+          // the other's counts with them: what is not finite in it stays so)
+          f[g] = x[g].x == -INFINITY ? (x[g].y == 0.f ? -INFINITY : NAN) : fast_exp2((x[g].x - mt) * scale_log2);
           lt += x[g].x == -INFINITY ? x[g].y : x[g].y * f[g];
         }
         const float inv = whole ? (lt == 0.f ? 0.f : 1.0f / lt) : 1.f;
@@ -737,8 +738,8 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid
           tmem_ld_wait();
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            t[e] = f[0] == 0.f ? 0.f : __uint_as_float(v[0][e]) * (f[0] * inv);
-            t[e] += f[1] == 0.f ? 0.f : __uint_as_float(v[1][e]) * (f[1] * inv);
+            t[e] = f[0] == -INFINITY ? 0.f : __uint_as_float(v[0][e]) * (f[0] * inv);
+            t[e] += f[1] == -INFINITY ? 0.f : __uint_as_float(v[1][e]) * (f[1] * inv);
           }
           if (there) {
             if (whole) {

@@ -172,9 +172,9 @@ class BranchOps:
         ``[pages, Hkv, page_size, hd]``, all bfloat16 or all float32. Token i of request r (its tokens are ``cu_q[r]`` to ``cu_q[r + 1]``, ``kv_lens[r]`` its length
         with them) reads the request's context, with a ``window`` w > 0 only positions above ``positions[i] - w``, and those of
         the request's drafted tokens whose bits are set in ``mask[i]`` (``tree_layout`` makes both; any other mask will do, and positions from the
-        context's length up to below ``kv_lens[r]``). One that reads nothing gets zeros. What is masked has no influence, whatever it holds; a
-        value that is no finite number makes those that read it no numbers (float32: in its channel). Pages that the block table does not
-        have (-1) count as zeros.
+        context's length up to below ``kv_lens[r]``). One that reads nothing gets zeros (and so does one whose scores are all -inf). What is masked
+        has no influence, whatever it holds; a value that is no finite number leaves none in its channel to those that read it, however small its weight (on the
+        tensor cores it may be NaN in all channels of the head). Pages that the block table does not have (-1) count as zeros.
 
         On the tensor cores for bfloat16, heads of 64 and 128 and pages of 8 to 128 (a power of two), with weights rounded to bfloat16; other shapes (heads of a
         multiple of 4 channels up to 256) and float32 in 32-bit arithmetic throughout."""

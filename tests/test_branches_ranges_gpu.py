@@ -90,7 +90,7 @@ def test_beam_of_equal_logits_far_below_the_largest(ops, V):
 
 
 # ------------------------------------------------------------------ values that are not finite
-@pytest.mark.parametrize("dtype, hd", [(torch.float32, 64), (torch.float32, 128), (torch.bfloat16, 96)])
+@pytest.mark.parametrize("dtype, hd", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float32, 64), (torch.float32, 128), (torch.bfloat16, 96)])
 @pytest.mark.parametrize("ctx, window, at, large", [(700, 0, 100, None), (700, 650, 100, None), (700, 0, 100, 600), (700, 0, 600, 100), (700, 650, 70, 130), (700, 650, 200, 600),
                                                     (700, 0, 70, 10), (700, 0, 705, 100), (700, 0, 702, 704), (9000, 0, 100, 8900), (9000, 8990, 8000, 200), (100, 0, 60, 99)])
 def test_a_value_that_is_read_and_not_finite_shows(ops, dtype, hd, ctx, window, at, large):
