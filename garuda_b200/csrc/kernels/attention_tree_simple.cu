@@ -352,11 +352,11 @@ struct Plan {
   float time;
 };
 
-// Clusters of `parts` blocks that run at once (of the device that was current first).
+// Clusters of `parts` blocks that run at once.
 template <typename T, int HDMAX, int R>
 int at_once(int parts) {
-  static int known[MOST_PARTS + 1] = {};       // (one more than that; 0: not asked for yet)
-  if (known[parts] == 0) {
+  static branches::AskedOnce<MOST_PARTS + 1> known;
+  return known.get(parts, [&] {
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(parts), config.blockDim = dim3(THREADS), config.dynamicSmemBytes = 4 * smem_floats<Shape<HDMAX, R>>(HDMAX);
     cudaLaunchAttribute shape;
@@ -365,9 +365,8 @@ int at_once(int parts) {
     config.attrs = &shape, config.numAttrs = 1;
     int n = 0;
     if (cudaOccupancyMaxActiveClusters(&n, attention_tree_simple_kernel<T, HDMAX, R>, &config) != cudaSuccess) n = 0, cudaGetLastError();
-    known[parts] = n + 1;
-  }
-  return known[parts] - 1;
+    return n;
+  });
 }
 
 template <typename T, int HDMAX, int R>

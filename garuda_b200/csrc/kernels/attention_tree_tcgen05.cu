@@ -836,12 +836,12 @@ int tensor_map(const void* ptr, int hd, long long d1, long long d2, long long d3
 // have in common left out: a tile takes 1.1, a piece of a stretch 0.4 to join.
 template <int HD>
 int cluster_ranks(long long units, int tiles, int sms, int smem) {
-  static int most[4] = {-1, -1, -1, -1};                         // clusters of 2^i CTAs that run at once (of the device that was current first)
+  static branches::AskedOnce<4> most;                            // clusters of 2^i CTAs that run at once
   const float stretch = (float)((units * (tiles + BLOCK_COST) + sms - 1) / sms < MIN_STRETCH ? MIN_STRETCH : (units * (tiles + BLOCK_COST) + sms - 1) / sms);
   float best = 3.f + 1.1f * stretch + 0.4f * (tiles / stretch);
   int ranks = 0;
   for (int i = 1; i <= 3; ++i) {
-    if (most[i] < 0) {
+    const int room = most.get(i, [&] {
       cudaLaunchConfig_t config = {};
       config.gridDim = dim3(1 << i), config.blockDim = dim3(THREADS), config.dynamicSmemBytes = smem;
       cudaLaunchAttribute shape;
@@ -850,10 +850,10 @@ int cluster_ranks(long long units, int tiles, int sms, int smem) {
       config.attrs = &shape, config.numAttrs = 1;
       int n = 0;
       if (cudaOccupancyMaxActiveClusters(&n, attention_tree_tc_kernel<HD, true>, &config) != cudaSuccess) n = 0, cudaGetLastError();
-      most[i] = n;
-    }
+      return n;
+    });
     const float time = 1.1f * ((tiles + (1 << i) - 1) >> i);
-    if (units <= most[i] && time < best) best = time, ranks = 1 << i;
+    if (units <= room && time < best) best = time, ranks = 1 << i;
   }
   return ranks;
 }

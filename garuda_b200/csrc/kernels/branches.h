@@ -1,9 +1,27 @@
 // The parts of garuda_branches that its kernel files share: attention of drafted trees.
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace branches {
+
+// Numbers 0 .. N - 1 that a device is asked for once. Threads that are first together ask twice and get the same.
+template <int N>
+class AskedOnce {
+  std::atomic<int> known_[gb::OncePerDevice::MAX_DEVICES][N] = {};       // one more than the number; 0: not asked for yet
+
+ public:
+  template <typename F>
+  int get(int i, F ask) {
+    const int d = gb::OncePerDevice::device();
+    if (d < 0) return ask();
+    int n = known_[d][i].load(std::memory_order_relaxed);
+    if (n == 0) known_[d][i].store(n = ask() + 1, std::memory_order_relaxed);
+    return n - 1;
+  }
+};
 
 // Attention of a request's drafted tokens over its pages. Token i of request r reads the keys of the context, positions 0 to
 // kv_lens[r] - (cu_q[r + 1] - cu_q[r]) - 1 (with a window those above positions[i] - window), and those drafted tokens j of the request,

@@ -114,3 +114,38 @@ def test_a_value_that_is_read_and_not_finite_shows(ops, dtype, hd, ctx, window, 
     else:
         assert (got[:9, :2].isnan() | (got == want)[:9, :2])[..., rest].all()
     ops.check_branch_errors()
+
+
+# ------------------------------------------------------------------ threads
+def test_threads_that_call_at_once(ops):
+    """Several threads, each with a stream of its own, in calls of many shapes: what each gets is what it gets alone."""
+    import threading
+    shapes = [([(c, q)] * r, 8, 2, hd, 32, dtype) for dtype in (torch.bfloat16, torch.float32) for hd in (64, 128) for c, q, r in ((20, 3, 1), (900, 17, 2), (2500, 5, 40))]
+    steps = [Step(i, *shape) for i, shape in enumerate(shapes)]
+    got, failed = [[None] * len(steps) for _ in range(4)], []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for i in range(len(steps)):
+                    j = (i + 3 * k) % len(steps)
+                    s = steps[j]
+                    device = [x.cuda() for x in (s.q, s.k, s.v)]
+                    out = torch.empty(s.T, s.heads * s.hd, dtype=s.dtype, device="cuda")
+                    ops.tree_attention(*device, torch.from_numpy(s.table).cuda(), ints(s.cu), ints(s.kv), ints(s.positions),
+                                       torch.from_numpy(plain.mask_words(s.reads, s.words)).cuda(), out, s.scale, 0, 32, s.max_q, s.max_kv)
+                    got[k][j] = out
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:          # (told by the test's own thread)
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for j, s in enumerate(steps):
+        want = s.run(ops)
+        assert all(torch.equal(got[k][j], want) for k in range(4))
+    ops.check_branch_errors()
