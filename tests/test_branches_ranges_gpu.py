@@ -149,3 +149,83 @@ def test_threads_that_call_at_once(ops):
         want = s.run(ops)
         assert all(torch.equal(got[k][j], want) for k in range(4))
     ops.check_branch_errors()
+
+
+# ------------------------------------------------------------------ ranges
+@pytest.mark.parametrize("dtype, requests", [(torch.bfloat16, 2100), (torch.bfloat16, 4097), (torch.float32, 2100)])
+def test_attention_of_thousands_of_requests(ops, dtype, requests):
+    """More than one launch has places for: the second one has the same scratch memory."""
+    step = Step(requests, [(i * 37 % 150, i % 3) for i in range(requests)], 2, 1, 64, 16, dtype, 60 * (requests == 2100))
+    first = step.run(ops)
+    step.check(first, dtype is torch.bfloat16)
+    assert torch.equal(step.run(ops), first)
+    ops.check_branch_errors()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads, kv_heads, hd", [(16, 1, 64), (32, 2, 128), (12, 1, 128), (40, 1, 64), (65, 1, 64), (128, 1, 128), (130, 1, 64), (66, 2, 64)])
+def test_attention_of_wide_groups(ops, dtype, heads, kv_heads, hd):
+    """Blocks of 128 rows that have few tokens, or not a whole number of them; more query heads to a key/value head than a block has rows."""
+    step = Step(heads, [(300, 5), (0, 1), (127, 9), (40, 0), (1000, 2)], heads, kv_heads, hd, 32, dtype, reads=heads % 3 == 0)
+    step.check(step.run(ops), dtype is torch.bfloat16 and heads // kv_heads <= 128)
+    ops.check_branch_errors()
+
+
+@pytest.mark.parametrize("window", [0, 100, 5000])
+def test_layout_of_the_longest_trees(ops, window):
+    """A chain of 8,192 tokens, and a tree of as many."""
+    n, ctx = 8192, [7, 1000]
+    rng = np.random.default_rng(window)
+    bushy = [-1] + [int(rng.integers(0, i)) for i in range(1, n)]
+    positions, mask = ints([9] * (2 * n)), torch.full((2 * n, 256), 9, dtype=torch.int32, device="cuda")
+    ops.tree_layout(ints(list(range(-1, n - 1)) + bushy), ints([0, n, 2 * n]), ints([c + n for c in ctx]), positions, mask, n, window)
+    want, reads = plain.layout(bushy, [0, n], [ctx[1] + n], window)
+    assert positions[n:].tolist() == want
+    assert np.array_equal(mask[n:].cpu().numpy(), plain.mask_words(reads, 256))
+    i, j = torch.arange(n, device="cuda")[:, None], torch.arange(n, device="cuda")[None]
+    seen = (j <= i) & ((j > i - window) if window else True)
+    bits = (mask[:n, :, None] >> torch.arange(32, device="cuda", dtype=torch.int32)) & 1
+    assert torch.equal(bits.reshape(n, n).bool(), seen) and torch.equal(positions[:n], (i[:, 0] + ctx[0]).int())
+
+
+@pytest.mark.parametrize("n, page, steps", [(1000, 16, 400), (8192, 64, 500), (8191, 1, 150)])
+def test_accept_of_the_longest_trees(ops, n, page, steps):
+    """Paths that end near a tree's last token, beside a request of one: every row goes where it belongs."""
+    rng = np.random.default_rng(n)
+    path = [0] + sorted(rng.choice(np.arange(1, n), steps - 1, replace=False).tolist())
+    parents, tokens, targets = [-1] + [0] * (n - 1), [1] * n, [2] * n
+    for a, b in zip(path, path[1:]):
+        parents[b], tokens[b], targets[a] = a, 10 + b, 10 + b
+    ctx, cu = [70, 3], [0, n, n + 1]
+    parents, tokens, targets = parents + [-1], tokens + [5], targets + [6]
+    need = [-(-(c + q) // page) for c, q in zip(ctx, (n, 1))]
+    pages = sum(need)
+    order = rng.permutation(pages)
+    table = np.full((2, max(need)), -1, dtype=np.int32)
+    table[0, :need[0]], table[1, :need[1]] = order[:need[0]], order[need[0]:]
+    pool = torch.randn(2, pages, 2, page, 8, generator=torch.Generator().manual_seed(n))
+    want = pool.numpy().copy()
+    got, out, kept, after = pool.cuda(), torch.full((2, n), 9, dtype=torch.int32, device="cuda"), ints([9, 9]), ints([9, 9])
+    ops.tree_accept(ints(tokens), ints(targets), ints(parents), ints(cu), ints([ctx[0] + n, ctx[1] + 1]), out, kept, after, n, [got],
+                    torch.from_numpy(table).cuda(), page)
+    assert plain.accept(tokens, targets, parents, cu)[0] == [path, [0]]
+    assert kept.tolist() == [steps, 1] and after.tolist() == [2, 6]
+    assert out.tolist() == [path + [-1] * (n - steps), [0] + [-1] * (n - 1)]
+    plain.move_rows(want, table[0], page, ctx[0], path)
+    assert np.array_equal(got.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("items, beams, V, n", [(65535, 1, 5, 3), (1023, 64, 33, 64), (3000, 2, 4101, 5)])
+def test_beam_of_many_rows(ops, items, beams, V, n):
+    g = torch.Generator().manual_seed(items)
+    logits, scores = 3 * torch.randn(items, beams, V, generator=g), -torch.rand(items, beams, generator=g)
+    best, parents, tokens = torch.empty(items, n, device="cuda"), torch.empty(items, n, dtype=torch.int32, device="cuda"), torch.empty(items, n, dtype=torch.int32, device="cuda")
+    ops.beam_select(logits.reshape(-1, V).cuda(), scores.cuda(), best, parents, tokens)
+    value = scores.cuda().double()[:, :, None] + logits.cuda().double().log_softmax(-1)
+    exact, at = value.reshape(items, -1).sort(dim=1, descending=True, stable=True)
+    assert ((best.double() - exact[:, :n]).abs() <= 1.01 * 2.0 ** -24 * exact[:, :n].abs() + 1e-7).all()
+    # (scores as near as the sums' errors may change places)
+    here = (parents.long() * V + tokens.long())
+    assert (value.reshape(items, -1).gather(1, here) - exact[:, :n]).abs().max() <= 4e-7
+    assert float((here == at[:, :n]).double().mean()) > 0.999 and int(here.sort(1)[0].diff(dim=1).min()) > 0
+    ops.check_branch_errors()
